@@ -1,0 +1,260 @@
+// Building blocks of the segment attention kernels: the segment of a tile, tiles of rows staged in LDS, and the
+// operands of the matrix instructions.
+//
+// The query rows of a segment are taken per key head as nq * group packed rows (row r: query r / group, head
+// kv * group + r % group), so the query heads that share a key head share its tiles, and the sum over them in the
+// gradients of keys and values is part of the product's own sum.
+//
+// float32 operands are held as three bf16 planes (x3.h: a product is six bf16 products and keeps fp32 accuracy),
+// bf16 operands as one.
+#pragma once
+
+#include "common.h"
+#include "x3.h"
+
+typedef short fmd_s16x4 __attribute__((ext_vector_type(4)));
+
+struct AttnArgs {
+  const void *q, *k, *v;                    // rows [tokens, heads, dim], unit stride in dim
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // strides in elements
+  const int64_t *q_off, *k_off;             // [segments + 1]
+  int64_t tq, tk;
+  int32_t segments, heads, kv_heads, group, dim, causal;
+  float scale;
+};
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// A segment with its rows. The kernels see segments + 2 of them: the rows before the first offset and after the
+// last one (a fixed-capacity buffer's unused rows) are segments of their own without keys, or without queries.
+struct AttnSegment {
+  int64_t q0, k0;
+  int32_t nq, nk;
+};
+
+// start of extended segment i in 0 .. n + 2, with every offset clamped into the buffer
+__device__ __forceinline__ int64_t attn_start(const int64_t* off, int n, int64_t rows, int i) {
+  if (i == 0) return 0;
+  if (i == n + 2) return rows;
+  const int64_t o = off[i - 1];
+  return o < 0 ? 0 : o > rows ? rows : o;
+}
+
+// The tile of `bm` packed rows (rows * group of them) with number t: extended segment i owns the numbers from
+// floor(start(i) * group / bm) + i on, at least as many as it has tiles, so no table of tiles is needed and the grid
+// (rows * group / bm + segments + 2) is known without reading the offsets. The search probes 64 places at a time.
+// Returns the extended segment and the tile's first packed row in it; a number without a tile has first row >= rows.
+__device__ __forceinline__ int attn_find(const int64_t* off, int n, int64_t rows, int group, int bm, int64_t t,
+                                         int64_t* first) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, count = n + 2;
+  while (count > 1) {
+    const int step = (count + 63) >> 6;
+    const int i = lo + lane * step;
+    const bool at = lane * step < count && attn_start(off, n, rows, i) * group / bm + i <= t;
+    const int hits = __popcll(__ballot(at));
+    const int adv = (hits > 0 ? hits - 1 : 0) * step;
+    lo += adv;
+    count = count - adv < step ? count - adv : step;
+  }
+  *first = (t - (attn_start(off, n, rows, lo) * group / bm + lo)) * bm;
+  return lo;
+}
+
+__device__ __forceinline__ AttnSegment attn_segment(const AttnArgs& a, int i) {
+  AttnSegment s;
+  s.q0 = attn_start(a.q_off, a.segments, a.tq, i);
+  s.k0 = attn_start(a.k_off, a.segments, a.tk, i);
+  const int64_t nq = attn_start(a.q_off, a.segments, a.tq, i + 1) - s.q0;
+  const int64_t nk = attn_start(a.k_off, a.segments, a.tk, i + 1) - s.k0;
+  s.nq = nq > 0 ? (int)nq : 0;
+  s.nk = nk > 0 ? (int)nk : 0;
+  return s;
+}
+
+// whether extended segment i is one of the caller's (the first and last have no counterpart on the other side)
+__device__ __forceinline__ bool attn_real(const AttnArgs& a, int i) { return i >= 1 && i <= a.segments; }
+
+// ------------------------------------------------------------------------------------ operands
+
+template <int NP>
+struct Planes {
+  fmd_bf16x8 p[NP];
+};
+
+template <typename T>
+struct AttnType;
+template <>
+struct AttnType<__bf16> {
+  static constexpr int planes = 1;
+};
+template <>
+struct AttnType<float> {
+  static constexpr int planes = 3;
+};
+
+// eight values of a row as they lie in memory
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<__bf16> {
+  uint4 v;
+};
+template <>
+struct Raw8<float> {
+  float4 a, b;
+};
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> raw_zero() {
+  Raw8<T> r;
+  __builtin_memset(&r, 0, sizeof(r));
+  return r;
+}
+
+__device__ __forceinline__ Raw8<__bf16> raw_load(const __bf16* p) { return {*reinterpret_cast<const uint4*>(p)}; }
+__device__ __forceinline__ Raw8<float> raw_load(const float* p) {
+  return {reinterpret_cast<const float4*>(p)[0], reinterpret_cast<const float4*>(p)[1]};
+}
+
+__device__ __forceinline__ Planes<1> raw_planes(const Raw8<__bf16>& r) {
+  Planes<1> o;
+  o.p[0] = __builtin_bit_cast(fmd_bf16x8, r.v);
+  return o;
+}
+__device__ __forceinline__ Planes<3> raw_planes(const Raw8<float>& r) {
+  fmd_bf16x4 lo[3], hi[3];
+  x3_split(r.a, lo[0], lo[1], lo[2]);
+  x3_split(r.b, hi[0], hi[1], hi[2]);
+  Planes<3> o;
+#pragma unroll
+  for (int p = 0; p < 3; ++p) o.p[p] = __builtin_shufflevector(lo[p], hi[p], 0, 1, 2, 3, 4, 5, 6, 7);
+  return o;
+}
+
+__device__ __forceinline__ void planes_of(const float* x, Planes<1>& o) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o.p[0][e] = (__bf16)x[e];
+}
+__device__ __forceinline__ void planes_of(const float* x, Planes<3>& o) {
+  Raw8<float> r = {make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7])};
+  o = raw_planes(r);
+}
+
+__device__ __forceinline__ fmd_f32x16 mma(const Planes<1>& a, const Planes<1>& b, fmd_f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[0], b.p[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ fmd_f32x16 mma(const Planes<3>& a, const Planes<3>& b, fmd_f32x16 c) {
+  return x3_mfma(a.p, b.p, c);
+}
+
+__device__ __forceinline__ fmd_f32x16 zero16() {
+  fmd_f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+
+// ------------------------------------------------------------------------------------ tiles in LDS
+
+// A tile of ROWS rows of DP values (NP planes), row-major, its 16-byte chunks permuted within a row so that both
+// reads are free of bank conflicts: the same chunk of eight consecutive rows (operands along a row) and two chunks of
+// four consecutive rows (ds_read_b64_tr_b16, operands along a column).
+template <int NP, int ROWS, int DP>
+struct AttnTile {
+  static constexpr int LD = DP == 96 ? 128 : DP;  // a power of two, for the permutation
+  static constexpr int CHUNKS = DP / 8, PLANE = ROWS * LD, SIZE = NP * PLANE;
+
+  __device__ static __forceinline__ int at(int row, int chunk) {
+    const int f = LD >= 64 ? ((row & 3) << 1) | ((row >> 2) & 1) : (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
+    return row * LD + ((chunk ^ f) << 3);
+  }
+
+  __device__ static __forceinline__ void put(__bf16* s, int row, int chunk, const Planes<NP>& v) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<fmd_bf16x8*>(s + p * PLANE + at(row, chunk)) = v.p[p];
+  }
+
+  // operand of 32 rows (lane: row base + lane % 32) over 16 columns: eight columns from 16 step + 8 (lane / 32)
+  __device__ static __forceinline__ Planes<NP> rows(const __bf16* s, int base, int step) {
+    const int lane = threadIdx.x & 63;
+    Planes<NP> o;
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+      o.p[p] = *reinterpret_cast<const fmd_bf16x8*>(s + p * PLANE + at(base + (lane & 31), 2 * step + (lane >> 5)));
+    return o;
+  }
+
+  // operand of 32 columns (lane: column 32 block + lane % 32) over the 16 rows from `base`, in the order in which a
+  // 32 x 32 product holds its rows: for lane half h rows 4 h .. 4 h + 3, then 8 + 4 h .. 8 + 4 h + 3
+  __device__ static __forceinline__ Planes<NP> cols(const __bf16* s, int base, int block) {
+    const int lane = threadIdx.x & 63;
+    const int row = base + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int chunk = 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) * 4;
+    Planes<NP> o;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const __bf16 *x = s + p * PLANE + at(row, chunk) + sub, *y = s + p * PLANE + at(row + 8, chunk) + sub;
+      typedef __attribute__((address_space(3))) fmd_s16x4* lds_ptr;
+      const fmd_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)x);
+      const fmd_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)y);
+      o.p[p] = __builtin_bit_cast(fmd_bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return o;
+  }
+};
+
+// Rows of a tile on their way to LDS: THREADS threads load NV chunks each (issued together, written after the
+// previous tile has been read). Chunks past the rows or past dim are zero: nothing of another segment is read.
+template <typename T, int NP, int ROWS, int DP, int THREADS>
+struct AttnLoad {
+  using Tile = AttnTile<NP, ROWS, DP>;
+  static constexpr int N = ROWS * Tile::CHUNKS, NV = (N + THREADS - 1) / THREADS;
+  Raw8<T> r[NV];
+
+  // row(i): address of row i of the tile, or null
+  template <typename Row>
+  __device__ __forceinline__ void load(int t, int dim, const Row& row) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int i = t + n * THREADS, chunk = i % Tile::CHUNKS;
+      const T* p = (N % THREADS == 0 || i < N) && 8 * chunk < dim ? row(i / Tile::CHUNKS) : nullptr;
+      r[n] = p ? raw_load(p + 8 * chunk) : raw_zero<T>();
+    }
+  }
+  __device__ __forceinline__ void store(__bf16* s, int t) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int i = t + n * THREADS;
+      if (N % THREADS == 0 || i < N) Tile::put(s, i / Tile::CHUNKS, i % Tile::CHUNKS, raw_planes(r[n]));
+    }
+  }
+};
+
+// row index of register v of a 32 x 32 product in lane half h
+__device__ __forceinline__ int prod_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// max over the two lane halves
+__device__ __forceinline__ float max_halves(float x) {
+  float y = x;
+  swap_halves32(x, y);
+  return fmaxf(x, y);
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
+template <>
+__device__ __forceinline__ void store4<float>(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+template <>
+__device__ __forceinline__ void store4<__bf16>(__bf16* p, float a, float b, float c, float d) {
+  fmd_bf16x4 v;
+  v[0] = (__bf16)a;
+  v[1] = (__bf16)b;
+  v[2] = (__bf16)c;
+  v[3] = (__bf16)d;
+  *reinterpret_cast<fmd_bf16x4*>(p) = v;
+}

@@ -1,0 +1,738 @@
+// Attention of the query rows of each segment over the key rows of the same segment, and its VJP.
+#include "attention.h"
+
+namespace {
+
+// ------------------------------------------------------------------------------------ forward
+
+// One workgroup: 32 WM packed query rows of one key head, WM KW waves. Wave (wm, kw) holds 32 rows and walks the key
+// tiles kw, kw + KW, ... of its split; the KW partial softmaxes are joined through LDS at the end. The scores are
+// formed transposed, S^T = K Q^T (lane: a query, registers: keys), so the softmax statistics are one value per lane, the
+// sums over keys stay in the lane but for one exchange of the halves, and exp(S^T) is already the operand of
+// O^T = V^T P^T. Statistics and sums are fp32; P is rounded to bf16 for bf16 inputs (the output is, too) and kept as
+// three planes for fp32.
+template <typename T, int DP, int BN, int WM, int KW>
+__global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int64_t tiles, int splits, T* out, float* lse,
+                                                                float* part_o, float* part_m, float* part_l) {
+  constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, JB = BN / 32;
+  using Tile = AttnTile<NP, BN, DP>;
+  constexpr int kMerge = (KW - 1) * WM * (DB * 16 + 2) * 64 * 2;  // in bf16 units
+  constexpr int kTiles = 2 * KW * Tile::SIZE;
+  __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, kw = wave / WM;
+  const int kvh = blockIdx.x % a.kv_heads;
+  int64_t t = blockIdx.x / a.kv_heads;
+  if (a.causal) t = tiles - 1 - t;  // the rows with the most keys first
+  int64_t first;
+  const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first);
+  AttnSegment sg = attn_segment(a, ext);
+  if (!attn_real(a, ext)) sg.nk = 0;
+  const int rows = sg.nq * a.group;
+  if (first >= rows) return;
+  const int row0 = (int)first, row = row0 + 32 * wm + (lane & 31);
+  const bool live = row < rows;
+  const int tok = (live ? row : rows - 1) / a.group, head = kvh * a.group + (live ? row : rows - 1) % a.group;
+  const int64_t qt = sg.q0 + tok;
+
+  // keys that this row sees, and that any row of the workgroup sees
+  const int shift = sg.nk - sg.nq;
+  const int sees = a.causal ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
+  const int last_tok = min(row0 + 32 * WM, rows) - 1;
+  const int reach = a.causal ? max(0, min(sg.nk, last_tok / a.group + shift + 1)) : sg.nk;
+  const int least = a.causal ? max(0, min(sg.nk, row0 / a.group + shift + 1)) : sg.nk;
+  const int all_tiles = (reach + BN - 1) / BN;
+  const int per = (all_tiles + splits - 1) / splits;
+  const int tile_lo = min(all_tiles, (int)blockIdx.y * per), tile_hi = min(all_tiles, tile_lo + per);
+
+  Planes<NP> qf[KS];
+  {
+    const T* qp = static_cast<const T*>(a.q) + qt * a.q_row + head * a.q_head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int chunk = 2 * ks + half;
+      qf[ks] = raw_planes(live && 8 * chunk < a.dim ? raw_load(qp + 8 * chunk) : raw_zero<T>());
+    }
+  }
+
+  fmd_f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = zero16();
+  float m = -INFINITY, l = 0.f;
+  const float c = a.scale * kLog2e;
+
+  __bf16* ks_ = lds + kw * 2 * Tile::SIZE;
+  __bf16* vs_ = ks_ + Tile::SIZE;
+  const int lt = threadIdx.x - kw * WM * 64;  // thread among those that load this group's tiles
+  const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
+  const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
+  AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
+  auto issue = [&](int tile) {
+    const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
+    kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
+    vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
+  };
+
+  const int rounds = (tile_hi - tile_lo + KW - 1) / KW;  // the same for every wave
+  if (rounds > 0) issue(tile_lo + kw);
+  for (int it = 0; it < rounds; ++it) {
+    const int tile = tile_lo + it * KW + kw, j0 = tile * BN;
+    __syncthreads();  // the tiles before are read
+    kl.store(ks_, lt);
+    vl.store(vs_, lt);
+    __syncthreads();
+    if (it + 1 < rounds) issue(tile + KW);
+    if (tile >= tile_hi) continue;
+
+    fmd_f32x16 s[JB];
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+      s[j] = zero16();
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) s[j] = mma(Tile::rows(ks_, 32 * j, ks), qf[ks], s[j]);
+    }
+    if (j0 + BN > least) {  // some row does not see all of the tile
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (j0 + 32 * j + prod_row(v, half) >= sees) s[j][v] = -INFINITY;
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) top = fmaxf(top, s[j][v]);
+    top = max_halves(top);
+    const float base = top == -INFINITY ? 0.f : top * c;  // a row that has seen nothing yet: all exponents -inf
+    const float fade = exp2_hw(fmaf(m, c, -base));
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const float p = exp2_hw(fmaf(s[j][v], c, -base));
+        s[j][v] = p;
+        sum += p;
+      }
+    l = l * fade + sum;  // of this lane's half of the keys
+    m = top;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) o[d][v] *= fade;
+#pragma unroll
+    for (int j = 0; j < JB; ++j)
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[j][8 * step + e];
+        Planes<NP> pf;
+        planes_of(x, pf);
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(vs_, 32 * j + 16 * step, d), pf, o[d]);
+      }
+  }
+  l = add_halves(l);
+
+  if constexpr (KW > 1) {  // join the key groups, in their order
+    float* mg = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    if (kw > 0) {
+      float* w = mg + ((kw - 1) * WM + wm) * (DB * 16 + 2) * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) w[(d * 16 + v) * 64] = o[d][v];
+      w[DB * 16 * 64] = m;
+      w[(DB * 16 + 1) * 64] = l;
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int g = 0; g < KW - 1; ++g) {
+      const float* w = mg + (g * WM + wm) * (DB * 16 + 2) * 64 + lane;
+      const float gm = w[DB * 16 * 64], gl = w[(DB * 16 + 1) * 64];
+      const float top = fmaxf(m, gm), base = top == -INFINITY ? 0.f : top * c;
+      const float fa = exp2_hw(fmaf(m, c, -base)), fb = exp2_hw(fmaf(gm, c, -base));
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] = o[d][v] * fa + w[(d * 16 + v) * 64] * fb;
+      l = l * fa + gl * fb;
+      m = top;
+    }
+  }
+  if (!live) return;
+
+  if (splits == 1) {
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees no key gives zero
+    T* op = out + (qt * a.heads + head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * d + 8 * r + 4 * half;
+        if (col < a.dim)
+          store4<T>(op + col, o[d][4 * r] * inv, o[d][4 * r + 1] * inv, o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv);
+      }
+    if (lse && half == 0) lse[head * a.tq + qt] = l == 0.f ? -INFINITY : (m * c + __log2f(l)) * kLn2;
+  } else {
+    const int64_t at = ((int64_t)blockIdx.y * a.tq + qt) * a.heads + head;
+    float* op = part_o + at * a.dim;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * d + 8 * r + 4 * half;
+        if (col < a.dim) store4<float>(op + col, o[d][4 * r], o[d][4 * r + 1], o[d][4 * r + 2], o[d][4 * r + 3]);
+      }
+    if (half == 0) {
+      part_m[at] = m;
+      part_l[at] = l;
+    }
+  }
+}
+
+// The splits of a row joined in their order: one wave per (query, head), the lanes along dim.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, const float* part_o, const float* part_m,
+                                                        const float* part_l, T* out, float* lse) {
+  const int64_t n = a.tq * a.heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (at >= n) return;
+  const float c = a.scale * kLog2e;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_m[s * n + at]);
+  const float base = top == -INFINITY ? 0.f : top * c;
+  float l = 0.f, o[2] = {0.f, 0.f};
+  for (int s = 0; s < splits; ++s) {
+    const float f = exp2_hw(fmaf(part_m[s * n + at], c, -base));
+    l += f * part_l[s * n + at];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (lane + 64 * k < a.dim) o[k] += f * part_o[(s * n + at) * a.dim + lane + 64 * k];
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (lane + 64 * k < a.dim) out[at * a.dim + lane + 64 * k] = (T)(o[k] * inv);
+  if (lse && lane == 0) lse[(at % a.heads) * a.tq + at / a.heads] = l == 0.f ? -INFINITY : (top * c + __log2f(l)) * kLn2;
+}
+
+// ------------------------------------------------------------------------------------ backward
+
+struct AttnBwd {
+  const void* g;  // gradient of the output
+  int64_t g_row, g_head;
+  const float *lse, *delta;  // [heads, tq]
+};
+
+// delta[head, i] = g_i . o_i : 16 lanes a row
+template <typename T>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const T* g, int64_t g_row, int64_t g_head, const T* out, int64_t tq,
+                                                         int heads, int dim, float* delta) {
+  const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int sub = threadIdx.x & 15;
+  const int64_t tok = at / heads;
+  const int head = (int)(at % heads);
+  float s = 0.f;
+  if (tok < tq) {
+    const T *gp = g + tok * g_row + head * g_head, *op = out + at * dim;
+    for (int d = sub * 8; d < dim; d += 128) {
+      const Raw8<T> x = raw_load(gp + d), y = raw_load(op + d);
+      const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (float)xe[e] * (float)ye[e];
+    }
+  }
+#pragma unroll
+  for (int off = 8; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+  if (tok < tq && sub == 0) delta[head * tq + tok] = s;
+}
+
+// Gradients of keys and values. One workgroup: 32 WM keys of one key head; wave (wm, rw) holds 32 keys and walks the
+// tiles rw, rw + RW, ... of 32 packed query rows. S = Q K^T (lane: a key, registers: query rows), so exp(S - lse) and
+// dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of the group.
+template <typename T, int DP, int WM, int RW>
+__global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
+  constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
+  using Tile = AttnTile<NP, BR, DP>;
+  constexpr int kGroup = 2 * Tile::SIZE + 4 * BR;  // Q, G, lse and delta of BR rows (bf16 units)
+  constexpr int kMerge = (RW - 1) * WM * DB * 16 * 64 * 2;
+  __shared__ __attribute__((aligned(16))) __bf16 lds[RW * kGroup > kMerge ? RW * kGroup : kMerge];
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, rw = wave / WM;
+  const int kvh = blockIdx.x % a.kv_heads;
+  int64_t first;
+  const int ext = attn_find(a.k_off, a.segments, a.tk, 1, 32 * WM, blockIdx.x / a.kv_heads, &first);
+  AttnSegment sg = attn_segment(a, ext);
+  if (!attn_real(a, ext)) sg.nq = 0;
+  if (first >= sg.nk) return;
+  const int key0 = (int)first, key = key0 + 32 * wm + (lane & 31);
+  const bool live = key < sg.nk;
+  const int64_t kt = sg.k0 + (live ? key : 0);
+  const int rows = sg.nq * a.group, shift = sg.nk - sg.nq;
+  // the first query that sees this key, and that sees any key of the workgroup
+  const int from = a.causal ? max(0, key - shift) : 0;
+  const int tile_lo = a.causal ? min(rows, max(0, key0 - shift) * a.group) / BR : 0;
+  const int tile_hi = (rows + BR - 1) / BR;
+  const int full = a.causal ? max(0, key0 + 32 * WM - 1 - shift) : 0;  // from this query on, all keys are seen
+
+  Planes<NP> kf[KS], vf[KS];
+  {
+    const T* kp = static_cast<const T*>(a.k) + kt * a.k_row + kvh * a.k_head;
+    const T* vp = static_cast<const T*>(a.v) + kt * a.v_row + kvh * a.v_head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int chunk = 2 * ks + half;
+      const bool ok = live && 8 * chunk < a.dim;
+      kf[ks] = raw_planes(ok ? raw_load(kp + 8 * chunk) : raw_zero<T>());
+      vf[ks] = raw_planes(ok ? raw_load(vp + 8 * chunk) : raw_zero<T>());
+    }
+  }
+  fmd_f32x16 ak[DB], av[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) ak[d] = av[d] = zero16();
+  const float c = a.scale * kLog2e;
+
+  __bf16* qs = lds + rw * kGroup;
+  __bf16* gs = qs + Tile::SIZE;
+  float* stat = reinterpret_cast<float*>(gs + Tile::SIZE);  // [lse (log2 units), delta][BR]
+  const int lt = threadIdx.x - rw * WM * 64;
+  const T *qb = static_cast<const T*>(a.q), *gb = static_cast<const T*>(b.g);
+  AttnLoad<T, NP, BR, DP, 64 * WM> ql, gl;
+  float st = 0.f;
+  auto issue = [&](int tile) {
+    const int r0 = tile * BR, n = tile < tile_hi ? rows - r0 : 0;
+    ql.load(lt, a.dim, [&](int i) {
+      const int r = r0 + i;
+      return i < n ? qb + (sg.q0 + r / a.group) * a.q_row + (kvh * a.group + r % a.group) * a.q_head : nullptr;
+    });
+    gl.load(lt, a.dim, [&](int i) {
+      const int r = r0 + i;
+      return i < n ? gb + (sg.q0 + r / a.group) * b.g_row + (kvh * a.group + r % a.group) * b.g_head : nullptr;
+    });
+    if (lt < 2 * BR) {
+      const int i = lt % BR, r = r0 + i;
+      const int64_t at = i < n ? (kvh * a.group + r % a.group) * a.tq + sg.q0 + r / a.group : 0;
+      // a row that sees nothing, and one past the end: exp(s - inf) = 0
+      if (lt < BR) {
+        const float x = i < n ? b.lse[at] : -INFINITY;
+        st = x == -INFINITY ? INFINITY : x * kLog2e;
+      } else {
+        st = i < n ? b.delta[at] : 0.f;
+      }
+    }
+  };
+
+  const int rounds = (max(0, tile_hi - tile_lo) + RW - 1) / RW;
+  if (rounds > 0) issue(tile_lo + rw);
+  for (int it = 0; it < rounds; ++it) {
+    const int tile = tile_lo + it * RW + rw, r0 = tile * BR;
+    __syncthreads();
+    ql.store(qs, lt);
+    gl.store(gs, lt);
+    if (lt < 2 * BR) stat[lt] = st;
+    __syncthreads();
+    if (it + 1 < rounds) issue(tile + RW);
+    if (tile >= tile_hi) continue;
+
+    fmd_f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(qs, 0, ks), kf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(gs, 0, ks), vf[ks], dp);
+    const bool masked = a.causal && r0 / a.group < full;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float4 ls = *reinterpret_cast<const float4*>(stat + 8 * r + 4 * half);
+      const float4 dl = *reinterpret_cast<const float4*>(stat + BR + 8 * r + 4 * half);
+      const float le[4] = {ls.x, ls.y, ls.z, ls.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int v = 4 * r + e;
+        float p = exp2_hw(fmaf(s[v], c, -le[e]));
+        float ds = p * (dp[v] - de[e]);
+        if (masked && (r0 + prod_row(v, half)) / a.group < from) p = ds = 0.f;
+        s[v] = p;
+        dp[v] = ds;
+      }
+    }
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      float x[8], y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = s[8 * step + e];
+        y[e] = dp[8 * step + e];
+      }
+      Planes<NP> pf, df;
+      planes_of(x, pf);
+      planes_of(y, df);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        av[d] = mma(Tile::cols(gs, 16 * step, d), pf, av[d]);
+        ak[d] = mma(Tile::cols(qs, 16 * step, d), df, ak[d]);
+      }
+    }
+  }
+
+  if constexpr (RW > 1) {  // add the row groups, in their order, one gradient after the other
+    float* mg = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+      if (rw > 0) {
+        float* w = mg + ((rw - 1) * WM + wm) * DB * 16 * 64 + lane;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) w[(d * 16 + v) * 64] = which ? av[d][v] : ak[d][v];
+      }
+      __syncthreads();
+      if (rw == 0) {
+#pragma unroll
+        for (int g = 0; g < RW - 1; ++g) {
+          const float* w = mg + (g * WM + wm) * DB * 16 * 64 + lane;
+#pragma unroll
+          for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              if (which) av[d][v] += w[(d * 16 + v) * 64];
+              else ak[d][v] += w[(d * 16 + v) * 64];
+            }
+        }
+      }
+    }
+    if (rw > 0) return;
+  }
+  if (!live) return;
+  const int64_t at = (kt * a.kv_heads + kvh) * a.dim;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int col = 32 * d + 8 * r + 4 * half;
+      if (col >= a.dim) continue;
+      const float f = a.scale;
+      store4<T>(gk + at + col, ak[d][4 * r] * f, ak[d][4 * r + 1] * f, ak[d][4 * r + 2] * f, ak[d][4 * r + 3] * f);
+      store4<T>(gv + at + col, av[d][4 * r], av[d][4 * r + 1], av[d][4 * r + 2], av[d][4 * r + 3]);
+    }
+}
+
+// Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T.
+template <typename T, int DP, int WM, int KW>
+__global__ void __launch_bounds__(64 * WM * KW) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gq) {
+  constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = 32;
+  using Tile = AttnTile<NP, BN, DP>;
+  constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * DB * 16 * 64 * 2;
+  __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, kw = wave / WM;
+  const int kvh = blockIdx.x % a.kv_heads;
+  int64_t t = blockIdx.x / a.kv_heads;
+  if (a.causal) t = tiles - 1 - t;
+  int64_t first;
+  const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first);
+  AttnSegment sg = attn_segment(a, ext);
+  if (!attn_real(a, ext)) sg.nk = 0;
+  const int rows = sg.nq * a.group;
+  if (first >= rows) return;
+  const int row0 = (int)first, row = row0 + 32 * wm + (lane & 31);
+  const bool live = row < rows;
+  const int tok = (live ? row : rows - 1) / a.group, head = kvh * a.group + (live ? row : rows - 1) % a.group;
+  const int64_t qt = sg.q0 + tok;
+  const int shift = sg.nk - sg.nq;
+  const int sees = a.causal ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
+  const int last_tok = min(row0 + 32 * WM, rows) - 1;
+  const int reach = a.causal ? max(0, min(sg.nk, last_tok / a.group + shift + 1)) : sg.nk;
+  const int least = a.causal ? max(0, min(sg.nk, row0 / a.group + shift + 1)) : sg.nk;
+  const int tile_hi = (reach + BN - 1) / BN;
+
+  Planes<NP> qf[KS], gf[KS];
+  {
+    const T* qp = static_cast<const T*>(a.q) + qt * a.q_row + head * a.q_head;
+    const T* gp = static_cast<const T*>(b.g) + qt * b.g_row + head * b.g_head;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int chunk = 2 * ks + half;
+      const bool ok = live && 8 * chunk < a.dim;
+      qf[ks] = raw_planes(ok ? raw_load(qp + 8 * chunk) : raw_zero<T>());
+      gf[ks] = raw_planes(ok ? raw_load(gp + 8 * chunk) : raw_zero<T>());
+    }
+  }
+  const float x = b.lse[head * a.tq + qt], ls = x == -INFINITY ? INFINITY : x * kLog2e;
+  const float dl = b.delta[head * a.tq + qt];
+  fmd_f32x16 o[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) o[d] = zero16();
+  const float c = a.scale * kLog2e;
+
+  __bf16* ks_ = lds + kw * 2 * Tile::SIZE;
+  __bf16* vs_ = ks_ + Tile::SIZE;
+  const int lt = threadIdx.x - kw * WM * 64;
+  const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
+  const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
+  AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
+  auto issue = [&](int tile) {
+    const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
+    kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
+    vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
+  };
+  const int rounds = (tile_hi + KW - 1) / KW;
+  if (rounds > 0) issue(kw);
+  for (int it = 0; it < rounds; ++it) {
+    const int tile = it * KW + kw, j0 = tile * BN;
+    __syncthreads();
+    kl.store(ks_, lt);
+    vl.store(vs_, lt);
+    __syncthreads();
+    if (it + 1 < rounds) issue(tile + KW);
+    if (tile >= tile_hi) continue;
+    fmd_f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, 0, ks), qf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, 0, ks), gf[ks], dp);
+    const bool masked = j0 + BN > least;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      float ds = exp2_hw(fmaf(s[v], c, -ls)) * (dp[v] - dl);
+      if (masked && j0 + prod_row(v, half) >= sees) ds = 0.f;
+      s[v] = ds;
+    }
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = s[8 * step + e];
+      Planes<NP> df;
+      planes_of(y, df);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, 16 * step, d), df, o[d]);
+    }
+  }
+  if constexpr (KW > 1) {
+    float* mg = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    if (kw > 0) {
+      float* w = mg + ((kw - 1) * WM + wm) * DB * 16 * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) w[(d * 16 + v) * 64] = o[d][v];
+    }
+    __syncthreads();
+    if (kw > 0) return;
+#pragma unroll
+    for (int g = 0; g < KW - 1; ++g) {
+      const float* w = mg + (g * WM + wm) * DB * 16 * 64 + lane;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] += w[(d * 16 + v) * 64];
+    }
+  }
+  if (!live) return;
+  T* op = gq + (qt * a.heads + head) * a.dim;
+#pragma unroll
+  for (int d = 0; d < DB; ++d)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int col = 32 * d + 8 * r + 4 * half;
+      const float f = a.scale;
+      if (col < a.dim) store4<T>(op + col, o[d][4 * r] * f, o[d][4 * r + 1] * f, o[d][4 * r + 2] * f, o[d][4 * r + 3] * f);
+    }
+}
+
+// ------------------------------------------------------------------------------------ launches
+
+// tiles of `bm` rows: the numbers that attn_find hands out
+int64_t tile_count(int64_t rows, int group, int segments, int bm) { return rows * group / bm + segments + 2; }
+
+// Rows of a tile from which its four waves take 32 rows each; below, they take the same rows and share the keys
+// (too few tiles to fill the card otherwise, and segments shorter than a tile).
+bool wide_tiles(int64_t rows, int group, int heads, int segments) {
+  return rows * group / 128 * heads >= 256 && rows * group >= (int64_t)64 * segments;
+}
+
+// Key splits of the forward: as many as bring the workgroups to four per CU, each with kSplitKeys keys at least of a
+// segment of mean length. Their partial sums (dim + 2 floats a row) are joined by a second launch.
+constexpr int kSplitKeys = 512, kSplitGroups = 1024;
+
+int split_count(int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
+  if (tq <= 0 || tk <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
+  const int group = heads / kv_heads;
+  const bool wide = wide_tiles(tq, group, kv_heads, segments);
+  const int64_t tiles = fmd_cdiv(fmd_cdiv(tq * group, segments), wide ? 128 : 32) * segments * kv_heads;
+  const int64_t fill = fmd_cdiv(kSplitGroups, tiles), most = tk / segments / kSplitKeys;
+  const int64_t n = fill < most ? fill : most;
+  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+}
+
+template <typename T, int DP>
+int run_fwd(const AttnArgs& a, int splits, T* out, float* lse, float* work, hipStream_t stream) {
+  constexpr bool f32 = AttnType<T>::planes == 3;
+  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4;
+  const int64_t n = a.tq * a.heads;
+  float *po = work, *pm = work ? work + splits * n * a.dim : nullptr, *pl = work ? pm + splits * n : nullptr;
+  if (wide_tiles(a.tq, a.group, a.kv_heads, a.segments)) {
+    const int64_t tiles = tile_count(a.tq, a.group, a.segments, 128);
+    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+    attn_fwd_kernel<T, DP, 64, 4, 1><<<dim3((unsigned)(tiles * a.kv_heads), splits), 256, 0, stream>>>(a, tiles, splits, out, lse,
+                                                                                                     po, pm, pl);
+  } else {
+    const int64_t tiles = tile_count(a.tq, a.group, a.segments, 32);
+    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+    attn_fwd_kernel<T, DP, 32, 1, kKeyWaves><<<dim3((unsigned)(tiles * a.kv_heads), splits), 64 * kKeyWaves, 0, stream>>>(
+        a, tiles, splits, out, lse, po, pm, pl);
+  }
+  FMD_CHECK_LAUNCH();
+  if (splits > 1) {
+    attn_join_kernel<T><<<(unsigned)fmd_cdiv(n, 4), 256, 0, stream>>>(a, splits, po, pm, pl, out, lse);
+    FMD_CHECK_LAUNCH();
+  }
+  return FMD_OK;
+}
+
+template <typename T, int DP>
+int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream) {
+  constexpr bool f32 = AttnType<T>::planes == 3;
+  constexpr int kWaves = f32 && DP > 64 ? 2 : 4;
+  if (gk) {
+    if (wide_tiles(a.tk, 1, a.kv_heads, a.segments)) {
+      const int64_t tiles = tile_count(a.tk, 1, a.segments, 128);
+      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+      attn_bwd_kv_kernel<T, DP, 4, 1><<<(unsigned)(tiles * a.kv_heads), 256, 0, stream>>>(a, b, tiles, gk, gv);
+    } else {
+      const int64_t tiles = tile_count(a.tk, 1, a.segments, 32);
+      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+      attn_bwd_kv_kernel<T, DP, 1, kWaves><<<(unsigned)(tiles * a.kv_heads), 64 * kWaves, 0, stream>>>(a, b, tiles, gk, gv);
+    }
+    FMD_CHECK_LAUNCH();
+  }
+  if (gq) {
+    if (wide_tiles(a.tq, a.group, a.kv_heads, a.segments)) {
+      const int64_t tiles = tile_count(a.tq, a.group, a.segments, 128);
+      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+      attn_bwd_q_kernel<T, DP, 4, 1><<<(unsigned)(tiles * a.kv_heads), 256, 0, stream>>>(a, b, tiles, gq);
+    } else {
+      const int64_t tiles = tile_count(a.tq, a.group, a.segments, 32);
+      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+      attn_bwd_q_kernel<T, DP, 1, kWaves><<<(unsigned)(tiles * a.kv_heads), 64 * kWaves, 0, stream>>>(a, b, tiles, gq);
+    }
+    FMD_CHECK_LAUNCH();
+  }
+  return FMD_OK;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// what the kernels' 16-byte loads and index arithmetic assume
+int check(const AttnArgs& a, int size) {
+  FMD_REQUIRE(a.tq >= 0 && a.tk >= 0 && a.segments >= 0 && a.heads > 0 && a.kv_heads > 0 && a.dim > 0);
+  FMD_REQUIRE(a.heads % a.kv_heads == 0 && a.q_off && a.k_off);
+  FMD_REQUIRE(a.tq * a.group < (1ll << 31) && a.tk < (1ll << 31) && a.segments < (1 << 30));
+  if (a.dim > 128 || a.dim % 8 != 0) return FMD_EUNSUPPORTED;
+  FMD_REQUIRE((a.q || a.tq == 0) && (a.tk == 0 || (a.k && a.v)));
+  const int64_t unit = 16 / size;
+  FMD_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v));
+  FMD_REQUIRE(a.q_row % unit == 0 && a.q_head % unit == 0 && a.k_row % unit == 0 && a.k_head % unit == 0 &&
+              a.v_row % unit == 0 && a.v_head % unit == 0);
+  FMD_REQUIRE(a.scale > 0.f);
+  return FMD_OK;
+}
+
+template <typename T>
+int forward(const AttnArgs& a, int splits, T* out, float* lse, float* work, hipStream_t stream) {
+  const int status = check(a, sizeof(T));
+  if (status != FMD_OK) return status;
+  FMD_REQUIRE(splits >= 1 && splits <= 1024 && (splits == 1 || work));
+  if (a.tq == 0) return FMD_OK;
+  FMD_REQUIRE(out && aligned16(out));
+  if (a.dim <= 32) return run_fwd<T, 32>(a, splits, out, lse, work, stream);
+  if (a.dim <= 64) return run_fwd<T, 64>(a, splits, out, lse, work, stream);
+  if (a.dim <= 96) return run_fwd<T, 96>(a, splits, out, lse, work, stream);
+  return run_fwd<T, 128>(a, splits, out, lse, work, stream);
+}
+
+template <typename T>
+int backward(const AttnArgs& a, AttnBwd b, const T* out, T* gq, T* gk, T* gv, float* delta, hipStream_t stream) {
+  const int status = check(a, sizeof(T));
+  if (status != FMD_OK) return status;
+  const int64_t unit = 16 / sizeof(T);
+  FMD_REQUIRE(a.tq == 0 || (b.g && out && b.lse && delta && aligned16(b.g) && aligned16(out)));
+  FMD_REQUIRE(b.g_row % unit == 0 && b.g_head % unit == 0);
+  FMD_REQUIRE((gk == nullptr) == (gv == nullptr) && aligned16(gq) && aligned16(gk) && aligned16(gv));
+  b.delta = delta;
+  if (a.tq > 0) {
+    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(
+        static_cast<const T*>(b.g), b.g_row, b.g_head, out, a.tq, a.heads, a.dim, delta);
+    FMD_CHECK_LAUNCH();
+  }
+  if (a.tq == 0) gq = nullptr;
+  if (a.tk == 0) gk = gv = nullptr;
+  if (a.dim <= 32) return run_bwd<T, 32>(a, b, gq, gk, gv, stream);
+  if (a.dim <= 64) return run_bwd<T, 64>(a, b, gq, gk, gv, stream);
+  if (a.dim <= 96) return run_bwd<T, 96>(a, b, gq, gk, gv, stream);
+  return run_bwd<T, 128>(a, b, gq, gk, gv, stream);
+}
+
+AttnArgs args_of(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
+                 int64_t v_row, int64_t v_head, const int64_t* q_off, const int64_t* k_off, int64_t tq, int64_t tk,
+                 int32_t segments, int32_t heads, int32_t kv_heads, int32_t dim, int32_t causal, float scale) {
+  AttnArgs a = {};
+  a.q = q, a.k = k, a.v = v;
+  a.q_row = q_row, a.q_head = q_head, a.k_row = k_row, a.k_head = k_head, a.v_row = v_row, a.v_head = v_head;
+  a.q_off = q_off, a.k_off = k_off, a.tq = tq, a.tk = tk;
+  a.segments = segments, a.heads = heads, a.kv_heads = kv_heads, a.group = kv_heads > 0 ? heads / kv_heads : 0;
+  a.dim = dim, a.causal = causal, a.scale = scale;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+#define FMD_ATTN_PARAMS                                                                                          \
+  const void *q, int64_t q_row, int64_t q_head, const void *k, int64_t k_row, int64_t k_head, const void *v,     \
+      int64_t v_row, int64_t v_head, const int64_t *q_offsets, const int64_t *k_offsets, int64_t tq, int64_t tk, \
+      int32_t segments, int32_t heads, int32_t kv_heads, int32_t dim, int32_t causal, float scale
+#define FMD_ATTN_ARGS                                                                                            \
+  args_of(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, q_offsets, k_offsets, tq, tk, segments, heads,   \
+          kv_heads, dim, causal, scale)
+
+int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads) {
+  return split_count(tq, tk, segments, heads, kv_heads);
+}
+
+int64_t fmd_segment_attention_work_size(int32_t splits, int64_t tq, int32_t heads, int32_t dim) {
+  return splits > 1 && tq > 0 && heads > 0 && dim > 0 ? (int64_t)splits * tq * heads * (dim + 2) : 0;
+}
+
+int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* out, float* lse, float* work,
+                          hipStream_t stream) {
+  const AttnArgs a = FMD_ATTN_ARGS;
+  return bf16 ? forward(a, splits, static_cast<__bf16*>(out), lse, work, stream)
+              : forward(a, splits, static_cast<float*>(out), lse, work, stream);
+}
+
+int fmd_segment_attention_bwd(int32_t bf16, FMD_ATTN_PARAMS, const void* gout, int64_t g_row, int64_t g_head, const void* out,
+                              const float* lse, float* delta, void* gq, void* gk, void* gv, hipStream_t stream) {
+  const AttnArgs a = FMD_ATTN_ARGS;
+  const AttnBwd b = {gout, g_row, g_head, lse, delta};
+  return bf16 ? backward(a, b, static_cast<const __bf16*>(out), static_cast<__bf16*>(gq), static_cast<__bf16*>(gk),
+                         static_cast<__bf16*>(gv), delta, stream)
+              : backward(a, b, static_cast<const float*>(out), static_cast<float*>(gq), static_cast<float*>(gk),
+                         static_cast<float*>(gv), delta, stream);
+}
+
+}  // extern "C"

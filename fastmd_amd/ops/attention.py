@@ -1,0 +1,176 @@
+"""(g) Attention within segments on the GPU (HIP kernels), with a deterministic VJP.
+
+``segment_attention(q, k, v, q_offsets, k_offsets=None, causal=False, scale=None)``:
+
+    out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h // group]) v[j, h // group]
+
+over the key rows j of query i's segment. Segment s has the query rows ``[q_offsets[s], q_offsets[s + 1])`` and the
+key rows ``[k_offsets[s], k_offsets[s + 1])``; the offsets are those of a CSR over sorted rows (the atoms of each system
+of a batch, the neighbour rows of each atom, packed sequences), read on the device only: a call neither
+synchronises nor depends on lengths that the host would have to know. ``group = heads / kv_heads`` query heads share a
+key head. ``causal``: the last query of a segment sees all its keys, each one before it one key less. A query that sees
+no key, and a row outside every segment (the unused rows of a fixed-capacity buffer), gives zero and gets zero gradient;
+rows outside a query's segment are not read for it, whatever they hold.
+
+float32 is computed on the bf16 matrix cores with every operand split into three planes (float32 accuracy; an
+infinite value in a row that is seen gives NaN), bfloat16 with products of bfloat16 operands. Scores, softmax statistics
+and sums are float32 in both. For bfloat16, the probabilities and (in the VJP) the score gradients are rounded to
+bfloat16 as operands of the second product, as the inputs and outputs are. Gradients take no atomics: the same call gives
+the same bits.
+"""
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+from torch.autograd import Function
+
+from fastmd_amd import _abi
+from fastmd_amd._device import require_cuda, stream
+
+MAX_DIM = 128
+
+
+def heads_view(x: Tensor) -> tuple[Tensor, int, int]:
+    """(tensor, row stride, head stride) of ``x`` [rows, heads, dim] with unit stride in dim and 16-byte aligned rows;
+    copies only when needed (any strides otherwise: columns of a packed projection are read in place)."""
+    rows, heads, dim = x.shape
+    unit = 16 // x.element_size()
+    sr, sh, sd = x.stride()
+    if rows <= 1:
+        sr = heads * dim
+    if heads <= 1:
+        sh = dim
+    if (sd != 1 and dim > 1) or sr % unit or sh % unit or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        sr, sh = heads * dim, dim
+    return x, sr, sh
+
+
+def _check(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor, scale) -> float:
+    require_cuda(q, k, v, q_offsets, k_offsets)
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"q, k and v must be [rows, heads, dim], got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v must all be float32 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if k.shape != v.shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    heads, dim, kv_heads = q.shape[1], q.shape[2], k.shape[1]
+    if k.shape[2] != dim:
+        raise ValueError(f"q and k must have one head width, got {dim} and {k.shape[2]}")
+    if dim % 8 or not 8 <= dim <= MAX_DIM:
+        raise ValueError(f"the head width must be a multiple of 8 up to {MAX_DIM}, got {dim}")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"the query heads must be a multiple of the key heads, got {heads} and {kv_heads}")
+    for name, off in (("q_offsets", q_offsets), ("k_offsets", k_offsets)):
+        if off.dim() != 1 or off.numel() < 1 or off.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be an integer vector [segments + 1]")
+    if q_offsets.numel() != k_offsets.numel():
+        raise ValueError(f"q_offsets has {q_offsets.numel() - 1} segments, k_offsets {k_offsets.numel() - 1}")
+    if q.shape[0] * heads // kv_heads >= 2 ** 31 or k.shape[0] >= 2 ** 31:
+        raise ValueError("segment attention takes fewer than 2^31 packed query rows and key rows")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
+
+
+def _offsets(off: Tensor) -> Tensor:
+    if off.dtype != torch.int64 or not off.is_contiguous():
+        off = off.to(torch.int64).contiguous()
+    return off
+
+
+def _common(q, k, v, q_offsets, k_offsets, causal, scale):
+    """The arguments that both directions share, and the tensors that they point into."""
+    (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = heads_view(q), heads_view(k), heads_view(v)
+    same = k_offsets is q_offsets
+    q_offsets = _offsets(q_offsets)
+    k_offsets = q_offsets if same else _offsets(k_offsets)
+    args = (1 if q.dtype == torch.bfloat16 else 0, q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head,
+            v.data_ptr(), v_row, v_head, q_offsets.data_ptr(), k_offsets.data_ptr(), q.shape[0], k.shape[0],
+            q_offsets.numel() - 1, q.shape[1], k.shape[1], q.shape[2], 1 if causal else 0, scale)
+    return args, (q, k, v, q_offsets, k_offsets)
+
+
+def _forward(q, k, v, q_offsets, k_offsets, causal, scale, with_lse):
+    args, keep = _common(q, k, v, q_offsets, k_offsets, causal, scale)
+    tq, heads, dim = q.shape
+    out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((heads, tq), dtype=torch.float32, device=q.device) if with_lse else None
+    lib = _abi.load()
+    splits = lib.fmd_segment_attention_splits(tq, k.shape[0], args[14], heads, k.shape[1])
+    work = None
+    if splits > 1:
+        work = torch.empty(lib.fmd_segment_attention_work_size(splits, tq, heads, dim), dtype=torch.float32,
+                           device=q.device)
+    _abi.call("fmd_segment_attention", *args, splits, out.data_ptr(), _abi.ptr(lse), _abi.ptr(work), stream())
+    del keep
+    return out, lse
+
+
+def segment_attention_forward(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor | None = None, *,
+                              causal: bool = False, scale: float | None = None) -> tuple[Tensor, Tensor]:
+    """``(out, lse)`` without autograd: the output and the logarithm of each row's sum of exponentials (float32
+    [heads, rows], -inf for a row that sees no key), which ``segment_attention_vjp`` takes."""
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    scale = _check(q, k, v, q_offsets, k_offsets, scale)
+    return _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
+
+
+def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, q_offsets: Tensor,
+                          k_offsets: Tensor | None = None, *, causal: bool = False, scale: float | None = None,
+                          need_q: bool = True, need_kv: bool = True):
+    """``(gq, gk, gv)`` from the gradient of the output and the results of ``segment_attention_forward`` (None where
+    not needed; the gradients of k and v come together)."""
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    scale = _check(q, k, v, q_offsets, k_offsets, scale)
+    require_cuda(q, gout, out, lse)
+    if gout.shape != q.shape or gout.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"gout and out must be {q.dtype} {tuple(q.shape)}, got {gout.dtype} {tuple(gout.shape)} and "
+                         f"{out.dtype} {tuple(out.shape)}")
+    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 {(q.shape[1], q.shape[0])}, got {lse.dtype} {tuple(lse.shape)}")
+    args, keep = _common(q, k, v, q_offsets, k_offsets, causal, scale)
+    gout, g_row, g_head = heads_view(gout)
+    out, lse = out.contiguous(), lse.contiguous()
+    if out.data_ptr() % 16:
+        out = out.clone()
+    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
+    gk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None
+    gv = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None
+    delta = torch.empty_like(lse)
+    _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), lse.data_ptr(),
+              delta.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
+    del keep
+    return gq, gk, gv
+
+
+class _SegmentAttention(Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale):
+        out, lse = _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, q_offsets, k_offsets)
+        ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    def backward(ctx, gout):
+        q, k, v, out, lse, q_offsets, k_offsets = ctx.saved_tensors
+        grads = segment_attention_vjp(gout, q, k, v, out, lse, q_offsets, k_offsets, causal=ctx.causal,
+                                      scale=ctx.scale, need_q=ctx.needs_input_grad[0],
+                                      need_kv=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return (*grads, None, None, None, None)
+
+
+def segment_attention(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor | None = None, *,
+                      causal: bool = False, scale: float | None = None) -> Tensor:
+    """Attention within segments (see the module): ``q`` [rows, heads, dim], ``k`` and ``v`` [key rows, kv_heads, dim],
+    float32 or bfloat16, any strides; offsets [segments + 1] on the device (``k_offsets`` None: ``q_offsets``); ``scale``
+    None: ``dim ** -0.5``. One query per segment (the next token of a sequence over its cache, an atom over its neighbours) is the
+    same call: a long key axis is then split over the card and joined. Differentiable in q, k and v."""
+    k_offsets = q_offsets if k_offsets is None else k_offsets
+    scale = _check(q, k, v, q_offsets, k_offsets, scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _SegmentAttention.apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
+    return _forward(q, k, v, q_offsets, k_offsets, causal, scale, False)[0]

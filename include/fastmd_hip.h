@@ -813,6 +813,61 @@ int64_t fmd_edge_virial_work_size(void);
 int fmd_edge_stress_f32(const float* geo, const float* gvec, const int64_t* n_edges, int64_t e_cap, const float* cell,
                         double* work, float* stress, hipStream_t stream);
 
+/* ----------------------------------------------------------------------------------------
+ * (g) Attention within segments, and the norm and rotation of its queries and keys. Not in the
+ * reference. `bf16`: 1 for bf16 storage of all feature buffers, 0 for float32.
+ * -------------------------------------------------------------------------------------- */
+
+/* out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / (heads / kv_heads)]) v[j, .] over the key rows j of query i's
+ * segment: segment s has the query rows [q_offsets[s], q_offsets[s + 1]) and the key rows
+ * [k_offsets[s], k_offsets[s + 1]) (device int64, ascending; every offset is clamped into the buffer). causal: query i of
+ * n sees the first i + m - n + 1 of the m keys. A query that sees no key, and one outside every segment, gives zero.
+ * q [tq, heads, dim], k and v [tk, kv_heads, dim] with row and head strides in elements (unit stride in dim, 16-byte
+ * aligned rows); dim a multiple of 8 up to 128 (FMD_EUNSUPPORTED otherwise); scale > 0. out [tq, heads, dim] contiguous;
+ * lse [heads, tq] (nullable): log of the sum of exponentials, -inf for a row that sees nothing.
+ * splits: fmd_segment_attention_splits(); with more than one, `work` holds fmd_segment_attention_work_size() floats. */
+int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads);
+int64_t fmd_segment_attention_work_size(int32_t splits, int64_t tq, int32_t heads, int32_t dim);
+int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                          int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
+                          const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
+                          int32_t kv_heads, int32_t dim, int32_t causal, float scale, int32_t splits, void* out,
+                          float* lse, float* work, hipStream_t stream);
+
+/* VJP of fmd_segment_attention: gq [tq, heads, dim], gk and gv [tk, kv_heads, dim] (contiguous; gq, or gk and gv
+ * together, nullable) from the gradient `gout` of `out`, the forward's `out` and `lse`. Rows outside every segment get
+ * zero. delta: scratch of heads * tq floats. No atomics: the same inputs give the same bits. */
+int fmd_segment_attention_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                              int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
+                              const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
+                              int32_t kv_heads, int32_t dim, int32_t causal, float scale, const void* gout, int64_t g_row,
+                              int64_t g_head, const void* out, const float* lse, float* delta, void* gq, void* gk, void* gv,
+                              hipStream_t stream);
+
+/* Each head x of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (row and head strides in elements, 16-byte aligned
+ * rows, dim a multiple of 8 up to 256): with norm, x (mean x^2 + eps)^(-1/2) weight (weights [dim] of the features' type,
+ * null: ones); then its first `rot` columns turned by the token's angles: columns (i, i + rot / 2), or (2 i, 2 i + 1) when
+ * interleaved, by cos_table / sin_table [table_rows, rot / 2] (float32, row stride table_ld, 16-byte aligned base) at row
+ * positions[token] (int32, or int64 with positions64; null: the token itself). A position outside the table gives NaN in
+ * the turned columns. heads or kv_heads may be 0. Outputs contiguous. */
+int fmd_qk_norm_rotary(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, int32_t heads, const void* k,
+                       int64_t k_row, int64_t k_head, int32_t kv_heads, int64_t tokens, int32_t dim, int32_t norm, float eps,
+                       const void* q_weight, const void* k_weight, const float* cos_table, const float* sin_table,
+                       int64_t table_rows, int64_t table_ld, int32_t rot, int32_t interleaved, const void* positions,
+                       int32_t positions64, void* q_out, void* k_out, hipStream_t stream);
+
+/* VJP of fmd_qk_norm_rotary from the gradients of its outputs (strided as q and k): gq, gk (contiguous) and, with norm,
+ * gq_weight and gk_weight [dim] (each nullable), summed over tokens and heads in fp32 in a fixed order through `work`
+ * (fmd_qk_norm_rotary_work_size() floats). */
+int64_t fmd_qk_norm_rotary_work_size(int64_t tokens, int32_t heads, int32_t kv_heads, int32_t dim);
+int fmd_qk_norm_rotary_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, int32_t heads, const void* k,
+                           int64_t k_row, int64_t k_head, int32_t kv_heads, int64_t tokens, int32_t dim, int32_t norm,
+                           float eps, const void* q_weight, const void* k_weight, const float* cos_table,
+                           const float* sin_table, int64_t table_rows, int64_t table_ld, int32_t rot, int32_t interleaved,
+                           const void* positions, int32_t positions64, const void* gq_out, int64_t gq_row, int64_t gq_head,
+                           const void* gk_out, int64_t gk_row, int64_t gk_head, void* gq, void* gk, void* gq_weight,
+                           void* gk_weight, float* work, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
