@@ -23,6 +23,22 @@ struct AttnArgs {
   float scale;
 };
 
+// What the VJP needs of the forward besides its output. A row's probabilities are exp2(s scale log2(e) - base) inverse; its
+// output before rounding is out + residual (bf16: delta = g . o cancels against g . v where few keys count, and the rounding
+// of the output alone took the error of gq and gk from 1.4 to 1.7 times that of rounding them).
+struct AttnSaved {
+  float *base, *inverse;  // [heads, tq]: largest scaled score in log2 units, 1 / row sum (both 0 for a row that sees nothing)
+  void* residual;         // bf16 only: [tq, heads, dim]
+};
+
+struct AttnBwd {
+  const void* g;  // gradient of the output
+  int64_t g_row, g_head;
+  const void* out;
+  AttnSaved saved;
+  const float* delta;  // [heads, tq]
+};
+
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A segment with its rows. The kernels see segments + 2 of them: the rows before the first offset and after the
@@ -243,6 +259,16 @@ __device__ __forceinline__ float max_halves(float x) {
   return fmaxf(x, y);
 }
 
+// sum over aligned groups of LG <= 16 lanes, on the DPP paths
+template <int LG>
+__device__ __forceinline__ float lanes_sum(float x) {
+  if (LG >= 2) x += dpp_read<kDppQuadXor1>(x);
+  if (LG >= 4) x += dpp_read<kDppQuadXor2>(x);
+  if (LG >= 8) x += dpp_read<kDppHalfMirror>(x);
+  if (LG >= 16) x += dpp_read<kDppRowRor8>(x);
+  return x;
+}
+
 template <typename T>
 __device__ __forceinline__ void store4(T* p, float a, float b, float c, float d);
 template <>
@@ -258,3 +284,23 @@ __device__ __forceinline__ void store4<__bf16>(__bf16* p, float a, float b, floa
   v[3] = (__bf16)d;
   *reinterpret_cast<fmd_bf16x4*>(p) = v;
 }
+
+// the part of eight (four) outputs that their rounding to bf16 dropped
+template <typename T, int N>
+__device__ __forceinline__ void saved_residual(const AttnSaved& s, int64_t at, const float (&o)[N]) {
+  if constexpr (sizeof(T) == 2) {
+    if (s.residual) {
+      T* p = static_cast<T*>(s.residual) + at;
+#pragma unroll
+      for (int e = 0; e < N; e += 4)
+        store4<T>(p + e, o[e] - (float)(T)o[e], o[e + 1] - (float)(T)o[e + 1], o[e + 2] - (float)(T)o[e + 2],
+                  o[e + 3] - (float)(T)o[e + 3]);
+    }
+  }
+}
+
+// attention_rows.hip
+template <typename T>
+int attn_rows_fwd(const AttnArgs& a, T* out, const AttnSaved& saved, hipStream_t stream);
+template <typename T>
+int attn_rows_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream);

@@ -12,7 +12,7 @@ namespace {
 // O^T = V^T P^T. Statistics and sums are fp32; P is rounded to bf16 for bf16 inputs (the output is, too) and kept as
 // three planes for fp32.
 template <typename T, int DP, int BN, int WM, int KW>
-__global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int64_t tiles, int splits, T* out, float* lse,
+__global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int64_t tiles, int splits, T* out, AttnSaved saved,
                                                                 float* part_o, float* part_m, float* part_l) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, JB = BN / 32;
   using Tile = AttnTile<NP, BN, DP>;
@@ -170,16 +170,21 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int6
 
   if (splits == 1) {
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;  // a row that sees no key gives zero
-    T* op = out + (qt * a.heads + head) * a.dim;
+    const int64_t at = (qt * a.heads + head) * a.dim;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int col = 32 * d + 8 * r + 4 * half;
-        if (col < a.dim)
-          store4<T>(op + col, o[d][4 * r] * inv, o[d][4 * r + 1] * inv, o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv);
+        if (col >= a.dim) continue;
+        const float x[4] = {o[d][4 * r] * inv, o[d][4 * r + 1] * inv, o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv};
+        store4<T>(out + at + col, x[0], x[1], x[2], x[3]);
+        saved_residual<T>(saved, at + col, x);
       }
-    if (lse && half == 0) lse[head * a.tq + qt] = l == 0.f ? -INFINITY : (m * c + __log2f(l)) * kLn2;
+    if (saved.base && half == 0) {
+      saved.base[head * a.tq + qt] = m == -INFINITY ? 0.f : m * c;
+      saved.inverse[head * a.tq + qt] = inv;
+    }
   } else {
     const int64_t at = ((int64_t)blockIdx.y * a.tq + qt) * a.heads + head;
     float* op = part_o + at * a.dim;
@@ -200,7 +205,7 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int6
 // The splits of a row joined in their order: one wave per (query, head), the lanes along dim.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, const float* part_o, const float* part_m,
-                                                        const float* part_l, T* out, float* lse) {
+                                                        const float* part_l, T* out, AttnSaved saved) {
   const int64_t n = a.tq * a.heads, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (at >= n) return;
@@ -219,38 +224,40 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, 
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
   for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < a.dim) out[at * a.dim + lane + 64 * k] = (T)(o[k] * inv);
-  if (lse && lane == 0) lse[(at % a.heads) * a.tq + at / a.heads] = l == 0.f ? -INFINITY : (top * c + __log2f(l)) * kLn2;
+    if (lane + 64 * k < a.dim) {
+      const int64_t i = at * a.dim + lane + 64 * k;
+      const float x = o[k] * inv;
+      out[i] = (T)x;
+      if (sizeof(T) == 2 && saved.residual) static_cast<T*>(saved.residual)[i] = (T)(x - (float)(T)x);
+    }
+  if (saved.base && lane == 0) {
+    saved.base[(at % a.heads) * a.tq + at / a.heads] = base;
+    saved.inverse[(at % a.heads) * a.tq + at / a.heads] = inv;
+  }
 }
 
 // ------------------------------------------------------------------------------------ backward
 
-struct AttnBwd {
-  const void* g;  // gradient of the output
-  int64_t g_row, g_head;
-  const float *lse, *delta;  // [heads, tq]
-};
-
 // delta[head, i] = g_i . o_i : 16 lanes a row
 template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const T* g, int64_t g_row, int64_t g_head, const T* out, int64_t tq,
-                                                         int heads, int dim, float* delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, int heads, int dim, float* delta) {
   const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int sub = threadIdx.x & 15;
   const int64_t tok = at / heads;
   const int head = (int)(at % heads);
   float s = 0.f;
   if (tok < tq) {
-    const T *gp = g + tok * g_row + head * g_head, *op = out + at * dim;
-    for (int d = sub * 8; d < dim; d += 128) {
-      const Raw8<T> x = raw_load(gp + d), y = raw_load(op + d);
-      const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y);
+    const T *gp = static_cast<const T*>(b.g) + tok * b.g_row + head * b.g_head, *op = static_cast<const T*>(b.out) + at * dim;
+    const T* rp = static_cast<const T*>(b.saved.residual) + at * dim;
+    const int d = sub * 8;
+    if (d < dim) {
+      const Raw8<T> x = raw_load(gp + d), y = raw_load(op + d), z = sizeof(T) == 2 ? raw_load(rp + d) : raw_zero<T>();
+      const T *xe = reinterpret_cast<const T*>(&x), *ye = reinterpret_cast<const T*>(&y), *ze = reinterpret_cast<const T*>(&z);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += (float)xe[e] * (float)ye[e];
+      for (int e = 0; e < 8; ++e) s += (float)xe[e] * ((float)ye[e] + (float)ze[e]);
     }
   }
-#pragma unroll
-  for (int off = 8; off >= 1; off >>= 1) s += __shfl_xor(s, off, 64);
+  s = lanes_sum<16>(s);
   if (tok < tq && sub == 0) delta[head * tq + tok] = s;
 }
 
@@ -261,7 +268,7 @@ template <typename T, int DP, int WM, int RW>
 __global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
   using Tile = AttnTile<NP, BR, DP>;
-  constexpr int kGroup = 2 * Tile::SIZE + 4 * BR;  // Q, G, lse and delta of BR rows (bf16 units)
+  constexpr int kGroup = 2 * Tile::SIZE + 6 * BR;  // Q, G, base, delta and inverse of BR rows (bf16 units)
   constexpr int kMerge = (RW - 1) * WM * DB * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[RW * kGroup > kMerge ? RW * kGroup : kMerge];
 
@@ -303,11 +310,15 @@ __global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, A
 
   __bf16* qs = lds + rw * kGroup;
   __bf16* gs = qs + Tile::SIZE;
-  float* stat = reinterpret_cast<float*>(gs + Tile::SIZE);  // [lse (log2 units), delta][BR]
+  // [base, delta, inverse][BR]; bf16 takes the inverse into the exponent (the rounding of their sum, 2^-24 of it, is far
+  // below the rounding of P), fp32 multiplies
+  float* stat = reinterpret_cast<float*>(gs + Tile::SIZE);
+  constexpr int kStats = NP == 3 ? 3 * BR : 2 * BR;
   const int lt = threadIdx.x - rw * WM * 64;
   const T *qb = static_cast<const T*>(a.q), *gb = static_cast<const T*>(b.g);
   AttnLoad<T, NP, BR, DP, 64 * WM> ql, gl;
-  float st = 0.f;
+  constexpr int kStatLoads = (kStats + 64 * WM - 1) / (64 * WM);
+  float st[kStatLoads];
   auto issue = [&](int tile) {
     const int r0 = tile * BR, n = tile < tile_hi ? rows - r0 : 0;
     ql.load(lt, a.dim, [&](int i) {
@@ -318,16 +329,15 @@ __global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, A
       const int r = r0 + i;
       return i < n ? gb + (sg.q0 + r / a.group) * b.g_row + (kvh * a.group + r % a.group) * b.g_head : nullptr;
     });
-    if (lt < 2 * BR) {
-      const int i = lt % BR, r = r0 + i;
+    for (int n_ = 0; n_ < kStatLoads; ++n_) {
+      const int x = lt + n_ * 64 * WM, i = x % BR, r = r0 + i;
+      if (x >= kStats) break;
       const int64_t at = i < n ? (kvh * a.group + r % a.group) * a.tq + sg.q0 + r / a.group : 0;
+      const float inv = i < n && x / BR != 1 ? b.saved.inverse[at] : 0.f;
       // a row that sees nothing, and one past the end: exp(s - inf) = 0
-      if (lt < BR) {
-        const float x = i < n ? b.lse[at] : -INFINITY;
-        st = x == -INFINITY ? INFINITY : x * kLog2e;
-      } else {
-        st = i < n ? b.delta[at] : 0.f;
-      }
+      if (x < BR) st[n_] = inv == 0.f ? INFINITY : NP == 3 ? b.saved.base[at] : b.saved.base[at] - __log2f(inv);
+      else if (x < 2 * BR) st[n_] = i < n ? b.delta[at] : 0.f;
+      else st[n_] = inv;
     }
   };
 
@@ -338,7 +348,9 @@ __global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, A
     __syncthreads();
     ql.store(qs, lt);
     gl.store(gs, lt);
-    if (lt < 2 * BR) stat[lt] = st;
+#pragma unroll
+    for (int n = 0; n < kStatLoads; ++n)
+      if (lt + n * 64 * WM < kStats) stat[lt + n * 64 * WM] = st[n];
     __syncthreads();
     if (it + 1 < rounds) issue(tile + RW);
     if (tile >= tile_hi) continue;
@@ -353,11 +365,13 @@ __global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, A
     for (int r = 0; r < 4; ++r) {
       const float4 ls = *reinterpret_cast<const float4*>(stat + 8 * r + 4 * half);
       const float4 dl = *reinterpret_cast<const float4*>(stat + BR + 8 * r + 4 * half);
-      const float le[4] = {ls.x, ls.y, ls.z, ls.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
+      const float4 iv = NP == 3 ? *reinterpret_cast<const float4*>(stat + 2 * BR + 8 * r + 4 * half) : make_float4(1.f, 1.f, 1.f, 1.f);
+      const float le[4] = {ls.x, ls.y, ls.z, ls.w}, de[4] = {dl.x, dl.y, dl.z, dl.w}, ie[4] = {iv.x, iv.y, iv.z, iv.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int v = 4 * r + e;
         float p = exp2_hw(fmaf(s[v], c, -le[e]));
+        if (NP == 3) p *= ie[e];
         float ds = p * (dp[v] - de[e]);
         if (masked && (r0 + prod_row(v, half)) / a.group < from) p = ds = 0.f;
         s[v] = p;
@@ -469,8 +483,8 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_bwd_q_kernel(AttnArgs a, At
       gf[ks] = raw_planes(ok ? raw_load(gp + 8 * chunk) : raw_zero<T>());
     }
   }
-  const float x = b.lse[head * a.tq + qt], ls = x == -INFINITY ? INFINITY : x * kLog2e;
-  const float dl = b.delta[head * a.tq + qt];
+  const float inv = b.saved.inverse[head * a.tq + qt], ls = inv == 0.f ? INFINITY : b.saved.base[head * a.tq + qt];
+  const float dl = b.delta[head * a.tq + qt] * inv;
   fmd_f32x16 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = zero16();
@@ -505,7 +519,7 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_bwd_q_kernel(AttnArgs a, At
     const bool masked = j0 + BN > least;
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
-      float ds = exp2_hw(fmaf(s[v], c, -ls)) * (dp[v] - dl);
+      float ds = exp2_hw(fmaf(s[v], c, -ls)) * fmaf(dp[v], inv, -dl);
       if (masked && j0 + prod_row(v, half) >= sees) ds = 0.f;
       s[v] = ds;
     }
@@ -564,12 +578,18 @@ bool wide_tiles(int64_t rows, int group, int heads, int segments) {
   return rows * group / 128 * heads >= 256 && rows * group >= (int64_t)64 * segments;
 }
 
+// About one query per segment over a few keys each, and enough segments to fill the card with a wave each: the row kernels.
+bool few_rows(int64_t tq, int64_t tk, int segments, int kv_heads) {
+  return segments >= 256 && tq <= segments && tk <= (int64_t)128 * segments;
+}
+
 // Key splits of the forward: as many as bring the workgroups to four per CU, each with kSplitKeys keys at least of a
 // segment of mean length. Their partial sums (dim + 2 floats a row) are joined by a second launch.
 constexpr int kSplitKeys = 512, kSplitGroups = 1024;
 
 int split_count(int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
   if (tq <= 0 || tk <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
+  if (few_rows(tq, tk, segments, kv_heads)) return 1;
   const int group = heads / kv_heads;
   const bool wide = wide_tiles(tq, group, kv_heads, segments);
   const int64_t tiles = fmd_cdiv(fmd_cdiv(tq * group, segments), wide ? 128 : 32) * segments * kv_heads;
@@ -579,7 +599,7 @@ int split_count(int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
 }
 
 template <typename T, int DP>
-int run_fwd(const AttnArgs& a, int splits, T* out, float* lse, float* work, hipStream_t stream) {
+int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
   constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4;
   const int64_t n = a.tq * a.heads;
@@ -587,17 +607,17 @@ int run_fwd(const AttnArgs& a, int splits, T* out, float* lse, float* work, hipS
   if (wide_tiles(a.tq, a.group, a.kv_heads, a.segments)) {
     const int64_t tiles = tile_count(a.tq, a.group, a.segments, 128);
     FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    attn_fwd_kernel<T, DP, 64, 4, 1><<<dim3((unsigned)(tiles * a.kv_heads), splits), 256, 0, stream>>>(a, tiles, splits, out, lse,
+    attn_fwd_kernel<T, DP, 64, 4, 1><<<dim3((unsigned)(tiles * a.kv_heads), splits), 256, 0, stream>>>(a, tiles, splits, out, saved,
                                                                                                      po, pm, pl);
   } else {
     const int64_t tiles = tile_count(a.tq, a.group, a.segments, 32);
     FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
     attn_fwd_kernel<T, DP, 32, 1, kKeyWaves><<<dim3((unsigned)(tiles * a.kv_heads), splits), 64 * kKeyWaves, 0, stream>>>(
-        a, tiles, splits, out, lse, po, pm, pl);
+        a, tiles, splits, out, saved, po, pm, pl);
   }
   FMD_CHECK_LAUNCH();
   if (splits > 1) {
-    attn_join_kernel<T><<<(unsigned)fmd_cdiv(n, 4), 256, 0, stream>>>(a, splits, po, pm, pl, out, lse);
+    attn_join_kernel<T><<<(unsigned)fmd_cdiv(n, 4), 256, 0, stream>>>(a, splits, po, pm, pl, out, saved);
     FMD_CHECK_LAUNCH();
   }
   return FMD_OK;
@@ -652,34 +672,36 @@ int check(const AttnArgs& a, int size) {
 }
 
 template <typename T>
-int forward(const AttnArgs& a, int splits, T* out, float* lse, float* work, hipStream_t stream) {
+int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
   FMD_REQUIRE(splits >= 1 && splits <= 1024 && (splits == 1 || work));
   if (a.tq == 0) return FMD_OK;
-  FMD_REQUIRE(out && aligned16(out));
-  if (a.dim <= 32) return run_fwd<T, 32>(a, splits, out, lse, work, stream);
-  if (a.dim <= 64) return run_fwd<T, 64>(a, splits, out, lse, work, stream);
-  if (a.dim <= 96) return run_fwd<T, 96>(a, splits, out, lse, work, stream);
-  return run_fwd<T, 128>(a, splits, out, lse, work, stream);
+  FMD_REQUIRE(out && aligned16(out) && aligned16(saved.residual) && (saved.base == nullptr) == (saved.inverse == nullptr));
+  if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_fwd<T>(a, out, saved, stream);
+  if (a.dim <= 32) return run_fwd<T, 32>(a, splits, out, saved, work, stream);
+  if (a.dim <= 64) return run_fwd<T, 64>(a, splits, out, saved, work, stream);
+  if (a.dim <= 96) return run_fwd<T, 96>(a, splits, out, saved, work, stream);
+  return run_fwd<T, 128>(a, splits, out, saved, work, stream);
 }
 
 template <typename T>
-int backward(const AttnArgs& a, AttnBwd b, const T* out, T* gq, T* gk, T* gv, float* delta, hipStream_t stream) {
+int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* delta, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
   const int64_t unit = 16 / sizeof(T);
-  FMD_REQUIRE(a.tq == 0 || (b.g && out && b.lse && delta && aligned16(b.g) && aligned16(out)));
+  FMD_REQUIRE(a.tq == 0 || (b.g && b.out && b.saved.base && b.saved.inverse && delta && (sizeof(T) == 4 || b.saved.residual)));
+  FMD_REQUIRE(aligned16(b.g) && aligned16(b.out) && aligned16(b.saved.residual));
   FMD_REQUIRE(b.g_row % unit == 0 && b.g_head % unit == 0);
   FMD_REQUIRE((gk == nullptr) == (gv == nullptr) && aligned16(gq) && aligned16(gk) && aligned16(gv));
   b.delta = delta;
-  if (a.tq > 0) {
-    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(
-        static_cast<const T*>(b.g), b.g_row, b.g_head, out, a.tq, a.heads, a.dim, delta);
-    FMD_CHECK_LAUNCH();
-  }
   if (a.tq == 0) gq = nullptr;
   if (a.tk == 0) gk = gv = nullptr;
+  if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_bwd<T>(a, b, gq, gk, gv, stream);
+  if (a.tq > 0) {
+    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(b, a.tq, a.heads, a.dim, delta);
+    FMD_CHECK_LAUNCH();
+  }
   if (a.dim <= 32) return run_bwd<T, 32>(a, b, gq, gk, gv, stream);
   if (a.dim <= 64) return run_bwd<T, 64>(a, b, gq, gk, gv, stream);
   if (a.dim <= 96) return run_bwd<T, 96>(a, b, gq, gk, gv, stream);
@@ -718,21 +740,22 @@ int64_t fmd_segment_attention_work_size(int32_t splits, int64_t tq, int32_t head
   return splits > 1 && tq > 0 && heads > 0 && dim > 0 ? (int64_t)splits * tq * heads * (dim + 2) : 0;
 }
 
-int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* out, float* lse, float* work,
-                          hipStream_t stream) {
+int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* out, float* base, float* inverse,
+                          void* residual, float* work, hipStream_t stream) {
   const AttnArgs a = FMD_ATTN_ARGS;
-  return bf16 ? forward(a, splits, static_cast<__bf16*>(out), lse, work, stream)
-              : forward(a, splits, static_cast<float*>(out), lse, work, stream);
+  const AttnSaved saved = {base, inverse, bf16 ? residual : nullptr};
+  return bf16 ? forward(a, splits, static_cast<__bf16*>(out), saved, work, stream)
+              : forward(a, splits, static_cast<float*>(out), saved, work, stream);
 }
 
 int fmd_segment_attention_bwd(int32_t bf16, FMD_ATTN_PARAMS, const void* gout, int64_t g_row, int64_t g_head, const void* out,
-                              const float* lse, float* delta, void* gq, void* gk, void* gv, hipStream_t stream) {
+                              const float* base, const float* inverse, const void* residual, float* delta, void* gq,
+                              void* gk, void* gv, hipStream_t stream) {
   const AttnArgs a = FMD_ATTN_ARGS;
-  const AttnBwd b = {gout, g_row, g_head, lse, delta};
-  return bf16 ? backward(a, b, static_cast<const __bf16*>(out), static_cast<__bf16*>(gq), static_cast<__bf16*>(gk),
-                         static_cast<__bf16*>(gv), delta, stream)
-              : backward(a, b, static_cast<const float*>(out), static_cast<float*>(gq), static_cast<float*>(gk),
-                         static_cast<float*>(gv), delta, stream);
+  const AttnSaved saved = {const_cast<float*>(base), const_cast<float*>(inverse), const_cast<void*>(residual)};
+  const AttnBwd b = {gout, g_row, g_head, out, saved, nullptr};
+  return bf16 ? backward(a, b, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), delta, stream)
+              : backward(a, b, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), delta, stream);
 }
 
 }  // extern "C"

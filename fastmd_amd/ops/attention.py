@@ -20,6 +20,9 @@ the same bits.
 """
 from __future__ import annotations
 
+import math
+from typing import NamedTuple
+
 import torch
 from torch import Tensor
 from torch.autograd import Function
@@ -28,6 +31,21 @@ from fastmd_amd import _abi
 from fastmd_amd._device import require_cuda, stream
 
 MAX_DIM = 128
+
+
+class AttentionSaved(NamedTuple):
+    """What the VJP needs of the forward besides its output: a probability is ``exp2(score log2(e) - base) * inverse``
+    (both float32 [heads, rows], 0 for a row that sees no key); ``residual`` (bfloat16 only, the output's shape) is what the
+    rounding of the output dropped."""
+
+    base: Tensor
+    inverse: Tensor
+    residual: Tensor | None
+
+    @property
+    def lse(self) -> Tensor:
+        """Logarithm of each row's sum of exponentials [heads, rows], -inf for a row that sees no key."""
+        return self.base * math.log(2.0) - torch.log(self.inverse.masked_fill(self.inverse == 0, float("inf")))
 
 
 def heads_view(x: Tensor) -> tuple[Tensor, int, int]:
@@ -93,55 +111,63 @@ def _common(q, k, v, q_offsets, k_offsets, causal, scale):
     return args, (q, k, v, q_offsets, k_offsets)
 
 
-def _forward(q, k, v, q_offsets, k_offsets, causal, scale, with_lse):
+def _forward(q, k, v, q_offsets, k_offsets, causal, scale, save):
     args, keep = _common(q, k, v, q_offsets, k_offsets, causal, scale)
     tq, heads, dim = q.shape
     out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((heads, tq), dtype=torch.float32, device=q.device) if with_lse else None
+    saved, base, inverse, residual = None, None, None, None
+    if save:
+        rows = torch.empty((2, heads, tq), dtype=torch.float32, device=q.device)
+        saved = AttentionSaved(rows[0], rows[1], torch.empty_like(out) if q.dtype == torch.bfloat16 else None)
+        base, inverse, residual = (_abi.ptr(x) for x in saved)
     lib = _abi.load()
     splits = lib.fmd_segment_attention_splits(tq, k.shape[0], args[14], heads, k.shape[1])
     work = None
     if splits > 1:
         work = torch.empty(lib.fmd_segment_attention_work_size(splits, tq, heads, dim), dtype=torch.float32,
                            device=q.device)
-    _abi.call("fmd_segment_attention", *args, splits, out.data_ptr(), _abi.ptr(lse), _abi.ptr(work), stream())
+    _abi.call("fmd_segment_attention", *args, splits, out.data_ptr(), base, inverse, residual, _abi.ptr(work), stream())
     del keep
-    return out, lse
+    return out, saved
 
 
 def segment_attention_forward(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor | None = None, *,
-                              causal: bool = False, scale: float | None = None) -> tuple[Tensor, Tensor]:
-    """``(out, lse)`` without autograd: the output and the logarithm of each row's sum of exponentials (float32
-    [heads, rows], -inf for a row that sees no key), which ``segment_attention_vjp`` takes."""
+                              causal: bool = False, scale: float | None = None) -> tuple[Tensor, AttentionSaved]:
+    """``(out, saved)`` without autograd: the output and what ``segment_attention_vjp`` takes besides it."""
     k_offsets = q_offsets if k_offsets is None else k_offsets
     scale = _check(q, k, v, q_offsets, k_offsets, scale)
     return _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
 
 
-def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, q_offsets: Tensor,
-                          k_offsets: Tensor | None = None, *, causal: bool = False, scale: float | None = None,
-                          need_q: bool = True, need_kv: bool = True):
+def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, saved: AttentionSaved,
+                          q_offsets: Tensor, k_offsets: Tensor | None = None, *, causal: bool = False,
+                          scale: float | None = None, need_q: bool = True, need_kv: bool = True):
     """``(gq, gk, gv)`` from the gradient of the output and the results of ``segment_attention_forward`` (None where
     not needed; the gradients of k and v come together)."""
     k_offsets = q_offsets if k_offsets is None else k_offsets
     scale = _check(q, k, v, q_offsets, k_offsets, scale)
-    require_cuda(q, gout, out, lse)
+    base, inverse, residual = saved
+    require_cuda(q, gout, out, base, inverse, residual)
     if gout.shape != q.shape or gout.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
         raise ValueError(f"gout and out must be {q.dtype} {tuple(q.shape)}, got {gout.dtype} {tuple(gout.shape)} and "
                          f"{out.dtype} {tuple(out.shape)}")
-    if lse.shape != (q.shape[1], q.shape[0]) or lse.dtype != torch.float32:
-        raise ValueError(f"lse must be float32 {(q.shape[1], q.shape[0])}, got {lse.dtype} {tuple(lse.shape)}")
+    rows = (q.shape[1], q.shape[0])
+    for x in (base, inverse):
+        if x.shape != rows or x.dtype != torch.float32 or not x.is_contiguous():
+            raise ValueError(f"saved must be the forward's: float32 {rows} rows, got {x.dtype} {tuple(x.shape)}")
+    if q.dtype == torch.bfloat16 and (residual is None or residual.shape != q.shape or residual.dtype != q.dtype
+                                      or not residual.is_contiguous() or residual.data_ptr() % 16):
+        raise ValueError("saved must be the forward's: the residual of a bfloat16 output")
     args, keep = _common(q, k, v, q_offsets, k_offsets, causal, scale)
     gout, g_row, g_head = heads_view(gout)
-    out, lse = out.contiguous(), lse.contiguous()
-    if out.data_ptr() % 16:
-        out = out.clone()
+    if not out.is_contiguous() or out.data_ptr() % 16:
+        out = out.clone(memory_format=torch.contiguous_format)
     gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
     gk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None
     gv = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None
-    delta = torch.empty_like(lse)
-    _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), lse.data_ptr(),
-              delta.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
+    delta = torch.empty_like(base)
+    _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), base.data_ptr(),
+              inverse.data_ptr(), _abi.ptr(residual), delta.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
     del keep
     return gq, gk, gv
 
@@ -149,16 +175,16 @@ def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Te
 class _SegmentAttention(Function):
     @staticmethod
     def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale):
-        out, lse = _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
-        ctx.save_for_backward(q, k, v, out, lse, q_offsets, k_offsets)
+        out, saved = _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, q_offsets, k_offsets, *saved)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     def backward(ctx, gout):
-        q, k, v, out, lse, q_offsets, k_offsets = ctx.saved_tensors
-        grads = segment_attention_vjp(gout, q, k, v, out, lse, q_offsets, k_offsets, causal=ctx.causal,
-                                      scale=ctx.scale, need_q=ctx.needs_input_grad[0],
+        q, k, v, out, q_offsets, k_offsets, *saved = ctx.saved_tensors
+        grads = segment_attention_vjp(gout, q, k, v, out, AttentionSaved(*saved), q_offsets, k_offsets,
+                                      causal=ctx.causal, scale=ctx.scale, need_q=ctx.needs_input_grad[0],
                                       need_kv=ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
         return (*grads, None, None, None, None)
 

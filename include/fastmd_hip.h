@@ -823,8 +823,10 @@ int fmd_edge_stress_f32(const float* geo, const float* gvec, const int64_t* n_ed
  * [k_offsets[s], k_offsets[s + 1]) (device int64, ascending; every offset is clamped into the buffer). causal: query i of
  * n sees the first i + m - n + 1 of the m keys. A query that sees no key, and one outside every segment, gives zero.
  * q [tq, heads, dim], k and v [tk, kv_heads, dim] with row and head strides in elements (unit stride in dim, 16-byte
- * aligned rows); dim a multiple of 8 up to 128 (FMD_EUNSUPPORTED otherwise); scale > 0. out [tq, heads, dim] contiguous;
- * lse [heads, tq] (nullable): log of the sum of exponentials, -inf for a row that sees nothing.
+ * aligned rows); dim a multiple of 8 up to 128 (FMD_EUNSUPPORTED otherwise); scale > 0. out [tq, heads, dim] contiguous.
+ * For the VJP (all nullable): base and inverse [heads, tq], such that a probability is
+ * exp2(score log2(e) - base) inverse (both 0 for a row that sees nothing), and for bf16 residual [tq, heads, dim], what the
+ * rounding of out dropped.
  * splits: fmd_segment_attention_splits(); with more than one, `work` holds fmd_segment_attention_work_size() floats. */
 int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads);
 int64_t fmd_segment_attention_work_size(int32_t splits, int64_t tq, int32_t heads, int32_t dim);
@@ -832,17 +834,18 @@ int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_
                           int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
                           const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
                           int32_t kv_heads, int32_t dim, int32_t causal, float scale, int32_t splits, void* out,
-                          float* lse, float* work, hipStream_t stream);
+                          float* base, float* inverse, void* residual, float* work, hipStream_t stream);
 
 /* VJP of fmd_segment_attention: gq [tq, heads, dim], gk and gv [tk, kv_heads, dim] (contiguous; gq, or gk and gv
- * together, nullable) from the gradient `gout` of `out`, the forward's `out` and `lse`. Rows outside every segment get
+ * together, nullable) from the gradient `gout` of `out`, the forward's `out`, `base`,
+ * `inverse` and (bf16) `residual`. Rows outside every segment get
  * zero. delta: scratch of heads * tq floats. No atomics: the same inputs give the same bits. */
 int fmd_segment_attention_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                               int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
                               const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
                               int32_t kv_heads, int32_t dim, int32_t causal, float scale, const void* gout, int64_t g_row,
-                              int64_t g_head, const void* out, const float* lse, float* delta, void* gq, void* gk, void* gv,
-                              hipStream_t stream);
+                              int64_t g_head, const void* out, const float* base, const float* inverse, const void* residual,
+                              float* delta, void* gq, void* gk, void* gv, hipStream_t stream);
 
 /* Each head x of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (row and head strides in elements, 16-byte aligned
  * rows, dim a multiple of 8 up to 256): with norm, x (mean x^2 + eps)^(-1/2) weight (weights [dim] of the features' type,

@@ -60,7 +60,8 @@ def check(q, k, v, g, q_off, k_off, *, causal, scale=None, device="cuda"):
     r = oracle.segment_attention(q, k, v, q_off, k_off, causal=causal, scale=scale, gout=g)
     b = bounds(r, q.dtype)
     d = [x.to(device) for x in (q, k, v, g, q_off, k_off)]
-    out, lse = segment_attention_forward(*d[:3], *d[4:], causal=causal, scale=scale)
+    out, saved = segment_attention_forward(*d[:3], *d[4:], causal=causal, scale=scale)
+    lse = saved.lse
     compare(out, r["out"], b["out"], "out")
     seen = torch.isfinite(r["lse"])
     assert torch.equal(lse.cpu()[~seen], torch.full_like(lse.cpu()[~seen], -math.inf))
@@ -69,7 +70,7 @@ def check(q, k, v, g, q_off, k_off, *, causal, scale=None, device="cuda"):
         far = (lse.cpu().double() - r["lse"])[seen].abs()
         tol = 2.0 * (16.0 * 2.0 ** -24 * r["scores"] + 2.0 ** -20) + 2.0 ** -22 * r["lse"][seen].abs()
         assert bool((far <= tol).all())
-    grads = segment_attention_vjp(d[3], *d[:3], out, lse, *d[4:], causal=causal, scale=scale)
+    grads = segment_attention_vjp(d[3], *d[:3], out, saved, *d[4:], causal=causal, scale=scale)
     for name, x in zip(("gq", "gk", "gv"), grads):
         compare(x, r[name], b[name], name)
     return out, lse, grads
@@ -152,6 +153,20 @@ def test_neighbour_rows(heads, kv_heads, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(1, 1, 8), (8, 2, 16), (3, 1, 40), (10, 5, 128), (4, 2, 96), (9, 9, 64)])
+def test_few_rows_of_any_group_and_width(heads, kv_heads, dim, dtype, causal):
+    """Mostly single queries, some segments with none and some with several."""
+    g = torch.Generator().manual_seed(dim)
+    lk = torch.randint(0, 30, (300,), generator=g).tolist()
+    lq = [1] * 300
+    lq[5], lq[6], lq[7], lq[200], lq[201], lq[299] = 0, 4, 0, 3, 0, 0
+    q, k, v, go, q_off, k_off = make(lq, lk, heads, kv_heads, dim, dtype, seed=dim)
+    check(q, k, v, go, q_off, k_off, causal=causal)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lq,lk", [([60, 90], [60, 90]), ([1, 1], [200, 30]), ([1100, 1500], [1100, 1500])])
 def test_rows_outside_the_segments(lq, lk, dtype):
@@ -179,8 +194,8 @@ def test_values_of_other_segments_do_not_matter(dtype):
     def run(q, k, v, g):
         a = [x.cuda() for x in (q, k, v)]
         off = q_off.cuda()
-        out, lse = segment_attention_forward(*a, off)
-        return (out, *segment_attention_vjp(g.cuda(), *a, out, lse, off))
+        out, saved = segment_attention_forward(*a, off)
+        return (out, *segment_attention_vjp(g.cuda(), *a, out, saved, off))
 
     want = run(q, k, v, g)
     for x, bad in ((q, float("nan")), (k, float("inf")), (v, float("nan")), (g, float("-inf"))):
@@ -202,8 +217,8 @@ def test_strided_inputs(dtype):
     q, k, v, g = (x.cuda() for x in (q, k, v, g))
 
     def run(q, k, v, g):
-        out, lse = segment_attention_forward(q, k, v, off, causal=True)
-        return (out, lse, *segment_attention_vjp(g, q, k, v, out, lse, off, causal=True))
+        out, saved = segment_attention_forward(q, k, v, off, causal=True)
+        return (out, saved.lse, *segment_attention_vjp(g, q, k, v, out, saved, off, causal=True))
 
     want = run(q, k, v, g)
     packed = torch.cat((q, k, v), 1)
@@ -228,8 +243,8 @@ def test_runs_are_bitwise_repeatable(lq, lk, heads, dtype):
     q, k, v, g, q_off, k_off = (x.cuda() for x in make(lq, lk, heads, heads, 32, dtype))
 
     def run():
-        out, lse = segment_attention_forward(q, k, v, q_off, k_off)
-        return (out, lse, *segment_attention_vjp(g, q, k, v, out, lse, q_off, k_off))
+        out, saved = segment_attention_forward(q, k, v, q_off, k_off)
+        return (out, saved.lse, *segment_attention_vjp(g, q, k, v, out, saved, q_off, k_off))
 
     for a, b in zip(run(), run()):
         assert torch.equal(a, b)
@@ -286,8 +301,8 @@ def test_nothing_to_do():
     for tq, tk, off in ((0, 0, [0]), (0, 5, [0, 0]), (5, 0, [0, 0]), (4, 4, [0])):
         q, k = torch.ones(tq, 2, 16, device="cuda"), torch.ones(tk, 2, 16, device="cuda")
         o = torch.tensor(off, device="cuda")
-        out, lse = segment_attention_forward(q, k, k, o)
-        grads = segment_attention_vjp(q, q, k, k, out, lse, o)
+        out, saved = segment_attention_forward(q, k, k, o)
+        grads = segment_attention_vjp(q, q, k, k, out, saved, o)
         for x in (out, *grads):
             assert not x.any()
 
@@ -320,8 +335,9 @@ def test_other_stream(dtype):
 
 @pytest.mark.gpu
 def test_refusals():
-    from fastmd_amd.ops.attention import segment_attention, segment_attention_vjp
+    from fastmd_amd.ops.attention import AttentionSaved, segment_attention, segment_attention_vjp
 
+    row = torch.zeros(4, 6, device="cuda")
     q = torch.zeros(6, 4, 16, device="cuda")
     k = torch.zeros(6, 2, 16, device="cuda")
     off = torch.tensor([0, 6], device="cuda")
@@ -339,8 +355,10 @@ def test_refusals():
         (lambda: segment_attention(q, k, k, off, scale=0.0), "scale"),
         (lambda: segment_attention(q, k, k, off, scale=float("nan")), "scale"),
         (lambda: segment_attention(q, k, k, off.cpu()), "GPU"),
-        (lambda: segment_attention_vjp(q[:5], q, k, k, q, torch.zeros(4, 6, device="cuda"), off), "gout"),
-        (lambda: segment_attention_vjp(q, q, k, k, q, torch.zeros(6, 4, device="cuda"), off), "lse"),
+        (lambda: segment_attention_vjp(q[:5], q, k, k, q, AttentionSaved(row, row, None), off), "gout"),
+        (lambda: segment_attention_vjp(q, q, k, k, q, AttentionSaved(row, row.T, None), off), "saved"),
+        (lambda: segment_attention_vjp(*[x.bfloat16() for x in (q, q, k, k, q)], AttentionSaved(row, row, None), off),
+         "residual"),
     ]
     for call, match in bad:
         with pytest.raises(ValueError, match=match):
@@ -361,7 +379,7 @@ def test_entry_points_refuse_what_no_launch_can_honour():
     lib = _abi.load()
     call = lambda **kw: lib.fmd_segment_attention(  # noqa: E731
         0, 16, 32, 32, 16, 32, 32, 16, 32, 32, 16, 16, kw.get("tq", 4), 4, 1, kw.get("heads", 2), kw.get("kv", 2),
-        kw.get("dim", 16), 0, kw.get("scale", 1.0), kw.get("splits", 1), 16, None, None, None)
+        kw.get("dim", 16), 0, kw.get("scale", 1.0), kw.get("splits", 1), 16, None, None, None, None, None)
     assert call(heads=3) == 10001 and call(tq=-1) == 10001 and call(scale=0.0) == 10001 and call(splits=2) == 10001
     assert call(dim=136) == 10002 and call(dim=12) == 10002
 
