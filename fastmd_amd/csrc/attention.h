@@ -27,7 +27,7 @@ struct AttnArgs {
 // output before rounding is out + residual (bf16: delta = g . o cancels against g . v where few keys count, and the rounding
 // of the output alone took the error of gq and gk from 1.4 to 1.7 times that of rounding them).
 struct AttnSaved {
-  float *base, *inverse;  // [heads, tq]: largest scaled score in log2 units, 1 / row sum (both 0 for a row that sees nothing)
+  float *base, *inverse;  // [heads, tq]: near the largest scaled score, in log2 units, 1 / row sum (both 0 for a row that sees nothing)
   void* residual;         // bf16 only: [tq, heads, dim]
 };
 
@@ -39,6 +39,7 @@ struct AttnBwd {
   const float* delta;  // [heads, tq]
 };
 
+constexpr int kWaitVm0 = 0 | (7 << 4) | (15 << 8);  // s_waitcnt vmcnt(0)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // A segment with its rows. The kernels see segments + 2 of them: the rows before the first offset and after the
@@ -243,6 +244,38 @@ struct AttnLoad {
     for (int n = 0; n < NV; ++n) {
       const int i = t + n * THREADS;
       if (N % THREADS == 0 || i < N) Tile::put(s, i / Tile::CHUNKS, i % Tile::CHUNKS, raw_planes(r[n]));
+    }
+  }
+};
+
+__device__ __attribute__((aligned(16))) const uint32_t g_attn_zero_chunk[4] = {0, 0, 0, 0};
+
+// bf16 rows of a tile straight into LDS (no register stage): thread t of THREADS fills the 16-byte slots t, t + THREADS, ...
+// of the tile, each with the chunk that the permutation puts there. Per lane one 32-bit offset into the tile's rows; the
+// chunks past the rows or past dim come from a zero chunk.
+template <int ROWS, int DP, int THREADS>
+struct AttnDma {
+  using Tile = AttnTile<1, ROWS, DP>;
+  static constexpr int CH = Tile::LD / 8, N = ROWS * CH / THREADS, STEP = THREADS / CH;
+  static_assert(ROWS * CH % THREADS == 0 && THREADS % CH == 0, "whole passes");
+
+  // rows [0, n) of the tile at `base` (row stride `ld`), by thread t; `wave_slot`: the wave's first slot
+  __device__ static __forceinline__ void issue(const __bf16* base, int64_t ld, int n, int dim, int t, __bf16* lds) {
+    const int wave_slot = __builtin_amdgcn_readfirstlane(t & ~63);
+    const bool plain = n >= ROWS && dim == DP && DP == Tile::LD;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int row0 = t / CH, pos = t % CH;  // of pass 0
+      const int row = row0 + i * STEP;
+      const int chunk = (Tile::at(row, pos) - row * Tile::LD) >> 3;  // the permutation is its own inverse
+      const __bf16* p = base + i * STEP * ld + (uint32_t)(row0 * (int)ld + 8 * chunk);
+      if (!plain) {
+        p = row < n && 8 * chunk < dim ? p : reinterpret_cast<const __bf16*>(g_attn_zero_chunk);
+        asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
+      }
+      typedef const __attribute__((address_space(1))) void* global_ptr;
+      typedef __attribute__((address_space(3))) void* lds_ptr;
+      __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)(lds + (wave_slot + i * THREADS) * 8), 16, 0, 0);
     }
   }
 };

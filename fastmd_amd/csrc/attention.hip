@@ -3,6 +3,10 @@
 
 namespace {
 
+// Waves per SIMD that a kernel is compiled for. Two leave 256 registers, which the compiler then uses as one file; with
+// one it puts the sums into accumulation registers and moves them out and back at every rescaling.
+static constexpr int attn_waves(int planes, int dp, int sums) { return planes * dp * sums <= 192 ? 2 : 1; }
+
 // ------------------------------------------------------------------------------------ forward
 
 // One workgroup: 32 WM packed query rows of one key head, WM KW waves. Wave (wm, kw) holds 32 rows and walks the key
@@ -12,13 +16,17 @@ namespace {
 // O^T = V^T P^T. Statistics and sums are fp32; P is rounded to bf16 for bf16 inputs (the output is, too) and kept as
 // three planes for fp32.
 template <typename T, int DP, int BN, int WM, int KW>
-__global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int64_t tiles, int splits, T* out, AttnSaved saved,
+__global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_fwd_kernel(AttnArgs a, int64_t tiles, int splits, T* out, AttnSaved saved,
                                                                 float* part_o, float* part_m, float* part_l) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, JB = BN / 32;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kMerge = (KW - 1) * WM * (DB * 16 + 2) * 64 * 2;  // in bf16 units
   constexpr int kTiles = 2 * KW * Tile::SIZE;
+  // bf16 tiles are copied straight into LDS, a tile ahead, into two buffers; fp32 tiles go through registers, where they are
+  // split, into one
+  constexpr bool kDma = NP == 1;
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
+  __shared__ __attribute__((aligned(16))) __bf16 lds2[kDma ? kTiles : 8];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -63,29 +71,17 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int6
   float m = -INFINITY, l = 0.f;
   const float c = a.scale * kLog2e;
 
-  __bf16* ks_ = lds + kw * 2 * Tile::SIZE;
-  __bf16* vs_ = ks_ + Tile::SIZE;
   const int lt = threadIdx.x - kw * WM * 64;  // thread among those that load this group's tiles
   const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
   const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
-  AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
-  auto issue = [&](int tile) {
-    const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
-    kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
-    vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
-  };
+  // The maximum follows the scores only where one outgrows it by kSlack (in log2 units): exponentials up to 2^kSlack are
+  // as exact as those below one, and the sums are rescaled a few times per row instead of once per tile.
+  constexpr float kSlack = 8.f;
+  const float slack = kSlack / c;
 
-  const int rounds = (tile_hi - tile_lo + KW - 1) / KW;  // the same for every wave
-  if (rounds > 0) issue(tile_lo + kw);
-  for (int it = 0; it < rounds; ++it) {
-    const int tile = tile_lo + it * KW + kw, j0 = tile * BN;
-    __syncthreads();  // the tiles before are read
-    kl.store(ks_, lt);
-    vl.store(vs_, lt);
-    __syncthreads();
-    if (it + 1 < rounds) issue(tile + KW);
-    if (tile >= tile_hi) continue;
-
+  auto step = [&](const __bf16* ks_, int tile) {
+    const __bf16* vs_ = ks_ + Tile::SIZE;
+    const int j0 = tile * BN;
     fmd_f32x16 s[JB];
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
@@ -100,29 +96,33 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int6
         for (int v = 0; v < 16; ++v)
           if (j0 + 32 * j + prod_row(v, half) >= sees) s[j][v] = -INFINITY;
     }
-    float top = m;
+    float top = s[0][0];
 #pragma unroll
     for (int j = 0; j < JB; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) top = fmaxf(top, s[j][v]);
     top = max_halves(top);
-    const float base = top == -INFINITY ? 0.f : top * c;  // a row that has seen nothing yet: all exponents -inf
-    const float fade = exp2_hw(fmaf(m, c, -base));
-    float sum = 0.f;
+    if (__any(top > m + slack)) {
+      top = fmaxf(top, m);
+      const float fade = exp2_hw(fmaf(m, c, top == -INFINITY ? 0.f : -top * c));
+      l *= fade;
+      m = top;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= fade;
+    }
+    const float base = m == -INFINITY ? 0.f : m * c;  // a row that has seen nothing yet: all exponents -inf
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < JB; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
         const float p = exp2_hw(fmaf(s[j][v], c, -base));
         s[j][v] = p;
-        sum += p;
+        sum[v & 1] += p;
       }
-    l = l * fade + sum;  // of this lane's half of the keys
-    m = top;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) o[d][v] *= fade;
+    l += sum[0] + sum[1];  // of this lane's half of the keys
 #pragma unroll
     for (int j = 0; j < JB; ++j)
 #pragma unroll
@@ -135,6 +135,48 @@ __global__ void __launch_bounds__(64 * WM * KW) attn_fwd_kernel(AttnArgs a, int6
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(vs_, 32 * j + 16 * step, d), pf, o[d]);
       }
+  };
+
+  const int rounds = (tile_hi - tile_lo + KW - 1) / KW;  // the same for every wave
+  if constexpr (kDma) {
+    using Dma = AttnDma<BN, DP, 64 * WM>;
+    auto issue = [&](int tile, __bf16* to) {
+      const int n = tile < tile_hi ? sg.nk - tile * BN : 0;
+      const int64_t j0 = n > 0 ? tile * BN : 0;
+      Dma::issue(kb + j0 * a.k_row, a.k_row, n, a.dim, lt, to);
+      Dma::issue(vb + j0 * a.v_row, a.v_row, n, a.dim, lt, to + Tile::SIZE);
+    };
+    __bf16 *st0 = lds + kw * 2 * Tile::SIZE, *st1 = lds2 + kw * 2 * Tile::SIZE;
+    auto round = [&](int it, const __bf16* here, __bf16* next) {
+      const int tile = tile_lo + it * KW + kw;
+      __builtin_amdgcn_s_waitcnt(kWaitVm0);  // this wave's part of the tile has landed
+      __syncthreads();                       // everyone's has, and the other buffer is read
+      if (it + 1 < rounds) issue(tile + KW, next);
+      if (tile < tile_hi) step(here, tile);
+    };
+    if (rounds > 0) issue(tile_lo + kw, st0);
+    for (int it = 0; it < rounds; it += 2) {
+      round(it, st0, st1);
+      if (it + 1 < rounds) round(it + 1, st1, st0);
+    }
+  } else {
+    __bf16* st = lds + kw * 2 * Tile::SIZE;
+    AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
+    auto issue = [&](int tile) {
+      const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
+      kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
+      vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
+    };
+    if (rounds > 0) issue(tile_lo + kw);
+    for (int it = 0; it < rounds; ++it) {
+      const int tile = tile_lo + it * KW + kw;
+      __syncthreads();  // the tiles before are read
+      kl.store(st, lt);
+      vl.store(st + Tile::SIZE, lt);
+      __syncthreads();
+      if (it + 1 < rounds) issue(tile + KW);
+      if (tile < tile_hi) step(st, tile);
+    }
   }
   l = add_halves(l);
 
@@ -265,7 +307,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // tiles rw, rw + RW, ... of 32 packed query rows. S = Q K^T (lane: a key, registers: query rows), so exp(S - lse) and
 // dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of the group.
 template <typename T, int DP, int WM, int RW>
-__global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
+__global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
   using Tile = AttnTile<NP, BR, DP>;
   constexpr int kGroup = 2 * Tile::SIZE + 6 * BR;  // Q, G, base, delta and inverse of BR rows (bf16 units)
@@ -442,7 +484,7 @@ __global__ void __launch_bounds__(64 * WM * RW) attn_bwd_kv_kernel(AttnArgs a, A
 
 // Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T.
 template <typename T, int DP, int WM, int KW>
-__global__ void __launch_bounds__(64 * WM * KW) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gq) {
+__global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gq) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = 32;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * DB * 16 * 64 * 2;
@@ -667,6 +709,7 @@ int check(const AttnArgs& a, int size) {
   FMD_REQUIRE(aligned16(a.q) && aligned16(a.k) && aligned16(a.v));
   FMD_REQUIRE(a.q_row % unit == 0 && a.q_head % unit == 0 && a.k_row % unit == 0 && a.k_head % unit == 0 &&
               a.v_row % unit == 0 && a.v_head % unit == 0);
+  FMD_REQUIRE(a.q_row < (1 << 24) && a.k_row < (1 << 24) && a.v_row < (1 << 24));
   FMD_REQUIRE(a.scale > 0.f);
   return FMD_OK;
 }

@@ -31,6 +31,7 @@ from fastmd_amd import _abi
 from fastmd_amd._device import require_cuda, stream
 
 MAX_DIM = 128
+MAX_ROW_STRIDE = 2 ** 24  # elements; the kernels hold a lane's offset in a tile of rows in 32 bits
 
 
 class AttentionSaved(NamedTuple):
@@ -49,7 +50,7 @@ class AttentionSaved(NamedTuple):
 
 
 def heads_view(x: Tensor) -> tuple[Tensor, int, int]:
-    """(tensor, row stride, head stride) of ``x`` [rows, heads, dim] with unit stride in dim and 16-byte aligned rows;
+    """(tensor, row stride, head stride) of ``x`` [rows, heads, dim] with unit stride in dim and 16-byte aligned rows below MAX_ROW_STRIDE;
     copies only when needed (any strides otherwise: columns of a packed projection are read in place)."""
     rows, heads, dim = x.shape
     unit = 16 // x.element_size()
@@ -58,7 +59,7 @@ def heads_view(x: Tensor) -> tuple[Tensor, int, int]:
         sr = heads * dim
     if heads <= 1:
         sh = dim
-    if (sd != 1 and dim > 1) or sr % unit or sh % unit or x.data_ptr() % 16:
+    if (sd != 1 and dim > 1) or sr % unit or sh % unit or x.data_ptr() % 16 or sr >= MAX_ROW_STRIDE:
         x = x.clone(memory_format=torch.contiguous_format)
         sr, sh = heads * dim, dim
     return x, sr, sh
