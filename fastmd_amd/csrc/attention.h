@@ -21,7 +21,12 @@ struct AttnArgs {
   int64_t tq, tk;
   int32_t segments, heads, kv_heads, group, dim, causal;
   float scale;
+  uint32_t group_mul, group_shift;          // row / group = row * group_mul >> group_shift for rows below 2^31
 };
+
+__device__ __forceinline__ int attn_token(const AttnArgs& a, int row) {
+  return (int)((uint64_t)(uint32_t)row * a.group_mul >> a.group_shift);
+}
 
 // What the VJP needs of the forward besides its output. A row's probabilities are exp2(s scale log2(e) - base) inverse; its
 // output before rounding is out + residual (bf16: delta = g . o cancels against g . v where few keys count, and the rounding
@@ -175,15 +180,16 @@ __device__ __forceinline__ fmd_f32x16 zero16() {
 // ------------------------------------------------------------------------------------ tiles in LDS
 
 // A tile of ROWS rows of DP values (NP planes), row-major, its 16-byte chunks permuted within a row so that both
-// reads are free of bank conflicts: the same chunk of eight consecutive rows (operands along a row) and two chunks of
-// four consecutive rows (ds_read_b64_tr_b16, operands along a column).
+// reads are free of conflicts on the 64 banks: the same chunk of sixteen consecutive rows (a quarter of a 16-byte read,
+// operands along a row) and four chunks of four consecutive rows (half of a ds_read_b64_tr_b16, operands along a column).
 template <int NP, int ROWS, int DP>
 struct AttnTile {
   static constexpr int LD = DP == 96 ? 128 : DP;  // a power of two, for the permutation
   static constexpr int CHUNKS = DP / 8, PLANE = ROWS * LD, SIZE = NP * PLANE;
 
   __device__ static __forceinline__ int at(int row, int chunk) {
-    const int f = LD >= 64 ? ((row & 3) << 1) | ((row >> 2) & 1) : (((row >> 1) & 1) << 1) | ((row >> 2) & 1);
+    const int high = (row >> 2) & 3;
+    const int f = LD == 128 ? ((row & 3) << 2) | high : LD == 64 ? (((row >> 1) & 1) << 2) | high : high;
     return row * LD + ((chunk ^ f) << 3);
   }
 
@@ -192,26 +198,35 @@ struct AttnTile {
     for (int p = 0; p < NP; ++p) *reinterpret_cast<fmd_bf16x8*>(s + p * PLANE + at(row, chunk)) = v.p[p];
   }
 
-  // operand of 32 rows (lane: row base + lane % 32) over 16 columns: eight columns from 16 step + 8 (lane / 32)
-  __device__ static __forceinline__ Planes<NP> rows(const __bf16* s, int base, int step) {
+  // A lane's place in the two operand reads. Tiles start at multiples of LD, so the rest of an address is an exclusive or of
+  // bits within a row and a constant.
+  __device__ static __forceinline__ int lane_rows() {
     const int lane = threadIdx.x & 63;
+    return at(lane & 31, lane >> 5);
+  }
+  __device__ static __forceinline__ int lane_cols() {
+    const int lane = threadIdx.x & 63;
+    return at(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 4;
+  }
+
+  // operand of 32 rows (lane: row base + lane % 32) over 16 columns: eight columns from 16 step + 8 (lane / 32);
+  // base a multiple of 32
+  __device__ static __forceinline__ Planes<NP> rows(const __bf16* s, int lane_at, int base, int step) {
     Planes<NP> o;
 #pragma unroll
     for (int p = 0; p < NP; ++p)
-      o.p[p] = *reinterpret_cast<const fmd_bf16x8*>(s + p * PLANE + at(base + (lane & 31), 2 * step + (lane >> 5)));
+      o.p[p] = *reinterpret_cast<const fmd_bf16x8*>(s + p * PLANE + base * LD + (lane_at ^ (step << 4)));
     return o;
   }
 
-  // operand of 32 columns (lane: column 32 block + lane % 32) over the 16 rows from `base`, in the order in which a
-  // 32 x 32 product holds its rows: for lane half h rows 4 h .. 4 h + 3, then 8 + 4 h .. 8 + 4 h + 3
-  __device__ static __forceinline__ Planes<NP> cols(const __bf16* s, int base, int block) {
-    const int lane = threadIdx.x & 63;
-    const int row = base + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int chunk = 4 * block + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), sub = (lane & 1) * 4;
+  // operand of 32 columns (lane: column 32 block + lane % 32) over the 16 rows from `base` (a multiple of 16), in the order
+  // in which a 32 x 32 product holds its rows: for lane half h rows 4 h .. 4 h + 3, then 8 + 4 h .. 8 + 4 h + 3
+  __device__ static __forceinline__ Planes<NP> cols(const __bf16* s, int lane_at, int base, int block) {
     Planes<NP> o;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const __bf16 *x = s + p * PLANE + at(row, chunk) + sub, *y = s + p * PLANE + at(row + 8, chunk) + sub;
+      const __bf16* x = s + p * PLANE + base * LD + (lane_at ^ (block << 5));
+      const __bf16* y = s + p * PLANE + (base + 8) * LD + (lane_at ^ (block << 5) ^ 16);
       typedef __attribute__((address_space(3))) fmd_s16x4* lds_ptr;
       const fmd_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)x);
       const fmd_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)y);
@@ -262,21 +277,32 @@ struct AttnDma {
   // rows [0, n) of the tile at `base` (row stride `ld`), by thread t; `wave_slot`: the wave's first slot
   __device__ static __forceinline__ void issue(const __bf16* base, int64_t ld, int n, int dim, int t, __bf16* lds) {
     const int wave_slot = __builtin_amdgcn_readfirstlane(t & ~63);
-    const bool plain = n >= ROWS && dim == DP && DP == Tile::LD;
+    const int row0 = t / CH, pos = t % CH;  // of pass 0
+    uint32_t off = row0 * (int)ld;
+    asm volatile("" : "+v"(off));  // one register for all passes, not an address each
+    if (n >= ROWS && dim == DP && DP == Tile::LD) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        copy16(base + i * STEP * ld + (off + 8 * chunk_at(row0 + i * STEP, pos)), lds + (wave_slot + i * THREADS) * 8);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int row0 = t / CH, pos = t % CH;  // of pass 0
-      const int row = row0 + i * STEP;
-      const int chunk = (Tile::at(row, pos) - row * Tile::LD) >> 3;  // the permutation is its own inverse
-      const __bf16* p = base + i * STEP * ld + (uint32_t)(row0 * (int)ld + 8 * chunk);
-      if (!plain) {
-        p = row < n && 8 * chunk < dim ? p : reinterpret_cast<const __bf16*>(g_attn_zero_chunk);
-        asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
-      }
-      typedef const __attribute__((address_space(1))) void* global_ptr;
-      typedef __attribute__((address_space(3))) void* lds_ptr;
-      __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)(lds + (wave_slot + i * THREADS) * 8), 16, 0, 0);
+      const int row = row0 + i * STEP, chunk = chunk_at(row, pos);
+      const __bf16* p = base + i * STEP * ld + (off + 8 * chunk);
+      p = row < n && 8 * chunk < dim ? p : reinterpret_cast<const __bf16*>(g_attn_zero_chunk);
+      asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
+      copy16(p, lds + (wave_slot + i * THREADS) * 8);
     }
+  }
+
+  // the chunk that lies at place `pos` of a row (the permutation is its own inverse)
+  __device__ static __forceinline__ int chunk_at(int row, int pos) { return (Tile::at(row, pos) - row * Tile::LD) >> 3; }
+
+  __device__ static __forceinline__ void copy16(const __bf16* p, __bf16* to) {
+    typedef const __attribute__((address_space(1))) void* global_ptr;
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 16, 0, 0);
   }
 };
 

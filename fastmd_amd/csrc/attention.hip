@@ -42,15 +42,15 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   if (first >= rows) return;
   const int row0 = (int)first, row = row0 + 32 * wm + (lane & 31);
   const bool live = row < rows;
-  const int tok = (live ? row : rows - 1) / a.group, head = kvh * a.group + (live ? row : rows - 1) % a.group;
+  const int tok = attn_token(a, live ? row : rows - 1), head = kvh * a.group + (live ? row : rows - 1) - tok * a.group;
   const int64_t qt = sg.q0 + tok;
 
   // keys that this row sees, and that any row of the workgroup sees
   const int shift = sg.nk - sg.nq;
   const int sees = a.causal ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
-  const int last_tok = min(row0 + 32 * WM, rows) - 1;
-  const int reach = a.causal ? max(0, min(sg.nk, last_tok / a.group + shift + 1)) : sg.nk;
-  const int least = a.causal ? max(0, min(sg.nk, row0 / a.group + shift + 1)) : sg.nk;
+  const int last_row = min(row0 + 32 * WM, rows) - 1;
+  const int reach = a.causal ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
+  const int least = a.causal ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
   const int all_tiles = (reach + BN - 1) / BN;
   const int per = (all_tiles + splits - 1) / splits;
   const int tile_lo = min(all_tiles, (int)blockIdx.y * per), tile_hi = min(all_tiles, tile_lo + per);
@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   constexpr float kSlack = 8.f;
   const float slack = kSlack / c;
 
+  const int lr = Tile::lane_rows(), lc = Tile::lane_cols();
   auto step = [&](const __bf16* ks_, int tile) {
     const __bf16* vs_ = ks_ + Tile::SIZE;
     const int j0 = tile * BN;
@@ -87,14 +88,15 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     for (int j = 0; j < JB; ++j) {
       s[j] = zero16();
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[j] = mma(Tile::rows(ks_, 32 * j, ks), qf[ks], s[j]);
+      for (int ks = 0; ks < KS; ++ks) s[j] = mma(Tile::rows(ks_, lr, 32 * j, ks), qf[ks], s[j]);
     }
     if (j0 + BN > least) {  // some row does not see all of the tile
+      const int left = sees - j0 - 4 * half;
 #pragma unroll
       for (int j = 0; j < JB; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          if (j0 + 32 * j + prod_row(v, half) >= sees) s[j][v] = -INFINITY;
+          if (32 * j + prod_row(v, 0) >= left) s[j][v] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
@@ -133,7 +135,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         Planes<NP> pf;
         planes_of(x, pf);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(vs_, 32 * j + 16 * step, d), pf, o[d]);
+        for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(vs_, lc, 32 * j + 16 * step, d), pf, o[d]);
       }
   };
 
@@ -304,15 +306,23 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 }
 
 // Gradients of keys and values. One workgroup: 32 WM keys of one key head; wave (wm, rw) holds 32 keys and walks the
-// tiles rw, rw + RW, ... of 32 packed query rows. S = Q K^T (lane: a key, registers: query rows), so exp(S - lse) and
+// tiles rw, rw + RW, ... of 32 queries, of one query head of the group after the other. S = Q K^T (lane: a key, registers: query rows), so exp(S - lse) and
 // dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of the group.
 template <typename T, int DP, int WM, int RW>
-__global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
+__global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
   using Tile = AttnTile<NP, BR, DP>;
-  constexpr int kGroup = 2 * Tile::SIZE + 6 * BR;  // Q, G, base, delta and inverse of BR rows (bf16 units)
-  constexpr int kMerge = (RW - 1) * WM * DB * 16 * 64 * 2;
+  constexpr bool kDma = NP == 1;
+  constexpr int kStats = NP == 3 ? 3 * BR : 2 * BR;  // base, delta (and inverse) of BR rows
+  constexpr int kGroup = 2 * Tile::SIZE + 2 * kStats;  // in bf16 units
+  constexpr int MB = DB < 2 ? DB : 2;  // column blocks of a gradient that are joined at a time
+  constexpr int kMerge = (RW - 1) * WM * MB * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[RW * kGroup > kMerge ? RW * kGroup : kMerge];
+  __shared__ __attribute__((aligned(16))) __bf16 lds2[kDma ? RW * kGroup : 8];
+  // the values of the workgroup's keys stay in LDS where they and the keys do not both fit into registers
+  constexpr bool kLdsV = kDma && DP > 96 && RW > 1;
+  using VTile = AttnTile<NP, 32 * WM, DP>;
+  __shared__ __attribute__((aligned(16))) __bf16 lds_v[kLdsV ? VTile::SIZE : 8];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -326,14 +336,14 @@ __global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, 
   const int key0 = (int)first, key = key0 + 32 * wm + (lane & 31);
   const bool live = key < sg.nk;
   const int64_t kt = sg.k0 + (live ? key : 0);
-  const int rows = sg.nq * a.group, shift = sg.nk - sg.nq;
-  // the first query that sees this key, and that sees any key of the workgroup
+  const int shift = sg.nk - sg.nq;
+  // the first query that sees this key and the first that sees all keys of the workgroup; the tiles of a head that see any
   const int from = a.causal ? max(0, key - shift) : 0;
-  const int tile_lo = a.causal ? min(rows, max(0, key0 - shift) * a.group) / BR : 0;
-  const int tile_hi = (rows + BR - 1) / BR;
-  const int full = a.causal ? max(0, key0 + 32 * WM - 1 - shift) : 0;  // from this query on, all keys are seen
+  const int full = a.causal ? max(0, key0 + 32 * WM - 1 - shift) : 0;
+  const int tile_lo = a.causal ? min(sg.nq, max(0, key0 - shift)) / BR : 0;
+  const int head_tiles = (sg.nq + BR - 1) / BR - tile_lo, all_tiles = head_tiles * a.group;
 
-  Planes<NP> kf[KS], vf[KS];
+  Planes<NP> kf[KS], vf[kLdsV ? 1 : KS];
   {
     const T* kp = static_cast<const T*>(a.k) + kt * a.k_row + kvh * a.k_head;
     const T* vp = static_cast<const T*>(a.v) + kt * a.v_row + kvh * a.v_head;
@@ -342,7 +352,12 @@ __global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, 
       const int chunk = 2 * ks + half;
       const bool ok = live && 8 * chunk < a.dim;
       kf[ks] = raw_planes(ok ? raw_load(kp + 8 * chunk) : raw_zero<T>());
-      vf[ks] = raw_planes(ok ? raw_load(vp + 8 * chunk) : raw_zero<T>());
+      const Planes<NP> v = raw_planes(ok ? raw_load(vp + 8 * chunk) : raw_zero<T>());
+      if constexpr (kLdsV) {
+        if (rw == 0) VTile::put(lds_v, 32 * wm + (lane & 31), chunk, v);  // read after the first barrier
+      } else {
+        vf[ks] = v;
+      }
     }
   }
   fmd_f32x16 ak[DB], av[DB];
@@ -350,59 +365,57 @@ __global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, 
   for (int d = 0; d < DB; ++d) ak[d] = av[d] = zero16();
   const float c = a.scale * kLog2e;
 
-  __bf16* qs = lds + rw * kGroup;
-  __bf16* gs = qs + Tile::SIZE;
-  // [base, delta, inverse][BR]; bf16 takes the inverse into the exponent (the rounding of their sum, 2^-24 of it, is far
-  // below the rounding of P), fp32 multiplies
-  float* stat = reinterpret_cast<float*>(gs + Tile::SIZE);
-  constexpr int kStats = NP == 3 ? 3 * BR : 2 * BR;
   const int lt = threadIdx.x - rw * WM * 64;
-  const T *qb = static_cast<const T*>(a.q), *gb = static_cast<const T*>(b.g);
-  AttnLoad<T, NP, BR, DP, 64 * WM> ql, gl;
-  constexpr int kStatLoads = (kStats + 64 * WM - 1) / (64 * WM);
-  float st[kStatLoads];
-  auto issue = [&](int tile) {
-    const int r0 = tile * BR, n = tile < tile_hi ? rows - r0 : 0;
-    ql.load(lt, a.dim, [&](int i) {
-      const int r = r0 + i;
-      return i < n ? qb + (sg.q0 + r / a.group) * a.q_row + (kvh * a.group + r % a.group) * a.q_head : nullptr;
-    });
-    gl.load(lt, a.dim, [&](int i) {
-      const int r = r0 + i;
-      return i < n ? gb + (sg.q0 + r / a.group) * b.g_row + (kvh * a.group + r % a.group) * b.g_head : nullptr;
-    });
-    for (int n_ = 0; n_ < kStatLoads; ++n_) {
-      const int x = lt + n_ * 64 * WM, i = x % BR, r = r0 + i;
-      if (x >= kStats) break;
-      const int64_t at = i < n ? (kvh * a.group + r % a.group) * a.tq + sg.q0 + r / a.group : 0;
-      const float inv = i < n && x / BR != 1 ? b.saved.inverse[at] : 0.f;
-      // a row that sees nothing, and one past the end: exp(s - inf) = 0
-      if (x < BR) st[n_] = inv == 0.f ? INFINITY : NP == 3 ? b.saved.base[at] : b.saved.base[at] - __log2f(inv);
-      else if (x < 2 * BR) st[n_] = i < n ? b.delta[at] : 0.f;
-      else st[n_] = inv;
+  const T* qb = static_cast<const T*>(a.q) + sg.q0 * a.q_row + (int64_t)kvh * a.group * a.q_head;
+  const T* gb = static_cast<const T*>(b.g) + sg.q0 * b.g_row + (int64_t)kvh * a.group * b.g_head;
+  // the tile that is loaded next: its number, head of the group and first query
+  int next_tile = rw, next_head = 0, next_row = (tile_lo + rw) * BR;
+  auto wrap = [&] {
+    while (next_row >= (tile_lo + head_tiles) * BR && next_tile < all_tiles) {
+      next_row -= head_tiles * BR;
+      ++next_head;
     }
   };
-
-  const int rounds = (max(0, tile_hi - tile_lo) + RW - 1) / RW;
-  if (rounds > 0) issue(tile_lo + rw);
-  for (int it = 0; it < rounds; ++it) {
-    const int tile = tile_lo + it * RW + rw, r0 = tile * BR;
-    __syncthreads();
-    ql.store(qs, lt);
-    gl.store(gs, lt);
+  auto advance = [&] {
+    next_tile += RW;
+    next_row += RW * BR;
+    wrap();
+  };
+  // Per row: base, delta and inverse. bf16 takes the inverse into the exponent (the rounding of their sum, 2^-24 of it, is far
+  // below the rounding of P), fp32 multiplies. A row that sees nothing, and one past the end: exp(s - inf) = 0.
+  constexpr int kStatLoads = (kStats + 64 * WM - 1) / (64 * WM);
+  float st[kStatLoads];
+  auto load_stats = [&](int n) {
+    const int64_t row = (kvh * a.group + next_head) * a.tq + sg.q0 + next_row;
 #pragma unroll
-    for (int n = 0; n < kStatLoads; ++n)
-      if (lt + n * 64 * WM < kStats) stat[lt + n * 64 * WM] = st[n];
-    __syncthreads();
-    if (it + 1 < rounds) issue(tile + RW);
-    if (tile >= tile_hi) continue;
+    for (int k = 0; k < kStatLoads; ++k) {
+      const int x = lt + k * 64 * WM, i = x % BR;
+      const bool ok = x < kStats && i < n;
+      const float inv = ok && x / BR != 1 ? b.saved.inverse[row + i] : 0.f;
+      if (x < BR) st[k] = inv == 0.f ? INFINITY : NP == 3 ? b.saved.base[row + i] : b.saved.base[row + i] - __log2f(inv);
+      else if (x < 2 * BR) st[k] = ok ? b.delta[row + i] : 0.f;
+      else st[k] = inv;
+    }
+  };
+  auto store_stats = [&](__bf16* group) {
+    float* stat = reinterpret_cast<float*>(group + 2 * Tile::SIZE);
+#pragma unroll
+    for (int k = 0; k < kStatLoads; ++k)
+      if (lt + k * 64 * WM < kStats) stat[lt + k * 64 * WM] = st[k];
+  };
 
+  const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
+  auto step = [&](const __bf16* qs, int r0) {
+    int lr = lane_r, lc = lane_c;
+    if constexpr (kLdsV) asm volatile("" : "+v"(lr), "+v"(lc));  // addresses formed here, not kept in registers
+    const __bf16* gs = qs + Tile::SIZE;
+    const float* stat = reinterpret_cast<const float*>(gs + Tile::SIZE);
     fmd_f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(qs, 0, ks), kf[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(qs, lr, 0, ks), kf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(gs, 0, ks), vf[ks], dp);
-    const bool masked = a.causal && r0 / a.group < full;
+    for (int ks = 0; ks < KS; ++ks)
+      dp = mma(Tile::rows(gs, lr, 0, ks), kLdsV ? VTile::rows(lds_v, lr, 32 * wm, ks) : vf[kLdsV ? 0 : ks], dp);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float4 ls = *reinterpret_cast<const float4*>(stat + 8 * r + 4 * half);
@@ -414,11 +427,15 @@ __global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, 
         const int v = 4 * r + e;
         float p = exp2_hw(fmaf(s[v], c, -le[e]));
         if (NP == 3) p *= ie[e];
-        float ds = p * (dp[v] - de[e]);
-        if (masked && (r0 + prod_row(v, half)) / a.group < from) p = ds = 0.f;
         s[v] = p;
-        dp[v] = ds;
+        dp[v] = p * (dp[v] - de[e]);
       }
+    }
+    if (r0 < full) {  // some key of the workgroup is not seen by some row of the tile
+      const int hidden = from - r0 - 4 * half;
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        if (prod_row(v, 0) < hidden) s[v] = dp[v] = 0.f;
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
@@ -431,41 +448,95 @@ __global__ void __launch_bounds__(64 * WM * RW, attn_waves(AttnType<T>::planes, 
       Planes<NP> pf, df;
       planes_of(x, pf);
       planes_of(y, df);
-#pragma unroll
+  #pragma unroll
       for (int d = 0; d < DB; ++d) {
-        av[d] = mma(Tile::cols(gs, 16 * step, d), pf, av[d]);
-        ak[d] = mma(Tile::cols(qs, 16 * step, d), df, ak[d]);
+        av[d] = mma(Tile::cols(gs, lc, 16 * step, d), pf, av[d]);
+        ak[d] = mma(Tile::cols(qs, lc, 16 * step, d), df, ak[d]);
       }
+    }
+  };
+
+  const int rounds = (all_tiles + RW - 1) / RW;
+  wrap();
+  if constexpr (kDma) {
+    using Dma = AttnDma<BR, DP, 64 * WM>;
+    __bf16 *st0 = lds + rw * kGroup, *st1 = lds2 + rw * kGroup;
+    auto issue = [&](__bf16* to) {
+      const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
+      const int64_t r = n > 0 ? next_row : 0, h = n > 0 ? next_head : 0;
+      Dma::issue(qb + r * a.q_row + h * a.q_head, a.q_row, n, a.dim, lt, to);
+      Dma::issue(gb + r * b.g_row + h * b.g_head, b.g_row, n, a.dim, lt, to + Tile::SIZE);
+      load_stats(n);
+    };
+    auto round = [&](int it, const __bf16* here, __bf16* next) {
+      const int tile = next_tile, r0 = next_row;
+      __builtin_amdgcn_s_waitcnt(kWaitVm0);
+      __syncthreads();
+      advance();
+      if (it + 1 < rounds) issue(next);
+      if (tile < all_tiles) step(here, r0);
+      if (it + 1 < rounds) store_stats(next);
+    };
+    if (rounds > 0) {
+      issue(st0);
+      store_stats(st0);
+    }
+    for (int it = 0; it < rounds; it += 2) {
+      round(it, st0, st1);
+      if (it + 1 < rounds) round(it + 1, st1, st0);
+    }
+  } else {
+    __bf16* qs = lds + rw * kGroup;
+    AttnLoad<T, NP, BR, DP, 64 * WM> ql, gl;
+    auto issue = [&] {
+      const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
+      const T *qp = qb + next_row * a.q_row + next_head * a.q_head, *gp = gb + next_row * b.g_row + next_head * b.g_head;
+      ql.load(lt, a.dim, [&](int i) { return i < n ? qp + i * a.q_row : nullptr; });
+      gl.load(lt, a.dim, [&](int i) { return i < n ? gp + i * b.g_row : nullptr; });
+      load_stats(n);
+    };
+    if (rounds > 0) issue();
+    for (int it = 0; it < rounds; ++it) {
+      const int tile = next_tile, r0 = next_row;
+      __syncthreads();
+      ql.store(qs, lt);
+      gl.store(qs + Tile::SIZE, lt);
+      store_stats(qs);
+      __syncthreads();
+      advance();
+      if (it + 1 < rounds) issue();
+      if (tile < all_tiles) step(qs, r0);
     }
   }
 
-  if constexpr (RW > 1) {  // add the row groups, in their order, one gradient after the other
+  if constexpr (RW > 1) {  // add the row groups, in their order
     float* mg = reinterpret_cast<float*>(lds);
+    auto join = [&](fmd_f32x16(&acc)[DB]) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      __syncthreads();
-      if (rw > 0) {
-        float* w = mg + ((rw - 1) * WM + wm) * DB * 16 * 64 + lane;
+      for (int d0 = 0; d0 < DB; d0 += MB) {
+        __syncthreads();
+        float* mine = mg + ((rw - 1) * WM + wm) * MB * 16 * 64 + lane;
+        if (rw > 0) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+          for (int d = d0; d < d0 + MB && d < DB; ++d)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) w[(d * 16 + v) * 64] = which ? av[d][v] : ak[d][v];
-      }
-      __syncthreads();
-      if (rw == 0) {
+            for (int v = 0; v < 16; ++v) mine[((d - d0) * 16 + v) * 64] = acc[d][v];
+        }
+        __syncthreads();
+        if (rw == 0) {
 #pragma unroll
-        for (int g = 0; g < RW - 1; ++g) {
-          const float* w = mg + (g * WM + wm) * DB * 16 * 64 + lane;
+          for (int g = 0; g < RW - 1; ++g) {
+            const float* w = mg + (g * WM + wm) * MB * 16 * 64 + lane;
 #pragma unroll
-          for (int d = 0; d < DB; ++d)
+            for (int d = d0; d < d0 + MB && d < DB; ++d)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              if (which) av[d][v] += w[(d * 16 + v) * 64];
-              else ak[d][v] += w[(d * 16 + v) * 64];
-            }
+              for (int v = 0; v < 16; ++v) acc[d][v] += w[((d - d0) * 16 + v) * 64];
+          }
         }
       }
-    }
+    };
+    join(ak);
+    join(av);
     if (rw > 0) return;
   }
   if (!live) return;
@@ -504,13 +575,13 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   if (first >= rows) return;
   const int row0 = (int)first, row = row0 + 32 * wm + (lane & 31);
   const bool live = row < rows;
-  const int tok = (live ? row : rows - 1) / a.group, head = kvh * a.group + (live ? row : rows - 1) % a.group;
+  const int tok = attn_token(a, live ? row : rows - 1), head = kvh * a.group + (live ? row : rows - 1) - tok * a.group;
   const int64_t qt = sg.q0 + tok;
   const int shift = sg.nk - sg.nq;
   const int sees = a.causal ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
-  const int last_tok = min(row0 + 32 * WM, rows) - 1;
-  const int reach = a.causal ? max(0, min(sg.nk, last_tok / a.group + shift + 1)) : sg.nk;
-  const int least = a.causal ? max(0, min(sg.nk, row0 / a.group + shift + 1)) : sg.nk;
+  const int last_row = min(row0 + 32 * WM, rows) - 1;
+  const int reach = a.causal ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
+  const int least = a.causal ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
   const int tile_hi = (reach + BN - 1) / BN;
 
   Planes<NP> qf[KS], gf[KS];
@@ -543,6 +614,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
     vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
   };
+  const int lr = Tile::lane_rows(), lc = Tile::lane_cols();
   const int rounds = (tile_hi + KW - 1) / KW;
   if (rounds > 0) issue(kw);
   for (int it = 0; it < rounds; ++it) {
@@ -555,15 +627,16 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     if (tile >= tile_hi) continue;
     fmd_f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, 0, ks), qf[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, lr, 0, ks), qf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, 0, ks), gf[ks], dp);
-    const bool masked = j0 + BN > least;
+    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, 0, ks), gf[ks], dp);
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      float ds = exp2_hw(fmaf(s[v], c, -ls)) * fmaf(dp[v], inv, -dl);
-      if (masked && j0 + prod_row(v, half) >= sees) ds = 0.f;
-      s[v] = ds;
+    for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * fmaf(dp[v], inv, -dl);
+    if (j0 + BN > least) {
+      const int left = sees - j0 - 4 * half;
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        if (prod_row(v, 0) >= left) s[v] = 0.f;
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
@@ -573,7 +646,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       Planes<NP> df;
       planes_of(y, df);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, 16 * step, d), df, o[d]);
+      for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, lc, 16 * step, d), df, o[d]);
     }
   }
   if constexpr (KW > 1) {
@@ -671,9 +744,10 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_
   constexpr int kWaves = f32 && DP > 64 ? 2 : 4;
   if (gk) {
     if (wide_tiles(a.tk, 1, a.kv_heads, a.segments)) {
-      const int64_t tiles = tile_count(a.tk, 1, a.segments, 128);
+      constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4;
+      const int64_t tiles = tile_count(a.tk, 1, a.segments, 32 * kWM);
       FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-      attn_bwd_kv_kernel<T, DP, 4, 1><<<(unsigned)(tiles * a.kv_heads), 256, 0, stream>>>(a, b, tiles, gk, gv);
+      attn_bwd_kv_kernel<T, DP, kWM, kRW><<<(unsigned)(tiles * a.kv_heads), 64 * kWM * kRW, 0, stream>>>(a, b, tiles, gk, gv);
     } else {
       const int64_t tiles = tile_count(a.tk, 1, a.segments, 32);
       FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
@@ -760,6 +834,10 @@ AttnArgs args_of(const void* q, int64_t q_row, int64_t q_head, const void* k, in
   a.q_off = q_off, a.k_off = k_off, a.tq = tq, a.tk = tk;
   a.segments = segments, a.heads = heads, a.kv_heads = kv_heads, a.group = kv_heads > 0 ? heads / kv_heads : 0;
   a.dim = dim, a.causal = causal, a.scale = scale;
+  // ceil(2^(31 + s) / group) with group <= 2^s: exact for rows below 2^31
+  while ((1ll << (a.group_shift)) < a.group) ++a.group_shift;
+  a.group_shift += 31;
+  a.group_mul = a.group > 0 ? (uint32_t)(((1ull << a.group_shift) + a.group - 1) / a.group) : 0;
   return a;
 }
 
