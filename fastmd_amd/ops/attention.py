@@ -20,6 +20,7 @@ the same bits.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -50,27 +51,29 @@ class AttentionSaved(NamedTuple):
 
 
 def heads_view(x: Tensor) -> tuple[Tensor, int, int]:
-    """(tensor, row stride, head stride) of ``x`` [rows, heads, dim] with unit stride in dim and 16-byte aligned rows below MAX_ROW_STRIDE;
-    copies only when needed (any strides otherwise: columns of a packed projection are read in place)."""
+    """(tensor, row stride, head stride) of ``x`` [rows, heads, dim] with unit stride in dim and 16-byte aligned rows
+    below MAX_ROW_STRIDE; copies only when needed (any strides otherwise: columns of a packed projection are read in
+    place)."""
     rows, heads, dim = x.shape
-    unit = 16 // x.element_size()
     sr, sh, sd = x.stride()
     if rows <= 1:
         sr = heads * dim
     if heads <= 1:
         sh = dim
-    if (sd != 1 and dim > 1) or sr % unit or sh % unit or x.data_ptr() % 16 or sr >= MAX_ROW_STRIDE:
+    if (sd != 1 or (sr | sh) % (16 // x.element_size()) or x.data_ptr() % 16 or sr >= MAX_ROW_STRIDE) and (
+            rows and heads):
         x = x.clone(memory_format=torch.contiguous_format)
         sr, sh = heads * dim, dim
     return x, sr, sh
 
 
-def _check(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor, scale) -> float:
+def _refuse(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor, scale) -> None:
+    """ValueError for arguments that segment attention does not take (nothing for those that it does)."""
     require_cuda(q, k, v, q_offsets, k_offsets)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"q, k and v must be [rows, heads, dim], got {tuple(q.shape)}, {tuple(k.shape)}, "
                          f"{tuple(v.shape)}")
-    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    if q.dtype not in _TYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"q, k and v must all be float32 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
     if k.shape != v.shape:
         raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
@@ -88,45 +91,63 @@ def _check(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor
         raise ValueError(f"q_offsets has {q_offsets.numel() - 1} segments, k_offsets {k_offsets.numel() - 1}")
     if q.shape[0] * heads // kv_heads >= 2 ** 31 or k.shape[0] >= 2 ** 31:
         raise ValueError("segment attention takes fewer than 2^31 packed query rows and key rows")
-    scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
+    if scale is not None and not 0.0 < float(scale) < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
-    return scale
 
 
-def _offsets(off: Tensor) -> Tensor:
-    if off.dtype != torch.int64 or not off.is_contiguous():
-        off = off.to(torch.int64).contiguous()
-    return off
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
-def _common(q, k, v, q_offsets, k_offsets, causal, scale):
-    """The arguments that both directions share, and the tensors that they point into."""
+def _prepare(q, k, v, q_offsets, k_offsets, causal, scale):
+    """Checks, then the arguments that both directions share and the tensors that they point into. The smallest calls are
+    bound by host time: the usual case passes one condition, and what it excludes is named by ``_refuse``."""
+    shape, dtype, device = q.shape, q.dtype, q.get_device()
+    if k_offsets is None:
+        k_offsets = q_offsets
+    if not (len(shape) == 3 and device >= 0 and k.get_device() == device and v.get_device() == device
+            and q_offsets.get_device() == device and k_offsets.get_device() == device and dtype in _TYPES
+            and k.dtype is dtype and v.dtype is dtype and k.shape == v.shape and len(k.shape) == 3
+            and q_offsets.dtype is torch.int64 and k_offsets.dtype is torch.int64
+            and q_offsets.dim() == 1 and q_offsets.shape == k_offsets.shape and scale is None):
+        _refuse(q, k, v, q_offsets, k_offsets, scale)
+    tq, heads, dim = shape
+    tk, kv_heads, kdim = k.shape
+    segments = q_offsets.shape[0] - 1
+    if not (kdim == dim and 8 <= dim <= MAX_DIM and dim % 8 == 0 and heads and kv_heads and heads % kv_heads == 0
+            and segments >= 0 and tq * heads < 2 ** 31 and tk < 2 ** 31):
+        _refuse(q, k, v, q_offsets, k_offsets, scale)
     (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = heads_view(q), heads_view(k), heads_view(v)
     same = k_offsets is q_offsets
-    q_offsets = _offsets(q_offsets)
-    k_offsets = q_offsets if same else _offsets(k_offsets)
-    args = (1 if q.dtype == torch.bfloat16 else 0, q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head,
-            v.data_ptr(), v_row, v_head, q_offsets.data_ptr(), k_offsets.data_ptr(), q.shape[0], k.shape[0],
-            q_offsets.numel() - 1, q.shape[1], k.shape[1], q.shape[2], 1 if causal else 0, scale)
-    return args, (q, k, v, q_offsets, k_offsets)
+    if q_offsets.dtype is not torch.int64 or not q_offsets.is_contiguous():
+        q_offsets = q_offsets.to(torch.int64).contiguous()
+    if same:
+        k_offsets = q_offsets
+    elif k_offsets.dtype is not torch.int64 or not k_offsets.is_contiguous():
+        k_offsets = k_offsets.to(torch.int64).contiguous()
+    return ((_TYPES[dtype], q.data_ptr(), q_row, q_head, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head,
+             q_offsets.data_ptr(), k_offsets.data_ptr(), tq, tk, segments, heads, kv_heads, dim, 1 if causal else 0,
+             dim ** -0.5 if scale is None else float(scale)), (q, k, v, q_offsets, k_offsets))
+
+
+@functools.lru_cache(maxsize=256)
+def _plan(tq: int, tk: int, segments: int, heads: int, kv_heads: int, dim: int) -> tuple[int, int]:
+    """(key splits, floats of workspace) of the forward at these sizes."""
+    lib = _abi.load()
+    splits = lib.fmd_segment_attention_splits(tq, tk, segments, heads, kv_heads)
+    return splits, lib.fmd_segment_attention_work_size(splits, tq, heads, dim)
 
 
 def _forward(q, k, v, q_offsets, k_offsets, causal, scale, save):
-    args, keep = _common(q, k, v, q_offsets, k_offsets, causal, scale)
-    tq, heads, dim = q.shape
-    out = torch.empty((tq, heads, dim), dtype=q.dtype, device=q.device)
-    saved, base, inverse, residual = None, None, None, None
+    args, keep = _prepare(q, k, v, q_offsets, k_offsets, causal, scale)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    saved = base = inverse = residual = work = None
     if save:
-        rows = torch.empty((2, heads, tq), dtype=torch.float32, device=q.device)
-        saved = AttentionSaved(rows[0], rows[1], torch.empty_like(out) if q.dtype == torch.bfloat16 else None)
+        rows = torch.empty((2, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+        saved = AttentionSaved(rows[0], rows[1], torch.empty_like(out) if args[0] else None)
         base, inverse, residual = (_abi.ptr(x) for x in saved)
-    lib = _abi.load()
-    splits = lib.fmd_segment_attention_splits(tq, k.shape[0], args[14], heads, k.shape[1])
-    work = None
+    splits, size = _plan(*args[12:18])
     if splits > 1:
-        work = torch.empty(lib.fmd_segment_attention_work_size(splits, tq, heads, dim), dtype=torch.float32,
-                           device=q.device)
+        work = torch.empty(size, dtype=torch.float32, device=q.device)
     _abi.call("fmd_segment_attention", *args, splits, out.data_ptr(), base, inverse, residual, _abi.ptr(work), stream())
     del keep
     return out, saved
@@ -135,8 +156,6 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, scale, save):
 def segment_attention_forward(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tensor | None = None, *,
                               causal: bool = False, scale: float | None = None) -> tuple[Tensor, AttentionSaved]:
     """``(out, saved)`` without autograd: the output and what ``segment_attention_vjp`` takes besides it."""
-    k_offsets = q_offsets if k_offsets is None else k_offsets
-    scale = _check(q, k, v, q_offsets, k_offsets, scale)
     return _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
 
 
@@ -145,8 +164,7 @@ def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Te
                           scale: float | None = None, need_q: bool = True, need_kv: bool = True):
     """``(gq, gk, gv)`` from the gradient of the output and the results of ``segment_attention_forward`` (None where
     not needed; the gradients of k and v come together)."""
-    k_offsets = q_offsets if k_offsets is None else k_offsets
-    scale = _check(q, k, v, q_offsets, k_offsets, scale)
+    args, keep = _prepare(q, k, v, q_offsets, k_offsets, causal, scale)
     base, inverse, residual = saved
     require_cuda(q, gout, out, base, inverse, residual)
     if gout.shape != q.shape or gout.dtype != q.dtype or out.shape != q.shape or out.dtype != q.dtype:
@@ -159,13 +177,12 @@ def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Te
     if q.dtype == torch.bfloat16 and (residual is None or residual.shape != q.shape or residual.dtype != q.dtype
                                       or not residual.is_contiguous() or residual.data_ptr() % 16):
         raise ValueError("saved must be the forward's: the residual of a bfloat16 output")
-    args, keep = _common(q, k, v, q_offsets, k_offsets, causal, scale)
     gout, g_row, g_head = heads_view(gout)
     if not out.is_contiguous() or out.data_ptr() % 16:
         out = out.clone(memory_format=torch.contiguous_format)
-    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
-    gk = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None
-    gv = torch.empty(k.shape, dtype=q.dtype, device=q.device) if need_kv else None
+    gq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
+    gk = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
+    gv = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
     delta = torch.empty_like(base)
     _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), base.data_ptr(),
               inverse.data_ptr(), _abi.ptr(residual), delta.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
@@ -196,8 +213,6 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offs
     float32 or bfloat16, any strides; offsets [segments + 1] on the device (``k_offsets`` None: ``q_offsets``); ``scale``
     None: ``dim ** -0.5``. One query per segment (the next token of a sequence over its cache, an atom over its neighbours) is the
     same call: a long key axis is then split over the card and joined. Differentiable in q, k and v."""
-    k_offsets = q_offsets if k_offsets is None else k_offsets
-    scale = _check(q, k, v, q_offsets, k_offsets, scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SegmentAttention.apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
     return _forward(q, k, v, q_offsets, k_offsets, causal, scale, False)[0]

@@ -23,6 +23,7 @@ from fastmd_amd._device import require_cuda, stream
 from fastmd_amd.ops.attention import heads_view
 
 MAX_DIM = 256
+_TYPES = (torch.float32, torch.bfloat16)
 
 
 def rotary_frequencies(width: int, *, base: float = 10000.0, factor: float = 1.0, trained_length: int | None = None,
@@ -59,7 +60,23 @@ def rotary_tables(positions, width: int, *, device=None, amplitude: float = 1.0,
     return (angle.cos() * amplitude).float(), (angle.sin() * amplitude).float()
 
 
-def _check(q: Tensor, k: Tensor | None, q_weight, k_weight, cos: Tensor, sin: Tensor, positions, norm: bool) -> None:
+def _check(q: Tensor, k: Tensor | None, q_weight, k_weight, cos: Tensor, sin: Tensor, positions) -> None:
+    """ValueError for arguments that the kernels do not take. The smallest calls are bound by host time: the usual case
+    (both inputs, both weights, positions) passes one condition."""
+    if k is not None and q_weight is not None and k_weight is not None and positions is not None:
+        shape, dtype, device = q.shape, q.dtype, q.get_device()
+        if (len(shape) == 3 and len(k.shape) == 3 and device >= 0 and k.get_device() == device
+                and q_weight.get_device() == device and k_weight.get_device() == device and cos.get_device() == device
+                and sin.get_device() == device and positions.get_device() == device and dtype in _TYPES
+                and k.dtype is dtype and q_weight.dtype is dtype and k_weight.dtype is dtype
+                and cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.dim() == 2
+                and cos.shape == sin.shape and positions.dtype in (torch.int32, torch.int64)):
+            tokens, heads, dim = shape
+            kv_tokens, kv_heads, kv_dim = k.shape
+            if (kv_tokens == tokens and kv_dim == dim and heads and kv_heads and dim % 8 == 0 and 8 <= dim <= MAX_DIM
+                    and q_weight.shape == k_weight.shape == (dim,) and 2 * cos.shape[1] <= dim
+                    and positions.shape == (tokens,) and tokens * (heads + kv_heads) < 2 ** 31):
+                return
     require_cuda(q, k, q_weight, k_weight, cos, sin, positions)
     for name, x in (("q", q), ("k", k)):
         if x is None:
@@ -91,16 +108,11 @@ def _check(q: Tensor, k: Tensor | None, q_weight, k_weight, cos: Tensor, sin: Te
         raise ValueError("the norm and rotation take fewer than 2^31 rows")
 
 
-def _table(t: Tensor) -> Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
-def _weight(w: Tensor | None) -> Tensor | None:
-    if w is None:
-        return None
-    w = w.contiguous()
-    return w.clone() if w.data_ptr() % 16 else w
+def _aligned(t: Tensor | None) -> Tensor | None:
+    """A contiguous tensor on a 16-byte address (the same one if it is)."""
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _common(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm):
@@ -109,8 +121,7 @@ def _common(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, nor
     if k is not None:
         k, k_row, k_head = heads_view(k)
         kv_heads = k.shape[1]
-    q_weight, k_weight = _weight(q_weight), _weight(k_weight)
-    cos, sin = _table(cos), _table(sin)
+    q_weight, k_weight, cos, sin = _aligned(q_weight), _aligned(k_weight), _aligned(cos), _aligned(sin)
     if positions is not None:
         positions = positions.contiguous()
     rot = 2 * cos.shape[1]
@@ -123,8 +134,8 @@ def _common(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, nor
 
 def _forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm):
     args, keep = _common(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     _abi.call("fmd_qk_norm_rotary", *args, q_out.data_ptr(), _abi.ptr(k_out), stream())
     del keep
     return q_out, k_out
@@ -140,8 +151,8 @@ def _vjp(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved
     gk_row = gk_head = 0
     if gk is not None:
         gk, gk_row, gk_head = heads_view(gk)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     dim, work = q.shape[2], None
     dqw = torch.empty(dim, dtype=q.dtype, device=q.device) if weights and q_weight is not None else None
     dkw = torch.empty(dim, dtype=q.dtype, device=q.device) if weights and k_weight is not None else None
@@ -174,8 +185,7 @@ class _NormRotary(Function):
 
 
 def _apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm):
-    inputs = [x for x in (q, k, q_weight, k_weight) if x is not None]
-    if torch.is_grad_enabled() and any(x.requires_grad for x in inputs):
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
         out = _NormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm)
         return (out, None) if k is None else out
     return _forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm)
@@ -188,7 +198,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
     a packed projection are read in place) in one launch; weights [dim] of their type (None: ones), shared by the
     heads. Tables without columns give the norm alone. A position outside the tables gives NaN in the turned columns.
     Differentiable in q, k and the weights."""
-    _check(q, k, q_weight, k_weight, cos, sin, positions, True)
+    _check(q, k, q_weight, k_weight, cos, sin, positions)
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
     return _apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), True)
@@ -199,11 +209,11 @@ def qk_norm_rotary_vjp(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, q_weight: T
                        interleaved: bool = False):
     """``(gradient of q, of k, of q_weight, of k_weight)`` from the gradients of both outputs (the last two None for
     absent weights)."""
-    _check(q, k, q_weight, k_weight, cos, sin, positions, True)
+    _check(q, k, q_weight, k_weight, cos, sin, positions)
     return _vjp(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), True, True)
 
 
 def rotary(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor | None = None, *, interleaved: bool = False) -> Tensor:
     """The rotation alone, of x [tokens, heads, dim]. Differentiable in x."""
-    _check(x, None, None, None, cos, sin, positions, False)
+    _check(x, None, None, None, cos, sin, positions)
     return _apply(x, None, None, None, cos, sin, positions, 0.0, bool(interleaved), False)[0]
