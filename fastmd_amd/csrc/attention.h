@@ -41,7 +41,7 @@ struct AttnBwd {
   int64_t g_row, g_head;
   const void* out;
   AttnSaved saved;
-  const float* delta;  // [heads, tq]
+  const float* rows;  // scratch [2, heads, tq]: the exponents' offset and delta (attn_delta_kernel)
 };
 
 constexpr int kWaitVm0 = 0 | (7 << 4) | (15 << 8);  // s_waitcnt vmcnt(0)
@@ -299,12 +299,21 @@ struct AttnDma {
   // the chunk that lies at place `pos` of a row (the permutation is its own inverse)
   __device__ static __forceinline__ int chunk_at(int row, int pos) { return (Tile::at(row, pos) - row * Tile::LD) >> 3; }
 
+  // 64 lanes' words to consecutive ones
+  __device__ static __forceinline__ void copy4(const float* p, __bf16* to) {
+    typedef const __attribute__((address_space(1))) void* global_ptr;
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 4, 0, 0);
+  }
+
   __device__ static __forceinline__ void copy16(const __bf16* p, __bf16* to) {
     typedef const __attribute__((address_space(1))) void* global_ptr;
     typedef __attribute__((address_space(3))) void* lds_ptr;
     __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 16, 0, 0);
   }
 };
+
+__device__ const float g_attn_no_row[2] = {INFINITY, 0.f};  // offset and delta of a row past the end: exp(s - inf) = 0
 
 // row index of register v of a 32 x 32 product in lane half h
 __device__ __forceinline__ int prod_row(int v, int h) { return 8 * (v >> 2) + 4 * h + (v & 3); }

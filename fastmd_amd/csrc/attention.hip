@@ -282,9 +282,11 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, 
 
 // ------------------------------------------------------------------------------------ backward
 
-// delta[head, i] = g_i . o_i : 16 lanes a row
+// Per query and head: delta = g . o, and the offset that the exponents are formed with: base - log2(inverse) for bf16 (the
+// rounding of the sum, 2^-24 of it, is far below the rounding of P), base for fp32, which multiplies by the inverse; +inf for
+// a row that sees nothing. 16 lanes a row.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, int heads, int dim, float* delta) {
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, int heads, int dim, float* rows) {
   const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
   const int sub = threadIdx.x & 15;
   const int64_t tok = at / heads;
@@ -302,7 +304,12 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
     }
   }
   s = lanes_sum<16>(s);
-  if (tok < tq && sub == 0) delta[head * tq + tok] = s;
+  if (tok < tq && sub == 0) {
+    const int64_t i = head * tq + tok;
+    const float inv = b.saved.inverse[i];
+    rows[i] = inv == 0.f ? INFINITY : b.saved.base[i] - (sizeof(T) == 2 ? __log2f(inv) : 0.f);
+    rows[heads * tq + i] = s;
+  }
 }
 
 // Gradients of keys and values. One workgroup: 32 WM keys of one key head; wave (wm, rw) holds 32 keys and walks the
@@ -313,7 +320,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
   using Tile = AttnTile<NP, BR, DP>;
   constexpr bool kDma = NP == 1;
-  constexpr int kStats = NP == 3 ? 3 * BR : 2 * BR;  // base, delta (and inverse) of BR rows
+  constexpr int kStats = NP == 3 ? 3 * BR : 2 * BR;  // offset, delta (and inverse) of BR rows
   constexpr int kGroup = 2 * Tile::SIZE + 2 * kStats;  // in bf16 units
   constexpr int MB = DB < 2 ? DB : 2;  // column blocks of a gradient that are joined at a time
   constexpr int kMerge = (RW - 1) * WM * MB * 16 * 64 * 2;
@@ -381,29 +388,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     next_row += RW * BR;
     wrap();
   };
-  // Per row: base, delta and inverse. bf16 takes the inverse into the exponent (the rounding of their sum, 2^-24 of it, is far
-  // below the rounding of P), fp32 multiplies. A row that sees nothing, and one past the end: exp(s - inf) = 0.
-  constexpr int kStatLoads = (kStats + 64 * WM - 1) / (64 * WM);
-  float st[kStatLoads];
-  auto load_stats = [&](int n) {
-    const int64_t row = (kvh * a.group + next_head) * a.tq + sg.q0 + next_row;
-#pragma unroll
-    for (int k = 0; k < kStatLoads; ++k) {
-      const int x = lt + k * 64 * WM, i = x % BR;
-      const bool ok = x < kStats && i < n;
-      const float inv = ok && x / BR != 1 ? b.saved.inverse[row + i] : 0.f;
-      if (x < BR) st[k] = inv == 0.f ? INFINITY : NP == 3 ? b.saved.base[row + i] : b.saved.base[row + i] - __log2f(inv);
-      else if (x < 2 * BR) st[k] = ok ? b.delta[row + i] : 0.f;
-      else st[k] = inv;
-    }
-  };
-  auto store_stats = [&](__bf16* group) {
-    float* stat = reinterpret_cast<float*>(group + 2 * Tile::SIZE);
-#pragma unroll
-    for (int k = 0; k < kStatLoads; ++k)
-      if (lt + k * 64 * WM < kStats) stat[lt + k * 64 * WM] = st[k];
-  };
-
+  const float *offset = b.rows, *delta = b.rows + a.heads * a.tq;
   const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
   auto step = [&](const __bf16* qs, int r0) {
     int lr = lane_r, lc = lane_c;
@@ -466,7 +451,13 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
       const int64_t r = n > 0 ? next_row : 0, h = n > 0 ? next_head : 0;
       Dma::issue(qb + r * a.q_row + h * a.q_head, a.q_row, n, a.dim, lt, to);
       Dma::issue(gb + r * b.g_row + h * b.g_head, b.g_row, n, a.dim, lt, to + Tile::SIZE);
-      load_stats(n);
+      if (wm == 0) {  // offsets and deltas: lane i of each half the row i
+        const int i = lane & 31;
+        const float* p = (half ? delta : offset) + (kvh * a.group + h) * a.tq + sg.q0 + r + i;
+        if (i >= n) p = g_attn_no_row + half;
+        asm volatile("" : "+v"(p));
+        Dma::copy4(p, to + 2 * Tile::SIZE);
+      }
     };
     auto round = [&](int it, const __bf16* here, __bf16* next) {
       const int tile = next_tile, r0 = next_row;
@@ -475,12 +466,8 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
       advance();
       if (it + 1 < rounds) issue(next);
       if (tile < all_tiles) step(here, r0);
-      if (it + 1 < rounds) store_stats(next);
     };
-    if (rounds > 0) {
-      issue(st0);
-      store_stats(st0);
-    }
+    if (rounds > 0) issue(st0);
     for (int it = 0; it < rounds; it += 2) {
       round(it, st0, st1);
       if (it + 1 < rounds) round(it + 1, st1, st0);
@@ -488,12 +475,20 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   } else {
     __bf16* qs = lds + rw * kGroup;
     AttnLoad<T, NP, BR, DP, 64 * WM> ql, gl;
+    constexpr int kStatLoads = (kStats + 64 * WM - 1) / (64 * WM);
+    float st[kStatLoads];
     auto issue = [&] {
       const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
       const T *qp = qb + next_row * a.q_row + next_head * a.q_head, *gp = gb + next_row * b.g_row + next_head * b.g_head;
       ql.load(lt, a.dim, [&](int i) { return i < n ? qp + i * a.q_row : nullptr; });
       gl.load(lt, a.dim, [&](int i) { return i < n ? gp + i * b.g_row : nullptr; });
-      load_stats(n);
+      const int64_t row = (kvh * a.group + next_head) * a.tq + sg.q0 + next_row;
+#pragma unroll
+      for (int k = 0; k < kStatLoads; ++k) {
+        const int x = lt + k * 64 * WM, i = x % BR, which = x / BR;
+        const float* p = which == 0 ? offset : which == 1 ? delta : b.saved.inverse;
+        st[k] = which < 3 && i < n ? p[row + i] : which == 0 ? INFINITY : 0.f;
+      }
     };
     if (rounds > 0) issue();
     for (int it = 0; it < rounds; ++it) {
@@ -501,7 +496,9 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
       __syncthreads();
       ql.store(qs, lt);
       gl.store(qs + Tile::SIZE, lt);
-      store_stats(qs);
+#pragma unroll
+      for (int k = 0; k < kStatLoads; ++k)
+        if (lt + k * 64 * WM < kStats) reinterpret_cast<float*>(qs + 2 * Tile::SIZE)[lt + k * 64 * WM] = st[k];
       __syncthreads();
       advance();
       if (it + 1 < rounds) issue();
@@ -596,8 +593,9 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       gf[ks] = raw_planes(ok ? raw_load(gp + 8 * chunk) : raw_zero<T>());
     }
   }
-  const float inv = b.saved.inverse[head * a.tq + qt], ls = inv == 0.f ? INFINITY : b.saved.base[head * a.tq + qt];
-  const float dl = b.delta[head * a.tq + qt] * inv;
+  // fp32: P = exp2(s - offset) inverse, the inverse taken into the other factor of dS
+  const float inv = NP == 3 ? b.saved.inverse[head * a.tq + qt] : 1.f, ls = b.rows[head * a.tq + qt];
+  const float dl = b.rows[(a.heads + head) * a.tq + qt] * inv;
   fmd_f32x16 o[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) o[d] = zero16();
@@ -631,7 +629,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, 0, ks), gf[ks], dp);
 #pragma unroll
-    for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * fmaf(dp[v], inv, -dl);
+    for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * (NP == 3 ? fmaf(dp[v], inv, -dl) : dp[v] - dl);
     if (j0 + BN > least) {
       const int left = sees - j0 - 4 * half;
 #pragma unroll
@@ -803,20 +801,20 @@ int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
 }
 
 template <typename T>
-int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* delta, hipStream_t stream) {
+int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* rows, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
   const int64_t unit = 16 / sizeof(T);
-  FMD_REQUIRE(a.tq == 0 || (b.g && b.out && b.saved.base && b.saved.inverse && delta && (sizeof(T) == 4 || b.saved.residual)));
+  FMD_REQUIRE(a.tq == 0 || (b.g && b.out && b.saved.base && b.saved.inverse && rows && (sizeof(T) == 4 || b.saved.residual)));
   FMD_REQUIRE(aligned16(b.g) && aligned16(b.out) && aligned16(b.saved.residual));
   FMD_REQUIRE(b.g_row % unit == 0 && b.g_head % unit == 0);
   FMD_REQUIRE((gk == nullptr) == (gv == nullptr) && aligned16(gq) && aligned16(gk) && aligned16(gv));
-  b.delta = delta;
+  b.rows = rows;
   if (a.tq == 0) gq = nullptr;
   if (a.tk == 0) gk = gv = nullptr;
   if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_bwd<T>(a, b, gq, gk, gv, stream);
   if (a.tq > 0) {
-    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(b, a.tq, a.heads, a.dim, delta);
+    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(b, a.tq, a.heads, a.dim, rows);
     FMD_CHECK_LAUNCH();
   }
   if (a.dim <= 32) return run_bwd<T, 32>(a, b, gq, gk, gv, stream);
@@ -870,13 +868,13 @@ int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* o
 }
 
 int fmd_segment_attention_bwd(int32_t bf16, FMD_ATTN_PARAMS, const void* gout, int64_t g_row, int64_t g_head, const void* out,
-                              const float* base, const float* inverse, const void* residual, float* delta, void* gq,
+                              const float* base, const float* inverse, const void* residual, float* rows, void* gq,
                               void* gk, void* gv, hipStream_t stream) {
   const AttnArgs a = FMD_ATTN_ARGS;
   const AttnSaved saved = {const_cast<float*>(base), const_cast<float*>(inverse), const_cast<void*>(residual)};
   const AttnBwd b = {gout, g_row, g_head, out, saved, nullptr};
-  return bf16 ? backward(a, b, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), delta, stream)
-              : backward(a, b, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), delta, stream);
+  return bf16 ? backward(a, b, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), rows, stream)
+              : backward(a, b, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), rows, stream);
 }
 
 }  // extern "C"

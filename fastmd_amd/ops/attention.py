@@ -183,9 +183,9 @@ def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Te
     gq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
     gk = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
     gv = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
-    delta = torch.empty_like(base)
+    work = torch.empty((2, *rows), dtype=torch.float32, device=q.device)
     _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), base.data_ptr(),
-              inverse.data_ptr(), _abi.ptr(residual), delta.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
+              inverse.data_ptr(), _abi.ptr(residual), work.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
     del keep
     return gq, gk, gv
 

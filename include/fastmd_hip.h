@@ -839,13 +839,13 @@ int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_
 /* VJP of fmd_segment_attention: gq [tq, heads, dim], gk and gv [tk, kv_heads, dim] (contiguous; gq, or gk and gv
  * together, nullable) from the gradient `gout` of `out`, the forward's `out`, `base`,
  * `inverse` and (bf16) `residual`. Rows outside every segment get
- * zero. delta: scratch of heads * tq floats. No atomics: the same inputs give the same bits. */
+ * zero. rows: scratch of 2 * heads * tq floats. No atomics: the same inputs give the same bits. */
 int fmd_segment_attention_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                               int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
                               const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
                               int32_t kv_heads, int32_t dim, int32_t causal, float scale, const void* gout, int64_t g_row,
                               int64_t g_head, const void* out, const float* base, const float* inverse, const void* residual,
-                              float* delta, void* gq, void* gk, void* gv, hipStream_t stream);
+                              float* rows, void* gq, void* gk, void* gv, hipStream_t stream);
 
 /* Each head x of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (row and head strides in elements, 16-byte aligned
  * rows, dim a multiple of 8 up to 256): with norm, x (mean x^2 + eps)^(-1/2) weight (weights [dim] of the features' type,
