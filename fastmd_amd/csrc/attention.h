@@ -274,22 +274,36 @@ struct AttnDma {
   static constexpr int CH = Tile::LD / 8, N = ROWS * CH / THREADS, STEP = THREADS / CH;
   static_assert(ROWS * CH % THREADS == 0 && THREADS % CH == 0, "whole passes");
 
-  // rows [0, n) of the tile at `base` (row stride `ld`), by thread t; `wave_slot`: the wave's first slot
-  __device__ static __forceinline__ void issue(const __bf16* base, int64_t ld, int n, int dim, int t, __bf16* lds) {
-    const int wave_slot = __builtin_amdgcn_readfirstlane(t & ~63);
-    const int row0 = t / CH, pos = t % CH;  // of pass 0
-    uint32_t off = row0 * (int)ld;
-    asm volatile("" : "+v"(off));  // one register for all passes, not an address each
-    if (n >= ROWS && dim == DP && DP == Tile::LD) {
+  // thread t's byte offset in the rows of a tile, for even and odd passes (the permutation of rows eight apart differs)
+  __device__ static __forceinline__ void offsets(int t, int64_t ld, uint32_t (&off)[2]) {
+    const int row0 = t / CH, pos = t % CH;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        copy16(base + i * STEP * ld + (off + 8 * chunk_at(row0 + i * STEP, pos)), lds + (wave_slot + i * THREADS) * 8);
+    for (int i = 0; i < 2; ++i) {
+      const int chunk = chunk_at(row0 + i * STEP, pos);  // one past DP is never read: any value will do
+      off[i] = 2 * (row0 * (uint32_t)ld + 8 * (chunk < Tile::CHUNKS ? chunk : 0));
+    }
+  }
+
+  // rows [0, n) of the tile at `base` (row stride `ld`), by thread t with its offsets. STEP is a multiple of four rows, and
+  // the permutation repeats after sixteen: passes two apart have the same chunks where STEP is a multiple of eight.
+  __device__ static __forceinline__ void issue(const __bf16* base, int64_t ld, int n, int dim, int t, const uint32_t (&off)[2],
+                                               __bf16* lds) {
+    const int wave_slot = __builtin_amdgcn_readfirstlane(t & ~63);
+    if (STEP % 8 == 0 && n >= ROWS && dim == DP) {
+      const char* p = reinterpret_cast<const char*>(base);  // uniform; a lane adds its 32-bit offset
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        copy16(p + off[i & 1], lds + (wave_slot + i * THREADS) * 8);
+        p += 2 * STEP * ld;
+      }
       return;
     }
+    asm volatile("" : "+v"(t));  // nothing of the rare path is kept in registers over the caller's loop
+    const int row0 = t / CH, pos = t % CH;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = row0 + i * STEP, chunk = chunk_at(row, pos);
-      const __bf16* p = base + i * STEP * ld + (off + 8 * chunk);
+      const __bf16* p = base + row * ld + 8 * chunk;
       p = row < n && 8 * chunk < dim ? p : reinterpret_cast<const __bf16*>(g_attn_zero_chunk);
       asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
       copy16(p, lds + (wave_slot + i * THREADS) * 8);
@@ -306,7 +320,7 @@ struct AttnDma {
     __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 4, 0, 0);
   }
 
-  __device__ static __forceinline__ void copy16(const __bf16* p, __bf16* to) {
+  __device__ static __forceinline__ void copy16(const void* p, __bf16* to) {
     typedef const __attribute__((address_space(1))) void* global_ptr;
     typedef __attribute__((address_space(3))) void* lds_ptr;
     __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 16, 0, 0);

@@ -142,11 +142,18 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int rounds = (tile_hi - tile_lo + KW - 1) / KW;  // the same for every wave
   if constexpr (kDma) {
     using Dma = AttnDma<BN, DP, 64 * WM>;
+    uint32_t k_at[2], v_at[2];
+    Dma::offsets(lt, a.k_row, k_at);
+    Dma::offsets(lt, a.v_row, v_at);
+    // the tile that is loaded next; one past the last reads nothing
+    const T *kp = kb + (int64_t)(tile_lo + kw) * BN * a.k_row, *vp = vb + (int64_t)(tile_lo + kw) * BN * a.v_row;
+    const int64_t k_by = (int64_t)KW * BN * a.k_row, v_by = (int64_t)KW * BN * a.v_row;
     auto issue = [&](int tile, __bf16* to) {
       const int n = tile < tile_hi ? sg.nk - tile * BN : 0;
-      const int64_t j0 = n > 0 ? tile * BN : 0;
-      Dma::issue(kb + j0 * a.k_row, a.k_row, n, a.dim, lt, to);
-      Dma::issue(vb + j0 * a.v_row, a.v_row, n, a.dim, lt, to + Tile::SIZE);
+      Dma::issue(kp, a.k_row, n, a.dim, lt, k_at, to);
+      Dma::issue(vp, a.v_row, n, a.dim, lt, v_at, to + Tile::SIZE);
+      kp += k_by;
+      vp += v_by;
     };
     __bf16 *st0 = lds + kw * 2 * Tile::SIZE, *st1 = lds2 + kw * 2 * Tile::SIZE;
     auto round = [&](int it, const __bf16* here, __bf16* next) {
@@ -375,20 +382,29 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   const int lt = threadIdx.x - rw * WM * 64;
   const T* qb = static_cast<const T*>(a.q) + sg.q0 * a.q_row + (int64_t)kvh * a.group * a.q_head;
   const T* gb = static_cast<const T*>(b.g) + sg.q0 * b.g_row + (int64_t)kvh * a.group * b.g_head;
-  // the tile that is loaded next: its number, head of the group and first query
-  int next_tile = rw, next_head = 0, next_row = (tile_lo + rw) * BR;
+  // the tile that is loaded next: its number, first query, and where its rows and their statistics lie
+  int next_tile = rw, next_row = (tile_lo + rw) * BR;
+  const float *offset = b.rows, *delta = b.rows + a.heads * a.tq;
+  const T *qp = qb + (int64_t)next_row * a.q_row, *gp = gb + (int64_t)next_row * b.g_row;
+  int64_t stat_at = (int64_t)kvh * a.group * a.tq + sg.q0 + next_row;
+  const int64_t q_by = (int64_t)RW * BR * a.q_row, g_by = (int64_t)RW * BR * b.g_row;
+  const int64_t q_head = a.q_head - (int64_t)head_tiles * BR * a.q_row, g_head = b.g_head - (int64_t)head_tiles * BR * b.g_row;
   auto wrap = [&] {
-    while (next_row >= (tile_lo + head_tiles) * BR && next_tile < all_tiles) {
+    while (next_row >= (tile_lo + head_tiles) * BR && next_tile < all_tiles) {  // the next head's tiles
       next_row -= head_tiles * BR;
-      ++next_head;
+      qp += q_head;
+      gp += g_head;
+      stat_at += a.tq - head_tiles * BR;
     }
   };
   auto advance = [&] {
     next_tile += RW;
     next_row += RW * BR;
+    qp += q_by;
+    gp += g_by;
+    stat_at += RW * BR;
     wrap();
   };
-  const float *offset = b.rows, *delta = b.rows + a.heads * a.tq;
   const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
   auto step = [&](const __bf16* qs, int r0) {
     int lr = lane_r, lc = lane_c;
@@ -446,15 +462,20 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   if constexpr (kDma) {
     using Dma = AttnDma<BR, DP, 64 * WM>;
     __bf16 *st0 = lds + rw * kGroup, *st1 = lds2 + rw * kGroup;
+    uint32_t q_off[2], g_off[2];
+    Dma::offsets(lt, a.q_row, q_off);
+    Dma::offsets(lt, b.g_row, g_off);
     auto issue = [&](__bf16* to) {
       const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
-      const int64_t r = n > 0 ? next_row : 0, h = n > 0 ? next_head : 0;
-      Dma::issue(qb + r * a.q_row + h * a.q_head, a.q_row, n, a.dim, lt, to);
-      Dma::issue(gb + r * b.g_row + h * b.g_head, b.g_row, n, a.dim, lt, to + Tile::SIZE);
+      Dma::issue(qp, a.q_row, n, a.dim, lt, q_off, to);
+      Dma::issue(gp, b.g_row, n, a.dim, lt, g_off, to + Tile::SIZE);
       if (wm == 0) {  // offsets and deltas: lane i of each half the row i
-        const int i = lane & 31;
-        const float* p = (half ? delta : offset) + (kvh * a.group + h) * a.tq + sg.q0 + r + i;
-        if (i >= n) p = g_attn_no_row + half;
+        int i = lane;
+        asm volatile("" : "+v"(i));
+        const bool which = i >= 32;
+        i &= 31;
+        const float* p = (which ? delta : offset) + stat_at + i;
+        if (i >= n) p = g_attn_no_row + which;
         asm volatile("" : "+v"(p));
         Dma::copy4(p, to + 2 * Tile::SIZE);
       }
@@ -479,15 +500,13 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     float st[kStatLoads];
     auto issue = [&] {
       const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
-      const T *qp = qb + next_row * a.q_row + next_head * a.q_head, *gp = gb + next_row * b.g_row + next_head * b.g_head;
       ql.load(lt, a.dim, [&](int i) { return i < n ? qp + i * a.q_row : nullptr; });
       gl.load(lt, a.dim, [&](int i) { return i < n ? gp + i * b.g_row : nullptr; });
-      const int64_t row = (kvh * a.group + next_head) * a.tq + sg.q0 + next_row;
 #pragma unroll
       for (int k = 0; k < kStatLoads; ++k) {
         const int x = lt + k * 64 * WM, i = x % BR, which = x / BR;
         const float* p = which == 0 ? offset : which == 1 ? delta : b.saved.inverse;
-        st[k] = which < 3 && i < n ? p[row + i] : which == 0 ? INFINITY : 0.f;
+        st[k] = which < 3 && i < n ? p[stat_at + i] : which == 0 ? INFINITY : 0.f;
       }
     };
     if (rounds > 0) issue();
