@@ -572,10 +572,12 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 // Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T.
 template <typename T, int DP, int WM, int KW>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gq) {
-  constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = 32;
+  constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = WM > 1 && NP == 1 ? 64 : 32;
   using Tile = AttnTile<NP, BN, DP>;
-  constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * DB * 16 * 64 * 2;
+  constexpr bool kDma = NP == 1;
+  constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
+  __shared__ __attribute__((aligned(16))) __bf16 lds2[kDma ? kTiles : 8];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -620,36 +622,23 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   for (int d = 0; d < DB; ++d) o[d] = zero16();
   const float c = a.scale * kLog2e;
 
-  __bf16* ks_ = lds + kw * 2 * Tile::SIZE;
-  __bf16* vs_ = ks_ + Tile::SIZE;
   const int lt = threadIdx.x - kw * WM * 64;
   const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
   const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
-  AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
-  auto issue = [&](int tile) {
-    const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
-    kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
-    vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
-  };
   const int lr = Tile::lane_rows(), lc = Tile::lane_cols();
-  const int rounds = (tile_hi + KW - 1) / KW;
-  if (rounds > 0) issue(kw);
-  for (int it = 0; it < rounds; ++it) {
-    const int tile = it * KW + kw, j0 = tile * BN;
-    __syncthreads();
-    kl.store(ks_, lt);
-    vl.store(vs_, lt);
-    __syncthreads();
-    if (it + 1 < rounds) issue(tile + KW);
-    if (tile >= tile_hi) continue;
+  auto step = [&](const __bf16* ks_, int tile) {
+    const __bf16* vs_ = ks_ + Tile::SIZE;
+#pragma unroll
+    for (int jb = 0; jb < BN; jb += 32) {
+    const int j0 = tile * BN + jb;
     fmd_f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, lr, 0, ks), qf[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, lr, jb, ks), qf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, 0, ks), gf[ks], dp);
+    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, jb, ks), gf[ks], dp);
 #pragma unroll
     for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * (NP == 3 ? fmaf(dp[v], inv, -dl) : dp[v] - dl);
-    if (j0 + BN > least) {
+    if (j0 + 32 > least) {
       const int left = sees - j0 - 4 * half;
 #pragma unroll
       for (int v = 0; v < 16; ++v)
@@ -663,29 +652,75 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       Planes<NP> df;
       planes_of(y, df);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, lc, 16 * step, d), df, o[d]);
+      for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, lc, jb + 16 * step, d), df, o[d]);
+    }
+    }
+  };
+  const int rounds = (tile_hi + KW - 1) / KW;
+  if constexpr (kDma) {
+    using Dma = AttnDma<BN, DP, 64 * WM>;
+    __bf16 *st0 = lds + kw * 2 * Tile::SIZE, *st1 = lds2 + kw * 2 * Tile::SIZE;
+    uint32_t k_at[2], v_at[2];
+    Dma::offsets(lt, a.k_row, k_at);
+    Dma::offsets(lt, a.v_row, v_at);
+    const T *kp = kb + (int64_t)kw * BN * a.k_row, *vp = vb + (int64_t)kw * BN * a.v_row;
+    const int64_t k_by = (int64_t)KW * BN * a.k_row, v_by = (int64_t)KW * BN * a.v_row;
+    auto issue = [&](int tile, __bf16* to) {
+      const int n = tile < tile_hi ? sg.nk - tile * BN : 0;
+      Dma::issue(kp, a.k_row, n, a.dim, lt, k_at, to);
+      Dma::issue(vp, a.v_row, n, a.dim, lt, v_at, to + Tile::SIZE);
+      kp += k_by;
+      vp += v_by;
+    };
+    auto round = [&](int it, const __bf16* here, __bf16* next) {
+      const int tile = it * KW + kw;
+      __builtin_amdgcn_s_waitcnt(kWaitVm0);
+      __syncthreads();
+      if (it + 1 < rounds) issue(tile + KW, next);
+      if (tile < tile_hi) step(here, tile);
+    };
+    if (rounds > 0) issue(kw, st0);
+    for (int it = 0; it < rounds; it += 2) {
+      round(it, st0, st1);
+      if (it + 1 < rounds) round(it + 1, st1, st0);
+    }
+  } else {
+    __bf16* st = lds + kw * 2 * Tile::SIZE;
+    AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
+    auto issue = [&](int tile) {
+      const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
+      kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
+      vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
+    };
+    if (rounds > 0) issue(kw);
+    for (int it = 0; it < rounds; ++it) {
+      const int tile = it * KW + kw;
+      __syncthreads();
+      kl.store(st, lt);
+      vl.store(st + Tile::SIZE, lt);
+      __syncthreads();
+      if (it + 1 < rounds) issue(tile + KW);
+      if (tile < tile_hi) step(st, tile);
     }
   }
-  if constexpr (KW > 1) {
-    float* mg = reinterpret_cast<float*>(lds);
-    __syncthreads();
-    if (kw > 0) {
-      float* w = mg + ((kw - 1) * WM + wm) * DB * 16 * 64 + lane;
+  if constexpr (KW > 1) {  // add the key groups, in their order, a column block at a time
+    float* mg = reinterpret_cast<float*>(lds) + lane;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
+    for (int d = 0; d < DB; ++d) {
+      __syncthreads();
+      if (kw > 0) {
 #pragma unroll
-        for (int v = 0; v < 16; ++v) w[(d * 16 + v) * 64] = o[d][v];
+        for (int v = 0; v < 16; ++v) mg[(((kw - 1) * WM + wm) * 16 + v) * 64] = o[d][v];
+      }
+      __syncthreads();
+      if (kw == 0) {
+#pragma unroll
+        for (int g = 0; g < KW - 1; ++g)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[d][v] += mg[((g * WM + wm) * 16 + v) * 64];
+      }
     }
-    __syncthreads();
     if (kw > 0) return;
-#pragma unroll
-    for (int g = 0; g < KW - 1; ++g) {
-      const float* w = mg + (g * WM + wm) * DB * 16 * 64 + lane;
-#pragma unroll
-      for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[d][v] += w[(d * 16 + v) * 64];
-    }
   }
   if (!live) return;
   T* op = gq + (qt * a.heads + head) * a.dim;
