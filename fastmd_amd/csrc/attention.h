@@ -44,6 +44,13 @@ struct AttnBwd {
   const float* rows;  // scratch [2, heads, tq]: the exponents' offset and delta (attn_delta_kernel)
 };
 
+// The two arrays whose rows are staged in LDS by plain copies: keys and values, or queries and output gradients. bf16: the
+// caller's. fp32: their planes [rows, heads, 3, dim], split once for all workgroups that read them (attn_split_kernel).
+struct AttnTiles {
+  const __bf16 *x, *y;
+  int64_t x_row, x_head, y_row, y_head;
+};
+
 constexpr int kWaitVm0 = 0 | (7 << 4) | (15 << 8);  // s_waitcnt vmcnt(0)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -265,14 +272,15 @@ struct AttnLoad {
 
 __device__ __attribute__((aligned(16))) const uint32_t g_attn_zero_chunk[4] = {0, 0, 0, 0};
 
-// bf16 rows of a tile straight into LDS (no register stage): thread t of THREADS fills the 16-byte slots t, t + THREADS, ...
+// Rows of a tile straight into LDS (no register stage): thread t of THREADS fills the 16-byte slots t, t + THREADS, ...
 // of the tile, each with the chunk that the permutation puts there. Per lane one 32-bit offset into the tile's rows; the
 // chunks past the rows or past dim come from a zero chunk.
-template <int ROWS, int DP, int THREADS>
+template <int NP, int ROWS, int DP, int THREADS>
 struct AttnDma {
-  using Tile = AttnTile<1, ROWS, DP>;
-  static constexpr int CH = Tile::LD / 8, N = ROWS * CH / THREADS, STEP = THREADS / CH;
-  static_assert(ROWS * CH % THREADS == 0 && THREADS % CH == 0, "whole passes");
+  using Tile = AttnTile<NP, ROWS, DP>;
+  static constexpr int CH = Tile::LD / 8, ACTIVE = THREADS < ROWS * CH ? THREADS : ROWS * CH;  // threads that copy
+  static constexpr int N = ROWS * CH / ACTIVE, STEP = ACTIVE / CH;
+  static_assert(ROWS * CH % ACTIVE == 0 && ACTIVE % 64 == 0 && ACTIVE % CH == 0, "whole passes of whole waves");
 
   // thread t's byte offset in the rows of a tile, for even and odd passes (the permutation of rows eight apart differs)
   __device__ static __forceinline__ void offsets(int t, int64_t ld, uint32_t (&off)[2]) {
@@ -284,16 +292,24 @@ struct AttnDma {
     }
   }
 
-  // rows [0, n) of the tile at `base` (row stride `ld`), by thread t with its offsets. STEP is a multiple of four rows, and
-  // the permutation repeats after sixteen: passes two apart have the same chunks where STEP is a multiple of eight.
+  // the planes of a tile (plane stride dim)
   __device__ static __forceinline__ void issue(const __bf16* base, int64_t ld, int n, int dim, int t, const uint32_t (&off)[2],
                                                __bf16* lds) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) issue_plane(base + p * dim, ld, n, dim, t, off, lds + p * Tile::PLANE);
+  }
+
+  // rows [0, n) of the tile at `base` (row stride `ld`), by thread t with its offsets. STEP is a multiple of four rows, and
+  // the permutation repeats after sixteen: passes two apart have the same chunks where STEP is a multiple of eight.
+  __device__ static __forceinline__ void issue_plane(const __bf16* base, int64_t ld, int n, int dim, int t,
+                                                     const uint32_t (&off)[2], __bf16* lds) {
     const int wave_slot = __builtin_amdgcn_readfirstlane(t & ~63);
+    if (wave_slot >= ACTIVE) return;
     if (STEP % 8 == 0 && n >= ROWS && dim == DP) {
       const char* p = reinterpret_cast<const char*>(base);  // uniform; a lane adds its 32-bit offset
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        copy16(p + off[i & 1], lds + (wave_slot + i * THREADS) * 8);
+        copy16(p + off[i & 1], lds + (wave_slot + i * ACTIVE) * 8);
         p += 2 * STEP * ld;
       }
       return;
@@ -306,7 +322,7 @@ struct AttnDma {
       const __bf16* p = base + row * ld + 8 * chunk;
       p = row < n && 8 * chunk < dim ? p : reinterpret_cast<const __bf16*>(g_attn_zero_chunk);
       asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
-      copy16(p, lds + (wave_slot + i * THREADS) * 8);
+      copy16(p, lds + (wave_slot + i * ACTIVE) * 8);
     }
   }
 

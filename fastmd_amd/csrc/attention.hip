@@ -1,4 +1,6 @@
 // Attention of the query rows of each segment over the key rows of the same segment, and its VJP.
+#include <type_traits>
+
 #include "attention.h"
 
 namespace {
@@ -15,8 +17,9 @@ static constexpr int attn_waves(int planes, int dp, int sums) { return planes * 
 // sums over keys stay in the lane but for one exchange of the halves, and exp(S^T) is already the operand of
 // O^T = V^T P^T. Statistics and sums are fp32; P is rounded to bf16 for bf16 inputs (the output is, too) and kept as
 // three planes for fp32.
-template <typename T, int DP, int BN, int WM, int KW>
-__global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_fwd_kernel(AttnArgs a, int64_t tiles, int splits, T* out, AttnSaved saved,
+template <typename T, int DP, int BN, int WM, int KW, bool DMA>
+__global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_fwd_kernel(AttnArgs a, AttnTiles kv,
+                                                                int64_t tiles, int splits, T* out, AttnSaved saved,
                                                                 float* part_o, float* part_m, float* part_l) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, JB = BN / 32;
   using Tile = AttnTile<NP, BN, DP>;
@@ -26,7 +29,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   // split, into one
   constexpr bool kDma = NP == 1;
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
-  __shared__ __attribute__((aligned(16))) __bf16 lds2[kDma ? kTiles : 8];
+  __shared__ __attribute__((aligned(16))) __bf16 lds2[DMA ? kTiles : 8];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -72,8 +75,6 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const float c = a.scale * kLog2e;
 
   const int lt = threadIdx.x - kw * WM * 64;  // thread among those that load this group's tiles
-  const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
-  const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
   // The maximum follows the scores only where one outgrows it by kSlack (in log2 units): exponentials up to 2^kSlack are
   // as exact as those below one, and the sums are rescaled a few times per row instead of once per tile.
   constexpr float kSlack = 8.f;
@@ -140,18 +141,19 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   };
 
   const int rounds = (tile_hi - tile_lo + KW - 1) / KW;  // the same for every wave
-  if constexpr (kDma) {
-    using Dma = AttnDma<BN, DP, 64 * WM>;
+  if constexpr (DMA) {
+    using Dma = AttnDma<NP, BN, DP, 64 * WM>;
     uint32_t k_at[2], v_at[2];
-    Dma::offsets(lt, a.k_row, k_at);
-    Dma::offsets(lt, a.v_row, v_at);
+    Dma::offsets(lt, kv.x_row, k_at);
+    Dma::offsets(lt, kv.y_row, v_at);
     // the tile that is loaded next; one past the last reads nothing
-    const T *kp = kb + (int64_t)(tile_lo + kw) * BN * a.k_row, *vp = vb + (int64_t)(tile_lo + kw) * BN * a.v_row;
-    const int64_t k_by = (int64_t)KW * BN * a.k_row, v_by = (int64_t)KW * BN * a.v_row;
+    const __bf16* kp = kv.x + (sg.k0 + (int64_t)(tile_lo + kw) * BN) * kv.x_row + kvh * kv.x_head;
+    const __bf16* vp = kv.y + (sg.k0 + (int64_t)(tile_lo + kw) * BN) * kv.y_row + kvh * kv.y_head;
+    const int64_t k_by = (int64_t)KW * BN * kv.x_row, v_by = (int64_t)KW * BN * kv.y_row;
     auto issue = [&](int tile, __bf16* to) {
       const int n = tile < tile_hi ? sg.nk - tile * BN : 0;
-      Dma::issue(kp, a.k_row, n, a.dim, lt, k_at, to);
-      Dma::issue(vp, a.v_row, n, a.dim, lt, v_at, to + Tile::SIZE);
+      Dma::issue(kp, kv.x_row, n, a.dim, lt, k_at, to);
+      Dma::issue(vp, kv.y_row, n, a.dim, lt, v_at, to + Tile::SIZE);
       kp += k_by;
       vp += v_by;
     };
@@ -170,6 +172,8 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     }
   } else {
     __bf16* st = lds + kw * 2 * Tile::SIZE;
+    const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
+    const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
     AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
     auto issue = [&](int tile) {
       const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
@@ -322,19 +326,19 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // Gradients of keys and values. One workgroup: 32 WM keys of one key head; wave (wm, rw) holds 32 keys and walks the
 // tiles rw, rw + RW, ... of 32 queries, of one query head of the group after the other. S = Q K^T (lane: a key, registers: query rows), so exp(S - lse) and
 // dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of the group.
-template <typename T, int DP, int WM, int RW>
-__global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gk, T* gv) {
+template <typename T, int DP, int WM, int RW, bool DMA>
+__global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
+                                                                                              int64_t tiles, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
   using Tile = AttnTile<NP, BR, DP>;
-  constexpr bool kDma = NP == 1;
-  constexpr int kStats = NP == 3 ? 3 * BR : 2 * BR;  // offset, delta (and inverse) of BR rows
+  constexpr int kStats = NP == 3 ? 4 * BR : 2 * BR;  // offset, delta (inverse and nothing) of BR rows
   constexpr int kGroup = 2 * Tile::SIZE + 2 * kStats;  // in bf16 units
   constexpr int MB = DB < 2 ? DB : 2;  // column blocks of a gradient that are joined at a time
   constexpr int kMerge = (RW - 1) * WM * MB * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[RW * kGroup > kMerge ? RW * kGroup : kMerge];
-  __shared__ __attribute__((aligned(16))) __bf16 lds2[kDma ? RW * kGroup : 8];
+  __shared__ __attribute__((aligned(16))) __bf16 lds2[DMA ? RW * kGroup : 8];
   // the values of the workgroup's keys stay in LDS where they and the keys do not both fit into registers
-  constexpr bool kLdsV = kDma && DP > 96 && RW > 1;
+  constexpr bool kLdsV = NP == 1 && DP > 96 && RW > 1;
   using VTile = AttnTile<NP, 32 * WM, DP>;
   __shared__ __attribute__((aligned(16))) __bf16 lds_v[kLdsV ? VTile::SIZE : 8];
 
@@ -380,15 +384,17 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   const float c = a.scale * kLog2e;
 
   const int lt = threadIdx.x - rw * WM * 64;
-  const T* qb = static_cast<const T*>(a.q) + sg.q0 * a.q_row + (int64_t)kvh * a.group * a.q_head;
-  const T* gb = static_cast<const T*>(b.g) + sg.q0 * b.g_row + (int64_t)kvh * a.group * b.g_head;
   // the tile that is loaded next: its number, first query, and where its rows and their statistics lie
+  using S = std::conditional_t<DMA, __bf16, T>;
+  const int64_t q_ld = DMA ? qg.x_row : a.q_row, g_ld = DMA ? qg.y_row : b.g_row;
+  const int64_t q_hd = DMA ? qg.x_head : a.q_head, g_hd = DMA ? qg.y_head : b.g_head;
   int next_tile = rw, next_row = (tile_lo + rw) * BR;
-  const float *offset = b.rows, *delta = b.rows + a.heads * a.tq;
-  const T *qp = qb + (int64_t)next_row * a.q_row, *gp = gb + (int64_t)next_row * b.g_row;
+  const S* qp = static_cast<const S*>(DMA ? qg.x : a.q) + (sg.q0 + next_row) * q_ld + (int64_t)kvh * a.group * q_hd;
+  const S* gp = static_cast<const S*>(DMA ? qg.y : b.g) + (sg.q0 + next_row) * g_ld + (int64_t)kvh * a.group * g_hd;
   int64_t stat_at = (int64_t)kvh * a.group * a.tq + sg.q0 + next_row;
-  const int64_t q_by = (int64_t)RW * BR * a.q_row, g_by = (int64_t)RW * BR * b.g_row;
-  const int64_t q_head = a.q_head - (int64_t)head_tiles * BR * a.q_row, g_head = b.g_head - (int64_t)head_tiles * BR * b.g_row;
+  const float *offset = b.rows, *delta = b.rows + a.heads * a.tq;
+  const int64_t q_by = (int64_t)RW * BR * q_ld, g_by = (int64_t)RW * BR * g_ld;
+  const int64_t q_head = q_hd - (int64_t)head_tiles * BR * q_ld, g_head = g_hd - (int64_t)head_tiles * BR * g_ld;
   auto wrap = [&] {
     while (next_row >= (tile_lo + head_tiles) * BR && next_tile < all_tiles) {  // the next head's tiles
       next_row -= head_tiles * BR;
@@ -459,25 +465,26 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 
   const int rounds = (all_tiles + RW - 1) / RW;
   wrap();
-  if constexpr (kDma) {
-    using Dma = AttnDma<BR, DP, 64 * WM>;
+  if constexpr (DMA) {
+    using Dma = AttnDma<NP, BR, DP, 64 * WM>;
+    static_assert(NP == 1 || WM > 1, "the second wave copies the inverses");
     __bf16 *st0 = lds + rw * kGroup, *st1 = lds2 + rw * kGroup;
     uint32_t q_off[2], g_off[2];
-    Dma::offsets(lt, a.q_row, q_off);
-    Dma::offsets(lt, b.g_row, g_off);
+    Dma::offsets(lt, q_ld, q_off);
+    Dma::offsets(lt, g_ld, g_off);
     auto issue = [&](__bf16* to) {
       const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
-      Dma::issue(qp, a.q_row, n, a.dim, lt, q_off, to);
-      Dma::issue(gp, b.g_row, n, a.dim, lt, g_off, to + Tile::SIZE);
-      if (wm == 0) {  // offsets and deltas: lane i of each half the row i
+      Dma::issue(qp, q_ld, n, a.dim, lt, q_off, to);
+      Dma::issue(gp, g_ld, n, a.dim, lt, g_off, to + Tile::SIZE);
+      if (wm == 0 || (NP == 3 && wm == 1)) {  // offsets and deltas (inverses): lane i of each half the row i
         int i = lane;
         asm volatile("" : "+v"(i));
-        const bool which = i >= 32;
+        const bool second = i >= 32;
         i &= 31;
-        const float* p = (which ? delta : offset) + stat_at + i;
-        if (i >= n) p = g_attn_no_row + which;
+        const float* p = (wm == 1 ? b.saved.inverse : second ? delta : offset) + stat_at + i;
+        if (i >= n) p = g_attn_no_row + (second || wm == 1);
         asm volatile("" : "+v"(p));
-        Dma::copy4(p, to + 2 * Tile::SIZE);
+        Dma::copy4(p, to + 2 * Tile::SIZE + (wm == 1 ? 4 * BR : 0));
       }
     };
     auto round = [&](int it, const __bf16* here, __bf16* next) {
@@ -500,8 +507,8 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     float st[kStatLoads];
     auto issue = [&] {
       const int n = next_tile < all_tiles ? sg.nq - next_row : 0;
-      ql.load(lt, a.dim, [&](int i) { return i < n ? qp + i * a.q_row : nullptr; });
-      gl.load(lt, a.dim, [&](int i) { return i < n ? gp + i * b.g_row : nullptr; });
+      ql.load(lt, a.dim, [&](int i) { return i < n ? qp + i * q_ld : nullptr; });
+      gl.load(lt, a.dim, [&](int i) { return i < n ? gp + i * g_ld : nullptr; });
 #pragma unroll
       for (int k = 0; k < kStatLoads; ++k) {
         const int x = lt + k * 64 * WM, i = x % BR, which = x / BR;
@@ -570,14 +577,14 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 }
 
 // Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T.
-template <typename T, int DP, int WM, int KW>
-__global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, int64_t tiles, T* gq) {
+template <typename T, int DP, int WM, int KW, bool DMA>
+__global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, AttnTiles kv,
+                                                                                             int64_t tiles, T* gq) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = WM > 1 && NP == 1 ? 64 : 32;
   using Tile = AttnTile<NP, BN, DP>;
-  constexpr bool kDma = NP == 1;
   constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
-  __shared__ __attribute__((aligned(16))) __bf16 lds2[kDma ? kTiles : 8];
+  __shared__ __attribute__((aligned(16))) __bf16 lds2[DMA ? kTiles : 8];
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -623,52 +630,51 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const float c = a.scale * kLog2e;
 
   const int lt = threadIdx.x - kw * WM * 64;
-  const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
-  const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
   const int lr = Tile::lane_rows(), lc = Tile::lane_cols();
   auto step = [&](const __bf16* ks_, int tile) {
     const __bf16* vs_ = ks_ + Tile::SIZE;
 #pragma unroll
     for (int jb = 0; jb < BN; jb += 32) {
-    const int j0 = tile * BN + jb;
-    fmd_f32x16 s = zero16(), dp = zero16();
+      const int j0 = tile * BN + jb;
+      fmd_f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, lr, jb, ks), qf[ks], s);
+      for (int ks = 0; ks < KS; ++ks) s = mma(Tile::rows(ks_, lr, jb, ks), qf[ks], s);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, jb, ks), gf[ks], dp);
+      for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, jb, ks), gf[ks], dp);
 #pragma unroll
-    for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * (NP == 3 ? fmaf(dp[v], inv, -dl) : dp[v] - dl);
-    if (j0 + 32 > least) {
-      const int left = sees - j0 - 4 * half;
+      for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * (NP == 3 ? fmaf(dp[v], inv, -dl) : dp[v] - dl);
+      if (j0 + 32 > least) {
+        const int left = sees - j0 - 4 * half;
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
-        if (prod_row(v, 0) >= left) s[v] = 0.f;
-    }
+        for (int v = 0; v < 16; ++v)
+          if (prod_row(v, 0) >= left) s[v] = 0.f;
+      }
 #pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      float y[8];
+      for (int step = 0; step < 2; ++step) {
+        float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = s[8 * step + e];
-      Planes<NP> df;
-      planes_of(y, df);
+        for (int e = 0; e < 8; ++e) y[e] = s[8 * step + e];
+        Planes<NP> df;
+        planes_of(y, df);
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, lc, jb + 16 * step, d), df, o[d]);
-    }
+        for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, lc, jb + 16 * step, d), df, o[d]);
+      }
     }
   };
   const int rounds = (tile_hi + KW - 1) / KW;
-  if constexpr (kDma) {
-    using Dma = AttnDma<BN, DP, 64 * WM>;
+  if constexpr (DMA) {
+    using Dma = AttnDma<NP, BN, DP, 64 * WM>;
     __bf16 *st0 = lds + kw * 2 * Tile::SIZE, *st1 = lds2 + kw * 2 * Tile::SIZE;
     uint32_t k_at[2], v_at[2];
-    Dma::offsets(lt, a.k_row, k_at);
-    Dma::offsets(lt, a.v_row, v_at);
-    const T *kp = kb + (int64_t)kw * BN * a.k_row, *vp = vb + (int64_t)kw * BN * a.v_row;
-    const int64_t k_by = (int64_t)KW * BN * a.k_row, v_by = (int64_t)KW * BN * a.v_row;
+    Dma::offsets(lt, kv.x_row, k_at);
+    Dma::offsets(lt, kv.y_row, v_at);
+    const __bf16* kp = kv.x + (sg.k0 + (int64_t)kw * BN) * kv.x_row + kvh * kv.x_head;
+    const __bf16* vp = kv.y + (sg.k0 + (int64_t)kw * BN) * kv.y_row + kvh * kv.y_head;
+    const int64_t k_by = (int64_t)KW * BN * kv.x_row, v_by = (int64_t)KW * BN * kv.y_row;
     auto issue = [&](int tile, __bf16* to) {
       const int n = tile < tile_hi ? sg.nk - tile * BN : 0;
-      Dma::issue(kp, a.k_row, n, a.dim, lt, k_at, to);
-      Dma::issue(vp, a.v_row, n, a.dim, lt, v_at, to + Tile::SIZE);
+      Dma::issue(kp, kv.x_row, n, a.dim, lt, k_at, to);
+      Dma::issue(vp, kv.y_row, n, a.dim, lt, v_at, to + Tile::SIZE);
       kp += k_by;
       vp += v_by;
     };
@@ -686,6 +692,8 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     }
   } else {
     __bf16* st = lds + kw * 2 * Tile::SIZE;
+    const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + kvh * a.k_head;
+    const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + kvh * a.v_head;
     AttnLoad<T, NP, BN, DP, 64 * WM> kl, vl;
     auto issue = [&](int tile) {
       const int j0 = tile * BN, n = tile < tile_hi ? sg.nk - j0 : 0;
@@ -734,6 +742,24 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     }
 }
 
+// fp32 rows [rows, heads, dim] as planes [rows, heads, 3, dim], a thread per eight values
+__global__ void __launch_bounds__(256) attn_split_kernel(const float* x, int64_t x_row, int64_t x_head, const float* y, int64_t y_row,
+                                                         int64_t y_head, int64_t rows, int heads, int dim, __bf16* xp, __bf16* yp) {
+  const int chunks = dim / 8;
+  const int64_t n = rows * heads * chunks, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const int64_t rh = i / chunks, row = rh / heads;
+  const int chunk = (int)(i % chunks) * 8, head = (int)(rh % heads);
+  const float* src[2] = {x + row * x_row + head * x_head, y + row * y_row + head * y_head};
+  __bf16* dst[2] = {xp, yp};
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const Planes<3> v = raw_planes(raw_load(src[k] + chunk));
+#pragma unroll
+    for (int p = 0; p < 3; ++p) *reinterpret_cast<fmd_bf16x8*>(dst[k] + (rh * 3 + p) * dim + chunk) = v.p[p];
+  }
+}
+
 // ------------------------------------------------------------------------------------ launches
 
 // tiles of `bm` rows: the numbers that attn_find hands out
@@ -765,23 +791,67 @@ int split_count(int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
   return n < 1 ? 1 : n > 256 ? 256 : (int)n;
 }
 
+// Workspace, in floats from 16-byte aligned starts: the planes of two fp32 arrays of `rows` rows where the wide tiles take
+// them, then the splits' partial sums.
+int64_t planes_floats(int64_t rows, int heads, int dim) { return rows * heads * dim * 3; }  // two arrays of 3 bf16 planes
+
+int64_t forward_floats(bool bf16, int splits, int64_t tq, int64_t tk, int segments, int heads, int kv_heads, int dim) {
+  if (tq <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads) return 0;
+  const bool planes = !bf16 && !few_rows(tq, tk, segments, kv_heads) && wide_tiles(tq, heads / kv_heads, kv_heads, segments);
+  return (planes ? planes_floats(tk, kv_heads, dim) : 0) + (splits > 1 ? (int64_t)splits * tq * heads * (dim + 2) : 0);
+}
+
+int64_t backward_floats(bool bf16, int64_t tq, int64_t tk, int segments, int heads, int kv_heads, int dim) {
+  if (heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads || tq < 0 || tk < 0) return 0;
+  int64_t n = fmd_cdiv(2 * heads * tq, 4) * 4;  // offsets and deltas
+  if (!bf16 && !few_rows(tq, tk, segments, kv_heads)) {
+    if (wide_tiles(tq, heads / kv_heads, kv_heads, segments)) n += planes_floats(tk, kv_heads, dim);
+    if (wide_tiles(tk, 1, kv_heads, segments)) n += planes_floats(tq, heads, dim);
+  }
+  return n;
+}
+
+// the planes of two arrays, formed into `work`, which moves past them
+int split_planes(const void* x, int64_t x_row, int64_t x_head, const void* y, int64_t y_row, int64_t y_head, int64_t rows, int heads,
+                 int dim, float*& work, AttnTiles* t, hipStream_t stream) {
+  __bf16* xp = reinterpret_cast<__bf16*>(work);
+  __bf16* yp = xp + rows * heads * dim * 3;
+  work += planes_floats(rows, heads, dim);
+  const int64_t ld = (int64_t)heads * dim * 3;
+  *t = {xp, yp, ld, 3 * dim, ld, 3 * dim};
+  const int64_t n = rows * heads * (dim / 8);
+  if (n == 0) return FMD_OK;
+  FMD_REQUIRE(ld < (1 << 24) && n < (1ll << 38));
+  attn_split_kernel<<<(unsigned)fmd_cdiv(n, 256), 256, 0, stream>>>(static_cast<const float*>(x), x_row, x_head,
+                                                                    static_cast<const float*>(y), y_row, y_head, rows, heads, dim, xp, yp);
+  FMD_CHECK_LAUNCH();
+  return FMD_OK;
+}
+
+AttnTiles bf16_tiles(const void* x, int64_t x_row, int64_t x_head, const void* y, int64_t y_row, int64_t y_head) {
+  return {static_cast<const __bf16*>(x), static_cast<const __bf16*>(y), x_row, x_head, y_row, y_head};
+}
+
 template <typename T, int DP>
 int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
-  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4;
+  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = f32 && DP > 32 ? 32 : 64;
   const int64_t n = a.tq * a.heads;
-  float *po = work, *pm = work ? work + splits * n * a.dim : nullptr, *pl = work ? pm + splits * n : nullptr;
-  if (wide_tiles(a.tq, a.group, a.kv_heads, a.segments)) {
-    const int64_t tiles = tile_count(a.tq, a.group, a.segments, 128);
-    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    attn_fwd_kernel<T, DP, 64, 4, 1><<<dim3((unsigned)(tiles * a.kv_heads), splits), 256, 0, stream>>>(a, tiles, splits, out, saved,
-                                                                                                     po, pm, pl);
-  } else {
-    const int64_t tiles = tile_count(a.tq, a.group, a.segments, 32);
-    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    attn_fwd_kernel<T, DP, 32, 1, kKeyWaves><<<dim3((unsigned)(tiles * a.kv_heads), splits), 64 * kKeyWaves, 0, stream>>>(
-        a, tiles, splits, out, saved, po, pm, pl);
+  AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
+  const bool wide = wide_tiles(a.tq, a.group, a.kv_heads, a.segments);
+  FMD_REQUIRE(work || (splits == 1 && !(f32 && wide)));
+  if (f32 && wide) {
+    const int status = split_planes(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head, a.tk, a.kv_heads, a.dim, work, &t, stream);
+    if (status != FMD_OK) return status;
   }
+  float *po = work, *pm = work ? work + splits * n * a.dim : nullptr, *pl = work ? pm + splits * n : nullptr;
+  const int64_t tiles = tile_count(a.tq, a.group, a.segments, wide ? 128 : 32);
+  FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+  const dim3 grid((unsigned)(tiles * a.kv_heads), splits);
+  if (wide)
+    attn_fwd_kernel<T, DP, kWideKeys, 4, 1, true><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
+  else
+    attn_fwd_kernel<T, DP, 32, 1, kKeyWaves, !f32><<<grid, 64 * kKeyWaves, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
   FMD_CHECK_LAUNCH();
   if (splits > 1) {
     attn_join_kernel<T><<<(unsigned)fmd_cdiv(n, 4), 256, 0, stream>>>(a, splits, po, pm, pl, out, saved);
@@ -791,32 +861,36 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
 }
 
 template <typename T, int DP>
-int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream) {
+int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
   constexpr int kWaves = f32 && DP > 64 ? 2 : 4;
   if (gk) {
-    if (wide_tiles(a.tk, 1, a.kv_heads, a.segments)) {
-      constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4;
-      const int64_t tiles = tile_count(a.tk, 1, a.segments, 32 * kWM);
-      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-      attn_bwd_kv_kernel<T, DP, kWM, kRW><<<(unsigned)(tiles * a.kv_heads), 64 * kWM * kRW, 0, stream>>>(a, b, tiles, gk, gv);
-    } else {
-      const int64_t tiles = tile_count(a.tk, 1, a.segments, 32);
-      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-      attn_bwd_kv_kernel<T, DP, 1, kWaves><<<(unsigned)(tiles * a.kv_heads), 64 * kWaves, 0, stream>>>(a, b, tiles, gk, gv);
+    AttnTiles t = bf16_tiles(a.q, a.q_row, a.q_head, b.g, b.g_row, b.g_head);
+    const bool wide = wide_tiles(a.tk, 1, a.kv_heads, a.segments);
+    if (f32 && wide) {
+      const int status = split_planes(a.q, a.q_row, a.q_head, b.g, b.g_row, b.g_head, a.tq, a.heads, a.dim, work, &t, stream);
+      if (status != FMD_OK) return status;
     }
+    constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4;
+    const int64_t tiles = tile_count(a.tk, 1, a.segments, wide ? 32 * kWM : 32);
+    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+    const unsigned grid = (unsigned)(tiles * a.kv_heads);
+    if (wide) attn_bwd_kv_kernel<T, DP, kWM, kRW, true><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, tiles, gk, gv);
+    else attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gk, gv);
     FMD_CHECK_LAUNCH();
   }
   if (gq) {
-    if (wide_tiles(a.tq, a.group, a.kv_heads, a.segments)) {
-      const int64_t tiles = tile_count(a.tq, a.group, a.segments, 128);
-      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-      attn_bwd_q_kernel<T, DP, 4, 1><<<(unsigned)(tiles * a.kv_heads), 256, 0, stream>>>(a, b, tiles, gq);
-    } else {
-      const int64_t tiles = tile_count(a.tq, a.group, a.segments, 32);
-      FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-      attn_bwd_q_kernel<T, DP, 1, kWaves><<<(unsigned)(tiles * a.kv_heads), 64 * kWaves, 0, stream>>>(a, b, tiles, gq);
+    AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
+    const bool wide = wide_tiles(a.tq, a.group, a.kv_heads, a.segments);
+    if (f32 && wide) {
+      const int status = split_planes(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head, a.tk, a.kv_heads, a.dim, work, &t, stream);
+      if (status != FMD_OK) return status;
     }
+    const int64_t tiles = tile_count(a.tq, a.group, a.segments, wide ? 128 : 32);
+    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
+    const unsigned grid = (unsigned)(tiles * a.kv_heads);
+    if (wide) attn_bwd_q_kernel<T, DP, 4, 1, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, gq);
+    else attn_bwd_q_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gq);
     FMD_CHECK_LAUNCH();
   }
   return FMD_OK;
@@ -844,7 +918,7 @@ template <typename T>
 int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
-  FMD_REQUIRE(splits >= 1 && splits <= 1024 && (splits == 1 || work));
+  FMD_REQUIRE(splits >= 1 && splits <= 1024 && aligned16(work));
   if (a.tq == 0) return FMD_OK;
   FMD_REQUIRE(out && aligned16(out) && aligned16(saved.residual) && (saved.base == nullptr) == (saved.inverse == nullptr));
   if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_fwd<T>(a, out, saved, stream);
@@ -855,26 +929,28 @@ int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
 }
 
 template <typename T>
-int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* rows, hipStream_t stream) {
+int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
   const int64_t unit = 16 / sizeof(T);
-  FMD_REQUIRE(a.tq == 0 || (b.g && b.out && b.saved.base && b.saved.inverse && rows && (sizeof(T) == 4 || b.saved.residual)));
+  FMD_REQUIRE(a.tq == 0 || (b.g && b.out && b.saved.base && b.saved.inverse && (sizeof(T) == 4 || b.saved.residual)));
   FMD_REQUIRE(aligned16(b.g) && aligned16(b.out) && aligned16(b.saved.residual));
   FMD_REQUIRE(b.g_row % unit == 0 && b.g_head % unit == 0);
   FMD_REQUIRE((gk == nullptr) == (gv == nullptr) && aligned16(gq) && aligned16(gk) && aligned16(gv));
-  b.rows = rows;
+  FMD_REQUIRE(work && aligned16(work));
+  b.rows = work;
   if (a.tq == 0) gq = nullptr;
   if (a.tk == 0) gk = gv = nullptr;
   if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_bwd<T>(a, b, gq, gk, gv, stream);
   if (a.tq > 0) {
-    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(b, a.tq, a.heads, a.dim, rows);
+    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(b, a.tq, a.heads, a.dim, work);
     FMD_CHECK_LAUNCH();
   }
-  if (a.dim <= 32) return run_bwd<T, 32>(a, b, gq, gk, gv, stream);
-  if (a.dim <= 64) return run_bwd<T, 64>(a, b, gq, gk, gv, stream);
-  if (a.dim <= 96) return run_bwd<T, 96>(a, b, gq, gk, gv, stream);
-  return run_bwd<T, 128>(a, b, gq, gk, gv, stream);
+  work += fmd_cdiv(2 * a.heads * a.tq, 4) * 4;
+  if (a.dim <= 32) return run_bwd<T, 32>(a, b, gq, gk, gv, work, stream);
+  if (a.dim <= 64) return run_bwd<T, 64>(a, b, gq, gk, gv, work, stream);
+  if (a.dim <= 96) return run_bwd<T, 96>(a, b, gq, gk, gv, work, stream);
+  return run_bwd<T, 128>(a, b, gq, gk, gv, work, stream);
 }
 
 AttnArgs args_of(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -909,8 +985,14 @@ int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, i
   return split_count(tq, tk, segments, heads, kv_heads);
 }
 
-int64_t fmd_segment_attention_work_size(int32_t splits, int64_t tq, int32_t heads, int32_t dim) {
-  return splits > 1 && tq > 0 && heads > 0 && dim > 0 ? (int64_t)splits * tq * heads * (dim + 2) : 0;
+int64_t fmd_segment_attention_work_size(int32_t bf16, int32_t splits, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
+                                        int32_t kv_heads, int32_t dim) {
+  return forward_floats(bf16, splits, tq, tk, segments, heads, kv_heads, dim);
+}
+
+int64_t fmd_segment_attention_bwd_work_size(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
+                                            int32_t kv_heads, int32_t dim) {
+  return backward_floats(bf16, tq, tk, segments, heads, kv_heads, dim);
 }
 
 int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* out, float* base, float* inverse,
@@ -922,13 +1004,13 @@ int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* o
 }
 
 int fmd_segment_attention_bwd(int32_t bf16, FMD_ATTN_PARAMS, const void* gout, int64_t g_row, int64_t g_head, const void* out,
-                              const float* base, const float* inverse, const void* residual, float* rows, void* gq,
+                              const float* base, const float* inverse, const void* residual, float* work, void* gq,
                               void* gk, void* gv, hipStream_t stream) {
   const AttnArgs a = FMD_ATTN_ARGS;
   const AttnSaved saved = {const_cast<float*>(base), const_cast<float*>(inverse), const_cast<void*>(residual)};
   const AttnBwd b = {gout, g_row, g_head, out, saved, nullptr};
-  return bf16 ? backward(a, b, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), rows, stream)
-              : backward(a, b, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), rows, stream);
+  return bf16 ? backward(a, b, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), work, stream)
+              : backward(a, b, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), work, stream);
 }
 
 }  // extern "C"

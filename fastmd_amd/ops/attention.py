@@ -130,11 +130,11 @@ def _prepare(q, k, v, q_offsets, k_offsets, causal, scale):
 
 
 @functools.lru_cache(maxsize=256)
-def _plan(tq: int, tk: int, segments: int, heads: int, kv_heads: int, dim: int) -> tuple[int, int]:
+def _plan(bf16: int, tq: int, tk: int, segments: int, heads: int, kv_heads: int, dim: int) -> tuple[int, int]:
     """(key splits, floats of workspace) of the forward at these sizes."""
     lib = _abi.load()
     splits = lib.fmd_segment_attention_splits(tq, tk, segments, heads, kv_heads)
-    return splits, lib.fmd_segment_attention_work_size(splits, tq, heads, dim)
+    return splits, lib.fmd_segment_attention_work_size(bf16, splits, tq, tk, segments, heads, kv_heads, dim)
 
 
 def _forward(q, k, v, q_offsets, k_offsets, causal, scale, save):
@@ -145,8 +145,8 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, scale, save):
         rows = torch.empty((2, q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
         saved = AttentionSaved(rows[0], rows[1], torch.empty_like(out) if args[0] else None)
         base, inverse, residual = (_abi.ptr(x) for x in saved)
-    splits, size = _plan(*args[12:18])
-    if splits > 1:
+    splits, size = _plan(args[0], *args[12:18])
+    if size:
         work = torch.empty(size, dtype=torch.float32, device=q.device)
     _abi.call("fmd_segment_attention", *args, splits, out.data_ptr(), base, inverse, residual, _abi.ptr(work), stream())
     del keep
@@ -183,7 +183,8 @@ def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Te
     gq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
     gk = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
     gv = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
-    work = torch.empty((2, *rows), dtype=torch.float32, device=q.device)
+    size = _abi.load().fmd_segment_attention_bwd_work_size(args[0], *args[12:18])
+    work = torch.empty(max(4, size), dtype=torch.float32, device=q.device)
     _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), base.data_ptr(),
               inverse.data_ptr(), _abi.ptr(residual), work.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
     del keep

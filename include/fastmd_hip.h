@@ -827,9 +827,10 @@ int fmd_edge_stress_f32(const float* geo, const float* gvec, const int64_t* n_ed
  * For the VJP (all nullable): base and inverse [heads, tq], such that a probability is
  * exp2(score log2(e) - base) inverse (both 0 for a row that sees nothing), and for bf16 residual [tq, heads, dim], what the
  * rounding of out dropped.
- * splits: fmd_segment_attention_splits(); with more than one, `work` holds fmd_segment_attention_work_size() floats. */
+ * splits: fmd_segment_attention_splits(). work: fmd_segment_attention_work_size() floats on a 16-byte address (null for 0). */
 int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads);
-int64_t fmd_segment_attention_work_size(int32_t splits, int64_t tq, int32_t heads, int32_t dim);
+int64_t fmd_segment_attention_work_size(int32_t bf16, int32_t splits, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
+                                        int32_t kv_heads, int32_t dim);
 int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                           int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
                           const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
@@ -839,13 +840,15 @@ int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_
 /* VJP of fmd_segment_attention: gq [tq, heads, dim], gk and gv [tk, kv_heads, dim] (contiguous; gq, or gk and gv
  * together, nullable) from the gradient `gout` of `out`, the forward's `out`, `base`,
  * `inverse` and (bf16) `residual`. Rows outside every segment get
- * zero. rows: scratch of 2 * heads * tq floats. No atomics: the same inputs give the same bits. */
+ * zero. work: fmd_segment_attention_bwd_work_size() floats on a 16-byte address. No atomics: the same inputs give the same bits. */
+int64_t fmd_segment_attention_bwd_work_size(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
+                                            int32_t kv_heads, int32_t dim);
 int fmd_segment_attention_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                               int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
                               const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
                               int32_t kv_heads, int32_t dim, int32_t causal, float scale, const void* gout, int64_t g_row,
                               int64_t g_head, const void* out, const float* base, const float* inverse, const void* residual,
-                              float* rows, void* gq, void* gk, void* gv, hipStream_t stream);
+                              float* work, void* gq, void* gk, void* gv, hipStream_t stream);
 
 /* Each head x of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (row and head strides in elements, 16-byte aligned
  * rows, dim a multiple of 8 up to 256): with norm, x (mean x^2 + eps)^(-1/2) weight (weights [dim] of the features' type,
