@@ -257,7 +257,10 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   }
 }
 
-// The splits of a row joined in their order: one wave per (query, head), the lanes along dim.
+// The splits of a row joined in their order: one wave per (query, head). The lanes hold the splits' maxima and sums (at most 64
+// splits), then columns; the loads of eight splits are in flight together.
+constexpr int kMaxSplits = 64;
+
 template <typename T>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, const float* part_o, const float* part_m,
                                                         const float* part_l, T* out, AttnSaved saved) {
@@ -265,16 +268,26 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, 
   const int lane = threadIdx.x & 63;
   if (at >= n) return;
   const float c = a.scale * kLog2e;
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_m[s * n + at]);
-  const float base = top == -INFINITY ? 0.f : top * c;
-  float l = 0.f, o[2] = {0.f, 0.f};
-  for (int s = 0; s < splits; ++s) {
-    const float f = exp2_hw(fmaf(part_m[s * n + at], c, -base));
-    l += f * part_l[s * n + at];
+  const float m = lane < splits ? part_m[lane * n + at] : -INFINITY, pl = lane < splits ? part_l[lane * n + at] : 0.f;
+  const float top = wave_max(m), base = top == -INFINITY ? 0.f : top * c;
+  const float f = exp2_hw(fmaf(m, c, -base));
+  const float l = wave_sum(f * pl);
+  float o[2] = {0.f, 0.f};
+  for (int s0 = 0; s0 < splits; s0 += 8) {
+    float x[8][2];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      if (lane + 64 * k < a.dim) o[k] += f * part_o[(s * n + at) * a.dim + lane + 64 * k];
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int col = lane + 64 * k;
+        x[s][k] = s0 + s < splits && col < a.dim ? part_o[((s0 + s) * n + at) * a.dim + col] : 0.f;
+      }
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const float fs = __shfl(f, (s0 + s) & 63, 64);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) o[k] += fs * x[s][k];
+    }
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
@@ -765,30 +778,39 @@ __global__ void __launch_bounds__(256) attn_split_kernel(const float* x, int64_t
 // tiles of `bm` rows: the numbers that attn_find hands out
 int64_t tile_count(int64_t rows, int group, int segments, int bm) { return rows * group / bm + segments + 2; }
 
-// Rows of a tile from which its four waves take 32 rows each; below, they take the same rows and share the keys
-// (too few tiles to fill the card otherwise, and segments shorter than a tile).
-bool wide_tiles(int64_t rows, int group, int heads, int segments) {
-  return rows * group / 128 * heads >= 256 && rows * group >= (int64_t)64 * segments;
+// How a workgroup's waves share a tile. kWide: four waves of 32 rows each over the same keys. kNarrow: the waves take the same
+// 32 rows and share the keys, for calls with too few tiles to fill the card otherwise and segments shorter than a tile. kMid:
+// two and two, fp32 only, whose narrow form splits every tile into planes in the wave that reads it (fp32 heads above 64 have
+// room in LDS for wide tiles alone, and two narrow waves).
+enum AttnShape { kNarrow, kMid, kWide };
+
+AttnShape shape_of(bool f32, int dim, int64_t rows, int heads, int segments) {
+  const int64_t blocks = rows / 32 * heads;
+  if (rows < (int64_t)64 * segments) return kNarrow;
+  if (blocks >= 1024 || (f32 && dim > 64 && blocks >= 192)) return kWide;
+  return f32 && dim <= 64 && blocks >= 256 ? kMid : kNarrow;
 }
+
+constexpr int shape_rows(AttnShape s) { return s == kWide ? 128 : s == kMid ? 64 : 32; }
 
 // About one query per segment over a few keys each, and enough segments to fill the card with a wave each: the row kernels.
 bool few_rows(int64_t tq, int64_t tk, int segments, int kv_heads) {
   return segments >= 256 && tq <= segments && tk <= (int64_t)128 * segments;
 }
 
-// Key splits of the forward: as many as bring the workgroups to four per CU, each with kSplitKeys keys at least of a
+// Key splits of the forward: as many as bring the workgroups to one per CU, each with kSplitKeys keys at least of a
 // segment of mean length. Their partial sums (dim + 2 floats a row) are joined by a second launch.
-constexpr int kSplitKeys = 512, kSplitGroups = 1024;
+constexpr int kSplitKeys = 512, kSplitGroups = 256;
 
-int split_count(int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
+int split_count(bool f32, int dim, int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
   if (tq <= 0 || tk <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
   if (few_rows(tq, tk, segments, kv_heads)) return 1;
   const int group = heads / kv_heads;
-  const bool wide = wide_tiles(tq, group, kv_heads, segments);
-  const int64_t tiles = fmd_cdiv(fmd_cdiv(tq * group, segments), wide ? 128 : 32) * segments * kv_heads;
-  const int64_t fill = fmd_cdiv(kSplitGroups, tiles), most = tk / segments / kSplitKeys;
+  const int rows = shape_rows(shape_of(f32, dim, tq * group, kv_heads, segments));
+  const int64_t tiles = fmd_cdiv(fmd_cdiv(tq * group, segments), rows) * segments * kv_heads;
+  const int64_t fill = kSplitGroups / tiles, most = tk / segments / kSplitKeys;
   const int64_t n = fill < most ? fill : most;
-  return n < 1 ? 1 : n > 256 ? 256 : (int)n;
+  return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : (int)n;
 }
 
 // Workspace, in floats from 16-byte aligned starts: the planes of two fp32 arrays of `rows` rows where the wide tiles take
@@ -797,7 +819,8 @@ int64_t planes_floats(int64_t rows, int heads, int dim) { return rows * heads * 
 
 int64_t forward_floats(bool bf16, int splits, int64_t tq, int64_t tk, int segments, int heads, int kv_heads, int dim) {
   if (tq <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads) return 0;
-  const bool planes = !bf16 && !few_rows(tq, tk, segments, kv_heads) && wide_tiles(tq, heads / kv_heads, kv_heads, segments);
+  const bool planes = !bf16 && !few_rows(tq, tk, segments, kv_heads) &&
+                      shape_of(true, dim, tq * (heads / kv_heads), kv_heads, segments) != kNarrow;
   return (planes ? planes_floats(tk, kv_heads, dim) : 0) + (splits > 1 ? (int64_t)splits * tq * heads * (dim + 2) : 0);
 }
 
@@ -805,8 +828,8 @@ int64_t backward_floats(bool bf16, int64_t tq, int64_t tk, int segments, int hea
   if (heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads || tq < 0 || tk < 0) return 0;
   int64_t n = fmd_cdiv(2 * heads * tq, 4) * 4;  // offsets and deltas
   if (!bf16 && !few_rows(tq, tk, segments, kv_heads)) {
-    if (wide_tiles(tq, heads / kv_heads, kv_heads, segments)) n += planes_floats(tk, kv_heads, dim);
-    if (wide_tiles(tk, 1, kv_heads, segments)) n += planes_floats(tq, heads, dim);
+    if (shape_of(true, dim, tq * (heads / kv_heads), kv_heads, segments) != kNarrow) n += planes_floats(tk, kv_heads, dim);
+    if (shape_of(true, dim, tk, kv_heads, segments) != kNarrow) n += planes_floats(tq, heads, dim);
   }
   return n;
 }
@@ -838,20 +861,24 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = f32 && DP > 32 ? 32 : 64;
   const int64_t n = a.tq * a.heads;
   AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
-  const bool wide = wide_tiles(a.tq, a.group, a.kv_heads, a.segments);
-  FMD_REQUIRE(work || (splits == 1 && !(f32 && wide)));
-  if (f32 && wide) {
+  const AttnShape shape = shape_of(f32, a.dim, a.tq * a.group, a.kv_heads, a.segments);
+  FMD_REQUIRE(work || (splits == 1 && !(f32 && shape != kNarrow)));
+  if (f32 && shape != kNarrow) {
     const int status = split_planes(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head, a.tk, a.kv_heads, a.dim, work, &t, stream);
     if (status != FMD_OK) return status;
   }
   float *po = work, *pm = work ? work + splits * n * a.dim : nullptr, *pl = work ? pm + splits * n : nullptr;
-  const int64_t tiles = tile_count(a.tq, a.group, a.segments, wide ? 128 : 32);
+  const int64_t tiles = tile_count(a.tq, a.group, a.segments, shape_rows(shape));
   FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
   const dim3 grid((unsigned)(tiles * a.kv_heads), splits);
-  if (wide)
+  if (shape == kWide) {
     attn_fwd_kernel<T, DP, kWideKeys, 4, 1, true><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
-  else
+  } else if (shape == kMid) {
+    if constexpr (f32 && DP <= 64)
+      attn_fwd_kernel<T, DP, 32, 2, 2, true><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
+  } else {
     attn_fwd_kernel<T, DP, 32, 1, kKeyWaves, !f32><<<grid, 64 * kKeyWaves, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
+  }
   FMD_CHECK_LAUNCH();
   if (splits > 1) {
     attn_join_kernel<T><<<(unsigned)fmd_cdiv(n, 4), 256, 0, stream>>>(a, splits, po, pm, pl, out, saved);
@@ -866,31 +893,43 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, float* wor
   constexpr int kWaves = f32 && DP > 64 ? 2 : 4;
   if (gk) {
     AttnTiles t = bf16_tiles(a.q, a.q_row, a.q_head, b.g, b.g_row, b.g_head);
-    const bool wide = wide_tiles(a.tk, 1, a.kv_heads, a.segments);
-    if (f32 && wide) {
+    const AttnShape shape = shape_of(f32, a.dim, a.tk, a.kv_heads, a.segments);
+    if (f32 && shape != kNarrow) {
       const int status = split_planes(a.q, a.q_row, a.q_head, b.g, b.g_row, b.g_head, a.tq, a.heads, a.dim, work, &t, stream);
       if (status != FMD_OK) return status;
     }
-    constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4;
-    const int64_t tiles = tile_count(a.tk, 1, a.segments, wide ? 32 * kWM : 32);
+    // wide bf16: 64 keys and four row groups, two waves per SIMD in one workgroup
+    constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4, kMidRW = DP <= 32 ? 4 : 2;
+    const int64_t tiles = tile_count(a.tk, 1, a.segments, shape == kWide ? 32 * kWM : shape_rows(shape));
     FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
     const unsigned grid = (unsigned)(tiles * a.kv_heads);
-    if (wide) attn_bwd_kv_kernel<T, DP, kWM, kRW, true><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, tiles, gk, gv);
-    else attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gk, gv);
+    if (shape == kWide) {
+      attn_bwd_kv_kernel<T, DP, kWM, kRW, true><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, tiles, gk, gv);
+    } else if (shape == kMid) {
+      if constexpr (f32 && DP <= 64)
+        attn_bwd_kv_kernel<T, DP, 2, kMidRW, true><<<grid, 128 * kMidRW, 0, stream>>>(a, b, t, tiles, gk, gv);
+    } else {
+      attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gk, gv);
+    }
     FMD_CHECK_LAUNCH();
   }
   if (gq) {
     AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
-    const bool wide = wide_tiles(a.tq, a.group, a.kv_heads, a.segments);
-    if (f32 && wide) {
+    const AttnShape shape = shape_of(f32, a.dim, a.tq * a.group, a.kv_heads, a.segments);
+    if (f32 && shape != kNarrow) {
       const int status = split_planes(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head, a.tk, a.kv_heads, a.dim, work, &t, stream);
       if (status != FMD_OK) return status;
     }
-    const int64_t tiles = tile_count(a.tq, a.group, a.segments, wide ? 128 : 32);
+    const int64_t tiles = tile_count(a.tq, a.group, a.segments, shape_rows(shape));
     FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
     const unsigned grid = (unsigned)(tiles * a.kv_heads);
-    if (wide) attn_bwd_q_kernel<T, DP, 4, 1, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, gq);
-    else attn_bwd_q_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gq);
+    if (shape == kWide) {
+      attn_bwd_q_kernel<T, DP, 4, 1, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, gq);
+    } else if (shape == kMid) {
+      if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, gq);
+    } else {
+      attn_bwd_q_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gq);
+    }
     FMD_CHECK_LAUNCH();
   }
   return FMD_OK;
@@ -918,7 +957,7 @@ template <typename T>
 int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
-  FMD_REQUIRE(splits >= 1 && splits <= 1024 && aligned16(work));
+  FMD_REQUIRE(splits >= 1 && splits <= kMaxSplits && aligned16(work));
   if (a.tq == 0) return FMD_OK;
   FMD_REQUIRE(out && aligned16(out) && aligned16(saved.residual) && (saved.base == nullptr) == (saved.inverse == nullptr));
   if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_fwd<T>(a, out, saved, stream);
@@ -981,8 +1020,9 @@ extern "C" {
   args_of(q, q_row, q_head, k, k_row, k_head, v, v_row, v_head, q_offsets, k_offsets, tq, tk, segments, heads,   \
           kv_heads, dim, causal, scale)
 
-int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads) {
-  return split_count(tq, tk, segments, heads, kv_heads);
+int32_t fmd_segment_attention_splits(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads,
+                                     int32_t dim) {
+  return split_count(!bf16, dim, tq, tk, segments, heads, kv_heads);
 }
 
 int64_t fmd_segment_attention_work_size(int32_t bf16, int32_t splits, int64_t tq, int64_t tk, int32_t segments, int32_t heads,

@@ -133,7 +133,7 @@ def _prepare(q, k, v, q_offsets, k_offsets, causal, scale):
 def _plan(bf16: int, tq: int, tk: int, segments: int, heads: int, kv_heads: int, dim: int) -> tuple[int, int]:
     """(key splits, floats of workspace) of the forward at these sizes."""
     lib = _abi.load()
-    splits = lib.fmd_segment_attention_splits(tq, tk, segments, heads, kv_heads)
+    splits = lib.fmd_segment_attention_splits(bf16, tq, tk, segments, heads, kv_heads, dim)
     return splits, lib.fmd_segment_attention_work_size(bf16, splits, tq, tk, segments, heads, kv_heads, dim)
 
 

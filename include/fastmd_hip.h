@@ -828,7 +828,8 @@ int fmd_edge_stress_f32(const float* geo, const float* gvec, const int64_t* n_ed
  * exp2(score log2(e) - base) inverse (both 0 for a row that sees nothing), and for bf16 residual [tq, heads, dim], what the
  * rounding of out dropped.
  * splits: fmd_segment_attention_splits(). work: fmd_segment_attention_work_size() floats on a 16-byte address (null for 0). */
-int32_t fmd_segment_attention_splits(int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads);
+int32_t fmd_segment_attention_splits(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads,
+                                     int32_t dim);
 int64_t fmd_segment_attention_work_size(int32_t bf16, int32_t splits, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
                                         int32_t kv_heads, int32_t dim);
 int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,

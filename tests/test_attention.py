@@ -119,6 +119,15 @@ def test_wide_tiles(dim, dtype, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [16, 24, 64, 72, 128])
+def test_middle_sizes_in_float32(dim, causal):
+    """Enough rows for staged planes, too few for four waves of rows per tile."""
+    q, k, v, g, q_off, k_off = make([900, 1, 0, 801, 700], [900, 33, 5, 801, 650], 4, 4, dim, torch.float32, seed=dim)
+    check(q, k, v, g, q_off, k_off, causal=causal)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [32, 128])
 def test_wide_tiles_with_shared_heads_and_other_key_counts(dim, dtype):
@@ -135,7 +144,7 @@ def test_single_queries_over_long_keys(heads, kv_heads, dim, dtype):
 
     lk = [6000, 1, 0, 513, 2049]
     q, k, v, g, q_off, k_off = make([1] * 5, lk, heads, kv_heads, dim, dtype, seed=dim)
-    assert _abi.load().fmd_segment_attention_splits(5, sum(lk), 5, heads, kv_heads) > 1
+    assert _abi.load().fmd_segment_attention_splits(int(dtype == torch.bfloat16), 5, sum(lk), 5, heads, kv_heads, dim) > 1
     check(q, k, v, g, q_off, k_off, causal=False)
     check(q, k, v, g, q_off, k_off, causal=True)
 
