@@ -147,12 +147,13 @@ SIGNATURES: dict[str, tuple] = {
     "fmd_edge_stress_f32": (ctypes.c_int, [_p, _p, _p, _i64, _p, _p, _p, _p]),
     "fmd_segment_attention_splits": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _i32]),
     "fmd_segment_attention_work_size": (_i64, [_i32, _i32, _i64, _i64, _i32, _i32, _i32, _i32]),
-    "fmd_segment_attention_bwd_work_size": (_i64, [_i32, _i64, _i64, _i32, _i32, _i32, _i32]),
+    "fmd_segment_attention_bwd_splits": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32]),
+    "fmd_segment_attention_bwd_work_size": (_i64, [_i32, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32]),
     "fmd_segment_attention": (ctypes.c_int, [_i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64, _i64,
                                              _i32, _i32, _i32, _i32, _i32, _f32, _i32, _p, _p, _p, _p, _p, _p]),
     "fmd_segment_attention_bwd": (ctypes.c_int, [_i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _i64,
                                                  _i64, _i32, _i32, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p, _p, _p,
-                                                 _p, _p, _p, _p, _p, _p]),
+                                                 _p, _i32, _i32, _p, _p, _p, _p, _p]),
     "fmd_qk_norm_rotary": (ctypes.c_int, [_i32, _p, _i64, _i64, _i32, _p, _i64, _i64, _i32, _i64, _i32, _i32, _f32, _p,
                                           _p, _p, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _p, _p]),
     "fmd_qk_norm_rotary_work_size": (_i64, [_i64, _i32, _i32, _i32]),

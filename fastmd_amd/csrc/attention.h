@@ -383,6 +383,41 @@ __device__ __forceinline__ void store4<__bf16>(__bf16* p, float a, float b, floa
   *reinterpret_cast<fmd_bf16x4*>(p) = v;
 }
 
+// sixteen bytes past the caches (the `nt` bit) or through them: outputs larger than the last-level cache's share are not
+// read again before they are evicted
+template <bool NT>
+__device__ __forceinline__ void store16(void* p, uint4 v) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 x = {v.x, v.y, v.z, v.w};
+  if constexpr (NT) __builtin_nontemporal_store(x, static_cast<u32x4*>(p));
+  else *static_cast<u32x4*>(p) = x;
+}
+
+// eight values of a row, rounded once
+template <bool NT, typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    store16<NT>(p, make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])));
+    store16<NT>(p + 4, make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])));
+  } else {
+    fmd_bf16x8 v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (__bf16)x[i];
+    store16<NT>(p, __builtin_bit_cast(uint4, v));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  const Raw8<T> r = raw_load(p);
+  const T* e = reinterpret_cast<const T*>(&r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
+}
+
+// bytes of output from which a call's stores go past the caches
+constexpr int64_t kStreamBytes = 128 << 20;
+
 // the part of eight (four) outputs that their rounding to bf16 dropped
 template <typename T, int N>
 __device__ __forceinline__ void saved_residual(const AttnSaved& s, int64_t at, const float (&o)[N]) {

@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of the group.
 template <typename T, int DP, int WM, int RW, bool DMA>
 __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
-                                                                                              int64_t tiles, T* gk, T* gv) {
+                                                                                              int splits, float* part, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
   using Tile = AttnTile<NP, BR, DP>;
   constexpr int kStats = NP == 3 ? 4 * BR : 2 * BR;  // offset, delta (inverse and nothing) of BR rows
@@ -372,7 +372,10 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   const int from = a.causal ? max(0, key - shift) : 0;
   const int full = a.causal ? max(0, key0 + 32 * WM - 1 - shift) : 0;
   const int tile_lo = a.causal ? min(sg.nq, max(0, key0 - shift)) / BR : 0;
-  const int head_tiles = (sg.nq + BR - 1) / BR - tile_lo, all_tiles = head_tiles * a.group;
+  const int head_tiles = (sg.nq + BR - 1) / BR - tile_lo;
+  // this split's part of the tiles of all heads
+  const int per = (head_tiles * a.group + splits - 1) / splits, first_tile = blockIdx.y * per;
+  const int all_tiles = min(head_tiles * a.group, first_tile + per);
 
   Planes<NP> kf[KS], vf[kLdsV ? 1 : KS];
   {
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   using S = std::conditional_t<DMA, __bf16, T>;
   const int64_t q_ld = DMA ? qg.x_row : a.q_row, g_ld = DMA ? qg.y_row : b.g_row;
   const int64_t q_hd = DMA ? qg.x_head : a.q_head, g_hd = DMA ? qg.y_head : b.g_head;
-  int next_tile = rw, next_row = (tile_lo + rw) * BR;
+  int next_tile = first_tile + rw, next_row = (tile_lo + next_tile) * BR;
   const S* qp = static_cast<const S*>(DMA ? qg.x : a.q) + (sg.q0 + next_row) * q_ld + (int64_t)kvh * a.group * q_hd;
   const S* gp = static_cast<const S*>(DMA ? qg.y : b.g) + (sg.q0 + next_row) * g_ld + (int64_t)kvh * a.group * g_hd;
   int64_t stat_at = (int64_t)kvh * a.group * a.tq + sg.q0 + next_row;
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     }
   };
 
-  const int rounds = (all_tiles + RW - 1) / RW;
+  const int rounds = (max(0, all_tiles - first_tile) + RW - 1) / RW;
   wrap();
   if constexpr (DMA) {
     using Dma = AttnDma<NP, BR, DP, 64 * WM>;
@@ -576,7 +579,8 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     if (rw > 0) return;
   }
   if (!live) return;
-  const int64_t at = (kt * a.kv_heads + kvh) * a.dim;
+  const int64_t at = (kt * a.kv_heads + kvh) * a.dim, all = a.tk * a.kv_heads * a.dim;
+  float* pk = part + (int64_t)blockIdx.y * 2 * all + at;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -584,6 +588,11 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
       const int col = 32 * d + 8 * r + 4 * half;
       if (col >= a.dim) continue;
       const float f = a.scale;
+      if (splits > 1) {
+        store4<float>(pk + col, ak[d][4 * r] * f, ak[d][4 * r + 1] * f, ak[d][4 * r + 2] * f, ak[d][4 * r + 3] * f);
+        store4<float>(pk + all + col, av[d][4 * r], av[d][4 * r + 1], av[d][4 * r + 2], av[d][4 * r + 3]);
+        continue;
+      }
       store4<T>(gk + at + col, ak[d][4 * r] * f, ak[d][4 * r + 1] * f, ak[d][4 * r + 2] * f, ak[d][4 * r + 3] * f);
       store4<T>(gv + at + col, av[d][4 * r], av[d][4 * r + 1], av[d][4 * r + 2], av[d][4 * r + 3]);
     }
@@ -592,7 +601,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 // Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T.
 template <typename T, int DP, int WM, int KW, bool DMA>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, AttnTiles kv,
-                                                                                             int64_t tiles, T* gq) {
+                                                                                             int64_t tiles, int splits, float* part, T* gq) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = WM > 1 && NP == 1 ? 64 : 32;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * 16 * 64 * 2;
@@ -620,7 +629,8 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int last_row = min(row0 + 32 * WM, rows) - 1;
   const int reach = a.causal ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
   const int least = a.causal ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
-  const int tile_hi = (reach + BN - 1) / BN;
+  const int per = ((reach + BN - 1) / BN + splits - 1) / splits;
+  const int tile_lo = blockIdx.y * per, tile_hi = min((reach + BN - 1) / BN, tile_lo + per);
 
   Planes<NP> qf[KS], gf[KS];
   {
@@ -674,15 +684,15 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       }
     }
   };
-  const int rounds = (tile_hi + KW - 1) / KW;
+  const int rounds = (max(0, tile_hi - tile_lo) + KW - 1) / KW;
   if constexpr (DMA) {
     using Dma = AttnDma<NP, BN, DP, 64 * WM>;
     __bf16 *st0 = lds + kw * 2 * Tile::SIZE, *st1 = lds2 + kw * 2 * Tile::SIZE;
     uint32_t k_at[2], v_at[2];
     Dma::offsets(lt, kv.x_row, k_at);
     Dma::offsets(lt, kv.y_row, v_at);
-    const __bf16* kp = kv.x + (sg.k0 + (int64_t)kw * BN) * kv.x_row + kvh * kv.x_head;
-    const __bf16* vp = kv.y + (sg.k0 + (int64_t)kw * BN) * kv.y_row + kvh * kv.y_head;
+    const __bf16* kp = kv.x + (sg.k0 + (int64_t)(tile_lo + kw) * BN) * kv.x_row + kvh * kv.x_head;
+    const __bf16* vp = kv.y + (sg.k0 + (int64_t)(tile_lo + kw) * BN) * kv.y_row + kvh * kv.y_head;
     const int64_t k_by = (int64_t)KW * BN * kv.x_row, v_by = (int64_t)KW * BN * kv.y_row;
     auto issue = [&](int tile, __bf16* to) {
       const int n = tile < tile_hi ? sg.nk - tile * BN : 0;
@@ -692,13 +702,13 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       vp += v_by;
     };
     auto round = [&](int it, const __bf16* here, __bf16* next) {
-      const int tile = it * KW + kw;
+      const int tile = tile_lo + it * KW + kw;
       __builtin_amdgcn_s_waitcnt(kWaitVm0);
       __syncthreads();
       if (it + 1 < rounds) issue(tile + KW, next);
       if (tile < tile_hi) step(here, tile);
     };
-    if (rounds > 0) issue(kw, st0);
+    if (rounds > 0) issue(tile_lo + kw, st0);
     for (int it = 0; it < rounds; it += 2) {
       round(it, st0, st1);
       if (it + 1 < rounds) round(it + 1, st1, st0);
@@ -713,9 +723,9 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       kl.load(lt, a.dim, [&](int i) { return i < n ? kb + (int64_t)(j0 + i) * a.k_row : nullptr; });
       vl.load(lt, a.dim, [&](int i) { return i < n ? vb + (int64_t)(j0 + i) * a.v_row : nullptr; });
     };
-    if (rounds > 0) issue(kw);
+    if (rounds > 0) issue(tile_lo + kw);
     for (int it = 0; it < rounds; ++it) {
-      const int tile = it * KW + kw;
+      const int tile = tile_lo + it * KW + kw;
       __syncthreads();
       kl.store(st, lt);
       vl.store(st + Tile::SIZE, lt);
@@ -744,15 +754,31 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
     if (kw > 0) return;
   }
   if (!live) return;
-  T* op = gq + (qt * a.heads + head) * a.dim;
+  const int64_t at = (qt * a.heads + head) * a.dim;
+  float* pq = part + (int64_t)blockIdx.y * a.tq * a.heads * a.dim + at;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int col = 32 * d + 8 * r + 4 * half;
       const float f = a.scale;
-      if (col < a.dim) store4<T>(op + col, o[d][4 * r] * f, o[d][4 * r + 1] * f, o[d][4 * r + 2] * f, o[d][4 * r + 3] * f);
+      if (col >= a.dim) continue;
+      if (splits > 1) store4<float>(pq + col, o[d][4 * r] * f, o[d][4 * r + 1] * f, o[d][4 * r + 2] * f, o[d][4 * r + 3] * f);
+      else store4<T>(gq + at + col, o[d][4 * r] * f, o[d][4 * r + 1] * f, o[d][4 * r + 2] * f, o[d][4 * r + 3] * f);
     }
+}
+
+// The splits' sums added in their order, four values a thread: of x, and of y behind it in every split (or null)
+template <typename T>
+__global__ void __launch_bounds__(256) attn_add_kernel(const float* part, int64_t n, int splits, T* x, T* y) {
+  const int64_t all = y ? 2 * n : n, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= all) return;
+  float4 s = *reinterpret_cast<const float4*>(part + i);
+  for (int k = 1; k < splits; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(part + k * all + i);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  store4<T>(i < n ? x + i : y + i - n, s.x, s.y, s.z, s.w);
 }
 
 // fp32 rows [rows, heads, dim] as planes [rows, heads, 3, dim], a thread per eight values
@@ -824,13 +850,29 @@ int64_t forward_floats(bool bf16, int splits, int64_t tq, int64_t tk, int segmen
   return (planes ? planes_floats(tk, kv_heads, dim) : 0) + (splits > 1 ? (int64_t)splits * tq * heads * (dim + 2) : 0);
 }
 
-int64_t backward_floats(bool bf16, int64_t tq, int64_t tk, int segments, int heads, int kv_heads, int dim) {
+// Splits of the VJP's walks, for as few workgroups: of the query rows for gk and gv, and of the keys for gq.
+constexpr int kSplitRows = 256;
+
+int row_splits(bool f32, int dim, int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
+  const AttnShape shape = shape_of(f32, dim, tk, kv_heads, segments);
+  if (segments <= 0) return 1;
+  const int64_t tiles = fmd_cdiv(fmd_cdiv(tk, segments), shape_rows(shape)) * segments * kv_heads;
+  const int64_t fill = tiles > 0 ? kSplitGroups / tiles : 1, most = tq * (heads / kv_heads) / segments / kSplitRows;
+  const int64_t n = fill < most ? fill : most;
+  return n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : (int)n;
+}
+
+int64_t backward_floats(bool bf16, int64_t tq, int64_t tk, int segments, int heads, int kv_heads, int dim, int q_splits,
+                        int kv_splits) {
   if (heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads || tq < 0 || tk < 0) return 0;
   int64_t n = fmd_cdiv(2 * heads * tq, 4) * 4;  // offsets and deltas
-  if (!bf16 && !few_rows(tq, tk, segments, kv_heads)) {
+  if (few_rows(tq, tk, segments, kv_heads)) return n;
+  if (!bf16) {
     if (shape_of(true, dim, tq * (heads / kv_heads), kv_heads, segments) != kNarrow) n += planes_floats(tk, kv_heads, dim);
     if (shape_of(true, dim, tk, kv_heads, segments) != kNarrow) n += planes_floats(tq, heads, dim);
   }
+  if (q_splits > 1) n += q_splits * tq * heads * dim;
+  if (kv_splits > 1) n += kv_splits * 2 * tk * kv_heads * dim;
   return n;
 }
 
@@ -888,7 +930,7 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
 }
 
 template <typename T, int DP>
-int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
+int run_bwd(const AttnArgs& a, const AttnBwd& b, int q_splits, int kv_splits, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
   constexpr int kWaves = f32 && DP > 64 ? 2 : 4;
   if (gk) {
@@ -902,16 +944,24 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, float* wor
     constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4, kMidRW = DP <= 32 ? 4 : 2;
     const int64_t tiles = tile_count(a.tk, 1, a.segments, shape == kWide ? 32 * kWM : shape_rows(shape));
     FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    const unsigned grid = (unsigned)(tiles * a.kv_heads);
+    const dim3 grid((unsigned)(tiles * a.kv_heads), kv_splits);
+    float* part = work;
+    if (kv_splits > 1) work += kv_splits * 2 * a.tk * a.kv_heads * a.dim;
     if (shape == kWide) {
-      attn_bwd_kv_kernel<T, DP, kWM, kRW, true><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, tiles, gk, gv);
+      attn_bwd_kv_kernel<T, DP, kWM, kRW, true><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
     } else if (shape == kMid) {
       if constexpr (f32 && DP <= 64)
-        attn_bwd_kv_kernel<T, DP, 2, kMidRW, true><<<grid, 128 * kMidRW, 0, stream>>>(a, b, t, tiles, gk, gv);
+        attn_bwd_kv_kernel<T, DP, 2, kMidRW, true><<<grid, 128 * kMidRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
     } else {
-      attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gk, gv);
+      attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
     }
     FMD_CHECK_LAUNCH();
+    if (kv_splits > 1) {
+      const int64_t n = a.tk * a.kv_heads * a.dim;
+      FMD_REQUIRE(fmd_cdiv(2 * n, 1024) < (1ll << 31));
+      attn_add_kernel<T><<<(unsigned)fmd_cdiv(2 * n, 1024), 256, 0, stream>>>(part, n, kv_splits, gk, gv);
+      FMD_CHECK_LAUNCH();
+    }
   }
   if (gq) {
     AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
@@ -922,15 +972,22 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, float* wor
     }
     const int64_t tiles = tile_count(a.tq, a.group, a.segments, shape_rows(shape));
     FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    const unsigned grid = (unsigned)(tiles * a.kv_heads);
+    const dim3 grid((unsigned)(tiles * a.kv_heads), q_splits);
+    float* part = work;
     if (shape == kWide) {
-      attn_bwd_q_kernel<T, DP, 4, 1, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, gq);
+      attn_bwd_q_kernel<T, DP, 4, 1, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
     } else if (shape == kMid) {
-      if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, gq);
+      if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
     } else {
-      attn_bwd_q_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, gq);
+      attn_bwd_q_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
     }
     FMD_CHECK_LAUNCH();
+    if (q_splits > 1) {
+      const int64_t n = a.tq * a.heads * a.dim;
+      FMD_REQUIRE(fmd_cdiv(n, 1024) < (1ll << 31));
+      attn_add_kernel<T><<<(unsigned)fmd_cdiv(n, 1024), 256, 0, stream>>>(part, n, q_splits, gq, static_cast<T*>(nullptr));
+      FMD_CHECK_LAUNCH();
+    }
   }
   return FMD_OK;
 }
@@ -968,7 +1025,7 @@ int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
 }
 
 template <typename T>
-int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
+int backward(const AttnArgs& a, AttnBwd b, int q_splits, int kv_splits, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
   const int status = check(a, sizeof(T));
   if (status != FMD_OK) return status;
   const int64_t unit = 16 / sizeof(T);
@@ -976,6 +1033,7 @@ int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* work, hip
   FMD_REQUIRE(aligned16(b.g) && aligned16(b.out) && aligned16(b.saved.residual));
   FMD_REQUIRE(b.g_row % unit == 0 && b.g_head % unit == 0);
   FMD_REQUIRE((gk == nullptr) == (gv == nullptr) && aligned16(gq) && aligned16(gk) && aligned16(gv));
+  FMD_REQUIRE(q_splits >= 1 && q_splits <= kMaxSplits && kv_splits >= 1 && kv_splits <= kMaxSplits);
   FMD_REQUIRE(work && aligned16(work));
   b.rows = work;
   if (a.tq == 0) gq = nullptr;
@@ -986,10 +1044,10 @@ int backward(const AttnArgs& a, AttnBwd b, T* gq, T* gk, T* gv, float* work, hip
     FMD_CHECK_LAUNCH();
   }
   work += fmd_cdiv(2 * a.heads * a.tq, 4) * 4;
-  if (a.dim <= 32) return run_bwd<T, 32>(a, b, gq, gk, gv, work, stream);
-  if (a.dim <= 64) return run_bwd<T, 64>(a, b, gq, gk, gv, work, stream);
-  if (a.dim <= 96) return run_bwd<T, 96>(a, b, gq, gk, gv, work, stream);
-  return run_bwd<T, 128>(a, b, gq, gk, gv, work, stream);
+  if (a.dim <= 32) return run_bwd<T, 32>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
+  if (a.dim <= 64) return run_bwd<T, 64>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
+  if (a.dim <= 96) return run_bwd<T, 96>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
+  return run_bwd<T, 128>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
 }
 
 AttnArgs args_of(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,
@@ -1030,9 +1088,17 @@ int64_t fmd_segment_attention_work_size(int32_t bf16, int32_t splits, int64_t tq
   return forward_floats(bf16, splits, tq, tk, segments, heads, kv_heads, dim);
 }
 
+int32_t fmd_segment_attention_bwd_splits(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads,
+                                         int32_t dim, int32_t of_kv) {
+  if (tq <= 0 || tk <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
+  if (few_rows(tq, tk, segments, kv_heads)) return 1;
+  return of_kv ? row_splits(!bf16, dim, tq, tk, segments, heads, kv_heads)
+               : split_count(!bf16, dim, tq, tk, segments, heads, kv_heads);
+}
+
 int64_t fmd_segment_attention_bwd_work_size(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
-                                            int32_t kv_heads, int32_t dim) {
-  return backward_floats(bf16, tq, tk, segments, heads, kv_heads, dim);
+                                            int32_t kv_heads, int32_t dim, int32_t q_splits, int32_t kv_splits) {
+  return backward_floats(bf16, tq, tk, segments, heads, kv_heads, dim, q_splits, kv_splits);
 }
 
 int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* out, float* base, float* inverse,
@@ -1044,13 +1110,13 @@ int fmd_segment_attention(int32_t bf16, FMD_ATTN_PARAMS, int32_t splits, void* o
 }
 
 int fmd_segment_attention_bwd(int32_t bf16, FMD_ATTN_PARAMS, const void* gout, int64_t g_row, int64_t g_head, const void* out,
-                              const float* base, const float* inverse, const void* residual, float* work, void* gq,
-                              void* gk, void* gv, hipStream_t stream) {
+                              const float* base, const float* inverse, const void* residual, int32_t q_splits, int32_t kv_splits,
+                              float* work, void* gq, void* gk, void* gv, hipStream_t stream) {
   const AttnArgs a = FMD_ATTN_ARGS;
   const AttnSaved saved = {const_cast<float*>(base), const_cast<float*>(inverse), const_cast<void*>(residual)};
   const AttnBwd b = {gout, g_row, g_head, out, saved, nullptr};
-  return bf16 ? backward(a, b, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), work, stream)
-              : backward(a, b, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), work, stream);
+  return bf16 ? backward(a, b, q_splits, kv_splits, static_cast<__bf16*>(gq), static_cast<__bf16*>(gk), static_cast<__bf16*>(gv), work, stream)
+              : backward(a, b, q_splits, kv_splits, static_cast<float*>(gq), static_cast<float*>(gk), static_cast<float*>(gv), work, stream);
 }
 
 }  // extern "C"

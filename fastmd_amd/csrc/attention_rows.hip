@@ -10,30 +10,9 @@
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const Raw8<T> r = raw_load(p);
-  const T* e = reinterpret_cast<const T*>(&r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
-}
-
 __device__ __forceinline__ void zero8(float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = 0.f;
-}
-
-template <typename T>
-__device__ __forceinline__ void put8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    store4<T>(p, x[0], x[1], x[2], x[3]);
-    store4<T>(p + 4, x[4], x[5], x[6], x[7]);
-  } else {
-    fmd_bf16x8 v;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (__bf16)x[i];
-    *reinterpret_cast<fmd_bf16x8*>(p) = v;
-  }
 }
 
 __device__ __forceinline__ float dot8(const float (&x)[8], const float (&y)[8]) {
@@ -148,7 +127,7 @@ __global__ void __launch_bounds__(256) attn_rows_fwd_kernel(AttnArgs a, int hb, 
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[g][e] *= inv;
           const int64_t at = ((sg.q0 + i) * a.heads + head + g) * a.dim + r.col;
-          put8<T>(out + at, o[g]);
+          store8<false>(out + at, o[g]);
           saved_residual<T>(saved, at, o[g]);
           if (saved.base && r.col == 0) {
             const int64_t s = (head + g) * a.tq + sg.q0 + i;
@@ -183,7 +162,7 @@ __device__ __forceinline__ float delta_part(const AttnBwd& b, int64_t at, const 
 // GF: the group, for segments of one query: one pass over the keys forms all three gradients. A segment of another
 // number of queries, and GF = 0, takes a pass per query head for gq and one for gk and gv, whose sums run over all of
 // them in order.
-template <typename T, int LG, int GF>
+template <typename T, int LG, int GF, bool NT>
 __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd b, int hb, int head_blocks, T* gq, T* gk, T* gv) {
   constexpr int G = GF ? GF : 1;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -259,14 +238,14 @@ __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd 
         }
       }
       if (r.on && gk) {
-        put8<T>(gk + kat + j * kstep, dk);
-        put8<T>(gv + kat + j * kstep, dv);
+        store8<NT>(gk + kat + j * kstep, dk);
+        store8<NT>(gv + kat + j * kstep, dv);
       }
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       slots_sum(dq[g], r.stride);
-      if (r.on && r.slot == 0 && gq) put8<T>(gq + (sg.q0 * a.heads + r.kvh * a.group + g) * a.dim + r.col, dq[g]);
+      if (r.on && r.slot == 0 && gq) store8<false>(gq + (sg.q0 * a.heads + r.kvh * a.group + g) * a.dim + r.col, dq[g]);
     }
     return;
   }
@@ -291,7 +270,7 @@ __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd 
           for (int e = 0; e < 8; ++e) dq[e] = fmaf(ds, k[e], dq[e]);
         }
         slots_sum(dq, r.stride);
-        if (r.on && r.slot == 0) put8<T>(gq + ((sg.q0 + i) * a.heads + head) * a.dim + r.col, dq);
+        if (r.on && r.slot == 0) store8<false>(gq + ((sg.q0 + i) * a.heads + head) * a.dim + r.col, dq);
       }
   if (!gk) return;
   for (int j0 = 0; j0 < sg.nk; j0 += r.slots) {
@@ -320,8 +299,8 @@ __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd 
         }
       }
     if (live) {
-      put8<T>(gk + kat + j * kstep, dk);
-      put8<T>(gv + kat + j * kstep, dv);
+      store8<NT>(gk + kat + j * kstep, dk);
+      store8<NT>(gv + kat + j * kstep, dv);
     }
   }
 }
@@ -359,17 +338,23 @@ int fwd(const AttnArgs& a, T* out, const AttnSaved& s, hipStream_t stream) {
   return FMD_OK;
 }
 
-template <typename T, int LG>
-int bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream) {
+template <typename T, int LG, bool NT>
+int bwd_by_group(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream) {
   const RowGrid r = row_grid(a, LG);
   FMD_REQUIRE(r.blocks < (1ll << 31));
   const unsigned n = (unsigned)r.blocks;
-  if (a.group == 1) attn_rows_bwd_kernel<T, LG, 1><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
-  else if (a.group == 2) attn_rows_bwd_kernel<T, LG, 2><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
-  else if (a.group == 4) attn_rows_bwd_kernel<T, LG, 4><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
-  else attn_rows_bwd_kernel<T, LG, 0><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
+  if (a.group == 1) attn_rows_bwd_kernel<T, LG, 1, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
+  else if (a.group == 2) attn_rows_bwd_kernel<T, LG, 2, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
+  else if (a.group == 4) attn_rows_bwd_kernel<T, LG, 4, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
+  else attn_rows_bwd_kernel<T, LG, 0, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
   FMD_CHECK_LAUNCH();
   return FMD_OK;
+}
+
+template <typename T, int LG>
+int bwd(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream) {
+  const bool nt = a.tk * a.kv_heads * a.dim * 2 * (int64_t)sizeof(T) >= kStreamBytes;
+  return nt ? bwd_by_group<T, LG, true>(a, b, gq, gk, gv, stream) : bwd_by_group<T, LG, false>(a, b, gq, gk, gv, stream);
 }
 
 }  // namespace

@@ -3,13 +3,13 @@
 //   r = (mean x^2 + eps)^(-1/2),  y = x r w,  (a, b) -> (a cos - b sin, b cos + a sin) on the first `rot` columns
 //
 // A row (one head of one token) belongs to a group of LG lanes, eight columns each: one read, one write, the mean by
-// lane exchanges. A group takes kHeads heads of its token at a time, so their loads are in flight together and the
+// lane exchanges. A group takes a few heads of its token at a time, so their loads are in flight together and the
 // token's cosines, sines and weights are read once. All arithmetic is fp32, each output rounded once.
 #include "attention.h"
 
 namespace {
 
-constexpr int kHeads = 4;
+constexpr int kFwdHeads = 4, kBwdHeads = 2;  // heads of a unit: more loads in flight against more registers
 
 struct NormArgs {
   const void *q, *k;  // [tokens, heads, dim]; k may be null
@@ -24,33 +24,20 @@ struct NormArgs {
   int32_t pos64;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const Raw8<T> r = raw_load(p);
-  const T* e = reinterpret_cast<const T*>(&r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  store4<T>(p, x[0], x[1], x[2], x[3]);
-  store4<T>(p + 4, x[4], x[5], x[6], x[7]);
-}
-template <>
-__device__ __forceinline__ void store8<__bf16>(__bf16* p, const float (&x)[8]) {
-  fmd_bf16x8 v;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = (__bf16)x[i];
-  *reinterpret_cast<fmd_bf16x8*>(p) = v;
-}
-
 template <int LG>
 __device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int off = LG / 2; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
+  x = lanes_sum<(LG < 16 ? LG : 16)>(x);
+  if (LG == 32) {
+    float y = x;
+    swap_halves16(x, y);
+    x += y;
+  }
   return x;
 }
+
+// How the other column of a pair is reached: neighbours of a lane; the same place of another lane of the group (rot / 2 a
+// multiple of eight); anywhere.
+enum Turn { kNone, kNeighbours, kLanes, kAnywhere };
 
 __device__ __forceinline__ int64_t table_row(const NormArgs& a, int64_t tok) {
   const int64_t p = !a.positions ? tok
@@ -60,46 +47,49 @@ __device__ __forceinline__ int64_t table_row(const NormArgs& a, int64_t tok) {
 }
 
 // cosine and sine of each of the lane's columns (1 and 0 past `rot`; NaN for a position outside the table)
+template <Turn TURN>
 __device__ __forceinline__ void angles(const NormArgs& a, int64_t tok, int col0, float (&c)[8], float (&s)[8]) {
+  if constexpr (TURN == kNone) return;
   const int64_t p = table_row(a, tok);
   const int half = a.rot >> 1;
-  if (a.interleaved && col0 + 8 <= a.rot && p >= 0 && ((a.table_ld | (int64_t)(col0 >> 1)) & 3) == 0) {
-    const float4 x = *reinterpret_cast<const float4*>(a.cs + p * a.table_ld + (col0 >> 1));
-    const float4 y = *reinterpret_cast<const float4*>(a.sn + p * a.table_ld + (col0 >> 1));
+  const float *cs = a.cs + p * a.table_ld, *sn = a.sn + p * a.table_ld;
+  if (TURN == kNeighbours && col0 + 8 <= a.rot && p >= 0 && (a.table_ld & 3) == 0) {  // four angles in a row
+    const float4 x = *reinterpret_cast<const float4*>(cs + (col0 >> 1));
+    const float4 y = *reinterpret_cast<const float4*>(sn + (col0 >> 1));
     c[0] = c[1] = x.x, c[2] = c[3] = x.y, c[4] = c[5] = x.z, c[6] = c[7] = x.w;
     s[0] = s[1] = y.x, s[2] = s[3] = y.y, s[4] = s[5] = y.z, s[6] = s[7] = y.w;
     return;
   }
-  const int i0 = col0 < half ? col0 : col0 - half;
-  if (!a.interleaved && p >= 0 && ((a.table_ld | half) & 7) == 0 && col0 + 8 <= a.rot) {  // eight angles in a row
-    load8<float>(a.cs + p * a.table_ld + i0, c);
-    load8<float>(a.sn + p * a.table_ld + i0, s);
+  if (TURN == kLanes && p >= 0 && (a.table_ld & 3) == 0) {  // eight
+    if (col0 >= a.rot) return;
+    load8<float>(cs + (col0 < half ? col0 : col0 - half), c);
+    load8<float>(sn + (col0 < half ? col0 : col0 - half), s);
     return;
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const int col = col0 + e, i = a.interleaved ? col >> 1 : col < half ? col : col - half;
-    const bool turns = col < a.rot;
-    c[e] = !turns ? 1.f : p >= 0 ? a.cs[p * a.table_ld + i] : NAN;
-    s[e] = !turns ? 0.f : p >= 0 ? a.sn[p * a.table_ld + i] : NAN;
+    const int col = col0 + e, i = TURN == kNeighbours ? col >> 1 : col < half ? col : col - half;
+    if (col < a.rot) {
+      c[e] = p >= 0 ? cs[i] : NAN;
+      s[e] = p >= 0 ? sn[i] : NAN;
+    }
   }
 }
 
-// y -> rotated y (sign 1) or the transposed rotation (sign -1). The other column of a pair lies in the same lane
-// (interleaved), in the same place of another lane of the group (rot / 2 a multiple of eight), or anywhere.
-template <int LG>
+// y -> rotated y (sign 1) or the transposed rotation (sign -1)
+template <int LG, Turn TURN>
 __device__ __forceinline__ void rotate(const NormArgs& a, int col0, const float (&c)[8], const float (&s)[8], float sign,
                                        float (&y)[8]) {
+  if constexpr (TURN == kNone) return;
   const int half = a.rot >> 1;
   float o[8];
-  if (a.rot == 0) return;
-  if (a.interleaved) {
+  if constexpr (TURN == kNeighbours) {
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       o[e] = y[e] * c[e] - sign * s[e] * y[e + 1];
       o[e + 1] = y[e + 1] * c[e + 1] + sign * s[e + 1] * y[e];
     }
-  } else if (half % 8 == 0) {
+  } else if constexpr (TURN == kLanes) {
     const int lane = threadIdx.x & 63, sub = lane & (LG - 1), by = half >> 3;
     const bool low = col0 < half;
     const int from = (lane - sub) + (col0 < a.rot ? (low ? sub + by : sub - by) : sub);
@@ -125,28 +115,28 @@ __device__ __forceinline__ void rotate(const NormArgs& a, int col0, const float 
   for (int e = 0; e < 8; ++e) y[e] = o[e];
 }
 
-// the units of work of the whole call: (token, block of kHeads heads), queries and keys in blocks of their own
-__device__ __forceinline__ int head_blocks(const NormArgs& a) {
-  return (a.heads + kHeads - 1) / kHeads + (a.kv_heads + kHeads - 1) / kHeads;
+// the units of work of the whole call: (token, block of `by` heads), queries and keys in blocks of their own
+__device__ __forceinline__ int head_blocks(const NormArgs& a, int by) {
+  return (a.heads + by - 1) / by + (a.kv_heads + by - 1) / by;
 }
 
-template <typename T, int LG>
+template <typename T, int LG, Turn TURN, bool NT>
 __global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k_out) {
   const int sub = threadIdx.x & (LG - 1), col0 = 8 * sub;
   const int64_t unit = (int64_t)blockIdx.x * (256 / LG) + threadIdx.x / LG;
-  const int blocks = head_blocks(a), qb = (a.heads + kHeads - 1) / kHeads;
+  const int blocks = head_blocks(a, kFwdHeads), qb = (a.heads + kFwdHeads - 1) / kFwdHeads;
   int64_t tok = unit / blocks;
   const int hb = (int)(unit % blocks);
   const bool in = tok < a.tokens, is_k = hb >= qb;
   if (!in) tok = 0;
-  const int h0 = (is_k ? hb - qb : hb) * kHeads, heads = is_k ? a.kv_heads : a.heads;
+  const int h0 = (is_k ? hb - qb : hb) * kFwdHeads, heads = is_k ? a.kv_heads : a.heads;
   const T* x = static_cast<const T*>(is_k ? a.k : a.q) + tok * (is_k ? a.k_row : a.q_row);
   const int64_t hs = is_k ? a.k_head : a.q_head;
   T* out = (is_k ? k_out : q_out) + tok * heads * a.dim;
   const bool cols = col0 < a.dim;
-  float y[kHeads][8];
+  float y[kFwdHeads][8];
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
+  for (int h = 0; h < kFwdHeads; ++h) {
     if (in && cols && h0 + h < heads) load8<T>(x + (h0 + h) * hs + col0, y[h]);
     else
 #pragma unroll
@@ -157,9 +147,9 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k
   for (int e = 0; e < 8; ++e) w[e] = 1.f, c[e] = 1.f, s[e] = 0.f;
   const T* wp = static_cast<const T*>(is_k ? a.wk : a.wq);
   if (cols && wp) load8<T>(wp + col0, w);
-  if (in && cols) angles(a, tok, col0, c, s);
+  if (in && cols) angles<TURN>(a, tok, col0, c, s);
 #pragma unroll
-  for (int h = 0; h < kHeads; ++h) {
+  for (int h = 0; h < kFwdHeads; ++h) {
     if (a.norm) {
       float ss = 0.f;
 #pragma unroll
@@ -168,8 +158,8 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[h][e] = y[h][e] * r * w[e];
     }
-    rotate<LG>(a, col0, c, s, 1.f, y[h]);
-    if (in && cols && h0 + h < heads) store8<T>(out + (h0 + h) * a.dim + col0, y[h]);
+    rotate<LG, TURN>(a, col0, c, s, 1.f, y[h]);
+    if (in && cols && h0 + h < heads) store8<NT>(out + (h0 + h) * a.dim + col0, y[h]);
   }
 }
 
@@ -180,12 +170,12 @@ struct NormGrad {
 
 // A workgroup takes `per` consecutive units per group; its weight gradients are summed over them in registers, over its
 // groups in LDS in order, and written as one row per workgroup, which norm_weights_kernel adds in order.
-template <typename T, int LG>
+template <typename T, int LG, Turn TURN, bool NT>
 __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g, int per, T* gq_out, T* gk_out, float* part) {
   constexpr int GROUPS = 256 / LG;
   __shared__ float sum[2][256][8];
   const int sub = threadIdx.x & (LG - 1), col0 = 8 * sub, group = threadIdx.x / LG;
-  const int blocks = head_blocks(a), qb = (a.heads + kHeads - 1) / kHeads;
+  const int blocks = head_blocks(a, kBwdHeads), qb = (a.heads + kBwdHeads - 1) / kBwdHeads;
   const int64_t units = a.tokens * blocks;
   const bool cols = col0 < a.dim;
   float gw[2][8];
@@ -197,14 +187,14 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
     const int64_t tok = in ? unit / blocks : 0;
     const int hb = in ? (int)(unit % blocks) : 0;
     const bool is_k = hb >= qb;
-    const int h0 = (is_k ? hb - qb : hb) * kHeads, heads = is_k ? a.kv_heads : a.heads;
+    const int h0 = (is_k ? hb - qb : hb) * kBwdHeads, heads = is_k ? a.kv_heads : a.heads;
     const T* xp = static_cast<const T*>(is_k ? a.k : a.q) + tok * (is_k ? a.k_row : a.q_row) + col0;
     const T* gp = static_cast<const T*>(is_k ? g.gk : g.gq) + tok * (is_k ? g.gk_row : g.gq_row) + col0;
     const int64_t xh = is_k ? a.k_head : a.q_head, gh = is_k ? g.gk_head : g.gq_head;
     T* out = (is_k ? gk_out : gq_out) + tok * heads * a.dim + col0;
-    float x[kHeads][8], y[kHeads][8];
+    float x[kBwdHeads][8], y[kBwdHeads][8];
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
+    for (int h = 0; h < kBwdHeads; ++h) {
       if (in && cols && h0 + h < heads) {
         load8<T>(gp + (h0 + h) * gh, y[h]);
         if (a.norm) load8<T>(xp + (h0 + h) * xh, x[h]);
@@ -218,10 +208,10 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
     for (int e = 0; e < 8; ++e) w[e] = 1.f, c[e] = 1.f, s[e] = 0.f;
     const T* wp = static_cast<const T*>(is_k ? a.wk : a.wq);
     if (cols && wp) load8<T>(wp + col0, w);
-    if (in && cols) angles(a, tok, col0, c, s);
+    if (in && cols) angles<TURN>(a, tok, col0, c, s);
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-      rotate<LG>(a, col0, c, s, -1.f, y[h]);
+    for (int h = 0; h < kBwdHeads; ++h) {
+      rotate<LG, TURN>(a, col0, c, s, -1.f, y[h]);
       if (a.norm) {
         float ss = 0.f, dot = 0.f;
 #pragma unroll
@@ -241,7 +231,7 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[h][e] = r * (gn[e] - x[h][e] * mean);
       }
-      if (in && cols && h0 + h < heads) store8<T>(out + (h0 + h) * a.dim, y[h]);
+      if (in && cols && h0 + h < heads) store8<NT>(out + (h0 + h) * a.dim, y[h]);
     }
   }
   if (!part) return;
@@ -284,8 +274,8 @@ int groups_of(int dim) {
   return lg;
 }
 
-int64_t unit_count(int64_t tokens, int heads, int kv_heads) {
-  return tokens * ((heads + kHeads - 1) / kHeads + (kv_heads + kHeads - 1) / kHeads);
+int64_t unit_count(int64_t tokens, int heads, int kv_heads, int by) {
+  return tokens * ((heads + by - 1) / by + (kv_heads + by - 1) / by);
 }
 
 // workgroups of the VJP: at most 1 024 (four per CU), so that the partial sums stay few
@@ -308,26 +298,58 @@ int check_norm(const NormArgs& a) {
   const int64_t unit = 16 / sizeof(T);
   FMD_REQUIRE(ok16(a.q) && ok16(a.k) && ok16(a.wq) && ok16(a.wk));
   FMD_REQUIRE(a.q_row % unit == 0 && a.q_head % unit == 0 && a.k_row % unit == 0 && a.k_head % unit == 0);
-  FMD_REQUIRE(unit_count(a.tokens, a.heads, a.kv_heads) < (1ll << 31));
+  FMD_REQUIRE(unit_count(a.tokens, a.heads, a.kv_heads, 1) < (1ll << 31));
   return FMD_OK;
 }
 
-template <typename T, int LG>
-int norm_fwd(const NormArgs& a, T* q_out, T* k_out, hipStream_t stream) {
-  const int64_t units = unit_count(a.tokens, a.heads, a.kv_heads);
-  qk_norm_kernel<T, LG><<<(unsigned)fmd_cdiv(units, 256 / LG), 256, 0, stream>>>(a, q_out, k_out);
+Turn turn_of(const NormArgs& a) {
+  return a.rot == 0 ? kNone : a.interleaved ? kNeighbours : a.rot % 16 == 0 ? kLanes : kAnywhere;
+}
+
+template <typename T>
+bool streams(const NormArgs& a) {
+  return a.tokens * (a.heads + a.kv_heads) * a.dim * (int64_t)sizeof(T) >= kStreamBytes;
+}
+
+template <typename T, int LG, Turn TURN>
+int norm_fwd_turn(const NormArgs& a, T* q_out, T* k_out, hipStream_t stream) {
+  const unsigned grid = (unsigned)fmd_cdiv(unit_count(a.tokens, a.heads, a.kv_heads, kFwdHeads), 256 / LG);
+  if (streams<T>(a)) qk_norm_kernel<T, LG, TURN, true><<<grid, 256, 0, stream>>>(a, q_out, k_out);
+  else qk_norm_kernel<T, LG, TURN, false><<<grid, 256, 0, stream>>>(a, q_out, k_out);
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
 
 template <typename T, int LG>
+int norm_fwd(const NormArgs& a, T* q_out, T* k_out, hipStream_t stream) {
+  switch (turn_of(a)) {
+    case kNone: return norm_fwd_turn<T, LG, kNone>(a, q_out, k_out, stream);
+    case kNeighbours: return norm_fwd_turn<T, LG, kNeighbours>(a, q_out, k_out, stream);
+    case kLanes: return norm_fwd_turn<T, LG, kLanes>(a, q_out, k_out, stream);
+    default: return norm_fwd_turn<T, LG, kAnywhere>(a, q_out, k_out, stream);
+  }
+}
+
+template <typename T, int LG, Turn TURN>
+void norm_bwd_turn(const NormArgs& a, const NormGrad& g, int grid, int per, T* gq, T* gk, float* work, hipStream_t stream) {
+  if (streams<T>(a)) qk_norm_bwd_kernel<T, LG, TURN, true><<<grid, 256, 0, stream>>>(a, g, per, gq, gk, work);
+  else qk_norm_bwd_kernel<T, LG, TURN, false><<<grid, 256, 0, stream>>>(a, g, per, gq, gk, work);
+}
+
+template <typename T, int LG>
 int norm_bwd(const NormArgs& a, const NormGrad& g, T* gq, T* gk, T* gwq, T* gwk, float* work, hipStream_t stream) {
-  const int64_t units = unit_count(a.tokens, a.heads, a.kv_heads);
+  const int64_t units = unit_count(a.tokens, a.heads, a.kv_heads, kBwdHeads);
   const bool weights = gwq || gwk;
   int grid = 0, per = 0;
   bwd_grid(units, 256 / LG, &grid, &per);
   if (grid > 0) {
-    qk_norm_bwd_kernel<T, LG><<<grid, 256, 0, stream>>>(a, g, per, gq, gk, weights ? work : nullptr);
+    float* part = weights ? work : nullptr;
+    switch (turn_of(a)) {
+      case kNone: norm_bwd_turn<T, LG, kNone>(a, g, grid, per, gq, gk, part, stream); break;
+      case kNeighbours: norm_bwd_turn<T, LG, kNeighbours>(a, g, grid, per, gq, gk, part, stream); break;
+      case kLanes: norm_bwd_turn<T, LG, kLanes>(a, g, grid, per, gq, gk, part, stream); break;
+      default: norm_bwd_turn<T, LG, kAnywhere>(a, g, grid, per, gq, gk, part, stream);
+    }
     FMD_CHECK_LAUNCH();
   }
   if (weights) {
@@ -392,7 +414,7 @@ int fmd_qk_norm_rotary(int32_t bf16, FMD_NORM_PARAMS, void* q_out, void* k_out, 
 int64_t fmd_qk_norm_rotary_work_size(int64_t tokens, int32_t heads, int32_t kv_heads, int32_t dim) {
   if (tokens <= 0 || heads < 0 || kv_heads < 0 || dim <= 0 || dim > 256) return 0;
   int grid = 0, per = 0;
-  bwd_grid(unit_count(tokens, heads, kv_heads), 256 / groups_of(dim), &grid, &per);
+  bwd_grid(unit_count(tokens, heads, kv_heads, kBwdHeads), 256 / groups_of(dim), &grid, &per);
   return (int64_t)grid * 2 * dim;
 }
 

@@ -137,6 +137,14 @@ def _plan(bf16: int, tq: int, tk: int, segments: int, heads: int, kv_heads: int,
     return splits, lib.fmd_segment_attention_work_size(bf16, splits, tq, tk, segments, heads, kv_heads, dim)
 
 
+@functools.lru_cache(maxsize=256)
+def _plan_vjp(*sizes: int) -> tuple[int, int, int]:
+    """(key splits of gq, query splits of gk and gv, floats of workspace) of the VJP at these sizes (as of ``_plan``)."""
+    lib = _abi.load()
+    q_splits, kv_splits = (lib.fmd_segment_attention_bwd_splits(*sizes, of_kv) for of_kv in (0, 1))
+    return q_splits, kv_splits, lib.fmd_segment_attention_bwd_work_size(*sizes, q_splits, kv_splits)
+
+
 def _forward(q, k, v, q_offsets, k_offsets, causal, scale, save):
     args, keep = _prepare(q, k, v, q_offsets, k_offsets, causal, scale)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -183,10 +191,10 @@ def segment_attention_vjp(gout: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Te
     gq = torch.empty_like(q, memory_format=torch.contiguous_format) if need_q else None
     gk = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
     gv = torch.empty_like(k, memory_format=torch.contiguous_format) if need_kv else None
-    size = _abi.load().fmd_segment_attention_bwd_work_size(args[0], *args[12:18])
+    q_splits, kv_splits, size = _plan_vjp(args[0], *args[12:18])
     work = torch.empty(max(4, size), dtype=torch.float32, device=q.device)
     _abi.call("fmd_segment_attention_bwd", *args, gout.data_ptr(), g_row, g_head, out.data_ptr(), base.data_ptr(),
-              inverse.data_ptr(), _abi.ptr(residual), work.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
+              inverse.data_ptr(), _abi.ptr(residual), q_splits, kv_splits, work.data_ptr(), _abi.ptr(gq), _abi.ptr(gk), _abi.ptr(gv), stream())
     del keep
     return gq, gk, gv
 

@@ -840,16 +840,20 @@ int fmd_segment_attention(int32_t bf16, const void* q, int64_t q_row, int64_t q_
 
 /* VJP of fmd_segment_attention: gq [tq, heads, dim], gk and gv [tk, kv_heads, dim] (contiguous; gq, or gk and gv
  * together, nullable) from the gradient `gout` of `out`, the forward's `out`, `base`,
- * `inverse` and (bf16) `residual`. Rows outside every segment get
- * zero. work: fmd_segment_attention_bwd_work_size() floats on a 16-byte address. No atomics: the same inputs give the same bits. */
+ * `inverse` and (bf16) `residual`. Rows outside every segment get zero. q_splits, kv_splits:
+ * fmd_segment_attention_bwd_splits() of the keys for gq (of_kv 0) and of the queries for gk and gv (1).
+ * work: fmd_segment_attention_bwd_work_size() floats on a 16-byte address. No atomics: the same inputs give the same bits. */
+int32_t fmd_segment_attention_bwd_splits(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads,
+                                         int32_t dim, int32_t of_kv);
 int64_t fmd_segment_attention_bwd_work_size(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
-                                            int32_t kv_heads, int32_t dim);
+                                            int32_t kv_heads, int32_t dim, int32_t q_splits, int32_t kv_splits);
 int fmd_segment_attention_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                               int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const int64_t* q_offsets,
                               const int64_t* k_offsets, int64_t tq, int64_t tk, int32_t segments, int32_t heads,
                               int32_t kv_heads, int32_t dim, int32_t causal, float scale, const void* gout, int64_t g_row,
                               int64_t g_head, const void* out, const float* base, const float* inverse, const void* residual,
-                              float* work, void* gq, void* gk, void* gv, hipStream_t stream);
+                              int32_t q_splits, int32_t kv_splits, float* work, void* gq, void* gk, void* gv,
+                              hipStream_t stream);
 
 /* Each head x of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (row and head strides in elements, 16-byte aligned
  * rows, dim a multiple of 8 up to 256): with norm, x (mean x^2 + eps)^(-1/2) weight (weights [dim] of the features' type,
