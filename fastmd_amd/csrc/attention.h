@@ -243,6 +243,50 @@ struct AttnTile {
   }
 };
 
+// An infinity or a NaN in a row of a tile must not reach a lane that does not see the row, and a weight of zero would not
+// keep it out of a matrix product. Tiles that some lane does not see all of (causal calls) are looked through for such rows;
+// where there are any, the products take the finite values alone, and the rows' weights are NaN for the lanes that see them.
+
+// bits of the rows (of 32) of a tile that hold a value that is not finite, for the whole wave (of the first plane: what rounds
+// to an infinity counts as one)
+template <typename Tile>
+__device__ __forceinline__ uint32_t rows_not_finite(const __bf16* s) {
+  const int lane = threadIdx.x & 63;
+  uint32_t over = 0;
+  for (int i = lane >> 5; i < Tile::CHUNKS; i += 2) {
+    const uint4 v = *reinterpret_cast<const uint4*>(s + Tile::at(lane & 31, i));
+    over |= ((v.x & 0x7f807f80u) + 0x00800080u) | ((v.y & 0x7f807f80u) + 0x00800080u) |
+            ((v.z & 0x7f807f80u) + 0x00800080u) | ((v.w & 0x7f807f80u) + 0x00800080u);
+  }
+  const uint64_t b = __ballot((over & 0x80008000u) != 0);
+  return (uint32_t)b | (uint32_t)(b >> 32);
+}
+
+// whether a product of the wave holds a value that is not finite: as it does wherever one of its operands' rows does
+__device__ __forceinline__ bool not_finite(const fmd_f32x16& x, const fmd_f32x16& y) {
+  float t = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) t = fmaf(y[v], 0.f, fmaf(x[v], 0.f, t));
+  return __any(t != t);
+}
+
+// an operand with zeros in the place of values that are not finite
+template <int NP>
+__device__ __forceinline__ Planes<NP> finite_part(Planes<NP> x) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    uint4 v = __builtin_bit_cast(uint4, x.p[p]);
+    auto clean = [](uint32_t w) {
+      if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+      if ((w & 0x7f800000u) == 0x7f800000u) w &= 0xffffu;
+      return w;
+    };
+    v = make_uint4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+    x.p[p] = __builtin_bit_cast(fmd_bf16x8, v);
+  }
+  return x;
+}
+
 // Rows of a tile on their way to LDS: THREADS threads load NV chunks each (issued together, written after the
 // previous tile has been read). Chunks past the rows or past dim are zero: nothing of another segment is read.
 template <typename T, int NP, int ROWS, int DP, int THREADS>

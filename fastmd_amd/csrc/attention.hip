@@ -17,7 +17,7 @@ static constexpr int attn_waves(int planes, int dp, int sums) { return planes * 
 // sums over keys stay in the lane but for one exchange of the halves, and exp(S^T) is already the operand of
 // O^T = V^T P^T. Statistics and sums are fp32; P is rounded to bf16 for bf16 inputs (the output is, too) and kept as
 // three planes for fp32.
-template <typename T, int DP, int BN, int WM, int KW, bool DMA>
+template <typename T, int DP, int BN, int WM, int KW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_fwd_kernel(AttnArgs a, AttnTiles kv,
                                                                 int64_t tiles, int splits, T* out, AttnSaved saved,
                                                                 float* part_o, float* part_m, float* part_l) {
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int wm = wave % WM, kw = wave / WM;
   const int kvh = blockIdx.x % a.kv_heads;
   int64_t t = blockIdx.x / a.kv_heads;
-  if (a.causal) t = tiles - 1 - t;  // the rows with the most keys first
+  if (CAUSAL) t = tiles - 1 - t;  // the rows with the most keys first
   int64_t first;
   const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first);
   AttnSegment sg = attn_segment(a, ext);
@@ -50,10 +50,10 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
 
   // keys that this row sees, and that any row of the workgroup sees
   const int shift = sg.nk - sg.nq;
-  const int sees = a.causal ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
+  const int sees = CAUSAL ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
   const int last_row = min(row0 + 32 * WM, rows) - 1;
-  const int reach = a.causal ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
-  const int least = a.causal ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
+  const int reach = CAUSAL ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
+  const int least = CAUSAL ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
   const int all_tiles = (reach + BN - 1) / BN;
   const int per = (all_tiles + splits - 1) / splits;
   const int tile_lo = min(all_tiles, (int)blockIdx.y * per), tile_hi = min(all_tiles, tile_lo + per);
@@ -80,8 +80,11 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   constexpr float kSlack = 8.f;
   const float slack = kSlack / c;
 
-  const int lr = Tile::lane_rows(), lc = Tile::lane_cols();
-  auto step = [&](const __bf16* ks_, int tile) {
+  const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
+  auto step = [&](auto last, const __bf16* ks_, int tile) {
+    constexpr bool kLast = decltype(last)::value;  // a row may not see all of the tile
+    int lr = lane_r, lc = lane_c;
+    asm volatile("" : "+v"(lr), "+v"(lc));  // addresses formed here, not kept in registers
     const __bf16* vs_ = ks_ + Tile::SIZE;
     const int j0 = tile * BN;
     fmd_f32x16 s[JB];
@@ -91,7 +94,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) s[j] = mma(Tile::rows(ks_, lr, 32 * j, ks), qf[ks], s[j]);
     }
-    if (j0 + BN > least) {  // some row does not see all of the tile
+    if (kLast && j0 + BN > least) {  // some row does not see all of the tile
       const int left = sees - j0 - 4 * half;
 #pragma unroll
       for (int j = 0; j < JB; ++j)
@@ -126,6 +129,18 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         sum[v & 1] += p;
       }
     l += sum[0] + sum[1];  // of this lane's half of the keys
+    uint32_t bad = 0;
+    if (kLast && CAUSAL && j0 + BN > least) {
+      const int left = sees - j0 - 4 * half;
+#pragma unroll
+      for (int j = 0; j < JB; ++j) {
+        const uint32_t rows = rows_not_finite<Tile>(vs_ + 32 * j * Tile::LD), mine = rows >> 4 * half;
+        bad |= rows;
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (32 * j + prod_row(v, 0) < left && mine >> prod_row(v, 0) & 1) s[j][v] = NAN;
+      }
+    }
 #pragma unroll
     for (int j = 0; j < JB; ++j)
 #pragma unroll
@@ -136,7 +151,11 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         Planes<NP> pf;
         planes_of(x, pf);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(vs_, lc, 32 * j + 16 * step, d), pf, o[d]);
+        for (int d = 0; d < DB; ++d) {
+          Planes<NP> vc = Tile::cols(vs_, lc, 32 * j + 16 * step, d);
+          if (kLast && CAUSAL && bad) vc = finite_part<NP>(vc);
+          o[d] = mma(vc, pf, o[d]);
+        }
       }
   };
 
@@ -158,17 +177,23 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       vp += v_by;
     };
     __bf16 *st0 = lds + kw * 2 * Tile::SIZE, *st1 = lds2 + kw * 2 * Tile::SIZE;
-    auto round = [&](int it, const __bf16* here, __bf16* next) {
+    auto round = [&](auto last, int it, const __bf16* here, __bf16* next) {
       const int tile = tile_lo + it * KW + kw;
       __builtin_amdgcn_s_waitcnt(kWaitVm0);  // this wave's part of the tile has landed
       __syncthreads();                       // everyone's has, and the other buffer is read
       if (it + 1 < rounds) issue(tile + KW, next);
-      if (tile < tile_hi) step(here, tile);
+      if (tile < tile_hi) step(last, here, tile);
     };
     if (rounds > 0) issue(tile_lo + kw, st0);
-    for (int it = 0; it < rounds; it += 2) {
-      round(it, st0, st1);
-      if (it + 1 < rounds) round(it + 1, st1, st0);
+    int it = 0;
+    if constexpr (CAUSAL)  // rounds whose tiles every row sees all of: the masks' part is left out of their code
+      for (const int full = (least / BN - tile_lo) / KW; it + 2 <= full && it + 2 <= rounds; it += 2) {
+        round(std::false_type(), it, st0, st1);
+        round(std::false_type(), it + 1, st1, st0);
+      }
+    for (; it < rounds; it += 2) {
+      round(std::true_type(), it, st0, st1);
+      if (it + 1 < rounds) round(std::true_type(), it + 1, st1, st0);
     }
   } else {
     __bf16* st = lds + kw * 2 * Tile::SIZE;
@@ -188,7 +213,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       vl.store(st + Tile::SIZE, lt);
       __syncthreads();
       if (it + 1 < rounds) issue(tile + KW);
-      if (tile < tile_hi) step(st, tile);
+      if (tile < tile_hi) step(std::true_type(), st, tile);
     }
   }
   l = add_halves(l);
@@ -339,7 +364,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // Gradients of keys and values. One workgroup: 32 WM keys of one key head; wave (wm, rw) holds 32 keys and walks the
 // tiles rw, rw + RW, ... of 32 queries, of one query head of the group after the other. S = Q K^T (lane: a key, registers: query rows), so exp(S - lse) and
 // dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of the group.
-template <typename T, int DP, int WM, int RW, bool DMA>
+template <typename T, int DP, int WM, int RW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
                                                                                               int splits, float* part, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
@@ -350,8 +375,9 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   constexpr int kMerge = (RW - 1) * WM * MB * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[RW * kGroup > kMerge ? RW * kGroup : kMerge];
   __shared__ __attribute__((aligned(16))) __bf16 lds2[DMA ? RW * kGroup : 8];
-  // the values of the workgroup's keys stay in LDS where they and the keys do not both fit into registers
-  constexpr bool kLdsV = NP == 1 && DP > 96 && RW > 1;
+  // the values of the workgroup's keys stay in LDS where they and the keys do not both fit into registers (beside the masks of a
+  // causal call, from 96 columns on)
+  constexpr bool kLdsV = NP == 1 && DP > (CAUSAL ? 64 : 96) && RW > 1;
   using VTile = AttnTile<NP, 32 * WM, DP>;
   __shared__ __attribute__((aligned(16))) __bf16 lds_v[kLdsV ? VTile::SIZE : 8];
 
@@ -369,9 +395,9 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   const int64_t kt = sg.k0 + (live ? key : 0);
   const int shift = sg.nk - sg.nq;
   // the first query that sees this key and the first that sees all keys of the workgroup; the tiles of a head that see any
-  const int from = a.causal ? max(0, key - shift) : 0;
-  const int full = a.causal ? max(0, key0 + 32 * WM - 1 - shift) : 0;
-  const int tile_lo = a.causal ? min(sg.nq, max(0, key0 - shift)) / BR : 0;
+  const int from = CAUSAL ? max(0, key - shift) : 0;
+  const int full = CAUSAL ? max(0, key0 + 32 * WM - 1 - shift) : 0;
+  const int tile_lo = CAUSAL ? min(sg.nq, max(0, key0 - shift)) / BR : 0;
   const int head_tiles = (sg.nq + BR - 1) / BR - tile_lo;
   // this split's part of the tiles of all heads
   const int per = (head_tiles * a.group + splits - 1) / splits, first_tile = blockIdx.y * per;
@@ -428,7 +454,8 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     wrap();
   };
   const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
-  auto step = [&](const __bf16* qs, int r0) {
+  auto step = [&](auto partial, const __bf16* qs, int r0) {
+    constexpr bool kPartial = decltype(partial)::value;  // some key of the workgroup may not be seen by some row
     int lr = lane_r, lc = lane_c;
     if constexpr (kLdsV) asm volatile("" : "+v"(lr), "+v"(lc));  // addresses formed here, not kept in registers
     const __bf16* gs = qs + Tile::SIZE;
@@ -439,6 +466,8 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
       dp = mma(Tile::rows(gs, lr, 0, ks), kLdsV ? VTile::rows(lds_v, lr, 32 * wm, ks) : vf[kLdsV ? 0 : ks], dp);
+    uint32_t bad = 0;
+    if (kPartial && r0 < full && not_finite(s, dp)) bad = rows_not_finite<Tile>(qs) | rows_not_finite<Tile>(gs);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const float4 ls = *reinterpret_cast<const float4*>(stat + 8 * r + 4 * half);
@@ -454,11 +483,14 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
         dp[v] = p * (dp[v] - de[e]);
       }
     }
-    if (r0 < full) {  // some key of the workgroup is not seen by some row of the tile
+    if (kPartial && r0 < full) {
       const int hidden = from - r0 - 4 * half;
+      const uint32_t mine = bad >> 4 * half;
 #pragma unroll
-      for (int v = 0; v < 16; ++v)
+      for (int v = 0; v < 16; ++v) {
+        if (mine >> prod_row(v, 0) & 1) s[v] = dp[v] = NAN;
         if (prod_row(v, 0) < hidden) s[v] = dp[v] = 0.f;
+      }
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
@@ -471,10 +503,14 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
       Planes<NP> pf, df;
       planes_of(x, pf);
       planes_of(y, df);
-  #pragma unroll
+#pragma unroll
       for (int d = 0; d < DB; ++d) {
-        av[d] = mma(Tile::cols(gs, lc, 16 * step, d), pf, av[d]);
-        ak[d] = mma(Tile::cols(qs, lc, 16 * step, d), df, ak[d]);
+        Planes<NP> gc = Tile::cols(gs, lc, 16 * step, d);
+        if (kPartial && bad) gc = finite_part<NP>(gc);
+        av[d] = mma(gc, pf, av[d]);
+        Planes<NP> qc = Tile::cols(qs, lc, 16 * step, d);
+        if (kPartial && bad) qc = finite_part<NP>(qc);
+        ak[d] = mma(qc, df, ak[d]);
       }
     }
   };
@@ -503,18 +539,36 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
         Dma::copy4(p, to + 2 * Tile::SIZE + (wm == 1 ? 4 * BR : 0));
       }
     };
-    auto round = [&](int it, const __bf16* here, __bf16* next) {
+    auto round = [&](auto partial, int it, const __bf16* here, __bf16* next) {
       const int tile = next_tile, r0 = next_row;
       __builtin_amdgcn_s_waitcnt(kWaitVm0);
       __syncthreads();
       advance();
       if (it + 1 < rounds) issue(next);
-      if (tile < all_tiles) step(here, r0);
+      if (tile < all_tiles) step(partial, here, r0);
     };
     if (rounds > 0) issue(st0);
-    for (int it = 0; it < rounds; it += 2) {
-      round(it, st0, st1);
-      if (it + 1 < rounds) round(it + 1, st1, st0);
+    if constexpr (CAUSAL) {
+      // every head's tiles begin with those that some key is not seen by; the masks' part is left out of the others' code
+      const int hidden_tiles = (full + BR - 1) / BR - tile_lo;
+      int at = head_tiles > 0 ? first_tile % head_tiles : 0;
+      for (int it = 0; it < rounds;) {
+        for (; it < rounds && (at < hidden_tiles || at + 2 * RW > head_tiles); it += 2) {
+          round(std::true_type(), it, st0, st1);
+          if (it + 1 < rounds) round(std::true_type(), it + 1, st1, st0);
+          for (at += 2 * RW; at >= head_tiles;) at -= head_tiles;
+        }
+        for (; it < rounds && at >= hidden_tiles && at + 2 * RW <= head_tiles; it += 2, at += 2 * RW) {
+          round(std::false_type(), it, st0, st1);
+          if (it + 1 < rounds) round(std::false_type(), it + 1, st1, st0);
+        }
+        if (at >= head_tiles) at = 0;
+      }
+    } else {
+      for (int it = 0; it < rounds; it += 2) {
+        round(std::false_type(), it, st0, st1);
+        if (it + 1 < rounds) round(std::false_type(), it + 1, st1, st0);
+      }
     }
   } else {
     __bf16* qs = lds + rw * kGroup;
@@ -544,7 +598,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
       __syncthreads();
       advance();
       if (it + 1 < rounds) issue();
-      if (tile < all_tiles) step(qs, r0);
+      if (tile < all_tiles) step(std::bool_constant<CAUSAL>(), qs, r0);
     }
   }
 
@@ -599,7 +653,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 }
 
 // Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T.
-template <typename T, int DP, int WM, int KW, bool DMA>
+template <typename T, int DP, int WM, int KW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, AttnTiles kv,
                                                                                              int64_t tiles, int splits, float* part, T* gq) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = WM > 1 && NP == 1 ? 64 : 32;
@@ -613,7 +667,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int wm = wave % WM, kw = wave / WM;
   const int kvh = blockIdx.x % a.kv_heads;
   int64_t t = blockIdx.x / a.kv_heads;
-  if (a.causal) t = tiles - 1 - t;
+  if (CAUSAL) t = tiles - 1 - t;
   int64_t first;
   const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first);
   AttnSegment sg = attn_segment(a, ext);
@@ -625,10 +679,10 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int tok = attn_token(a, live ? row : rows - 1), head = kvh * a.group + (live ? row : rows - 1) - tok * a.group;
   const int64_t qt = sg.q0 + tok;
   const int shift = sg.nk - sg.nq;
-  const int sees = a.causal ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
+  const int sees = CAUSAL ? max(0, min(sg.nk, tok + shift + 1)) : sg.nk;
   const int last_row = min(row0 + 32 * WM, rows) - 1;
-  const int reach = a.causal ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
-  const int least = a.causal ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
+  const int reach = CAUSAL ? max(0, min(sg.nk, attn_token(a, last_row) + shift + 1)) : sg.nk;
+  const int least = CAUSAL ? max(0, min(sg.nk, attn_token(a, row0) + shift + 1)) : sg.nk;
   const int per = ((reach + BN - 1) / BN + splits - 1) / splits;
   const int tile_lo = blockIdx.y * per, tile_hi = min((reach + BN - 1) / BN, tile_lo + per);
 
@@ -653,8 +707,11 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const float c = a.scale * kLog2e;
 
   const int lt = threadIdx.x - kw * WM * 64;
-  const int lr = Tile::lane_rows(), lc = Tile::lane_cols();
-  auto step = [&](const __bf16* ks_, int tile) {
+  const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
+  auto step = [&](auto last, const __bf16* ks_, int tile) {
+    constexpr bool kLast = decltype(last)::value;  // a row may not see all of the tile
+    int lr = lane_r, lc = lane_c;
+    asm volatile("" : "+v"(lr), "+v"(lc));  // addresses formed here, not kept in registers
     const __bf16* vs_ = ks_ + Tile::SIZE;
 #pragma unroll
     for (int jb = 0; jb < BN; jb += 32) {
@@ -666,11 +723,16 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       for (int ks = 0; ks < KS; ++ks) dp = mma(Tile::rows(vs_, lr, jb, ks), gf[ks], dp);
 #pragma unroll
       for (int v = 0; v < 16; ++v) s[v] = exp2_hw(fmaf(s[v], c, -ls)) * (NP == 3 ? fmaf(dp[v], inv, -dl) : dp[v] - dl);
-      if (j0 + 32 > least) {
+      uint32_t bad = 0;
+      if (kLast && j0 + 32 > least) {
         const int left = sees - j0 - 4 * half;
+        if (CAUSAL) bad = rows_not_finite<Tile>(ks_ + jb * Tile::LD);
+        const uint32_t mine = bad >> 4 * half;
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
+        for (int v = 0; v < 16; ++v) {
+          if (mine >> prod_row(v, 0) & 1) s[v] = NAN;
           if (prod_row(v, 0) >= left) s[v] = 0.f;
+        }
       }
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
@@ -680,7 +742,11 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         Planes<NP> df;
         planes_of(y, df);
 #pragma unroll
-        for (int d = 0; d < DB; ++d) o[d] = mma(Tile::cols(ks_, lc, jb + 16 * step, d), df, o[d]);
+        for (int d = 0; d < DB; ++d) {
+          Planes<NP> kc = Tile::cols(ks_, lc, jb + 16 * step, d);
+          if (kLast && CAUSAL && bad) kc = finite_part<NP>(kc);
+          o[d] = mma(kc, df, o[d]);
+        }
       }
     }
   };
@@ -701,17 +767,23 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       kp += k_by;
       vp += v_by;
     };
-    auto round = [&](int it, const __bf16* here, __bf16* next) {
+    auto round = [&](auto last, int it, const __bf16* here, __bf16* next) {
       const int tile = tile_lo + it * KW + kw;
       __builtin_amdgcn_s_waitcnt(kWaitVm0);
       __syncthreads();
       if (it + 1 < rounds) issue(tile + KW, next);
-      if (tile < tile_hi) step(here, tile);
+      if (tile < tile_hi) step(last, here, tile);
     };
     if (rounds > 0) issue(tile_lo + kw, st0);
-    for (int it = 0; it < rounds; it += 2) {
-      round(it, st0, st1);
-      if (it + 1 < rounds) round(it + 1, st1, st0);
+    int it = 0;
+    if constexpr (CAUSAL)  // rounds whose tiles every row sees all of: the masks' part is left out of their code
+      for (const int full = (least / BN - tile_lo) / KW; it + 2 <= full && it + 2 <= rounds; it += 2) {
+        round(std::false_type(), it, st0, st1);
+        round(std::false_type(), it + 1, st1, st0);
+      }
+    for (; it < rounds; it += 2) {
+      round(std::true_type(), it, st0, st1);
+      if (it + 1 < rounds) round(std::true_type(), it + 1, st1, st0);
     }
   } else {
     __bf16* st = lds + kw * 2 * Tile::SIZE;
@@ -731,7 +803,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       vl.store(st + Tile::SIZE, lt);
       __syncthreads();
       if (it + 1 < rounds) issue(tile + KW);
-      if (tile < tile_hi) step(st, tile);
+      if (tile < tile_hi) step(std::true_type(), st, tile);
     }
   }
   if constexpr (KW > 1) {  // add the key groups, in their order, a column block at a time
@@ -897,7 +969,7 @@ AttnTiles bf16_tiles(const void* x, int64_t x_row, int64_t x_head, const void* y
   return {static_cast<const __bf16*>(x), static_cast<const __bf16*>(y), x_row, x_head, y_row, y_head};
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool CAUSAL>
 int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
   constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = f32 && DP > 32 ? 32 : 64;
@@ -914,12 +986,12 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
   const dim3 grid((unsigned)(tiles * a.kv_heads), splits);
   if (shape == kWide) {
-    attn_fwd_kernel<T, DP, kWideKeys, 4, 1, true><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
+    attn_fwd_kernel<T, DP, kWideKeys, 4, 1, true, CAUSAL><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
   } else if (shape == kMid) {
     if constexpr (f32 && DP <= 64)
-      attn_fwd_kernel<T, DP, 32, 2, 2, true><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
+      attn_fwd_kernel<T, DP, 32, 2, 2, true, CAUSAL><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
   } else {
-    attn_fwd_kernel<T, DP, 32, 1, kKeyWaves, !f32><<<grid, 64 * kKeyWaves, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
+    attn_fwd_kernel<T, DP, 32, 1, kKeyWaves, !f32, CAUSAL><<<grid, 64 * kKeyWaves, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
   }
   FMD_CHECK_LAUNCH();
   if (splits > 1) {
@@ -929,7 +1001,7 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   return FMD_OK;
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool CAUSAL>
 int run_bwd(const AttnArgs& a, const AttnBwd& b, int q_splits, int kv_splits, T* gq, T* gk, T* gv, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
   constexpr int kWaves = f32 && DP > 64 ? 2 : 4;
@@ -948,12 +1020,12 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, int q_splits, int kv_splits, T*
     float* part = work;
     if (kv_splits > 1) work += kv_splits * 2 * a.tk * a.kv_heads * a.dim;
     if (shape == kWide) {
-      attn_bwd_kv_kernel<T, DP, kWM, kRW, true><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
+      attn_bwd_kv_kernel<T, DP, kWM, kRW, true, CAUSAL><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
     } else if (shape == kMid) {
       if constexpr (f32 && DP <= 64)
-        attn_bwd_kv_kernel<T, DP, 2, kMidRW, true><<<grid, 128 * kMidRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
+        attn_bwd_kv_kernel<T, DP, 2, kMidRW, true, CAUSAL><<<grid, 128 * kMidRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
     } else {
-      attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
+      attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32, CAUSAL><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
     }
     FMD_CHECK_LAUNCH();
     if (kv_splits > 1) {
@@ -975,11 +1047,11 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, int q_splits, int kv_splits, T*
     const dim3 grid((unsigned)(tiles * a.kv_heads), q_splits);
     float* part = work;
     if (shape == kWide) {
-      attn_bwd_q_kernel<T, DP, 4, 1, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
+      attn_bwd_q_kernel<T, DP, 4, 1, true, CAUSAL><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
     } else if (shape == kMid) {
-      if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
+      if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true, CAUSAL><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
     } else {
-      attn_bwd_q_kernel<T, DP, 1, kWaves, !f32><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
+      attn_bwd_q_kernel<T, DP, 1, kWaves, !f32, CAUSAL><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
     }
     FMD_CHECK_LAUNCH();
     if (q_splits > 1) {
@@ -1010,6 +1082,12 @@ int check(const AttnArgs& a, int size) {
   return FMD_OK;
 }
 
+#define FMD_BY_WIDTH(F, ...)                                                                    \
+  if (a.dim <= 32) return a.causal ? F<T, 32, true>(__VA_ARGS__) : F<T, 32, false>(__VA_ARGS__); \
+  if (a.dim <= 64) return a.causal ? F<T, 64, true>(__VA_ARGS__) : F<T, 64, false>(__VA_ARGS__); \
+  if (a.dim <= 96) return a.causal ? F<T, 96, true>(__VA_ARGS__) : F<T, 96, false>(__VA_ARGS__); \
+  return a.causal ? F<T, 128, true>(__VA_ARGS__) : F<T, 128, false>(__VA_ARGS__);
+
 template <typename T>
 int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   const int status = check(a, sizeof(T));
@@ -1018,10 +1096,7 @@ int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   if (a.tq == 0) return FMD_OK;
   FMD_REQUIRE(out && aligned16(out) && aligned16(saved.residual) && (saved.base == nullptr) == (saved.inverse == nullptr));
   if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_fwd<T>(a, out, saved, stream);
-  if (a.dim <= 32) return run_fwd<T, 32>(a, splits, out, saved, work, stream);
-  if (a.dim <= 64) return run_fwd<T, 64>(a, splits, out, saved, work, stream);
-  if (a.dim <= 96) return run_fwd<T, 96>(a, splits, out, saved, work, stream);
-  return run_fwd<T, 128>(a, splits, out, saved, work, stream);
+  FMD_BY_WIDTH(run_fwd, a, splits, out, saved, work, stream)
 }
 
 template <typename T>
@@ -1044,10 +1119,7 @@ int backward(const AttnArgs& a, AttnBwd b, int q_splits, int kv_splits, T* gq, T
     FMD_CHECK_LAUNCH();
   }
   work += fmd_cdiv(2 * a.heads * a.tq, 4) * 4;
-  if (a.dim <= 32) return run_bwd<T, 32>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
-  if (a.dim <= 64) return run_bwd<T, 64>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
-  if (a.dim <= 96) return run_bwd<T, 96>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
-  return run_bwd<T, 128>(a, b, q_splits, kv_splits, gq, gk, gv, work, stream);
+  FMD_BY_WIDTH(run_bwd, a, b, q_splits, kv_splits, gq, gk, gv, work, stream)
 }
 
 AttnArgs args_of(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row, int64_t k_head, const void* v,

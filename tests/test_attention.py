@@ -216,6 +216,46 @@ def test_values_of_other_segments_do_not_matter(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [([80], 2, 1, 32), ([150, 61], 4, 4, 64), ([70], 6, 2, 96), ([200], 1, 1, 128),
+                                                        ([1500, 900], 16, 4, 64), ([1300, 1500], 16, 16, 32),
+                                                        ([1] * 300, 2, 2, 32)])
+def test_rows_that_are_not_seen_yet_do_not_matter(lengths, heads, kv_heads, dim, dtype):
+    """Causal, with infinities and NaN from the middle of each segment on: the rows before are as without them; and so are
+    the gradients of the keys after a query's gradient that is not finite."""
+    from fastmd_amd.ops.attention import segment_attention_forward, segment_attention_vjp
+
+    q, k, v, g, off, _ = make(lengths, lengths, heads, kv_heads, dim, dtype, seed=dim)
+    start = off.tolist()
+    cut = [a + (b - a) // 2 + 3 for a, b in zip(start, start[1:])]
+    before = torch.cat([torch.arange(a, min(c, b)) for a, c, b in zip(start, cut, start[1:])])
+    after = torch.cat([torch.arange(min(c, b), b) for c, b in zip(cut, start[1:])])
+
+    def run(q, k, v, g):
+        x = [t.cuda() for t in (q, k, v, g)]
+        o = off.cuda()
+        out, saved = segment_attention_forward(*x[:3], o, causal=True)
+        return [t.cpu() for t in (out, *segment_attention_vjp(x[3], *x[:3], out, saved, o, causal=True))]
+
+    want = run(q, k, v, g)
+    k2, v2 = k.clone(), v.clone()
+    k2[after], v2[after] = float("nan"), float("inf")
+    v2[after[::3]] = float("nan")
+    got = run(q, k2, v2, g)
+    assert torch.isfinite(got[0][before]).all() and torch.isfinite(got[1][before]).all()
+    r = oracle.segment_attention(q, k, v, off, off, causal=True, gout=g)
+    b = bounds(r, dtype)
+    for n, name in ((0, "out"), (1, "gq")):
+        compare(got[n][before], r[name][before], b[name][before], name)
+    # a gradient that is not finite in the first half: the keys after it are not seen by those queries
+    q2, g2 = q.clone(), g.clone()
+    g2[before], q2[before[::2]] = float("nan"), float("inf")
+    got = run(q2, k, v, g2)
+    for n, name in ((2, "gk"), (3, "gv")):
+        compare(got[n][after], r[name][after], b[name][after], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 def test_strided_inputs(dtype):
     """Columns of a packed projection, a head-major layout, a strided gradient, unaligned and broadcast inputs."""
     from fastmd_amd.ops.attention import segment_attention_forward, segment_attention_vjp
