@@ -181,3 +181,37 @@ def energy_forces_stress(node_energy_fn, positions, cell):
     grad, gstrain = torch.autograd.grad(energy, (leaf, strain))
     volume = torch.dot(cell[0], torch.linalg.cross(cell[1], cell[2])).abs()
     return energy.detach(), -grad, gstrain / volume
+
+
+def attention_like_node_energy(params: dict, config: dict, positions, cell, elem, center, neighbor, images, systems=None):
+    """Per-atom energies of the attention model specified in fastmd_amd/models/attention_like.py. ``systems``: (first row,
+    rows) of each system (None: one)."""
+    dt = positions.dtype
+    p = {k: v.to(dt) for k, v in params.items()}
+    n, nb, nel = positions.shape[0], config["n_basis"], len(config["elements"])
+    H, Hk, D = config["heads"], config["kv_heads"], config["head_dim"]
+    vec = edge_vectors(positions, cell.to(dt), center, neighbor, images)
+    ef, _ = radial_basis(vec.norm(dim=1), config["cutoff"], nb)
+    elem = elem.long()
+    d = torch.zeros(n * nel, nb, dtype=dt).index_add_(0, center * nel + elem[neighbor], ef)
+    x = d.view(n, nel * nb) / config["avg_num_neighbors"] @ p["W_in"].T + p["embedding"][elem]
+    turn = elem[:, None].to(dt) * 10000.0 ** (-torch.arange(0, D, 2, dtype=dt) / D)
+    cos, sin = turn.cos()[:, None], turn.sin()[:, None]
+
+    def head(t, weight):
+        t = t * torch.rsqrt((t * t).mean(-1, keepdim=True) + 1e-6) * weight
+        a, b = t[..., :D // 2], t[..., D // 2:]
+        return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+
+    for t in range(config["num_layers"]):
+        W = {k.split(".", 2)[2]: v for k, v in p.items() if k.startswith(f"layers.{t}.")}
+        qkv = (x @ W["W_qkv"].T).view(n, H + 2 * Hk, D)
+        q, k, v = head(qkv[:, :H], W["q_weight"]), head(qkv[:, H:H + Hk], W["k_weight"]), qkv[:, H + Hk:]
+        k, v = k.repeat_interleave(H // Hk, 1), v.repeat_interleave(H // Hk, 1)
+        out = []
+        for a, m in systems or [(0, n)]:
+            s = torch.einsum("ihd,jhd->hij", q[a:a + m], k[a:a + m]) / math.sqrt(D)
+            out.append(torch.einsum("hij,jhd->ihd", s.softmax(-1), v[a:a + m]))
+        x = x + torch.cat(out).reshape(n, H * D) @ W["W_o"].T
+        x = x + torch.nn.functional.silu(x @ W["W_1"].T) @ W["W_2"].T
+    return p["e0"][elem] + (x * p["wr"]).sum(1)
