@@ -25,9 +25,8 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kMerge = (KW - 1) * WM * (DB * 16 + 2) * 64 * 2;  // in bf16 units
   constexpr int kTiles = 2 * KW * Tile::SIZE;
-  // bf16 tiles are copied straight into LDS, a tile ahead, into two buffers; fp32 tiles go through registers, where they are
-  // split, into one
-  constexpr bool kDma = NP == 1;
+  // DMA: tiles of bf16 (or of planes) are copied straight into LDS, a tile ahead, into two buffers; else fp32 tiles go through
+  // registers, where they are split, into one
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
   __shared__ __attribute__((aligned(16))) __bf16 lds2[DMA ? kTiles : 8];
 
@@ -877,23 +876,34 @@ __global__ void __launch_bounds__(256) attn_split_kernel(const float* x, int64_t
 int64_t tile_count(int64_t rows, int group, int segments, int bm) { return rows * group / bm + segments + 2; }
 
 // How a workgroup's waves share a tile. kWide: four waves of 32 rows each over the same keys. kNarrow: the waves take the same
-// 32 rows and share the keys, for calls with too few tiles to fill the card otherwise and segments shorter than a tile. kMid:
-// two and two, fp32 only, whose narrow form splits every tile into planes in the wave that reads it (fp32 heads above 64 have
-// room in LDS for wide tiles alone, and two narrow waves).
+// 32 rows and share the keys, for calls with too few tiles to fill the card otherwise and segments not much longer than a
+// tile. kMid: two and two, fp32 only, whose narrow form splits every tile into planes in the wave that reads it (fp32 heads
+// above 64 have room in LDS for wide tiles alone, and two narrow waves).
+// Measured, us of forward + both halves of the VJP:
+//   one segment, bf16, 8 heads of 64: 2 000 rows narrow 87, wide 127; 4 000 rows 253, 245; 8 000 rows 868, 722
+//   ", 8 heads of 128: 1 000 rows 77, 110; 2 000 rows 227, 183; 4 000 rows 795, 372
+//   ", fp32, 4 heads of 32: 2 000 rows narrow 122, mid 135, wide 142; 4 000 rows 325, 300, 436; 8 000 rows 1 157, 913, 1 063
+//   ", 4 heads of 64: 1 000 rows 99, 125, 185; 2 000 rows 198, 178, 196; 8 000 rows 2 753, 1 734, 1 619
+//   ", 4 heads of 128: 1 000 rows narrow 320, wide 304; 2 000 rows 805, 296
+//   64 segments, 4 heads of 32, fp32: 80 rows narrow 54, mid 82, wide 67; 160 rows 102, 118, 105; 320 rows 210, 215, 193;
+//   bf16: 80 rows 50, -, 50; 160 rows 53, -, 54; 320 rows 90, -, 82
 enum AttnShape { kNarrow, kMid, kWide };
 
 AttnShape shape_of(bool f32, int dim, int64_t rows, int heads, int segments) {
   const int64_t blocks = rows / 32 * heads;
-  if (rows < (int64_t)64 * segments) return kNarrow;
-  if (blocks >= 1024 || (f32 && dim > 64 && blocks >= 192)) return kWide;
-  return f32 && dim <= 64 && blocks >= 256 ? kMid : kNarrow;
+  if (rows < (int64_t)(f32 && dim <= 64 ? 192 : 64) * segments) return kNarrow;
+  if (blocks >= (dim <= 64 ? 1024 : f32 ? 192 : 384)) return kWide;
+  return f32 && dim <= 64 && blocks >= (dim <= 32 ? 384 : 224) ? kMid : kNarrow;
 }
 
 constexpr int shape_rows(AttnShape s) { return s == kWide ? 128 : s == kMid ? 64 : 32; }
 
-// About one query per segment over a few keys each, and enough segments to fill the card with a wave each: the row kernels.
+// About one query per segment, and enough segments to fill the card with a wave each: the row kernels. The more segments,
+// the longer a wave may take over one. Measured, 4 heads of 32, us of forward + VJP on the row kernels (tiles):
+//   fp32: 10 000 segments of 18 keys 103 (1 004), 256 of 128 39 (61), 256 of 400 114 (100), 2 000 of 400 504 (762), 1 024 of
+//   500 338 (455); bf16: 54 (456), 42 (49), 115 (113), 269 (845), 224 (520)
 bool few_rows(int64_t tq, int64_t tk, int segments, int kv_heads) {
-  return segments >= 256 && tq <= segments && tk <= (int64_t)128 * segments;
+  return segments >= 256 && tq <= segments && tk <= (int64_t)(segments >= 1024 ? 512 : 128) * segments;
 }
 
 // Key splits of the forward: as many as bring the workgroups to one per CU, each with kSplitKeys keys at least of a
@@ -972,7 +982,10 @@ AttnTiles bf16_tiles(const void* x, int64_t x_row, int64_t x_head, const void* y
 template <typename T, int DP, bool CAUSAL>
 int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
-  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = f32 && DP > 32 ? 32 : 64;
+  // Keys of a wide tile: 64 (4 x 3 000 rows, 8 heads, bf16: 148 us against 165 of 32 keys at 96 columns, 117 against 128 at 64;
+  // fp32 at 32: 234 against 282), but 32 where more has no registers (fp32 above 32) or costs the third wave of a SIMD in
+  // long causal calls (five prompts of 12 000 rows together, 16 heads of 128: 237 us against 250; one full segment of 4 000: 105 against 88).
+  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = (f32 && DP > 32) || (CAUSAL && DP > 96) ? 32 : 64;
   const int64_t n = a.tq * a.heads;
   AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
   const AttnShape shape = shape_of(f32, a.dim, a.tq * a.group, a.kv_heads, a.segments);

@@ -4,8 +4,9 @@
 // One wave per segment and block of key heads. A unit of D / 8 lanes (a power of two) takes one key row of one head, eight
 // columns a lane; the units of a wave lie along the heads (a row's heads are contiguous) and then along keys. Every key row is
 // read once and, in the VJP of a single query, its two gradients are written in the same pass. The matrix kernels spend a
-// tile of 32 rows on such a segment's single one. [10 000 segments, 180 096 keys, 4 heads of 32, float32, forward and VJP:
-// see the launch rule in attention.hip]
+// tile of 32 rows on such a segment's single one. 10 000 segments, 180 096 keys, 4 heads of 32: 35 + 75 us forward and VJP in
+// float32 (195 and 389 MB: 5.6 and 5.1 TB/s, where a large copy reaches 4.8, the caches holding part of it; 1 004 us on the
+// matrix kernels), 20 + 34 us in bf16.
 #include "attention.h"
 
 namespace {

@@ -128,6 +128,25 @@ def test_middle_sizes_in_float32(dim, causal):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [16, 32])
+def test_middle_sizes_of_narrow_heads_in_float32(dim, causal):
+    q, k, v, g, q_off, k_off = make([1300, 1, 0, 1201, 900], [1300, 33, 5, 1201, 950], 4, 4, dim, torch.float32, seed=dim)
+    check(q, k, v, g, q_off, k_off, causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_segments_of_a_few_hundred_rows(dtype):
+    """Single queries, enough segments for a wave each over longer keys."""
+    g = torch.Generator().manual_seed(8)
+    lk = torch.randint(100, 260, (1030,), generator=g).tolist()
+    lk[3], lk[4], lk[1029] = 0, 900, 1
+    q, k, v, go, q_off, k_off = make([1] * 1030, lk, 2, 1, 24, dtype, seed=9)
+    check(q, k, v, go, q_off, k_off, causal=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("dim", [32, 128])
 def test_wide_tiles_with_shared_heads_and_other_key_counts(dim, dtype):
