@@ -459,7 +459,8 @@ __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
   for (int i = 0; i < 8; ++i) x[i] = (float)e[i];
 }
 
-// bytes of output from which a call's stores go past the caches
+// bytes of output from which a call's stores go past the caches (norm and rotation with 205 MB of output 86 us instead of 104,
+// the neighbours' VJP with 184 MB 75 instead of 90; with 69 MB 30.3 instead of 27.6)
 constexpr int64_t kStreamBytes = 128 << 20;
 
 // the part of eight (four) outputs that their rounding to bf16 dropped

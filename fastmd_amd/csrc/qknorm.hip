@@ -3,13 +3,19 @@
 //   r = (mean x^2 + eps)^(-1/2),  y = x r w,  (a, b) -> (a cos - b sin, b cos + a sin) on the first `rot` columns
 //
 // A row (one head of one token) belongs to a group of LG lanes, eight columns each: one read, one write, the mean by
-// lane exchanges. A group takes a few heads of its token at a time, so their loads are in flight together and the
-// token's cosines, sines and weights are read once. All arithmetic is fp32, each output rounded once.
+// lane exchanges. The angles come from tables, one row for all heads of a token. All arithmetic is fp32, each output rounded
+// once. Memory bounds both directions (of a large copy's 4.8 TB/s): 40 000 tokens of 20 heads of 128, bf16, half of the columns
+// turned, 85 us forward (4.8 TB/s), 208 VJP (3.0); 16 875 tokens of 16 heads of 64, fp32, 27 us (5.1) and 44 (4.7, with the
+// weights' gradients); below some 2 000 rows the host's time for a launch does.
 #include "attention.h"
 
 namespace {
 
-constexpr int kFwdHeads = 4, kBwdHeads = 2;  // heads of a unit: more loads in flight against more registers
+// The forward takes four heads of a token in a unit: their loads are in flight together and the token's angles and weights are
+// read once (16 875 x 16 x 64 fp32 27.3 us, of two 26.9, of eight 26.0; 40 000 x 20 x 128 bf16 86, 88, 83; 40 000 x 3 x 256
+// 39, -, 60; 100 000 x 8 x 32 fp32 38, -, 42). The VJP, which holds twice as much of each, takes one: 44 us in the first
+// of these against 54 of two and 52 of four, 208 against 250 of two in the second, 58 against 74, 73 against 92.
+constexpr int kFwdHeads = 4;
 
 struct NormArgs {
   const void *q, *k;  // [tokens, heads, dim]; k may be null
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
   constexpr int GROUPS = 256 / LG;
   __shared__ float sum[2][256][8];
   const int sub = threadIdx.x & (LG - 1), col0 = 8 * sub, group = threadIdx.x / LG;
-  const int blocks = head_blocks(a, kBwdHeads), qb = (a.heads + kBwdHeads - 1) / kBwdHeads;
+  const int blocks = a.heads + a.kv_heads;  // a unit: one head of one token
   const int64_t units = a.tokens * blocks;
   const bool cols = col0 < a.dim;
   float gw[2][8];
@@ -186,22 +192,18 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
     const bool in = unit < units;
     const int64_t tok = in ? unit / blocks : 0;
     const int hb = in ? (int)(unit % blocks) : 0;
-    const bool is_k = hb >= qb;
-    const int h0 = (is_k ? hb - qb : hb) * kBwdHeads, heads = is_k ? a.kv_heads : a.heads;
-    const T* xp = static_cast<const T*>(is_k ? a.k : a.q) + tok * (is_k ? a.k_row : a.q_row) + col0;
-    const T* gp = static_cast<const T*>(is_k ? g.gk : g.gq) + tok * (is_k ? g.gk_row : g.gq_row) + col0;
-    const int64_t xh = is_k ? a.k_head : a.q_head, gh = is_k ? g.gk_head : g.gq_head;
-    T* out = (is_k ? gk_out : gq_out) + tok * heads * a.dim + col0;
-    float x[kBwdHeads][8], y[kBwdHeads][8];
+    const bool is_k = hb >= a.heads;
+    const int h = is_k ? hb - a.heads : hb;
+    const T* xp = static_cast<const T*>(is_k ? a.k : a.q) + tok * (is_k ? a.k_row : a.q_row) + h * (is_k ? a.k_head : a.q_head);
+    const T* gp = static_cast<const T*>(is_k ? g.gk : g.gq) + tok * (is_k ? g.gk_row : g.gq_row) +
+                  h * (is_k ? g.gk_head : g.gq_head);
+    T* out = (is_k ? gk_out : gq_out) + (tok * (is_k ? a.kv_heads : a.heads) + h) * a.dim;
+    float x[8], y[8];
 #pragma unroll
-    for (int h = 0; h < kBwdHeads; ++h) {
-      if (in && cols && h0 + h < heads) {
-        load8<T>(gp + (h0 + h) * gh, y[h]);
-        if (a.norm) load8<T>(xp + (h0 + h) * xh, x[h]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[h][e] = y[h][e] = 0.f;
-      }
+    for (int e = 0; e < 8; ++e) x[e] = y[e] = 0.f;
+    if (in && cols) {
+      load8<T>(gp + col0, y);
+      if (a.norm) load8<T>(xp + col0, x);
     }
     float w[8], c[8], s[8];
 #pragma unroll
@@ -209,30 +211,27 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
     const T* wp = static_cast<const T*>(is_k ? a.wk : a.wq);
     if (cols && wp) load8<T>(wp + col0, w);
     if (in && cols) angles<TURN>(a, tok, col0, c, s);
+    rotate<LG, TURN>(a, col0, c, s, -1.f, y);
+    if (a.norm) {
+      float ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int h = 0; h < kBwdHeads; ++h) {
-      rotate<LG, TURN>(a, col0, c, s, -1.f, y[h]);
-      if (a.norm) {
-        float ss = 0.f, dot = 0.f;
+      for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
+      const float r = 1.f / sqrtf(group_sum<LG>(ss) / a.dim + a.eps);
+      float gn[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss += x[h][e] * x[h][e];
-        const float r = 1.f / sqrtf(group_sum<LG>(ss) / a.dim + a.eps);
-        float gn[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[h][e] *= r;  // the normalised value
-          gn[e] = y[h][e] * w[e];
-          dot += gn[e] * x[h][e];
-          const float t = y[h][e] * x[h][e];
-          gw[0][e] += is_k ? 0.f : t;
-          gw[1][e] += is_k ? t : 0.f;
-        }
-        const float mean = group_sum<LG>(dot) / a.dim;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) y[h][e] = r * (gn[e] - x[h][e] * mean);
+      for (int e = 0; e < 8; ++e) {
+        x[e] *= r;  // the normalised value
+        gn[e] = y[e] * w[e];
+        dot += gn[e] * x[e];
+        const float t = y[e] * x[e];
+        gw[0][e] += is_k ? 0.f : t;
+        gw[1][e] += is_k ? t : 0.f;
       }
-      if (in && cols && h0 + h < heads) store8<NT>(out + (h0 + h) * a.dim, y[h]);
+      const float mean = group_sum<LG>(dot) / a.dim;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = r * (gn[e] - x[e] * mean);
     }
+    if (in && cols) store8<NT>(out + col0, y);
   }
   if (!part) return;
 #pragma unroll
@@ -248,7 +247,7 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
   }
 }
 
-// column sums of the workgroups' rows: 16 columns a workgroup, 64 threads each over every 64th row, joined in order
+// gradient of the weights: column sums of the workgroups' rows: 16 columns a workgroup, 64 threads each over every 64th row, joined in order
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_weights_kernel(const float* part, int rows, int dim, T* gwq, T* gwk) {
   __shared__ float sum[64][16];
@@ -278,7 +277,8 @@ int64_t unit_count(int64_t tokens, int heads, int kv_heads, int by) {
   return tokens * ((heads + by - 1) / by + (kv_heads + by - 1) / by);
 }
 
-// workgroups of the VJP: at most 1 024 (four per CU), so that the partial sums stay few
+// workgroups of the VJP: at most 1 024 (four per CU), so that the partial sums stay few (at most 2 048: 49 us against 44 and 215
+// against 207 in the cases above)
 void bwd_grid(int64_t units, int groups, int* grid, int* per) {
   const int64_t n = fmd_cdiv(units, groups);
   *per = n > 1024 ? (int)fmd_cdiv(n, 1024) : 1;
@@ -338,7 +338,7 @@ void norm_bwd_turn(const NormArgs& a, const NormGrad& g, int grid, int per, T* g
 
 template <typename T, int LG>
 int norm_bwd(const NormArgs& a, const NormGrad& g, T* gq, T* gk, T* gwq, T* gwk, float* work, hipStream_t stream) {
-  const int64_t units = unit_count(a.tokens, a.heads, a.kv_heads, kBwdHeads);
+  const int64_t units = unit_count(a.tokens, a.heads, a.kv_heads, 1);
   const bool weights = gwq || gwk;
   int grid = 0, per = 0;
   bwd_grid(units, 256 / LG, &grid, &per);
@@ -414,7 +414,7 @@ int fmd_qk_norm_rotary(int32_t bf16, FMD_NORM_PARAMS, void* q_out, void* k_out, 
 int64_t fmd_qk_norm_rotary_work_size(int64_t tokens, int32_t heads, int32_t kv_heads, int32_t dim) {
   if (tokens <= 0 || heads < 0 || kv_heads < 0 || dim <= 0 || dim > 256) return 0;
   int grid = 0, per = 0;
-  bwd_grid(unit_count(tokens, heads, kv_heads, kBwdHeads), 256 / groups_of(dim), &grid, &per);
+  bwd_grid(unit_count(tokens, heads, kv_heads, 1), 256 / groups_of(dim), &grid, &per);
   return (int64_t)grid * 2 * dim;
 }
 
