@@ -5,8 +5,9 @@
 // A row (one head of one token) belongs to a group of LG lanes, eight columns each: one read, one write, the mean by
 // lane exchanges. The angles come from tables, one row for all heads of a token. All arithmetic is fp32, each output rounded
 // once. Memory bounds both directions (of a large copy's 4.8 TB/s): 40 000 tokens of 20 heads of 128, bf16, half of the columns
-// turned, 85 us forward (4.8 TB/s), 208 VJP (3.0); 16 875 tokens of 16 heads of 64, fp32, 27 us (5.1) and 44 (4.7, with the
-// weights' gradients); below some 2 000 rows the host's time for a launch does.
+// turned, 83 us forward (5.0 TB/s), 192 VJP (3.2); 16 875 tokens of 16 heads of 64, fp32, 26 us (5.2) and 42 (5.0, with the
+// weights' gradients); below some 2 000 rows the host's time for a launch does. The bf16 VJP issues as many instructions as its
+// loads can hide: units counted in 32 bits instead of 64, and the reciprocal root in one instruction, took 5 % off it.
 #include "attention.h"
 
 namespace {
@@ -129,10 +130,10 @@ __device__ __forceinline__ int head_blocks(const NormArgs& a, int by) {
 template <typename T, int LG, Turn TURN, bool NT>
 __global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k_out) {
   const int sub = threadIdx.x & (LG - 1), col0 = 8 * sub;
-  const int64_t unit = (int64_t)blockIdx.x * (256 / LG) + threadIdx.x / LG;
+  const uint32_t unit = blockIdx.x * (256 / LG) + threadIdx.x / LG;  // fewer than 2^31 of them
   const int blocks = head_blocks(a, kFwdHeads), qb = (a.heads + kFwdHeads - 1) / kFwdHeads;
-  int64_t tok = unit / blocks;
-  const int hb = (int)(unit % blocks);
+  int64_t tok = unit / (uint32_t)blocks;
+  const int hb = (int)(unit % (uint32_t)blocks);
   const bool in = tok < a.tokens, is_k = hb >= qb;
   if (!in) tok = 0;
   const int h0 = (is_k ? hb - qb : hb) * kFwdHeads, heads = is_k ? a.kv_heads : a.heads;
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k
   const int64_t hs = is_k ? a.k_head : a.q_head;
   T* out = (is_k ? k_out : q_out) + tok * heads * a.dim;
   const bool cols = col0 < a.dim;
+  const float inv_dim = 1.f / a.dim;
   float y[kFwdHeads][8];
 #pragma unroll
   for (int h = 0; h < kFwdHeads; ++h) {
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += y[h][e] * y[h][e];
-      const float r = 1.f / sqrtf(group_sum<LG>(ss) / a.dim + a.eps);
+      const float r = rsqrtf(fmaf(group_sum<LG>(ss), inv_dim, a.eps));
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[h][e] = y[h][e] * r * w[e];
     }
@@ -181,14 +183,14 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
   constexpr int GROUPS = 256 / LG;
   __shared__ float sum[2][256][8];
   const int sub = threadIdx.x & (LG - 1), col0 = 8 * sub, group = threadIdx.x / LG;
-  const int blocks = a.heads + a.kv_heads;  // a unit: one head of one token
-  const int64_t units = a.tokens * blocks;
+  const uint32_t blocks = a.heads + a.kv_heads, units = (uint32_t)a.tokens * blocks;  // a unit: one head of one token; below 2^31
   const bool cols = col0 < a.dim;
+  const float inv_dim = 1.f / a.dim;
   float gw[2][8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) gw[0][e] = gw[1][e] = 0.f;
   for (int n = 0; n < per; ++n) {
-    const int64_t unit = ((int64_t)blockIdx.x * per + n) * GROUPS + group;
+    const uint32_t unit = (blockIdx.x * per + n) * GROUPS + group;
     const bool in = unit < units;
     const int64_t tok = in ? unit / blocks : 0;
     const int hb = in ? (int)(unit % blocks) : 0;
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
       float ss = 0.f, dot = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss += x[e] * x[e];
-      const float r = 1.f / sqrtf(group_sum<LG>(ss) / a.dim + a.eps);
+      const float r = rsqrtf(fmaf(group_sum<LG>(ss), inv_dim, a.eps));
       float gn[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(256) qk_norm_bwd_kernel(NormArgs a, NormGrad g
         gw[0][e] += is_k ? 0.f : t;
         gw[1][e] += is_k ? t : 0.f;
       }
-      const float mean = group_sum<LG>(dot) / a.dim;
+      const float mean = group_sum<LG>(dot) * inv_dim;
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = r * (gn[e] - x[e] * mean);
     }
