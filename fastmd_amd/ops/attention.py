@@ -10,7 +10,8 @@ of a batch, the neighbour rows of each atom, packed sequences), read on the devi
 synchronises nor depends on lengths that the host would have to know. ``group = heads / kv_heads`` query heads share a
 key head. ``causal``: the last query of a segment sees all its keys, each one before it one key less. A query that sees
 no key, and a row outside every segment (the unused rows of a fixed-capacity buffer), gives zero and gets zero gradient;
-rows outside a query's segment are not read for it, whatever they hold.
+rows outside a query's segment are not read for it, whatever they hold, and neither an infinity nor a NaN in a key row that a
+causal query does not see reaches it (nor, in the VJP, one in a query's row the keys that it does not see).
 
 float32 is computed on the bf16 matrix cores with every operand split into three planes (float32 accuracy; an
 infinite value in a row that is seen gives NaN), bfloat16 with products of bfloat16 operands. Scores, softmax statistics
