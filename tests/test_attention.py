@@ -237,6 +237,7 @@ def test_values_of_other_segments_do_not_matter(dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lengths,heads,kv_heads,dim", [([80], 2, 1, 32), ([150, 61], 4, 4, 64), ([70], 6, 2, 96), ([200], 1, 1, 128),
                                                         ([1500, 900], 16, 4, 64), ([1300, 1500], 16, 16, 32),
+                                                        ([900, 1000], 4, 4, 64), ([1300, 900], 16, 4, 128),
                                                         ([1] * 300, 2, 2, 32)])
 def test_rows_that_are_not_seen_yet_do_not_matter(lengths, heads, kv_heads, dim, dtype):
     """Causal, with infinities and NaN from the middle of each segment on: the rows before are as without them; and so are
