@@ -403,6 +403,64 @@ def test_other_stream(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths,dtype,causal", [([135], torch.float32, False), ([900, 1, 700], torch.bfloat16, True),
+                                                  ([1500, 1300], torch.float32, False)])
+def test_captured_and_replayed(lengths, dtype, causal):
+    """Forward and VJP in a graph: every replay on new values equals the eager call, which runs between the replays."""
+    from fastmd_amd.ops.attention import segment_attention_forward, segment_attention_vjp
+
+    def run(q, k, v, g, off):
+        out, saved = segment_attention_forward(q, k, v, off, causal=causal)
+        return (out, *segment_attention_vjp(g, q, k, v, out, saved, off, causal=causal))
+
+    held = [x.cuda() for x in make(lengths, lengths, 4, 2, 64, dtype)[:5]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(*held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(*held)
+    for seed in range(1, 5):
+        new = [x.cuda() for x in make(lengths, lengths, 4, 2, 64, dtype, seed=seed)[:5]]
+        for x, y in zip(held, new):
+            x.copy_(y)
+        graph.replay()
+        want = run(*new)
+        torch.cuda.synchronize()
+        for x, y in zip(got, want):
+            assert torch.equal(x, y), seed
+
+
+@pytest.mark.gpu
+def test_rows_past_32_bits():
+    """A cache of more than 2^31 elements, segments at both ends, nothing but their rows written."""
+    from fastmd_amd.ops.attention import segment_attention_forward, segment_attention_vjp
+
+    q, k, v, g, q_off, k_off = make([3, 5], [70, 300], 8, 4, 128, torch.bfloat16)
+    rows = 2 ** 31 // 512 + 5000
+    r = oracle.segment_attention(q, k, v, q_off, k_off, causal=True, gout=g)
+    b = bounds(r, torch.bfloat16)
+
+    def spread(x):
+        y = torch.empty(rows, 4, 128, dtype=x.dtype, device="cuda")
+        y[:70], y[-300:] = x[:70].cuda(), x[70:].cuda()
+        return y
+
+    k, v = spread(k), spread(v)
+    q, g, q_off = q.cuda(), g.cuda(), torch.tensor([0, 3, 3, 8], device="cuda")
+    k_off = torch.tensor([0, 70, rows - 300, rows], device="cuda")
+    out, saved = segment_attention_forward(q, k, v, q_off, k_off, causal=True)
+    compare(out, r["out"], b["out"], "out")
+    gq, gk, gv = segment_attention_vjp(g, q, k, v, out, saved, q_off, k_off, causal=True)
+    compare(gq, r["gq"], b["gq"], "gq")
+    for x, name in ((gk, "gk"), (gv, "gv")):
+        compare(torch.cat((x[:70], x[-300:])), r[name], b[name], name)
+        assert not any(bool(part.any()) for part in x[70:-300].split(1 << 20))
+
+
+@pytest.mark.gpu
 def test_refusals():
     from fastmd_amd.ops.attention import AttentionSaved, segment_attention, segment_attention_vjp
 

@@ -209,6 +209,31 @@ def test_no_tokens():
 
 
 @pytest.mark.gpu
+def test_rows_past_32_bits():
+    from fastmd_amd.ops.qk_norm import qk_norm_rotary, qk_norm_rotary_vjp
+
+    tokens = 2 ** 31 // 2048 + 70
+    q, k, _, _, gq, gk = make(70, 16, 1, 128, torch.bfloat16)
+    cos, sin = tables(100, 128)
+
+    def last(x):
+        y = torch.empty(tokens, *x.shape[1:], dtype=x.dtype, device="cuda")
+        y[-70:] = x.cuda()
+        return y
+
+    positions = torch.arange(tokens, dtype=torch.int32, device="cuda") % 100
+    args = (last(q), last(k), None, None, cos.cuda(), sin.cuda(), positions)
+    out = qk_norm_rotary(*args)
+    grads = qk_norm_rotary_vjp(last(gq), last(gk), *args)
+    at = positions[-70:].cpu()
+    for n, (x, g) in enumerate(((q, gq), (k, gk))):
+        y, gx, _ = oracle.norm_rotary(x, None, cos, sin, at, g=g)
+        near(out[n][-70:], y, y.norm(dim=-1, keepdim=True), x.dtype, 12)
+        rms = torch.sqrt((x.double() ** 2).mean(-1, keepdim=True) + 1e-6)
+        near(grads[n][-70:], gx, g.double().norm(dim=-1, keepdim=True) / rms * 2, x.dtype, 32)
+
+
+@pytest.mark.gpu
 def test_refusals():
     from fastmd_amd.ops.qk_norm import qk_norm_rotary, qk_norm_rotary_vjp, rotary
 
