@@ -16,6 +16,21 @@ namespace {
 // one it puts the sums into accumulation registers and moves them out and back at every rescaling.
 static constexpr int attn_waves(int planes, int dp, int sums) { return planes * dp * sums <= 192 ? 2 : 1; }
 
+// bf16 weights (P, dS) in the calls of the narrow shape, WM = 1, are two bf16 parts, the second what the rounding of the first
+// dropped: a product more of five, where few rows with few keys each may make most of a result and the rounding of their
+// weights does not average out (gq of 245 causal rows of 24 heads of 16: 1.5 times the error of rounding the result alone, now
+// 1.0). It costs 45 -> 48 us forward and 106 -> 110 VJP at 801 queries over 12 003 keys of 8 heads on 2 of 128, nothing where
+// memory bounds (16 x 40 000 keys: 235 us).
+template <int NP>
+__device__ __forceinline__ Planes<NP> rest_of(const float (&x)[8], const Planes<NP>& first) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = x[e] - (float)first.p[0][e];
+  Planes<NP> o;
+  planes_of(y, o);
+  return o;
+}
+
 // ------------------------------------------------------------------------------------ forward
 
 // One workgroup: 32 WM packed query rows of one key head, WM KW waves. Wave (wm, kw) holds 32 rows and walks the key
@@ -34,6 +49,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
                                                                 int64_t tiles, int splits, T* out, AttnSaved saved,
                                                                 float* part_o, float* part_m, float* part_l) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, JB = BN / 32;
+  constexpr bool kTwoParts = NP == 1 && WM == 1;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kMerge = (KW - 1) * WM * (DB * 16 + 2) * 64 * 2;  // in bf16 units
   constexpr int kTiles = 2 * KW * Tile::SIZE;
@@ -160,13 +176,15 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = s[j][8 * step + e];
-        Planes<NP> pf;
+        Planes<NP> pf, rest;
         planes_of(x, pf);
+        if (kTwoParts) rest = rest_of(x, pf);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           Planes<NP> vc = Tile::cols(vs_, lc, 32 * j + 16 * step, d);
           if (kLast && CAUSAL && bad) vc = finite_part<NP>(vc);
           o[d] = mma(vc, pf, o[d]);
+          if (kTwoParts) o[d] = mma(vc, rest, o[d]);
         }
       }
   };
@@ -386,6 +404,7 @@ template <typename T, int DP, int WM, int RW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
                                                                                               int splits, float* part, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
+  constexpr bool kTwoParts = NP == 1 && WM == 1;
   using Tile = AttnTile<NP, BR, DP>;
   constexpr int kStats = NP == 3 ? 4 * BR : 2 * BR;  // offset, delta (inverse and nothing) of BR rows
   constexpr int kGroup = 2 * Tile::SIZE + 2 * kStats;  // in bf16 units
@@ -518,17 +537,20 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
         x[e] = s[8 * step + e];
         y[e] = dp[8 * step + e];
       }
-      Planes<NP> pf, df;
+      Planes<NP> pf, df, pf_rest, df_rest;
       planes_of(x, pf);
       planes_of(y, df);
+      if (kTwoParts) pf_rest = rest_of(x, pf), df_rest = rest_of(y, df);
 #pragma unroll
       for (int d = 0; d < DB; ++d) {
         Planes<NP> gc = Tile::cols(gs, lc, 16 * step, d);
         if (kPartial && bad) gc = finite_part<NP>(gc);
         av[d] = mma(gc, pf, av[d]);
+        if (kTwoParts) av[d] = mma(gc, pf_rest, av[d]);
         Planes<NP> qc = Tile::cols(qs, lc, 16 * step, d);
         if (kPartial && bad) qc = finite_part<NP>(qc);
         ak[d] = mma(qc, df, ak[d]);
+        if (kTwoParts) ak[d] = mma(qc, df_rest, ak[d]);
       }
     }
   };
@@ -676,6 +698,7 @@ template <typename T, int DP, int WM, int KW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, AttnTiles kv,
                                                                                              int64_t tiles, int splits, float* part, T* gq) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = WM > 1 && NP == 1 ? 64 : 32;
+  constexpr bool kTwoParts = NP == 1 && WM == 1;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];
@@ -758,13 +781,15 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = s[8 * step + e];
-        Planes<NP> df;
+        Planes<NP> df, rest;
         planes_of(y, df);
+        if (kTwoParts) rest = rest_of(y, df);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           Planes<NP> kc = Tile::cols(ks_, lc, jb + 16 * step, d);
           if (kLast && CAUSAL && bad) kc = finite_part<NP>(kc);
           o[d] = mma(kc, df, o[d]);
+          if (kTwoParts) o[d] = mma(kc, rest, o[d]);
         }
       }
     }
@@ -914,18 +939,22 @@ enum AttnShape { kNarrow, kMid, kWide };
 AttnShape shape_of(bool f32, int dim, int64_t rows, int heads, int segments) {
   const int64_t blocks = rows / 32 * heads;
   if (rows < (int64_t)(f32 && dim <= 64 ? 192 : 64) * segments) return kNarrow;
-  if (blocks >= (dim <= 64 ? 1024 : f32 ? 192 : 384)) return kWide;
+  if (blocks >= (dim <= 64 ? (f32 ? 1024 : 900) : f32 ? 192 : 384)) return kWide;
   return f32 && dim <= 64 && blocks >= (dim <= 32 ? 384 : 224) ? kMid : kNarrow;
 }
 
 constexpr int shape_rows(AttnShape s) { return s == kWide ? 128 : s == kMid ? 64 : 32; }
 
-// About one query per segment, and enough segments to fill the card with a wave each: the row kernels. The more segments,
-// the longer a wave may take over one. Measured, 4 heads of 32, us of forward + VJP on the row kernels (tiles):
-//   fp32: 10 000 segments of 18 keys 103 (1 004), 256 of 128 39 (61), 256 of 400 114 (100), 2 000 of 400 504 (762), 1 024 of
-//   500 338 (455); bf16: 54 (456), 42 (49), 115 (113), 269 (845), 224 (520)
+// About one query per segment, and enough segments to fill the card with a wave each or so few keys that a tile is mostly
+// empty: the row kernels. The more segments, the longer a wave may take over one. Measured, us of forward + VJP on the row
+// kernels (tiles):
+//   4 heads of 32, fp32: 10 000 segments of 18 keys 103 (1 004), 256 of 128 39 (61), 256 of 400 114 (100), 2 000 of 400 504 (762),
+//   1 024 of 500 338 (455); bf16: 54 (456), 42 (49), 115 (113), 269 (845), 224 (520)
+//   8 heads of 128, fp32: 153 segments of 21 keys 47 (240), of 64 104 (223), of 128 202 (404); bf16 47 (150), 113 (216), 212 (236);
+//   8 heads of 32, 40 of 21 44 (48)
 bool few_rows(int64_t tq, int64_t tk, int segments, int kv_heads) {
-  return segments >= 256 && tq <= segments && tk <= (int64_t)(segments >= 1024 ? 512 : 128) * segments;
+  const int64_t keys = segments >= 1024 ? 512 : segments >= 256 ? 128 : 64;
+  return tq <= segments && tk <= keys * segments;
 }
 
 // Key splits of the forward: as many as bring the workgroups to one per CU, each with kSplitKeys keys at least of a
