@@ -926,7 +926,8 @@ int64_t tile_count(int64_t rows, int group, int segments, int bm) { return rows 
 // 32 rows and share the keys, for calls with too few tiles to fill the card otherwise and segments not much longer than a
 // tile. kMid: two and two, fp32 only, whose narrow form splits every tile into planes in the wave that reads it (fp32 heads
 // above 64 have room in LDS for wide tiles alone, and two narrow waves).
-// Measured, us of forward + both halves of the VJP:
+// Measured, us of forward + both halves of the VJP (bf16 narrow with weights in one part; the second adds 5 to 10 %, a quarter to
+// gk and gv at 1 000 blocks of 64 columns):
 //   one segment, bf16, 8 heads of 64: 2 000 rows narrow 87, wide 127; 4 000 rows 253, 245; 8 000 rows 868, 722
 //   ", 8 heads of 128: 1 000 rows 77, 110; 2 000 rows 227, 183; 4 000 rows 795, 372
 //   ", fp32, 4 heads of 32: 2 000 rows narrow 122, mid 135, wide 142; 4 000 rows 325, 300, 436; 8 000 rows 1 157, 913, 1 063
