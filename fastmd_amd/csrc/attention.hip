@@ -16,11 +16,11 @@ namespace {
 // one it puts the sums into accumulation registers and moves them out and back at every rescaling.
 static constexpr int attn_waves(int planes, int dp, int sums) { return planes * dp * sums <= 192 ? 2 : 1; }
 
-// bf16 weights (P, dS) in the calls of the narrow shape, WM = 1, are two bf16 parts, the second what the rounding of the first
-// dropped: a product more of five, where few rows with few keys each may make most of a result and the rounding of their
-// weights does not average out (gq of 245 causal rows of 24 heads of 16: 1.5 times the error of rounding the result alone, now
-// 1.0). It costs 45 -> 48 us forward and 106 -> 110 VJP at 801 queries over 12 003 keys of 8 heads on 2 of 128, nothing where
-// memory bounds (16 x 40 000 keys: 235 us).
+// bf16 weights (P, dS) are two bf16 parts, the second what the rounding of the first dropped (16 bits together): a product more
+// of two forward, of three for gq and two more of four for gk and gv. With one part the rounding of the weights is as large as that of the
+// result, however many keys a row has (the terms' errors and the terms add up alike), and the results were 1.4 times as far from
+// the exact ones as those rounded once; with two they are as near. It costs 308 -> 430 us at 10 000 rows of 8 heads of 64, 261 -> 374
+// in prompts of 12 000 causal rows of 16 heads of 128, forward and VJP of 8 192 such rows 535 -> 674; where memory bounds, nothing.
 template <int NP>
 __device__ __forceinline__ Planes<NP> rest_of(const float (&x)[8], const Planes<NP>& first) {
   float y[8];
@@ -37,8 +37,8 @@ __device__ __forceinline__ Planes<NP> rest_of(const float (&x)[8], const Planes<
 // tiles kw, kw + KW, ... of its split; the KW partial softmaxes are joined through LDS at the end. The scores are
 // formed transposed, S^T = K Q^T (lane: a query, registers: keys), so the softmax statistics are one value per lane, the
 // sums over keys stay in the lane but for one exchange of the halves, and exp(S^T) is already the operand of
-// O^T = V^T P^T. Statistics and sums are fp32; P is rounded to bf16 for bf16 inputs (the output is, too) and kept as
-// three planes for fp32.
+// O^T = V^T P^T. Statistics and sums are fp32; P is kept in two bf16 parts for bf16 inputs and as three planes
+// for fp32.
 // Measured: bf16, 10 000 rows, 8 heads of 64: 281 us, 727 TFLOP/s (a large library product 1 125): the matrix pipes are busy
 // 37 % of the time, the vector ones with the exponentials (quarter rate), their arguments, maxima and sums for most of the rest, and
 // waves of a SIMD overlap the two in part. 5 prompts of 12 000 causal rows together, 16 heads of 128: 242 us, 870 TFLOP/s. fp32,
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
                                                                 int64_t tiles, int splits, T* out, AttnSaved saved,
                                                                 float* part_o, float* part_m, float* part_l) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, JB = BN / 32;
-  constexpr bool kTwoParts = NP == 1 && WM == 1;
+  constexpr bool kTwoParts = NP == 1;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kMerge = (KW - 1) * WM * (DB * 16 + 2) * 64 * 2;  // in bf16 units
   constexpr int kTiles = 2 * KW * Tile::SIZE;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // Gradients of keys and values. One workgroup: 32 WM keys of one key head; wave (wm, rw) holds 32 keys and walks the
 // tiles rw, rw + RW, ... of 32 queries, of one query head of the group after the other. S = Q K^T (lane: a key, registers:
 // query rows), so exp(S - lse) and dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of
-// the group. For bf16, P and dS are rounded to bf16 as those operands (the gradients are, too); sums are fp32.
+// the group. For bf16, P and dS are operands in two bf16 parts; sums are fp32.
 // Measured: bf16, causal, 4 sequences of 8 192 rows together, 16 heads on 4 of 128: 216 us, 680 TFLOP/s, matrix pipes busy 38 % of
 // the time: two waves a SIMD, for which the two sums take half of the registers, wait on each other's rounds. fp32, 5 systems of
 // 5 000 rows, 4 heads of 64: 145 us, 112 TFLOP/s. Two waves of keys and four of rows in one workgroup, so that a tile's copy
@@ -404,7 +404,7 @@ template <typename T, int DP, int WM, int RW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
                                                                                               int splits, float* part, T* gk, T* gv) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BR = 32;
-  constexpr bool kTwoParts = NP == 1 && WM == 1;
+  constexpr bool kTwoParts = NP == 1;
   using Tile = AttnTile<NP, BR, DP>;
   constexpr int kStats = NP == 3 ? 4 * BR : 2 * BR;  // offset, delta (inverse and nothing) of BR rows
   constexpr int kGroup = 2 * Tile::SIZE + 2 * kStats;  // in bf16 units
@@ -692,13 +692,13 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     }
 }
 
-// Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T (dS rounded to bf16 for
+// Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T (dS in two parts for
 // bf16). Measured in the cases above: bf16 128 us, 855 TFLOP/s, matrix pipes busy 48 % of the time; fp32 110 us, 112 TFLOP/s.
 template <typename T, int DP, int WM, int KW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, AttnTiles kv,
                                                                                              int64_t tiles, int splits, float* part, T* gq) {
   constexpr int NP = AttnType<T>::planes, DB = DP / 32, KS = DP / 16, BN = WM > 1 && NP == 1 ? 64 : 32;
-  constexpr bool kTwoParts = NP == 1 && WM == 1;
+  constexpr bool kTwoParts = NP == 1;
   using Tile = AttnTile<NP, BN, DP>;
   constexpr int kTiles = 2 * KW * Tile::SIZE, kMerge = (KW - 1) * WM * 16 * 64 * 2;
   __shared__ __attribute__((aligned(16))) __bf16 lds[kTiles > kMerge ? kTiles : kMerge];

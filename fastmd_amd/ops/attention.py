@@ -15,8 +15,8 @@ causal query does not see reaches it (nor, in the VJP, one in a query's row the 
 
 float32 is computed on the bf16 matrix cores with every operand split into three planes (float32 accuracy; an
 infinite value in a row that is seen gives NaN), bfloat16 with products of bfloat16 operands. Scores, softmax statistics
-and sums are float32 in both. For bfloat16, the probabilities and (in the VJP) the score gradients are rounded to
-bfloat16 as operands of the second product, as the inputs and outputs are (small calls keep them in two bfloat16 parts).
+and sums are float32 in both. For bfloat16, the probabilities and (in the VJP) the score gradients are operands of the
+second product in two bfloat16 parts (16 bits), so that each result is as near to the exact one as its one rounding allows.
 Gradients take no atomics: the same call gives the same bits.
 """
 from __future__ import annotations
