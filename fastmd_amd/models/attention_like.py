@@ -15,7 +15,8 @@ Sums over a system's atoms are softmax-weighted means, so the energy is extensiv
 atoms. Random init from ``torch.Generator().manual_seed(seed)``; parameters are frozen as those of the other models are, and
 ``module.requires_grad_()`` trains them (``node_energy`` is differentiable in them).
 
-A union of systems is one call: the systems are the segments, and the vacant rows of a slot are segments of their own.
+A union of systems, or of replicas of one, is one call: the systems are the segments, and the vacant rows of a slot are
+segments of their own.
 """
 from __future__ import annotations
 
@@ -108,7 +109,7 @@ class AttentionInput:
     batch: GraphBatch
     elem: Tensor  # [rows] int64
     columns: Tensor  # [elements, elements] float32 identity
-    rows: Tensor  # [0, rows]: the one system's offsets
+    rows: Tensor  # offsets of the one system's rows, or of equal replicas'
 
 
 class _Surroundings(Function):
@@ -182,7 +183,10 @@ class AttentionAdapter:
         if bool(((species < 1) | (species > _ELEMENTS)).any()) or bool((table[species.clamp(1, _ELEMENTS)] < 0).any()):
             raise ValueError(f"the attention model supports atomic numbers {list(self.module.config.elements)}")
         columns = torch.eye(len(self.module.config.elements), dtype=torch.float32, device=species.device)
-        rows = torch.tensor([0, batch.n_real], dtype=torch.int64, device=species.device)
+        size = getattr(batch, "max_system_rows", 0) or batch.n_real or 1  # of a replica, or of the one system
+        if getattr(batch, "systems", None) is None and batch.n_real % size:
+            raise ValueError(f"{batch.n_real} atom rows are not whole replicas of {size}")
+        rows = torch.arange(0, batch.n_real + 1, size, dtype=torch.int64, device=species.device)
         return AttentionInput(batch, table[species].long(), columns, rows)
 
     @staticmethod
