@@ -13,7 +13,7 @@ Model (atom features x [N, C], H query heads on Hk key heads of width D):
   readout:   E_i = e0[Z_i] + x_i . wr
 Sums over a system's atoms are softmax-weighted means, so the energy is extensive and does not depend on the order of the
 atoms. Random init from ``torch.Generator().manual_seed(seed)``; parameters are frozen as those of the other models are, and
-``module.requires_grad_()`` trains them (``node_energy`` is differentiable in them).
+``module.requires_grad_()`` trains them (``node_energy`` is differentiable once: losses on energies, not on forces).
 
 A union of systems, or of replicas of one, is one call: the systems are the segments, and the vacant rows of a slot are
 segments of their own.
@@ -28,6 +28,7 @@ from torch import Tensor, nn
 from torch.autograd import Function
 
 from fastmd_amd import _abi
+from fastmd_amd._autograd import first_derivatives
 from fastmd_amd.adapters.protocol import (CapacityStep, GraphBatch, PaddingRule, TopologySpec, require_atom_rows,
                                          system_rows)
 from fastmd_amd.ops.attention import segment_attention
@@ -118,6 +119,7 @@ class _Surroundings(Function):
     @staticmethod
     def forward(ctx, positions, cell, model: AttentionLike, inputs: AttentionInput):
         cfg, batch, dev = model.config, inputs.batch, positions.device
+        ctx.save_for_backward(positions)
         positions = positions.detach().contiguous()
         cell = cell.detach().to(torch.float32).contiguous()
         e_cap, nb, n = batch.edge_index.shape[0], cfg.n_basis, positions.shape[0]
@@ -145,6 +147,7 @@ class _Surroundings(Function):
         _abi.call("fmd_edge_forces_f32", geo.data_ptr(), de.data_ptr(), nb, gef.data_ptr(), nb, None, 0, None,
                   batch.edge_offsets.data_ptr(), batch.edge_reverse.data_ptr(), batch.n_edges.data_ptr(), e_cap, ctx.n,
                   1.0, gpos.data_ptr(), None, _abi.stream_handle())
+        (gpos,) = first_derivatives("the attention model's energy", (gpos,), g, *ctx.saved_tensors)
         return gpos, None, None, None
 
 

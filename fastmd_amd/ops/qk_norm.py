@@ -19,6 +19,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from fastmd_amd import _abi
+from fastmd_amd._autograd import first_derivatives
 from fastmd_amd._device import require_cuda, stream
 from fastmd_amd.ops.attention import heads_view
 
@@ -181,7 +182,8 @@ class _NormRotary(Function):
         if k is not None and gk is None:
             gk = torch.zeros_like(k)
         grads = _vjp(gq, gk, q, k, *rest, *ctx.options, ctx.needs_input_grad[2] or ctx.needs_input_grad[3])
-        return (*grads, None, None, None, None, None, None)
+        inputs = (gq, gk, q, k, rest[0], rest[1])
+        return (*first_derivatives("qk_norm_rotary", grads, *inputs), None, None, None, None, None, None)
 
 
 def _apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm):
@@ -197,7 +199,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
     """Norm and rotation of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (float32 or bfloat16, any strides: columns of
     a packed projection are read in place) in one launch; weights [dim] of their type (None: ones), shared by the
     heads. Tables without columns give the norm alone. A position outside the tables gives NaN in the turned columns.
-    Differentiable in q, k and the weights."""
+    Differentiable once in q, k and the weights."""
     _check(q, k, q_weight, k_weight, cos, sin, positions)
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
@@ -214,6 +216,6 @@ def qk_norm_rotary_vjp(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, q_weight: T
 
 
 def rotary(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor | None = None, *, interleaved: bool = False) -> Tensor:
-    """The rotation alone, of x [tokens, heads, dim]. Differentiable in x."""
+    """The rotation alone, of x [tokens, heads, dim]. Differentiable once in x."""
     _check(x, None, None, None, cos, sin, positions)
     return _apply(x, None, None, None, cos, sin, positions, 0.0, bool(interleaved), False)[0]
