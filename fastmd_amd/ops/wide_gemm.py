@@ -509,6 +509,22 @@ def gemm_gather(parts, b: Tensor, *, out: Tensor | None = None, bias: Tensor | N
     return out
 
 
+class _InputGradient(Function):
+    """``gy @ weight`` as an operation of its own, for gradients that are differentiated again."""
+
+    @staticmethod
+    def forward(ctx, gy, weight):
+        ctx.save_for_backward(gy, weight)
+        return gemm(gy, weight, b_layout=1)
+
+    @staticmethod
+    def backward(ctx, g):
+        gy, weight = ctx.saved_tensors
+        g = g.contiguous()
+        return (linear(g, weight) if ctx.needs_input_grad[0] else None,
+                gy.t().mm(g) if ctx.needs_input_grad[1] else None)
+
+
 class _Linear(Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -521,7 +537,9 @@ class _Linear(Function):
     def backward(ctx, gy):
         x, weight = ctx.saved_tensors
         gy = gy.contiguous()
-        gx = gemm(gy, weight, b_layout=1) if ctx.needs_input_grad[0] else None
+        gx = None
+        if ctx.needs_input_grad[0]:
+            gx = _InputGradient.apply(gy, weight) if torch.is_grad_enabled() else gemm(gy, weight, b_layout=1)
         # trainable weights are outside the MD path (the reference declines them too,
         # triton_wide_gemm.py:242-243): their gradient is formed by torch
         gw = gy.t().mm(x) if ctx.needs_input_grad[1] else None

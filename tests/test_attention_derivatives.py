@@ -87,3 +87,22 @@ def test_a_loss_on_the_models_forces_raises(device):
     (gradient,) = torch.autograd.grad(energy, positions, create_graph=True)
     with pytest.raises(NotImplementedError, match="first derivatives only"):
         (energy + (gradient ** 2).sum()).backward()
+
+
+@pytest.mark.gpu
+def test_second_derivatives_of_the_linear_layer(device):
+    """A penalty on the input's gradient beside the value, against float64: sums of 40 products of order one, to 1e-5."""
+    from fastmd_amd.ops.wide_gemm import linear
+
+    def grads(x, w, b, layer):
+        y = layer(x, w, b)
+        value = (y ** 3).sum()
+        (gx,) = torch.autograd.grad(value, x, create_graph=True)
+        return gx, *torch.autograd.grad(0.1 * value + (gx ** 2).sum(), (x, w, b))
+
+    gen = torch.Generator().manual_seed(6)
+    data = [0.2 * torch.randn(*s, generator=gen) for s in ((50, 24), (40, 24), (40,))]
+    want = grads(*[t.double().requires_grad_() for t in data], torch.nn.functional.linear)
+    got = grads(*[t.to(device).requires_grad_() for t in data], linear)
+    for a, b in zip(got, want):
+        assert float((a.double().cpu() - b).abs().max()) < 1e-5 * float(b.abs().max())
