@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 
 
 class _FirstOnly(Function):
@@ -26,3 +26,13 @@ def first_derivatives(name: str, grads: tuple, *inputs: Tensor | None) -> tuple:
     if not torch.is_grad_enabled() or not any(x is not None and x.requires_grad for x in inputs):
         return grads
     return _FirstOnly.apply(name, len(grads), *grads, *inputs)
+
+
+def differentiated(*tensors: Tensor | None) -> bool:
+    """Whether a call on these tensors belongs to autograd: gradients are wanted, or one of them carries a tangent (for which
+    an autograd function without a forward-mode rule raises)."""
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in tensors):
+        return True
+    if forward_ad._current_level < 0:  # outside every dual level, as nearly always
+        return False
+    return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)

@@ -30,7 +30,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from fastmd_amd import _abi
-from fastmd_amd._autograd import first_derivatives
+from fastmd_amd._autograd import differentiated, first_derivatives
 from fastmd_amd._device import require_cuda, stream
 
 MAX_DIM = 128
@@ -223,7 +223,7 @@ def segment_attention(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offs
     """Attention within segments (see the module): ``q`` [rows, heads, dim], ``k`` and ``v`` [key rows, kv_heads, dim],
     float32 or bfloat16, any strides; offsets [segments + 1] on the device (``k_offsets`` None: ``q_offsets``); ``scale``
     None: ``dim ** -0.5``. One query per segment (the next token of a sequence over its cache, an atom over its neighbours) is the
-    same call: a long key axis is then split over the card and joined. Differentiable once in q, k and v."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    same call: a long key axis is then split over the card and joined. Differentiable once in q, k and v, in reverse mode."""
+    if differentiated(q, k, v):
         return _SegmentAttention.apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
     return _forward(q, k, v, q_offsets, k_offsets, causal, scale, False)[0]

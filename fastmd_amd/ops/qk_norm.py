@@ -19,7 +19,7 @@ from torch import Tensor
 from torch.autograd import Function
 
 from fastmd_amd import _abi
-from fastmd_amd._autograd import first_derivatives
+from fastmd_amd._autograd import differentiated, first_derivatives
 from fastmd_amd._device import require_cuda, stream
 from fastmd_amd.ops.attention import heads_view
 
@@ -187,7 +187,7 @@ class _NormRotary(Function):
 
 
 def _apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm):
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
+    if differentiated(q, k, q_weight, k_weight):
         out = _NormRotary.apply(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm)
         return (out, None) if k is None else out
     return _forward(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, norm)
@@ -199,7 +199,8 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
     """Norm and rotation of q [tokens, heads, dim] and k [tokens, kv_heads, dim] (float32 or bfloat16, any strides: columns of
     a packed projection are read in place) in one launch; weights [dim] of their type (None: ones), shared by the
     heads. Tables without columns give the norm alone. A position outside the tables gives NaN in the turned columns.
-    Differentiable once in q, k and the weights."""
+    Differentiable once in q, k and the weights, in reverse
+    mode."""
     _check(q, k, q_weight, k_weight, cos, sin, positions)
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
@@ -216,6 +217,6 @@ def qk_norm_rotary_vjp(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, q_weight: T
 
 
 def rotary(x: Tensor, cos: Tensor, sin: Tensor, positions: Tensor | None = None, *, interleaved: bool = False) -> Tensor:
-    """The rotation alone, of x [tokens, heads, dim]. Differentiable once in x."""
+    """The rotation alone, of x [tokens, heads, dim]. Differentiable once in x, in reverse mode."""
     _check(x, None, None, None, cos, sin, positions)
     return _apply(x, None, None, None, cos, sin, positions, 0.0, bool(interleaved), False)[0]

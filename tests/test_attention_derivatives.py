@@ -106,3 +106,21 @@ def test_second_derivatives_of_the_linear_layer(device):
     got = grads(*[t.to(device).requires_grad_() for t in data], linear)
     for a, b in zip(got, want):
         assert float((a.double().cpu() - b).abs().max()) < 1e-5 * float(b.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("operator", [_attention, _norm, _rotary])
+def test_forward_mode_raises(operator):
+    """An input with a tangent, none that wants a gradient; outside the dual level the call is as ever."""
+    from torch.autograd import forward_ad
+
+    leaves, call = operator()
+    leaves = [x.detach() for x in leaves]
+    want = call(*leaves)
+    for n in range(len(leaves)):
+        with forward_ad.dual_level():
+            assert torch.equal(call(*leaves), want)
+            dual = [forward_ad.make_dual(x, torch.ones_like(x)) if i == n else x for i, x in enumerate(leaves)]
+            with pytest.raises((NotImplementedError, RuntimeError), match="jvp|forward"):
+                call(*dual)
+    assert torch.equal(call(*leaves), want)
