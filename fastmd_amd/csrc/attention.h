@@ -9,6 +9,7 @@
 // bf16 operands as one.
 #pragma once
 
+#include "attention_find.h"
 #include "common.h"
 #include "x3.h"
 
@@ -54,41 +55,10 @@ struct AttnTiles {
 constexpr int kWaitVm0 = 0 | (7 << 4) | (15 << 8);  // s_waitcnt vmcnt(0)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// A segment with its rows. The kernels see segments + 2 of them: the rows before the first offset and after the
-// last one (a fixed-capacity buffer's unused rows) are segments of their own without keys, or without queries.
 struct AttnSegment {
   int64_t q0, k0;
   int32_t nq, nk;
 };
-
-// start of extended segment i in 0 .. n + 2, with every offset clamped into the buffer
-__device__ __forceinline__ int64_t attn_start(const int64_t* off, int n, int64_t rows, int i) {
-  if (i == 0) return 0;
-  if (i == n + 2) return rows;
-  const int64_t o = off[i - 1];
-  return o < 0 ? 0 : o > rows ? rows : o;
-}
-
-// The tile of `bm` packed rows (rows * group of them) with number t: extended segment i owns the numbers from
-// floor(start(i) * group / bm) + i on, at least as many as it has tiles, so no table of tiles is needed and the grid
-// (rows * group / bm + segments + 2) is known without reading the offsets. The search probes 64 places at a time.
-// Returns the extended segment and the tile's first packed row in it; a number without a tile has first row >= rows.
-__device__ __forceinline__ int attn_find(const int64_t* off, int n, int64_t rows, int group, int bm, int64_t t,
-                                         int64_t* first) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, count = n + 2;
-  while (count > 1) {
-    const int step = (count + 63) >> 6;
-    const int i = lo + lane * step;
-    const bool at = lane * step < count && attn_start(off, n, rows, i) * group / bm + i <= t;
-    const int hits = __popcll(__ballot(at));
-    const int adv = (hits > 0 ? hits - 1 : 0) * step;
-    lo += adv;
-    count = count - adv < step ? count - adv : step;
-  }
-  *first = (t - (attn_start(off, n, rows, lo) * group / bm + lo)) * bm;
-  return lo;
-}
 
 __device__ __forceinline__ AttnSegment attn_segment(const AttnArgs& a, int i) {
   AttnSegment s;

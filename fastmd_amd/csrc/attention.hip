@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   int64_t t = blockIdx.x / a.kv_heads;
   if (CAUSAL) t = tiles - 1 - t;  // the rows with the most keys first
   int64_t first;
-  const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first);
+  const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first, WaveLanes());
   AttnSegment sg = attn_segment(a, ext);
   if (!attn_real(a, ext)) sg.nk = 0;
   const int rows = sg.nq * a.group;
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   const int wm = wave % WM, rw = wave / WM;
   const int kvh = blockIdx.x % a.kv_heads;
   int64_t first;
-  const int ext = attn_find(a.k_off, a.segments, a.tk, 1, 32 * WM, blockIdx.x / a.kv_heads, &first);
+  const int ext = attn_find(a.k_off, a.segments, a.tk, 1, 32 * WM, blockIdx.x / a.kv_heads, &first, WaveLanes());
   AttnSegment sg = attn_segment(a, ext);
   if (!attn_real(a, ext)) sg.nq = 0;
   if (first >= sg.nk) return;
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   int64_t t = blockIdx.x / a.kv_heads;
   if (CAUSAL) t = tiles - 1 - t;
   int64_t first;
-  const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first);
+  const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first, WaveLanes());
   AttnSegment sg = attn_segment(a, ext);
   if (!attn_real(a, ext)) sg.nk = 0;
   const int rows = sg.nq * a.group;

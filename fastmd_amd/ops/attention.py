@@ -5,7 +5,7 @@
     out[i, h] = sum_j softmax_j(scale * q[i, h] . k[j, h // group]) v[j, h // group]
 
 over the key rows j of query i's segment. Segment s has the query rows ``[q_offsets[s], q_offsets[s + 1])`` and the
-key rows ``[k_offsets[s], k_offsets[s + 1])``; the offsets are those of a CSR over sorted rows (the atoms of each system
+key rows ``[k_offsets[s], k_offsets[s + 1])``; the offsets, which ascend, are those of a CSR over sorted rows (the atoms of each system
 of a batch, the neighbour rows of each atom, packed sequences), read on the device only: a call neither
 synchronises nor depends on lengths that the host would have to know. ``group = heads / kv_heads`` query heads share a
 key head. ``causal``: the last query of a segment sees all its keys, each one before it one key less. A query that sees

@@ -820,7 +820,8 @@ int fmd_edge_stress_f32(const float* geo, const float* gvec, const int64_t* n_ed
 
 /* out[i, h] = sum_j softmax_j(scale q[i, h] . k[j, h / (heads / kv_heads)]) v[j, .] over the key rows j of query i's
  * segment: segment s has the query rows [q_offsets[s], q_offsets[s + 1]) and the key rows
- * [k_offsets[s], k_offsets[s + 1]) (device int64, ascending; every offset is clamped into the buffer). causal: query i of
+ * [k_offsets[s], k_offsets[s + 1]) (device int64, ascending; every offset is clamped into the buffer; where offsets
+ * descend all the same, nothing outside the buffers is touched, but which rows are computed is open). causal: query i of
  * n sees the first i + m - n + 1 of the m keys. A query that sees no key, and one outside every segment, gives zero.
  * q [tq, heads, dim], k and v [tk, kv_heads, dim] with row and head strides in elements (unit stride in dim, 16-byte
  * aligned rows); dim a multiple of 8 up to 128 (FMD_EUNSUPPORTED otherwise); scale > 0. out [tq, heads, dim] contiguous.
