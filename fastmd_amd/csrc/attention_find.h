@@ -51,3 +51,26 @@ __host__ __device__ __forceinline__ int attn_find(const int64_t* off, int n, int
   *first = tile < 0 ? INT64_MAX : tile * bm;
   return i;
 }
+
+// The row kernels give a segment to one wave. One of kLongQueries queries or kLongKeys keys and more, whatever the mean over all
+// segments is, is dealt out over workgroups instead: its share of numbers from floor(q / kLongQueries) + floor(k / kLongKeys) on,
+// q and k its first rows, at least one. The grid (tq / kLongQueries + tk / kLongKeys) is known without reading the offsets. Nearly always
+// they find no such segment: us of forward, VJP without them and with, and with four times as many for the queries: 10 000 segments of 18 keys,
+// 4 heads of 32, bf16 20, 34; 20, 34; 22, 36; 100 000 of 20 keys 191, 378; 208, 392; 232, 425, fp32 380, 850; 389, 865; 412, 895. (Between the
+// rows' workgroups instead of after them they shift those from one CU to another: 1 024 segments of 500 keys, VJP 225; 226; 315.)
+constexpr int kLongQueries = 32, kLongKeys = 1024;
+
+__host__ __device__ __forceinline__ bool attn_long(int nq, int nk) { return nq >= kLongQueries || nk >= kLongKeys; }
+__host__ __device__ __forceinline__ int64_t attn_long_numbers(int64_t tq, int64_t tk) { return tq / kLongQueries + tk / kLongKeys; }
+
+// The extended segment of number t, and which of its parts the number is (part >= parts: none).
+template <typename Lanes>
+__host__ __device__ __forceinline__ int attn_share(const int64_t* q_off, const int64_t* k_off, int n, int64_t tq, int64_t tk, int64_t t,
+                                                   int64_t* part, int64_t* parts, const Lanes& lanes) {
+  const auto number = [&](int i) { return attn_long_numbers(attn_start(q_off, n, tq, i), attn_start(k_off, n, tk, i)); };
+  const int i = attn_last(n + 2, t, number, lanes);
+  *part = t - number(i);
+  *parts = *part < 0 ? 0 : number(i + 1) - number(i);
+  if (*part < 0) *part = 0;
+  return i;
+}

@@ -1,7 +1,8 @@
 // Segment attention of about one query per segment over a few keys each (an atom over its neighbour rows), and its VJP:
 // memory-bound, on the vector units, in fp32.
 //
-// One wave per segment and block of key heads. A unit of D / 8 lanes (a power of two) takes one key row of one head, eight
+// One wave per segment and block of key heads, but for long segments (attn_long): a wave's work is bounded whatever the offsets
+// are (2 048 slots, one of 1 500 queries over as many keys, 4 heads of 32, fp32: 0.95 ms forward, 2.5 VJP). A unit of D / 8 lanes (a power of two) takes one key row of one head, eight
 // columns a lane; the units of a wave lie along the heads (a row's heads are contiguous) and then along keys. Every key row is
 // read once and, in the VJP of a single query, its two gradients are written in the same pass. The matrix kernels spend a
 // tile of 32 rows on such a segment's single one. 10 000 segments, 180 096 keys, 4 heads of 32: 35 + 75 us forward and VJP in
@@ -60,11 +61,140 @@ __device__ __forceinline__ void clear_outside(const int64_t* off, int segments, 
   }
 }
 
+// One query row over the keys first, first + step, ... below `sees`, for G heads of its group: their weighted values, maxima and sums,
+// joined over the wave's key slots.
+template <typename T, int LG, int G>
+struct RowSoftmax {
+  float o[G][8], m[G], l[G];
+
+  __device__ __forceinline__ void walk(const AttnArgs& a, const RowLane& r, const AttnSegment& sg, int i, int head, uint32_t first,
+                                       uint32_t step) {
+    const uint32_t sees = a.causal ? max(0, min(sg.nk, i + sg.nk - sg.nq + 1)) : sg.nk;
+    const float c = a.scale * kLog2e;
+    const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + r.kvh * a.k_head + r.col;
+    const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + r.kvh * a.v_head + r.col;
+    const T* qp = static_cast<const T*>(a.q) + (sg.q0 + i) * a.q_row + head * a.q_head + r.col;
+    float q[G][8];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      zero8(q[g]);
+      zero8(o[g]);
+      if (r.on) load8<T>(qp + g * a.q_head, q[g]);
+      m[g] = -INFINITY;
+      l[g] = 0.f;
+    }
+    for (uint32_t j = first; j < sees; j += step) {
+      float k[8], v[8];
+      zero8(k);
+      zero8(v);
+      if (r.on) {
+        load8<T>(kb + j * a.k_row, k);
+        load8<T>(vb + j * a.v_row, v);
+      }
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float s = lanes_sum<LG>(dot8(q[g], k)) * c;
+        const float top = fmaxf(m[g], s), shift = top == -INFINITY ? 0.f : top;
+        const float fade = exp2_hw(m[g] - shift), p = exp2_hw(s - shift);
+        l[g] = fmaf(l[g], fade, p);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[g][e] = fmaf(o[g][e], fade, p * v[e]);
+        m[g] = top;
+      }
+    }
+    for (int by = r.stride; by < 64; by *= 2) {  // the key slots of a head
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        float oo[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) oo[e] = __shfl_xor(o[g][e], by, 64);
+        const float om = __shfl_xor(m[g], by, 64), ol = __shfl_xor(l[g], by, 64);
+        join(g, om, ol, oo);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void join(int g, float om, float ol, const float (&oo)[8]) {
+    const float top = fmaxf(m[g], om), shift = top == -INFINITY ? 0.f : top;
+    const float fa = exp2_hw(m[g] - shift), fb = exp2_hw(om - shift);
+    l[g] = l[g] * fa + ol * fb;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[g][e] = o[g][e] * fa + oo[e] * fb;
+    m[g] = top;
+  }
+
+  __device__ __forceinline__ void store(const AttnArgs& a, const RowLane& r, int64_t row, int head, int g, T* out, const AttnSaved& saved) {
+    const float inv = l[g] > 0.f || l[g] != l[g] ? 1.f / l[g] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[g][e] *= inv;
+    const int64_t at = (row * a.heads + head + g) * a.dim + r.col;
+    store8<false>(out + at, o[g]);
+    saved_residual<T>(saved, at, o[g]);
+    if (saved.base && r.col == 0) {
+      const int64_t s = (head + g) * a.tq + row;
+      saved.base[s] = m[g] == -INFINITY ? 0.f : m[g];
+      saved.inverse[s] = inv;
+    }
+  }
+};
+
+// The part of a long segment that a workgroup past the `row_blocks` takes: its queries part, part + parts, ..., with the keys of each dealt
+// out to its four waves.
+struct LongPart {
+  AttnSegment sg;
+  int64_t part, parts;
+  int head_block;
+  bool any;
+};
+
+__device__ __forceinline__ LongPart long_part(const AttnArgs& a, int64_t number, int head_blocks) {
+  LongPart p;
+  p.head_block = (int)(number % head_blocks);
+  const int i = attn_share(a.q_off, a.k_off, a.segments, a.tq, a.tk, number / head_blocks, &p.part, &p.parts, WaveLanes());
+  p.sg = attn_segment(a, i);
+  p.any = attn_real(a, i) && attn_long(p.sg.nq, p.sg.nk) && p.part < p.parts;
+  return p;
+}
+
 // GF: query heads taken together (the whole group); 0: one after the other, with a walk over the keys each
 template <typename T, int LG, int GF>
-__global__ void __launch_bounds__(256) attn_rows_fwd_kernel(AttnArgs a, int hb, int head_blocks, T* out, AttnSaved saved) {
+__global__ void __launch_bounds__(256) attn_rows_fwd_kernel(AttnArgs a, int hb, int head_blocks, int64_t row_blocks, T* out, AttnSaved saved) {
   constexpr int G = GF ? GF : 1;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  RowSoftmax<T, LG, G> x;
+  if (blockIdx.x >= row_blocks) {
+    __shared__ float part[3][10][64];
+    const LongPart p = long_part(a, blockIdx.x - row_blocks, head_blocks);
+    if (!p.any) return;
+    const RowLane r = row_lane<LG>(a, p.head_block, hb);
+    for (int64_t i = p.part; i < p.sg.nq; i += p.parts)
+      for (int g0 = 0; g0 < a.group; g0 += G) {
+        const int head = r.kvh * a.group + g0;
+        x.walk(a, r, p.sg, (int)i, head, wave * r.slots + r.slot, 4 * r.slots);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          __syncthreads();  // the part before is read
+          if (wave > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) part[wave - 1][e][lane] = x.o[g][e];
+            part[wave - 1][8][lane] = x.m[g];
+            part[wave - 1][9][lane] = x.l[g];
+          }
+          __syncthreads();
+          if (wave == 0) {
+            for (int n = 0; n < 3; ++n) {
+              float o[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) o[e] = part[n][e][lane];
+              x.join(g, part[n][8][lane], part[n][9][lane], o);
+            }
+            if (r.on && r.slot == 0) x.store(a, r, p.sg.q0 + i, head, g, out, saved);
+          }
+        }
+      }
+    return;
+  }
+  const int64_t w = (int64_t)blockIdx.x * 4 + wave;
   const int64_t seg = w / head_blocks;
   const RowLane r = row_lane<LG>(a, (int)(w % head_blocks), hb);
   if (seg >= a.segments) {
@@ -73,72 +203,16 @@ __global__ void __launch_bounds__(256) attn_rows_fwd_kernel(AttnArgs a, int hb, 
     return;
   }
   const AttnSegment sg = attn_segment(a, (int)seg + 1);
-  const float c = a.scale * kLog2e;
-  const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + r.kvh * a.k_head + r.col;
-  const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + r.kvh * a.v_head + r.col;
-  for (int i = 0; i < sg.nq; ++i) {
-    const int sees = a.causal ? max(0, min(sg.nk, i + sg.nk - sg.nq + 1)) : sg.nk;
+  if (attn_long(sg.nq, sg.nk)) return;
+  for (int i = 0; i < sg.nq; ++i)
     for (int g0 = 0; g0 < a.group; g0 += G) {
       const int head = r.kvh * a.group + g0;
-      const T* qp = static_cast<const T*>(a.q) + (sg.q0 + i) * a.q_row + head * a.q_head + r.col;
-      float q[G][8], o[G][8], m[G], l[G];
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        zero8(q[g]);
-        zero8(o[g]);
-        if (r.on) load8<T>(qp + g * a.q_head, q[g]);
-        m[g] = -INFINITY;
-        l[g] = 0.f;
-      }
-      for (int j = r.slot; j < sees; j += r.slots) {
-        float k[8], v[8];
-        zero8(k);
-        zero8(v);
-        if (r.on) {
-          load8<T>(kb + j * a.k_row, k);
-          load8<T>(vb + j * a.v_row, v);
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float s = lanes_sum<LG>(dot8(q[g], k)) * c;
-          const float top = fmaxf(m[g], s), shift = top == -INFINITY ? 0.f : top;
-          const float fade = exp2_hw(m[g] - shift), p = exp2_hw(s - shift);
-          l[g] = fmaf(l[g], fade, p);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[g][e] = fmaf(o[g][e], fade, p * v[e]);
-          m[g] = top;
-        }
-      }
-      for (int by = r.stride; by < 64; by *= 2) {  // the key slots of a head
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float om = __shfl_xor(m[g], by, 64), ol = __shfl_xor(l[g], by, 64);
-          const float top = fmaxf(m[g], om), shift = top == -INFINITY ? 0.f : top;
-          const float fa = exp2_hw(m[g] - shift), fb = exp2_hw(om - shift);
-          l[g] = l[g] * fa + ol * fb;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[g][e] = o[g][e] * fa + __shfl_xor(o[g][e], by, 64) * fb;
-          m[g] = top;
-        }
-      }
+      x.walk(a, r, sg, i, head, r.slot, r.slots);
       if (r.on && r.slot == 0) {
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          const float inv = l[g] > 0.f || l[g] != l[g] ? 1.f / l[g] : 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) o[g][e] *= inv;
-          const int64_t at = ((sg.q0 + i) * a.heads + head + g) * a.dim + r.col;
-          store8<false>(out + at, o[g]);
-          saved_residual<T>(saved, at, o[g]);
-          if (saved.base && r.col == 0) {
-            const int64_t s = (head + g) * a.tq + sg.q0 + i;
-            saved.base[s] = m[g] == -INFINITY ? 0.f : m[g];
-            saved.inverse[s] = inv;
-          }
-        }
+        for (int g = 0; g < G; ++g) x.store(a, r, sg.q0 + i, head, g, out, saved);
       }
     }
-  }
 }
 
 // sum of x over the lanes of all key slots
@@ -162,25 +236,41 @@ __device__ __forceinline__ float delta_part(const AttnBwd& b, int64_t at, const 
 
 // GF: the group, for segments of one query: one pass over the keys forms all three gradients. A segment of another
 // number of queries, and GF = 0, takes a pass per query head for gq and one for gk and gv, whose sums run over all of
-// them in order.
+// them in order; so do the parts of a long segment.
 template <typename T, int LG, int GF, bool NT>
-__global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd b, int hb, int head_blocks, T* gq, T* gk, T* gv) {
+__global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd b, int hb, int head_blocks, int64_t row_blocks, T* gq, T* gk,
+                                                            T* gv) {
   constexpr int G = GF ? GF : 1;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t seg = w / head_blocks;
-  const RowLane r = row_lane<LG>(a, (int)(w % head_blocks), hb);
-  if (seg >= a.segments) {
-    if (seg - a.segments < kTail && w % head_blocks == 0) {
-      const int tail = (int)(seg - a.segments);
-      if (gq) clear_outside<T>(a.q_off, a.segments, a.tq, a.heads * a.dim, tail, gq, nullptr, nullptr, 0);
-      if (gk) {
-        clear_outside<T>(a.k_off, a.segments, a.tk, a.kv_heads * a.dim, tail, gk, nullptr, nullptr, 0);
-        clear_outside<T>(a.k_off, a.segments, a.tk, a.kv_heads * a.dim, tail, gv, nullptr, nullptr, 0);
+  const bool is_long = blockIdx.x >= row_blocks;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  int64_t part = 0, parts = 1;
+  AttnSegment sg;
+  RowLane r;
+  if (is_long) {
+    const LongPart p = long_part(a, blockIdx.x - row_blocks, head_blocks);
+    if (!p.any) return;
+    sg = p.sg;
+    part = p.part;
+    parts = p.parts;
+    r = row_lane<LG>(a, p.head_block, hb);
+  } else {
+    const int64_t w = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t seg = w / head_blocks;
+    r = row_lane<LG>(a, (int)(w % head_blocks), hb);
+    if (seg >= a.segments) {
+      if (seg - a.segments < kTail && w % head_blocks == 0) {
+        const int tail = (int)(seg - a.segments);
+        if (gq) clear_outside<T>(a.q_off, a.segments, a.tq, a.heads * a.dim, tail, gq, nullptr, nullptr, 0);
+        if (gk) {
+          clear_outside<T>(a.k_off, a.segments, a.tk, a.kv_heads * a.dim, tail, gk, nullptr, nullptr, 0);
+          clear_outside<T>(a.k_off, a.segments, a.tk, a.kv_heads * a.dim, tail, gv, nullptr, nullptr, 0);
+        }
       }
+      return;
     }
-    return;
+    sg = attn_segment(a, (int)seg + 1);
+    if (attn_long(sg.nq, sg.nk)) return;
   }
-  const AttnSegment sg = attn_segment(a, (int)seg + 1);
   const float c = a.scale * kLog2e;
   const T* kb = static_cast<const T*>(a.k) + sg.k0 * a.k_row + r.kvh * a.k_head + r.col;
   const T* vb = static_cast<const T*>(a.v) + sg.k0 * a.v_row + r.kvh * a.v_head + r.col;
@@ -209,7 +299,7 @@ __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd 
     ds = p * (dp - x.delta) * a.scale;
   };
 
-  if (GF && sg.nq == 1) {
+  if (GF && sg.nq == 1 && !is_long) {
     Query x[G];
     float dq[G][8];
 #pragma unroll
@@ -250,15 +340,18 @@ __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd 
     }
     return;
   }
+  // the walk's first key and step: the wave's slots, or the workgroup's
+  const uint32_t waves = is_long ? 4 : 1, place = is_long ? wave : 0;
   if (gq)
-    for (int i = 0; i < sg.nq; ++i)
+    for (int64_t i = part; i < sg.nq; i += parts)
       for (int g = 0; g < a.group; ++g) {
-        const int head = r.kvh * a.group + g, n = sees(i);
+        const int head = r.kvh * a.group + g;
+        const uint32_t n = sees((int)i);
         Query x;
-        query(i, head, x);
+        query((int)i, head, x);
         float dq[8];
         zero8(dq);
-        for (int j = r.slot; j < n; j += r.slots) {
+        for (uint32_t j = place * r.slots + r.slot; j < n; j += waves * r.slots) {
           float k[8], v[8], p, ds;
           zero8(k);
           zero8(v);
@@ -271,11 +364,23 @@ __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd 
           for (int e = 0; e < 8; ++e) dq[e] = fmaf(ds, k[e], dq[e]);
         }
         slots_sum(dq, r.stride);
-        if (r.on && r.slot == 0) store8<false>(gq + ((sg.q0 + i) * a.heads + head) * a.dim + r.col, dq);
+        if (is_long) {
+          __shared__ float sum[3][8][64];
+          __syncthreads();  // the sum before is read
+          if (wave > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sum[wave - 1][e][lane] = dq[e];
+          }
+          __syncthreads();
+          for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dq[e] += sum[k][e][lane];  // of the first wave's use alone
+        }
+        if (r.on && r.slot == 0 && place == 0) store8<false>(gq + ((sg.q0 + i) * a.heads + head) * a.dim + r.col, dq);
       }
   if (!gk) return;
-  for (int j0 = 0; j0 < sg.nk; j0 += r.slots) {
-    const int j = j0 + r.slot;
+  for (int64_t j0 = (part * waves + place) * r.slots; j0 < sg.nk; j0 += parts * waves * r.slots) {
+    const int64_t j = j0 + r.slot;
     const bool live = r.on && j < sg.nk;
     float k[8], v[8], dk[8], dv[8];
     zero8(k);
@@ -314,7 +419,7 @@ int pow2_at_least(int x) {
 
 struct RowGrid {
   int hb, head_blocks;
-  int64_t blocks;
+  int64_t row_blocks, blocks;
 };
 
 RowGrid row_grid(const AttnArgs& a, int lg) {
@@ -322,7 +427,8 @@ RowGrid row_grid(const AttnArgs& a, int lg) {
   const int most = 64 / lg, want = pow2_at_least(a.kv_heads);
   r.hb = want < most ? want : most;
   r.head_blocks = (int)fmd_cdiv(a.kv_heads, r.hb);
-  r.blocks = fmd_cdiv(((int64_t)a.segments + kTail) * r.head_blocks, 4);
+  r.row_blocks = fmd_cdiv(((int64_t)a.segments + kTail) * r.head_blocks, 4);
+  r.blocks = r.row_blocks + attn_long_numbers(a.tq, a.tk) * r.head_blocks;
   return r;
 }
 
@@ -331,10 +437,10 @@ int fwd(const AttnArgs& a, T* out, const AttnSaved& s, hipStream_t stream) {
   const RowGrid r = row_grid(a, LG);
   FMD_REQUIRE(r.blocks < (1ll << 31));
   const unsigned n = (unsigned)r.blocks;
-  if (a.group == 1) attn_rows_fwd_kernel<T, LG, 1><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, out, s);
-  else if (a.group == 2) attn_rows_fwd_kernel<T, LG, 2><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, out, s);
-  else if (a.group == 4) attn_rows_fwd_kernel<T, LG, 4><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, out, s);
-  else attn_rows_fwd_kernel<T, LG, 0><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, out, s);
+  if (a.group == 1) attn_rows_fwd_kernel<T, LG, 1><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
+  else if (a.group == 2) attn_rows_fwd_kernel<T, LG, 2><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
+  else if (a.group == 4) attn_rows_fwd_kernel<T, LG, 4><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
+  else attn_rows_fwd_kernel<T, LG, 0><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
@@ -344,10 +450,10 @@ int bwd_by_group(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipSt
   const RowGrid r = row_grid(a, LG);
   FMD_REQUIRE(r.blocks < (1ll << 31));
   const unsigned n = (unsigned)r.blocks;
-  if (a.group == 1) attn_rows_bwd_kernel<T, LG, 1, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
-  else if (a.group == 2) attn_rows_bwd_kernel<T, LG, 2, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
-  else if (a.group == 4) attn_rows_bwd_kernel<T, LG, 4, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
-  else attn_rows_bwd_kernel<T, LG, 0, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, gq, gk, gv);
+  if (a.group == 1) attn_rows_bwd_kernel<T, LG, 1, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+  else if (a.group == 2) attn_rows_bwd_kernel<T, LG, 2, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+  else if (a.group == 4) attn_rows_bwd_kernel<T, LG, 4, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+  else attn_rows_bwd_kernel<T, LG, 0, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
