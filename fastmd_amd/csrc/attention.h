@@ -23,7 +23,21 @@ struct AttnArgs {
   int32_t segments, heads, kv_heads, group, dim, causal;
   float scale;
   uint32_t group_mul, group_shift;          // row / group = row * group_mul >> group_shift for rows below 2^31
+  uint32_t block0;                          // first workgroup of this launch (launch_ranges)
 };
+
+// A launch takes fewer than 2^32 threads a dimension. More workgroups go in several launches, each told its first one:
+// launch(workgroups, first).
+constexpr int64_t kMostBlocks = 1 << 22;
+
+template <typename Launch>
+int launch_ranges(int64_t blocks, const Launch& launch) {
+  for (int64_t first = 0; first < blocks; first += kMostBlocks) {
+    launch((unsigned)(blocks - first < kMostBlocks ? blocks - first : kMostBlocks), first);
+    FMD_CHECK_LAUNCH();
+  }
+  return FMD_OK;
+}
 
 __device__ __forceinline__ int attn_token(const AttnArgs& a, int row) {
   return (int)((uint64_t)(uint32_t)row * a.group_mul >> a.group_shift);

@@ -1,4 +1,5 @@
 // Attention of the query rows of each segment over the key rows of the same segment, and its VJP.
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.h"
@@ -61,8 +62,9 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, kw = wave / WM;
-  const int kvh = blockIdx.x % a.kv_heads;
-  int64_t t = blockIdx.x / a.kv_heads;
+  const uint32_t block = a.block0 + blockIdx.x;
+  const int kvh = block % a.kv_heads;
+  int64_t t = block / a.kv_heads;
   if (CAUSAL) t = tiles - 1 - t;  // the rows with the most keys first
   int64_t first;
   const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first, WaveLanes());
@@ -366,8 +368,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int splits, 
 // rounding of the sum, 2^-24 of it, is far below the rounding of P), base for fp32, which multiplies by the inverse; +inf for
 // a row that sees nothing. 16 lanes a row. Memory bounds it: 8 192 rows of 16 heads of 128, bf16, 21 us (100 MB).
 template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, int heads, int dim, float* rows) {
-  const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+__global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, int heads, int dim, int64_t block0, float* rows) {
+  const int64_t at = (block0 + blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int sub = threadIdx.x & 15;
   const int64_t tok = at / heads;
   const int head = (int)(at % heads);
@@ -421,9 +423,10 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, rw = wave / WM;
-  const int kvh = blockIdx.x % a.kv_heads;
+  const uint32_t block = a.block0 + blockIdx.x;
+  const int kvh = block % a.kv_heads;
   int64_t first;
-  const int ext = attn_find(a.k_off, a.segments, a.tk, 1, 32 * WM, blockIdx.x / a.kv_heads, &first, WaveLanes());
+  const int ext = attn_find(a.k_off, a.segments, a.tk, 1, 32 * WM, block / a.kv_heads, &first, WaveLanes());
   AttnSegment sg = attn_segment(a, ext);
   if (!attn_real(a, ext)) sg.nq = 0;
   if (first >= sg.nk) return;
@@ -707,8 +710,9 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % WM, kw = wave / WM;
-  const int kvh = blockIdx.x % a.kv_heads;
-  int64_t t = blockIdx.x / a.kv_heads;
+  const uint32_t block = a.block0 + blockIdx.x;
+  const int kvh = block % a.kv_heads;
+  int64_t t = block / a.kv_heads;
   if (CAUSAL) t = tiles - 1 - t;
   int64_t first;
   const int ext = attn_find(a.q_off, a.segments, a.tq, a.group, 32 * WM, t, &first, WaveLanes());
@@ -1024,7 +1028,7 @@ int split_planes(const void* x, int64_t x_row, int64_t x_head, const void* y, in
   *t = {xp, yp, ld, 3 * dim, ld, 3 * dim};
   const int64_t n = rows * heads * (dim / 8);
   if (n == 0) return FMD_OK;
-  FMD_REQUIRE(ld < (1 << 24) && n < (1ll << 38));
+  FMD_REQUIRE(ld < (1 << 24) && n < (1ll << 32));
   attn_split_kernel<<<(unsigned)fmd_cdiv(n, 256), 256, 0, stream>>>(static_cast<const float*>(x), x_row, x_head,
                                                                     static_cast<const float*>(y), y_row, y_head, rows, heads, dim, xp, yp);
   FMD_CHECK_LAUNCH();
@@ -1052,18 +1056,21 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   }
   float *po = work, *pm = work ? work + splits * n * a.dim : nullptr, *pl = work ? pm + splits * n : nullptr;
   const int64_t tiles = tile_count(a.tq, a.group, a.segments, shape_rows(shape));
-  FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-  const dim3 grid((unsigned)(tiles * a.kv_heads), splits);
-  if (shape == kWide) {
-    attn_fwd_kernel<T, DP, kWideKeys, 4, 1, true, CAUSAL><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
-  } else if (shape == kMid) {
-    if constexpr (f32 && DP <= 64)
-      attn_fwd_kernel<T, DP, 32, 2, 2, true, CAUSAL><<<grid, 256, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
-  } else {
-    attn_fwd_kernel<T, DP, 32, 1, kKeyWaves, !f32, CAUSAL><<<grid, 64 * kKeyWaves, 0, stream>>>(a, t, tiles, splits, out, saved, po, pm, pl);
-  }
-  FMD_CHECK_LAUNCH();
-  if (splits > 1) {
+  const int status = launch_ranges(tiles * a.kv_heads, [&](unsigned blocks, int64_t first) {
+    const dim3 grid(blocks, splits);
+    AttnArgs b = a;
+    b.block0 = (uint32_t)first;
+    if (shape == kWide) {
+      attn_fwd_kernel<T, DP, kWideKeys, 4, 1, true, CAUSAL><<<grid, 256, 0, stream>>>(b, t, tiles, splits, out, saved, po, pm, pl);
+    } else if (shape == kMid) {
+      if constexpr (f32 && DP <= 64)
+        attn_fwd_kernel<T, DP, 32, 2, 2, true, CAUSAL><<<grid, 256, 0, stream>>>(b, t, tiles, splits, out, saved, po, pm, pl);
+    } else {
+      attn_fwd_kernel<T, DP, 32, 1, kKeyWaves, !f32, CAUSAL><<<grid, 64 * kKeyWaves, 0, stream>>>(b, t, tiles, splits, out, saved, po, pm, pl);
+    }
+  });
+  if (status != FMD_OK) return status;
+  if (splits > 1) {  // of calls with too few tiles to fill the card: few rows
     attn_join_kernel<T><<<(unsigned)fmd_cdiv(n, 4), 256, 0, stream>>>(a, splits, po, pm, pl, out, saved);
     FMD_CHECK_LAUNCH();
   }
@@ -1084,22 +1091,24 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, int q_splits, int kv_splits, T*
     // wide bf16: 64 keys and four row groups, two waves per SIMD in one workgroup
     constexpr int kWM = f32 ? 4 : 2, kRW = f32 ? 1 : 4, kMidRW = DP <= 32 ? 4 : 2;
     const int64_t tiles = tile_count(a.tk, 1, a.segments, shape == kWide ? 32 * kWM : shape_rows(shape));
-    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    const dim3 grid((unsigned)(tiles * a.kv_heads), kv_splits);
     float* part = work;
     if (kv_splits > 1) work += kv_splits * 2 * a.tk * a.kv_heads * a.dim;
-    if (shape == kWide) {
-      attn_bwd_kv_kernel<T, DP, kWM, kRW, true, CAUSAL><<<grid, 64 * kWM * kRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
-    } else if (shape == kMid) {
-      if constexpr (f32 && DP <= 64)
-        attn_bwd_kv_kernel<T, DP, 2, kMidRW, true, CAUSAL><<<grid, 128 * kMidRW, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
-    } else {
-      attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32, CAUSAL><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, kv_splits, part, gk, gv);
-    }
-    FMD_CHECK_LAUNCH();
+    const int status = launch_ranges(tiles * a.kv_heads, [&](unsigned blocks, int64_t first) {
+      const dim3 grid(blocks, kv_splits);
+      AttnArgs c = a;
+      c.block0 = (uint32_t)first;
+      if (shape == kWide) {
+        attn_bwd_kv_kernel<T, DP, kWM, kRW, true, CAUSAL><<<grid, 64 * kWM * kRW, 0, stream>>>(c, b, t, kv_splits, part, gk, gv);
+      } else if (shape == kMid) {
+        if constexpr (f32 && DP <= 64)
+          attn_bwd_kv_kernel<T, DP, 2, kMidRW, true, CAUSAL><<<grid, 128 * kMidRW, 0, stream>>>(c, b, t, kv_splits, part, gk, gv);
+      } else {
+        attn_bwd_kv_kernel<T, DP, 1, kWaves, !f32, CAUSAL><<<grid, 64 * kWaves, 0, stream>>>(c, b, t, kv_splits, part, gk, gv);
+      }
+    });
+    if (status != FMD_OK) return status;
     if (kv_splits > 1) {
       const int64_t n = a.tk * a.kv_heads * a.dim;
-      FMD_REQUIRE(fmd_cdiv(2 * n, 1024) < (1ll << 31));
       attn_add_kernel<T><<<(unsigned)fmd_cdiv(2 * n, 1024), 256, 0, stream>>>(part, n, kv_splits, gk, gv);
       FMD_CHECK_LAUNCH();
     }
@@ -1112,20 +1121,22 @@ int run_bwd(const AttnArgs& a, const AttnBwd& b, int q_splits, int kv_splits, T*
       if (status != FMD_OK) return status;
     }
     const int64_t tiles = tile_count(a.tq, a.group, a.segments, shape_rows(shape));
-    FMD_REQUIRE(tiles * a.kv_heads < (1ll << 31));
-    const dim3 grid((unsigned)(tiles * a.kv_heads), q_splits);
     float* part = work;
-    if (shape == kWide) {
-      attn_bwd_q_kernel<T, DP, 4, 1, true, CAUSAL><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
-    } else if (shape == kMid) {
-      if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true, CAUSAL><<<grid, 256, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
-    } else {
-      attn_bwd_q_kernel<T, DP, 1, kWaves, !f32, CAUSAL><<<grid, 64 * kWaves, 0, stream>>>(a, b, t, tiles, q_splits, part, gq);
-    }
-    FMD_CHECK_LAUNCH();
+    const int status = launch_ranges(tiles * a.kv_heads, [&](unsigned blocks, int64_t first) {
+      const dim3 grid(blocks, q_splits);
+      AttnArgs c = a;
+      c.block0 = (uint32_t)first;
+      if (shape == kWide) {
+        attn_bwd_q_kernel<T, DP, 4, 1, true, CAUSAL><<<grid, 256, 0, stream>>>(c, b, t, tiles, q_splits, part, gq);
+      } else if (shape == kMid) {
+        if constexpr (f32 && DP <= 64) attn_bwd_q_kernel<T, DP, 2, 2, true, CAUSAL><<<grid, 256, 0, stream>>>(c, b, t, tiles, q_splits, part, gq);
+      } else {
+        attn_bwd_q_kernel<T, DP, 1, kWaves, !f32, CAUSAL><<<grid, 64 * kWaves, 0, stream>>>(c, b, t, tiles, q_splits, part, gq);
+      }
+    });
+    if (status != FMD_OK) return status;
     if (q_splits > 1) {
       const int64_t n = a.tq * a.heads * a.dim;
-      FMD_REQUIRE(fmd_cdiv(n, 1024) < (1ll << 31));
       attn_add_kernel<T><<<(unsigned)fmd_cdiv(n, 1024), 256, 0, stream>>>(part, n, q_splits, gq, static_cast<T*>(nullptr));
       FMD_CHECK_LAUNCH();
     }
@@ -1148,6 +1159,8 @@ int check(const AttnArgs& a, int size) {
               a.v_row % unit == 0 && a.v_head % unit == 0);
   FMD_REQUIRE(a.q_row < (1 << 24) && a.k_row < (1 << 24) && a.v_row < (1 << 24));
   FMD_REQUIRE(a.scale > 0.f);
+  // workgroups are numbered in 32 bits
+  FMD_REQUIRE((std::max(a.tq * a.group, a.tk) / 32 + a.segments + 2) * a.kv_heads < (1ll << 31));
   return FMD_OK;
 }
 
@@ -1184,8 +1197,10 @@ int backward(const AttnArgs& a, AttnBwd b, int q_splits, int kv_splits, T* gq, T
   if (a.tk == 0) gk = gv = nullptr;
   if (few_rows(a.tq, a.tk, a.segments, a.kv_heads)) return attn_rows_bwd<T>(a, b, gq, gk, gv, stream);
   if (a.tq > 0) {
-    attn_delta_kernel<T><<<(unsigned)fmd_cdiv(a.tq * a.heads, 16), 256, 0, stream>>>(b, a.tq, a.heads, a.dim, work);
-    FMD_CHECK_LAUNCH();
+    const int launched = launch_ranges(fmd_cdiv(a.tq * a.heads, 16), [&](unsigned blocks, int64_t first) {
+      attn_delta_kernel<T><<<blocks, 256, 0, stream>>>(b, a.tq, a.heads, a.dim, first, work);
+    });
+    if (launched != FMD_OK) return launched;
   }
   work += fmd_cdiv(2 * a.heads * a.tq, 4) * 4;
   FMD_BY_WIDTH(run_bwd, a, b, q_splits, kv_splits, gq, gk, gv, work, stream)

@@ -162,9 +162,10 @@ __global__ void __launch_bounds__(256) attn_rows_fwd_kernel(AttnArgs a, int hb, 
   constexpr int G = GF ? GF : 1;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   RowSoftmax<T, LG, G> x;
-  if (blockIdx.x >= row_blocks) {
+  const int64_t block = (int64_t)a.block0 + blockIdx.x;
+  if (block >= row_blocks) {
     __shared__ float part[3][10][64];
-    const LongPart p = long_part(a, blockIdx.x - row_blocks, head_blocks);
+    const LongPart p = long_part(a, block - row_blocks, head_blocks);
     if (!p.any) return;
     const RowLane r = row_lane<LG>(a, p.head_block, hb);
     for (int64_t i = p.part; i < p.sg.nq; i += p.parts)
@@ -194,7 +195,7 @@ __global__ void __launch_bounds__(256) attn_rows_fwd_kernel(AttnArgs a, int hb, 
       }
     return;
   }
-  const int64_t w = (int64_t)blockIdx.x * 4 + wave;
+  const int64_t w = block * 4 + wave;
   const int64_t seg = w / head_blocks;
   const RowLane r = row_lane<LG>(a, (int)(w % head_blocks), hb);
   if (seg >= a.segments) {
@@ -241,20 +242,21 @@ template <typename T, int LG, int GF, bool NT>
 __global__ void __launch_bounds__(256) attn_rows_bwd_kernel(AttnArgs a, AttnBwd b, int hb, int head_blocks, int64_t row_blocks, T* gq, T* gk,
                                                             T* gv) {
   constexpr int G = GF ? GF : 1;
-  const bool is_long = blockIdx.x >= row_blocks;
+  const int64_t block = (int64_t)a.block0 + blockIdx.x;
+  const bool is_long = block >= row_blocks;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   int64_t part = 0, parts = 1;
   AttnSegment sg;
   RowLane r;
   if (is_long) {
-    const LongPart p = long_part(a, blockIdx.x - row_blocks, head_blocks);
+    const LongPart p = long_part(a, block - row_blocks, head_blocks);
     if (!p.any) return;
     sg = p.sg;
     part = p.part;
     parts = p.parts;
     r = row_lane<LG>(a, p.head_block, hb);
   } else {
-    const int64_t w = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t w = block * 4 + wave;
     const int64_t seg = w / head_blocks;
     r = row_lane<LG>(a, (int)(w % head_blocks), hb);
     if (seg >= a.segments) {
@@ -435,27 +437,29 @@ RowGrid row_grid(const AttnArgs& a, int lg) {
 template <typename T, int LG>
 int fwd(const AttnArgs& a, T* out, const AttnSaved& s, hipStream_t stream) {
   const RowGrid r = row_grid(a, LG);
-  FMD_REQUIRE(r.blocks < (1ll << 31));
-  const unsigned n = (unsigned)r.blocks;
-  if (a.group == 1) attn_rows_fwd_kernel<T, LG, 1><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
-  else if (a.group == 2) attn_rows_fwd_kernel<T, LG, 2><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
-  else if (a.group == 4) attn_rows_fwd_kernel<T, LG, 4><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
-  else attn_rows_fwd_kernel<T, LG, 0><<<n, 256, 0, stream>>>(a, r.hb, r.head_blocks, r.row_blocks, out, s);
-  FMD_CHECK_LAUNCH();
-  return FMD_OK;
+  FMD_REQUIRE(r.blocks < (1ll << 32));
+  return launch_ranges(r.blocks, [&](unsigned n, int64_t first) {
+    AttnArgs c = a;
+    c.block0 = (uint32_t)first;
+    if (a.group == 1) attn_rows_fwd_kernel<T, LG, 1><<<n, 256, 0, stream>>>(c, r.hb, r.head_blocks, r.row_blocks, out, s);
+    else if (a.group == 2) attn_rows_fwd_kernel<T, LG, 2><<<n, 256, 0, stream>>>(c, r.hb, r.head_blocks, r.row_blocks, out, s);
+    else if (a.group == 4) attn_rows_fwd_kernel<T, LG, 4><<<n, 256, 0, stream>>>(c, r.hb, r.head_blocks, r.row_blocks, out, s);
+    else attn_rows_fwd_kernel<T, LG, 0><<<n, 256, 0, stream>>>(c, r.hb, r.head_blocks, r.row_blocks, out, s);
+  });
 }
 
 template <typename T, int LG, bool NT>
 int bwd_by_group(const AttnArgs& a, const AttnBwd& b, T* gq, T* gk, T* gv, hipStream_t stream) {
   const RowGrid r = row_grid(a, LG);
-  FMD_REQUIRE(r.blocks < (1ll << 31));
-  const unsigned n = (unsigned)r.blocks;
-  if (a.group == 1) attn_rows_bwd_kernel<T, LG, 1, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
-  else if (a.group == 2) attn_rows_bwd_kernel<T, LG, 2, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
-  else if (a.group == 4) attn_rows_bwd_kernel<T, LG, 4, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
-  else attn_rows_bwd_kernel<T, LG, 0, NT><<<n, 256, 0, stream>>>(a, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
-  FMD_CHECK_LAUNCH();
-  return FMD_OK;
+  FMD_REQUIRE(r.blocks < (1ll << 32));
+  return launch_ranges(r.blocks, [&](unsigned n, int64_t first) {
+    AttnArgs c = a;
+    c.block0 = (uint32_t)first;
+    if (a.group == 1) attn_rows_bwd_kernel<T, LG, 1, NT><<<n, 256, 0, stream>>>(c, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+    else if (a.group == 2) attn_rows_bwd_kernel<T, LG, 2, NT><<<n, 256, 0, stream>>>(c, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+    else if (a.group == 4) attn_rows_bwd_kernel<T, LG, 4, NT><<<n, 256, 0, stream>>>(c, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+    else attn_rows_bwd_kernel<T, LG, 0, NT><<<n, 256, 0, stream>>>(c, b, r.hb, r.head_blocks, r.row_blocks, gq, gk, gv);
+  });
 }
 
 template <typename T, int LG>

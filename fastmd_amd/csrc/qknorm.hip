@@ -128,9 +128,9 @@ __device__ __forceinline__ int head_blocks(const NormArgs& a, int by) {
 }
 
 template <typename T, int LG, Turn TURN, bool NT>
-__global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, T* q_out, T* k_out) {
+__global__ void __launch_bounds__(256) qk_norm_kernel(NormArgs a, uint32_t block0, T* q_out, T* k_out) {
   const int sub = threadIdx.x & (LG - 1), col0 = 8 * sub;
-  const uint32_t unit = blockIdx.x * (256 / LG) + threadIdx.x / LG;  // fewer than 2^31 of them
+  const uint32_t unit = (block0 + blockIdx.x) * (256 / LG) + threadIdx.x / LG;  // fewer than 2^31 of them
   const int blocks = head_blocks(a, kFwdHeads), qb = (a.heads + kFwdHeads - 1) / kFwdHeads;
   int64_t tok = unit / (uint32_t)blocks;
   const int hb = (int)(unit % (uint32_t)blocks);
@@ -315,11 +315,10 @@ bool streams(const NormArgs& a) {
 
 template <typename T, int LG, Turn TURN>
 int norm_fwd_turn(const NormArgs& a, T* q_out, T* k_out, hipStream_t stream) {
-  const unsigned grid = (unsigned)fmd_cdiv(unit_count(a.tokens, a.heads, a.kv_heads, kFwdHeads), 256 / LG);
-  if (streams<T>(a)) qk_norm_kernel<T, LG, TURN, true><<<grid, 256, 0, stream>>>(a, q_out, k_out);
-  else qk_norm_kernel<T, LG, TURN, false><<<grid, 256, 0, stream>>>(a, q_out, k_out);
-  FMD_CHECK_LAUNCH();
-  return FMD_OK;
+  return launch_ranges(fmd_cdiv(unit_count(a.tokens, a.heads, a.kv_heads, kFwdHeads), 256 / LG), [&](unsigned n, int64_t first) {
+    if (streams<T>(a)) qk_norm_kernel<T, LG, TURN, true><<<n, 256, 0, stream>>>(a, (uint32_t)first, q_out, k_out);
+    else qk_norm_kernel<T, LG, TURN, false><<<n, 256, 0, stream>>>(a, (uint32_t)first, q_out, k_out);
+  });
 }
 
 template <typename T, int LG>

@@ -93,6 +93,9 @@ def _refuse(q: Tensor, k: Tensor, v: Tensor, q_offsets: Tensor, k_offsets: Tenso
         raise ValueError(f"q_offsets has {q_offsets.numel() - 1} segments, k_offsets {k_offsets.numel() - 1}")
     if q.shape[0] * heads // kv_heads >= 2 ** 31 or k.shape[0] >= 2 ** 31:
         raise ValueError("segment attention takes fewer than 2^31 packed query rows and key rows")
+    if (max(q.shape[0] * (heads // kv_heads), k.shape[0]) // 32 + q_offsets.numel() + 1) * kv_heads >= 2 ** 31:
+        raise ValueError("segment attention takes fewer than 2^31 tiles (32 rows of a key head, and one for each segment and key "
+                         f"head), got {q_offsets.numel() - 1} segments of {kv_heads} key heads")
     if scale is not None and not 0.0 < float(scale) < float("inf"):
         raise ValueError(f"scale must be positive and finite, got {scale}")
 
@@ -116,7 +119,8 @@ def _prepare(q, k, v, q_offsets, k_offsets, causal, scale):
     tk, kv_heads, kdim = k.shape
     segments = q_offsets.shape[0] - 1
     if not (kdim == dim and 8 <= dim <= MAX_DIM and dim % 8 == 0 and heads and kv_heads and heads % kv_heads == 0
-            and segments >= 0 and tq * heads < 2 ** 31 and tk < 2 ** 31):
+            and segments >= 0 and tq * heads < 2 ** 31 and tk < 2 ** 31
+            and (tq * heads + tk * kv_heads) // 32 + (segments + 2) * kv_heads < 2 ** 31):
         _refuse(q, k, v, q_offsets, k_offsets, scale)
     (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = heads_view(q), heads_view(k), heads_view(v)
     same = k_offsets is q_offsets

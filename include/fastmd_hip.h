@@ -828,6 +828,7 @@ int fmd_edge_stress_f32(const float* geo, const float* gvec, const int64_t* n_ed
  * For the VJP (all nullable): base and inverse [heads, tq], such that a probability is
  * exp2(score log2(e) - base) inverse (both 0 for a row that sees nothing), and for bf16 residual [tq, heads, dim], what the
  * rounding of out dropped.
+ * Packed rows tq heads / kv_heads, key rows, and (max of both / 32 + segments + 2) kv_heads below 2^31 (FMD_EINVAL otherwise).
  * splits: fmd_segment_attention_splits(). work: fmd_segment_attention_work_size() floats on a 16-byte address (null for 0). */
 int32_t fmd_segment_attention_splits(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads,
                                      int32_t dim);
