@@ -1049,7 +1049,7 @@ int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   const int64_t n = a.tq * a.heads;
   AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
   const AttnShape shape = shape_of(f32, a.dim, a.tq * a.group, a.kv_heads, a.segments);
-  FMD_REQUIRE(work || (splits == 1 && !(f32 && shape != kNarrow)));
+  FMD_REQUIRE(work || (splits == 1 && !(f32 && shape != kNarrow && a.tk > 0)));
   if (f32 && shape != kNarrow) {
     const int status = split_planes(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head, a.tk, a.kv_heads, a.dim, work, &t, stream);
     if (status != FMD_OK) return status;
