@@ -83,7 +83,8 @@ __device__ __forceinline__ void angles(const NormArgs& a, int64_t tok, int col0,
   }
 }
 
-// y -> rotated y (sign 1) or the transposed rotation (sign -1)
+// y -> rotated y (sign 1) or the transposed rotation (sign -1). Columns past `rot` stay as they are, whatever they hold (a product
+// with a sine of zero would make NaN of an infinity, and of a NaN beside them).
 template <int LG, Turn TURN>
 __device__ __forceinline__ void rotate(const NormArgs& a, int col0, const float (&c)[8], const float (&s)[8], float sign,
                                        float (&y)[8]) {
@@ -93,8 +94,9 @@ __device__ __forceinline__ void rotate(const NormArgs& a, int col0, const float 
   if constexpr (TURN == kNeighbours) {
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      o[e] = y[e] * c[e] - sign * s[e] * y[e + 1];
-      o[e + 1] = y[e + 1] * c[e + 1] + sign * s[e + 1] * y[e];
+      const bool turned = col0 + e < a.rot;
+      o[e] = turned ? y[e] * c[e] - sign * s[e] * y[e + 1] : y[e];
+      o[e + 1] = turned ? y[e + 1] * c[e + 1] + sign * s[e + 1] * y[e] : y[e + 1];
     }
   } else if constexpr (TURN == kLanes) {
     const int lane = threadIdx.x & 63, sub = lane & (LG - 1), by = half >> 3;
@@ -102,7 +104,10 @@ __device__ __forceinline__ void rotate(const NormArgs& a, int col0, const float 
     const int from = (lane - sub) + (col0 < a.rot ? (low ? sub + by : sub - by) : sub);
     const float f = low ? -sign : sign;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = y[e] * c[e] + f * s[e] * __shfl(y[e], from, 64);
+    for (int e = 0; e < 8; ++e) {
+      const float other = __shfl(y[e], from, 64);
+      o[e] = col0 < a.rot ? y[e] * c[e] + f * s[e] * other : y[e];
+    }
   } else {
     const int lane = threadIdx.x & 63, base = lane & ~(LG - 1);
 #pragma unroll
@@ -115,7 +120,7 @@ __device__ __forceinline__ void rotate(const NormArgs& a, int col0, const float 
         const float x = __shfl(y[k], base + (other >> 3), 64);
         v = (other & 7) == k ? x : v;
       }
-      o[e] = y[e] * c[e] + (col < half ? -sign : sign) * s[e] * v;
+      o[e] = col < a.rot ? y[e] * c[e] + (col < half ? -sign : sign) * s[e] * v : y[e];
     }
   }
 #pragma unroll

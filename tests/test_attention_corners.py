@@ -19,3 +19,27 @@ def test_many_queries_without_keys(rows, heads, dim, dtype):
     assert not out.any() and bool((saved.lse == -float("inf")).all())
     gq, gk, gv = segment_attention_vjp(q, q, k, k, out, saved, q_off, k_off)
     assert not gq.any() and gk.shape == gv.shape == (0, heads, dim)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot", [(64, 32), (64, 16), (64, 20), (40, 6), (128, 64), (8, 2), (256, 128)])
+def test_columns_that_do_not_turn_stay_as_they_are(dim, rot, interleaved, dtype):
+    """Infinities and NaN among them too, and what lies beside those; forward and in the gradient."""
+    from fastmd_amd.ops.qk_norm import rotary, rotary_tables
+
+    gen = torch.Generator().manual_seed(rot)
+    x = torch.randn(30, 3, dim, generator=gen).to(dtype)
+    tables = rotary_tables(30, rot, device="cuda")
+    plain = rotary(x.cuda(), *tables, interleaved=interleaved)
+    odd = x.clone()
+    for n, value in enumerate((float("inf"), -float("inf"), float("nan"))):
+        odd[n::7, :, rot + n::4] = value
+    odd = odd.cuda().requires_grad_()
+    out = rotary(odd, *tables, interleaved=interleaved)
+    (grad,) = torch.autograd.grad(out, odd, odd.detach())
+    assert torch.equal(out[..., :rot], plain[..., :rot])
+    assert torch.equal(out[..., rot:].nan_to_num(3.0, 7.0, -7.0), odd[..., rot:].nan_to_num(3.0, 7.0, -7.0))
+    assert torch.equal(grad[..., rot:].nan_to_num(3.0, 7.0, -7.0), odd[..., rot:].nan_to_num(3.0, 7.0, -7.0))
+    assert bool(torch.isfinite(grad[..., :rot]).all())
