@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   // always, 4 x 3 000 rows, 8 heads of 64, bf16): exponentials up to 2^kSlack are
   // as exact as those below one, and the sums are rescaled a few times per row instead of once per tile.
   constexpr float kSlack = 8.f;
-  const float slack = kSlack / c;
+  const float slack = fminf(kSlack / c, 0x1p127f);  // finite for the smallest scale too: -inf + slack stays below any score
 
   const int lane_r = Tile::lane_rows(), lane_c = Tile::lane_cols();
   auto step = [&](auto last, const __bf16* ks_, int tile) {

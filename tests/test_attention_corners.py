@@ -43,3 +43,24 @@ def test_columns_that_do_not_turn_stay_as_they_are(dim, rot, interleaved, dtype)
     assert torch.equal(out[..., rot:].nan_to_num(3.0, 7.0, -7.0), odd[..., rot:].nan_to_num(3.0, 7.0, -7.0))
     assert torch.equal(grad[..., rot:].nan_to_num(3.0, 7.0, -7.0), odd[..., rot:].nan_to_num(3.0, 7.0, -7.0))
     assert bool(torch.isfinite(grad[..., :rot]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [1e-30, 1e-38, 1e-42])
+@pytest.mark.parametrize("lq,lk,heads", [([40, 7], [90, 130], 4), ([3, 2], [5000, 4000], 4), ([1500, 1500], [1500, 1500], 8),
+                                         ([1] * 70, [20] * 70, 4)])
+def test_smallest_scales_give_the_mean(lq, lk, heads, scale, dtype):
+    """Weights equal to within 1e-27: narrow tiles whose waves join, split keys, wide tiles, the row kernels. Bounds: sums of
+    up to 5 000 float32 terms, rounded once (2^-24 sqrt(5000) < 2^-17 of the absolute mean, and of the type's rounding)."""
+    from fastmd_amd.ops.attention import segment_attention_forward
+    from test_attention import U, make
+
+    q, k, v, _, q_off, k_off = make(lq, lk, heads, heads, 32, dtype)
+    out, saved = segment_attention_forward(*(x.cuda() for x in (q, k, v, q_off, k_off)), scale=scale)
+    out, lse = out.double().cpu(), saved.lse.double().cpu()
+    for n in range(len(lq)):
+        rows, keys = slice(q_off[n], q_off[n + 1]), slice(k_off[n], k_off[n + 1])
+        mean, size = v[keys].double().mean(0), v[keys].double().abs().mean(0)
+        assert bool(((out[rows] - mean).abs() <= 2.0 ** -17 * size + 1.01 * U[dtype] * mean.abs()).all())
+        assert bool((lse[:, rows] - torch.log(torch.tensor(float(lk[n])).double())).abs().max() < 1e-5)
