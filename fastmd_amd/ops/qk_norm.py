@@ -109,6 +109,11 @@ def _check(q: Tensor, k: Tensor | None, q_weight, k_weight, cos: Tensor, sin: Te
         raise ValueError("the norm and rotation take fewer than 2^31 rows")
 
 
+def _check_eps(eps) -> None:
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+
+
 def _aligned(t: Tensor | None) -> Tensor | None:
     """A contiguous tensor on a 16-byte address (the same one if it is)."""
     if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
@@ -202,8 +207,7 @@ def qk_norm_rotary(q: Tensor, k: Tensor, q_weight: Tensor | None, k_weight: Tens
     Differentiable once in q, k and the weights, in reverse
     mode."""
     _check(q, k, q_weight, k_weight, cos, sin, positions)
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative, got {eps}")
+    _check_eps(eps)
     return _apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), True)
 
 
@@ -213,6 +217,7 @@ def qk_norm_rotary_vjp(gq: Tensor, gk: Tensor, q: Tensor, k: Tensor, q_weight: T
     """``(gradient of q, of k, of q_weight, of k_weight)`` from the gradients of both outputs (the last two None for
     absent weights)."""
     _check(q, k, q_weight, k_weight, cos, sin, positions)
+    _check_eps(eps)
     return _vjp(gq, gk, q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved), True, True)
 
 

@@ -64,3 +64,15 @@ def test_smallest_scales_give_the_mean(lq, lk, heads, scale, dtype):
         mean, size = v[keys].double().mean(0), v[keys].double().abs().mean(0)
         assert bool(((out[rows] - mean).abs() <= 2.0 ** -17 * size + 1.01 * U[dtype] * mean.abs()).all())
         assert bool((lse[:, rows] - torch.log(torch.tensor(float(lk[n])).double())).abs().max() < 1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eps", [-1e-6, float("nan")])
+def test_both_directions_of_the_norm_refuse_an_eps(eps):
+    from fastmd_amd.ops.qk_norm import qk_norm_rotary, qk_norm_rotary_vjp, rotary_tables
+
+    x, w = torch.ones(3, 2, 16, device="cuda"), torch.ones(16, device="cuda")
+    args = (x, x, w, w, *rotary_tables(3, 16, device="cuda"))
+    for call in (lambda: qk_norm_rotary(*args, eps=eps), lambda: qk_norm_rotary_vjp(x, x, *args, eps=eps)):
+        with pytest.raises(ValueError, match="eps"):
+            call()
