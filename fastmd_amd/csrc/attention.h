@@ -229,7 +229,8 @@ struct AttnTile {
 
 // An infinity or a NaN in a row of a tile must not reach a lane that does not see the row, and a weight of zero would not
 // keep it out of a matrix product. Tiles that some lane does not see all of (causal calls) are looked through for such rows;
-// where there are any, the products take the finite values alone, and the rows' weights are NaN for the lanes that see them.
+// where there are any, the products take the finite values alone, and a lane that sees such a row has NaN in the columns of the others
+// (in a tile that all see, the product leaves NaN or an infinity there).
 
 // bits of the rows (of 32) of a tile that hold a value that is not finite, for the whole wave (of the first plane: what rounds
 // to an infinity counts as one)
@@ -269,6 +270,27 @@ __device__ __forceinline__ Planes<NP> finite_part(Planes<NP> x) {
     x.p[p] = __builtin_bit_cast(fmd_bf16x8, v);
   }
   return x;
+}
+
+// NaN in the sums of every column in which one of `rows` (bits) of a tile holds a value that is not finite, for lanes that see the
+// row: from <= row < to. Sums as a 32 x 32 product holds them, a column block each.
+template <typename Tile, int DB>
+__device__ __forceinline__ void mark_not_finite(fmd_f32x16 (&o)[DB], const __bf16* s, uint32_t rows, int from, int to) {
+  const int half = (threadIdx.x & 63) >> 5;
+  for (; rows; rows &= rows - 1) {
+    const int row = __builtin_ctz(rows);
+    const bool sees = row >= from && row < to;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint2 x = *reinterpret_cast<const uint2*>(s + Tile::at(row, 4 * d + r) + 4 * half);
+        const uint32_t e[4] = {x.x << 16, x.x, x.y << 16, x.y};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (sees && (e[k] & 0x7f800000u) == 0x7f800000u) o[d][4 * r + k] = NAN;
+      }
+  }
 }
 
 // Rows of a tile on their way to LDS: THREADS threads load NV chunks each (issued together, written after the

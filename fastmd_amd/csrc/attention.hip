@@ -159,17 +159,10 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
         sum[v & 1] += p;
       }
     l += sum[0] + sum[1];  // of this lane's half of the keys
-    uint32_t bad = 0;
+    uint32_t bad[JB] = {}, any_bad = 0;
     if (kLast && CAUSAL && j0 + BN > least) {
-      const int left = sees - j0 - 4 * half;
 #pragma unroll
-      for (int j = 0; j < JB; ++j) {
-        const uint32_t rows = rows_not_finite<Tile>(vs_ + 32 * j * Tile::LD), mine = rows >> 4 * half;
-        bad |= rows;
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (32 * j + prod_row(v, 0) < left && mine >> prod_row(v, 0) & 1) s[j][v] = NAN;
-      }
+      for (int j = 0; j < JB; ++j) any_bad |= bad[j] = rows_not_finite<Tile>(vs_ + 32 * j * Tile::LD);
     }
 #pragma unroll
     for (int j = 0; j < JB; ++j)
@@ -184,11 +177,15 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           Planes<NP> vc = Tile::cols(vs_, lc, 32 * j + 16 * step, d);
-          if (kLast && CAUSAL && bad) vc = finite_part<NP>(vc);
+          if (kLast && CAUSAL && any_bad) vc = finite_part<NP>(vc);
           o[d] = mma(vc, pf, o[d]);
           if (kTwoParts) o[d] = mma(vc, rest, o[d]);
         }
       }
+    if (kLast && CAUSAL && any_bad) {
+#pragma unroll
+      for (int j = 0; j < JB; ++j) mark_not_finite<Tile>(o, vs_ + 32 * j * Tile::LD, bad[j], 0, sees - j0 - 32 * j);
+    }
   };
 
   const int rounds = (tile_hi - tile_lo + KW - 1) / KW;  // the same for every wave
@@ -525,12 +522,9 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
     }
     if (kPartial && r0 < full) {
       const int hidden = from - r0 - 4 * half;
-      const uint32_t mine = bad >> 4 * half;
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        if (mine >> prod_row(v, 0) & 1) s[v] = dp[v] = NAN;
+      for (int v = 0; v < 16; ++v)
         if (prod_row(v, 0) < hidden) s[v] = dp[v] = 0.f;
-      }
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
@@ -555,6 +549,10 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
         ak[d] = mma(qc, df, ak[d]);
         if (kTwoParts) ak[d] = mma(qc, df_rest, ak[d]);
       }
+    }
+    if (kPartial && bad) {
+      mark_not_finite<Tile>(av, gs, bad, from - r0, BR);
+      mark_not_finite<Tile>(ak, qs, bad, from - r0, BR);
     }
   };
 
@@ -773,12 +771,9 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
       if (kLast && j0 + 32 > least) {
         const int left = sees - j0 - 4 * half;
         if (CAUSAL) bad = rows_not_finite<Tile>(ks_ + jb * Tile::LD);
-        const uint32_t mine = bad >> 4 * half;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-          if (mine >> prod_row(v, 0) & 1) s[v] = NAN;
+        for (int v = 0; v < 16; ++v)
           if (prod_row(v, 0) >= left) s[v] = 0.f;
-        }
       }
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
@@ -796,6 +791,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
           if (kTwoParts) o[d] = mma(kc, rest, o[d]);
         }
       }
+      if (kLast && CAUSAL && bad) mark_not_finite<Tile>(o, ks_ + jb * Tile::LD, bad, 0, sees - j0);
     }
   };
   const int rounds = (max(0, tile_hi - tile_lo) + KW - 1) / KW;

@@ -11,10 +11,11 @@ synchronises nor depends on lengths that the host would have to know. ``group = 
 key head. ``causal``: the last query of a segment sees all its keys, each one before it one key less. A query that sees
 no key, and a row outside every segment (the unused rows of a fixed-capacity buffer), gives zero and gets zero gradient;
 rows outside a query's segment are not read for it, whatever they hold, and neither an infinity nor a NaN in a key row that a
-causal query does not see reaches it (nor, in the VJP, one in a query's row the keys that it does not see).
+causal query does not see reaches it (nor, in the VJP, one in a query's row the keys that it does not see). One that is seen
+makes the results that it is a term of NaN or infinite (a value its own column), and no others.
 
-float32 is computed on the bf16 matrix cores with every operand split into three planes (float32 accuracy; an
-infinite value in a row that is seen gives NaN), bfloat16 with products of bfloat16 operands. Scores, softmax statistics
+float32 is computed on the bf16 matrix cores with every operand split into three planes (float32 accuracy), bfloat16 with
+products of bfloat16 operands. Scores, softmax statistics
 and sums are float32 in both. For bfloat16, the probabilities and (in the VJP) the score gradients are operands of the
 second product in two bfloat16 parts (16 bits), so that each result is as near to the exact one as its one rounding allows.
 Gradients take no atomics: the same call gives the same bits.

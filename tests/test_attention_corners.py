@@ -76,3 +76,49 @@ def test_both_directions_of_the_norm_refuse_an_eps(eps):
     for call in (lambda: qk_norm_rotary(*args, eps=eps), lambda: qk_norm_rotary_vjp(x, x, *args, eps=eps)):
         with pytest.raises(ValueError, match="eps"):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim", [([80, 45], 2, 1, 32), ([150, 61], 4, 4, 64), ([1500, 900], 16, 4, 64),
+                                                        ([1300, 1500], 16, 16, 32), ([900, 1000], 4, 4, 64),
+                                                        ([1300, 900], 16, 4, 128), ([700], 6, 2, 96), ([1] * 300, 2, 2, 32)])
+def test_a_value_that_is_not_finite_reaches_its_own_column_only(lengths, heads, kv_heads, dim, causal, dtype):
+    """Infinities and NaN in single columns of some values: those columns of the rows that see them are not finite, and every other
+    result is bit for bit that without them, in tiles that all rows see and in those that some do not. The same for the
+    gradient of the output and the values' gradient."""
+    from fastmd_amd.ops.attention import segment_attention_forward, segment_attention_vjp
+    from test_attention import make
+
+    q, k, v, g, off, _ = (x.cuda() for x in make(lengths, lengths, heads, kv_heads, dim, dtype, seed=dim))
+    run = lambda v: segment_attention_forward(q, k, v, off, causal=causal)  # noqa: E731
+    want, saved = run(v)
+    gen = torch.Generator().manual_seed(dim)
+    rows = v.shape[0]
+    odd, spoilt = v.clone(), torch.zeros(v.shape, dtype=torch.bool, device="cuda")
+    odd_g, spoilt_g = g.clone(), torch.zeros(g.shape, dtype=torch.bool, device="cuda")
+    for n in range(12):
+        row, col, value = int(torch.randint(rows, (1,), generator=gen)), n % dim, (float("inf"), -float("inf"), float("nan"))[n % 3]
+        odd[row, n % kv_heads, col], spoilt[row, n % kv_heads, col] = value, True
+        odd_g[row, n % heads, col], spoilt_g[row, n % heads, col] = value, True
+    segment = torch.searchsorted(off[1:], torch.arange(rows, device="cuda"), right=True)
+    sees = segment[:, None] == segment[None]
+    if causal:
+        sees &= torch.arange(rows, device="cuda")[:, None] >= torch.arange(rows, device="cuda")[None]
+    group = heads // kv_heads
+    reached = lambda mask, by: (by.float() @ mask.float().flatten(1)).view(-1, *mask.shape[1:]) > 0  # noqa: E731
+    hit = reached(spoilt, sees).repeat_interleave(group, 1)
+    got = run(odd)[0]
+    assert not torch.isfinite(got[hit]).any()
+    assert torch.equal(got[~hit], want[~hit])
+
+    vjp = lambda g: segment_attention_vjp(g, q, k, v, want, saved, off, causal=causal)  # noqa: E731
+    plain, grads = vjp(g), vjp(odd_g)
+    hit = reached(spoilt_g, sees.T).view(rows, kv_heads, group, dim).any(2)
+    assert not torch.isfinite(grads[2][hit]).any()
+    assert torch.equal(grads[2][~hit], plain[2][~hit])
+    rows_hit = spoilt_g.any(2)
+    assert torch.equal(grads[0][~rows_hit], plain[0][~rows_hit])
+    keys_hit = reached(rows_hit, sees.T).view(rows, kv_heads, group).any(2)
+    assert torch.equal(grads[1][~keys_hit], plain[1][~keys_hit])
