@@ -67,7 +67,7 @@ struct AttnTiles {
 };
 
 constexpr int kWaitVm0 = 0 | (7 << 4) | (15 << 8);  // s_waitcnt vmcnt(0)
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnSegment {
   int64_t q0, k0;
