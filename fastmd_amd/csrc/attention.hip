@@ -24,9 +24,14 @@ static constexpr int attn_waves(int planes, int dp, int sums) { return planes * 
 // in prompts of 12 000 causal rows of 16 heads of 128, forward and VJP of 8 192 such rows 535 -> 674; where memory bounds, nothing.
 template <int NP>
 __device__ __forceinline__ Planes<NP> rest_of(const float (&x)[8], const Planes<NP>& first) {
+  const uint4 w = __builtin_bit_cast(uint4, first.p[0]);  // the parts as they lie in pairs: unpacked, not converted one by one again
+  const uint32_t pair[4] = {w.x, w.y, w.z, w.w};
   float y[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = x[e] - (float)first.p[0][e];
+  for (int e = 0; e < 4; ++e) {
+    y[2 * e] = x[2 * e] - __uint_as_float(pair[e] << 16);
+    y[2 * e + 1] = x[2 * e + 1] - __uint_as_float(pair[e] & 0xffff0000u);
+  }
   Planes<NP> o;
   planes_of(y, o);
   return o;
@@ -104,7 +109,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const float c = a.scale * kLog2e;
 
   const int lt = threadIdx.x - kw * WM * 64;  // thread among those that load this group's tiles
-  // The maximum follows the scores only where one outgrows it by kSlack (in log2 units; 117 us against 125 of following
+  // The maximum follows the scores only where one outgrows it by kSlack (in log2 units; 165 us against 171 of following
   // always, 4 x 3 000 rows, 8 heads of 64, bf16): exponentials up to 2^kSlack are
   // as exact as those below one, and the sums are rescaled a few times per row instead of once per tile.
   constexpr float kSlack = 8.f;
@@ -926,15 +931,14 @@ int64_t tile_count(int64_t rows, int group, int segments, int bm) { return rows 
 // 32 rows and share the keys, for calls with too few tiles to fill the card otherwise and segments not much longer than a
 // tile. kMid: two and two, fp32 only, whose narrow form splits every tile into planes in the wave that reads it (fp32 heads
 // above 64 have room in LDS for wide tiles alone, and two narrow waves).
-// Measured, us of forward + both halves of the VJP (bf16 narrow with weights in one part; the second adds 5 to 10 %, a quarter to
-// gk and gv at 1 000 blocks of 64 columns):
-//   one segment, bf16, 8 heads of 64: 2 000 rows narrow 87, wide 127; 4 000 rows 253, 245; 8 000 rows 868, 722
-//   ", 8 heads of 128: 1 000 rows 77, 110; 2 000 rows 227, 183; 4 000 rows 795, 372
+// Measured, us of forward + both halves of the VJP:
+//   one segment, bf16, 8 heads of 64: 2 000 rows narrow 104, wide 150; 4 000 rows 314, 318; 8 000 rows 1 086, 972
+//   ", 8 heads of 128: 1 000 rows 82, 122; 2 000 rows 243, 213; 4 000 rows 859, 461
 //   ", fp32, 4 heads of 32: 2 000 rows narrow 122, mid 135, wide 142; 4 000 rows 325, 300, 436; 8 000 rows 1 157, 913, 1 063
 //   ", 4 heads of 64: 1 000 rows 99, 125, 185; 2 000 rows 198, 178, 196; 8 000 rows 2 753, 1 734, 1 619
 //   ", 4 heads of 128: 1 000 rows narrow 320, wide 304; 2 000 rows 805, 296
 //   64 segments, 4 heads of 32, fp32: 80 rows narrow 54, mid 82, wide 67; 160 rows 102, 118, 105; 320 rows 210, 215, 193;
-//   bf16: 80 rows 50, -, 50; 160 rows 53, -, 54; 320 rows 90, -, 82
+//   bf16: 80 rows 49, -, 50; 160 rows 57, -, 62; 320 rows 101, -, 106; 40 segments, 4 heads of 64, 200 rows 77, -, 70; 400 rows 156, -, 135
 enum AttnShape { kNarrow, kMid, kWide };
 
 AttnShape shape_of(bool f32, int dim, int64_t rows, int heads, int segments) {
@@ -1038,10 +1042,10 @@ AttnTiles bf16_tiles(const void* x, int64_t x_row, int64_t x_head, const void* y
 template <typename T, int DP, bool CAUSAL>
 int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
-  // Keys of a wide tile: 64 (4 x 3 000 rows, 8 heads, bf16: 148 us against 165 of 32 keys at 96 columns, 117 against 128 at 64;
-  // fp32 at 32: 234 against 282), but 32 where more has no registers (fp32 above 32) or costs the third wave of a SIMD in
-  // long causal calls (five prompts of 12 000 rows together, 16 heads of 128: 237 us against 250; one full segment of 4 000: 105 against 88).
-  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = (f32 && DP > 32) || (CAUSAL && DP > 96) ? 32 : 64;
+  // Keys of a wide tile: 64 (4 x 3 000 rows, 8 heads, bf16: 184 us against 220 of 32 keys at 96 columns, 165 against 169 at 64, 226
+  // against 220 at 128; causal, 16 heads of 128: one segment of 4 000 rows 128 against 141, five prompts of 12 000 together 330 against
+  // 328; fp32 at 32: 234 against 282), but 32 where more has no registers (fp32 above 32).
+  constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = f32 && DP > 32 ? 32 : 64;
   const int64_t n = a.tq * a.heads;
   AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);
   const AttnShape shape = shape_of(f32, a.dim, a.tq * a.group, a.kv_heads, a.segments);
