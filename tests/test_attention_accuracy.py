@@ -46,3 +46,31 @@ def ratios(lq, lk, heads, kv_heads, dim, causal, seed):
 def test_results_are_rounded_once(lq, lk, heads, kv_heads, dim, causal):
     for name, ratio in ratios(lq, lk, heads, kv_heads, dim, causal, seed=dim).items():
         assert ratio <= BOUND, f"{name}: {ratio:.3f} times the error of rounding the exact result"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 64), (16, 4, 128)])
+def test_first_rows_of_long_causal_sequences(heads, kv_heads, dim):
+    """The rows that see few keys, in the tiles of calls with many."""
+    from fastmd_amd.ops.attention import segment_attention_forward
+
+    q, k, v, _, off, _ = make([1900, 1900], [1900, 1900], heads, kv_heads, dim, torch.bfloat16, seed=dim)
+    out, _ = segment_attention_forward(*(x.cuda() for x in (q, k, v, off)), causal=True)
+    for start in (0, 1900):
+        few = slice(start, start + 60)  # causal: they see each other only
+        want = oracle.segment_attention(q[few], k[few], v[few], [0, 60], [0, 60], causal=True)["out"]
+        once = float((want.bfloat16().double() - want).square().sum().sqrt())
+        assert float((out[few].double().cpu() - want).square().sum().sqrt()) <= BOUND * once
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk", [([64] * 60, [64] * 60), ([245], [245]), ([1] * 70, [9] * 70)])
+def test_the_saved_residual_is_what_the_outputs_rounding_dropped(lq, lk):
+    """out + residual has 16 bits of the exact output: 2^-16 of its size, and the weights' and scores' 2^-16 of the terms."""
+    from fastmd_amd.ops.attention import segment_attention_forward
+
+    q, k, v, _, q_off, k_off = make(lq, lk, 8, 8, 64, torch.bfloat16)
+    r = oracle.segment_attention(q, k, v, q_off, k_off)
+    out, saved = segment_attention_forward(*(x.cuda() for x in (q, k, v, q_off, k_off)))
+    far = (out.double() + saved.residual.double()).cpu() - r["out"]
+    assert bool((far.abs() <= 2.0 ** -16 * r["out"].abs() + 2.0 ** -15 * r["abs_out"] + 1e-30).all())
