@@ -20,8 +20,9 @@ static constexpr int attn_waves(int planes, int dp, int sums) { return planes * 
 // bf16 weights (P, dS) are two bf16 parts, the second what the rounding of the first dropped (16 bits together): a product more
 // of two forward, of three for gq and two more of four for gk and gv. With one part the rounding of the weights is as large as that of the
 // result, however many keys a row has (the terms' errors and the terms add up alike), and the results were 1.4 times as far from
-// the exact ones as those rounded once; with two they are as near. It costs 308 -> 430 us at 10 000 rows of 8 heads of 64, 261 -> 374
-// in prompts of 12 000 causal rows of 16 heads of 128, forward and VJP of 8 192 such rows 535 -> 674; where memory bounds, nothing.
+// the exact ones as those rounded once; with two they are as near. It costs, on one box, 287 -> 396 us at 10 000 rows of 8 heads of
+// 64, 247 -> 329 in prompts of 12 000 causal rows of 16 heads of 128, 495 -> 608 forward and VJP of 8 192 such rows; where memory bounds,
+// nothing.
 template <int NP>
 __device__ __forceinline__ Planes<NP> rest_of(const float (&x)[8], const Planes<NP>& first) {
   const uint4 w = __builtin_bit_cast(uint4, first.p[0]);  // the parts as they lie in pairs: unpacked, not converted one by one again
@@ -45,11 +46,12 @@ __device__ __forceinline__ Planes<NP> rest_of(const float (&x)[8], const Planes<
 // sums over keys stay in the lane but for one exchange of the halves, and exp(S^T) is already the operand of
 // O^T = V^T P^T. Statistics and sums are fp32; P is kept in two bf16 parts for bf16 inputs and as three planes
 // for fp32.
-// Measured: bf16, 10 000 rows, 8 heads of 64: 281 us, 727 TFLOP/s (a large library product 1 125): the matrix pipes are busy
-// 37 % of the time, the vector ones with the exponentials (quarter rate), their arguments, maxima and sums for most of the rest, and
-// waves of a SIMD overlap the two in part. 5 prompts of 12 000 causal rows together, 16 heads of 128: 242 us, 870 TFLOP/s. fp32,
-// 16 systems of 16 875 rows, 4 heads of 32: 97-103 us, 120 TFLOP/s (the library's fp32 154; six bf16 products each, and as much
-// again for splitting P). One query each over 16 x 40 000 keys, 4 heads of 128, bf16: 234 us, 5.6 TB/s, memory.
+// Measured: bf16, 10 000 rows, 8 heads of 64: 396-404 us, 510 TFLOP/s of the 4 D operations, 770 with the second part's (a large
+// library product 1 125): the matrix pipes are busy 40 % of the time, the vector ones with the exponentials (quarter rate), their
+// arguments, maxima, sums and parts for most of the rest, and waves of a SIMD overlap the two in part. 5 prompts of 12 000 causal rows
+// together, 16 heads of 128: 329-341 us, 630 TFLOP/s (940). fp32, 16 systems of 16 875 rows, 4 heads of 32: 95-103 us, 120 TFLOP/s (the
+// library's fp32 154; six bf16 products each, and as much again for splitting P). One query each over 16 x 40 000 keys, 4 heads of 128,
+// bf16: 235 us, 5.6 TB/s, memory.
 template <typename T, int DP, int BN, int WM, int KW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_fwd_kernel(AttnArgs a, AttnTiles kv,
                                                                 int64_t tiles, int splits, T* out, AttnSaved saved,
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, 
   const float c = a.scale * kLog2e;
 
   const int lt = threadIdx.x - kw * WM * 64;  // thread among those that load this group's tiles
-  // The maximum follows the scores only where one outgrows it by kSlack (in log2 units; 165 us against 171 of following
+  // The maximum follows the scores only where one outgrows it by kSlack (in log2 units; 161 us against 166 of following
   // always, 4 x 3 000 rows, 8 heads of 64, bf16): exponentials up to 2^kSlack are
   // as exact as those below one, and the sums are rescaled a few times per row instead of once per tile.
   constexpr float kSlack = 8.f;
@@ -400,9 +402,9 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // tiles rw, rw + RW, ... of 32 queries, of one query head of the group after the other. S = Q K^T (lane: a key, registers:
 // query rows), so exp(S - lse) and dS are the operands of gv^T = G^T P and gk^T = Q^T dS, whose sums run over all query heads of
 // the group. For bf16, P and dS are operands in two bf16 parts; sums are fp32.
-// Measured: bf16, causal, 4 sequences of 8 192 rows together, 16 heads on 4 of 128: 216 us, 680 TFLOP/s, matrix pipes busy 38 % of
-// the time: two waves a SIMD, for which the two sums take half of the registers, wait on each other's rounds. fp32, 5 systems of
-// 5 000 rows, 4 heads of 64: 145 us, 112 TFLOP/s. Two waves of keys and four of rows in one workgroup, so that a tile's copy
+// Measured: bf16, causal, 4 sequences of 8 192 rows together, 16 heads on 4 of 128: 280 us, 525 TFLOP/s of the 8 D operations, 790
+// with the second parts', matrix pipes busy 47 % of the time: two waves a SIMD, for which the two sums take half of the
+// registers, wait on each other's rounds. fp32, 5 systems of 5 000 rows, 4 heads of 64: 150 us, 150 TFLOP/s. Two waves of keys and four of rows in one workgroup, so that a tile's copy
 // serves both and each SIMD has two waves.
 template <typename T, int DP, int WM, int RW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
@@ -699,7 +701,8 @@ __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : a
 }
 
 // Gradient of the queries: the forward's walk with S^T = K Q^T and dP^T = V G^T, then gq^T = K^T dS^T (dS in two parts for
-// bf16). Measured in the cases above: bf16 128 us, 855 TFLOP/s, matrix pipes busy 48 % of the time; fp32 110 us, 112 TFLOP/s.
+// bf16). Measured in the cases above: bf16 160 us, 690 TFLOP/s of the 6 D operations, 920 with the second part's, matrix pipes busy 54 %
+// of the time; fp32 113 us, 149 TFLOP/s.
 template <typename T, int DP, int WM, int KW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * KW, attn_waves(AttnType<T>::planes, DP, 1)) attn_bwd_q_kernel(AttnArgs a, AttnBwd b, AttnTiles kv,
                                                                                              int64_t tiles, int splits, float* part, T* gq) {
@@ -932,13 +935,13 @@ int64_t tile_count(int64_t rows, int group, int segments, int bm) { return rows 
 // tile. kMid: two and two, fp32 only, whose narrow form splits every tile into planes in the wave that reads it (fp32 heads
 // above 64 have room in LDS for wide tiles alone, and two narrow waves).
 // Measured, us of forward + both halves of the VJP:
-//   one segment, bf16, 8 heads of 64: 2 000 rows narrow 104, wide 150; 4 000 rows 314, 318; 8 000 rows 1 086, 972
-//   ", 8 heads of 128: 1 000 rows 82, 122; 2 000 rows 243, 213; 4 000 rows 859, 461
+//   one segment, bf16, 8 heads of 64: 2 000 rows narrow 101, wide 148; 4 000 rows 307, 308; 8 000 rows 1 110, 976
+//   ", 8 heads of 128: 1 000 rows 83, 123; 2 000 rows 242, 212; 4 000 rows 853, 475
 //   ", fp32, 4 heads of 32: 2 000 rows narrow 122, mid 135, wide 142; 4 000 rows 325, 300, 436; 8 000 rows 1 157, 913, 1 063
 //   ", 4 heads of 64: 1 000 rows 99, 125, 185; 2 000 rows 198, 178, 196; 8 000 rows 2 753, 1 734, 1 619
 //   ", 4 heads of 128: 1 000 rows narrow 320, wide 304; 2 000 rows 805, 296
 //   64 segments, 4 heads of 32, fp32: 80 rows narrow 54, mid 82, wide 67; 160 rows 102, 118, 105; 320 rows 210, 215, 193;
-//   bf16: 80 rows 49, -, 50; 160 rows 57, -, 62; 320 rows 101, -, 106; 40 segments, 4 heads of 64, 200 rows 77, -, 70; 400 rows 156, -, 135
+//   bf16: 80 rows 53, -, 54; 160 rows 57, -, 63; 320 rows 100, -, 104; 40 segments, 4 heads of 64, 200 rows 77, -, 70; 400 rows 155, -, 133
 enum AttnShape { kNarrow, kMid, kWide };
 
 AttnShape shape_of(bool f32, int dim, int64_t rows, int heads, int segments) {
@@ -964,8 +967,8 @@ bool few_rows(int64_t tq, int64_t tk, int segments) {
 
 // Key splits of the forward: as many as bring the workgroups to one per CU, each with kSplitKeys keys at least of a
 // segment of mean length. Their partial sums (dim + 2 floats a row) are joined by a second launch. Measured, us for one split,
-// the taken number and twice as many: one query over 10 000 keys, fp32 245, 26 (19), 22; over 40 000, 16 heads on 4, bf16 501, 36
-// (64), -; 16 such 600, 234 (4), 238; 2 000 rows of 1 head, fp32 55, 29 (3), 33; 2 000 rows of 8 heads, bf16 42 (1), 61.
+// the taken number and twice as many: one query over 10 000 keys, fp32 245, 26 (19), 22; over 40 000, 16 heads on 4, bf16 538, 37
+// (64), -; 16 such 616, 235 (4), 237; 2 000 rows of 1 head, fp32 55, 29 (3), 33; 2 000 rows of 8 heads of 64, bf16 28 (1), 40.
 constexpr int kSplitKeys = 512, kSplitGroups = 256;
 
 int split_count(bool f32, int dim, int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
@@ -991,8 +994,8 @@ int64_t forward_floats(bool bf16, int splits, int64_t tq, int64_t tk, int segmen
 }
 
 // Splits of the VJP's walks, for as few workgroups: of the query rows for gk and gv, and of the keys for gq. Measured, us
-// for one split, the taken number and twice as many: 2 000 causal rows of 8 heads on one of 128, bf16, gk and gv 281, 89 (4), 98;
-// 2 000 rows of one head of 64, fp32, 75, 33 (4), 42 and gq 66, 35 (3), 40; 10 000 rows of 8 heads of 64, bf16, 501 (1), 541.
+// for one split, the taken number and twice as many: 2 000 causal rows of 8 heads on one of 128, bf16, gk and gv 303, 96 (4), 105;
+// 2 000 rows of one head of 64, fp32, 75, 33 (4), 42 and gq 66, 35 (3), 40; 10 000 rows of 8 heads of 64, bf16, 689 (1), 725.
 constexpr int kSplitRows = 256;
 
 int row_splits(bool f32, int dim, int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
@@ -1042,9 +1045,9 @@ AttnTiles bf16_tiles(const void* x, int64_t x_row, int64_t x_head, const void* y
 template <typename T, int DP, bool CAUSAL>
 int run_fwd(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float* work, hipStream_t stream) {
   constexpr bool f32 = AttnType<T>::planes == 3;
-  // Keys of a wide tile: 64 (4 x 3 000 rows, 8 heads, bf16: 184 us against 220 of 32 keys at 96 columns, 165 against 169 at 64, 226
-  // against 220 at 128; causal, 16 heads of 128: one segment of 4 000 rows 128 against 141, five prompts of 12 000 together 330 against
-  // 328; fp32 at 32: 234 against 282), but 32 where more has no registers (fp32 above 32).
+  // Keys of a wide tile: 64 (4 x 3 000 rows, 8 heads, bf16: 182 us against 221 of 32 keys at 96 columns, 161 against 170 at 64, 219
+  // against 222 at 128; causal, 16 heads of 128: one segment of 4 000 rows 130 against 143, five prompts of 12 000 together 337 against
+  // 332; fp32 at 32: 234 against 282), but 32 where more has no registers (fp32 above 32).
   constexpr int kKeyWaves = f32 && DP > 64 ? 2 : 4, kWideKeys = f32 && DP > 32 ? 32 : 64;
   const int64_t n = a.tq * a.heads;
   AttnTiles t = bf16_tiles(a.k, a.k_row, a.k_head, a.v, a.v_row, a.v_head);

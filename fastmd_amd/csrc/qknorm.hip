@@ -5,7 +5,7 @@
 // A row (one head of one token) belongs to a group of LG lanes, eight columns each: one read, one write, the mean by
 // lane exchanges. The angles come from tables, one row for all heads of a token. All arithmetic is fp32, each output rounded
 // once. Memory bounds both directions (of a large copy's 4.8 TB/s): 40 000 tokens of 20 heads of 128, bf16, half of the columns
-// turned, 83 us forward (5.0 TB/s), 192 VJP (3.2); 16 875 tokens of 16 heads of 64, fp32, 26 us (5.2) and 42 (5.0, with the
+// turned, 84-87 us forward (4.9 TB/s), 192 VJP (3.2); 16 875 tokens of 16 heads of 64, fp32, 27 us (5.1) and 43 (4.9, with the
 // weights' gradients); below some 2 000 rows the host's time for a launch does. The bf16 VJP issues as many instructions as its
 // loads can hide: units counted in 32 bits instead of 64, and the reciprocal root in one instruction, took 5 % off it.
 #include "attention.h"
@@ -43,7 +43,8 @@ __device__ __forceinline__ float group_sum(float x) {
 }
 
 // How the other column of a pair is reached: neighbours of a lane; the same place of another lane of the group (rot / 2 a
-// multiple of eight); anywhere.
+// multiple of eight); anywhere, by eight exchanges a column, which then bound it (16 875 tokens of 16 heads of 64, fp32, 20 columns
+// turned 40 us forward and 62 VJP, 64 columns 27 and 43; 40 000 of 20 heads of 128, bf16, 40 columns 139 and 273, 64 neighbouring 84 and 194).
 enum Turn { kNone, kNeighbours, kLanes, kAnywhere };
 
 __device__ __forceinline__ int64_t table_row(const NormArgs& a, int64_t tok) {
