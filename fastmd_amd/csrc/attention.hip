@@ -20,7 +20,7 @@ static constexpr int attn_waves(int planes, int dp, int sums) { return planes * 
 // bf16 weights (P, dS) are two bf16 parts, the second what the rounding of the first dropped (16 bits together): a product more
 // of two forward, of three for gq and two more of four for gk and gv. With one part the rounding of the weights is as large as that of the
 // result, however many keys a row has (the terms' errors and the terms add up alike), and the results were 1.4 times as far from
-// the exact ones as those rounded once; with two they are as near. It costs, on one box, 287 -> 396 us at 10 000 rows of 8 heads of
+// the exact ones as those rounded once; with two they are as near. It costs, on one card, 287 -> 396 us at 10 000 rows of 8 heads of
 // 64, 247 -> 329 in prompts of 12 000 causal rows of 16 heads of 128, 495 -> 608 forward and VJP of 8 192 such rows; where memory bounds,
 // nothing.
 template <int NP>
@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(AttnBwd b, int64_t tq, 
 // the group. For bf16, P and dS are operands in two bf16 parts; sums are fp32.
 // Measured: bf16, causal, 4 sequences of 8 192 rows together, 16 heads on 4 of 128: 280 us, 525 TFLOP/s of the 8 D operations, 790
 // with the second parts', matrix pipes busy 47 % of the time: two waves a SIMD, for which the two sums take half of the
-// registers, wait on each other's rounds. fp32, 5 systems of 5 000 rows, 4 heads of 64: 150 us, 150 TFLOP/s. Two waves of keys and four of rows in one workgroup, so that a tile's copy
-// serves both and each SIMD has two waves.
+// registers, wait on each other's rounds. fp32, 5 systems of 5 000 rows, 4 heads of 64: 150 us, 150 TFLOP/s. Two waves of keys
+// and four of rows in one workgroup, so that a tile's copy serves both and each SIMD has two waves.
 template <typename T, int DP, int WM, int RW, bool DMA, bool CAUSAL>
 __global__ void __launch_bounds__(64 * WM * RW, AttnType<T>::planes == 1 ? 2 : attn_waves(AttnType<T>::planes, DP, 2)) attn_bwd_kv_kernel(AttnArgs a, AttnBwd b, AttnTiles qg,
                                                                                               int splits, float* part, T* gk, T* gv) {
