@@ -960,8 +960,16 @@ constexpr int shape_rows(AttnShape s) { return s == kWide ? 128 : s == kMid ? 64
 //   1 024 of 500 338 (455); bf16: 54 (456), 42 (49), 115 (113), 269 (845), 224 (520)
 //   8 heads of 128, fp32: 153 segments of 21 keys 47 (240), of 64 104 (223), of 128 202 (404); bf16 47 (150), 113 (216), 212 (236);
 //   8 heads of 32, 40 of 21 44 (48)
-bool few_rows(int64_t tq, int64_t tk, int segments) {
-  const int64_t keys = segments >= 1024 ? 512 : segments >= 256 ? 128 : 64;
+// These are of groups whose heads a wave takes together (1, 2 and 4; of 4: fp32, 256 segments of 128 keys, 4 heads on one of 64, 35 (95);
+// bf16, 1 024 of 500, 16 heads on 4 of 128, 1 284 (2 412)). Of other groups it walks the keys for each head, and many segments of few keys
+// are left to it: 8 heads on one of 64, fp32: 10 000 segments of 18 keys 285 (1 530), 600 of 60 91 (148), 1 100 of 128 264 (372), 300 of 20
+// 46 (69), 256 of 128 160 (116), 1 024 of 500 912 (834), 100 of 60 88 (43); bf16: 10 000 of 18 201 (471), 600 of 20 48 (45), 2 000 of 100
+// 225 (253), 1 100 of 60 108 (87), 300 of 20 47 (36), 256 of 128 176 (52), 1 024 of 500 863 (396); 16 heads on 2 of 128, bf16: 10 000 of 18
+// 757 (2 725), 600 of 20 119 (170), 2 000 of 100 972 (852).
+bool few_rows(bool f32, int64_t tq, int64_t tk, int segments, int group) {
+  const bool together = group == 1 || group == 2 || group == 4;
+  const int64_t keys = together ? (segments >= 1024 ? 512 : segments >= 256 ? 128 : 64)
+                                : (segments >= 512 ? (f32 ? 128 : 32) : f32 && segments >= 256 ? 32 : 0);
   return tq <= segments && tk <= keys * segments;
 }
 
@@ -973,8 +981,8 @@ constexpr int kSplitKeys = 512, kSplitGroups = 256;
 
 int split_count(bool f32, int dim, int64_t tq, int64_t tk, int segments, int heads, int kv_heads) {
   if (tq <= 0 || tk <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
-  if (few_rows(tq, tk, segments)) return 1;
   const int group = heads / kv_heads;
+  if (few_rows(f32, tq, tk, segments, group)) return 1;
   const int rows = shape_rows(shape_of(f32, dim, tq * group, kv_heads, segments));
   const int64_t tiles = fmd_cdiv(fmd_cdiv(tq * group, segments), rows) * segments * kv_heads;
   const int64_t fill = kSplitGroups / tiles, most = tk / segments / kSplitKeys;
@@ -988,7 +996,7 @@ int64_t planes_floats(int64_t rows, int heads, int dim) { return rows * heads * 
 
 int64_t forward_floats(bool bf16, int splits, int64_t tq, int64_t tk, int segments, int heads, int kv_heads, int dim) {
   if (tq <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads) return 0;
-  const bool planes = !bf16 && !few_rows(tq, tk, segments) &&
+  const bool planes = !bf16 && !few_rows(true, tq, tk, segments, heads / kv_heads) &&
                       shape_of(true, dim, tq * (heads / kv_heads), kv_heads, segments) != kNarrow;
   return (planes ? planes_floats(tk, kv_heads, dim) : 0) + (splits > 1 ? (int64_t)splits * tq * heads * (dim + 2) : 0);
 }
@@ -1011,7 +1019,7 @@ int64_t backward_floats(bool bf16, int64_t tq, int64_t tk, int segments, int hea
                         int kv_splits) {
   if (heads <= 0 || kv_heads <= 0 || dim <= 0 || heads % kv_heads || tq < 0 || tk < 0) return 0;
   int64_t n = fmd_cdiv(2 * heads * tq, 4) * 4;  // offsets and deltas
-  if (few_rows(tq, tk, segments)) return n;
+  if (few_rows(!bf16, tq, tk, segments, heads / kv_heads)) return n;
   if (!bf16) {
     if (shape_of(true, dim, tq * (heads / kv_heads), kv_heads, segments) != kNarrow) n += planes_floats(tk, kv_heads, dim);
     if (shape_of(true, dim, tk, kv_heads, segments) != kNarrow) n += planes_floats(tq, heads, dim);
@@ -1180,7 +1188,7 @@ int forward(const AttnArgs& a, int splits, T* out, const AttnSaved& saved, float
   FMD_REQUIRE(splits >= 1 && splits <= kMaxSplits && aligned16(work));
   if (a.tq == 0) return FMD_OK;
   FMD_REQUIRE(out && aligned16(out) && aligned16(saved.residual) && (saved.base == nullptr) == (saved.inverse == nullptr));
-  if (few_rows(a.tq, a.tk, a.segments)) return attn_rows_fwd<T>(a, out, saved, stream);
+  if (few_rows(sizeof(T) == 4, a.tq, a.tk, a.segments, a.group)) return attn_rows_fwd<T>(a, out, saved, stream);
   FMD_BY_WIDTH(run_fwd, a, splits, out, saved, work, stream)
 }
 
@@ -1198,7 +1206,7 @@ int backward(const AttnArgs& a, AttnBwd b, int q_splits, int kv_splits, T* gq, T
   b.rows = work;
   if (a.tq == 0) gq = nullptr;
   if (a.tk == 0) gk = gv = nullptr;
-  if (few_rows(a.tq, a.tk, a.segments)) return attn_rows_bwd<T>(a, b, gq, gk, gv, stream);
+  if (few_rows(sizeof(T) == 4, a.tq, a.tk, a.segments, a.group)) return attn_rows_bwd<T>(a, b, gq, gk, gv, stream);
   if (a.tq > 0) {
     const int launched = launch_ranges(fmd_cdiv(a.tq * a.heads, 16), [&](unsigned blocks, int64_t first) {
       attn_delta_kernel<T><<<blocks, 256, 0, stream>>>(b, a.tq, a.heads, a.dim, first, work);
@@ -1250,7 +1258,7 @@ int64_t fmd_segment_attention_work_size(int32_t bf16, int32_t splits, int64_t tq
 int32_t fmd_segment_attention_bwd_splits(int32_t bf16, int64_t tq, int64_t tk, int32_t segments, int32_t heads, int32_t kv_heads,
                                          int32_t dim, int32_t of_kv) {
   if (tq <= 0 || tk <= 0 || segments <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 1;
-  if (few_rows(tq, tk, segments)) return 1;
+  if (few_rows(!bf16, tq, tk, segments, heads / kv_heads)) return 1;
   return of_kv ? row_splits(!bf16, dim, tq, tk, segments, heads, kv_heads)
                : split_count(!bf16, dim, tq, tk, segments, heads, kv_heads);
 }
