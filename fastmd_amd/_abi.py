@@ -160,6 +160,12 @@ SIGNATURES: dict[str, tuple] = {
     "fmd_qk_norm_rotary_bwd": (ctypes.c_int, [_i32, _p, _i64, _i64, _i32, _p, _i64, _i64, _i32, _i64, _i32, _i32, _f32,
                                               _p, _p, _p, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _i64, _i64, _p,
                                               _i64, _i64, _p, _p, _p, _p, _p, _p]),
+    "fmd_gated_ffn_work_size": (_i64, [_i32, _i64, _i64, _i64, _i64, _i32, _i32]),
+    "fmd_gated_ffn": (ctypes.c_int, [_i32, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
+                                     _p, _p, _p, _p, _p]),
+    "fmd_gated_ffn_bwd_work_size": (_i64, [_i32, _i64, _i64, _i64, _i64, _i32, _i32, _i32]),
+    "fmd_gated_ffn_bwd": (ctypes.c_int, [_i32, _i32, _i32, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
+                                         _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p]),
 }
 
 _lock = threading.Lock()

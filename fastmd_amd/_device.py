@@ -1,6 +1,8 @@
 """Argument checks shared by the HIP wrappers (host side, before any launch)."""
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 from torch import Tensor
 
@@ -46,3 +48,9 @@ def rows_view(t: Tensor) -> tuple[Tensor, int]:
 
 def stream() -> int:
     return _abi.stream_handle()
+
+
+def on_device_of(t: Tensor):
+    """A context in which launches go to the device of ``t`` (and its current stream)."""
+    index = t.get_device()
+    return nullcontext() if index == torch._C._cuda_getDevice() else torch.cuda.device(index)

@@ -1,0 +1,455 @@
+// The gated feed-forward block y = h Wd^T, h = act(x Wg^T) * (x Wu^T), and its gradients.
+//
+// Four or five launches, each a product of tile_product.h with what follows it as its epilogue:
+//   gate, up -> h            both projections of a tile in one workgroup; the factors stay in registers and h alone is written
+//   y = h Wd^T
+//   gh = gy Wd -> dg, du     dg = gh u act'(g), du = gh act(g)
+//   gx = dg Wg + du Wu       one product with K of two parts
+//   gWg = dg^T x, gWu = du^T x, gWd = gy^T h   one launch
+// The backward pass takes g and u from the forward in float32: in bf16 their rounding alone would leave dg and du two roundings off,
+// and gx with them. h, dg and du are rounded to bf16 once, as operands of the next product (float32: split into three planes),
+// so that a bf16 result has the error of two roundings, its own and its operand's.
+#include "activation.h"
+#include "tile_product.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------------------- operands
+
+// A matrix [rows, cols] as the products read it: bf16, rows of `ld` elements (a multiple of 8, the rest zero), three planes of
+// float32.
+struct LayJob {
+  const void* src;
+  int64_t src_ld;
+  __bf16* dst;
+  int64_t rows, cols, ld, plane;
+  int32_t wide;  // source rows in whole 16-byte vectors
+  uint32_t first;
+};
+
+constexpr int kLayJobs = 5;
+
+struct LayArgs {
+  LayJob job[kLayJobs];
+  int32_t count, blocks;
+};
+
+template <bool F32>
+__global__ void __launch_bounds__(256) ffn_lay_kernel(LayArgs a) {
+  int n = 0;
+#pragma unroll
+  for (int i = 1; i < kLayJobs; ++i)
+    if (i < a.count && blockIdx.x >= a.job[i].first) n = i;
+  const LayJob& j = a.job[n];
+  const int64_t chunks = j.ld / 8, i = (int64_t)(blockIdx.x - j.first) * 256 + threadIdx.x;
+  if (i >= j.rows * chunks) return;
+  const int64_t row = i / chunks, col = (i - row * chunks) * 8;
+  const bool whole = j.wide && col + 8 <= j.cols;
+  __bf16* dst = j.dst + row * j.ld + col;
+  if (F32) {
+    const float* src = static_cast<const float*>(j.src) + row * j.src_ld + col;
+    float4 lo, hi;
+    if (whole) {
+      lo = reinterpret_cast<const float4*>(src)[0];
+      hi = reinterpret_cast<const float4*>(src)[1];
+    } else {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = col + e < j.cols ? src[e] : 0.f;
+      lo = make_float4(v[0], v[1], v[2], v[3]);
+      hi = make_float4(v[4], v[5], v[6], v[7]);
+    }
+    fmd_bf16x4 l[3], h[3];
+    x3_split(lo, l[0], l[1], l[2]);
+    x3_split(hi, h[0], h[1], h[2]);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<fmd_bf16x8*>(dst + p * j.plane) = __builtin_shufflevector(l[p], h[p], 0, 1, 2, 3, 4, 5, 6, 7);
+  } else {
+    const __bf16* src = static_cast<const __bf16*>(j.src) + row * j.src_ld + col;
+    fmd_bf16x8 v;
+    if (whole) {
+      v = *reinterpret_cast<const fmd_bf16x8*>(src);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = col + e < j.cols ? src[e] : (__bf16)0.f;
+    }
+    *reinterpret_cast<fmd_bf16x8*>(dst) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------------------- epilogues
+
+// four values as bf16, or as the three planes of float32
+__device__ __forceinline__ void put_operand(__bf16* p, int64_t plane, int planes, const float (&v)[4]) {
+  if (planes == 3) {
+    fmd_bf16x4 x[3];
+    x3_split(make_float4(v[0], v[1], v[2], v[3]), x[0], x[1], x[2]);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<fmd_bf16x4*>(p + i * plane) = x[i];
+  } else {
+    fmd_bf16x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (__bf16)v[e];
+    *reinterpret_cast<fmd_bf16x4*>(p) = x;
+  }
+}
+
+// h [rows, ld] (zero in the columns past hidden), and g, u [rows, ld] for the backward pass
+struct GatedEpi {
+  __bf16* h;
+  float *gate, *up;  // nullable
+  int64_t rows, hidden, ld, plane;
+  int32_t act, planes;
+  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, float4 g, float4 u) const {
+    if (m >= rows || n >= ld) return;
+    const float gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = n + e < hidden ? activation(gv[e], act).value * uv[e] : 0.f;
+    put_operand(h + m * ld + n, plane, planes, v);
+    if (gate) {
+      *reinterpret_cast<float4*>(gate + m * ld + n) = g;
+      *reinterpret_cast<float4*>(up + m * ld + n) = u;
+    }
+  }
+};
+
+// dg, du [2, rows, ld] from gh
+struct GatedBackEpi {
+  __bf16* d;
+  const float *gate, *up;
+  int64_t rows, hidden, ld, plane;
+  int32_t act, planes;
+  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, float4 gh, float4) const {
+    if (m >= rows || n >= ld) return;
+    const float4 g = *reinterpret_cast<const float4*>(gate + m * ld + n), u = *reinterpret_cast<const float4*>(up + m * ld + n);
+    const float hv[4] = {gh.x, gh.y, gh.z, gh.w}, gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
+    float dg[4], du[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const ActValue a = activation(gv[e], act);
+      const bool in = n + e < hidden;
+      dg[e] = in ? hv[e] * uv[e] * a.slope : 0.f;
+      du[e] = in ? hv[e] * a.value : 0.f;
+    }
+    put_operand(d + m * ld + n, plane, planes, dg);
+    put_operand(d + (rows + m) * ld + n, plane, planes, du);
+  }
+};
+
+// results [rows_m, rows_n] of each problem, in the features' type
+struct StoreEpi {
+  void* out[kTpProblems];
+  int64_t rows_m[kTpProblems], rows_n[kTpProblems];
+  int32_t bf16;
+  __device__ __forceinline__ void operator()(int i, int64_t m, int64_t n, float4 v, float4) const {
+    const int64_t width = i == 0 ? rows_n[0] : i == 1 ? rows_n[1] : rows_n[2];
+    if (m >= (i == 0 ? rows_m[0] : i == 1 ? rows_m[1] : rows_m[2]) || n >= width) return;
+    void* o = i == 0 ? out[0] : i == 1 ? out[1] : out[2];
+    const float e[4] = {v.x, v.y, v.z, v.w};
+    if (bf16) {
+      __bf16* p = static_cast<__bf16*>(o) + m * width + n;
+      if (width % 4 == 0) {
+        fmd_bf16x4 x;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = (__bf16)e[k];
+        *reinterpret_cast<fmd_bf16x4*>(p) = x;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n + k < width) p[k] = (__bf16)e[k];
+      }
+    } else {
+      float* p = static_cast<float*>(o) + m * width + n;
+      if (width % 4 == 0) {
+        *reinterpret_cast<float4*>(p) = v;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n + k < width) p[k] = e[k];
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------------------------------- host
+
+template <bool NA, bool MA, bool GATED>
+struct Shapes {
+  typedef TpShape<TpBf16, 2, 4, 4, 2, NA, MA, GATED, 2> Large;   // 256 x 256, 8 waves, one workgroup a CU
+  typedef TpShape<TpBf16, 2, 2, 2, 2, NA, MA, GATED, 2> Middle;  // 128 x 128, 4 waves, two
+  typedef TpShape<TpBf16, 1, 2, 2, 1, NA, MA, GATED, 2> Small;   // 64 x 64, 2 waves
+};
+
+template <typename S>
+int64_t count_tiles(TpArgs& a) {
+  int64_t tiles = 0;
+  for (int i = 0; i < a.count; ++i) tiles = tp_tiles<S>(a.p[i], tiles);
+  return tiles;
+}
+
+// The tile: 256 x 256 where these fill the card once, 128 x 128 where those fill half of it, 64 x 64 otherwise.
+template <typename Sh, typename Fn>
+int with_shape(TpArgs& a, const Fn& fn) {
+  int64_t slices = 0;
+  for (int i = 0; i < a.count; ++i) {
+    const int64_t s = fmd_cdiv(a.p[i].k, 64) * a.p[i].parts * (a.p[i].planes == 3 ? 6 : 1);
+    slices = i == 0 || s < slices ? s : slices;
+  }
+  int64_t tiles = count_tiles<typename Sh::Large>(a);
+  if (tiles > kTpMostTiles) return FMD_EINVAL;
+  if (tiles >= 192) return fn(typename Sh::Large{}, tp_plan<typename Sh::Large>(tiles, slices));
+  tiles = count_tiles<typename Sh::Middle>(a);
+  if (tiles >= 256) return fn(typename Sh::Middle{}, tp_plan<typename Sh::Middle>(tiles, slices));
+  tiles = count_tiles<typename Sh::Small>(a);
+  return fn(typename Sh::Small{}, tp_plan<typename Sh::Small>(tiles, slices));
+}
+
+int64_t up8(int64_t x) { return (x + 7) & ~int64_t(7); }
+int64_t up256(int64_t x) { return (x + 255) & ~int64_t(255); }
+
+// Everything that a call lays out in its workspace; with a null base the sizes alone.
+struct Space {
+  char* base;
+  int64_t used = 0;
+  template <typename T = void>
+  T* take(int64_t bytes) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += up256(bytes);
+    return p;
+  }
+};
+
+struct Ffn {
+  int32_t bf16, act, lay;  // lay: bits of the operands that are laid out in the workspace: x, gate and up, down, gy
+  int64_t rows, width, hidden, out;
+  int64_t hp() const { return up8(hidden); }
+  int planes() const { return bf16 ? 1 : 3; }
+};
+
+// an operand: the caller's matrix, or its layout in the workspace
+struct Matrix {
+  const void* p;
+  int64_t ld, plane;
+};
+
+struct Layer {
+  LayArgs args{};
+  int64_t blocks = 0;
+  Matrix add(const Ffn& f, Space& s, bool lay, const void* src, int64_t ld, int64_t rows, int64_t cols) {
+    if (!lay) return {src, ld, 0};
+    const int64_t wide = up8(cols);
+    __bf16* dst = s.take<__bf16>(rows * wide * 2 * f.planes());
+    LayJob& j = args.job[args.count++];
+    const int size = f.bf16 ? 2 : 4;
+    j = {src, ld, dst, rows, cols, wide, rows * wide,
+         (int32_t)(ld * size % 16 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0), (uint32_t)blocks};
+    blocks += fmd_cdiv(rows * wide / 8, 256);
+    return {dst, wide, rows * wide};
+  }
+  int launch(const Ffn& f, hipStream_t stream) {
+    if (!blocks) return FMD_OK;
+    FMD_REQUIRE(blocks < (int64_t(1) << 23));
+    if (f.bf16)
+      ffn_lay_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(args);
+    else
+      ffn_lay_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(args);
+    FMD_CHECK_LAUNCH();
+    return FMD_OK;
+  }
+};
+
+TpOperand operand(const Matrix& a, const Matrix& b) { return tp_operand(a.p, b.p, a.ld, a.plane, 2); }
+
+bool direct(const void* p, int64_t ld, int64_t cols) {
+  return ld % 8 == 0 && cols % 8 == 0 && ld * 2 <= kTpMostLd && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// A launch of one kind of product: its partial sums' size, or the launch itself
+template <typename Sh, typename Epi>
+int product(TpArgs& a, Space& s, bool run, const Epi& epi, hipStream_t stream) {
+  return with_shape<Sh>(a, [&](auto shape, const TpPlan& plan) {
+    typedef decltype(shape) S;
+    const int64_t before = s.used;
+    void* partial = s.take(plan.partial);
+    const int status = run ? tp_launch<S>(a, plan, partial, epi, stream) : FMD_OK;
+    s.used = before;  // the next product's sums take the same place
+    a.partial = nullptr;
+    if (!run) s.used += up256(plan.partial);  // sizes: the caller keeps the largest
+    return status;
+  });
+}
+
+TpArgs one(const TpOperand& n, const TpOperand& m, int64_t rows_n, int64_t rows_m, int64_t k, int parts, int planes) {
+  TpArgs a{};
+  a.p[0] = {n, m, rows_n, rows_m, k, parts, planes, 0, 0, 0};
+  a.count = 1;
+  return a;
+}
+
+struct Forward {
+  const void *x, *gate, *up, *down;
+  int64_t x_ld, gate_ld, up_ld, down_ld;
+  void* y;
+  float* saved;    // g, u [2, rows, hp], or null
+  __bf16* hidden;  // [planes, rows, hp], or null: in the workspace
+};
+
+int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t stream, int64_t* size) {
+  Layer lay;
+  const Matrix x = lay.add(f, s, f.lay & 1, io.x, io.x_ld, f.rows, f.width);
+  const Matrix g = lay.add(f, s, f.lay & 2, io.gate, io.gate_ld, f.hidden, f.width);
+  const Matrix u = lay.add(f, s, f.lay & 2, io.up, io.up_ld, f.hidden, f.width);
+  const Matrix d = lay.add(f, s, f.lay & 4, io.down, io.down_ld, f.out, f.hidden);
+  const int64_t hp = f.hp(), plane = f.rows * hp;
+  __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.planes());
+  if (run) {
+    const int status = lay.launch(f, stream);
+    if (status) return status;
+  }
+  int64_t most = s.used;
+  const int64_t base = s.used;
+  TpArgs a = one(operand(g, u), operand(x, x), f.hidden, f.rows, f.width, 1, f.planes());
+  const GatedEpi gated{h, io.saved, io.saved ? io.saved + plane : nullptr, f.rows, f.hidden, hp, plane, f.act, f.planes()};
+  int status = product<Shapes<false, false, true>>(a, s, run, gated, stream);
+  if (status) return status;
+  most = s.used > most ? s.used : most;
+  s.used = base;
+  const Matrix hm{h, hp, plane};
+  a = one(operand(d, d), operand(hm, hm), f.out, f.rows, f.hidden, 1, f.planes());
+  const StoreEpi store{{io.y}, {f.rows}, {f.out}, f.bf16};
+  status = product<Shapes<false, false, false>>(a, s, run, store, stream);
+  if (status) return status;
+  most = s.used > most ? s.used : most;
+  if (size) *size = most;
+  return FMD_OK;
+}
+
+struct Backward {
+  Forward in;
+  const void* gy;
+  int64_t gy_ld;
+  void *gx, *g_gate, *g_up, *g_down;  // gx, or the three weights', nullable
+};
+
+int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& s, bool run, hipStream_t stream, int64_t* size) {
+  Layer lay;
+  Matrix x{}, g{}, u{};
+  if (want_w) x = lay.add(f, s, f.lay & 1, io.in.x, io.in.x_ld, f.rows, f.width);
+  if (want_x) {
+    g = lay.add(f, s, f.lay & 2, io.in.gate, io.in.gate_ld, f.hidden, f.width);
+    u = lay.add(f, s, f.lay & 2, io.in.up, io.in.up_ld, f.hidden, f.width);
+  }
+  const Matrix d = lay.add(f, s, f.lay & 4, io.in.down, io.in.down_ld, f.out, f.hidden);
+  const Matrix gy = lay.add(f, s, f.lay & 8, io.gy, io.gy_ld, f.rows, f.out);
+  const int64_t hp = f.hp(), plane = f.rows * hp;
+  __bf16* dgu = s.take<__bf16>(2 * plane * 2 * f.planes());
+  if (run) {
+    const int status = lay.launch(f, stream);
+    if (status) return status;
+  }
+  int64_t most = s.used;
+  const int64_t base = s.used;
+  TpArgs a = one(operand(d, d), operand(gy, gy), f.hidden, f.rows, f.out, 1, f.planes());
+  const GatedBackEpi back{dgu, io.in.saved, io.in.saved ? io.in.saved + plane : nullptr, f.rows, f.hidden, hp, 2 * plane, f.act, f.planes()};
+  int status = product<Shapes<true, false, false>>(a, s, run, back, stream);
+  if (status) return status;
+  most = s.used > most ? s.used : most;
+  const Matrix dg{dgu, hp, 2 * plane}, du{dgu + plane, hp, 2 * plane};
+  if (want_x) {
+    s.used = base;
+    a = one(operand(g, u), operand(dg, du), f.width, f.rows, f.hidden, 2, f.planes());
+    const StoreEpi store{{io.gx}, {f.rows}, {f.width}, f.bf16};
+    status = product<Shapes<true, false, false>>(a, s, run, store, stream);
+    if (status) return status;
+    most = s.used > most ? s.used : most;
+  }
+  if (want_w) {
+    s.used = base;
+    const Matrix h{io.in.hidden, hp, plane};
+    a = one(operand(x, x), operand(dg, dg), f.width, f.hidden, f.rows, 1, f.planes());
+    a.p[1] = {operand(x, x), operand(du, du), f.width, f.hidden, f.rows, 1, f.planes(), 0, 0, 0};
+    a.p[2] = {operand(h, h), operand(gy, gy), f.hidden, f.out, f.rows, 1, f.planes(), 0, 0, 0};
+    a.count = 3;
+    const StoreEpi store{{io.g_gate, io.g_up, io.g_down}, {f.hidden, f.hidden, f.out}, {f.width, f.width, f.hidden}, f.bf16};
+    status = product<Shapes<true, true, false>>(a, s, run, store, stream);
+    if (status) return status;
+    most = s.used > most ? s.used : most;
+  }
+  if (size) *size = most;
+  return FMD_OK;
+}
+
+bool sizes_fit(const Ffn& f) {
+  return f.rows >= 1 && f.width >= 1 && f.hidden >= 1 && f.out >= 1 && f.rows < (int64_t(1) << 31) &&
+         (f.bf16 || f.lay == 15) && up8(f.width) * 2 <= kTpMostLd && up8(f.hidden) * 2 <= kTpMostLd && up8(f.out) * 2 <= kTpMostLd &&
+         f.act >= kActNone && f.act <= kActRelu;
+}
+
+bool layouts_fit(const Ffn& f, const Forward& io) {
+  if (!f.bf16) return true;
+  return ((f.lay & 1) || direct(io.x, io.x_ld, f.width)) &&
+         ((f.lay & 2) || (direct(io.gate, io.gate_ld, f.width) && direct(io.up, io.up_ld, f.width) && io.gate_ld == io.up_ld)) &&
+         ((f.lay & 4) || direct(io.down, io.down_ld, f.hidden));
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fmd_gated_ffn_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
+                                int32_t keep_hidden) {
+  const Ffn f{bf16, 0, lay, rows, width, hidden, out};
+  if (!sizes_fit(f)) return 0;
+  Space s{nullptr};
+  Forward io{};
+  io.hidden = keep_hidden ? reinterpret_cast<__bf16*>(16) : nullptr;
+  int64_t size = 0;
+  forward(f, io, s, false, nullptr, &size);
+  return size;
+}
+
+int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate, int64_t gate_ld,
+                  const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width, int64_t hidden,
+                  int64_t out, void* y, float* saved, void* hidden_out, void* work, hipStream_t stream) {
+  const Ffn f{bf16, act, lay, rows, width, hidden, out};
+  const Forward io{x, gate, up, down, x_ld, gate_ld, up_ld, down_ld, y, saved, static_cast<__bf16*>(hidden_out)};
+  FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io) && x && gate && up && down && y && work);
+  Space s{static_cast<char*>(work)};
+  return forward(f, io, s, true, stream, nullptr);
+}
+
+int64_t fmd_gated_ffn_bwd_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
+                                    int32_t want_x, int32_t want_w) {
+  const Ffn f{bf16, 0, lay, rows, width, hidden, out};
+  if (!sizes_fit(f)) return 0;
+  Space s{nullptr};
+  const Backward io{};
+  int64_t size = 0;
+  backward(f, io, want_x, want_w, s, false, nullptr, &size);
+  return size;
+}
+
+int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate, int64_t gate_ld,
+                      const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width,
+                      int64_t hidden, int64_t out, const void* gy, int64_t gy_ld, const float* saved, const void* hidden_in,
+                      void* gx, void* g_gate, void* g_up, void* g_down, void* work, hipStream_t stream) {
+  const Ffn f{bf16, act, lay, rows, width, hidden, out};
+  Backward io{};
+  io.in = {x, gate, up, down, x_ld, gate_ld, up_ld, down_ld, nullptr, const_cast<float*>(saved),
+           static_cast<__bf16*>(const_cast<void*>(hidden_in))};
+  io.gy = gy;
+  io.gy_ld = gy_ld;
+  io.gx = gx;
+  io.g_gate = g_gate;
+  io.g_up = g_up;
+  io.g_down = g_down;
+  FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io.in) && x && gate && up && down && gy && saved && work);
+  FMD_REQUIRE(!bf16 || (lay & 8) || direct(gy, gy_ld, out));
+  FMD_REQUIRE(!g_gate || (g_up && g_down && hidden_in));
+  Space s{static_cast<char*>(work)};
+  return backward(f, io, gx != nullptr, g_gate != nullptr, s, true, stream, nullptr);
+}
+
+}  // extern "C"

@@ -1,0 +1,428 @@
+// Products out[m, n] = sum_k n_op[n, k] m_op[m, k] on the matrix cores, with the result's own use as an epilogue: what the
+// gated feed-forward block and the 8-bit product are made of.
+//
+// Both operands of a slice of K are copied straight from global memory into LDS (no register stage), two slices in turn: while
+// the matrix instructions run on one, the next one lands. An operand is stored along K (its rows are rows of the product, K
+// contiguous) or across it (its rows are K, as a weight is in the products of the backward pass); the second kind is
+// transposed by the LDS reads (ds_read_b64_tr_b16), never in memory. The n operand is the matrix instruction's first: a
+// lane's four consecutive results then lie side by side in a row of the output.
+//
+// float32 operands come as three bf16 planes (x3.h); their six plane products follow each other along K, the small ones
+// first, in one accumulator: K is six times as long, the kernel is the same.
+#pragma once
+
+#include "common.h"
+#include "x3.h"
+
+typedef int tp_i32x4 __attribute__((ext_vector_type(4)));
+typedef int tp_i32x16 __attribute__((ext_vector_type(16)));
+typedef short tp_s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int64_t kTpMostLd = int64_t(1) << 23;  // bytes: a lane's offset in the 256 rows of a tile fits 32 bits
+
+// base: of each part of K (a sum of two products), or, for a gated product, of the two matrices whose rows share a tile
+struct TpOperand {
+  const char* base[2];
+  int64_t ld, plane;  // bytes from a stored row to the next, and from a plane to the next
+};
+
+struct TpProblem {
+  TpOperand n, m;
+  int64_t rows_n, rows_m, k;  // of one part
+  int32_t parts, planes;      // parts of K; planes 1 or 3
+  int32_t tiles_n, tiles_m, first;  // tiles, and the number of the first one
+};
+
+constexpr int kTpProblems = 3;
+
+// Tiles [0, full) are whole; each of the others is shared by `splits` workgroups that take a part of its K each and leave their
+// sums in `partial`, [tile, split, value, thread] in units of four, for tile_join_kernel.
+struct TpArgs {
+  TpProblem p[kTpProblems];
+  int32_t count, tiles, full, splits;
+  void* partial;
+};
+
+__device__ __attribute__((aligned(16))) const uint32_t g_tp_zero_chunk[4] = {0, 0, 0, 0};
+
+constexpr int kTpVm0 = 0 | (7 << 4) | (15 << 8);        // s_waitcnt vmcnt(0)
+constexpr int kTpVm0Lgkm0 = 0 | (7 << 4) | (0 << 8);    // s_waitcnt vmcnt(0) lgkmcnt(0)
+
+struct TpBf16 {
+  typedef fmd_f32x16 Acc;
+  static constexpr int SIZE = 2;
+  __device__ static __forceinline__ Acc mma(tp_i32x4 a, tp_i32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(fmd_bf16x8, a), __builtin_bit_cast(fmd_bf16x8, b), c, 0, 0, 0);
+  }
+};
+struct TpInt8 {
+  typedef tp_i32x16 Acc;
+  static constexpr int SIZE = 1;
+  __device__ static __forceinline__ Acc mma(tp_i32x4 a, tp_i32x4 b, Acc c) {
+    return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0);
+  }
+};
+
+// One operand's rows in LDS: ROWS rows of the product, SLICE bytes of K each (along), or SLICE / 2 rows of K (across). 16-byte
+// chunks are permuted so that neither kind of read meets a bank twice: sixteen consecutive rows' same chunk (along; both on
+// the 64 banks and, for eight rows, on any 32), or four chunks of four consecutive rows of K (across).
+constexpr int kTpSlice = 128;  // bytes of K in a slice (64 bf16 values, 128 8-bit ones)
+
+template <int ROWS, bool ACROSS_, bool GATED, int THREADS>
+struct TpStage {
+  static constexpr bool ACROSS = ACROSS_;
+  static constexpr int BYTES = ROWS * kTpSlice, LOADS = BYTES / 16 / THREADS;
+  static constexpr int WIDTH = ROWS * 2, CHUNKS = ROWS / 8;  // across: bytes and chunks of a row of K
+  static_assert(BYTES % (16 * THREADS) == 0, "whole passes");
+  static_assert(!(ACROSS && GATED), "a gated product's weights lie along K");
+
+  __device__ static __forceinline__ int swap_along(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+  __device__ static __forceinline__ int swap_across(int row) { return CHUNKS >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
+
+  uint32_t off[LOADS];
+  const char* at[GATED ? 2 : 1];
+  int64_t step;
+
+  // this thread's offsets for the tile whose first row is `row0` (below `rows`)
+  __device__ __forceinline__ void place(const TpOperand& o, int64_t row0, int64_t rows, int wave, int lane) {
+    step = ACROSS ? (kTpSlice / 2) * o.ld : kTpSlice;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int slot = (wave * LOADS + j) * 64 + lane;
+      if (ACROSS) {
+        const int row = slot / CHUNKS, chunk = (slot % CHUNKS) ^ swap_across(row);
+        const int64_t last = ((rows + 7) & ~int64_t(7)) - 8 - row0;  // chunks past the rows: the last one again, never used
+        off[j] = (uint32_t)(row * o.ld) + 2 * (uint32_t)(chunk * 8 < last ? chunk * 8 : last);
+      } else {
+        int row = slot / 8;
+        const int chunk = (slot % 8) ^ swap_along(row);
+        if (GATED && row >= ROWS / 2) row -= ROWS / 2;
+        const int64_t last = rows - 1 - row0;
+        off[j] = (uint32_t)((row < last ? row : last) * o.ld) + 16 * chunk;
+      }
+    }
+  }
+
+  // the copies start at slice `slice` of a part and plane
+  __device__ __forceinline__ void begin(const TpOperand& o, int part, int plane, int64_t row0, int slice) {
+    const int64_t from = plane * o.plane + slice * step + row0 * (ACROSS ? 2 : o.ld);
+    if (GATED) {
+      at[0] = o.base[0] + from;
+      at[GATED ? 1 : 0] = o.base[1] + from;
+    } else {
+      at[0] = o.base[part] + from;
+    }
+  }
+
+  __device__ static __forceinline__ void copy16(const void* p, char* to) {
+    typedef const __attribute__((address_space(1))) void* global_ptr;
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 16, 0, 0);
+  }
+
+  // the slice at `at` into LDS; `left`: bytes of K from it on, past them is zero
+  __device__ __forceinline__ void issue(char* lds, int64_t left, int wave, int lane) {
+    if (left >= kTpSlice) {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const char* p = GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0];
+        copy16(p + off[j], lds + (wave * LOADS + j) * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const char* p = (GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0]) + off[j];
+        const int slot = (wave * LOADS + j) * 64 + lane;
+        const int k = ACROSS ? slot / CHUNKS * 2 : ((slot % 8) ^ swap_along(slot / 8)) * 16;
+        p = k < left ? p : reinterpret_cast<const char*>(g_tp_zero_chunk);
+        asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
+        copy16(p, lds + (wave * LOADS + j) * 1024);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < (GATED ? 2 : 1); ++g) at[g] += step;
+  }
+
+  // a lane's place in the operand reads
+  __device__ static __forceinline__ int lane_at(int lane) {
+    const int h = lane >> 5;
+    if (ACROSS) {
+      const int row = 8 * h + ((lane & 15) >> 2);
+      return row * WIDTH + ((((lane >> 4) & 1) * 32 + (lane & 3) * 8) ^ (swap_across(row) * 16));
+    }
+    const int row = lane & 31;
+    return row * kTpSlice + ((h ^ swap_along(row)) << 4);
+  }
+
+  // operand of the 32 rows from `row` (a multiple of 32) over step kk of four: 16 bytes, from K 32 kk + 16 (lane / 32) bytes
+  __device__ static __forceinline__ tp_i32x4 read(const char* lds, int at, int row, int kk) {
+    if (ACROSS) {
+      typedef __attribute__((address_space(3))) tp_s16x4* lds_ptr;
+      const char* x = lds + kk * 16 * WIDTH + (at ^ (row * 2));
+      const tp_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)x);
+      const tp_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(x + 4 * WIDTH));
+      return __builtin_bit_cast(tp_i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    return *reinterpret_cast<const tp_i32x4*>(lds + row * kTpSlice + (at ^ (kk << 5)));
+  }
+};
+
+// WN x WM waves, each with NB x MB blocks of 32 x 32. A wave's n blocks are half in the tile's first half of n, half in the
+// second: of a gated product these are the two factors of the same results.
+template <typename TYPE, int WN_, int WM_, int NB_, int MB_, bool N_ACROSS, bool M_ACROSS, bool GATED_, int WAVES_EU_>
+struct TpShape {
+  typedef TYPE Type;
+  static constexpr int WN = WN_, WM = WM_, NB = NB_, MB = MB_, THREADS = 64 * WN * WM, BN = 32 * WN * NB, BM = 32 * WM * MB;
+  static constexpr bool GATED = GATED_;
+  static constexpr int OUT_N = GATED ? BN / 2 : BN, WAVES_EU = WAVES_EU_, GROUPS = (GATED ? NB / 2 : NB) * MB * 4;
+  typedef TpStage<BN, N_ACROSS, GATED, THREADS> StageN;
+  typedef TpStage<BM, M_ACROSS, false, THREADS> StageM;
+  static constexpr int STAGE = StageN::BYTES + StageM::BYTES;
+  static_assert(NB % 2 == 0, "two halves");
+
+  __device__ static __forceinline__ int block_n(int i, int wn) { return (i / (NB / 2)) * (BN / 2) + (wn * (NB / 2) + i % (NB / 2)) * 32; }
+};
+
+__device__ __forceinline__ float4 tp_four(const fmd_f32x16& v, int q) { return make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]); }
+__device__ __forceinline__ int4 tp_four(const tp_i32x16& v, int q) { return make_int4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]); }
+
+template <typename Four>
+__device__ __forceinline__ Four tp_sum(const Four* x, int64_t step, int splits) {
+  Four s = x[0];
+  for (int i = 1; i < splits; ++i) {
+    const Four v = x[i * step];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  return s;
+}
+
+struct TpTile {
+  int32_t problem, tn, tm;
+};
+
+// Tiles in bands of eight rows of tiles, column by column: those that run at once on an XCD (which takes one contiguous run of
+// them) share their operands in its L2.
+__device__ __forceinline__ TpTile tp_tile(const TpArgs& a, int tile) {
+  TpTile t{0, 0, 0};
+#pragma unroll
+  for (int i = 1; i < kTpProblems; ++i)
+    if (i < a.count && tile >= a.p[i].first) t.problem = i;
+  const TpProblem& p = a.p[t.problem];
+  const int r = tile - p.first, band = 8 * p.tiles_n, b = r / band, in = r - b * band;
+  const int rows = min(8, p.tiles_m - 8 * b);
+  t.tn = in / rows;
+  t.tm = 8 * b + in - t.tn * rows;
+  return t;
+}
+
+template <typename S, typename Epi>
+__global__ void __launch_bounds__(S::THREADS) __attribute__((amdgpu_waves_per_eu(S::WAVES_EU)))
+tile_product_kernel(TpArgs a, Epi epi) {
+  typedef typename S::Type T;
+  typedef typename T::Acc Acc;
+  constexpr int NB = S::NB, MB = S::MB;
+  __shared__ __attribute__((aligned(1024))) char st0[S::STAGE];
+  __shared__ __attribute__((aligned(1024))) char st1[S::STAGE];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int wn = wave / S::WM, wm = wave % S::WM;
+  int tile, split = 0, splits = 1;
+  if ((int)blockIdx.x < a.full) {
+    tile = (int)fmd_xcd_block(blockIdx.x, a.full);
+  } else {
+    const int r = (int)fmd_xcd_block(blockIdx.x - a.full, (int64_t)(a.tiles - a.full) * a.splits);
+    splits = a.splits;
+    tile = a.full + r / splits;
+    split = r % splits;
+  }
+  const TpTile tt = tp_tile(a, tile);
+  const TpProblem& p = a.p[tt.problem];
+  const int64_t n0 = (int64_t)tt.tn * S::OUT_N, m0 = (int64_t)tt.tm * S::BM;
+
+  // slices of K of all passes (parts, planes), and those of this workgroup
+  const int64_t k_bytes = p.k * T::SIZE;
+  const int nk = (int)((k_bytes + kTpSlice - 1) / kTpSlice), passes = p.parts * (p.planes == 3 ? 6 : 1);
+  const int total = nk * passes;
+  const int begin = (int)((int64_t)total * split / splits), end = (int)((int64_t)total * (split + 1) / splits);
+
+  typename S::StageN sn;
+  typename S::StageM sm;
+  sn.place(p.n, n0, p.rows_n, wave, lane);
+  sm.place(p.m, m0, p.rows_m, wave, lane);
+  int pass = begin / nk, ks = begin - pass * nk;  // of the next slice to copy
+  auto open = [&]() {
+    const int pair = p.planes == 3 ? pass / p.parts : 5, part = p.planes == 3 ? pass - pair * p.parts : pass;
+    // planes of the six products: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0)
+    sn.begin(p.n, part, (0x124 >> (2 * pair)) & 3, n0, ks);
+    sm.begin(p.m, part, (0x046 >> (2 * pair)) & 3, m0, ks);
+  };
+  auto issue = [&](char* st) {
+    const int64_t left = k_bytes - (int64_t)ks * kTpSlice;
+    sn.issue(st, left, wave, lane);
+    sm.issue(st + S::StageN::BYTES, left, wave, lane);
+    if (++ks == nk) {
+      ks = 0;
+      ++pass;
+      if (pass < passes) open();
+    }
+  };
+  const int ln = S::StageN::lane_at(lane), lm = S::StageM::lane_at(lane);
+  tp_i32x4 fn[2][NB], fm[2][MB];
+  auto read = [&](const char* st, int kk, int to) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) fn[to][i] = S::StageN::read(st, ln, S::block_n(i, wn), kk);
+#pragma unroll
+    for (int j = 0; j < MB; ++j) fm[to][j] = S::StageM::read(st + S::StageN::BYTES, lm, (wm * MB + j) * 32, kk);
+  };
+  Acc acc[NB][MB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
+
+  if (begin < end) {
+    open();
+    issue(st0);
+    if (begin + 1 < end) issue(st1);
+    // A slice is four steps. The operands of a step are read while the one before runs; before the last step every wave has
+    // read the whole slice, so its place takes the slice after the next.
+    auto slice = [&](char* st, char* next, int s) {
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        if (kk < 3) {
+          read(st, kk + 1, (kk + 1) & 1);
+        } else if (s + 1 < end) {
+          __builtin_amdgcn_s_waitcnt(kTpVm0Lgkm0);
+          __builtin_amdgcn_s_barrier();
+          if (s + 2 < end) issue(st);
+          read(next, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < MB; ++j) acc[i][j] = T::mma(fn[kk & 1][i], fm[kk & 1][j], acc[i][j]);
+      }
+    };
+    if (begin + 1 < end)
+      __builtin_amdgcn_s_waitcnt(((S::StageN::LOADS + S::StageM::LOADS) & 15) | (7 << 4) | (15 << 8));
+    else
+      __builtin_amdgcn_s_waitcnt(kTpVm0);
+    __builtin_amdgcn_s_barrier();
+    read(st0, 0, 0);
+    int s = begin;
+    for (; s + 1 < end; s += 2) {
+      slice(st0, st1, s);
+      slice(st1, st0, s + 1);
+    }
+    if (s < end) slice(st0, st1, s);
+  }
+
+  // results: row m0 + wm 32 MB + 32 j + lane % 32, four columns from n0 + block + 8 q + 4 (lane / 32)
+  if (splits > 1) {
+    typedef decltype(tp_four(acc[0][0], 0)) Four;
+    Four* out = static_cast<Four*>(a.partial) + (int64_t)((tile - a.full) * splits + split) * (NB * MB * 4) * S::THREADS + t;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          out[((i * MB + j) * 4 + q) * S::THREADS] = tp_four(acc[i][j], q);
+        }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < (S::GATED ? NB / 2 : NB); ++i)
+#pragma unroll
+    for (int j = 0; j < MB; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t m = m0 + (wm * MB + j) * 32 + (lane & 31), n = n0 + S::block_n(i, wn) + 8 * q + 4 * (lane >> 5);
+        const int u = S::GATED ? i + NB / 2 : i;
+        epi(tt.problem, m, n, tp_four(acc[i][j], q), tp_four(acc[u][j], q));
+      }
+}
+
+// The tiles that several workgroups share: their sums added in order, then the same epilogue. One workgroup per group of four
+// results of each thread.
+template <typename S, typename Epi>
+__global__ void __launch_bounds__(S::THREADS) tile_join_kernel(TpArgs a, Epi epi) {
+  constexpr int NB = S::NB, MB = S::MB;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, wn = wave / S::WM, wm = wave % S::WM;
+  const int rel = blockIdx.x / S::GROUPS, group = blockIdx.x % S::GROUPS;
+  const int i = group / (4 * MB), j = group / 4 % MB, q = group % 4;
+  const TpTile tt = tp_tile(a, a.full + rel);
+  auto sum = [&](int block) {
+    typedef decltype(tp_four(typename S::Type::Acc{}, 0)) Four;
+    constexpr int64_t step = (int64_t)(NB * MB * 4) * S::THREADS;
+    return tp_sum(static_cast<const Four*>(a.partial) + rel * a.splits * step + ((block * MB + j) * 4 + q) * S::THREADS + t, step,
+                  a.splits);
+  };
+  const int64_t m = (int64_t)tt.tm * S::BM + (wm * MB + j) * 32 + (lane & 31);
+  const int64_t n = (int64_t)tt.tn * S::OUT_N + S::block_n(i, wn) + 8 * q + 4 * (lane >> 5);
+  const auto v = sum(i);
+  if (S::GATED)
+    epi(tt.problem, m, n, v, sum(i + NB / 2));
+  else
+    epi(tt.problem, m, n, v, v);
+}
+
+// Host side: sizes, the split of the tiles that do not fill the card, launches.
+
+constexpr int kTpCus = 256;
+constexpr int64_t kTpMostTiles = 1 << 21;
+
+// The operand rows of [base, ld elements of `size` bytes]
+inline TpOperand tp_operand(const void* a, const void* b, int64_t ld, int64_t plane, int size) {
+  return {{static_cast<const char*>(a), static_cast<const char*>(b)}, ld * size, plane * size};
+}
+
+struct TpPlan {
+  int32_t tiles, full, splits;
+  int64_t partial;  // bytes
+};
+
+// Tiles that fill whole rounds of the card (WAVES_EU workgroups of four waves' worth a CU) run whole; where what is left fills
+// less than half of a round, its tiles are shared out over the K axis, at least `least` slices to a workgroup.
+template <typename S>
+inline TpPlan tp_plan(int64_t tiles, int64_t slices) {
+  constexpr int64_t per_cu = 4 * S::WAVES_EU * 64 / S::THREADS, round = kTpCus * per_cu;
+  const int64_t least = 4;
+  TpPlan r{(int32_t)tiles, (int32_t)tiles, 1, 0};
+  const int64_t left = tiles % round;
+  if (left == 0 || 2 * left > round) return r;
+  int64_t splits = round / left;
+  if (splits > slices / least) splits = slices / least;
+  if (splits > 16) splits = 16;
+  if (splits < 2) return r;
+  r.full = (int32_t)(tiles - left);
+  r.splits = (int32_t)splits;
+  r.partial = left * splits * S::NB * S::MB * 16 * S::THREADS * 4;
+  return r;
+}
+
+template <typename S, typename Epi>
+inline int tp_launch(TpArgs& a, const TpPlan& plan, void* partial, const Epi& epi, hipStream_t stream) {
+  a.tiles = plan.tiles;
+  a.full = plan.full;
+  a.splits = plan.splits;
+  a.partial = partial;
+  const int shared = plan.tiles - plan.full;
+  tile_product_kernel<S, Epi><<<plan.full + shared * plan.splits, S::THREADS, 0, stream>>>(a, epi);
+  FMD_CHECK_LAUNCH();
+  if (shared) {
+    tile_join_kernel<S, Epi><<<shared * S::GROUPS, S::THREADS, 0, stream>>>(a, epi);
+    FMD_CHECK_LAUNCH();
+  }
+  return FMD_OK;
+}
+
+// the tiles of a problem, numbered after those before it
+template <typename S>
+inline int64_t tp_tiles(TpProblem& p, int64_t first) {
+  p.tiles_n = (int32_t)fmd_cdiv(p.rows_n, S::OUT_N);
+  p.tiles_m = (int32_t)fmd_cdiv(p.rows_m, S::BM);
+  p.first = (int32_t)first;
+  return first + (int64_t)p.tiles_n * p.tiles_m;
+}
