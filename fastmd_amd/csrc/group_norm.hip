@@ -1,0 +1,1023 @@
+// Norm over groups of channels with its activation, channels last, and its gradients:
+//   n = (x - mean) / sqrt(var + eps), y = act(n weight + bias)
+// mean and variance over the `width` channels of a group, of one row or of all rows of a segment.
+//
+// Rows by themselves: a row's group is held by 1 to 64 lanes, or by a workgroup; one read, one write.
+//
+// Segments: tiles of rows of one segment (attention_find.h: the host knows no length) in registers. A segment that is one tile
+// is done with it. Longer ones leave their tiles' means and squares (merged by the counts: no difference of large sums), are
+// joined, and read a second time, mostly from the last-level cache. The backward pass does the same with the channels' sums of gz
+// and gz n (gz: the gradient before the activation): they are the weights' gradients, and weighted they are the two means that
+// gx needs.
+#include "activation.h"
+#include "attention_find.h"
+#include "common.h"
+#include "x3.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kTileValues = 64;  // of a thread's registers
+
+struct GnArgs {
+  const void *x, *g;  // rows [rows, channels], row strides x_ld, g_ld; g: gradient of y
+  int64_t x_ld, g_ld;
+  const void *weight, *bias;  // [channels], or null: ones, zeros
+  const int64_t* off;         // [segments + 1]
+  int64_t rows;
+  int32_t segments, channels, groups, width, act;
+  float eps;
+  void *y, *gx;          // contiguous
+  float *mean, *inverse;  // [rows or segments, groups]
+  float *part;           // scratch (see the kernels)
+  int32_t chunk;         // channels of a workgroup's share (whole groups)
+  int32_t tile_rows, tx;  // rows of a tile, vectors of a row of the share
+  int32_t lanes;         // rows by themselves: lanes of a group
+  int32_t blocks;        // of rows, in x
+  uint32_t block0;
+};
+
+template <int V>
+struct Vec {
+  float v[V];
+};
+
+template <typename T, int V>
+struct RawVec {
+  typedef T Type __attribute__((ext_vector_type(V)));
+};
+template <typename T>
+struct RawVec<T, 1> {
+  typedef T Type;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ typename RawVec<T, V>::Type raw_load(const T* p) {
+  return *reinterpret_cast<const typename RawVec<T, V>::Type*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ float raw_get(const typename RawVec<T, V>::Type& r, int i) {
+  if constexpr (V == 1)
+    return (float)r;
+  else
+    return (float)r[i];
+}
+template <typename T, int V>
+__device__ __forceinline__ void raw_store(T* p, const float (&v)[V]) {
+  typename RawVec<T, V>::Type r;
+  if constexpr (V == 1) {
+    r = (T)v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r[i] = (T)v[i];
+  }
+  *reinterpret_cast<typename RawVec<T, V>::Type*>(p) = r;
+}
+
+template <typename T>
+__device__ __forceinline__ float param(const void* p, int64_t i, float none) {
+  return p ? (float)static_cast<const T*>(p)[i] : none;
+}
+
+// ---------------------------------------------------------------------------------------- rows by themselves
+
+// sum over the `lanes` lanes (a power of two) that hold a row's group, or over the workgroup
+template <bool WIDE>
+__device__ __forceinline__ float unit_sum(float s, int lanes, float* lds) {
+  if constexpr (WIDE) {
+    s = wave_sum(s);
+    __syncthreads();  // lds may still be read
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
+  }
+  for (int off = lanes >> 1; off; off >>= 1) s += __shfl_xor(s, off, 64);
+  return s;
+}
+
+// A workgroup's units: lane groups q, of `at_once` groups of a row and `rows` rows.
+struct GnUnits {
+  int at_once, rows, q, lane;
+  __device__ __forceinline__ GnUnits(const GnArgs& a) {
+    const int n = kThreads / a.lanes;
+    q = threadIdx.x / a.lanes;
+    lane = threadIdx.x % a.lanes;
+    at_once = a.groups < n ? a.groups : n;
+    rows = n / at_once;
+  }
+};
+
+template <typename T, int V, int NV, bool WIDE>
+__global__ void __launch_bounds__(kThreads) gn_rows_kernel(GnArgs a) {
+  __shared__ float lds[4];
+  const GnUnits u(a);
+  const int g = blockIdx.y * u.at_once + u.q % u.at_once;
+  const int64_t row = (int64_t)(blockIdx.x + a.block0) * u.rows + u.q / u.at_once;
+  const bool live = u.q < u.at_once * u.rows && g < a.groups && row < a.rows;
+  const int64_t c0 = (int64_t)g * a.width;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_ld + c0;
+  float v[NV][V];
+  float s = 0.f;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = (u.lane + n * a.lanes) * V;
+    const bool in = live && c < a.width;
+    typename RawVec<T, V>::Type r{};
+    if (in) r = raw_load<T, V>(x + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) s += v[n][i] = raw_get<T, V>(r, i);
+  }
+  const float mean = unit_sum<WIDE>(s, a.lanes, lds) / a.width;
+  float d = 0.f;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[n][i] -= mean;
+      if ((u.lane + n * a.lanes) * V < a.width) d += v[n][i] * v[n][i];
+    }
+  const float inverse = 1.f / sqrtf(unit_sum<WIDE>(d, a.lanes, lds) / a.width + a.eps);
+  if (!live) return;
+  if (a.mean && u.lane == 0) {
+    a.mean[row * a.groups + g] = mean;
+    a.inverse[row * a.groups + g] = inverse;
+  }
+  T* y = static_cast<T*>(a.y) + row * a.channels + c0;
+#pragma unroll
+  for (int n = 0; n < NV; ++n) {
+    const int c = (u.lane + n * a.lanes) * V;
+    if (c >= a.width) break;
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      o[i] = activation(v[n][i] * inverse * param<T>(a.weight, c0 + c + i, 1.f) + param<T>(a.bias, c0 + c + i, 0.f), a.act).value;
+    raw_store<T, V>(y + c, o);
+  }
+}
+
+// the same group of rows `blocks` apart; the channels' sums of gz n and gz in part [blocks, rows of a workgroup, 2, channels]
+template <typename T, int V, int NV, bool WIDE>
+__global__ void __launch_bounds__(kThreads) gn_rows_bwd_kernel(GnArgs a) {
+  __shared__ float lds[4];
+  const GnUnits u(a);
+  const int g = blockIdx.y * u.at_once + u.q % u.at_once;
+  const bool mine = u.q < u.at_once * u.rows && g < a.groups;
+  const int64_t c0 = (int64_t)g * a.width;
+  float w[NV][V], b[NV][V], gw[NV][V], gb[NV][V];
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (u.lane + n * a.lanes) * V + i;
+      const bool in = mine && c < a.width;
+      w[n][i] = in ? param<T>(a.weight, c0 + c, 1.f) : 0.f;
+      b[n][i] = in ? param<T>(a.bias, c0 + c, 0.f) : 0.f;
+      gw[n][i] = gb[n][i] = 0.f;
+    }
+  for (int64_t base = (int64_t)blockIdx.x * u.rows; base < a.rows; base += (int64_t)a.blocks * u.rows) {
+    const int64_t row = base + u.q / u.at_once;
+    const bool live = mine && row < a.rows;
+    const float mean = live ? a.mean[row * a.groups + g] : 0.f, inverse = live ? a.inverse[row * a.groups + g] : 0.f;
+    const T *x = static_cast<const T*>(a.x) + row * a.x_ld + c0, *gy = static_cast<const T*>(a.g) + row * a.g_ld + c0;
+    float h[NV][V], z[NV][V];
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = (u.lane + n * a.lanes) * V;
+      const bool in = live && c < a.width;
+      typename RawVec<T, V>::Type r{}, q{};
+      if (in) r = raw_load<T, V>(x + c);
+      if (in) q = raw_load<T, V>(gy + c);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        h[n][i] = in ? (raw_get<T, V>(r, i) - mean) * inverse : 0.f;
+        z[n][i] = in ? raw_get<T, V>(q, i) * activation(h[n][i] * w[n][i] + b[n][i], a.act).slope : 0.f;
+        gw[n][i] += z[n][i] * h[n][i];
+        gb[n][i] += z[n][i];
+        z[n][i] *= w[n][i];
+        s += z[n][i];
+        t += z[n][i] * h[n][i];
+      }
+    }
+    s = unit_sum<WIDE>(s, a.lanes, lds) / a.width;
+    t = unit_sum<WIDE>(t, a.lanes, lds) / a.width;
+    if (!live) continue;
+    T* gx = static_cast<T*>(a.gx) + row * a.channels + c0;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int c = (u.lane + n * a.lanes) * V;
+      if (c >= a.width) break;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = inverse * (z[n][i] - s - h[n][i] * t);
+      raw_store<T, V>(gx + c, o);
+    }
+  }
+  if (!a.part || !mine) return;
+  float* p = a.part + ((int64_t)blockIdx.x * u.rows + u.q / u.at_once) * 2 * a.channels + c0;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int c = (u.lane + n * a.lanes) * V + i;
+      if (c < a.width) {
+        p[c] = gw[n][i];
+        p[a.channels + c] = gb[n][i];
+      }
+    }
+}
+
+// Sums of the columns of part [count, 2, channels] over its rows, in a fixed order: the weights' gradients, or, in several
+// blocks of rows, the rows of the next such sum.
+template <typename T>
+__global__ void __launch_bounds__(1024) gn_columns_kernel(const float* part, int64_t count, int64_t columns, int64_t each, float* sums,
+                                                          T* gw, T* gb) {
+  __shared__ float lds[32][33];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t c = (int64_t)blockIdx.x * 32 + tx, from = blockIdx.y * each, to = from + each < count ? from + each : count;
+  float s = 0.f;
+  if (c < columns) {
+    int64_t r = from + ty;
+    for (; r + 96 < to; r += 128) {
+      const float* p = part + r * columns + c;
+      s += (p[0] + p[32 * columns]) + (p[64 * columns] + p[96 * columns]);
+    }
+    for (; r < to; r += 32) s += part[r * columns + c];
+  }
+  lds[ty][tx] = s;
+  __syncthreads();
+  for (int n = 16; n; n >>= 1) {
+    if (ty < n) lds[ty][tx] += lds[ty + n][tx];
+    __syncthreads();
+  }
+  if (ty || c >= columns) return;
+  s = lds[0][tx];
+  const int64_t half = columns / 2;
+  if (sums)
+    sums[blockIdx.y * columns + c] = s;
+  else if (c < half)
+    gw[c] = (T)s;
+  else
+    gb[c - half] = (T)s;
+}
+
+// ---------------------------------------------------------------------------------------- segments
+
+// A workgroup's share of the channels [c0, c0 + nc), `tx` vectors of a row (NV apart from each other by the workgroup's width),
+// and a thread's place in it.
+template <int V, int NV>
+struct GnPlace {
+  int c0, nc, groups, x, y, step;
+  bool in;
+  __device__ __forceinline__ GnPlace(const GnArgs& a) {
+    c0 = blockIdx.y * a.chunk;
+    nc = min(a.chunk, a.channels - c0);
+    groups = nc / a.width;
+    step = NV > 1 ? 1 : kThreads / a.tx;
+    x = NV > 1 ? threadIdx.x : threadIdx.x % a.tx;
+    y = NV > 1 ? 0 : threadIdx.x / a.tx;
+    in = y < step;
+  }
+  __device__ __forceinline__ int column(int n) const { return (x + n * kThreads) * V; }  // within the share
+  __device__ __forceinline__ bool has(int n) const { return in && column(n) < nc; }
+};
+
+// Sums over the share's groups of `count` rows of values per channel in lds [count, nc]: out[g], in the same order for every call.
+// Power of two lanes a group.
+__device__ __forceinline__ void group_sums(const float* lds, int count, int nc, int width, int groups, float* out) {
+  int lanes = 64;
+  while (lanes > 1 && lanes * groups > kThreads) lanes >>= 1;
+  const int lane = threadIdx.x % lanes, total = count * width, each = kThreads / lanes;
+  for (int g = threadIdx.x / lanes; g < max(groups, each); g += each) {  // several lanes a group: one pass, all take part
+    float s = 0.f;
+    if (g < groups)
+      for (int i = lane; i < total; i += lanes) {
+        const int r = i / width;
+        s += lds[r * nc + g * width + (i - r * width)];
+      }
+    for (int off = lanes >> 1; off; off >>= 1) s += __shfl_xor(s, off, 64);
+    if (lane == 0 && g < groups) out[g] = s;
+  }
+}
+
+struct GnTile {
+  int segment;         // extended: 0 and segments + 1 are the rows outside
+  int64_t start, rows, first;
+  bool real, whole;
+};
+
+__device__ __forceinline__ GnTile gn_tile(const GnArgs& a, int64_t number) {
+  GnTile t;
+  t.segment = attn_find(a.off, a.segments, a.rows, 1, a.tile_rows, number, &t.first, WaveLanes());
+  t.start = attn_start(a.off, a.segments, a.rows, t.segment);
+  t.rows = attn_start(a.off, a.segments, a.rows, t.segment + 1) - t.start;
+  t.real = t.segment >= 1 && t.segment <= a.segments;
+  t.whole = t.rows <= a.tile_rows;
+  return t;
+}
+
+// Tiles of long segments, for the second read: numbers from floor(2 start / tile) on, of which such a segment owns at least as
+// many as it has tiles, and a shorter one any.
+__device__ __forceinline__ GnTile gn_long_tile(const GnArgs& a, int64_t number) {
+  GnTile t;
+  const auto num = [&](int i) { return 2 * attn_start(a.off, a.segments, a.rows, i) / a.tile_rows; };
+  t.segment = attn_last(a.segments + 2, number, num, WaveLanes());
+  t.start = attn_start(a.off, a.segments, a.rows, t.segment);
+  t.rows = attn_start(a.off, a.segments, a.rows, t.segment + 1) - t.start;
+  t.real = t.segment >= 1 && t.segment <= a.segments;
+  t.whole = t.rows <= a.tile_rows;
+  const int64_t tile = number - num(t.segment);
+  t.first = tile < 0 ? INT64_MAX : tile * a.tile_rows;
+  return t;
+}
+
+template <typename T, int V, int NV, int NR>
+struct GnRegs {
+  typename RawVec<T, V>::Type r[NR][NV];
+  __device__ __forceinline__ void load(const GnPlace<V, NV>& p, const T* x, int64_t ld, int rows) {
+#pragma unroll
+    for (int k = 0; k < NR; ++k)
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int row = p.y + k * p.step;
+        r[k][n] = typename RawVec<T, V>::Type{};
+        if (p.has(n) && row < rows) r[k][n] = raw_load<T, V>(x + row * ld + p.c0 + p.column(n));
+      }
+  }
+  __device__ __forceinline__ float get(int k, int n, int i) const { return raw_get<T, V>(r[k][n], i); }
+};
+
+// per channel of this thread: the group's value from lds
+template <int V, int NV>
+__device__ __forceinline__ void spread(const GnPlace<V, NV>& p, int width, const float* of_group, float (&v)[NV][V]) {
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[n][i] = p.has(n) ? of_group[(p.column(n) + i) / width] : 0.f;
+}
+
+template <typename T, int V, int NV>
+__device__ __forceinline__ void spread_param(const GnPlace<V, NV>& p, const void* src, float none, float (&v)[NV][V]) {
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[n][i] = p.has(n) ? param<T>(src, p.c0 + p.column(n) + i, none) : 0.f;
+}
+
+// values per channel, a row of lds for each of the workgroup's rows of threads
+template <int V, int NV>
+__device__ __forceinline__ void put_channels(const GnPlace<V, NV>& p, float* lds, const float (&v)[NV][V]) {
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+    if (p.has(n))
+#pragma unroll
+      for (int i = 0; i < V; ++i) lds[p.y * p.nc + p.column(n) + i] = v[n][i];
+}
+
+template <typename T, int V, int NV, int NR>
+__device__ __forceinline__ void write_zero(const GnPlace<V, NV>& p, T* y, int64_t ld, int rows) {
+  const float zero[V] = {};
+#pragma unroll
+  for (int k = 0; k < NR; ++k)
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int row = p.y + k * p.step;
+      if (p.has(n) && row < rows) raw_store<T, V>(y + row * ld + p.c0 + p.column(n), zero);
+    }
+}
+
+template <typename T, int V, int NV, int NR>
+__device__ __forceinline__ void write_norm(const GnArgs& a, const GnPlace<V, NV>& p, const GnRegs<T, V, NV, NR>& x, T* y, int rows,
+                                           const float (&mean)[NV][V], const float (&inverse)[NV][V]) {
+  float w[NV][V], b[NV][V];
+  spread_param<T, V, NV>(p, a.weight, 1.f, w);
+  spread_param<T, V, NV>(p, a.bias, 0.f, b);
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[n][i] *= inverse[n][i];
+#pragma unroll
+  for (int k = 0; k < NR; ++k)
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int row = p.y + k * p.step;
+      if (!p.has(n) || row >= rows) continue;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = activation((x.get(k, n, i) - mean[n][i]) * w[n][i] + b[n][i], a.act).value;
+      raw_store<T, V>(y + (int64_t)row * a.channels + p.c0 + p.column(n), o);
+    }
+}
+
+// First read. part: [tiles, groups, 2], mean and sum of squared distances of a tile of a longer segment.
+template <typename T, int V, int NV, int NR>
+__global__ void __launch_bounds__(kThreads) gn_tile_kernel(GnArgs a) {
+  extern __shared__ float lds[];  // [rows of threads, share], then the groups' values twice
+  const GnPlace<V, NV> p(a);
+  const int64_t number = (int64_t)blockIdx.x + a.block0;
+  const GnTile t = gn_tile(a, number);
+  if (t.first >= t.rows) return;
+  const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
+  const int64_t row0 = t.start + t.first;
+  T* y = static_cast<T*>(a.y) + row0 * a.channels;
+  if (!t.real) return write_zero<T, V, NV, NR>(p, y, a.channels, rows);
+  GnRegs<T, V, NV, NR> x;
+  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
+  float* of_group = lds + p.step * p.nc;
+  const float count = (float)((int64_t)rows * a.width);
+  float s[NV][V];
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) s[n][i] += x.get(k, n, i);  // zero past the rows
+    }
+  put_channels<V, NV>(p, lds, s);
+  __syncthreads();
+  group_sums(lds, p.step, p.nc, a.width, p.groups, of_group);
+  __syncthreads();
+  float mean[NV][V];
+  spread<V, NV>(p, a.width, of_group, mean);
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      mean[n][i] /= count;
+      s[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        const float d = p.y + k * p.step < rows ? x.get(k, n, i) - mean[n][i] : 0.f;
+        s[n][i] += d * d;
+      }
+    }
+  put_channels<V, NV>(p, lds, s);
+  __syncthreads();
+  float* squares = of_group + p.groups;
+  group_sums(lds, p.step, p.nc, a.width, p.groups, squares);
+  __syncthreads();
+  const int g0 = p.c0 / a.width;
+  if (!t.whole) {
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+      float2* out = reinterpret_cast<float2*>(a.part) + number * a.groups + g0 + g;
+      *out = make_float2(of_group[g] / count, squares[g]);
+    }
+    return;
+  }
+  float inverse[NV][V];
+  spread<V, NV>(p, a.width, squares, inverse);
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) inverse[n][i] = 1.f / sqrtf(inverse[n][i] / count + a.eps);
+  if (a.mean)
+    for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+      const int64_t at = (int64_t)(t.segment - 1) * a.groups + g0 + g;
+      a.mean[at] = of_group[g] / count;
+      a.inverse[at] = 1.f / sqrtf(squares[g] / count + a.eps);
+    }
+  write_norm<T, V, NV, NR>(a, p, x, y, rows, mean, inverse);
+}
+
+// A longer segment's tiles joined, a wave a group: numbers from floor(start / tile) on, of which such a segment owns one at least.
+__global__ void __launch_bounds__(kThreads) gn_join_kernel(GnArgs a) {
+  const auto num = [&](int i) { return attn_start(a.off, a.segments, a.rows, i) / a.tile_rows; };
+  const int64_t number = (int64_t)blockIdx.x + a.block0;
+  const int i = attn_last(a.segments + 2, number, num, WaveLanes());
+  const int64_t start = attn_start(a.off, a.segments, a.rows, i), rows = attn_start(a.off, a.segments, a.rows, i + 1) - start;
+  if (i < 1 || i > a.segments || rows <= a.tile_rows || num(i) != number) return;
+  const int g = blockIdx.y * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+  if (g >= a.groups) return;
+  const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows;
+  const float2* part = reinterpret_cast<const float2*>(a.part) + (start / a.tile_rows + i) * a.groups + g;
+  const float full = (float)a.tile_rows * a.width, last = (float)(rows - (tiles - 1) * a.tile_rows) * a.width;
+  // means about the first tile's, so that nothing large cancels
+  const float pivot = part[0].x;
+  const double total = (double)rows * a.width;
+  double s = 0.0;
+  for (int64_t k = lane; k < tiles; k += 64) s += (double)(part[k * a.groups].x - pivot) * (k == tiles - 1 ? last : full);
+  const float mean = (float)(pivot + wave_sum(s) / total);
+  double d = 0.0;
+  for (int64_t k = lane; k < tiles; k += 64) {
+    const float2 v = part[k * a.groups];
+    const double e = (double)v.x - mean;
+    d += (double)v.y + e * e * (k == tiles - 1 ? last : full);
+  }
+  d = wave_sum(d);
+  if (lane) return;
+  a.mean[(int64_t)(i - 1) * a.groups + g] = mean;
+  a.inverse[(int64_t)(i - 1) * a.groups + g] = (float)(1.0 / sqrt(d / total + (double)a.eps));
+}
+
+template <int V, int NV>
+__device__ __forceinline__ void load_stats(const GnArgs& a, const GnPlace<V, NV>& p, int segment, float (&mean)[NV][V],
+                                           float (&inverse)[NV][V]) {
+  const int64_t at = (int64_t)(segment - 1) * a.groups + p.c0 / a.width;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int g = (p.column(n) + i) / a.width;
+      mean[n][i] = p.has(n) ? a.mean[at + g] : 0.f;
+      inverse[n][i] = p.has(n) ? a.inverse[at + g] : 0.f;
+    }
+}
+
+// Second read of the longer segments.
+template <typename T, int V, int NV, int NR>
+__global__ void __launch_bounds__(kThreads) gn_apply_kernel(GnArgs a) {
+  const GnPlace<V, NV> p(a);
+  const GnTile t = gn_long_tile(a, (int64_t)blockIdx.x + a.block0);
+  if (!t.real || t.whole || t.first >= t.rows) return;
+  const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
+  const int64_t row0 = t.start + t.first;
+  GnRegs<T, V, NV, NR> x;
+  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
+  float mean[NV][V], inverse[NV][V];
+  load_stats<V, NV>(a, p, t.segment, mean, inverse);
+  write_norm<T, V, NV, NR>(a, p, x, static_cast<T*>(a.y) + row0 * a.channels, rows, mean, inverse);
+}
+
+// gx of a tile: the two means over its segment's group in s (of gz w) and q (of gz w n)
+template <typename T, int V, int NV, int NR>
+__device__ __forceinline__ void write_grad(const GnArgs& a, const GnPlace<V, NV>& p, const GnRegs<T, V, NV, NR>& x,
+                                           const GnRegs<T, V, NV, NR>& gy, T* gx, int rows, const float (&mean)[NV][V],
+                                           const float (&inverse)[NV][V], const float (&w)[NV][V], const float (&b)[NV][V],
+                                           const float (&s)[NV][V], const float (&q)[NV][V]) {
+#pragma unroll
+  for (int k = 0; k < NR; ++k)
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int row = p.y + k * p.step;
+      if (!p.has(n) || row >= rows) continue;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
+        const float z = gy.get(k, n, i) * activation(h * w[n][i] + b[n][i], a.act).slope * w[n][i];
+        o[i] = inverse[n][i] * (z - s[n][i] - h * q[n][i]);
+      }
+      raw_store<T, V>(gx + (int64_t)row * a.channels + p.c0 + p.column(n), o);
+    }
+}
+
+// First read of the backward pass. part: [tiles, 2, channels], the channels' sums of gz n and gz.
+template <typename T, int V, int NV, int NR>
+__global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a) {
+  extern __shared__ float lds[];  // [rows of threads, share], then the groups' values twice
+  const GnPlace<V, NV> p(a);
+  const int64_t number = (int64_t)blockIdx.x + a.block0;
+  const GnTile t = gn_tile(a, number);
+  float* part = a.part + number * 2 * a.channels + p.c0;
+  if (t.first >= t.rows || !t.real) {
+    for (int c = threadIdx.x; c < p.nc; c += kThreads) part[c] = part[a.channels + c] = 0.f;
+    if (t.first >= t.rows) return;
+  }
+  const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
+  const int64_t row0 = t.start + t.first;
+  T* gx = static_cast<T*>(a.gx) + row0 * a.channels;
+  if (!t.real) return write_zero<T, V, NV, NR>(p, gx, a.channels, rows);
+  GnRegs<T, V, NV, NR> x, gy;
+  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
+  gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
+  float mean[NV][V], inverse[NV][V], w[NV][V], b[NV][V], gw[NV][V], gb[NV][V];
+  load_stats<V, NV>(a, p, t.segment, mean, inverse);
+  spread_param<T, V, NV>(p, a.weight, 1.f, w);
+  spread_param<T, V, NV>(p, a.bias, 0.f, b);
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      gw[n][i] = gb[n][i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        if (p.y + k * p.step >= rows) break;
+        const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
+        const float z = gy.get(k, n, i) * activation(h * w[n][i] + b[n][i], a.act).slope;
+        gw[n][i] += z * h;
+        gb[n][i] += z;
+      }
+    }
+  float* of_group = lds + p.step * p.nc;
+  auto channels = [&](const float (&v)[NV][V], float* out, float* groups) {
+    put_channels<V, NV>(p, lds, v);
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.nc; c += kThreads) {
+      float s = 0.f;
+      for (int y = 0; y < p.step; ++y) s += lds[y * p.nc + c];
+      out[c] = s;
+      lds[c] = s * param<T>(a.weight, p.c0 + c, 1.f);  // row 0 of this channel has been read
+    }
+    __syncthreads();
+    if (t.whole) group_sums(lds, 1, p.nc, a.width, p.groups, groups);
+    __syncthreads();
+  };
+  channels(gw, part, of_group);
+  channels(gb, part + a.channels, of_group + p.groups);
+  if (!t.whole) return;
+  const float count = (float)((int64_t)rows * a.width);
+  float s[NV][V], q[NV][V];
+  spread<V, NV>(p, a.width, of_group + p.groups, s);
+  spread<V, NV>(p, a.width, of_group, q);
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      s[n][i] /= count;
+      q[n][i] /= count;
+    }
+  write_grad<T, V, NV, NR>(a, p, x, gy, gx, rows, mean, inverse, w, b, s, q);
+}
+
+// The two means of a longer segment's groups, a wave a group, into means [segments, groups, 2].
+template <typename T>
+__global__ void __launch_bounds__(kThreads) gn_join_bwd_kernel(GnArgs a, float2* means) {
+  const auto num = [&](int i) { return attn_start(a.off, a.segments, a.rows, i) / a.tile_rows; };
+  const int64_t number = (int64_t)blockIdx.x + a.block0;
+  const int i = attn_last(a.segments + 2, number, num, WaveLanes());
+  const int64_t start = attn_start(a.off, a.segments, a.rows, i), rows = attn_start(a.off, a.segments, a.rows, i + 1) - start;
+  if (i < 1 || i > a.segments || rows <= a.tile_rows || num(i) != number) return;
+  const int g = blockIdx.y * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+  if (g >= a.groups) return;
+  const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows, total = tiles * a.width;
+  const float* part = a.part + (start / a.tile_rows + i) * 2 * a.channels + (int64_t)g * a.width;
+  float s = 0.f, q = 0.f;
+  for (int64_t k = lane; k < total; k += 64) {
+    const int64_t tile = k / a.width;
+    const int c = (int)(k - tile * a.width);
+    const float w = param<T>(a.weight, (int64_t)g * a.width + c, 1.f);
+    q += part[tile * 2 * a.channels + c] * w;
+    s += part[tile * 2 * a.channels + a.channels + c] * w;
+  }
+  s = wave_sum(s);
+  q = wave_sum(q);
+  const float count = (float)((double)rows * a.width);
+  if (lane == 0) means[(int64_t)(i - 1) * a.groups + g] = make_float2(s / count, q / count);
+}
+
+template <typename T, int V, int NV, int NR>
+__global__ void __launch_bounds__(kThreads) gn_apply_bwd_kernel(GnArgs a, const float2* means) {
+  const GnPlace<V, NV> p(a);
+  const GnTile t = gn_long_tile(a, (int64_t)blockIdx.x + a.block0);
+  if (!t.real || t.whole || t.first >= t.rows) return;
+  const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
+  const int64_t row0 = t.start + t.first;
+  GnRegs<T, V, NV, NR> x, gy;
+  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
+  gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
+  float mean[NV][V], inverse[NV][V], w[NV][V], b[NV][V], s[NV][V], q[NV][V];
+  load_stats<V, NV>(a, p, t.segment, mean, inverse);
+  spread_param<T, V, NV>(p, a.weight, 1.f, w);
+  spread_param<T, V, NV>(p, a.bias, 0.f, b);
+  const float2* m = means + (int64_t)(t.segment - 1) * a.groups + p.c0 / a.width;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float2 v = p.has(n) ? m[(p.column(n) + i) / a.width] : make_float2(0.f, 0.f);
+      s[n][i] = v.x;
+      q[n][i] = v.y;
+    }
+  write_grad<T, V, NV, NR>(a, p, x, gy, static_cast<T*>(a.gx) + row0 * a.channels, rows, mean, inverse, w, b, s, q);
+}
+
+// ---------------------------------------------------------------------------------------- host
+
+constexpr int64_t kMostBlocks = 1 << 22;
+
+// more workgroups than one launch takes go in several, each told its first one
+template <typename Launch>
+int in_launches(GnArgs& a, int64_t blocks, const Launch& launch) {
+  for (int64_t first = 0; first < blocks; first += kMostBlocks) {
+    a.block0 = (uint32_t)first;
+    launch((unsigned)(blocks - first < kMostBlocks ? blocks - first : kMostBlocks));
+    FMD_CHECK_LAUNCH();
+  }
+  return FMD_OK;
+}
+
+bool aligned(const void* p, int64_t ld, int64_t bytes, int size) {
+  return (reinterpret_cast<uintptr_t>(p) % bytes) == 0 && ld * size % bytes == 0;
+}
+
+// the widest vector, of up to 16 bytes, of which `unit` channels are whole ones and on which the rows start
+int vector_of(const GnArgs& a, int size, int64_t unit) {
+  for (int v = 16 / size; v > 1; v >>= 1)
+    if (unit % v == 0 && a.channels % v == 0 && aligned(a.x, a.x_ld, v * size, size) && (!a.g || aligned(a.g, a.g_ld, v * size, size)))
+      return v;
+  return 1;
+}
+
+// Rows by themselves: lanes of a group and vectors of a lane
+struct RowShape {
+  int v, nv, lanes;
+  bool wide;
+};
+
+RowShape row_shape(const GnArgs& a, int size) {
+  RowShape s{};
+  s.v = vector_of(a, size, a.width);
+  const int vectors = a.width / s.v;
+  s.wide = vectors > 256;
+  if (s.wide) {
+    s.lanes = kThreads;
+    s.nv = (vectors + kThreads - 1) / kThreads;
+  } else {
+    for (s.lanes = 1; s.lanes < 64 && s.lanes < vectors; s.lanes *= 2) {}
+    s.nv = (vectors + s.lanes - 1) / s.lanes;
+  }
+  return s;
+}
+
+// rows and groups of a workgroup, as GnUnits
+int row_groups(const GnArgs& a, const RowShape& s) {
+  const int n = kThreads / s.lanes;
+  return a.groups < n ? a.groups : n;
+}
+
+// The backward pass's workgroups: each walks rows, and its channels' sums are a row of the last step's input
+constexpr int64_t kRowBlocks = 512;
+
+int64_t row_blocks(const GnArgs& a, const RowShape& s) {
+  const int at_once = row_groups(a, s), rows = kThreads / s.lanes / at_once;
+  const int64_t all = fmd_cdiv(a.rows, rows);
+  return all < kRowBlocks ? all : kRowBlocks;
+}
+
+// fn(vector, vectors of a lane, wide) as constants
+template <typename T, typename Fn>
+int with_rows(const RowShape& s, const Fn& fn) {
+#define GN_ROWS(V, NV, WIDE) return fn(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, std::integral_constant<bool, WIDE>{})
+#define GN_ROWS_V(V, MOST)                                                    \
+  if (s.v == V) {                                                             \
+    if (!s.wide && s.nv == 1) GN_ROWS(V, 1, false);                           \
+    if (!s.wide && s.nv == 2) GN_ROWS(V, 2, false);                           \
+    if (!s.wide && s.nv <= 4) GN_ROWS(V, 4, false);                           \
+    if (s.nv <= MOST) GN_ROWS(V, MOST, true);                                 \
+  }
+  if constexpr (sizeof(T) == 2) { GN_ROWS_V(8, 4) }
+  GN_ROWS_V(4, 8)
+  GN_ROWS_V(2, 16)
+  GN_ROWS_V(1, 32)
+#undef GN_ROWS_V
+#undef GN_ROWS
+  return FMD_EUNSUPPORTED;
+}
+
+// Segments: a workgroup's share of the channels, whole groups of them; its tile's rows
+struct TileShape {
+  int v, nv, nr, chunk, tx, rows, chunks, lds;
+};
+
+TileShape tile_shape(const GnArgs& a, int size) {
+  TileShape s{};
+  for (s.v = vector_of(a, size, a.channels);; s.v >>= 1) {
+    const int most = kThreads * s.v;
+    s.chunk = a.channels;
+    if (a.channels > most) {
+      int groups = most / a.width;  // the most groups that a row of threads takes, as whole vectors
+      while (groups > 1 && groups * a.width % s.v) --groups;
+      s.chunk = (groups > 0 ? groups : 1) * a.width;
+    }
+    if (s.v == 1 || s.chunk % s.v == 0) break;
+  }
+  s.tx = s.chunk / s.v;
+  s.nv = s.tx > kThreads ? (s.tx + kThreads - 1) / kThreads : 1;
+  const int most = s.v == 1 ? 32 : 32 / s.v;  // registers of the wide form: 8 192 channels of a group at most
+  if (s.nv > 1) s.nv = s.nv <= most ? most : -1;
+  s.nr = kTileValues / (s.v * (s.nv > 1 ? s.nv : 1));
+  if (s.v == 1 && s.nv == 1) s.nr = 32;
+  s.rows = s.nr * (s.nv > 1 ? 1 : kThreads / s.tx);
+  s.chunks = (a.channels + s.chunk - 1) / s.chunk;
+  const int rows = s.nv > 1 ? 1 : kThreads / s.tx;
+  s.lds = (rows * s.chunk + 2 * (s.chunk / a.width)) * 4;
+  return s;
+}
+
+template <typename T, typename Fn>
+int with_tiles(const TileShape& s, const Fn& fn) {
+#define GN_TILE(V, NV, NR) return fn(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, NR>{})
+  if constexpr (sizeof(T) == 2) {
+    if (s.v == 8 && s.nv == 1) GN_TILE(8, 1, 8);
+    if (s.v == 8 && s.nv == 4) GN_TILE(8, 4, 2);
+  }
+  if (s.v == 4 && s.nv == 1) GN_TILE(4, 1, 16);
+  if (s.v == 4 && s.nv == 8) GN_TILE(4, 8, 2);
+  if (s.v == 2 && s.nv == 1) GN_TILE(2, 1, 32);
+  if (s.v == 2 && s.nv == 16) GN_TILE(2, 16, 2);
+  if (s.v == 1 && s.nv == 1) GN_TILE(1, 1, 32);
+  if (s.v == 1 && s.nv == 32) GN_TILE(1, 32, 2);
+#undef GN_TILE
+  return FMD_EUNSUPPORTED;
+}
+
+int64_t tile_count(const GnArgs& a, const TileShape& s) { return a.rows / s.rows + a.segments + 2; }
+
+void set_tiles(GnArgs& a, const TileShape& s) {
+  a.chunk = s.chunk;
+  a.tx = s.tx;
+  a.tile_rows = s.rows;
+}
+
+template <typename T>
+int norm(GnArgs a, hipStream_t stream) {
+  if (!a.off) {
+    const RowShape s = row_shape(a, sizeof(T));
+    a.lanes = s.lanes;
+    const int at_once = row_groups(a, s), rows = kThreads / s.lanes / at_once;
+    const unsigned y = (unsigned)fmd_cdiv(a.groups, at_once);
+    FMD_REQUIRE(y < 65536);
+    return with_rows<T>(s, [&](auto v, auto nv, auto wide) {
+      return in_launches(a, fmd_cdiv(a.rows, rows), [&](unsigned blocks) {
+        gn_rows_kernel<T, decltype(v)::value, decltype(nv)::value, decltype(wide)::value><<<dim3(blocks, y), kThreads, 0, stream>>>(a);
+      });
+    });
+  }
+  const TileShape s = tile_shape(a, sizeof(T));
+  FMD_REQUIRE(s.chunks < 65536);
+  set_tiles(a, s);
+  return with_tiles<T>(s, [&](auto v, auto nv, auto nr) {
+    constexpr int V = decltype(v)::value, NV = decltype(nv)::value, NR = decltype(nr)::value;
+    int status = in_launches(a, tile_count(a, s), [&](unsigned blocks) {
+      gn_tile_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a);
+    });
+    if (status || a.rows <= s.rows) return status;  // no segment is longer than a tile
+    status = in_launches(a, a.rows / s.rows, [&](unsigned blocks) {
+      gn_join_kernel<<<dim3(blocks, (a.groups + 3) / 4), kThreads, 0, stream>>>(a);
+    });
+    if (status) return status;
+    return in_launches(a, 2 * a.rows / s.rows + 1, [&](unsigned blocks) {
+      gn_apply_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 0, stream>>>(a);
+    });
+  });
+}
+
+// rows of the weights' last sum; from kColumnRows on, blocks of them are summed first
+constexpr int64_t kColumnRows = 1024, kColumnBlocks = 64;
+
+template <typename T>
+int columns(const float* part, int64_t count, int64_t channels, float* sums, void* gw, void* gb, hipStream_t stream) {
+  const unsigned x = (unsigned)fmd_cdiv(2 * channels, 32);
+  if (count > kColumnRows) {
+    const int64_t each = fmd_cdiv(count, kColumnBlocks), blocks = fmd_cdiv(count, each);
+    gn_columns_kernel<T><<<dim3(x, (unsigned)blocks), 1024, 0, stream>>>(part, count, 2 * channels, each, sums, nullptr, nullptr);
+    FMD_CHECK_LAUNCH();
+    part = sums;
+    count = blocks;
+  }
+  gn_columns_kernel<T><<<dim3(x, 1), 1024, 0, stream>>>(part, count, 2 * channels, count, nullptr, static_cast<T*>(gw),
+                                                        static_cast<T*>(gb));
+  FMD_CHECK_LAUNCH();
+  return FMD_OK;
+}
+
+// floats of the backward pass's scratch: the partial sums, the long segments' means, the sums of blocks
+struct BackSpace {
+  int64_t part, means, sums;
+};
+
+BackSpace back_space(const GnArgs& a, int size) {
+  BackSpace s{};
+  if (!a.off) {
+    const RowShape r = row_shape(a, size);
+    s.part = row_blocks(a, r) * (kThreads / r.lanes / row_groups(a, r)) * 2 * a.channels;
+  } else {
+    s.part = tile_count(a, tile_shape(a, size)) * 2 * a.channels;
+    s.means = 2 * (int64_t)a.segments * a.groups;
+  }
+  s.sums = kColumnBlocks * 2 * a.channels;
+  return s;
+}
+
+template <typename T>
+int norm_bwd(GnArgs a, float* work, void* gw, void* gb, hipStream_t stream) {
+  const BackSpace space = back_space(a, sizeof(T));
+  float* part = work;
+  float2* means = reinterpret_cast<float2*>(work + space.part);
+  float* sums = work + space.part + space.means;
+  a.part = part;
+  if (!a.off) {
+    const RowShape s = row_shape(a, sizeof(T));
+    a.lanes = s.lanes;
+    const int at_once = row_groups(a, s), rows = kThreads / s.lanes / at_once;
+    const unsigned y = (unsigned)fmd_cdiv(a.groups, at_once);
+    FMD_REQUIRE(y < 65536);
+    a.blocks = (int32_t)row_blocks(a, s);
+    if (!gw) a.part = nullptr;
+    const int status = with_rows<T>(s, [&](auto v, auto nv, auto wide) {
+      gn_rows_bwd_kernel<T, decltype(v)::value, decltype(nv)::value, decltype(wide)::value><<<dim3(a.blocks, y), kThreads, 0, stream>>>(a);
+      FMD_CHECK_LAUNCH();
+      return (int)FMD_OK;
+    });
+    if (status || !gw) return status;
+    return columns<T>(part, (int64_t)a.blocks * rows, a.channels, sums, gw, gb, stream);
+  }
+  const TileShape s = tile_shape(a, sizeof(T));
+  FMD_REQUIRE(s.chunks < 65536);
+  set_tiles(a, s);
+  const int status = with_tiles<T>(s, [&](auto v, auto nv, auto nr) {
+    constexpr int V = decltype(v)::value, NV = decltype(nv)::value, NR = decltype(nr)::value;
+    int status = in_launches(a, tile_count(a, s), [&](unsigned blocks) {
+      gn_tile_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a);
+    });
+    if (status || a.rows <= s.rows) return status;
+    status = in_launches(a, a.rows / s.rows, [&](unsigned blocks) {
+      gn_join_bwd_kernel<T><<<dim3(blocks, (a.groups + 3) / 4), kThreads, 0, stream>>>(a, means);
+    });
+    if (status) return status;
+    return in_launches(a, 2 * a.rows / s.rows + 1, [&](unsigned blocks) {
+      gn_apply_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 0, stream>>>(a, means);
+    });
+  });
+  if (status || !gw) return status;
+  return columns<T>(part, tile_count(a, s), a.channels, sums, gw, gb, stream);
+}
+
+constexpr int kMostWidth = 8192;
+
+bool sizes_fit(const GnArgs& a) {
+  return a.rows >= 1 && a.channels >= 1 && a.groups >= 1 && a.channels % a.groups == 0 && a.width <= kMostWidth && a.segments >= 0 &&
+         a.rows < (int64_t(1) << 40) && a.act >= kActNone && a.act <= kActRelu && a.groups <= 65535 * 4;
+}
+
+GnArgs arguments(int32_t act, int64_t rows, int32_t channels, int32_t groups, int32_t segments, const int64_t* offsets) {
+  GnArgs a{};
+  a.act = act;
+  a.rows = rows;
+  a.channels = channels;
+  a.groups = groups;
+  a.width = groups > 0 ? channels / groups : 0;
+  a.segments = segments;
+  a.off = offsets;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t fmd_group_norm_work_size(int32_t bf16, int64_t rows, int32_t channels, int32_t groups, int32_t segments) {
+  GnArgs a = arguments(0, rows, channels, groups, segments, nullptr);
+  if (!sizes_fit(a) || segments < 1) return 0;
+  // the largest number of tiles that any alignment leads to: that of the smallest tile
+  a.x_ld = 1;
+  int64_t most = 0;
+  for (int v = 1; v <= 8; v *= 2) {
+    a.x_ld = channels % v == 0 ? v : 1;
+    const int64_t n = tile_count(a, tile_shape(a, bf16 ? 2 : 4));
+    most = n > most ? n : most;
+  }
+  return 2 * most * groups;
+}
+
+int fmd_group_norm(int32_t bf16, int32_t act, const void* x, int64_t x_ld, const void* weight, const void* bias, int64_t rows,
+                   int32_t channels, int32_t groups, const int64_t* offsets, int32_t segments, float eps, void* y, float* mean,
+                   float* inverse, float* work, hipStream_t stream) {
+  GnArgs a = arguments(act, rows, channels, groups, segments, offsets);
+  a.x = x;
+  a.x_ld = x_ld;
+  a.weight = weight;
+  a.bias = bias;
+  a.eps = eps;
+  a.y = y;
+  a.mean = mean;
+  a.inverse = inverse;
+  a.part = work;
+  FMD_REQUIRE(sizes_fit(a) && x && y && eps >= 0.f && (!offsets || (mean && inverse && work)));
+  return bf16 ? norm<__bf16>(a, stream) : norm<float>(a, stream);
+}
+
+int64_t fmd_group_norm_bwd_work_size(int32_t bf16, int64_t rows, int32_t channels, int32_t groups, int32_t segments) {
+  GnArgs a = arguments(0, rows, channels, groups, segments, nullptr);
+  if (!sizes_fit(a)) return 0;
+  const int64_t none = 0;
+  if (segments >= 1) a.off = &none;
+  int64_t most = 0;
+  for (int v = 1; v <= 8; v *= 2) {
+    a.x_ld = channels % v == 0 ? v : 1;
+    const BackSpace s = back_space(a, bf16 ? 2 : 4);
+    most = s.part + s.means + s.sums > most ? s.part + s.means + s.sums : most;
+  }
+  return most;
+}
+
+int fmd_group_norm_bwd(int32_t bf16, int32_t act, const void* gy, int64_t gy_ld, const void* x, int64_t x_ld, const void* weight,
+                       const void* bias, int64_t rows, int32_t channels, int32_t groups, const int64_t* offsets, int32_t segments,
+                       const float* mean, const float* inverse, void* gx, void* g_weight, void* g_bias, float* work,
+                       hipStream_t stream) {
+  GnArgs a = arguments(act, rows, channels, groups, segments, offsets);
+  a.x = x;
+  a.x_ld = x_ld;
+  a.g = gy;
+  a.g_ld = gy_ld;
+  a.weight = weight;
+  a.bias = bias;
+  a.gx = gx;
+  a.mean = const_cast<float*>(mean);
+  a.inverse = const_cast<float*>(inverse);
+  FMD_REQUIRE(sizes_fit(a) && x && gy && gx && mean && inverse && work && (!g_weight || g_bias));
+  return bf16 ? norm_bwd<__bf16>(a, work, g_weight, g_bias, stream) : norm_bwd<float>(a, work, g_weight, g_bias, stream);
+}
+
+}  // extern "C"

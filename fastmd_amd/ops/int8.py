@@ -1,0 +1,123 @@
+"""(h) Products with weights held in 8-bit integers, with a scale for each row and channel, on the GPU (HIP kernels).
+
+``quantize_rows(x)``: each row of a float32 or bfloat16 matrix as 8-bit integers with one float32 scale,
+
+    scale = max |x| / 127,  value = x / scale rounded to the nearest integer (ties to even)
+
+(the quotients in float32). ``linear_int8(x, weight, bias=None)``: ``linear`` on a weight [out, in] so rounded,
+
+    y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]
+
+with the rows of x rounded on the way, or given as ``Int8Rows``. The sums are exact (32-bit integers on the matrix cores), each
+result is rounded once. A row of zeros has the scale 0; one that holds a value that is not finite gives NaN. For evaluation:
+there are no gradients, and inputs that need them are refused.
+"""
+from __future__ import annotations
+
+import functools
+from typing import NamedTuple
+
+import torch
+from torch import Tensor
+
+from fastmd_amd import _abi
+from fastmd_amd._autograd import differentiated
+from fastmd_amd._device import on_device_of, require_cuda, rows_view, stream
+
+MAX_WIDTH = 131071  # 127^2 times more terms could overflow 32 bits
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+class Int8Rows(NamedTuple):
+    """A matrix [rows, width] as 8-bit integers with a scale for each row: ``values * scales[:, None]``."""
+
+    values: Tensor  # int8 [rows, width]
+    scales: Tensor  # float32 [rows]
+
+    def dense(self) -> Tensor:
+        """The values that it stands for, float32."""
+        return self.values.float() * self.scales[:, None]
+
+
+def quantize_rows(x: Tensor) -> Int8Rows:
+    """The rows of ``x`` [rows, width] (float32 or bfloat16) as ``Int8Rows``. The values' rows start on 16 bytes, so that
+    ``linear_int8`` reads them in place."""
+    require_cuda(x)
+    if x.dim() != 2 or x.dtype not in _TYPES:
+        raise ValueError(f"quantize_rows takes a float32 or bfloat16 matrix, got {x.dtype} {tuple(x.shape)}")
+    if differentiated(x):
+        raise ValueError("quantize_rows has no gradient: detach its input")
+    rows, width = x.shape
+    if width < 1:
+        raise ValueError("quantize_rows takes at least one column")
+    ld = -(-width // 16) * 16
+    values = torch.empty((rows, ld), dtype=torch.int8, device=x.device)
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    x, x_ld = rows_view(x)
+    with on_device_of(x):
+        _abi.call("fmd_quantize_rows", _TYPES[x.dtype], x.data_ptr(), x_ld, rows, width, values.data_ptr(), ld,
+                  scales.data_ptr(), stream())
+    return Int8Rows(values[:, :width], scales)
+
+
+def _in_place(values: Tensor, padded: bool) -> tuple[Tensor, int]:
+    """(values, row stride in bytes) of rows on 16 bytes that can be read to the width's last 16 bytes, and, with ``padded``,
+    are zero from the width on; a copy where they do not lie so."""
+    rows, width = values.shape
+    whole = -(-width // 16) * 16
+    ld = values.stride(0) if rows > 1 else whole
+    if ((values.stride(1) == 1 or width == 1) and ld % 16 == 0 and whole <= ld <= 2 ** 23 and values.data_ptr() % 16 == 0
+            and (whole == width or (not padded and values.untyped_storage().nbytes()
+                                    >= values.storage_offset() + (rows - 1) * ld + whole))):
+        return values, ld
+    out = torch.zeros((rows, whole), dtype=torch.int8, device=values.device)
+    out[:, :width] = values
+    return out, whole
+
+
+@functools.lru_cache(maxsize=256)
+def _work_size(*sizes: int) -> int:
+    return max(1, _abi.load().fmd_linear_int8_work_size(*sizes))
+
+
+def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, dtype: torch.dtype | None = None) -> Tensor:
+    """``x weight^T + bias`` in 8 bits (see the module): ``x`` [rows, width] float32 or bfloat16, or ``Int8Rows``;
+    ``weight`` [out, width] (``quantize_rows`` of it, once); ``bias`` float32 [out]; ``dtype`` of the result: x's, float32 for
+    ``Int8Rows``."""
+    if not isinstance(weight, Int8Rows):
+        raise ValueError("weight must be Int8Rows (quantize_rows)")
+    rounded = not isinstance(x, Int8Rows)
+    if not rounded:
+        kind = torch.float32 if dtype is None else dtype
+    else:
+        kind = x.dtype if dtype is None else dtype
+        if differentiated(x, bias):
+            raise ValueError("linear_int8 has no gradient: detach its inputs")
+        x = quantize_rows(x)
+    require_cuda(x.values, x.scales, weight.values, weight.scales, bias)
+    if kind not in _TYPES:
+        raise ValueError(f"the result must be float32 or bfloat16, got {kind}")
+    for name, q in (("x", x), ("weight", weight)):
+        if (q.values.dim() != 2 or q.values.dtype != torch.int8 or q.scales.shape != q.values.shape[:1]
+                or q.scales.dtype != torch.float32):
+            raise ValueError(f"{name} must be int8 [rows, width] with float32 scales [rows], got {q.values.dtype} "
+                             f"{tuple(q.values.shape)} and {q.scales.dtype} {tuple(q.scales.shape)}")
+    (rows, width), out = x.values.shape, weight.values.shape[0]
+    if weight.values.shape[1] != width or not 1 <= width <= MAX_WIDTH:
+        raise ValueError(f"x and weight must have one width, from 1 to {MAX_WIDTH}, got {width} and {weight.values.shape[1]}")
+    if rows >= 2 ** 31 or out >= 2 ** 31:
+        raise ValueError("linear_int8 takes fewer than 2^31 rows and channels")
+    if bias is not None and (bias.shape != (out,) or bias.dtype != torch.float32):
+        raise ValueError(f"bias must be float32 [{out}], got {bias.dtype} {tuple(bias.shape)}")
+    y = torch.empty((rows, out), dtype=kind, device=x.values.device)
+    if rows == 0 or out == 0:
+        return y
+    # past the width one of the two has to be zero: rows that were rounded here are
+    (xv, x_ld), (wv, w_ld) = _in_place(x.values, not rounded), _in_place(weight.values, False)
+    x_scales, w_scales = x.scales.contiguous(), weight.scales.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    work = torch.empty(_work_size(rows, width, out), dtype=torch.uint8, device=y.device)
+    with on_device_of(y):
+        _abi.call("fmd_linear_int8", _TYPES[kind], xv.data_ptr(), x_ld, x_scales.data_ptr(), wv.data_ptr(), w_ld,
+                  w_scales.data_ptr(), _abi.ptr(bias), rows, width, out, y.data_ptr(), work.data_ptr(), stream())
+    return y

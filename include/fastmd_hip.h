@@ -882,7 +882,8 @@ int fmd_qk_norm_rotary_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q
                            void* gk_weight, float* work, hipStream_t stream);
 
 /* ----------------------------------------------------------------------------------------
- * (h) Between the attention layers: the gated feed-forward block. Not in the reference.
+ * (h) Between the attention layers: the gated feed-forward block, the norm over groups of channels, the product with
+ * 8-bit weights. Not in the reference.
  * -------------------------------------------------------------------------------------- */
 
 /* y = (act(x gate^T) * (x up^T)) down^T with x [rows, width], gate and up [hidden, width], down [out, hidden] (row strides in
@@ -909,6 +910,42 @@ int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int
                       const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width,
                       int64_t hidden, int64_t out, const void* gy, int64_t gy_ld, const float* saved, const void* hidden_in,
                       void* gx, void* g_gate, void* g_up, void* g_down, void* work, hipStream_t stream);
+
+/* y = act(n weight + bias), n = (x - mean) / sqrt(variance + eps) over each of `groups` groups of channels / groups channels side
+ * by side of x [rows, channels] (row stride x_ld): of every row by itself (offsets null), or of all rows
+ * [offsets[s], offsets[s + 1]) of segment s (device int64, ascending, clamped into the buffer; where they descend nothing
+ * outside the buffers is touched; rows outside every segment are written as zero). weight, bias [channels] of the features'
+ * type, null: ones, zeros. act as above. y contiguous. mean, inverse (1 / sqrt(variance + eps)): float32 [rows or segments, groups],
+ * for the VJP; nullable without offsets; of an empty segment not written. channels / groups at most 8 192.
+ * work: fmd_group_norm_work_size() floats (null without offsets; segments 0 there). */
+int64_t fmd_group_norm_work_size(int32_t bf16, int64_t rows, int32_t channels, int32_t groups, int32_t segments);
+int fmd_group_norm(int32_t bf16, int32_t act, const void* x, int64_t x_ld, const void* weight, const void* bias, int64_t rows,
+                   int32_t channels, int32_t groups, const int64_t* offsets, int32_t segments, float eps, void* y, float* mean,
+                   float* inverse, float* work, hipStream_t stream);
+
+/* VJP of fmd_group_norm: gx [rows, channels] contiguous (zero outside the segments) and g_weight, g_bias [channels] (nullable
+ * together), summed in float32 in a fixed order. work: fmd_group_norm_bwd_work_size() floats. */
+int64_t fmd_group_norm_bwd_work_size(int32_t bf16, int64_t rows, int32_t channels, int32_t groups, int32_t segments);
+int fmd_group_norm_bwd(int32_t bf16, int32_t act, const void* gy, int64_t gy_ld, const void* x, int64_t x_ld, const void* weight,
+                       const void* bias, int64_t rows, int32_t channels, int32_t groups, const int64_t* offsets, int32_t segments,
+                       const float* mean, const float* inverse, void* gx, void* g_weight, void* g_bias, float* work,
+                       hipStream_t stream);
+
+/* Rows of x [rows, width] (row stride x_ld) as 8-bit integers: scale = max |x| / 127 of the row, value = x / scale rounded to the
+ * nearest (ties to even), both in float32, at most 127 in size; a row of zeros has scale 0, a value that is not finite leaves a
+ * scale that is not. values [rows, values_ld] (values_ld at least width, the rest zero), scales [rows]. */
+int fmd_quantize_rows(int32_t bf16, const void* x, int64_t x_ld, int64_t rows, int64_t width, int8_t* values, int64_t values_ld,
+                      float* scales, hipStream_t stream);
+
+/* out[m, n] = x_scales[m] w_scales[n] sum_k x[m, k] w[n, k] (+ bias[n]) with 8-bit x [rows, width] and w [out, width] (row strides
+ * in bytes: multiples of 16 up to 2^23, rows on 16 bytes; both are read up to the width's next multiple of 16, where x is zero),
+ * exact sums in 32 bits;
+ * bias float32, nullable; out [rows, out] of bf16 or float32, contiguous. width below 131 072 (no sum overflows).
+ * work: fmd_linear_int8_work_size() bytes. */
+int64_t fmd_linear_int8_work_size(int64_t rows, int64_t width, int64_t out);
+int fmd_linear_int8(int32_t bf16, const int8_t* x, int64_t x_ld, const float* x_scales, const int8_t* w, int64_t w_ld,
+                    const float* w_scales, const float* bias, int64_t rows, int64_t width, int64_t out, void* y, void* work,
+                    hipStream_t stream);
 
 #ifdef __cplusplus
 }
