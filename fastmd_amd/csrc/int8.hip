@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, int64
   top = wave_nan_max(top);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
   __syncthreads();
-  const float scale = nan_max(nan_max(lds[0], lds[1]), nan_max(lds[2], lds[3])) / 127.f;
+  const float scale = nan_max(nan_max(lds[0], lds[1]), nan_max(lds[2], lds[3])) * (1.f / 127.f);
   if (threadIdx.x == 0) scales[row] = scale;
   for (int64_t k = threadIdx.x; k < q_ld; k += 256) q[row * q_ld + k] = k < width ? to_int8((float)src[k], scale) : 0;
 }

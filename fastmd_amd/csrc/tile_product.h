@@ -114,29 +114,28 @@ struct TpStage {
     }
   }
 
-  __device__ static __forceinline__ void copy16(const void* p, char* to) {
-    typedef const __attribute__((address_space(1))) void* global_ptr;
-    typedef __attribute__((address_space(3))) void* lds_ptr;
-    __builtin_amdgcn_global_load_lds((global_ptr)(uintptr_t)p, (lds_ptr)to, 16, 0, 0);
+  // 64 lanes' 16 bytes at base + off (or at p) to LDS from `to` on. As instructions: after the compiler's own form every read of
+  // LDS waits for all copies, those of the other place too. tile_product_kernel holds the waits.
+  __device__ static __forceinline__ void copy16(const char* base, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory", "m0");
+  }
+  __device__ static __forceinline__ void copy16(const char* p, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(p) : "memory", "m0");
   }
 
   // the slice at `at` into LDS; `left`: bytes of K from it on, past them is zero
-  __device__ __forceinline__ void issue(char* lds, int64_t left, int wave, int lane) {
+  __device__ __forceinline__ void issue(uint32_t lds, int64_t left, int wave, int lane) {
     if (left >= kTpSlice) {
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        const char* p = GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0];
-        copy16(p + off[j], lds + (wave * LOADS + j) * 1024);
-      }
+      for (int j = 0; j < LOADS; ++j)
+        copy16(GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0], off[j], lds + (wave * LOADS + j) * 1024);
     } else {
 #pragma unroll
       for (int j = 0; j < LOADS; ++j) {
         const char* p = (GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0]) + off[j];
         const int slot = (wave * LOADS + j) * 64 + lane;
         const int k = ACROSS ? slot / CHUNKS * 2 : ((slot % 8) ^ swap_along(slot / 8)) * 16;
-        p = k < left ? p : reinterpret_cast<const char*>(g_tp_zero_chunk);
-        asm volatile("" : "+v"(p));  // one load instruction with a per-lane address
-        copy16(p, lds + (wave * LOADS + j) * 1024);
+        copy16(k < left ? p : reinterpret_cast<const char*>(g_tp_zero_chunk), lds + (wave * LOADS + j) * 1024);
       }
     }
 #pragma unroll
@@ -255,7 +254,8 @@ tile_product_kernel(TpArgs a, Epi epi) {
     sn.begin(p.n, part, (0x124 >> (2 * pair)) & 3, n0, ks);
     sm.begin(p.m, part, (0x046 >> (2 * pair)) & 3, m0, ks);
   };
-  auto issue = [&](char* st) {
+  auto issue = [&](const char* place) {
+    const uint32_t st = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)place;
     const int64_t left = k_bytes - (int64_t)ks * kTpSlice;
     sn.issue(st, left, wave, lane);
     sm.issue(st + S::StageN::BYTES, left, wave, lane);
@@ -267,11 +267,14 @@ tile_product_kernel(TpArgs a, Epi epi) {
   };
   const int ln = S::StageN::lane_at(lane), lm = S::StageM::lane_at(lane);
   tp_i32x4 fn[2][NB], fm[2][MB];
+  constexpr int READS = (S::StageN::ACROSS ? 2 : 1) * NB + (S::StageM::ACROSS ? 2 : 1) * MB;
   auto read = [&](const char* st, int kk, int to) {
-#pragma unroll
-    for (int i = 0; i < NB; ++i) fn[to][i] = S::StageN::read(st, ln, S::block_n(i, wn), kk);
+    // in the order in which the products take them
+    fn[to][0] = S::StageN::read(st, ln, S::block_n(0, wn), kk);
 #pragma unroll
     for (int j = 0; j < MB; ++j) fm[to][j] = S::StageM::read(st + S::StageN::BYTES, lm, (wm * MB + j) * 32, kk);
+#pragma unroll
+    for (int i = 1; i < NB; ++i) fn[to][i] = S::StageN::read(st, ln, S::block_n(i, wn), kk);
   };
   Acc acc[NB][MB];
 #pragma unroll
@@ -287,22 +290,31 @@ tile_product_kernel(TpArgs a, Epi epi) {
     if (begin + 1 < end) issue(st1);
     // A slice is four steps. The operands of a step are read while the one before runs; before the last step every wave has
     // read the whole slice, so its place takes the slice after the next.
+    auto step = [&](int kk) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j) acc[i][j] = T::mma(fn[kk & 1][i], fm[kk & 1][j], acc[i][j]);
+      // a read after each of the first products
+#pragma unroll
+      for (int i = 0; i < NB * MB; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, (READS + NB * MB - 1) / (NB * MB), 0);
+      }
+    };
     auto slice = [&](char* st, char* next, int s) {
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        if (kk < 3) {
-          read(st, kk + 1, (kk + 1) & 1);
-        } else if (s + 1 < end) {
-          __builtin_amdgcn_s_waitcnt(kTpVm0Lgkm0);
-          __builtin_amdgcn_s_barrier();
-          if (s + 2 < end) issue(st);
-          read(next, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-          for (int j = 0; j < MB; ++j) acc[i][j] = T::mma(fn[kk & 1][i], fm[kk & 1][j], acc[i][j]);
+      for (int kk = 0; kk < 3; ++kk) {
+        read(st, kk + 1, (kk + 1) & 1);
+        step(kk);
       }
+      if (s + 1 < end) {
+        __builtin_amdgcn_s_waitcnt(kTpVm0Lgkm0);
+        __builtin_amdgcn_s_barrier();
+        if (s + 2 < end) issue(st);
+        read(next, 0, 0);
+      }
+      step(3);
     };
     if (begin + 1 < end)
       __builtin_amdgcn_s_waitcnt(((S::StageN::LOADS + S::StageM::LOADS) & 15) | (7 << 4) | (15 << 8));
@@ -318,10 +330,10 @@ tile_product_kernel(TpArgs a, Epi epi) {
     if (s < end) slice(st0, st1, s);
   }
 
-  // results: row m0 + wm 32 MB + 32 j + lane % 32, four columns from n0 + block + 8 q + 4 (lane / 32)
+  // a lane's results: row m0 + wm 32 MB + 32 j + lane % 32, four columns from n0 + block + 8 q + 4 (lane / 32)
   if (splits > 1) {
-    typedef decltype(tp_four(acc[0][0], 0)) Four;
-    Four* out = static_cast<Four*>(a.partial) + (int64_t)((tile - a.full) * splits + split) * (NB * MB * 4) * S::THREADS + t;
+    typedef decltype(tp_four(acc[0][0], 0)) Part;
+    Part* out = static_cast<Part*>(a.partial) + (int64_t)((tile - a.full) * splits + split) * (NB * MB * 4) * S::THREADS + t;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -332,16 +344,30 @@ tile_product_kernel(TpArgs a, Epi epi) {
         }
     return;
   }
+  // Each wave turns its 32 rows at a time round in LDS, so that the epilogue has whole rows side by side in its lanes, and its code
+  // once. Chunks of four are permuted by the row: neither the writes (a column of sixteen rows) nor the reads meet a bank twice.
+  typedef decltype(tp_four(acc[0][0], 0)) Four;
+  constexpr int CHUNKS = NB * 8, REGION = 32 * CHUNKS * 16, EACH = S::GATED ? CHUNKS / 2 : CHUNKS;
+  static_assert(REGION * S::THREADS / 64 <= 2 * S::STAGE, "a place for each wave");
+  __syncthreads();
+  char* mine = wave * REGION < S::STAGE ? st0 + wave * REGION : st1 + (wave * REGION - S::STAGE);
 #pragma unroll
-  for (int i = 0; i < (S::GATED ? NB / 2 : NB); ++i)
+  for (int j = 0; j < MB; ++j) {
+    const int r = lane & 31;
 #pragma unroll
-    for (int j = 0; j < MB; ++j)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t m = m0 + (wm * MB + j) * 32 + (lane & 31), n = n0 + S::block_n(i, wn) + 8 * q + 4 * (lane >> 5);
-        const int u = S::GATED ? i + NB / 2 : i;
-        epi(tt.problem, m, n, tp_four(acc[i][j], q), tp_four(acc[u][j], q));
-      }
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<Four*>(mine + (r * CHUNKS + ((i * 8 + 2 * q + (lane >> 5)) ^ (r & (CHUNKS - 1)))) * 16) = tp_four(acc[i][j], q);
+#pragma unroll 2
+    for (int k = lane; k < 32 * EACH; k += 64) {
+      const int row = k / EACH, c = k % EACH;
+      const Four* x = reinterpret_cast<const Four*>(mine) + row * CHUNKS;
+      const Four v = x[c ^ (row & (CHUNKS - 1))], u = S::GATED ? x[(c + CHUNKS / 2) ^ (row & (CHUNKS - 1))] : v;
+      const int half = c / (CHUNKS / 2);
+      epi(tt.problem, m0 + (wm * MB + j) * 32 + row, n0 + half * (S::BN / 2) + wn * (NB * 16) + (c - half * (CHUNKS / 2)) * 4, v, u);
+    }
+  }
 }
 
 // The tiles that several workgroups share: their sums added in order, then the same epilogue. One workgroup per group of four

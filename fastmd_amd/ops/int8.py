@@ -2,9 +2,9 @@
 
 ``quantize_rows(x)``: each row of a float32 or bfloat16 matrix as 8-bit integers with one float32 scale,
 
-    scale = max |x| / 127,  value = x / scale rounded to the nearest integer (ties to even)
+    scale = max |x| (1 / 127),  value = x / scale rounded to the nearest integer (ties to even)
 
-(the quotients in float32). ``linear_int8(x, weight, bias=None)``: ``linear`` on a weight [out, in] so rounded,
+(product, quotient and 1 / 127 in float32). ``linear_int8(x, weight, bias=None)``: ``linear`` on a weight [out, in] so rounded,
 
     y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]
 
