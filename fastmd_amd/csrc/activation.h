@@ -16,10 +16,16 @@ __device__ __forceinline__ float exp_near(float x) {
   return __builtin_amdgcn_exp2f(t) * fmaf(rest, 0.69314718f, 1.f);
 }
 
-// silu: z s, s (1 + z (1 - s)) with s = 1 / (1 + exp(-z)) (reciprocal to 1 ulp; 1 - s = exp(-z) s where s is near 1); gelu: z P, P + z p with the normal
-// distribution P(z) = (1 + erf(z / sqrt 2)) / 2 and its density p
+// silu: z s, s (1 + z (1 - s)) with s = 1 / (1 + exp(-z)) (reciprocal to 1 ulp; 1 - s = exp(-z) s where s is near 1); gelu: z P,
+// P + z p with the normal distribution P(z) = (1 + erf(z / sqrt 2)) / 2 and its density p. FAST, for results that are rounded
+// to bf16 at once: silu's exponential by the instruction alone, off by |z| 2^-24 of itself, and 1 - s as it is.
+template <bool FAST = false>
 __device__ __forceinline__ ActValue activation(float z, int act) {
   if (act == kActSilu) {
+    if (FAST) {
+      const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+      return {z * s, s * fmaf(z, 1.f - s, 1.f)};
+    }
     const float e = exp_near(-z), s = __builtin_amdgcn_rcpf(1.f + e);
     return {z * s, s * (1.f + z * (z < 0.f ? 1.f - s : e * s))};
   }

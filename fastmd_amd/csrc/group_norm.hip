@@ -5,10 +5,10 @@
 // Rows by themselves: a row's group is held by 1 to 64 lanes, or by a workgroup; one read, one write.
 //
 // Segments: tiles of rows of one segment (attention_find.h: the host knows no length) in registers. A segment that is one tile
-// is done with it. Longer ones leave their tiles' means and squares (merged by the counts: no difference of large sums), are
-// joined, and read a second time, mostly from the last-level cache. The backward pass does the same with the channels' sums of gz
-// and gz n (gz: the gradient before the activation): they are the weights' gradients, and weighted they are the two means that
-// gx needs.
+// is done with it. Longer ones leave their tiles' means and squares, and are read a second time, mostly from the last-level cache,
+// by workgroups that merge them first (by the counts, in 64 bits: no difference of large sums). The backward pass does the
+// same with the channels' sums of gz and gz n (gz: the gradient before the activation): they are the weights'
+// gradients, and weighted they are the two means that gx needs.
 #include "activation.h"
 #include "attention_find.h"
 #include "common.h"
@@ -18,6 +18,16 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTileValues = 64;  // of a thread's registers
+#ifndef FEW
+#define FEW 1024
+#endif
+#ifndef NRBACK
+#define NRBACK 1
+#endif
+#ifndef MERGE
+#define MERGE 16
+#endif
+constexpr int64_t kFewTiles = FEW;
 
 struct GnArgs {
   const void *x, *g;  // rows [rows, channels], row strides x_ld, g_ld; g: gradient of y
@@ -150,7 +160,7 @@ __global__ void __launch_bounds__(kThreads) gn_rows_kernel(GnArgs a) {
     float o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      o[i] = activation(v[n][i] * inverse * param<T>(a.weight, c0 + c + i, 1.f) + param<T>(a.bias, c0 + c + i, 0.f), a.act).value;
+      o[i] = activation<sizeof(T) == 2>(v[n][i] * inverse * param<T>(a.weight, c0 + c + i, 1.f) + param<T>(a.bias, c0 + c + i, 0.f), a.act).value;
     raw_store<T, V>(y + c, o);
   }
 }
@@ -191,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) gn_rows_bwd_kernel(GnArgs a) {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         h[n][i] = in ? (raw_get<T, V>(r, i) - mean) * inverse : 0.f;
-        z[n][i] = in ? raw_get<T, V>(q, i) * activation(h[n][i] * w[n][i] + b[n][i], a.act).slope : 0.f;
+        z[n][i] = in ? raw_get<T, V>(q, i) * activation<sizeof(T) == 2>(h[n][i] * w[n][i] + b[n][i], a.act).slope : 0.f;
         gw[n][i] += z[n][i] * h[n][i];
         gb[n][i] += z[n][i];
         z[n][i] *= w[n][i];
@@ -268,11 +278,13 @@ __global__ void __launch_bounds__(1024) gn_columns_kernel(const float* part, int
 template <int V, int NV>
 struct GnPlace {
   int c0, nc, groups, x, y, step;
+  float per;  // groups per channel
   bool in;
   __device__ __forceinline__ GnPlace(const GnArgs& a) {
     c0 = blockIdx.y * a.chunk;
     nc = min(a.chunk, a.channels - c0);
     groups = nc / a.width;
+    per = 1.f / a.width;
     step = NV > 1 ? 1 : kThreads / a.tx;
     x = NV > 1 ? threadIdx.x : threadIdx.x % a.tx;
     y = NV > 1 ? 0 : threadIdx.x / a.tx;
@@ -280,6 +292,8 @@ struct GnPlace {
   }
   __device__ __forceinline__ int column(int n) const { return (x + n * kThreads) * V; }  // within the share
   __device__ __forceinline__ bool has(int n) const { return in && column(n) < nc; }
+  // channel / width, for fewer than 2^13 channels: the half keeps the rounded product off the whole numbers
+  __device__ __forceinline__ int group(int channel) const { return (int)(((float)channel + 0.5f) * per); }
 };
 
 // Sums over the share's groups of `count` rows of values per channel in lds [count, nc]: out[g], in the same order for every call.
@@ -288,11 +302,12 @@ __device__ __forceinline__ void group_sums(const float* lds, int count, int nc, 
   int lanes = 64;
   while (lanes > 1 && lanes * groups > kThreads) lanes >>= 1;
   const int lane = threadIdx.x % lanes, total = count * width, each = kThreads / lanes;
+  const float per = 1.f / width;
   for (int g = threadIdx.x / lanes; g < max(groups, each); g += each) {  // several lanes a group: one pass, all take part
     float s = 0.f;
     if (g < groups)
       for (int i = lane; i < total; i += lanes) {
-        const int r = i / width;
+        const int r = (int)(((float)i + 0.5f) * per);  // i / width (fewer than 2^14 values)
         s += lds[r * nc + g * width + (i - r * width)];
       }
     for (int off = lanes >> 1; off; off >>= 1) s += __shfl_xor(s, off, 64);
@@ -334,34 +349,35 @@ __device__ __forceinline__ GnTile gn_long_tile(const GnArgs& a, int64_t number) 
 template <typename T, int V, int NV, int NR>
 struct GnRegs {
   typename RawVec<T, V>::Type r[NR][NV];
+  // rows and columns past the end: the last row, or the first column, again
   __device__ __forceinline__ void load(const GnPlace<V, NV>& p, const T* x, int64_t ld, int rows) {
 #pragma unroll
     for (int k = 0; k < NR; ++k)
 #pragma unroll
-      for (int n = 0; n < NV; ++n) {
-        const int row = p.y + k * p.step;
-        r[k][n] = typename RawVec<T, V>::Type{};
-        if (p.has(n) && row < rows) r[k][n] = raw_load<T, V>(x + row * ld + p.c0 + p.column(n));
-      }
+      for (int n = 0; n < NV; ++n)
+        r[k][n] = raw_load<T, V>(x + min(p.y + k * p.step, rows - 1) * ld + p.c0 + (p.has(n) ? p.column(n) : 0));
   }
   __device__ __forceinline__ float get(int k, int n, int i) const { return raw_get<T, V>(r[k][n], i); }
 };
 
 // per channel of this thread: the group's value from lds
 template <int V, int NV>
-__device__ __forceinline__ void spread(const GnPlace<V, NV>& p, int width, const float* of_group, float (&v)[NV][V]) {
+__device__ __forceinline__ void spread(const GnPlace<V, NV>& p, const float* of_group, float (&v)[NV][V]) {
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[n][i] = p.has(n) ? of_group[(p.column(n) + i) / width] : 0.f;
+    for (int i = 0; i < V; ++i) v[n][i] = of_group[p.has(n) ? p.group(p.column(n) + i) : 0];
 }
 
 template <typename T, int V, int NV>
 __device__ __forceinline__ void spread_param(const GnPlace<V, NV>& p, const void* src, float none, float (&v)[NV][V]) {
 #pragma unroll
-  for (int n = 0; n < NV; ++n)
+  for (int n = 0; n < NV; ++n) {
+    typename RawVec<T, V>::Type r{};
+    if (src) r = raw_load<T, V>(static_cast<const T*>(src) + p.c0 + (p.has(n) ? p.column(n) : 0));
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[n][i] = p.has(n) ? param<T>(src, p.c0 + p.column(n) + i, none) : 0.f;
+    for (int i = 0; i < V; ++i) v[n][i] = src ? raw_get<T, V>(r, i) : none;
+  }
 }
 
 // values per channel, a row of lds for each of the workgroup's rows of threads
@@ -404,7 +420,7 @@ __device__ __forceinline__ void write_norm(const GnArgs& a, const GnPlace<V, NV>
       if (!p.has(n) || row >= rows) continue;
       float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = activation((x.get(k, n, i) - mean[n][i]) * w[n][i] + b[n][i], a.act).value;
+      for (int i = 0; i < V; ++i) o[i] = activation<sizeof(T) == 2>((x.get(k, n, i) - mean[n][i]) * w[n][i] + b[n][i], a.act).value;
       raw_store<T, V>(y + (int64_t)row * a.channels + p.c0 + p.column(n), o);
     }
 }
@@ -432,14 +448,14 @@ __global__ void __launch_bounds__(kThreads) gn_tile_kernel(GnArgs a) {
     for (int i = 0; i < V; ++i) {
       s[n][i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < NR; ++k) s[n][i] += x.get(k, n, i);  // zero past the rows
+      for (int k = 0; k < NR; ++k) s[n][i] += p.y + k * p.step < rows ? x.get(k, n, i) : 0.f;
     }
   put_channels<V, NV>(p, lds, s);
   __syncthreads();
   group_sums(lds, p.step, p.nc, a.width, p.groups, of_group);
   __syncthreads();
   float mean[NV][V];
-  spread<V, NV>(p, a.width, of_group, mean);
+  spread<V, NV>(p, of_group, mean);
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -466,7 +482,7 @@ __global__ void __launch_bounds__(kThreads) gn_tile_kernel(GnArgs a) {
     return;
   }
   float inverse[NV][V];
-  spread<V, NV>(p, a.width, squares, inverse);
+  spread<V, NV>(p, squares, inverse);
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -480,53 +496,95 @@ __global__ void __launch_bounds__(kThreads) gn_tile_kernel(GnArgs a) {
   write_norm<T, V, NV, NR>(a, p, x, y, rows, mean, inverse);
 }
 
-// A longer segment's tiles joined, a wave a group: numbers from floor(start / tile) on, of which such a segment owns one at least.
-__global__ void __launch_bounds__(kThreads) gn_join_kernel(GnArgs a) {
-  const auto num = [&](int i) { return attn_start(a.off, a.segments, a.rows, i) / a.tile_rows; };
-  const int64_t number = (int64_t)blockIdx.x + a.block0;
-  const int i = attn_last(a.segments + 2, number, num, WaveLanes());
-  const int64_t start = attn_start(a.off, a.segments, a.rows, i), rows = attn_start(a.off, a.segments, a.rows, i + 1) - start;
-  if (i < 1 || i > a.segments || rows <= a.tile_rows || num(i) != number) return;
-  const int g = blockIdx.y * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
-  if (g >= a.groups) return;
+// Where a segment has more tiles than this, their sums are merged once, by gn_merge_kernel, not by each of the workgroups.
+constexpr int kMergeTiles = MERGE;
+
+__device__ __forceinline__ bool merged_apart(const GnArgs& a, int64_t rows) { return rows > (int64_t)kMergeTiles * a.tile_rows; }
+
+struct GnStats {
+  float x, y;
+};
+
+// Of group g of a longer segment, by `lanes` (a power of two) lanes that all call it: mean and inverse, or the two means of the
+// backward pass. `tile`: number of its first tile.
+template <bool BACK>
+__device__ __forceinline__ GnStats merge(const GnArgs& a, int64_t tile, int64_t rows, int g, int lane, int lanes) {
   const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows;
-  const float2* part = reinterpret_cast<const float2*>(a.part) + (start / a.tile_rows + i) * a.groups + g;
-  const float full = (float)a.tile_rows * a.width, last = (float)(rows - (tiles - 1) * a.tile_rows) * a.width;
-  // means about the first tile's, so that nothing large cancels
-  const float pivot = part[0].x;
+  const float2* part = reinterpret_cast<const float2*>(a.part) + tile * a.groups + g;
   const double total = (double)rows * a.width;
-  double s = 0.0;
-  for (int64_t k = lane; k < tiles; k += 64) s += (double)(part[k * a.groups].x - pivot) * (k == tiles - 1 ? last : full);
-  const float mean = (float)(pivot + wave_sum(s) / total);
-  double d = 0.0;
-  for (int64_t k = lane; k < tiles; k += 64) {
-    const float2 v = part[k * a.groups];
-    const double e = (double)v.x - mean;
-    d += (double)v.y + e * e * (k == tiles - 1 ? last : full);
+  double s = 0.0, q = 0.0;
+  if (BACK) {
+    for (int64_t k = lane; k < tiles; k += lanes) {
+      const float2 v = part[k * a.groups];
+      s += v.x;
+      q += v.y;
+    }
+  } else {
+    const double full = (double)a.tile_rows * a.width, last = (double)(rows - (tiles - 1) * a.tile_rows) * a.width;
+    const float pivot = part[0].x;
+    for (int64_t k = lane; k < tiles; k += lanes) {
+      const float2 v = part[k * a.groups];
+      const double d = (double)v.x - pivot, n = k == tiles - 1 ? last : full;
+      s += d * n;
+      q += v.y + d * d * n;
+    }
   }
-  d = wave_sum(d);
-  if (lane) return;
-  a.mean[(int64_t)(i - 1) * a.groups + g] = mean;
-  a.inverse[(int64_t)(i - 1) * a.groups + g] = (float)(1.0 / sqrt(d / total + (double)a.eps));
+  for (int off = lanes >> 1; off; off >>= 1) {
+    s += __shfl_xor(s, off, 64);
+    q += __shfl_xor(q, off, 64);
+  }
+  if (BACK) return {(float)(s / total), (float)(q / total)};
+  const double mean = s / total, square = q / total - mean * mean;
+  return {(float)(part[0].x + mean), (float)(1.0 / sqrt((square > 0.0 || square != square ? square : 0.0) + (double)a.eps))};
 }
 
-template <int V, int NV>
-__device__ __forceinline__ void load_stats(const GnArgs& a, const GnPlace<V, NV>& p, int segment, float (&mean)[NV][V],
-                                           float (&inverse)[NV][V]) {
-  const int64_t at = (int64_t)(segment - 1) * a.groups + p.c0 / a.width;
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int g = (p.column(n) + i) / a.width;
-      mean[n][i] = p.has(n) ? a.mean[at + g] : 0.f;
-      inverse[n][i] = p.has(n) ? a.inverse[at + g] : 0.f;
+// The segments of many tiles, a wave a group. A workgroup a segment, or, where there are more segments than could have so many tiles,
+// numbers from floor(start / (kMergeTiles tiles)) on, of which such a segment owns one at least.
+template <bool BACK>
+__global__ void __launch_bounds__(kThreads) gn_merge_kernel(GnArgs a, float* x, float* y, int stride, int by_number) {
+  const int64_t number = (int64_t)blockIdx.x + a.block0;
+  int i = (int)number + 1;
+  const auto num = [&](int i) { return attn_start(a.off, a.segments, a.rows, i) / ((int64_t)kMergeTiles * a.tile_rows); };
+  if (by_number) i = attn_last(a.segments + 2, number, num, WaveLanes());
+  const int64_t start = attn_start(a.off, a.segments, a.rows, i), rows = attn_start(a.off, a.segments, a.rows, i + 1) - start;
+  if (i < 1 || i > a.segments || !merged_apart(a, rows) || (by_number && num(i) != number)) return;
+  const int g = blockIdx.y * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
+  if (g >= a.groups) return;
+  const GnStats s = merge<BACK>(a, start / a.tile_rows + i, rows, g, lane, 64);
+  if (lane) return;
+  x[((int64_t)(i - 1) * a.groups + g) * stride] = s.x;
+  y[((int64_t)(i - 1) * a.groups + g) * stride] = s.y;
+}
+
+// the same for the share's groups, into lds [2, groups], by the workgroup
+template <bool BACK>
+__device__ __forceinline__ void merge_share(const GnArgs& a, const GnTile& t, int g0, int groups, float* lds) {
+  int lanes = 64;
+  while (lanes > 1 && lanes * groups > kThreads) lanes >>= 1;
+  const int lane = threadIdx.x % lanes, each = kThreads / lanes;
+  for (int g = threadIdx.x / lanes; g < max(groups, each); g += each) {  // several lanes a group: one pass, all take part
+    const GnStats s = merge<BACK>(a, t.start / a.tile_rows + t.segment, t.rows, g0 + min(g, groups - 1), lane, lanes);
+    if (lane == 0 && g < groups) {
+      lds[g] = s.x;
+      lds[groups + g] = s.y;
     }
+  }
+  __syncthreads();
+}
+
+// the share's groups' values of a segment from memory [segments, groups] (or interleaved, stride 2) into lds [2, groups]
+__device__ __forceinline__ void load_share(const float* x, const float* y, int stride, int64_t at, int groups, float* lds) {
+  for (int g = threadIdx.x; g < groups; g += kThreads) {
+    lds[g] = x[(at + g) * stride];
+    lds[groups + g] = y[(at + g) * stride];
+  }
+  __syncthreads();
 }
 
 // Second read of the longer segments.
 template <typename T, int V, int NV, int NR>
 __global__ void __launch_bounds__(kThreads) gn_apply_kernel(GnArgs a) {
+  extern __shared__ float lds[];  // [2, groups of the share]
   const GnPlace<V, NV> p(a);
   const GnTile t = gn_long_tile(a, (int64_t)blockIdx.x + a.block0);
   if (!t.real || t.whole || t.first >= t.rows) return;
@@ -535,7 +593,19 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(GnArgs a) {
   GnRegs<T, V, NV, NR> x;
   x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
   float mean[NV][V], inverse[NV][V];
-  load_stats<V, NV>(a, p, t.segment, mean, inverse);
+  const int g0 = p.c0 / a.width;
+  if (merged_apart(a, t.rows)) {
+    load_share(a.mean, a.inverse, 1, (int64_t)(t.segment - 1) * a.groups + g0, p.groups, lds);
+  } else {
+    merge_share<false>(a, t, g0, p.groups, lds);
+    if (t.first == 0)
+      for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+        a.mean[(int64_t)(t.segment - 1) * a.groups + g0 + g] = lds[g];
+        a.inverse[(int64_t)(t.segment - 1) * a.groups + g0 + g] = lds[p.groups + g];
+      }
+  }
+  spread<V, NV>(p, lds, mean);
+  spread<V, NV>(p, lds + p.groups, inverse);
   write_norm<T, V, NV, NR>(a, p, x, static_cast<T*>(a.y) + row0 * a.channels, rows, mean, inverse);
 }
 
@@ -555,23 +625,25 @@ __device__ __forceinline__ void write_grad(const GnArgs& a, const GnPlace<V, NV>
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
-        const float z = gy.get(k, n, i) * activation(h * w[n][i] + b[n][i], a.act).slope * w[n][i];
+        const float z = gy.get(k, n, i) * activation<sizeof(T) == 2>(h * w[n][i] + b[n][i], a.act).slope * w[n][i];
         o[i] = inverse[n][i] * (z - s[n][i] - h * q[n][i]);
       }
       raw_store<T, V>(gx + (int64_t)row * a.channels + p.c0 + p.column(n), o);
+      __builtin_amdgcn_sched_barrier(0);
     }
 }
 
-// First read of the backward pass. part: [tiles, 2, channels], the channels' sums of gz n and gz.
+// First read of the backward pass. columns: [tiles, 2, channels], the channels' sums of gz n and gz; part: [tiles, groups, 2], the
+// groups' of gz w and gz w n.
 template <typename T, int V, int NV, int NR>
-__global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a) {
-  extern __shared__ float lds[];  // [rows of threads, share], then the groups' values twice
+__global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a, float* columns) {
+  extern __shared__ float lds[];  // [2, rows of threads, share], then the groups' values twice
   const GnPlace<V, NV> p(a);
   const int64_t number = (int64_t)blockIdx.x + a.block0;
   const GnTile t = gn_tile(a, number);
-  float* part = a.part + number * 2 * a.channels + p.c0;
+  columns += number * 2 * a.channels + p.c0;
   if (t.first >= t.rows || !t.real) {
-    for (int c = threadIdx.x; c < p.nc; c += kThreads) part[c] = part[a.channels + c] = 0.f;
+    for (int c = threadIdx.x; c < p.nc; c += kThreads) columns[c] = columns[a.channels + c] = 0.f;
     if (t.first >= t.rows) return;
   }
   const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
@@ -582,44 +654,55 @@ __global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a) {
   x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
   gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
   float mean[NV][V], inverse[NV][V], w[NV][V], b[NV][V], gw[NV][V], gb[NV][V];
-  load_stats<V, NV>(a, p, t.segment, mean, inverse);
+  float* of_group = lds + 2 * p.step * p.nc;
+  load_share(a.mean, a.inverse, 1, (int64_t)(t.segment - 1) * a.groups + p.c0 / a.width, p.groups, of_group);
+  spread<V, NV>(p, of_group, mean);
+  spread<V, NV>(p, of_group + p.groups, inverse);
   spread_param<T, V, NV>(p, a.weight, 1.f, w);
   spread_param<T, V, NV>(p, a.bias, 0.f, b);
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      gw[n][i] = gb[n][i] = 0.f;
+    for (int i = 0; i < V; ++i) gw[n][i] = gb[n][i] = 0.f;
 #pragma unroll
-      for (int k = 0; k < NR; ++k) {
-        if (p.y + k * p.step >= rows) break;
+  for (int k = 0; k < NR; ++k) {
+    const float in = p.y + k * p.step < rows ? 1.f : 0.f;
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
         const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
-        const float z = gy.get(k, n, i) * activation(h * w[n][i] + b[n][i], a.act).slope;
+        const float z = (in != 0.f ? gy.get(k, n, i) : 0.f) * activation<sizeof(T) == 2>(h * w[n][i] + b[n][i], a.act).slope;
         gw[n][i] += z * h;
         gb[n][i] += z;
       }
-    }
-  float* of_group = lds + p.step * p.nc;
-  auto channels = [&](const float (&v)[NV][V], float* out, float* groups) {
-    put_channels<V, NV>(p, lds, v);
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.nc; c += kThreads) {
-      float s = 0.f;
-      for (int y = 0; y < p.step; ++y) s += lds[y * p.nc + c];
-      out[c] = s;
-      lds[c] = s * param<T>(a.weight, p.c0 + c, 1.f);  // row 0 of this channel has been read
-    }
-    __syncthreads();
-    if (t.whole) group_sums(lds, 1, p.nc, a.width, p.groups, groups);
-    __syncthreads();
-  };
-  channels(gw, part, of_group);
-  channels(gb, part + a.channels, of_group + p.groups);
-  if (!t.whole) return;
+    __builtin_amdgcn_sched_barrier(0);  // a row after the other: all at once took 256 registers
+  }
+  const int plane = p.step * p.nc;
+  put_channels<V, NV>(p, lds, gw);
+  put_channels<V, NV>(p, lds + plane, gb);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * p.nc; i += kThreads) {
+    const int which = i >= p.nc, c = i - which * p.nc;
+    float* of = lds + which * plane + c;
+    float s = 0.f;
+    for (int y = 0; y < p.step; ++y) s += of[y * p.nc];
+    columns[which * a.channels + c] = s;
+    *of = s * param<T>(a.weight, p.c0 + c, 1.f);  // the channel's first row has been read
+  }
+  __syncthreads();
+  group_sums(lds, 1, p.nc, a.width, p.groups, of_group);
+  group_sums(lds + plane, 1, p.nc, a.width, p.groups, of_group + p.groups);
+  __syncthreads();
+  if (!t.whole) {
+    for (int g = threadIdx.x; g < p.groups; g += kThreads)
+      reinterpret_cast<float2*>(a.part)[number * a.groups + p.c0 / a.width + g] = make_float2(of_group[p.groups + g], of_group[g]);
+    return;
+  }
   const float count = (float)((int64_t)rows * a.width);
   float s[NV][V], q[NV][V];
-  spread<V, NV>(p, a.width, of_group + p.groups, s);
-  spread<V, NV>(p, a.width, of_group, q);
+  spread<V, NV>(p, of_group + p.groups, s);
+  spread<V, NV>(p, of_group, q);
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -627,37 +710,16 @@ __global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a) {
       s[n][i] /= count;
       q[n][i] /= count;
     }
+  // read again, from the cache: kept over the sums, with what was formed of them, they took a hundred registers
+  asm volatile("" : : : "memory");
+  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
+  gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
   write_grad<T, V, NV, NR>(a, p, x, gy, gx, rows, mean, inverse, w, b, s, q);
 }
 
-// The two means of a longer segment's groups, a wave a group, into means [segments, groups, 2].
-template <typename T>
-__global__ void __launch_bounds__(kThreads) gn_join_bwd_kernel(GnArgs a, float2* means) {
-  const auto num = [&](int i) { return attn_start(a.off, a.segments, a.rows, i) / a.tile_rows; };
-  const int64_t number = (int64_t)blockIdx.x + a.block0;
-  const int i = attn_last(a.segments + 2, number, num, WaveLanes());
-  const int64_t start = attn_start(a.off, a.segments, a.rows, i), rows = attn_start(a.off, a.segments, a.rows, i + 1) - start;
-  if (i < 1 || i > a.segments || rows <= a.tile_rows || num(i) != number) return;
-  const int g = blockIdx.y * 4 + threadIdx.x / 64, lane = threadIdx.x & 63;
-  if (g >= a.groups) return;
-  const int64_t tiles = (rows + a.tile_rows - 1) / a.tile_rows, total = tiles * a.width;
-  const float* part = a.part + (start / a.tile_rows + i) * 2 * a.channels + (int64_t)g * a.width;
-  float s = 0.f, q = 0.f;
-  for (int64_t k = lane; k < total; k += 64) {
-    const int64_t tile = k / a.width;
-    const int c = (int)(k - tile * a.width);
-    const float w = param<T>(a.weight, (int64_t)g * a.width + c, 1.f);
-    q += part[tile * 2 * a.channels + c] * w;
-    s += part[tile * 2 * a.channels + a.channels + c] * w;
-  }
-  s = wave_sum(s);
-  q = wave_sum(q);
-  const float count = (float)((double)rows * a.width);
-  if (lane == 0) means[(int64_t)(i - 1) * a.groups + g] = make_float2(s / count, q / count);
-}
-
 template <typename T, int V, int NV, int NR>
-__global__ void __launch_bounds__(kThreads) gn_apply_bwd_kernel(GnArgs a, const float2* means) {
+__global__ void __launch_bounds__(kThreads) gn_apply_bwd_kernel(GnArgs a, const float* means) {
+  extern __shared__ float lds[];  // [4, groups of the share]
   const GnPlace<V, NV> p(a);
   const GnTile t = gn_long_tile(a, (int64_t)blockIdx.x + a.block0);
   if (!t.real || t.whole || t.first >= t.rows) return;
@@ -667,18 +729,19 @@ __global__ void __launch_bounds__(kThreads) gn_apply_bwd_kernel(GnArgs a, const 
   x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
   gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
   float mean[NV][V], inverse[NV][V], w[NV][V], b[NV][V], s[NV][V], q[NV][V];
-  load_stats<V, NV>(a, p, t.segment, mean, inverse);
+  const int g0 = p.c0 / a.width;
+  const int64_t at = (int64_t)(t.segment - 1) * a.groups + g0;
+  load_share(a.mean, a.inverse, 1, at, p.groups, lds + 2 * p.groups);
+  if (merged_apart(a, t.rows))
+    load_share(means, means + 1, 2, at, p.groups, lds);
+  else
+    merge_share<true>(a, t, g0, p.groups, lds);
+  spread<V, NV>(p, lds, s);
+  spread<V, NV>(p, lds + p.groups, q);
+  spread<V, NV>(p, lds + 2 * p.groups, mean);
+  spread<V, NV>(p, lds + 3 * p.groups, inverse);
   spread_param<T, V, NV>(p, a.weight, 1.f, w);
   spread_param<T, V, NV>(p, a.bias, 0.f, b);
-  const float2* m = means + (int64_t)(t.segment - 1) * a.groups + p.c0 / a.width;
-#pragma unroll
-  for (int n = 0; n < NV; ++n)
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float2 v = p.has(n) ? m[(p.column(n) + i) / a.width] : make_float2(0.f, 0.f);
-      s[n][i] = v.x;
-      q[n][i] = v.y;
-    }
   write_grad<T, V, NV, NR>(a, p, x, gy, static_cast<T*>(a.gx) + row0 * a.channels, rows, mean, inverse, w, b, s, q);
 }
 
@@ -770,7 +833,7 @@ struct TileShape {
   int v, nv, nr, chunk, tx, rows, chunks, lds;
 };
 
-TileShape tile_shape(const GnArgs& a, int size) {
+TileShape tile_shape(const GnArgs& a, int size, bool back) {
   TileShape s{};
   for (s.v = vector_of(a, size, a.channels);; s.v >>= 1) {
     const int most = kThreads * s.v;
@@ -786,28 +849,32 @@ TileShape tile_shape(const GnArgs& a, int size) {
   s.nv = s.tx > kThreads ? (s.tx + kThreads - 1) / kThreads : 1;
   const int most = s.v == 1 ? 32 : 32 / s.v;  // registers of the wide form: 8 192 channels of a group at most
   if (s.nv > 1) s.nv = s.nv <= most ? most : -1;
-  s.nr = kTileValues / (s.v * (s.nv > 1 ? s.nv : 1));
-  if (s.v == 1 && s.nv == 1) s.nr = 32;
-  s.rows = s.nr * (s.nv > 1 ? 1 : kThreads / s.tx);
-  s.chunks = (a.channels + s.chunk - 1) / s.chunk;
   const int rows = s.nv > 1 ? 1 : kThreads / s.tx;
-  s.lds = (rows * s.chunk + 2 * (s.chunk / a.width)) * 4;
+  // of up to 64 values a thread, fewer where the tiles would not fill the card
+  s.nr = s.nv > 1 ? 2 : s.v == 1 ? 32 : kTileValues / s.v;
+  if (s.nv == 1)
+    for (int i = 0; i < 2 && (a.rows / (s.nr * rows) < kFewTiles || i < NRBACK * back); ++i) s.nr /= 2;
+  s.rows = s.nr * rows;
+  s.chunks = (a.channels + s.chunk - 1) / s.chunk;
+  s.lds = ((back ? 2 : 1) * rows * s.chunk + 2 * (s.chunk / a.width)) * 4;
   return s;
 }
 
 template <typename T, typename Fn>
 int with_tiles(const TileShape& s, const Fn& fn) {
 #define GN_TILE(V, NV, NR) return fn(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, NR>{})
-  if constexpr (sizeof(T) == 2) {
-    if (s.v == 8 && s.nv == 1) GN_TILE(8, 1, 8);
-    if (s.v == 8 && s.nv == 4) GN_TILE(8, 4, 2);
-  }
-  if (s.v == 4 && s.nv == 1) GN_TILE(4, 1, 16);
-  if (s.v == 4 && s.nv == 8) GN_TILE(4, 8, 2);
-  if (s.v == 2 && s.nv == 1) GN_TILE(2, 1, 32);
-  if (s.v == 2 && s.nv == 16) GN_TILE(2, 16, 2);
-  if (s.v == 1 && s.nv == 1) GN_TILE(1, 1, 32);
-  if (s.v == 1 && s.nv == 32) GN_TILE(1, 32, 2);
+#define GN_TILES(V, NR)                               \
+  if (s.v == V && s.nv == 1) {                         \
+    if (s.nr == NR) GN_TILE(V, 1, NR);                 \
+    if (s.nr == NR / 2) GN_TILE(V, 1, NR / 2);         \
+    if (s.nr == NR / 4) GN_TILE(V, 1, NR / 4);         \
+  }                                                    \
+  if (s.v == V && s.nv == 32 / V) GN_TILE(V, 32 / V, 2)
+  if constexpr (sizeof(T) == 2) { GN_TILES(8, 8); }
+  GN_TILES(4, 16);
+  GN_TILES(2, 32);
+  GN_TILES(1, 32);
+#undef GN_TILES
 #undef GN_TILE
   return FMD_EUNSUPPORTED;
 }
@@ -834,7 +901,7 @@ int norm(GnArgs a, hipStream_t stream) {
       });
     });
   }
-  const TileShape s = tile_shape(a, sizeof(T));
+  const TileShape s = tile_shape(a, sizeof(T), false);
   FMD_REQUIRE(s.chunks < 65536);
   set_tiles(a, s);
   return with_tiles<T>(s, [&](auto v, auto nv, auto nr) {
@@ -843,12 +910,16 @@ int norm(GnArgs a, hipStream_t stream) {
       gn_tile_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a);
     });
     if (status || a.rows <= s.rows) return status;  // no segment is longer than a tile
-    status = in_launches(a, a.rows / s.rows, [&](unsigned blocks) {
-      gn_join_kernel<<<dim3(blocks, (a.groups + 3) / 4), kThreads, 0, stream>>>(a);
-    });
-    if (status) return status;
+    if (a.rows > kMergeTiles * s.rows) {
+      const int64_t numbers = a.rows / (kMergeTiles * s.rows);
+      const int by_number = numbers < a.segments;
+      status = in_launches(a, by_number ? numbers : a.segments, [&](unsigned blocks) {
+        gn_merge_kernel<false><<<dim3(blocks, (a.groups + 3) / 4), kThreads, 0, stream>>>(a, a.mean, a.inverse, 1, by_number);
+      });
+      if (status) return status;
+    }
     return in_launches(a, 2 * a.rows / s.rows + 1, [&](unsigned blocks) {
-      gn_apply_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 0, stream>>>(a);
+      gn_apply_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 2 * (s.chunk / a.width) * 4, stream>>>(a);
     });
   });
 }
@@ -872,18 +943,20 @@ int columns(const float* part, int64_t count, int64_t channels, float* sums, voi
   return FMD_OK;
 }
 
-// floats of the backward pass's scratch: the partial sums, the long segments' means, the sums of blocks
+// floats of the backward pass's scratch: the channels' sums, the groups' of tiles, the longest segments' means, the sums of blocks
 struct BackSpace {
-  int64_t part, means, sums;
+  int64_t columns, part, means, sums;
 };
 
 BackSpace back_space(const GnArgs& a, int size) {
   BackSpace s{};
   if (!a.off) {
     const RowShape r = row_shape(a, size);
-    s.part = row_blocks(a, r) * (kThreads / r.lanes / row_groups(a, r)) * 2 * a.channels;
+    s.columns = row_blocks(a, r) * (kThreads / r.lanes / row_groups(a, r)) * 2 * a.channels;
   } else {
-    s.part = tile_count(a, tile_shape(a, size)) * 2 * a.channels;
+    const int64_t tiles = tile_count(a, tile_shape(a, size, true));
+    s.columns = tiles * 2 * a.channels;
+    s.part = tiles * 2 * a.groups;
     s.means = 2 * (int64_t)a.segments * a.groups;
   }
   s.sums = kColumnBlocks * 2 * a.channels;
@@ -893,10 +966,8 @@ BackSpace back_space(const GnArgs& a, int size) {
 template <typename T>
 int norm_bwd(GnArgs a, float* work, void* gw, void* gb, hipStream_t stream) {
   const BackSpace space = back_space(a, sizeof(T));
-  float* part = work;
-  float2* means = reinterpret_cast<float2*>(work + space.part);
-  float* sums = work + space.part + space.means;
-  a.part = part;
+  float *part = work, *means = work + space.columns + space.part, *sums = means + space.means;
+  a.part = a.off ? work + space.columns : part;
   if (!a.off) {
     const RowShape s = row_shape(a, sizeof(T));
     a.lanes = s.lanes;
@@ -913,21 +984,25 @@ int norm_bwd(GnArgs a, float* work, void* gw, void* gb, hipStream_t stream) {
     if (status || !gw) return status;
     return columns<T>(part, (int64_t)a.blocks * rows, a.channels, sums, gw, gb, stream);
   }
-  const TileShape s = tile_shape(a, sizeof(T));
+  const TileShape s = tile_shape(a, sizeof(T), true);
   FMD_REQUIRE(s.chunks < 65536);
   set_tiles(a, s);
   const int status = with_tiles<T>(s, [&](auto v, auto nv, auto nr) {
     constexpr int V = decltype(v)::value, NV = decltype(nv)::value, NR = decltype(nr)::value;
     int status = in_launches(a, tile_count(a, s), [&](unsigned blocks) {
-      gn_tile_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a);
+      gn_tile_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a, part);
     });
     if (status || a.rows <= s.rows) return status;
-    status = in_launches(a, a.rows / s.rows, [&](unsigned blocks) {
-      gn_join_bwd_kernel<T><<<dim3(blocks, (a.groups + 3) / 4), kThreads, 0, stream>>>(a, means);
-    });
-    if (status) return status;
+    if (a.rows > kMergeTiles * s.rows) {
+      const int64_t numbers = a.rows / (kMergeTiles * s.rows);
+      const int by_number = numbers < a.segments;
+      status = in_launches(a, by_number ? numbers : a.segments, [&](unsigned blocks) {
+        gn_merge_kernel<true><<<dim3(blocks, (a.groups + 3) / 4), kThreads, 0, stream>>>(a, means, means + 1, 2, by_number);
+      });
+      if (status) return status;
+    }
     return in_launches(a, 2 * a.rows / s.rows + 1, [&](unsigned blocks) {
-      gn_apply_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 0, stream>>>(a, means);
+      gn_apply_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 4 * (s.chunk / a.width) * 4, stream>>>(a, means);
     });
   });
   if (status || !gw) return status;
@@ -965,7 +1040,7 @@ int64_t fmd_group_norm_work_size(int32_t bf16, int64_t rows, int32_t channels, i
   int64_t most = 0;
   for (int v = 1; v <= 8; v *= 2) {
     a.x_ld = channels % v == 0 ? v : 1;
-    const int64_t n = tile_count(a, tile_shape(a, bf16 ? 2 : 4));
+    const int64_t n = tile_count(a, tile_shape(a, bf16 ? 2 : 4, false));
     most = n > most ? n : most;
   }
   return 2 * most * groups;
@@ -997,7 +1072,8 @@ int64_t fmd_group_norm_bwd_work_size(int32_t bf16, int64_t rows, int32_t channel
   for (int v = 1; v <= 8; v *= 2) {
     a.x_ld = channels % v == 0 ? v : 1;
     const BackSpace s = back_space(a, bf16 ? 2 : 4);
-    most = s.part + s.means + s.sums > most ? s.part + s.means + s.sums : most;
+    const int64_t size = s.columns + s.part + s.means + s.sums;
+    most = size > most ? size : most;
   }
   return most;
 }

@@ -4,32 +4,126 @@
 
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float value_of(const void* x, int64_t i) {
-  return (float)static_cast<const T*>(x)[i];
-}
-
 // x / scale to the nearest integer; 0 where there is none (scale 0, or not finite: the product is then 0 or NaN by its scale)
 __device__ __forceinline__ int8_t to_int8(float x, float scale) {
   const float q = rintf(x / scale);
   return (int8_t)(scale == 0.f || !(fabsf(q) < INFINITY) ? 0.f : fminf(fmaxf(q, -127.f), 127.f));
 }
 
-// One workgroup a row, which it reads twice (the second time from the cache).
+struct Eight {
+  float v[8];
+};
+
+__device__ __forceinline__ Eight load8(const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  return {{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ Eight load8(const __bf16* p) {
+  const fmd_bf16x8 x = *reinterpret_cast<const fmd_bf16x8*>(p);
+  Eight r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r.v[e] = (float)x[e];
+  return r;
+}
+
+struct RowArgs {
+  const void* x;
+  int64_t x_ld, width, rows;
+  int8_t* q;
+  int64_t q_ld;  // a multiple of 8
+  float* scales;
+  int32_t wide;  // rows in whole 16-byte vectors
+  int64_t row0;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, int64_t x_ld, int64_t width, int8_t* q, int64_t q_ld,
-                                                            float* scales, int64_t row0) {
+__device__ __forceinline__ Eight row_part(const RowArgs& a, const T* src, int64_t k) {
+  if (a.wide && k + 8 <= a.width) return load8(src + k);
+  Eight r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r.v[e] = k + e < a.width ? (float)src[k + e] : 0.f;
+  return r;
+}
+
+__device__ __forceinline__ void put_part(int8_t* q, const Eight& x, float scale) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e / 4] |= (uint32_t)(uint8_t)to_int8(x.v[e], scale) << (8 * (e % 4));
+  *reinterpret_cast<uint2*>(q) = make_uint2(w[0], w[1]);
+}
+
+// A wave or (LANES 256) a workgroup a row, in registers: NV vectors of eight a lane; NV 0: read twice, whatever its width. 8 192 rows
+// of 4 096, bf16: 71 us with a value at a time, 26 so (3.9 TB/s).
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(RowArgs a) {
   __shared__ float lds[4];
-  const int64_t row = row0 + blockIdx.x;
-  const T* src = static_cast<const T*>(x) + row * x_ld;
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = a.row0 + (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const bool live = row < a.rows;
+  const T* src = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_ld;
+  Eight x[NV > 0 ? NV : 1];
   float top = 0.f;
-  for (int64_t k = threadIdx.x; k < width; k += 256) top = nan_max(top, fabsf((float)src[k]));
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) x[n] = row_part<T>(a, src, (int64_t)(lane + n * LANES) * 8);
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = nan_max(top, fabsf(x[n].v[e]));
+  } else {
+    for (int64_t k = lane * 8; k < a.width; k += LANES * 8) {
+      x[0] = row_part<T>(a, src, k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = nan_max(top, fabsf(x[0].v[e]));
+    }
+  }
   top = wave_nan_max(top);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
-  __syncthreads();
-  const float scale = nan_max(nan_max(lds[0], lds[1]), nan_max(lds[2], lds[3])) * (1.f / 127.f);
-  if (threadIdx.x == 0) scales[row] = scale;
-  for (int64_t k = threadIdx.x; k < q_ld; k += 256) q[row * q_ld + k] = k < width ? to_int8((float)src[k], scale) : 0;
+  if (LANES > 64) {
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = nan_max(nan_max(lds[0], lds[1]), nan_max(lds[2], lds[3]));
+  }
+  if (!live) return;
+  const float scale = top * (1.f / 127.f);
+  if (lane == 0) a.scales[row] = scale;
+  int8_t* q = a.q + row * a.q_ld;
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int64_t k = (int64_t)(lane + n * LANES) * 8;
+      if (k < a.q_ld) put_part(q + k, x[n], scale);
+    }
+  } else {
+    for (int64_t k = lane * 8; k < a.q_ld; k += LANES * 8) put_part(q + k, row_part<T>(a, src, k), scale);
+  }
+}
+
+template <typename T>
+int quantize(RowArgs a, hipStream_t stream) {
+  a.wide = a.x_ld * sizeof(T) % 16 == 0 && (reinterpret_cast<uintptr_t>(a.x) & 15) == 0;
+  const int64_t vectors = fmd_cdiv(a.q_ld, 8);
+  const int each = vectors <= 128 ? 4 : 1;  // rows of a workgroup
+  constexpr int64_t most = 1 << 22;
+  for (a.row0 = 0; a.row0 < a.rows; a.row0 += most * each) {
+    const int64_t left = fmd_cdiv(a.rows - a.row0, each);
+    const unsigned blocks = (unsigned)(left < most ? left : most);
+#define QUANTIZE(LANES, NV) quantize_rows_kernel<T, LANES, NV><<<blocks, 256, 0, stream>>>(a)
+    if (vectors <= 64)
+      QUANTIZE(64, 1);
+    else if (vectors <= 128)
+      QUANTIZE(64, 2);
+    else if (vectors <= 256)
+      QUANTIZE(256, 1);
+    else if (vectors <= 512)
+      QUANTIZE(256, 2);
+    else if (vectors <= 1024)
+      QUANTIZE(256, 4);
+    else
+      QUANTIZE(256, 0);
+#undef QUANTIZE
+    FMD_CHECK_LAUNCH();
+  }
+  return FMD_OK;
 }
 
 struct ScaleEpi {
@@ -109,17 +203,10 @@ extern "C" {
 
 int fmd_quantize_rows(int32_t bf16, const void* x, int64_t x_ld, int64_t rows, int64_t width, int8_t* values, int64_t values_ld,
                       float* scales, hipStream_t stream) {
-  FMD_REQUIRE(rows >= 0 && width >= 1 && values_ld >= width && (rows == 0 || (x && values && scales)));
-  constexpr int64_t most = 1 << 22;
-  for (int64_t r = 0; r < rows; r += most) {
-    const unsigned blocks = (unsigned)(rows - r < most ? rows - r : most);
-    if (bf16)
-      quantize_rows_kernel<__bf16><<<blocks, 256, 0, stream>>>(x, x_ld, width, values, values_ld, scales, r);
-    else
-      quantize_rows_kernel<float><<<blocks, 256, 0, stream>>>(x, x_ld, width, values, values_ld, scales, r);
-    FMD_CHECK_LAUNCH();
-  }
-  return FMD_OK;
+  FMD_REQUIRE(rows >= 0 && width >= 1 && values_ld >= width && values_ld % 8 == 0 && (reinterpret_cast<uintptr_t>(values) & 7) == 0 &&
+              (rows == 0 || (x && values && scales)));
+  const RowArgs a{x, x_ld, width, rows, values, values_ld, scales, 0, 0};
+  return bf16 ? quantize<__bf16>(a, stream) : quantize<float>(a, stream);
 }
 
 int64_t fmd_linear_int8_work_size(int64_t rows, int64_t width, int64_t out) {

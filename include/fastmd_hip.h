@@ -933,7 +933,7 @@ int fmd_group_norm_bwd(int32_t bf16, int32_t act, const void* gy, int64_t gy_ld,
 
 /* Rows of x [rows, width] (row stride x_ld) as 8-bit integers: scale = max |x| (1 / 127) of the row, value = x / scale rounded to the
  * nearest (ties to even), both in float32, at most 127 in size; a row of zeros has scale 0, a value that is not finite leaves a
- * scale that is not. values [rows, values_ld] (values_ld at least width, the rest zero), scales [rows]. */
+ * scale that is not. values [rows, values_ld] (values_ld at least width, a multiple of 8, the rest zero; 8-byte aligned), scales [rows]. */
 int fmd_quantize_rows(int32_t bf16, const void* x, int64_t x_ld, int64_t rows, int64_t width, int8_t* values, int64_t values_ld,
                       float* scales, hipStream_t stream);
 
