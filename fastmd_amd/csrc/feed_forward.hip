@@ -101,7 +101,9 @@ struct GatedEpi {
   float *gate, *up;  // nullable
   int64_t rows, hidden, ld, plane;
   int32_t act, planes;
-  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, float4 g, float4 u) const {
+  typedef TpNothing Fetch;
+  __device__ __forceinline__ Fetch fetch(int64_t, int64_t) const { return {}; }
+  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, float4 g, float4 u, Fetch) const {
     if (m >= rows || n >= ld) return;
     const float gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
     float v[4];
@@ -109,8 +111,8 @@ struct GatedEpi {
     for (int e = 0; e < 4; ++e) v[e] = n + e < hidden ? activation(gv[e], act).value * uv[e] : 0.f;
     put_operand(h + m * ld + n, plane, planes, v);
     if (gate) {
-      *reinterpret_cast<float4*>(gate + m * ld + n) = g;
-      *reinterpret_cast<float4*>(up + m * ld + n) = u;
+      store_stream(reinterpret_cast<float4*>(gate + m * ld + n), g);
+      store_stream(reinterpret_cast<float4*>(up + m * ld + n), u);
     }
   }
 };
@@ -121,9 +123,16 @@ struct GatedBackEpi {
   const float *gate, *up;
   int64_t rows, hidden, ld, plane;
   int32_t act, planes;
-  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, float4 gh, float4) const {
+  struct Fetch {
+    float4 g, u;
+  };
+  __device__ __forceinline__ Fetch fetch(int64_t m, int64_t n) const {
+    const int64_t at = (m < rows ? m : rows - 1) * ld + (n < ld ? n : ld - 4);
+    return {*reinterpret_cast<const float4*>(gate + at), *reinterpret_cast<const float4*>(up + at)};
+  }
+  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, float4 gh, float4, const Fetch& f) const {
     if (m >= rows || n >= ld) return;
-    const float4 g = *reinterpret_cast<const float4*>(gate + m * ld + n), u = *reinterpret_cast<const float4*>(up + m * ld + n);
+    const float4 g = f.g, u = f.u;
     const float hv[4] = {gh.x, gh.y, gh.z, gh.w}, gv[4] = {g.x, g.y, g.z, g.w}, uv[4] = {u.x, u.y, u.z, u.w};
     float dg[4], du[4];
 #pragma unroll
@@ -143,7 +152,9 @@ struct StoreEpi {
   void* out[kTpProblems];
   int64_t rows_m[kTpProblems], rows_n[kTpProblems];
   int32_t bf16;
-  __device__ __forceinline__ void operator()(int i, int64_t m, int64_t n, float4 v, float4) const {
+  typedef TpNothing Fetch;
+  __device__ __forceinline__ Fetch fetch(int64_t, int64_t) const { return {}; }
+  __device__ __forceinline__ void operator()(int i, int64_t m, int64_t n, float4 v, float4, Fetch) const {
     const int64_t width = i == 0 ? rows_n[0] : i == 1 ? rows_n[1] : rows_n[2];
     if (m >= (i == 0 ? rows_m[0] : i == 1 ? rows_m[1] : rows_m[2]) || n >= width) return;
     void* o = i == 0 ? out[0] : i == 1 ? out[1] : out[2];
@@ -189,21 +200,27 @@ int64_t count_tiles(TpArgs& a) {
   return tiles;
 }
 
-// The tile: 256 x 256 where these fill the card once, 128 x 128 where those fill half of it, 64 x 64 otherwise.
+// The tile and the split of K with the least time (tp_plan).
 template <typename Sh, typename Fn>
-int with_shape(TpArgs& a, const Fn& fn) {
+int with_shape(TpArgs& a, float heavy, const Fn& fn) {
   int64_t slices = 0;
   for (int i = 0; i < a.count; ++i) {
-    const int64_t s = fmd_cdiv(a.p[i].k, 64) * a.p[i].parts * (a.p[i].planes == 3 ? 6 : 1);
+    const int64_t s = fmd_cdiv(2 * a.p[i].k, kTpSlice) * a.p[i].parts * (a.p[i].planes == 3 ? 6 : 1);
     slices = i == 0 || s < slices ? s : slices;
   }
   int64_t tiles = count_tiles<typename Sh::Large>(a);
   if (tiles > kTpMostTiles) return FMD_EINVAL;
-  if (tiles >= 192) return fn(typename Sh::Large{}, tp_plan<typename Sh::Large>(tiles, slices));
-  tiles = count_tiles<typename Sh::Middle>(a);
-  if (tiles >= 256) return fn(typename Sh::Middle{}, tp_plan<typename Sh::Middle>(tiles, slices));
-  tiles = count_tiles<typename Sh::Small>(a);
-  return fn(typename Sh::Small{}, tp_plan<typename Sh::Small>(tiles, slices));
+  const TpPlan large = tp_plan<typename Sh::Large>(tiles, slices, heavy);
+  if (tiles >= 1024) return fn(typename Sh::Large{}, large);
+  const TpPlan middle = tp_plan<typename Sh::Middle>(count_tiles<typename Sh::Middle>(a), slices, heavy);
+  const TpPlan small = tp_plan<typename Sh::Small>(count_tiles<typename Sh::Small>(a), slices, heavy);
+  if (small.time < middle.time && small.time < large.time) return fn(typename Sh::Small{}, small);
+  if (middle.time < large.time) {
+    count_tiles<typename Sh::Middle>(a);
+    return fn(typename Sh::Middle{}, middle);
+  }
+  count_tiles<typename Sh::Large>(a);
+  return fn(typename Sh::Large{}, large);
 }
 
 int64_t up8(int64_t x) { return (x + 7) & ~int64_t(7); }
@@ -269,7 +286,7 @@ bool direct(const void* p, int64_t ld, int64_t cols) {
 // A launch of one kind of product: its partial sums' size, or the launch itself
 template <typename Sh, typename Epi>
 int product(TpArgs& a, Space& s, bool run, const Epi& epi, hipStream_t stream) {
-  return with_shape<Sh>(a, [&](auto shape, const TpPlan& plan) {
+  return with_shape<Sh>(a, sizeof(typename Epi::Fetch) > 16 ? 3.f : 1.f, [&](auto shape, const TpPlan& plan) {
     typedef decltype(shape) S;
     const int64_t before = s.used;
     void* partial = s.take(plan.partial);

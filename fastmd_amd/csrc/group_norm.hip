@@ -24,9 +24,6 @@ constexpr int kTileValues = 64;  // of a thread's registers
 #ifndef NRBACK
 #define NRBACK 1
 #endif
-#ifndef MERGE
-#define MERGE 16
-#endif
 constexpr int64_t kFewTiles = FEW;
 
 struct GnArgs {
@@ -40,6 +37,7 @@ struct GnArgs {
   void *y, *gx;          // contiguous
   float *mean, *inverse;  // [rows or segments, groups]
   float *part;           // scratch (see the kernels)
+  int32_t merge;         // whether gn_merge_kernel merges the sums of segments of many tiles
   int32_t chunk;         // channels of a workgroup's share (whole groups)
   int32_t tile_rows, tx;  // rows of a tile, vectors of a row of the share
   int32_t lanes;         // rows by themselves: lanes of a group
@@ -496,10 +494,13 @@ __global__ void __launch_bounds__(kThreads) gn_tile_kernel(GnArgs a) {
   write_norm<T, V, NV, NR>(a, p, x, y, rows, mean, inverse);
 }
 
-// Where a segment has more tiles than this, their sums are merged once, by gn_merge_kernel, not by each of the workgroups.
-constexpr int kMergeTiles = MERGE;
+// Each workgroup of the second read merges the sums of its segment's tiles itself where all tiles' together are few (kMergeValues);
+// otherwise those of a segment of more than kMergeTiles tiles are merged once, by gn_merge_kernel: 33 tiles of 8 groups each 48 us with
+// a launch for it, 41 without (16 875 rows of 128, float32, with VJP); 85 tiles of 32 groups 80 us by each workgroup, 38 by the launch.
+constexpr int kMergeTiles = 16;
+constexpr int64_t kMergeValues = 8192;
 
-__device__ __forceinline__ bool merged_apart(const GnArgs& a, int64_t rows) { return rows > (int64_t)kMergeTiles * a.tile_rows; }
+__device__ __forceinline__ bool merged_apart(const GnArgs& a, int64_t rows) { return a.merge && rows > (int64_t)kMergeTiles * a.tile_rows; }
 
 struct GnStats {
   float x, y;
@@ -885,6 +886,7 @@ void set_tiles(GnArgs& a, const TileShape& s) {
   a.chunk = s.chunk;
   a.tx = s.tx;
   a.tile_rows = s.rows;
+  a.merge = a.rows / s.rows * a.groups > kMergeValues && a.rows > (int64_t)kMergeTiles * s.rows;
 }
 
 template <typename T>
@@ -910,7 +912,7 @@ int norm(GnArgs a, hipStream_t stream) {
       gn_tile_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a);
     });
     if (status || a.rows <= s.rows) return status;  // no segment is longer than a tile
-    if (a.rows > kMergeTiles * s.rows) {
+    if (a.merge) {
       const int64_t numbers = a.rows / (kMergeTiles * s.rows);
       const int by_number = numbers < a.segments;
       status = in_launches(a, by_number ? numbers : a.segments, [&](unsigned blocks) {
@@ -993,7 +995,7 @@ int norm_bwd(GnArgs a, float* work, void* gw, void* gb, hipStream_t stream) {
       gn_tile_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, s.lds, stream>>>(a, part);
     });
     if (status || a.rows <= s.rows) return status;
-    if (a.rows > kMergeTiles * s.rows) {
+    if (a.merge) {
       const int64_t numbers = a.rows / (kMergeTiles * s.rows);
       const int by_number = numbers < a.segments;
       status = in_launches(a, by_number ? numbers : a.segments, [&](unsigned blocks) {

@@ -131,7 +131,9 @@ struct ScaleEpi {
   const float *row_scale, *col_scale, *bias;
   int64_t rows, cols;
   int32_t bf16;
-  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, int4 v, int4) const {
+  typedef TpNothing Fetch;
+  __device__ __forceinline__ Fetch fetch(int64_t, int64_t) const { return {}; }
+  __device__ __forceinline__ void operator()(int, int64_t m, int64_t n, int4 v, int4, Fetch) const {
     if (m >= rows || n >= cols) return;
     const float s = row_scale[m];
     const int e[4] = {v.x, v.y, v.z, v.w};
@@ -173,13 +175,19 @@ typedef TpShape<TpInt8, 1, 2, 2, 1, false, false, false, 2> Small;
 template <typename Fn>
 int with_shape(TpArgs& a, const Fn& fn) {
   const int64_t slices = fmd_cdiv(a.p[0].k, kTpSlice);
-  int64_t tiles = tp_tiles<Large>(a.p[0], 0);
+  const int64_t tiles = tp_tiles<Large>(a.p[0], 0);
   if (tiles > kTpMostTiles) return FMD_EINVAL;
-  if (tiles >= 192) return fn(Large{}, tp_plan<Large>(tiles, slices));
-  tiles = tp_tiles<Middle>(a.p[0], 0);
-  if (tiles >= 256) return fn(Middle{}, tp_plan<Middle>(tiles, slices));
-  tiles = tp_tiles<Small>(a.p[0], 0);
-  return fn(Small{}, tp_plan<Small>(tiles, slices));
+  const TpPlan large = tp_plan<Large>(tiles, slices, 1.f);
+  if (tiles >= 1024) return fn(Large{}, large);
+  const TpPlan middle = tp_plan<Middle>(tp_tiles<Middle>(a.p[0], 0), slices, 1.f);
+  const TpPlan small = tp_plan<Small>(tp_tiles<Small>(a.p[0], 0), slices, 1.f);
+  if (small.time < middle.time && small.time < large.time) return fn(Small{}, small);
+  if (middle.time < large.time) {
+    tp_tiles<Middle>(a.p[0], 0);
+    return fn(Middle{}, middle);
+  }
+  tp_tiles<Large>(a.p[0], 0);
+  return fn(Large{}, large);
 }
 
 TpArgs arguments(const int8_t* x, int64_t x_ld, const int8_t* w, int64_t w_ld, int64_t rows, int64_t width, int64_t out) {

@@ -1,8 +1,8 @@
 // Products out[m, n] = sum_k n_op[n, k] m_op[m, k] on the matrix cores, with the result's own use as an epilogue: what the
 // gated feed-forward block and the 8-bit product are made of.
 //
-// Both operands of a slice of K are copied straight from global memory into LDS (no register stage), two slices in turn: while
-// the matrix instructions run on one, the next one lands. An operand is stored along K (its rows are rows of the product, K
+// Both operands of a slice of K are copied straight from global memory into LDS (no register stage), into four places in turn: while
+// the matrix instructions run on one slice, three are on their way. An operand is stored along K (its rows are rows of the product, K
 // contiguous) or across it (its rows are K, as a weight is in the products of the backward pass); the second kind is
 // transposed by the LDS reads (ds_read_b64_tr_b16), never in memory. The n operand is the matrix instruction's first: a
 // lane's four consecutive results then lie side by side in a row of the output.
@@ -43,10 +43,9 @@ struct TpArgs {
   void* partial;
 };
 
-__device__ __attribute__((aligned(16))) const uint32_t g_tp_zero_chunk[4] = {0, 0, 0, 0};
+typedef uint32_t tp_u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTpVm0 = 0 | (7 << 4) | (15 << 8);        // s_waitcnt vmcnt(0)
-constexpr int kTpVm0Lgkm0 = 0 | (7 << 4) | (0 << 8);    // s_waitcnt vmcnt(0) lgkmcnt(0)
+constexpr int tp_wait(int vm, int lgkm) { return (vm & 15) | (7 << 4) | (lgkm << 8); }  // s_waitcnt vmcnt(vm) lgkmcnt(lgkm)
 
 struct TpBf16 {
   typedef fmd_f32x16 Acc;
@@ -64,9 +63,11 @@ struct TpInt8 {
 };
 
 // One operand's rows in LDS: ROWS rows of the product, SLICE bytes of K each (along), or SLICE / 2 rows of K (across). 16-byte
-// chunks are permuted so that neither kind of read meets a bank twice: sixteen consecutive rows' same chunk (along; both on
-// the 64 banks and, for eight rows, on any 32), or four chunks of four consecutive rows of K (across).
-constexpr int kTpSlice = 128;  // bytes of K in a slice (64 bf16 values, 128 8-bit ones)
+// chunks are permuted so that neither kind of read meets one of the 64 banks twice: sixteen consecutive rows' same chunk (along), or
+// four chunks of four consecutive rows of K (across).
+constexpr int kTpSlice = 128;  // bytes of K in a slice
+constexpr int kTpSteps = kTpSlice / 32, kTpRow = kTpSlice / 16;  // steps of the matrix instructions, chunks of a row
+constexpr int kTpPlaces = 256 / kTpSlice;
 
 template <int ROWS, bool ACROSS_, bool GATED, int THREADS>
 struct TpStage {
@@ -76,16 +77,18 @@ struct TpStage {
   static_assert(BYTES % (16 * THREADS) == 0, "whole passes");
   static_assert(!(ACROSS && GATED), "a gated product's weights lie along K");
 
-  __device__ static __forceinline__ int swap_along(int row) { return (row & 7) ^ ((row >> 3) & 1); }
+  __device__ static __forceinline__ int swap_along(int row) { return kTpRow == 4 ? (row >> 2) & 3 : (row & 7) ^ ((row >> 3) & 1); }
   __device__ static __forceinline__ int swap_across(int row) { return CHUNKS >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
 
   uint32_t off[LOADS];
+  int k;  // bytes of K before this lane's (of its first copy)
   const char* at[GATED ? 2 : 1];
   int64_t step;
 
   // this thread's offsets for the tile whose first row is `row0` (below `rows`)
   __device__ __forceinline__ void place(const TpOperand& o, int64_t row0, int64_t rows, int wave, int lane) {
     step = ACROSS ? (kTpSlice / 2) * o.ld : kTpSlice;
+    k = ACROSS ? lane / CHUNKS * 2 : ((lane % kTpRow) ^ swap_along(lane / kTpRow)) * 16;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
       const int slot = (wave * LOADS + j) * 64 + lane;
@@ -94,8 +97,8 @@ struct TpStage {
         const int64_t last = ((rows + 7) & ~int64_t(7)) - 8 - row0;  // chunks past the rows: the last one again, never used
         off[j] = (uint32_t)(row * o.ld) + 2 * (uint32_t)(chunk * 8 < last ? chunk * 8 : last);
       } else {
-        int row = slot / 8;
-        const int chunk = (slot % 8) ^ swap_along(row);
+        int row = slot / kTpRow;
+        const int chunk = (slot % kTpRow) ^ swap_along(row);
         if (GATED && row >= ROWS / 2) row -= ROWS / 2;
         const int64_t last = rows - 1 - row0;
         off[j] = (uint32_t)((row < last ? row : last) * o.ld) + 16 * chunk;
@@ -114,30 +117,21 @@ struct TpStage {
     }
   }
 
-  // 64 lanes' 16 bytes at base + off (or at p) to LDS from `to` on. As instructions: after the compiler's own form every read of
-  // LDS waits for all copies, those of the other place too. tile_product_kernel holds the waits.
-  __device__ static __forceinline__ void copy16(const char* base, uint32_t off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(off), "s"(base) : "memory", "m0");
+  // Copy j of the slice at `at` to LDS, 64 lanes' 16 bytes; of K `left` bytes are left, past them is zero (an offset past the
+  // buffer's end). As an instruction: after the compiler's own form every read of LDS waits for all copies, those to other places
+  // too. tile_product_kernel holds the waits.
+  __device__ __forceinline__ void copy(uint32_t lds, int j, int left, int wave) const {
+    const int n = wave * LOADS + j;
+    const char* base = GATED && n * (64 / kTpRow) >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0];
+    const tp_u32x4 buffer = {(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32) & 0xffff, 0x80000000u, 0x00027000u};
+    const int mine = ACROSS ? k : kTpRow == 8 ? k ^ (16 * (n & 1)) : k, rest = ACROSS ? left - n * (64 / CHUNKS) * 2 : left;
+    const uint32_t from = mine < rest ? off[j] : 0xffffffffu;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds + n * 1024), "v"(from), "s"(buffer)
+                 : "memory", "m0");
   }
-  __device__ static __forceinline__ void copy16(const char* p, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(to), "v"(p) : "memory", "m0");
-  }
-
-  // the slice at `at` into LDS; `left`: bytes of K from it on, past them is zero
-  __device__ __forceinline__ void issue(uint32_t lds, int64_t left, int wave, int lane) {
-    if (left >= kTpSlice) {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j)
-        copy16(GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0], off[j], lds + (wave * LOADS + j) * 1024);
-    } else {
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        const char* p = (GATED && (wave * LOADS + j) * 8 >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0]) + off[j];
-        const int slot = (wave * LOADS + j) * 64 + lane;
-        const int k = ACROSS ? slot / CHUNKS * 2 : ((slot % 8) ^ swap_along(slot / 8)) * 16;
-        copy16(k < left ? p : reinterpret_cast<const char*>(g_tp_zero_chunk), lds + (wave * LOADS + j) * 1024);
-      }
-    }
+  __device__ __forceinline__ void advance() {
 #pragma unroll
     for (int g = 0; g < (GATED ? 2 : 1); ++g) at[g] += step;
   }
@@ -153,7 +147,7 @@ struct TpStage {
     return row * kTpSlice + ((h ^ swap_along(row)) << 4);
   }
 
-  // operand of the 32 rows from `row` (a multiple of 32) over step kk of four: 16 bytes, from K 32 kk + 16 (lane / 32) bytes
+  // operand of the 32 rows from `row` (a multiple of 32) over step kk of a slice: 16 bytes, from K 32 kk + 16 (lane / 32) bytes
   __device__ static __forceinline__ tp_i32x4 read(const char* lds, int at, int row, int kk) {
     if (ACROSS) {
       typedef __attribute__((address_space(3))) tp_s16x4* lds_ptr;
@@ -195,6 +189,9 @@ __device__ __forceinline__ Four tp_sum(const Four* x, int64_t step, int splits) 
   return s;
 }
 
+// of an epilogue that reads nothing more
+struct TpNothing {};
+
 struct TpTile {
   int32_t problem, tn, tm;
 };
@@ -220,8 +217,7 @@ tile_product_kernel(TpArgs a, Epi epi) {
   typedef typename S::Type T;
   typedef typename T::Acc Acc;
   constexpr int NB = S::NB, MB = S::MB;
-  __shared__ __attribute__((aligned(1024))) char st0[S::STAGE];
-  __shared__ __attribute__((aligned(1024))) char st1[S::STAGE];
+  __shared__ __attribute__((aligned(1024))) char lds[kTpPlaces * S::STAGE];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wn = wave / S::WM, wm = wave % S::WM;
   int tile, split = 0, splits = 1;
@@ -240,7 +236,7 @@ tile_product_kernel(TpArgs a, Epi epi) {
   // slices of K of all passes (parts, planes), and those of this workgroup
   const int64_t k_bytes = p.k * T::SIZE;
   const int nk = (int)((k_bytes + kTpSlice - 1) / kTpSlice), passes = p.parts * (p.planes == 3 ? 6 : 1);
-  const int total = nk * passes;
+  const int total = nk * passes;  // at least one: K is not empty
   const int begin = (int)((int64_t)total * split / splits), end = (int)((int64_t)total * (split + 1) / splits);
 
   typename S::StageN sn;
@@ -254,27 +250,38 @@ tile_product_kernel(TpArgs a, Epi epi) {
     sn.begin(p.n, part, (0x124 >> (2 * pair)) & 3, n0, ks);
     sm.begin(p.m, part, (0x046 >> (2 * pair)) & 3, m0, ks);
   };
-  auto issue = [&](const char* place) {
+  int next = begin;  // slice to copy; past the end zeros, so that every wait counts the same copies
+  constexpr int COPIES = S::StageN::LOADS + S::StageM::LOADS;
+  auto left = [&]() {
+    const int64_t l = k_bytes - (int64_t)ks * kTpSlice;
+    return next < end ? (int)(l < kTpSlice ? l : kTpSlice) : 0;
+  };
+  auto copy_one = [&](const char* place, int j, int left) {
     const uint32_t st = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)place;
-    const int64_t left = k_bytes - (int64_t)ks * kTpSlice;
-    sn.issue(st, left, wave, lane);
-    sm.issue(st + S::StageN::BYTES, left, wave, lane);
+    if (j < S::StageN::LOADS)
+      sn.copy(st, j, left, wave);
+    else
+      sm.copy(st + S::StageN::BYTES, j - S::StageN::LOADS, left, wave);
+  };
+  auto copied = [&]() {
+    sn.advance();
+    sm.advance();
+    ++next;
     if (++ks == nk) {
       ks = 0;
       ++pass;
-      if (pass < passes) open();
+      if (next < end) open();
     }
   };
   const int ln = S::StageN::lane_at(lane), lm = S::StageM::lane_at(lane);
   tp_i32x4 fn[2][NB], fm[2][MB];
-  constexpr int READS = (S::StageN::ACROSS ? 2 : 1) * NB + (S::StageM::ACROSS ? 2 : 1) * MB;
-  auto read = [&](const char* st, int kk, int to) {
-    // in the order in which the products take them
-    fn[to][0] = S::StageN::read(st, ln, S::block_n(0, wn), kk);
-#pragma unroll
-    for (int j = 0; j < MB; ++j) fm[to][j] = S::StageM::read(st + S::StageN::BYTES, lm, (wm * MB + j) * 32, kk);
-#pragma unroll
-    for (int i = 1; i < NB; ++i) fn[to][i] = S::StageN::read(st, ln, S::block_n(i, wn), kk);
+  // the reads of a step, in the order in which the products take them
+  constexpr int READS = NB + MB;
+  auto read_one = [&](const char* st, int kk, int to, int i) {
+    if (i >= 1 && i <= MB)
+      fm[to][i - 1] = S::StageM::read(st + S::StageN::BYTES, lm, (wm * MB + i - 1) * 32, kk);
+    else
+      fn[to][i ? i - MB : 0] = S::StageN::read(st, ln, S::block_n(i ? i - MB : 0, wn), kk);
   };
   Acc acc[NB][MB];
 #pragma unroll
@@ -284,51 +291,54 @@ tile_product_kernel(TpArgs a, Epi epi) {
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0;
 
-  if (begin < end) {
-    open();
-    issue(st0);
-    if (begin + 1 < end) issue(st1);
-    // A slice is four steps. The operands of a step are read while the one before runs; before the last step every wave has
-    // read the whole slice, so its place takes the slice after the next.
-    auto step = [&](int kk) {
+  // A step's products with the next step's reads, and copies, between them, held in this order.
+  constexpr int SLOTS = NB * MB;
+  auto step = [&](int kk, const char* st, int next_kk, bool copies, const char* place) {
+    const int from = kk & 1, to = from ^ 1, rest = copies ? left() : 0;
 #pragma unroll
-      for (int i = 0; i < NB; ++i)
+    for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int j = 0; j < MB; ++j) acc[i][j] = T::mma(fn[kk & 1][i], fm[kk & 1][j], acc[i][j]);
-      // a read after each of the first products
+      for (int j = 0; j < MB; ++j) {
+        const int slot = i * MB + j;
+        acc[i][j] = T::mma(fn[from][i], fm[from][j], acc[i][j]);
 #pragma unroll
-      for (int i = 0; i < NB * MB; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, (READS + NB * MB - 1) / (NB * MB), 0);
+        for (int r = 0; r < READS; ++r)
+          if (r * SLOTS / READS == slot) read_one(st, next_kk, to, r);
+        if (copies)
+#pragma unroll
+          for (int c = 0; c < COPIES; ++c)
+            if (c * SLOTS / COPIES == slot) copy_one(place, c, rest);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    };
-    auto slice = [&](char* st, char* next, int s) {
+  };
+  // A slice is kTpSteps steps. The operands of a step are read while the one before runs; before the last step every wave has
+  // read the whole slice, so its place takes the slice that is kTpPlaces further.
+  static_assert((kTpPlaces - 1) * COPIES < 16, "in the low bits of the count");
+  auto slice = [&](char* st, char* following) {
 #pragma unroll
-      for (int kk = 0; kk < 3; ++kk) {
-        read(st, kk + 1, (kk + 1) & 1);
-        step(kk);
-      }
-      if (s + 1 < end) {
-        __builtin_amdgcn_s_waitcnt(kTpVm0Lgkm0);
-        __builtin_amdgcn_s_barrier();
-        if (s + 2 < end) issue(st);
-        read(next, 0, 0);
-      }
-      step(3);
-    };
-    if (begin + 1 < end)
-      __builtin_amdgcn_s_waitcnt(((S::StageN::LOADS + S::StageM::LOADS) & 15) | (7 << 4) | (15 << 8));
-    else
-      __builtin_amdgcn_s_waitcnt(kTpVm0);
+    for (int kk = 0; kk + 1 < kTpSteps; ++kk) step(kk, st, kk + 1, false, nullptr);
+    __builtin_amdgcn_s_waitcnt(tp_wait((kTpPlaces - 2) * COPIES, 0));  // of the slices on their way the first has landed
     __builtin_amdgcn_s_barrier();
-    read(st0, 0, 0);
-    int s = begin;
-    for (; s + 1 < end; s += 2) {
-      slice(st0, st1, s);
-      slice(st1, st0, s + 1);
-    }
-    if (s < end) slice(st0, st1, s);
+    step(kTpSteps - 1, following, 0, true, st);
+    copied();
+  };
+  open();
+#pragma unroll
+  for (int i = 0; i < kTpPlaces; ++i) {
+    const int rest = left();
+#pragma unroll
+    for (int j = 0; j < COPIES; ++j) copy_one(lds + i * S::STAGE, j, rest);
+    copied();
   }
+  __builtin_amdgcn_s_waitcnt(tp_wait((kTpPlaces - 1) * COPIES, 15));
+  __builtin_amdgcn_s_barrier();
+#pragma unroll
+  for (int r = 0; r < READS; ++r) read_one(lds, 0, 0, r);
+  for (int s = begin; s < end; s += kTpPlaces)
+#pragma unroll
+    for (int i = 0; i < kTpPlaces; ++i)
+      if (s + i < end) slice(lds + i * S::STAGE, lds + (i + 1) % kTpPlaces * S::STAGE);
+  __builtin_amdgcn_s_waitcnt(tp_wait(0, 0));  // no copy outlives the loop
 
   // a lane's results: row m0 + wm 32 MB + 32 j + lane % 32, four columns from n0 + block + 8 q + 4 (lane / 32)
   if (splits > 1) {
@@ -348,9 +358,9 @@ tile_product_kernel(TpArgs a, Epi epi) {
   // once. Chunks of four are permuted by the row: neither the writes (a column of sixteen rows) nor the reads meet a bank twice.
   typedef decltype(tp_four(acc[0][0], 0)) Four;
   constexpr int CHUNKS = NB * 8, REGION = 32 * CHUNKS * 16, EACH = S::GATED ? CHUNKS / 2 : CHUNKS;
-  static_assert(REGION * S::THREADS / 64 <= 2 * S::STAGE, "a place for each wave");
+  static_assert(REGION * S::THREADS / 64 <= kTpPlaces * S::STAGE, "a place for each wave");
   __syncthreads();
-  char* mine = wave * REGION < S::STAGE ? st0 + wave * REGION : st1 + (wave * REGION - S::STAGE);
+  char* mine = lds + wave * REGION;
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
     const int r = lane & 31;
@@ -359,13 +369,26 @@ tile_product_kernel(TpArgs a, Epi epi) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<Four*>(mine + (r * CHUNKS + ((i * 8 + 2 * q + (lane >> 5)) ^ (r & (CHUNKS - 1)))) * 16) = tp_four(acc[i][j], q);
-#pragma unroll 2
-    for (int k = lane; k < 32 * EACH; k += 64) {
-      const int row = k / EACH, c = k % EACH;
-      const Four* x = reinterpret_cast<const Four*>(mine) + row * CHUNKS;
-      const Four v = x[c ^ (row & (CHUNKS - 1))], u = S::GATED ? x[(c + CHUNKS / 2) ^ (row & (CHUNKS - 1))] : v;
-      const int half = c / (CHUNKS / 2);
-      epi(tt.problem, m0 + (wm * MB + j) * 32 + row, n0 + half * (S::BN / 2) + wn * (NB * 16) + (c - half * (CHUNKS / 2)) * 4, v, u);
+    // what the epilogue reads of memory is asked for some rows ahead of its results
+    constexpr int AHEAD = S::BN >= 256 && sizeof(typename Epi::Fetch) > 16 ? 2 : 4;
+    static_assert(32 * EACH % (64 * AHEAD) == 0, "whole groups");
+    for (int k0 = lane; k0 < 32 * EACH; k0 += 64 * AHEAD) {
+      int64_t m[AHEAD], n[AHEAD];
+      typename Epi::Fetch fetched[AHEAD];
+#pragma unroll
+      for (int g = 0; g < AHEAD; ++g) {
+        const int k = k0 + 64 * g, row = k / EACH, c = k % EACH, half = c / (CHUNKS / 2);
+        m[g] = m0 + (wm * MB + j) * 32 + row;
+        n[g] = n0 + half * (S::BN / 2) + wn * (NB * 16) + (c - half * (CHUNKS / 2)) * 4;
+        fetched[g] = epi.fetch(m[g], n[g]);
+      }
+#pragma unroll
+      for (int g = 0; g < AHEAD; ++g) {
+        const int k = k0 + 64 * g, row = k / EACH, c = k % EACH;
+        const Four* x = reinterpret_cast<const Four*>(mine) + row * CHUNKS;
+        const Four v = x[c ^ (row & (CHUNKS - 1))], u = S::GATED ? x[(c + CHUNKS / 2) ^ (row & (CHUNKS - 1))] : v;
+        epi(tt.problem, m[g], n[g], v, u, fetched[g]);
+      }
     }
   }
 }
@@ -387,11 +410,12 @@ __global__ void __launch_bounds__(S::THREADS) tile_join_kernel(TpArgs a, Epi epi
   };
   const int64_t m = (int64_t)tt.tm * S::BM + (wm * MB + j) * 32 + (lane & 31);
   const int64_t n = (int64_t)tt.tn * S::OUT_N + S::block_n(i, wn) + 8 * q + 4 * (lane >> 5);
+  const auto fetched = epi.fetch(m, n);
   const auto v = sum(i);
   if (S::GATED)
-    epi(tt.problem, m, n, v, sum(i + NB / 2));
+    epi(tt.problem, m, n, v, sum(i + NB / 2), fetched);
   else
-    epi(tt.problem, m, n, v, v);
+    epi(tt.problem, m, n, v, v, fetched);
 }
 
 // Host side: sizes, the split of the tiles that do not fill the card, launches.
@@ -407,25 +431,38 @@ inline TpOperand tp_operand(const void* a, const void* b, int64_t ld, int64_t pl
 struct TpPlan {
   int32_t tiles, full, splits;
   int64_t partial;  // bytes
+  float time;       // estimate, us
 };
 
-// Tiles that fill whole rounds of the card (WAVES_EU workgroups of four waves' worth a CU) run whole; where what is left fills
-// less than half of a round, its tiles are shared out over the K axis, at least `least` slices to a workgroup.
+// A shape's measured times (us): of a slice, alone on a CU and by each workgroup of a full one, and of a tile's begin and end.
 template <typename S>
-inline TpPlan tp_plan(int64_t tiles, int64_t slices) {
-  constexpr int64_t per_cu = 4 * S::WAVES_EU * 64 / S::THREADS, round = kTpCus * per_cu;
-  const int64_t least = 4;
-  TpPlan r{(int32_t)tiles, (int32_t)tiles, 1, 0};
+struct TpTimes {
+  static constexpr bool LARGE = S::BN * S::BM >= 65536, SMALL = S::BN * S::BM <= 4096;
+  static constexpr float alone = LARGE ? 1.95f : SMALL ? 0.6f : 0.9f, each = LARGE ? 1.95f : SMALL ? 0.31f : 0.69f;
+  static constexpr float ends = LARGE ? 12.f : SMALL ? 4.f : 6.f;
+};
+
+// Whole rounds of the card run tile by tile; the tiles of the last, partial one may be shared out over the K axis. Of the ways to
+// share them the one with the least time by the shape's measured times; `heavy`: of the epilogue, where it reads and writes more
+// than the result. (Joining costs a launch and the traffic of the sums.)
+template <typename S>
+inline TpPlan tp_plan(int64_t tiles, int64_t slices, float heavy) {
+  constexpr int64_t per_cu = 4 * S::WAVES_EU * 64 / S::THREADS, round = kTpCus * per_cu, sums = (int64_t)S::NB * S::MB * 16 * S::THREADS * 4;
+  typedef TpTimes<S> Times;
+  const auto of = [&](int64_t workgroups, float slices) {
+    const float k = (float)fmd_cdiv(workgroups, kTpCus);
+    const float slice = k * Times::each > Times::alone ? k * Times::each : Times::alone;
+    return slices * slice + Times::ends * heavy;
+  };
   const int64_t left = tiles % round;
-  if (left == 0 || 2 * left > round) return r;
-  int64_t splits = round / left;
-  if (splits > slices / least) splits = slices / least;
-  if (splits > 16) splits = 16;
-  if (splits < 2) return r;
-  r.full = (int32_t)(tiles - left);
-  r.splits = (int32_t)splits;
-  r.partial = left * splits * S::NB * S::MB * 16 * S::THREADS * 4;
-  return r;
+  const float before = (float)(tiles / round) * of(round, (float)slices);
+  TpPlan best{(int32_t)tiles, (int32_t)tiles, 1, 0, before + (left ? of(left, (float)slices) : 0.f)};
+  for (int64_t s = 2; left && s <= 64 && s <= slices && left * s <= round; ++s) {
+    const float traffic = (float)(left * s * sums) * 2.f / 3e6f;
+    const float time = before + of(left * s, (float)fmd_cdiv(slices, s)) + 8.f + traffic;
+    if (time < 0.95f * best.time) best = {(int32_t)tiles, (int32_t)(tiles - left), (int32_t)s, left * s * sums, time};
+  }
+  return best;
 }
 
 template <typename S, typename Epi>
