@@ -10,7 +10,7 @@
 // and gx with them. h, dg and du are rounded to bf16 once, as operands of the next product (float32: split into three planes),
 // so that a bf16 result has the error of two roundings, its own and its operand's.
 #include "activation.h"
-#include "tile_product.h"
+#include "direct_product.h"
 
 namespace {
 
@@ -307,19 +307,59 @@ TpArgs one(const TpOperand& n, const TpOperand& m, int64_t rows_n, int64_t rows_
 
 struct Forward {
   const void *x, *gate, *up, *down;
-  int64_t x_ld, gate_ld, up_ld, down_ld;
+  int64_t x_ld, gate_ld, down_ld;  // gate_ld: of both projections
   void* y;
   float* saved;    // g, u [2, rows, hp], or null
   __bf16* hidden;  // [planes, rows, hp], or null: in the workspace
 };
 
+// Whether the products of a pass go straight from memory to registers (direct_product.h) or through tiles in LDS: by the multiply-adds
+// of the forward pass, where the two forms' times meet. us of the forward pass and of the VJP for x, tiles and straight: float32, 10 000 rows of
+// 64 x 256 36 35, 44 46; 2 000 of 256 x 680 48 47, 58 52; 500 of 512 x 1 376 53 44, 67 52; 64 of 1 024 x 2 736 58 46, 62 75; 16 of
+// 2 048 x 5 504 148 58, 155 79. bf16, 2 000 rows of 128 x 344 14 12, 19 15; 10 000 of 64 x 256 16 22, 21 28; 135 of 512 x 1 376 18 17,
+// 23 26; 16 of 2 048 x 5 504 34 30, 36 56 (its VJP reads weights across their rows, two bytes a lane).
+bool direct_forward(const Ffn& f) {
+  const double work = (double)f.rows * f.hidden * (2 * f.width + f.out);
+  return f.bf16 ? work <= 5.5e8 : work <= 1.1e9 || f.rows <= 64;
+}
+bool direct_backward(const Ffn& f) {
+  const double weights = (double)f.hidden * (2 * f.width + f.out), work = weights * f.rows;
+  return f.bf16 ? work <= 2.7e8 && weights <= 2.2e6 : work <= 5e8 || f.rows <= 32;
+}
+
+DpOperand in_memory(const Ffn& f, const void* a, const void* b, int64_t ld, int64_t k) {
+  const int64_t bytes = f.bf16 ? 2 : 4;
+  const auto starts = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  return {{a, b}, ld, 0, (int32_t)(starts(a) && starts(b) && ld * bytes % 16 == 0 && k % 8 == 0)};
+}
+DpOperand planes_in_memory(const Ffn& f, const __bf16* a, const __bf16* b, int64_t plane) { return {{a, b}, f.hp(), plane, 1}; }
+
+template <bool N_ACROSS, bool GATED, bool OWN, typename Epi>
+int straight(const Ffn& f, const DpArgs& a, const Epi& epi, hipStream_t stream) {  // OWN: m is h, dg or du
+  if (f.bf16) return dp_product<__bf16, N_ACROSS, GATED, false>(a, epi, stream);
+  return dp_product<float, N_ACROSS, GATED, OWN>(a, epi, stream);
+}
+
 int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t stream, int64_t* size) {
+  const int64_t hp = f.hp(), plane = f.rows * hp;
+  const StoreEpi store{{io.y}, {f.rows}, {f.out}, f.bf16};
+  if (direct_forward(f)) {
+    __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.planes());
+    if (size) *size = s.used;
+    if (!run) return FMD_OK;
+    const GatedEpi gated{h, io.saved, io.saved ? io.saved + plane : nullptr, f.rows, f.hidden, hp, plane, f.act, f.planes()};
+    DpOperand weights = in_memory(f, io.gate, io.up, io.gate_ld, f.width);
+    const DpArgs first{weights, in_memory(f, io.x, io.x, io.x_ld, f.width), f.hidden, f.rows, f.width, 1, 0, 0};
+    int status = straight<false, true, false>(f, first, gated, stream);
+    if (status) return status;
+    const DpArgs second{in_memory(f, io.down, io.down, io.down_ld, f.hidden), planes_in_memory(f, h, h, plane), f.out, f.rows, f.hidden, 1, 0, 0};
+    return straight<false, false, true>(f, second, store, stream);
+  }
   Layer lay;
   const Matrix x = lay.add(f, s, f.lay & 1, io.x, io.x_ld, f.rows, f.width);
   const Matrix g = lay.add(f, s, f.lay & 2, io.gate, io.gate_ld, f.hidden, f.width);
-  const Matrix u = lay.add(f, s, f.lay & 2, io.up, io.up_ld, f.hidden, f.width);
+  const Matrix u = lay.add(f, s, f.lay & 2, io.up, io.gate_ld, f.hidden, f.width);
   const Matrix d = lay.add(f, s, f.lay & 4, io.down, io.down_ld, f.out, f.hidden);
-  const int64_t hp = f.hp(), plane = f.rows * hp;
   __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.planes());
   if (run) {
     const int status = lay.launch(f, stream);
@@ -335,7 +375,6 @@ int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t str
   s.used = base;
   const Matrix hm{h, hp, plane};
   a = one(operand(d, d), operand(hm, hm), f.out, f.rows, f.hidden, 1, f.planes());
-  const StoreEpi store{{io.y}, {f.rows}, {f.out}, f.bf16};
   status = product<Shapes<false, false, false>>(a, s, run, store, stream);
   if (status) return status;
   most = s.used > most ? s.used : most;
@@ -351,15 +390,16 @@ struct Backward {
 };
 
 int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& s, bool run, hipStream_t stream, int64_t* size) {
+  const bool straight_on = direct_backward(f);
   Layer lay;
-  Matrix x{}, g{}, u{};
+  Matrix x{}, g{}, u{}, d{}, gy{};
   if (want_w) x = lay.add(f, s, f.lay & 1, io.in.x, io.in.x_ld, f.rows, f.width);
-  if (want_x) {
+  if (want_x && !straight_on) {
     g = lay.add(f, s, f.lay & 2, io.in.gate, io.in.gate_ld, f.hidden, f.width);
-    u = lay.add(f, s, f.lay & 2, io.in.up, io.in.up_ld, f.hidden, f.width);
+    u = lay.add(f, s, f.lay & 2, io.in.up, io.in.gate_ld, f.hidden, f.width);
   }
-  const Matrix d = lay.add(f, s, f.lay & 4, io.in.down, io.in.down_ld, f.out, f.hidden);
-  const Matrix gy = lay.add(f, s, f.lay & 8, io.gy, io.gy_ld, f.rows, f.out);
+  if (!straight_on) d = lay.add(f, s, f.lay & 4, io.in.down, io.in.down_ld, f.out, f.hidden);
+  if (want_w || !straight_on) gy = lay.add(f, s, f.lay & 8, io.gy, io.gy_ld, f.rows, f.out);
   const int64_t hp = f.hp(), plane = f.rows * hp;
   __bf16* dgu = s.take<__bf16>(2 * plane * 2 * f.planes());
   if (run) {
@@ -368,19 +408,31 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   }
   int64_t most = s.used;
   const int64_t base = s.used;
-  TpArgs a = one(operand(d, d), operand(gy, gy), f.hidden, f.rows, f.out, 1, f.planes());
+  TpArgs a{};
   const GatedBackEpi back{dgu, io.in.saved, io.in.saved ? io.in.saved + plane : nullptr, f.rows, f.hidden, hp, 2 * plane, f.act, f.planes()};
-  int status = product<Shapes<true, false, false>>(a, s, run, back, stream);
+  int status = FMD_OK;
+  if (!straight_on) {
+    a = one(operand(d, d), operand(gy, gy), f.hidden, f.rows, f.out, 1, f.planes());
+    status = product<Shapes<true, false, false>>(a, s, run, back, stream);
+    most = s.used > most ? s.used : most;
+  } else if (run) {
+    const DpArgs first{in_memory(f, io.in.down, io.in.down, io.in.down_ld, f.out), in_memory(f, io.gy, io.gy, io.gy_ld, f.out), f.hidden, f.rows, f.out, 1, 0, 0};
+    status = straight<true, false, false>(f, first, back, stream);
+  }
   if (status) return status;
-  most = s.used > most ? s.used : most;
   const Matrix dg{dgu, hp, 2 * plane}, du{dgu + plane, hp, 2 * plane};
   if (want_x) {
     s.used = base;
-    a = one(operand(g, u), operand(dg, du), f.width, f.rows, f.hidden, 2, f.planes());
     const StoreEpi store{{io.gx}, {f.rows}, {f.width}, f.bf16};
-    status = product<Shapes<true, false, false>>(a, s, run, store, stream);
+    if (!straight_on) {
+      a = one(operand(g, u), operand(dg, du), f.width, f.rows, f.hidden, 2, f.planes());
+      status = product<Shapes<true, false, false>>(a, s, run, store, stream);
+      most = s.used > most ? s.used : most;
+    } else if (run) {
+      const DpArgs second{in_memory(f, io.in.gate, io.in.up, io.in.gate_ld, f.hidden), planes_in_memory(f, dgu, dgu + plane, 2 * plane), f.width, f.rows, f.hidden, 2, 0, 0};
+      status = straight<true, false, true>(f, second, store, stream);
+    }
     if (status) return status;
-    most = s.used > most ? s.used : most;
   }
   if (want_w) {
     s.used = base;
@@ -407,7 +459,7 @@ bool sizes_fit(const Ffn& f) {
 bool layouts_fit(const Ffn& f, const Forward& io) {
   if (!f.bf16) return true;
   return ((f.lay & 1) || direct(io.x, io.x_ld, f.width)) &&
-         ((f.lay & 2) || (direct(io.gate, io.gate_ld, f.width) && direct(io.up, io.up_ld, f.width) && io.gate_ld == io.up_ld)) &&
+         ((f.lay & 2) || (direct(io.gate, io.gate_ld, f.width) && direct(io.up, io.gate_ld, f.width))) &&
          ((f.lay & 4) || direct(io.down, io.down_ld, f.hidden));
 }
 
@@ -427,11 +479,11 @@ int64_t fmd_gated_ffn_work_size(int32_t bf16, int64_t rows, int64_t width, int64
   return size;
 }
 
-int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate, int64_t gate_ld,
-                  const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width, int64_t hidden,
+int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate,
+                  const void* up, int64_t gate_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width, int64_t hidden,
                   int64_t out, void* y, float* saved, void* hidden_out, void* work, hipStream_t stream) {
   const Ffn f{bf16, act, lay, rows, width, hidden, out};
-  const Forward io{x, gate, up, down, x_ld, gate_ld, up_ld, down_ld, y, saved, static_cast<__bf16*>(hidden_out)};
+  const Forward io{x, gate, up, down, x_ld, gate_ld, down_ld, y, saved, static_cast<__bf16*>(hidden_out)};
   FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io) && x && gate && up && down && y && work);
   Space s{static_cast<char*>(work)};
   return forward(f, io, s, true, stream, nullptr);
@@ -448,13 +500,13 @@ int64_t fmd_gated_ffn_bwd_work_size(int32_t bf16, int64_t rows, int64_t width, i
   return size;
 }
 
-int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate, int64_t gate_ld,
-                      const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width,
+int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate,
+                      const void* up, int64_t gate_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width,
                       int64_t hidden, int64_t out, const void* gy, int64_t gy_ld, const float* saved, const void* hidden_in,
                       void* gx, void* g_gate, void* g_up, void* g_down, void* work, hipStream_t stream) {
   const Ffn f{bf16, act, lay, rows, width, hidden, out};
   Backward io{};
-  io.in = {x, gate, up, down, x_ld, gate_ld, up_ld, down_ld, nullptr, const_cast<float*>(saved),
+  io.in = {x, gate, up, down, x_ld, gate_ld, down_ld, nullptr, const_cast<float*>(saved),
            static_cast<__bf16*>(const_cast<void*>(hidden_in))};
   io.gy = gy;
   io.gy_ld = gy_ld;

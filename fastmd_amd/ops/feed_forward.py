@@ -84,11 +84,13 @@ def _apart(t: Tensor, ld: int) -> bool:
 def _operands(x, w_gate, w_up, w_down, gy=None):
     """(bits of the operands to lay out, arguments, the tensors that they point into)"""
     (x, x_ld), (w_gate, g_ld), (w_up, u_ld), (w_down, d_ld) = (rows_view(t) for t in (x, w_gate, w_up, w_down))
+    if g_ld != u_ld:
+        w_gate, w_up, g_ld = w_gate.contiguous(), w_up.contiguous(), w_gate.shape[1]
     lay = 15
     if x.dtype is torch.bfloat16:
-        lay = ((1 if _apart(x, x_ld) else 0) | (2 if g_ld != u_ld or _apart(w_gate, g_ld) or _apart(w_up, u_ld) else 0)
+        lay = ((1 if _apart(x, x_ld) else 0) | (2 if _apart(w_gate, g_ld) or _apart(w_up, g_ld) else 0)
                | (4 if _apart(w_down, d_ld) else 0))
-    return lay, (x.data_ptr(), x_ld, w_gate.data_ptr(), g_ld, w_up.data_ptr(), u_ld, w_down.data_ptr(), d_ld, x.shape[0],
+    return lay, (x.data_ptr(), x_ld, w_gate.data_ptr(), w_up.data_ptr(), g_ld, w_down.data_ptr(), d_ld, x.shape[0],
                  x.shape[1], w_gate.shape[0], w_down.shape[0]), (x, w_gate, w_up, w_down)
 
 
@@ -115,7 +117,7 @@ def _forward(x, w_gate, w_up, w_down, activation, save):
     if rows == 0:
         return y, saved
     lay, args, keep = _operands(x, w_gate, w_up, w_down)
-    work = torch.empty(_work_size(bf16, *args[8:], lay, 1 if save else 0), dtype=torch.uint8, device=x.device)
+    work = torch.empty(_work_size(bf16, *args[7:], lay, 1 if save else 0), dtype=torch.uint8, device=x.device)
     with on_device_of(x):
         _abi.call("fmd_gated_ffn", bf16, act, lay, *args, y.data_ptr(), _abi.ptr(saved and saved.projections),
                   _abi.ptr(saved and saved.hidden), work.data_ptr(), stream())
@@ -152,7 +154,7 @@ def gated_feed_forward_vjp(gy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, 
     gy, gy_ld = rows_view(gy)
     if bf16 and _apart(gy, gy_ld):
         lay |= 8
-    work = torch.empty(_work_size_vjp(bf16, *args[8:], lay, 1 if need_x else 0, 1 if need_weights else 0), dtype=torch.uint8,
+    work = torch.empty(_work_size_vjp(bf16, *args[7:], lay, 1 if need_x else 0, 1 if need_weights else 0), dtype=torch.uint8,
                        device=x.device)
     with on_device_of(x):
         _abi.call("fmd_gated_ffn_bwd", bf16, act, lay, *args, gy.data_ptr(), gy_ld, projections.data_ptr(),

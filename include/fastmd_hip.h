@@ -890,15 +890,15 @@ int fmd_qk_norm_rotary_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q
  * elements, unit column stride), y [rows, out] contiguous; bf16: 1 for bf16 storage, 0 for float32 (computed as three bf16
  * planes per operand; a value that rounds to an infinite bf16 gives NaN). act: 0 none, 1 silu, 2 gelu (by erf), 3 relu.
  * lay: bits of the operands that the call lays out in `work` first: 1 x, 2 gate and up, 4 down, 8 gy. float32: 15. bf16: those
- * whose rows do not start on 16 bytes, whose width is no multiple of 8, whose row stride reaches 2^22, and gate and up
- * if their strides differ (FMD_EINVAL where such an operand's bit is missing).
+ * whose rows do not start on 16 bytes, whose width is no multiple of 8, whose row stride reaches 2^22 (FMD_EINVAL where such an
+ * operand's bit is missing). Few rows and small weights are read where they are.
  * For the VJP (nullable): saved, float32 [2, rows, hp], the two projections, and hidden, bf16 [planes, rows, hp] (planes 3 for
  * float32, else 1), the product of the two as `down` multiplies it; hp: hidden rounded up to 8; both 16-byte aligned.
  * rows below 2^31, widths below 2^22. work: fmd_gated_ffn_work_size() bytes on a 256-byte address (keep_hidden: `hidden` is given). */
 int64_t fmd_gated_ffn_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
                                 int32_t keep_hidden);
-int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate, int64_t gate_ld,
-                  const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width, int64_t hidden,
+int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate,
+                  const void* up, int64_t gate_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width, int64_t hidden,
                   int64_t out, void* y, float* saved, void* hidden_out, void* work, hipStream_t stream);
 
 /* VJP of fmd_gated_ffn from the gradient gy [rows, out] (row stride gy_ld) and the forward's `saved` and `hidden`: gx
@@ -906,8 +906,8 @@ int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t
  * features' type. Sums over rows in a fixed order, no atomics. work: fmd_gated_ffn_bwd_work_size() bytes. */
 int64_t fmd_gated_ffn_bwd_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
                                     int32_t want_x, int32_t want_w);
-int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate, int64_t gate_ld,
-                      const void* up, int64_t up_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width,
+int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate,
+                      const void* up, int64_t gate_ld, const void* down, int64_t down_ld, int64_t rows, int64_t width,
                       int64_t hidden, int64_t out, const void* gy, int64_t gy_ld, const float* saved, const void* hidden_in,
                       void* gx, void* g_gate, void* g_up, void* g_down, void* work, hipStream_t stream);
 

@@ -180,7 +180,7 @@ def test_entry_points_refuse_what_no_launch_can_honour():
                                           k.get("groups", 3), k.get("off"), 2, k.get("eps", 1e-5), 16, None, None, None, None)
     assert norm(groups=5) == 10001 and norm(rows=0) == 10001 and norm(act=4) == 10001 and norm(eps=-1.0) == 10001
     assert norm(channels=24600) == 10001 and norm(off=16) == 10001
-    ffn = lambda **k: lib.fmd_gated_ffn(1, k.get("act", 1), 0, k.get("x", 16), k.get("ld", 32), 16, 32, 16, k.get("up", 32), 16, 40,  # noqa: E731
+    ffn = lambda **k: lib.fmd_gated_ffn(1, k.get("act", 1), 0, k.get("x", 16), k.get("ld", 32), 16, 16, k.get("gate", 32), 16, 40,  # noqa: E731
                                         k.get("rows", 4), 32, k.get("hidden", 40), 8, 16, None, None, 16, None)
     assert ffn(rows=0) == 10001 and ffn(act=9) == 10001 and ffn(x=8) == 10001 and ffn(ld=33) == 10001 and ffn(hidden=36) == 10001
-    assert ffn(up=40) == 10001
+    assert ffn(gate=36) == 10001
