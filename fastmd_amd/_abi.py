@@ -160,6 +160,7 @@ SIGNATURES: dict[str, tuple] = {
     "fmd_qk_norm_rotary_bwd": (ctypes.c_int, [_i32, _p, _i64, _i64, _i32, _p, _i64, _i64, _i32, _i64, _i32, _i32, _f32,
                                               _p, _p, _p, _p, _i64, _i64, _i32, _i32, _p, _i32, _p, _i64, _i64, _p,
                                               _i64, _i64, _p, _p, _p, _p, _p, _p]),
+    "fmd_gated_ffn_saves": (_i32, [_i32, _i64, _i64, _i64, _i64]),
     "fmd_gated_ffn_work_size": (_i64, [_i32, _i64, _i64, _i64, _i64, _i32, _i32]),
     "fmd_gated_ffn": (ctypes.c_int, [_i32, _i32, _i32, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64,
                                      _p, _p, _p, _p, _p]),
@@ -172,7 +173,8 @@ SIGNATURES: dict[str, tuple] = {
     "fmd_group_norm_bwd": (ctypes.c_int, [_i32, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _i32, _i32, _p, _i32, _p, _p, _p, _p,
                                           _p, _p, _p]),
     "fmd_quantize_rows": (ctypes.c_int, [_i32, _p, _i64, _i64, _i64, _p, _i64, _p, _p]),
-    "fmd_linear_int8_work_size": (_i64, [_i64, _i64, _i64]),
+    "fmd_linear_int8_work_size": (_i64, [_i32, _i64, _i64, _i64]),
+    "fmd_linear_int8_rows": (ctypes.c_int, [_i32, _p, _i64, _i32, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _p]),
     "fmd_linear_int8": (ctypes.c_int, [_i32, _p, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _p]),
 }
 

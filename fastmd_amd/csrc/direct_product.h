@@ -215,7 +215,7 @@ inline int dp_product(const DpArgs& a, const Epi& epi, hipStream_t stream) {
     const int64_t waves = columns * fmd_cdiv(a.rows_m, 16 * MT);
     if constexpr (MT == 1)
       if (waves <= 192 && units >= 64) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 16>>(a, epi, stream);
-    if (waves < 2048 && units >= 8) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 8>>(a, epi, stream);
+    if (waves < 1024 && units >= 8) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 8>>(a, epi, stream);
     return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 1>>(a, epi, stream);
   };
   const bool much = a.rows_n * a.k * a.parts >= 1 << 20;

@@ -9,8 +9,7 @@
 // The backward pass takes g and u from the forward in float32: in bf16 their rounding alone would leave dg and du two roundings off,
 // and gx with them. h, dg and du are rounded to bf16 once, as operands of the next product (float32: split into three planes),
 // so that a bf16 result has the error of two roundings, its own and its operand's.
-#include "activation.h"
-#include "direct_product.h"
+#include "ffn_block.h"
 
 namespace {
 
@@ -327,10 +326,36 @@ bool direct_backward(const Ffn& f) {
   return f.bf16 ? work <= 2.7e8 && weights <= 2.2e6 : work <= 5e8 || f.rows <= 32;
 }
 
+// Whether the whole block is one kernel: its hidden layer (in the backward pass the two gradients of it) fits LDS for 16 rows, and the
+// weights, which every workgroup walks through, are few. us of the forward pass and of the VJP for x, straight from memory and in one kernel:
+// 64 x 128 float32, 135 rows 10.4 8.6, 10.9 13.5, 10 000 rows 24.7 18.6, 37.1 29.7; bf16 8.4 5.7, 11.1 10.0 and 13.8 10.4, 20.7 18.2. 64 x 256
+// float32, 135 rows 9.8 12.9, 11.7 23.7, 10 000 rows 38.8 30.0, 52.0 53.0; bf16 8.6 7.6, 11.4 17.2 and 18.9 15.7, 20.2 31.3.
+bool one_kernel(const Ffn& f) {
+  const int64_t weights = f.hidden * (2 * f.width + f.out);
+  return weights <= (!f.bf16 && f.rows >= 4096 ? 50000 : 25000) && block_lds((int)f.hidden, f.planes(), 16, true) <= kBlockLds;
+}
+
+template <typename T, bool BACK>
+int block(const Ffn& f, const FfnBlock& a, hipStream_t stream) {
+  const auto launch = [&](auto mt) {
+    constexpr int MT = decltype(mt)::value;
+    const int64_t blocks = fmd_cdiv(f.rows, 16 * MT);
+    FMD_REQUIRE(blocks < (int64_t(1) << 22));
+    ffn_block_kernel<T, MT, BACK><<<(unsigned)blocks, kBlockThreads, block_lds((int)f.hidden, f.planes(), 16 * MT, BACK), stream>>>(a);
+    FMD_CHECK_LAUNCH();
+    return (int)FMD_OK;
+  };
+  // 32 rows of a workgroup where those fill the card
+  if (f.rows >= 32 * kTpCus && block_lds((int)f.hidden, f.planes(), 32, BACK) <= kBlockLds) return launch(std::integral_constant<int, 2>{});
+  return launch(std::integral_constant<int, 1>{});
+}
+
+int32_t wide_rows(const Ffn& f, const void* p, int64_t ld, int64_t k) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * (f.bf16 ? 2 : 4) % 16 == 0 && k % 8 == 0;
+}
+
 DpOperand in_memory(const Ffn& f, const void* a, const void* b, int64_t ld, int64_t k) {
-  const int64_t bytes = f.bf16 ? 2 : 4;
-  const auto starts = [&](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  return {{a, b}, ld, 0, (int32_t)(starts(a) && starts(b) && ld * bytes % 16 == 0 && k % 8 == 0)};
+  return {{a, b}, ld, 0, wide_rows(f, a, ld, k) && wide_rows(f, b, ld, k)};
 }
 DpOperand planes_in_memory(const Ffn& f, const __bf16* a, const __bf16* b, int64_t plane) { return {{a, b}, f.hp(), plane, 1}; }
 
@@ -340,9 +365,21 @@ int straight(const Ffn& f, const DpArgs& a, const Epi& epi, hipStream_t stream) 
   return dp_product<float, N_ACROSS, GATED, OWN>(a, epi, stream);
 }
 
+FfnBlock block_args(const Ffn& f, const Forward& io, const void* gy, int64_t gy_ld, void* result) {
+  return {io.x, io.gate, io.up, io.down, gy, io.x_ld, io.gate_ld, io.down_ld, gy_ld, wide_rows(f, io.x, io.x_ld, f.width),
+          wide_rows(f, io.gate, io.gate_ld, f.width) && wide_rows(f, io.up, io.gate_ld, f.width), wide_rows(f, io.down, io.down_ld, f.hidden),
+          wide_rows(f, gy, gy_ld, f.out), f.rows, (int32_t)f.width, (int32_t)f.hidden, (int32_t)f.out, f.act, result, nullptr, nullptr, f.hp()};
+}
+
 int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t stream, int64_t* size) {
   const int64_t hp = f.hp(), plane = f.rows * hp;
   const StoreEpi store{{io.y}, {f.rows}, {f.out}, f.bf16};
+  if (one_kernel(f)) {
+    if (size) *size = 0;
+    if (!run) return FMD_OK;
+    const FfnBlock a = block_args(f, io, nullptr, 0, io.y);
+    return f.bf16 ? block<__bf16, false>(f, a, stream) : block<float, false>(f, a, stream);
+  }
   if (direct_forward(f)) {
     __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.planes());
     if (size) *size = s.used;
@@ -390,7 +427,7 @@ struct Backward {
 };
 
 int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& s, bool run, hipStream_t stream, int64_t* size) {
-  const bool straight_on = direct_backward(f);
+  const bool together = one_kernel(f), straight_on = together || direct_backward(f);
   Layer lay;
   Matrix x{}, g{}, u{}, d{}, gy{};
   if (want_w) x = lay.add(f, s, f.lay & 1, io.in.x, io.in.x_ld, f.rows, f.width);
@@ -401,17 +438,30 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   if (!straight_on) d = lay.add(f, s, f.lay & 4, io.in.down, io.in.down_ld, f.out, f.hidden);
   if (want_w || !straight_on) gy = lay.add(f, s, f.lay & 8, io.gy, io.gy_ld, f.rows, f.out);
   const int64_t hp = f.hp(), plane = f.rows * hp;
-  __bf16* dgu = s.take<__bf16>(2 * plane * 2 * f.planes());
+  __bf16* dgu = together && !want_w ? nullptr : s.take<__bf16>(2 * plane * 2 * f.planes());
   if (run) {
     const int status = lay.launch(f, stream);
     if (status) return status;
   }
   int64_t most = s.used;
-  const int64_t base = s.used;
+  __bf16* h = io.in.hidden;
   TpArgs a{};
+  if (together) {
+    h = want_w ? s.take<__bf16>(plane * 2 * f.planes()) : nullptr;
+    most = s.used;
+    if (run) {
+      FfnBlock b = block_args(f, io.in, io.gy, io.gy_ld, io.gx);
+      b.h = h;
+      b.d = want_w ? dgu : nullptr;
+      const int status = f.bf16 ? block<__bf16, true>(f, b, stream) : block<float, true>(f, b, stream);
+      if (status) return status;
+    }
+  }
+  const int64_t base = s.used;
   const GatedBackEpi back{dgu, io.in.saved, io.in.saved ? io.in.saved + plane : nullptr, f.rows, f.hidden, hp, 2 * plane, f.act, f.planes()};
   int status = FMD_OK;
-  if (!straight_on) {
+  if (together) {
+  } else if (!straight_on) {
     a = one(operand(d, d), operand(gy, gy), f.hidden, f.rows, f.out, 1, f.planes());
     status = product<Shapes<true, false, false>>(a, s, run, back, stream);
     most = s.used > most ? s.used : most;
@@ -421,7 +471,7 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   }
   if (status) return status;
   const Matrix dg{dgu, hp, 2 * plane}, du{dgu + plane, hp, 2 * plane};
-  if (want_x) {
+  if (want_x && !together) {
     s.used = base;
     const StoreEpi store{{io.gx}, {f.rows}, {f.width}, f.bf16};
     if (!straight_on) {
@@ -436,10 +486,10 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   }
   if (want_w) {
     s.used = base;
-    const Matrix h{io.in.hidden, hp, plane};
+    const Matrix hm{h, hp, plane};
     a = one(operand(x, x), operand(dg, dg), f.width, f.hidden, f.rows, 1, f.planes());
     a.p[1] = {operand(x, x), operand(du, du), f.width, f.hidden, f.rows, 1, f.planes(), 0, 0, 0};
-    a.p[2] = {operand(h, h), operand(gy, gy), f.hidden, f.out, f.rows, 1, f.planes(), 0, 0, 0};
+    a.p[2] = {operand(hm, hm), operand(gy, gy), f.hidden, f.out, f.rows, 1, f.planes(), 0, 0, 0};
     a.count = 3;
     const StoreEpi store{{io.g_gate, io.g_up, io.g_down}, {f.hidden, f.hidden, f.out}, {f.width, f.width, f.hidden}, f.bf16};
     status = product<Shapes<true, true, false>>(a, s, run, store, stream);
@@ -467,6 +517,11 @@ bool layouts_fit(const Ffn& f, const Forward& io) {
 
 extern "C" {
 
+int32_t fmd_gated_ffn_saves(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out) {
+  const Ffn f{bf16, 0, 15, rows, width, hidden, out};
+  return sizes_fit(f) && !one_kernel(f);
+}
+
 int64_t fmd_gated_ffn_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
                                 int32_t keep_hidden) {
   const Ffn f{bf16, 0, lay, rows, width, hidden, out};
@@ -484,8 +539,11 @@ int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t
                   int64_t out, void* y, float* saved, void* hidden_out, void* work, hipStream_t stream) {
   const Ffn f{bf16, act, lay, rows, width, hidden, out};
   const Forward io{x, gate, up, down, x_ld, gate_ld, down_ld, y, saved, static_cast<__bf16*>(hidden_out)};
-  FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io) && x && gate && up && down && y && work);
-  Space s{static_cast<char*>(work)};
+  FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io) && x && gate && up && down && y);
+  int64_t size = 0;
+  Space none{nullptr}, s{static_cast<char*>(work)};
+  forward(f, io, none, false, nullptr, &size);
+  FMD_REQUIRE(work || !size);
   return forward(f, io, s, true, stream, nullptr);
 }
 
@@ -514,10 +572,13 @@ int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int
   io.g_gate = g_gate;
   io.g_up = g_up;
   io.g_down = g_down;
-  FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io.in) && x && gate && up && down && gy && saved && work);
+  FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io.in) && x && gate && up && down && gy && (saved || one_kernel(f)));
   FMD_REQUIRE(!bf16 || (lay & 8) || direct(gy, gy_ld, out));
-  FMD_REQUIRE(!g_gate || (g_up && g_down && hidden_in));
-  Space s{static_cast<char*>(work)};
+  FMD_REQUIRE(!g_gate || (g_up && g_down && (hidden_in || one_kernel(f))));
+  int64_t size = 0;
+  Space none{nullptr}, s{static_cast<char*>(work)};
+  backward(f, io, gx != nullptr, g_gate != nullptr, none, false, nullptr, &size);
+  FMD_REQUIRE(work || !size);
   return backward(f, io, gx != nullptr, g_gate != nullptr, s, true, stream, nullptr);
 }
 

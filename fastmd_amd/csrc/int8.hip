@@ -1,6 +1,6 @@
 // Products with weights held in 8-bit integers: rows are rounded to 8 bits with a scale for each, the product is exact in 32-bit
 // integers, and its epilogue multiplies by the row's and the channel's scale.
-#include "tile_product.h"
+#include "direct_product.h"
 
 namespace {
 
@@ -168,6 +168,8 @@ struct ScaleEpi {
   }
 };
 
+constexpr double kDirectInt8 = 5e8;
+
 typedef TpShape<TpInt8, 2, 4, 4, 2, false, false, false, 2> Large;
 typedef TpShape<TpInt8, 2, 2, 2, 2, false, false, false, 2> Middle;
 typedef TpShape<TpInt8, 1, 2, 2, 1, false, false, false, 2> Small;
@@ -205,6 +207,27 @@ bool rows_fit(const int8_t* p, int64_t ld, int64_t width) {
   return p && ld >= width && ld % 16 == 0 && ld <= kTpMostLd && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
+// bytes of rounded rows and their scales
+int64_t rounded_size(int64_t rows, int64_t width) {
+  const int64_t ld = (width + 15) & ~int64_t(15);
+  return ((rows * ld + 255) & ~int64_t(255)) + ((rows * 4 + 255) & ~int64_t(255));
+}
+
+// Few rows, or a small product: straight from memory (direct_product.h), with nothing to join.
+bool few_rows(int64_t rows, int64_t width, int64_t out) { return rows <= 64 || (double)rows * width * out <= kDirectInt8; }
+
+int product(const int8_t* x, int64_t x_ld, const int8_t* w, int64_t w_ld, int64_t rows, int64_t width, int64_t out, const ScaleEpi& epi,
+            void* work, hipStream_t stream) {
+  if (few_rows(rows, width, out)) {
+    // whole vectors: past the width one of the two is zero, and both can be read
+    const int64_t k = (width + 15) & ~int64_t(15);
+    const DpArgs a{{{w, w}, w_ld, 0, 1}, {{x, x}, x_ld, 0, 1}, out, rows, k, 1, 0, 0};
+    return dp_product<int8_t, false, false, false>(a, epi, stream);
+  }
+  TpArgs a = arguments(x, x_ld, w, w_ld, rows, width, out);
+  return with_shape(a, [&](auto shape, const TpPlan& plan) { return tp_launch<decltype(shape)>(a, plan, work, epi, stream); });
+}
+
 }  // namespace
 
 extern "C" {
@@ -217,24 +240,37 @@ int fmd_quantize_rows(int32_t bf16, const void* x, int64_t x_ld, int64_t rows, i
   return bf16 ? quantize<__bf16>(a, stream) : quantize<float>(a, stream);
 }
 
-int64_t fmd_linear_int8_work_size(int64_t rows, int64_t width, int64_t out) {
+int64_t fmd_linear_int8_work_size(int32_t rounded, int64_t rows, int64_t width, int64_t out) {
   if (!sizes_fit(rows, width, out)) return 0;
+  int64_t size = rounded ? 0 : rounded_size(rows, width);
   TpArgs a = arguments(nullptr, 16, nullptr, 16, rows, width, out);
-  int64_t size = 0;
-  with_shape(a, [&](auto, const TpPlan& plan) {
-    size = plan.partial;
-    return (int)FMD_OK;
-  });
+  if (!few_rows(rows, width, out))
+    with_shape(a, [&](auto, const TpPlan& plan) {
+      size += plan.partial;
+      return (int)FMD_OK;
+    });
   return size;
 }
 
 int fmd_linear_int8(int32_t bf16, const int8_t* x, int64_t x_ld, const float* x_scales, const int8_t* w, int64_t w_ld,
                     const float* w_scales, const float* bias, int64_t rows, int64_t width, int64_t out, void* y, void* work,
                     hipStream_t stream) {
-  FMD_REQUIRE(sizes_fit(rows, width, out) && rows_fit(x, x_ld, width) && rows_fit(w, w_ld, width) && x_scales && w_scales && y && work);
-  TpArgs a = arguments(x, x_ld, w, w_ld, rows, width, out);
+  FMD_REQUIRE(sizes_fit(rows, width, out) && rows_fit(x, x_ld, width) && rows_fit(w, w_ld, width) && x_scales && w_scales && y);
+  FMD_REQUIRE(work || !fmd_linear_int8_work_size(1, rows, width, out));
   const ScaleEpi epi{y, x_scales, w_scales, bias, rows, out, bf16};
-  return with_shape(a, [&](auto shape, const TpPlan& plan) { return tp_launch<decltype(shape)>(a, plan, work, epi, stream); });
+  return product(x, x_ld, w, w_ld, rows, width, out, epi, work, stream);
+}
+
+int fmd_linear_int8_rows(int32_t x_bf16, const void* x, int64_t x_ld, int32_t bf16, const int8_t* w, int64_t w_ld, const float* w_scales,
+                         const float* bias, int64_t rows, int64_t width, int64_t out, void* y, void* work, hipStream_t stream) {
+  FMD_REQUIRE(sizes_fit(rows, width, out) && x && rows_fit(w, w_ld, width) && w_scales && y && work);
+  int8_t* q = static_cast<int8_t*>(work);
+  const int64_t q_ld = (width + 15) & ~int64_t(15);
+  float* scales = reinterpret_cast<float*>(q + ((rows * q_ld + 255) & ~int64_t(255)));
+  const int status = fmd_quantize_rows(x_bf16, x, x_ld, rows, width, q, q_ld, scales, stream);
+  if (status) return status;
+  const ScaleEpi epi{y, scales, w_scales, bias, rows, out, bf16};
+  return product(q, q_ld, w, w_ld, rows, width, out, epi, q + rounded_size(rows, width), stream);
 }
 
 }  // extern "C"

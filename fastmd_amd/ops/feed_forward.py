@@ -36,10 +36,10 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 class FeedForwardSaved(NamedTuple):
     """What the VJP needs of the forward besides its inputs, rows of the hidden width rounded up to a multiple of 8:
     ``projections`` float32 [2, rows, .], x w_gate^T and x w_up^T, and ``hidden`` bfloat16 [planes, rows, .], what w_down
-    multiplies (for float32 its three planes)."""
+    multiplies (for float32 its three planes). None for blocks of small weights, whose VJP forms both again."""
 
-    projections: Tensor
-    hidden: Tensor
+    projections: Tensor | None
+    hidden: Tensor | None
 
 
 def _refuse(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor) -> None:
@@ -81,9 +81,13 @@ def _apart(t: Tensor, ld: int) -> bool:
     return bool(t.shape[1] % 8 or ld % 8 or ld >= 2 ** 22 or t.data_ptr() % 16)
 
 
+def _rows(t: Tensor) -> tuple[Tensor, int]:
+    return (t, t.shape[1]) if t.is_contiguous() else rows_view(t)
+
+
 def _operands(x, w_gate, w_up, w_down, gy=None):
     """(bits of the operands to lay out, arguments, the tensors that they point into)"""
-    (x, x_ld), (w_gate, g_ld), (w_up, u_ld), (w_down, d_ld) = (rows_view(t) for t in (x, w_gate, w_up, w_down))
+    (x, x_ld), (w_gate, g_ld), (w_up, u_ld), (w_down, d_ld) = _rows(x), _rows(w_gate), _rows(w_up), _rows(w_down)
     if g_ld != u_ld:
         w_gate, w_up, g_ld = w_gate.contiguous(), w_up.contiguous(), w_gate.shape[1]
     lay = 15
@@ -95,32 +99,42 @@ def _operands(x, w_gate, w_up, w_down, gy=None):
 
 
 @functools.lru_cache(maxsize=256)
+def _saves(*sizes: int) -> bool:
+    return bool(_abi.load().fmd_gated_ffn_saves(*sizes))
+
+
+@functools.lru_cache(maxsize=256)
 def _work_size(*sizes: int) -> int:
-    return max(1, _abi.load().fmd_gated_ffn_work_size(*sizes))
+    return _abi.load().fmd_gated_ffn_work_size(*sizes)
 
 
 @functools.lru_cache(maxsize=256)
 def _work_size_vjp(*sizes: int) -> int:
-    return max(1, _abi.load().fmd_gated_ffn_bwd_work_size(*sizes))
+    return _abi.load().fmd_gated_ffn_bwd_work_size(*sizes)
+
+
+def _space(size: int, device) -> Tensor | None:
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _forward(x, w_gate, w_up, w_down, activation, save):
     act = _check(x, w_gate, w_up, w_down, activation)
-    rows, hidden = x.shape[0], w_gate.shape[0]
-    bf16 = _TYPES[x.dtype]
-    y = torch.empty((rows, w_down.shape[0]), dtype=x.dtype, device=x.device)
-    saved = None
+    (rows, width), hidden, out, device, bf16 = x.shape, w_gate.shape[0], w_down.shape[0], x.device, _TYPES[x.dtype]
+    y = torch.empty((rows, out), dtype=x.dtype, device=device)
+    saved = projections = kept = None
     if save:
-        padded = -(-hidden // 8) * 8
-        saved = FeedForwardSaved(torch.empty((2, rows, padded), dtype=torch.float32, device=x.device),
-                                 torch.empty((1 if bf16 else 3, rows, padded), dtype=torch.bfloat16, device=x.device))
+        if _saves(bf16, rows, width, hidden, out):
+            padded = -(-hidden // 8) * 8
+            projections = torch.empty((2, rows, padded), dtype=torch.float32, device=device)
+            kept = torch.empty((1 if bf16 else 3, rows, padded), dtype=torch.bfloat16, device=device)
+        saved = FeedForwardSaved(projections, kept)
     if rows == 0:
         return y, saved
     lay, args, keep = _operands(x, w_gate, w_up, w_down)
-    work = torch.empty(_work_size(bf16, *args[7:], lay, 1 if save else 0), dtype=torch.uint8, device=x.device)
+    work = _space(_work_size(bf16, rows, width, hidden, out, lay, 0 if kept is None else 1), device)
     with on_device_of(x):
-        _abi.call("fmd_gated_ffn", bf16, act, lay, *args, y.data_ptr(), _abi.ptr(saved and saved.projections),
-                  _abi.ptr(saved and saved.hidden), work.data_ptr(), stream())
+        _abi.call("fmd_gated_ffn", bf16, act, lay, *args, y.data_ptr(), _abi.ptr(projections), _abi.ptr(kept), _abi.ptr(work),
+                  stream())
     del keep
     return y, saved
 
@@ -136,29 +150,31 @@ def gated_feed_forward_vjp(gy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, 
     """``(gradient of x, of w_gate, of w_up, of w_down)`` from the gradient of the output and the forward's ``saved`` (None
     where not needed; the weights' come together)."""
     act = _check(x, w_gate, w_up, w_down, activation)
-    projections, hidden = saved
-    require_cuda(x, gy, projections, hidden)
-    rows, padded, bf16 = x.shape[0], -(-w_gate.shape[0] // 8) * 8, _TYPES[x.dtype]
-    if gy.shape != (rows, w_down.shape[0]) or gy.dtype != x.dtype:
-        raise ValueError(f"gy must be {x.dtype} {(rows, w_down.shape[0])}, got {gy.dtype} {tuple(gy.shape)}")
-    for t, shape, dtype in ((projections, (2, rows, padded), torch.float32),
-                            (hidden, (1 if bf16 else 3, rows, padded), torch.bfloat16)):
-        if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError(f"saved must be the forward's: {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    projections, kept = saved
+    (rows, width), hidden, out, device, bf16 = x.shape, w_gate.shape[0], w_down.shape[0], x.device, _TYPES[x.dtype]
+    require_cuda(x, gy, projections, kept)
+    if gy.shape != (rows, out) or gy.dtype != x.dtype:
+        raise ValueError(f"gy must be {x.dtype} {(rows, out)}, got {gy.dtype} {tuple(gy.shape)}")
+    if rows and _saves(bf16, rows, width, hidden, out):
+        padded = -(-hidden // 8) * 8
+        for t, shape, dtype in ((projections, (2, rows, padded), torch.float32),
+                                (kept, (1 if bf16 else 3, rows, padded), torch.bfloat16)):
+            if t is None or t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"saved must be the forward's: {dtype} {shape}, got "
+                                 f"{None if t is None else (t.dtype, tuple(t.shape))}")
     make = torch.empty if rows else torch.zeros
-    gx, *gw = (make(t.shape, dtype=x.dtype, device=x.device) if need else None
-               for t, need in ((x, need_x), (w_gate, need_weights), (w_up, need_weights), (w_down, need_weights)))
+    gx = make((rows, width), dtype=x.dtype, device=device) if need_x else None
+    gw = [make(t.shape, dtype=x.dtype, device=device) if need_weights else None for t in (w_gate, w_up, w_down)]
     if rows == 0 or not (need_x or need_weights):
         return (gx, *gw)
     lay, args, keep = _operands(x, w_gate, w_up, w_down)
-    gy, gy_ld = rows_view(gy)
+    gy, gy_ld = _rows(gy)
     if bf16 and _apart(gy, gy_ld):
         lay |= 8
-    work = torch.empty(_work_size_vjp(bf16, *args[7:], lay, 1 if need_x else 0, 1 if need_weights else 0), dtype=torch.uint8,
-                       device=x.device)
+    work = _space(_work_size_vjp(bf16, rows, width, hidden, out, lay, 1 if need_x else 0, 1 if need_weights else 0), device)
     with on_device_of(x):
-        _abi.call("fmd_gated_ffn_bwd", bf16, act, lay, *args, gy.data_ptr(), gy_ld, projections.data_ptr(),
-                  hidden.data_ptr(), _abi.ptr(gx), *(_abi.ptr(t) for t in gw), work.data_ptr(), stream())
+        _abi.call("fmd_gated_ffn_bwd", bf16, act, lay, *args, gy.data_ptr(), gy_ld, _abi.ptr(projections), _abi.ptr(kept),
+                  _abi.ptr(gx), *(_abi.ptr(t) for t in gw), _abi.ptr(work), stream())
     del keep
     return (gx, *gw)
 

@@ -77,7 +77,14 @@ def _in_place(values: Tensor, padded: bool) -> tuple[Tensor, int]:
 
 @functools.lru_cache(maxsize=256)
 def _work_size(*sizes: int) -> int:
-    return max(1, _abi.load().fmd_linear_int8_work_size(*sizes))
+    return _abi.load().fmd_linear_int8_work_size(*sizes)
+
+
+def _check_rows(name: str, q: Int8Rows) -> None:
+    if (q.values.dim() != 2 or q.values.dtype != torch.int8 or q.scales.shape != q.values.shape[:1]
+            or q.scales.dtype != torch.float32):
+        raise ValueError(f"{name} must be int8 [rows, width] with float32 scales [rows], got {q.values.dtype} "
+                         f"{tuple(q.values.shape)} and {q.scales.dtype} {tuple(q.scales.shape)}")
 
 
 def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, dtype: torch.dtype | None = None) -> Tensor:
@@ -86,38 +93,45 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = No
     ``Int8Rows``."""
     if not isinstance(weight, Int8Rows):
         raise ValueError("weight must be Int8Rows (quantize_rows)")
-    rounded = not isinstance(x, Int8Rows)
-    if not rounded:
-        kind = torch.float32 if dtype is None else dtype
+    _check_rows("weight", weight)
+    rounded = isinstance(x, Int8Rows)
+    if rounded:
+        _check_rows("x", x)
+        values, kind = x.values, torch.float32 if dtype is None else dtype
+        require_cuda(values, x.scales, weight.values, weight.scales, bias)
     else:
-        kind = x.dtype if dtype is None else dtype
+        values, kind = x, x.dtype if dtype is None else dtype
+        require_cuda(x, weight.values, weight.scales, bias)
+        if x.dim() != 2 or x.dtype not in _TYPES:
+            raise ValueError(f"x must be a float32 or bfloat16 matrix, or Int8Rows, got {x.dtype} {tuple(x.shape)}")
         if differentiated(x, bias):
             raise ValueError("linear_int8 has no gradient: detach its inputs")
-        x = quantize_rows(x)
-    require_cuda(x.values, x.scales, weight.values, weight.scales, bias)
     if kind not in _TYPES:
         raise ValueError(f"the result must be float32 or bfloat16, got {kind}")
-    for name, q in (("x", x), ("weight", weight)):
-        if (q.values.dim() != 2 or q.values.dtype != torch.int8 or q.scales.shape != q.values.shape[:1]
-                or q.scales.dtype != torch.float32):
-            raise ValueError(f"{name} must be int8 [rows, width] with float32 scales [rows], got {q.values.dtype} "
-                             f"{tuple(q.values.shape)} and {q.scales.dtype} {tuple(q.scales.shape)}")
-    (rows, width), out = x.values.shape, weight.values.shape[0]
+    (rows, width), out, device = values.shape, weight.values.shape[0], values.device
     if weight.values.shape[1] != width or not 1 <= width <= MAX_WIDTH:
         raise ValueError(f"x and weight must have one width, from 1 to {MAX_WIDTH}, got {width} and {weight.values.shape[1]}")
     if rows >= 2 ** 31 or out >= 2 ** 31:
         raise ValueError("linear_int8 takes fewer than 2^31 rows and channels")
-    if bias is not None and (bias.shape != (out,) or bias.dtype != torch.float32):
-        raise ValueError(f"bias must be float32 [{out}], got {bias.dtype} {tuple(bias.shape)}")
-    y = torch.empty((rows, out), dtype=kind, device=x.values.device)
+    if bias is not None:
+        if bias.shape != (out,) or bias.dtype != torch.float32:
+            raise ValueError(f"bias must be float32 [{out}], got {bias.dtype} {tuple(bias.shape)}")
+        bias = bias.contiguous()
+    y = torch.empty((rows, out), dtype=kind, device=device)
     if rows == 0 or out == 0:
         return y
-    # past the width one of the two has to be zero: rows that were rounded here are
-    (xv, x_ld), (wv, w_ld) = _in_place(x.values, not rounded), _in_place(weight.values, False)
-    x_scales, w_scales = x.scales.contiguous(), weight.scales.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    work = torch.empty(_work_size(rows, width, out), dtype=torch.uint8, device=y.device)
+    w, w_ld = _in_place(weight.values, False)
+    w_scales = weight.scales.contiguous()
+    size = _work_size(1 if rounded else 0, rows, width, out)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    rest = (_TYPES[kind], w.data_ptr(), w_ld, w_scales.data_ptr(), _abi.ptr(bias), rows, width, out, y.data_ptr(), _abi.ptr(work))
     with on_device_of(y):
-        _abi.call("fmd_linear_int8", _TYPES[kind], xv.data_ptr(), x_ld, x_scales.data_ptr(), wv.data_ptr(), w_ld,
-                  w_scales.data_ptr(), _abi.ptr(bias), rows, width, out, y.data_ptr(), work.data_ptr(), stream())
+        if rounded:
+            # past the width one of the two has to be zero: rows that the call rounds itself are
+            values, x_ld = _in_place(values, True)
+            scales = x.scales.contiguous()
+            _abi.call("fmd_linear_int8", rest[0], values.data_ptr(), x_ld, scales.data_ptr(), *rest[1:], stream())
+        else:
+            values, x_ld = rows_view(values)
+            _abi.call("fmd_linear_int8_rows", _TYPES[x.dtype], values.data_ptr(), x_ld, *rest, stream())
     return y

@@ -892,9 +892,11 @@ int fmd_qk_norm_rotary_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q
  * lay: bits of the operands that the call lays out in `work` first: 1 x, 2 gate and up, 4 down, 8 gy. float32: 15. bf16: those
  * whose rows do not start on 16 bytes, whose width is no multiple of 8, whose row stride reaches 2^22 (FMD_EINVAL where such an
  * operand's bit is missing). Few rows and small weights are read where they are.
- * For the VJP (nullable): saved, float32 [2, rows, hp], the two projections, and hidden, bf16 [planes, rows, hp] (planes 3 for
+ * For the VJP (nullable, and unused where fmd_gated_ffn_saves() is 0: it forms them again): saved, float32 [2, rows, hp], the two projections, and hidden, bf16 [planes, rows, hp] (planes 3 for
  * float32, else 1), the product of the two as `down` multiplies it; hp: hidden rounded up to 8; both 16-byte aligned.
- * rows below 2^31, widths below 2^22. work: fmd_gated_ffn_work_size() bytes on a 256-byte address (keep_hidden: `hidden` is given). */
+ * rows below 2^31, widths below 2^22. work: fmd_gated_ffn_work_size() bytes on a 256-byte address (keep_hidden: `hidden` is given;
+ * null for 0). */
+int32_t fmd_gated_ffn_saves(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out);
 int64_t fmd_gated_ffn_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
                                 int32_t keep_hidden);
 int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t x_ld, const void* gate,
@@ -941,11 +943,16 @@ int fmd_quantize_rows(int32_t bf16, const void* x, int64_t x_ld, int64_t rows, i
  * in bytes: multiples of 16 up to 2^23, rows on 16 bytes; both are read up to the width's next multiple of 16, where x is zero),
  * exact sums in 32 bits;
  * bias float32, nullable; out [rows, out] of bf16 or float32, contiguous. width below 131 072 (no sum overflows).
- * work: fmd_linear_int8_work_size() bytes. */
-int64_t fmd_linear_int8_work_size(int64_t rows, int64_t width, int64_t out);
+ * work: fmd_linear_int8_work_size(1, ...) bytes on a 256-byte address (null for 0). */
+int64_t fmd_linear_int8_work_size(int32_t rounded, int64_t rows, int64_t width, int64_t out);
 int fmd_linear_int8(int32_t bf16, const int8_t* x, int64_t x_ld, const float* x_scales, const int8_t* w, int64_t w_ld,
                     const float* w_scales, const float* bias, int64_t rows, int64_t width, int64_t out, void* y, void* work,
                     hipStream_t stream);
+
+/* fmd_quantize_rows of x [rows, width] (x_bf16: bf16, else float32) in `work`, then fmd_linear_int8 of them.
+ * work: fmd_linear_int8_work_size(0, ...) bytes. */
+int fmd_linear_int8_rows(int32_t x_bf16, const void* x, int64_t x_ld, int32_t bf16, const int8_t* w, int64_t w_ld, const float* w_scales,
+                         const float* bias, int64_t rows, int64_t width, int64_t out, void* y, void* work, hipStream_t stream);
 
 #ifdef __cplusplus
 }
