@@ -10,6 +10,9 @@ Model (atom features x [N, C], H query heads on Hk key heads of width D):
   per layer: q | k | v = x W_qkv^T; each head of q and k is normed over its columns and turned by its atom's element
              (position = element index: the scores of a pair depend on both elements, not on the atoms' order)
              x += attention(q, k, v over the atoms of the system) W_o^T;  x += silu(x W_1^T) W_2^T
+  with ``feed_forward="gated"`` the last is (silu(x W_gate^T) * (x W_up^T)) W_down^T, hidden width ``hidden`` (2 C for 0);
+  with ``norm_groups`` > 0 attention and feed-forward read the features normed over that many groups of channels, each atom
+  by itself (so that the energy stays extensive), with a weight and a bias
   readout:   E_i = e0[Z_i] + x_i . wr
 Sums over a system's atoms are softmax-weighted means, so the energy is extensive and does not depend on the order of the
 atoms. Random init from ``torch.Generator().manual_seed(seed)``; parameters are frozen as those of the other models are, and
@@ -33,6 +36,8 @@ from fastmd_amd.adapters.protocol import (CapacityStep, GraphBatch, PaddingRule,
                                          system_rows)
 from fastmd_amd.ops.attention import segment_attention
 from fastmd_amd.ops.csr_segment_sum import Csr, segment_sum_csr, segment_sum_t
+from fastmd_amd.ops.feed_forward import gated_feed_forward
+from fastmd_amd.ops.group_norm import group_norm
 from fastmd_amd.ops.qk_norm import qk_norm_rotary, rotary_tables
 from fastmd_amd.ops.wide_gemm import linear
 
@@ -51,6 +56,9 @@ class AttentionConfig:
     avg_num_neighbors: float = 15.0
     elements: tuple = (55, 50, 53)
     seed: int = 0
+    feed_forward: str = "two_layer"  # or "gated"
+    hidden: int = 0
+    norm_groups: int = 0
 
 
 class AttentionLike(nn.Module):
@@ -62,6 +70,11 @@ class AttentionLike(nn.Module):
         C, H, Hk, D = config.channels, config.heads, config.kv_heads, config.head_dim
         if H < 1 or Hk < 1 or H % Hk:
             raise ValueError(f"heads must be a multiple of kv_heads, got {H} and {Hk}")
+        if config.feed_forward not in ("two_layer", "gated"):
+            raise ValueError(f"feed_forward must be two_layer or gated, got {config.feed_forward!r}")
+        if config.norm_groups < 0 or (config.norm_groups and C % config.norm_groups):
+            raise ValueError(f"channels must be a multiple of norm_groups, got {C} and {config.norm_groups}")
+        F = config.hidden or 2 * C
         gen = torch.Generator().manual_seed(config.seed)
 
         def rnd(*shape, scale=1.0):
@@ -77,8 +90,15 @@ class AttentionLike(nn.Module):
             layer.q_weight = nn.Parameter(1.0 + 0.1 * torch.randn(D, generator=gen), requires_grad=False)
             layer.k_weight = nn.Parameter(1.0 + 0.1 * torch.randn(D, generator=gen), requires_grad=False)
             layer.W_o = rnd(C, H * D)
-            layer.W_1 = rnd(2 * C, C)
-            layer.W_2 = rnd(C, 2 * C)
+            if config.feed_forward == "gated":
+                layer.W_gate, layer.W_up, layer.W_down = rnd(F, C), rnd(F, C), rnd(C, F)
+            else:
+                layer.W_1, layer.W_2 = rnd(F, C), rnd(C, F)
+            if config.norm_groups:
+                for name in ("attention", "feed_forward"):
+                    weight = 1.0 + 0.1 * torch.randn(C, generator=gen)
+                    setattr(layer, name + "_norm_weight", nn.Parameter(weight, requires_grad=False))
+                    setattr(layer, name + "_norm_bias", nn.Parameter(0.1 * torch.randn(C, generator=gen), requires_grad=False))
             self.layers.append(layer)
         self.wr = rnd(C)
         self.e0 = nn.Parameter(-1.0 - torch.rand(nel, generator=gen), requires_grad=False)
@@ -90,6 +110,17 @@ class AttentionLike(nn.Module):
             table[z] = k
         self.register_buffer("z_table", table)
 
+    def _normed(self, x: Tensor, layer: nn.Module, name: str) -> Tensor:
+        groups = self.config.norm_groups
+        if not groups:
+            return x
+        return group_norm(x, groups, getattr(layer, name + "_norm_weight"), getattr(layer, name + "_norm_bias"))
+
+    def _feed_forward(self, x: Tensor, layer: nn.Module) -> Tensor:
+        if self.config.feed_forward == "gated":
+            return gated_feed_forward(x, layer.W_gate, layer.W_up, layer.W_down)
+        return linear(nn.functional.silu(linear(x, layer.W_1)), layer.W_2)
+
     def forward(self, surroundings: Tensor, elem: Tensor, offsets: Tensor) -> Tensor:
         """Energies [N] of atoms in packed systems: ``surroundings`` [N, elements * n_basis], element indices [N], and
         ``offsets`` [systems + 1] of the systems' rows."""
@@ -97,11 +128,11 @@ class AttentionLike(nn.Module):
         H, Hk, D = cfg.heads, cfg.kv_heads, cfg.head_dim
         x = linear(surroundings, self.W_in) + self.embedding[elem]
         for layer in self.layers:
-            qkv = linear(x, layer.W_qkv).view(-1, H + 2 * Hk, D)
+            qkv = linear(self._normed(x, layer, "attention"), layer.W_qkv).view(-1, H + 2 * Hk, D)
             q, k, v = qkv[:, :H], qkv[:, H:H + Hk], qkv[:, H + Hk:]  # read in place
             q, k = qk_norm_rotary(q, k, layer.q_weight, layer.k_weight, self.cos, self.sin, elem)
             x = x + linear(segment_attention(q, k, v, offsets).view(-1, H * D), layer.W_o)
-            x = x + linear(nn.functional.silu(linear(x, layer.W_1)), layer.W_2)
+            x = x + self._feed_forward(self._normed(x, layer, "feed_forward"), layer)
         return self.e0[elem] + (x * self.wr).sum(1)
 
 

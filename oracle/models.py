@@ -203,9 +203,18 @@ def attention_like_node_energy(params: dict, config: dict, positions, cell, elem
         a, b = t[..., :D // 2], t[..., D // 2:]
         return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
 
+    def normed(x, W, name):
+        groups = config.get("norm_groups", 0)
+        if not groups:
+            return x
+        y = x.view(n, groups, -1)
+        y = (y - y.mean(-1, keepdim=True)) * torch.rsqrt(y.var(-1, correction=0, keepdim=True) + 1e-5)
+        return y.reshape(n, -1) * W[name + "_norm_weight"] + W[name + "_norm_bias"]
+
+    silu = torch.nn.functional.silu
     for t in range(config["num_layers"]):
         W = {k.split(".", 2)[2]: v for k, v in p.items() if k.startswith(f"layers.{t}.")}
-        qkv = (x @ W["W_qkv"].T).view(n, H + 2 * Hk, D)
+        qkv = (normed(x, W, "attention") @ W["W_qkv"].T).view(n, H + 2 * Hk, D)
         q, k, v = head(qkv[:, :H], W["q_weight"]), head(qkv[:, H:H + Hk], W["k_weight"]), qkv[:, H + Hk:]
         k, v = k.repeat_interleave(H // Hk, 1), v.repeat_interleave(H // Hk, 1)
         out = []
@@ -213,5 +222,9 @@ def attention_like_node_energy(params: dict, config: dict, positions, cell, elem
             s = torch.einsum("ihd,jhd->hij", q[a:a + m], k[a:a + m]) / math.sqrt(D)
             out.append(torch.einsum("hij,jhd->ihd", s.softmax(-1), v[a:a + m]))
         x = x + torch.cat(out).reshape(n, H * D) @ W["W_o"].T
-        x = x + torch.nn.functional.silu(x @ W["W_1"].T) @ W["W_2"].T
+        y = normed(x, W, "feed_forward")
+        if "W_gate" in W:
+            x = x + (silu(y @ W["W_gate"].T) * (y @ W["W_up"].T)) @ W["W_down"].T
+        else:
+            x = x + silu(y @ W["W_1"].T) @ W["W_2"].T
     return p["e0"][elem] + (x * p["wr"]).sum(1)
