@@ -17,14 +17,10 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTileValues = 64;  // of a thread's registers
-#ifndef FEW
-#define FEW 1024
-#endif
-#ifndef NRBACK
-#define NRBACK 1
-#endif
-constexpr int64_t kFewTiles = FEW;
+constexpr int kTileValues = 64;     // of a thread's registers: the forward pass's rows of a tile
+constexpr int kBackParts = 8;       // the backward pass's: half as many values of both inputs, up to eight times over (262 144 rows of 128,
+                                    // bf16: first read 56 us with one part, 43 with four, 42 with eight; second 43, 39, 39)
+constexpr int64_t kFewTiles = 1024; // tiles are made smaller below this number of them
 
 struct GnArgs {
   const void *x, *g;  // rows [rows, channels], row strides x_ld, g_ld; g: gradient of y
@@ -37,9 +33,11 @@ struct GnArgs {
   void *y, *gx;          // contiguous
   float *mean, *inverse;  // [rows or segments, groups]
   float *part;           // scratch (see the kernels)
+  int64_t again;         // workgroups of the second read by the numbers of the first (a multiple of 8), or 0
   int32_t merge;         // whether gn_merge_kernel merges the sums of segments of many tiles
   int32_t chunk;         // channels of a workgroup's share (whole groups)
   int32_t tile_rows, tx;  // rows of a tile, vectors of a row of the share
+  int32_t part_rows;      // backward: rows that are in registers at once
   int32_t lanes;         // rows by themselves: lanes of a group
   int32_t blocks;        // of rows, in x
   uint32_t block0;
@@ -329,8 +327,18 @@ __device__ __forceinline__ GnTile gn_tile(const GnArgs& a, int64_t number) {
   return t;
 }
 
-// Tiles of long segments, for the second read: numbers from floor(2 start / tile) on, of which such a segment owns at least as
-// many as it has tiles, and a shorter one any.
+// Tiles of long segments, for the second read, where there are few beside the tiles: those of the first read, the last one first, each on
+// the XCD that read it (workgroup w runs on XCD w % 8), whose L2 holds what was read last (65 536 rows of 320, bf16: 38 -> 35 us).
+__device__ __forceinline__ GnTile gn_long_tile(const GnArgs& a, int64_t number);
+
+__device__ __forceinline__ GnTile gn_second_tile(const GnArgs& a, int64_t number) {
+  if (!a.again) return gn_long_tile(a, number);
+  const int64_t b = number & 7, group = number >> 3;
+  return gn_tile(a, ((a.again >> 3) - 1 - group) * 8 + b);
+}
+
+// Where there are many: numbers from floor(2 start / tile) on, of which such a segment owns at least as many as it has tiles, and
+// a shorter one any.
 __device__ __forceinline__ GnTile gn_long_tile(const GnArgs& a, int64_t number) {
   GnTile t;
   const auto num = [&](int i) { return 2 * attn_start(a.off, a.segments, a.rows, i) / a.tile_rows; };
@@ -587,7 +595,7 @@ template <typename T, int V, int NV, int NR>
 __global__ void __launch_bounds__(kThreads) gn_apply_kernel(GnArgs a) {
   extern __shared__ float lds[];  // [2, groups of the share]
   const GnPlace<V, NV> p(a);
-  const GnTile t = gn_long_tile(a, (int64_t)blockIdx.x + a.block0);
+  const GnTile t = gn_second_tile(a, (int64_t)blockIdx.x + a.block0);
   if (!t.real || t.whole || t.first >= t.rows) return;
   const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
   const int64_t row0 = t.start + t.first;
@@ -610,28 +618,39 @@ __global__ void __launch_bounds__(kThreads) gn_apply_kernel(GnArgs a) {
   write_norm<T, V, NV, NR>(a, p, x, static_cast<T*>(a.y) + row0 * a.channels, rows, mean, inverse);
 }
 
-// gx of a tile: the two means over its segment's group in s (of gz w) and q (of gz w n)
+// gx of a tile, some rows at a time: the two means over its segment's group in s (of gz w) and q (of gz w n)
 template <typename T, int V, int NV, int NR>
-__device__ __forceinline__ void write_grad(const GnArgs& a, const GnPlace<V, NV>& p, const GnRegs<T, V, NV, NR>& x,
-                                           const GnRegs<T, V, NV, NR>& gy, T* gx, int rows, const float (&mean)[NV][V],
+__device__ __forceinline__ void write_grad(const GnArgs& a, const GnPlace<V, NV>& p, int64_t row0, int rows, const float (&mean)[NV][V],
                                            const float (&inverse)[NV][V], const float (&w)[NV][V], const float (&b)[NV][V],
                                            const float (&s)[NV][V], const float (&q)[NV][V]) {
+  for (int r0 = 0; r0 < rows; r0 += a.part_rows) {
+    GnRegs<T, V, NV, NR> x, gy;
+    x.load(p, static_cast<const T*>(a.x) + (row0 + r0) * a.x_ld, a.x_ld, rows - r0);
+    gy.load(p, static_cast<const T*>(a.g) + (row0 + r0) * a.g_ld, a.g_ld, rows - r0);
+    T* gx = static_cast<T*>(a.gx) + (row0 + r0) * a.channels;
 #pragma unroll
-  for (int k = 0; k < NR; ++k)
+    for (int k = 0; k < NR; ++k)
 #pragma unroll
-    for (int n = 0; n < NV; ++n) {
-      const int row = p.y + k * p.step;
-      if (!p.has(n) || row >= rows) continue;
-      float o[V];
+      for (int n = 0; n < NV; ++n) {
+        const int row = p.y + k * p.step;
+        if (!p.has(n) || row >= rows - r0) continue;
+        float o[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
-        const float z = gy.get(k, n, i) * activation<sizeof(T) == 2>(h * w[n][i] + b[n][i], a.act).slope * w[n][i];
-        o[i] = inverse[n][i] * (z - s[n][i] - h * q[n][i]);
+        for (int i = 0; i < V; ++i) {
+          const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
+          const float z = gy.get(k, n, i) * activation<sizeof(T) == 2>(h * w[n][i] + b[n][i], a.act).slope * w[n][i];
+          o[i] = inverse[n][i] * (z - s[n][i] - h * q[n][i]);
+        }
+        raw_store<T, V>(gx + (int64_t)row * a.channels + p.c0 + p.column(n), o);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      raw_store<T, V>(gx + (int64_t)row * a.channels + p.c0 + p.column(n), o);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+  }
+}
+
+template <typename T, int V, int NV, int NR>
+__device__ __forceinline__ void write_zeros(const GnArgs& a, const GnPlace<V, NV>& p, T* to, int rows) {
+  for (int r0 = 0; r0 < rows; r0 += a.part_rows)
+    write_zero<T, V, NV, NR>(p, to + (int64_t)r0 * a.channels, a.channels, min(a.part_rows, rows - r0));
 }
 
 // First read of the backward pass. columns: [tiles, 2, channels], the channels' sums of gz n and gz; part: [tiles, groups, 2], the
@@ -649,11 +668,7 @@ __global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a, float* 
   }
   const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
   const int64_t row0 = t.start + t.first;
-  T* gx = static_cast<T*>(a.gx) + row0 * a.channels;
-  if (!t.real) return write_zero<T, V, NV, NR>(p, gx, a.channels, rows);
-  GnRegs<T, V, NV, NR> x, gy;
-  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
-  gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
+  if (!t.real) return write_zeros<T, V, NV, NR>(a, p, static_cast<T*>(a.gx) + row0 * a.channels, rows);
   float mean[NV][V], inverse[NV][V], w[NV][V], b[NV][V], gw[NV][V], gb[NV][V];
   float* of_group = lds + 2 * p.step * p.nc;
   load_share(a.mean, a.inverse, 1, (int64_t)(t.segment - 1) * a.groups + p.c0 / a.width, p.groups, of_group);
@@ -665,19 +680,24 @@ __global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a, float* 
   for (int n = 0; n < NV; ++n)
 #pragma unroll
     for (int i = 0; i < V; ++i) gw[n][i] = gb[n][i] = 0.f;
+  for (int r0 = 0; r0 < rows; r0 += a.part_rows) {
+    GnRegs<T, V, NV, NR> x, gy;
+    x.load(p, static_cast<const T*>(a.x) + (row0 + r0) * a.x_ld, a.x_ld, rows - r0);
+    gy.load(p, static_cast<const T*>(a.g) + (row0 + r0) * a.g_ld, a.g_ld, rows - r0);
 #pragma unroll
-  for (int k = 0; k < NR; ++k) {
-    const float in = p.y + k * p.step < rows ? 1.f : 0.f;
+    for (int k = 0; k < NR; ++k) {
+      const bool in = p.y + k * p.step < rows - r0;
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+      for (int n = 0; n < NV; ++n)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
-        const float z = (in != 0.f ? gy.get(k, n, i) : 0.f) * activation<sizeof(T) == 2>(h * w[n][i] + b[n][i], a.act).slope;
-        gw[n][i] += z * h;
-        gb[n][i] += z;
-      }
-    __builtin_amdgcn_sched_barrier(0);  // a row after the other: all at once took 256 registers
+        for (int i = 0; i < V; ++i) {
+          const float h = (x.get(k, n, i) - mean[n][i]) * inverse[n][i];
+          const float z = (in ? gy.get(k, n, i) : 0.f) * activation<sizeof(T) == 2>(h * w[n][i] + b[n][i], a.act).slope;
+          gw[n][i] += z * h;
+          gb[n][i] += z;
+        }
+      __builtin_amdgcn_sched_barrier(0);  // a row after the other: all at once took 256 registers
+    }
   }
   const int plane = p.step * p.nc;
   put_channels<V, NV>(p, lds, gw);
@@ -711,24 +731,17 @@ __global__ void __launch_bounds__(kThreads) gn_tile_bwd_kernel(GnArgs a, float* 
       s[n][i] /= count;
       q[n][i] /= count;
     }
-  // read again, from the cache: kept over the sums, with what was formed of them, they took a hundred registers
-  asm volatile("" : : : "memory");
-  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
-  gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
-  write_grad<T, V, NV, NR>(a, p, x, gy, gx, rows, mean, inverse, w, b, s, q);
+  write_grad<T, V, NV, NR>(a, p, row0, rows, mean, inverse, w, b, s, q);
 }
 
 template <typename T, int V, int NV, int NR>
 __global__ void __launch_bounds__(kThreads) gn_apply_bwd_kernel(GnArgs a, const float* means) {
   extern __shared__ float lds[];  // [4, groups of the share]
   const GnPlace<V, NV> p(a);
-  const GnTile t = gn_long_tile(a, (int64_t)blockIdx.x + a.block0);
+  const GnTile t = gn_second_tile(a, (int64_t)blockIdx.x + a.block0);
   if (!t.real || t.whole || t.first >= t.rows) return;
   const int rows = (int)(t.rows - t.first < a.tile_rows ? t.rows - t.first : a.tile_rows);
   const int64_t row0 = t.start + t.first;
-  GnRegs<T, V, NV, NR> x, gy;
-  x.load(p, static_cast<const T*>(a.x) + row0 * a.x_ld, a.x_ld, rows);
-  gy.load(p, static_cast<const T*>(a.g) + row0 * a.g_ld, a.g_ld, rows);
   float mean[NV][V], inverse[NV][V], w[NV][V], b[NV][V], s[NV][V], q[NV][V];
   const int g0 = p.c0 / a.width;
   const int64_t at = (int64_t)(t.segment - 1) * a.groups + g0;
@@ -743,7 +756,7 @@ __global__ void __launch_bounds__(kThreads) gn_apply_bwd_kernel(GnArgs a, const 
   spread<V, NV>(p, lds + 3 * p.groups, inverse);
   spread_param<T, V, NV>(p, a.weight, 1.f, w);
   spread_param<T, V, NV>(p, a.bias, 0.f, b);
-  write_grad<T, V, NV, NR>(a, p, x, gy, static_cast<T*>(a.gx) + row0 * a.channels, rows, mean, inverse, w, b, s, q);
+  write_grad<T, V, NV, NR>(a, p, row0, rows, mean, inverse, w, b, s, q);
 }
 
 // ---------------------------------------------------------------------------------------- host
@@ -831,7 +844,7 @@ int with_rows(const RowShape& s, const Fn& fn) {
 
 // Segments: a workgroup's share of the channels, whole groups of them; its tile's rows
 struct TileShape {
-  int v, nv, nr, chunk, tx, rows, chunks, lds;
+  int v, nv, nr, chunk, tx, rows, part_rows, chunks, lds;
 };
 
 TileShape tile_shape(const GnArgs& a, int size, bool back) {
@@ -848,14 +861,19 @@ TileShape tile_shape(const GnArgs& a, int size, bool back) {
   }
   s.tx = s.chunk / s.v;
   s.nv = s.tx > kThreads ? (s.tx + kThreads - 1) / kThreads : 1;
-  const int most = s.v == 1 ? 32 : 32 / s.v;  // registers of the wide form: 8 192 channels of a group at most
-  if (s.nv > 1) s.nv = s.nv <= most ? most : -1;
+  const int most = 32 / s.v;  // registers of the wide forms: 8 192 channels of a group at most
+  if (s.nv > 1) s.nv = s.nv <= 4 ? 4 : s.nv <= most ? most : -1;
   const int rows = s.nv > 1 ? 1 : kThreads / s.tx;
-  // of up to 64 values a thread, fewer where the tiles would not fill the card
-  s.nr = s.nv > 1 ? 2 : s.v == 1 ? 32 : kTileValues / s.v;
+  // forward: up to 64 values of a thread, all in registers; backward: 32 of each input at a time, eight times over. Fewer where the tiles
+  // would not fill the card.
+  s.nr = s.nv > 1 ? (s.v * s.nv < 16 ? 16 / (s.v * s.nv) * 2 : 2) : s.v == 1 ? 32 : kTileValues / s.v;
+  int passes = back ? kBackParts : 1;
+  if (back && s.nv == 1) s.nr /= 2;
+  while (passes > 1 && a.rows / (passes * s.nr * rows) < kFewTiles) passes /= 2;
   if (s.nv == 1)
-    for (int i = 0; i < 2 && (a.rows / (s.nr * rows) < kFewTiles || i < NRBACK * back); ++i) s.nr /= 2;
-  s.rows = s.nr * rows;
+    for (int i = back ? 1 : 0; i < 2 && a.rows / (s.nr * rows) < kFewTiles; ++i) s.nr /= 2;
+  s.part_rows = s.nr * rows;
+  s.rows = passes * s.part_rows;
   s.chunks = (a.channels + s.chunk - 1) / s.chunk;
   s.lds = ((back ? 2 : 1) * rows * s.chunk + 2 * (s.chunk / a.width)) * 4;
   return s;
@@ -864,12 +882,13 @@ TileShape tile_shape(const GnArgs& a, int size, bool back) {
 template <typename T, typename Fn>
 int with_tiles(const TileShape& s, const Fn& fn) {
 #define GN_TILE(V, NV, NR) return fn(std::integral_constant<int, V>{}, std::integral_constant<int, NV>{}, std::integral_constant<int, NR>{})
-#define GN_TILES(V, NR)                               \
+#define GN_TILES(V, NR)                                \
   if (s.v == V && s.nv == 1) {                         \
     if (s.nr == NR) GN_TILE(V, 1, NR);                 \
     if (s.nr == NR / 2) GN_TILE(V, 1, NR / 2);         \
     if (s.nr == NR / 4) GN_TILE(V, 1, NR / 4);         \
   }                                                    \
+  if (s.v == V && s.nv == 4) GN_TILE(V, 4, (V < 4 ? 8 / V : 2)); \
   if (s.v == V && s.nv == 32 / V) GN_TILE(V, 32 / V, 2)
   if constexpr (sizeof(T) == 2) { GN_TILES(8, 8); }
   GN_TILES(4, 16);
@@ -881,11 +900,14 @@ int with_tiles(const TileShape& s, const Fn& fn) {
 }
 
 int64_t tile_count(const GnArgs& a, const TileShape& s) { return a.rows / s.rows + a.segments + 2; }
+int64_t second_count(const GnArgs& a, const TileShape& s) { return a.again ? a.again : 2 * a.rows / s.rows + 1; }
 
 void set_tiles(GnArgs& a, const TileShape& s) {
   a.chunk = s.chunk;
   a.tx = s.tx;
   a.tile_rows = s.rows;
+  a.part_rows = s.part_rows;
+  a.again = a.segments <= a.rows / s.rows ? (a.rows / s.rows + a.segments + 2 + 7) / 8 * 8 : 0;
   a.merge = a.rows / s.rows * a.groups > kMergeValues && a.rows > (int64_t)kMergeTiles * s.rows;
 }
 
@@ -920,7 +942,7 @@ int norm(GnArgs a, hipStream_t stream) {
       });
       if (status) return status;
     }
-    return in_launches(a, 2 * a.rows / s.rows + 1, [&](unsigned blocks) {
+    return in_launches(a, second_count(a, s), [&](unsigned blocks) {
       gn_apply_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 2 * (s.chunk / a.width) * 4, stream>>>(a);
     });
   });
@@ -1003,7 +1025,7 @@ int norm_bwd(GnArgs a, float* work, void* gw, void* gb, hipStream_t stream) {
       });
       if (status) return status;
     }
-    return in_launches(a, 2 * a.rows / s.rows + 1, [&](unsigned blocks) {
+    return in_launches(a, second_count(a, s), [&](unsigned blocks) {
       gn_apply_bwd_kernel<T, V, NV, NR><<<dim3(blocks, s.chunks), kThreads, 4 * (s.chunk / a.width) * 4, stream>>>(a, means);
     });
   });

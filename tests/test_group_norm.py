@@ -56,7 +56,7 @@ def ragged(lengths, lead=0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("channels,groups", [(8, 1), (6, 2), (128, 8), (128, 32), (320, 32), (24, 3), (35, 7), (640, 4), (2048, 2), (4100, 1),
-                                             (3, 1), (999, 3), (1000, 1000), (2600, 1300)])
+                                             (3, 1), (999, 3), (1000, 1000), (2600, 1300), (1031, 1), (4099, 1), (1042, 1)])
 @pytest.mark.parametrize("lengths", [[5, 0, 17, 33, 9], [300], [0, 0, 700, 1, 64], [2] * 40 + [190]])
 def test_segments(channels, groups, lengths, dtype):
     """Empty segments, long ones between short ones, a tile's edge inside a segment, rows before and behind all."""
