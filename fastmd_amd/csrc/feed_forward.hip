@@ -1,6 +1,8 @@
 // The gated feed-forward block y = h Wd^T, h = act(x Wg^T) * (x Wu^T), and its gradients.
 //
-// Four or five launches, each a product of tile_product.h with what follows it as its epilogue:
+// In one of three forms, by measured times (one_kernel, direct_forward, direct_backward): one kernel each way for small weights
+// (ffn_block.h); products straight from memory to registers for few rows (direct_product.h); otherwise tiles in LDS (tile_product.h). The
+// last two are four or five launches, each a product with what follows it as its epilogue:
 //   gate, up -> h            both projections of a tile in one workgroup; the factors stay in registers and h alone is written
 //   y = h Wd^T
 //   gh = gy Wd -> dg, du     dg = gh u act'(g), du = gh act(g)
@@ -9,6 +11,10 @@
 // The backward pass takes g and u from the forward in float32: in bf16 their rounding alone would leave dg and du two roundings off,
 // and gx with them. h, dg and du are rounded to bf16 once, as operands of the next product (float32: split into three planes),
 // so that a bf16 result has the error of two roundings, its own and its operand's.
+//
+// Bound by the matrix cores from some hundred rows on, by reading the weights below. bf16, 8 192 rows of 2 048 x 5 504: projections
+// 430 us (860 TFLOP/s), y 170 (1 090), dg and du 320 (580: their epilogue moves 553 MB besides), gx 323 (1 140), weights 503 (1 100).
+// float32 (six bf16 products a multiply-add), 16 875 rows of 256 x 680, all gradients: 577 us (92 TFLOP/s). bf16, 16 rows of 2 048 x 5 504: 28 us.
 #include "ffn_block.h"
 
 namespace {
@@ -27,10 +33,12 @@ struct LayJob {
 };
 
 constexpr int kLayJobs = 5;
+constexpr int64_t kMostBlocks = 1 << 22;
 
 struct LayArgs {
   LayJob job[kLayJobs];
-  int32_t count, blocks;
+  int32_t count;
+  uint32_t block0;  // first workgroup of this launch
 };
 
 template <bool F32>
@@ -38,9 +46,9 @@ __global__ void __launch_bounds__(256) ffn_lay_kernel(LayArgs a) {
   int n = 0;
 #pragma unroll
   for (int i = 1; i < kLayJobs; ++i)
-    if (i < a.count && blockIdx.x >= a.job[i].first) n = i;
+    if (i < a.count && a.block0 + blockIdx.x >= a.job[i].first) n = i;
   const LayJob& j = a.job[n];
-  const int64_t chunks = j.ld / 8, i = (int64_t)(blockIdx.x - j.first) * 256 + threadIdx.x;
+  const int64_t chunks = j.ld / 8, i = (int64_t)(a.block0 + blockIdx.x - j.first) * 256 + threadIdx.x;
   if (i >= j.rows * chunks) return;
   const int64_t row = i / chunks, col = (i - row * chunks) * 8;
   const bool whole = j.wide && col + 8 <= j.cols;
@@ -265,13 +273,16 @@ struct Layer {
     return {dst, wide, rows * wide};
   }
   int launch(const Ffn& f, hipStream_t stream) {
-    if (!blocks) return FMD_OK;
-    FMD_REQUIRE(blocks < (int64_t(1) << 23));
-    if (f.bf16)
-      ffn_lay_kernel<false><<<(unsigned)blocks, 256, 0, stream>>>(args);
-    else
-      ffn_lay_kernel<true><<<(unsigned)blocks, 256, 0, stream>>>(args);
-    FMD_CHECK_LAUNCH();
+    FMD_REQUIRE(blocks < (int64_t(1) << 32));
+    for (int64_t first = 0; first < blocks; first += kMostBlocks) {  // a launch takes fewer than 2^32 threads
+      const unsigned n = (unsigned)(blocks - first < kMostBlocks ? blocks - first : kMostBlocks);
+      args.block0 = (uint32_t)first;
+      if (f.bf16)
+        ffn_lay_kernel<false><<<n, 256, 0, stream>>>(args);
+      else
+        ffn_lay_kernel<true><<<n, 256, 0, stream>>>(args);
+      FMD_CHECK_LAUNCH();
+    }
     return FMD_OK;
   }
 };
@@ -336,13 +347,15 @@ bool one_kernel(const Ffn& f) {
 }
 
 template <typename T, bool BACK>
-int block(const Ffn& f, const FfnBlock& a, hipStream_t stream) {
+int block(const Ffn& f, FfnBlock a, hipStream_t stream) {
   const auto launch = [&](auto mt) {
     constexpr int MT = decltype(mt)::value;
-    const int64_t blocks = fmd_cdiv(f.rows, 16 * MT);
-    FMD_REQUIRE(blocks < (int64_t(1) << 22));
-    ffn_block_kernel<T, MT, BACK><<<(unsigned)blocks, kBlockThreads, block_lds((int)f.hidden, f.planes(), 16 * MT, BACK), stream>>>(a);
-    FMD_CHECK_LAUNCH();
+    for (a.row0 = 0; a.row0 < f.rows; a.row0 += kMostBlocks * 16 * MT) {
+      const int64_t left = fmd_cdiv(f.rows - a.row0, 16 * MT);
+      ffn_block_kernel<T, MT, BACK><<<(unsigned)(left < kMostBlocks ? left : kMostBlocks), kBlockThreads,
+                                      block_lds((int)f.hidden, f.planes(), 16 * MT, BACK), stream>>>(a);
+      FMD_CHECK_LAUNCH();
+    }
     return (int)FMD_OK;
   };
   // 32 rows of a workgroup where those fill the card
@@ -368,7 +381,7 @@ int straight(const Ffn& f, const DpArgs& a, const Epi& epi, hipStream_t stream) 
 FfnBlock block_args(const Ffn& f, const Forward& io, const void* gy, int64_t gy_ld, void* result) {
   return {io.x, io.gate, io.up, io.down, gy, io.x_ld, io.gate_ld, io.down_ld, gy_ld, wide_rows(f, io.x, io.x_ld, f.width),
           wide_rows(f, io.gate, io.gate_ld, f.width) && wide_rows(f, io.up, io.gate_ld, f.width), wide_rows(f, io.down, io.down_ld, f.hidden),
-          wide_rows(f, gy, gy_ld, f.out), f.rows, (int32_t)f.width, (int32_t)f.hidden, (int32_t)f.out, f.act, result, nullptr, nullptr, f.hp()};
+          wide_rows(f, gy, gy_ld, f.out), f.rows, (int32_t)f.width, (int32_t)f.hidden, (int32_t)f.out, f.act, result, nullptr, nullptr, f.hp(), 0};
 }
 
 int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t stream, int64_t* size) {

@@ -18,6 +18,7 @@ struct FfnBlock {
   void* result;     // y [rows, out], or gx [rows, width] (nullable), contiguous
   __bf16 *h, *d;    // backward, nullable: [planes, rows, hp], [planes, 2, rows, hp]
   int64_t hp;
+  int64_t row0;     // first row of this launch
 };
 
 constexpr int kBlockWaves = 8, kBlockThreads = 64 * kBlockWaves;
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(kBlockThreads) ffn_block_kernel(FfnBlock a) {
   __bf16* lds = reinterpret_cast<__bf16*>(block_lds_space);  // [BACK ? dg, du : h][planes][ROWS][ld]
   const int ld = block_ld(a.hidden), plane = ROWS * ld;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.x * ROWS;
+  const int64_t m0 = a.row0 + (int64_t)blockIdx.x * ROWS;
   const DpOperand ox{{a.x, a.x}, a.x_ld, 0, a.x_wide}, og{{a.gy, a.gy}, a.gy_ld, 0, a.gy_wide};
   const DpOperand ow{{a.gate, a.up}, a.w_ld, 0, a.w_wide}, od{{a.down, a.down}, a.d_ld, 0, a.d_wide};
 

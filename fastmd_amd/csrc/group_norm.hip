@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kThreads) gn_tile_kernel(GnArgs a) {
 
 // Each workgroup of the second read merges the sums of its segment's tiles itself where all tiles' together are few (kMergeValues);
 // otherwise those of a segment of more than kMergeTiles tiles are merged once, by gn_merge_kernel: 33 tiles of 8 groups each 48 us with
-// a launch for it, 41 without (16 875 rows of 128, float32, with VJP); 85 tiles of 32 groups 80 us by each workgroup, 38 by the launch.
+// a launch for it, 47 without (16 875 rows of 128, float32, with VJP); 85 tiles of 32 groups 80 us by each workgroup, 38 by the launch.
 constexpr int kMergeTiles = 16;
 constexpr int64_t kMergeValues = 8192;
 

@@ -53,7 +53,7 @@ __device__ __forceinline__ void put_part(int8_t* q, const Eight& x, float scale)
 }
 
 // A wave or (LANES 256) a workgroup a row, in registers: NV vectors of eight a lane; NV 0: read twice, whatever its width. 8 192 rows
-// of 4 096, bf16: 71 us with a value at a time, 26 so (3.9 TB/s).
+// of 4 096, bf16: 71 us with a value at a time, 31 so (3.2 TB/s).
 template <typename T, int LANES, int NV>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(RowArgs a) {
   __shared__ float lds[4];
@@ -168,8 +168,6 @@ struct ScaleEpi {
   }
 };
 
-constexpr double kDirectInt8 = 5e8;
-
 typedef TpShape<TpInt8, 2, 4, 4, 2, false, false, false, 2> Large;
 typedef TpShape<TpInt8, 2, 2, 2, 2, false, false, false, 2> Middle;
 typedef TpShape<TpInt8, 1, 2, 2, 1, false, false, false, 2> Small;
@@ -213,8 +211,14 @@ int64_t rounded_size(int64_t rows, int64_t width) {
   return ((rows * ld + 255) & ~int64_t(255)) + ((rows * 4 + 255) & ~int64_t(255));
 }
 
-// Few rows, or a small product: straight from memory (direct_product.h), with nothing to join.
-bool few_rows(int64_t rows, int64_t width, int64_t out) { return rows <= 64 || (double)rows * width * out <= kDirectInt8; }
+// A small product with small weights: straight from memory (direct_product.h), with nothing to join. us of rounding and product
+// in graphs, tiles and straight: 16 rows of 1 024 x 1 024 12.8 12.0, of 2 048 x 2 048 15.5 12.1, of 4 096 x 4 096 16.9 18.2 (eagerly, weights not
+// in caches, 18.5 16.8), of 8 192 x 8 192 26.4 37.4; one of 11 008 x 4 096 24.0 30.2; 64 of 2 048 x 2 048 16.8 12.7, of 4 096 x 4 096 17.2 19.6;
+// 128 of 1 024 x 1 024 14.1 11.4; 500 of 1 024 x 1 024 14.9 14.3; 2 000 of 512 x 512 12.5 14.3, of 1 024 x 1 024 17.6 28.2.
+bool few_rows(int64_t rows, int64_t width, int64_t out) {
+  if (fmd_cdiv(rows, 16) * fmd_cdiv(out, 16) >= int64_t(1) << 22) return false;  // one launch
+  return (double)rows * width * out <= 4e8 && (double)width * out <= 2.5e7;
+}
 
 int product(const int8_t* x, int64_t x_ld, const int8_t* w, int64_t w_ld, int64_t rows, int64_t width, int64_t out, const ScaleEpi& epi,
             void* work, hipStream_t stream) {

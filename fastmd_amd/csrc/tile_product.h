@@ -1,8 +1,8 @@
 // Products out[m, n] = sum_k n_op[n, k] m_op[m, k] on the matrix cores, with the result's own use as an epilogue: what the
 // gated feed-forward block and the 8-bit product are made of.
 //
-// Both operands of a slice of K are copied straight from global memory into LDS (no register stage), into four places in turn: while
-// the matrix instructions run on one slice, three are on their way. An operand is stored along K (its rows are rows of the product, K
+// Both operands of a slice of K are copied straight from global memory into LDS (no register stage), into two places in turn: while
+// the matrix instructions run on one slice, the next is on its way. An operand is stored along K (its rows are rows of the product, K
 // contiguous) or across it (its rows are K, as a weight is in the products of the backward pass); the second kind is
 // transposed by the LDS reads (ds_read_b64_tr_b16), never in memory. The n operand is the matrix instruction's first: a
 // lane's four consecutive results then lie side by side in a row of the output.
@@ -67,7 +67,9 @@ struct TpInt8 {
 // four chunks of four consecutive rows of K (across).
 constexpr int kTpSlice = 128;  // bytes of K in a slice
 constexpr int kTpSteps = kTpSlice / 32, kTpRow = kTpSlice / 16;  // steps of the matrix instructions, chunks of a row
-constexpr int kTpPlaces = 256 / kTpSlice;
+// Two places: four of half a slice each (four chunks a row: half lines of memory, twice the barriers) took 202 us for 8 192 x 2 048 over
+// K = 5 504, bf16, against 186, and 480 us against 296 in tiles of 64 x 64.
+constexpr int kTpPlaces = 2;
 
 template <int ROWS, bool ACROSS_, bool GATED, int THREADS>
 struct TpStage {
@@ -77,7 +79,7 @@ struct TpStage {
   static_assert(BYTES % (16 * THREADS) == 0, "whole passes");
   static_assert(!(ACROSS && GATED), "a gated product's weights lie along K");
 
-  __device__ static __forceinline__ int swap_along(int row) { return kTpRow == 4 ? (row >> 2) & 3 : (row & 7) ^ ((row >> 3) & 1); }
+  __device__ static __forceinline__ int swap_along(int row) { return (row & 7) ^ ((row >> 3) & 1); }
   __device__ static __forceinline__ int swap_across(int row) { return CHUNKS >= 16 ? (row & 3) << 2 : ((row >> 1) & 1) << 2; }
 
   uint32_t off[LOADS];
@@ -124,7 +126,7 @@ struct TpStage {
     const int n = wave * LOADS + j;
     const char* base = GATED && n * (64 / kTpRow) >= ROWS / 2 ? at[GATED ? 1 : 0] : at[0];
     const tp_u32x4 buffer = {(uint32_t)(uintptr_t)base, (uint32_t)((uintptr_t)base >> 32) & 0xffff, 0x80000000u, 0x00027000u};
-    const int mine = ACROSS ? k : kTpRow == 8 ? k ^ (16 * (n & 1)) : k, rest = ACROSS ? left - n * (64 / CHUNKS) * 2 : left;
+    const int mine = ACROSS ? k : k ^ (16 * (n & 1)), rest = ACROSS ? left - n * (64 / CHUNKS) * 2 : left;
     const uint32_t from = mine < rest ? off[j] : 0xffffffffu;
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :
@@ -317,8 +319,10 @@ tile_product_kernel(TpArgs a, Epi epi) {
   auto slice = [&](char* st, char* following) {
 #pragma unroll
     for (int kk = 0; kk + 1 < kTpSteps; ++kk) step(kk, st, kk + 1, false, nullptr);
+    asm volatile("" : : : "memory");
     __builtin_amdgcn_s_waitcnt(tp_wait((kTpPlaces - 2) * COPIES, 0));  // of the slices on their way the first has landed
     __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
     step(kTpSteps - 1, following, 0, true, st);
     copied();
   };
@@ -332,6 +336,7 @@ tile_product_kernel(TpArgs a, Epi epi) {
   }
   __builtin_amdgcn_s_waitcnt(tp_wait((kTpPlaces - 1) * COPIES, 15));
   __builtin_amdgcn_s_barrier();
+  asm volatile("" : : : "memory");
 #pragma unroll
   for (int r = 0; r < READS; ++r) read_one(lds, 0, 0, r);
   for (int s = begin; s < end; s += kTpPlaces)
@@ -369,7 +374,8 @@ tile_product_kernel(TpArgs a, Epi epi) {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<Four*>(mine + (r * CHUNKS + ((i * 8 + 2 * q + (lane >> 5)) ^ (r & (CHUNKS - 1)))) * 16) = tp_four(acc[i][j], q);
-    // what the epilogue reads of memory is asked for some rows ahead of its results
+    // What the epilogue reads of memory is asked for some rows ahead of its results: four, or two where four would not fit the registers
+    // beside a large tile's sums (they spilt).
     constexpr int AHEAD = S::BN >= 256 && sizeof(typename Epi::Fetch) > 16 ? 2 : 4;
     static_assert(32 * EACH % (64 * AHEAD) == 0, "whole groups");
     for (int k0 = lane; k0 < 32 * EACH; k0 += 64 * AHEAD) {
@@ -434,7 +440,9 @@ struct TpPlan {
   float time;       // estimate, us
 };
 
-// A shape's measured times (us): of a slice, alone on a CU and by each workgroup of a full one, and of a tile's begin and end.
+// A shape's measured times (us): of a slice, alone on a CU and by each workgroup of a full one, and of a tile's begin and end. (Fitted to
+// products of 16 to 16 875 rows: with tiles chosen by their count alone the float32 block of 16 875 rows of 256 x 680, all gradients, took
+// 750 us, by these 571.)
 template <typename S>
 struct TpTimes {
   static constexpr bool LARGE = S::BN * S::BM >= 65536, SMALL = S::BN * S::BM <= 4096;

@@ -30,6 +30,7 @@ from fastmd_amd._device import on_device_of, require_cuda, rows_view, stream
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 MAX_WIDTH = 2 ** 22 - 8
+MAX_ROWS, MAX_VALUES = 2 ** 29, 2 ** 36  # of 2^21 tiles
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -56,8 +57,10 @@ def _refuse(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor) -> None:
                          f"{tuple(w_down.shape)} do not fit together")
     if not (1 <= width <= MAX_WIDTH and 1 <= hidden <= MAX_WIDTH and 1 <= w_down.shape[0] <= MAX_WIDTH):
         raise ValueError(f"the widths must be from 1 to {MAX_WIDTH}")
-    if x.shape[0] >= 2 ** 31:
-        raise ValueError("the feed-forward block takes fewer than 2^31 rows")
+    rows, widest = x.shape[0], max(width, hidden, w_down.shape[0])
+    if rows >= MAX_ROWS or max(rows, width, hidden, w_down.shape[0]) * widest >= MAX_VALUES:
+        raise ValueError(f"the feed-forward block takes fewer than 2^29 rows, and 2^36 values of a matrix, got {rows} rows, "
+                         f"widths {width}, {hidden} and {w_down.shape[0]}")
 
 
 def _check(x, w_gate, w_up, w_down, activation) -> int:
@@ -69,7 +72,8 @@ def _check(x, w_gate, w_up, w_down, activation) -> int:
             and w_down.dtype is dtype and len(w_gate.shape) == 2 and w_gate.shape == w_up.shape
             and len(w_down.shape) == 2 and w_gate.shape[1] == shape[1] and w_down.shape[1] == w_gate.shape[0]
             and 1 <= shape[1] <= MAX_WIDTH and 1 <= w_gate.shape[0] <= MAX_WIDTH
-            and 1 <= w_down.shape[0] <= MAX_WIDTH and shape[0] < 2 ** 31):
+            and 1 <= w_down.shape[0] <= MAX_WIDTH and shape[0] < MAX_ROWS
+            and max(shape[0], shape[1], w_down.shape[0], w_down.shape[1]) * max(shape[1], *w_down.shape) < MAX_VALUES):
         _refuse(x, w_gate, w_up, w_down)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")

@@ -29,6 +29,7 @@ from fastmd_amd._device import on_device_of, require_cuda, rows_view, stream
 from fastmd_amd.ops.feed_forward import ACTIVATIONS
 
 MAX_GROUP = 8192  # channels of a group
+MAX_GROUPS = 65535
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
@@ -52,6 +53,8 @@ def _check(x: Tensor, groups: int, weight, bias, offsets, activation) -> int:
         raise ValueError(f"the channels must be a multiple of the groups, got {channels} and {groups}")
     if channels // groups > MAX_GROUP or channels >= 2 ** 24:
         raise ValueError(f"a group has at most {MAX_GROUP} channels, all fewer than 2^24, got {channels // groups} and {channels}")
+    if groups > MAX_GROUPS:
+        raise ValueError(f"at most {MAX_GROUPS} groups, got {groups}")
     for name, p in (("weight", weight), ("bias", bias)):
         if p is not None and (p.shape != (channels,) or p.dtype != x.dtype):
             raise ValueError(f"{name} must be {x.dtype} [{channels}], got {p.dtype} {tuple(p.shape)}")

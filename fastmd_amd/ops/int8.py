@@ -111,8 +111,8 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = No
     (rows, width), out, device = values.shape, weight.values.shape[0], values.device
     if weight.values.shape[1] != width or not 1 <= width <= MAX_WIDTH:
         raise ValueError(f"x and weight must have one width, from 1 to {MAX_WIDTH}, got {width} and {weight.values.shape[1]}")
-    if rows >= 2 ** 31 or out >= 2 ** 31:
-        raise ValueError("linear_int8 takes fewer than 2^31 rows and channels")
+    if rows >= 2 ** 29 or out >= 2 ** 29 or rows * out >= 2 ** 36:
+        raise ValueError(f"linear_int8 takes fewer than 2^29 rows and channels, and 2^36 results, got {rows} and {out}")
     if bias is not None:
         if bias.shape != (out,) or bias.dtype != torch.float32:
             raise ValueError(f"bias must be float32 [{out}], got {bias.dtype} {tuple(bias.shape)}")

@@ -313,6 +313,7 @@ def test_refusals():
         (lambda: gated_feed_forward(x[:, :0], wg[:, :0], wu[:, :0], wd), "from 1"),
         (lambda: gated_feed_forward(x, wg[:0], wu[:0], wd[:, :0]), "from 1"),
         (lambda: gated_feed_forward(x, wg, wu, wd, activation="tanh"), "activation"),
+        (lambda: gated_feed_forward(x[:1].expand(2 ** 29, 24), wg, wu, wd), "fewer than 2\\^29 rows"),
         (lambda: gated_feed_forward_vjp(gy[:, :8], x, wg, wu, wd, saved), "gy"),
         (lambda: gated_feed_forward_vjp(gy.bfloat16(), x, wg, wu, wd, saved), "gy"),
         (lambda: gated_feed_forward_vjp(gy, x[:4], wg, wu, wd, saved), "gy"),

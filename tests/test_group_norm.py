@@ -307,6 +307,7 @@ def test_refusals():
         (lambda: group_norm(x, 0), "multiple of the groups"),
         (lambda: group_norm(x, 48), "multiple of the groups"),
         (lambda: group_norm(torch.zeros(2, 8200, device="cuda"), 1), "at most"),
+        (lambda: group_norm(torch.zeros(2, 65536, device="cuda"), 65536), "at most 65535 groups"),
         (lambda: group_norm(x, 3, w[:20]), "weight"),
         (lambda: group_norm(x, 3, w, b.bfloat16()), "bias"),
         (lambda: group_norm(x, 3, offsets=off.float()), "offsets"),

@@ -149,6 +149,7 @@ def test_nothing_to_do_and_refusals():
         (lambda: linear_int8(x, w.values), "Int8Rows"),
         (lambda: linear_int8(x.clone().requires_grad_(), w), "no gradient"),
         (lambda: linear_int8(x[:, :31], w), "one width"),
+        (lambda: linear_int8(x[:1].expand(2 ** 29, 32), w), "fewer than 2\\^29 rows"),
         (lambda: linear_int8(x, Int8Rows(w.values.short(), w.scales)), "weight must be int8"),
         (lambda: linear_int8(x, Int8Rows(w.values, w.scales[:5])), "weight must be int8"),
         (lambda: linear_int8(x, Int8Rows(w.values, w.scales.double())), "weight must be int8"),
