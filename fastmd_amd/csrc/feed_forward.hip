@@ -555,7 +555,8 @@ int fmd_gated_ffn(int32_t bf16, int32_t act, int32_t lay, const void* x, int64_t
   FMD_REQUIRE(sizes_fit(f) && layouts_fit(f, io) && x && gate && up && down && y);
   int64_t size = 0;
   Space none{nullptr}, s{static_cast<char*>(work)};
-  forward(f, io, none, false, nullptr, &size);
+  const int status = forward(f, io, none, false, nullptr, &size);
+  if (status) return status;  // before anything is laid out
   FMD_REQUIRE(work || !size);
   return forward(f, io, s, true, stream, nullptr);
 }
@@ -590,7 +591,8 @@ int fmd_gated_ffn_bwd(int32_t bf16, int32_t act, int32_t lay, const void* x, int
   FMD_REQUIRE(!g_gate || (g_up && g_down && (hidden_in || one_kernel(f))));
   int64_t size = 0;
   Space none{nullptr}, s{static_cast<char*>(work)};
-  backward(f, io, gx != nullptr, g_gate != nullptr, none, false, nullptr, &size);
+  const int status = backward(f, io, gx != nullptr, g_gate != nullptr, none, false, nullptr, &size);
+  if (status) return status;
   FMD_REQUIRE(work || !size);
   return backward(f, io, gx != nullptr, g_gate != nullptr, s, true, stream, nullptr);
 }

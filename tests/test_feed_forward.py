@@ -331,3 +331,16 @@ def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 8)
     with pytest.raises(ValueError, match="GPU"):
         gated_feed_forward(x, torch.zeros(4, 8), torch.zeros(4, 8), torch.zeros(8, 4))
+
+
+def test_entry_points_refuse_more_tiles_than_a_launch_takes():
+    """Before anything is launched: the operands' layouts would go to a workspace that is not there."""
+    from fastmd_amd import _abi
+
+    lib = _abi.load()
+    rows, width, hidden, out = 2 ** 31 - 1, 64, 2048, 64
+    for bf16 in (0, 1):
+        assert lib.fmd_gated_ffn(bf16, 1, 15, 16, width, 16, 16, width, 16, hidden, rows, width, hidden, out, 16, None, None, None,
+                                 None) == 10001
+        assert lib.fmd_gated_ffn_bwd(bf16, 1, 15, 16, width, 16, 16, width, 16, hidden, rows, width, hidden, out, 16, out, 16, 16,
+                                     16, 16, 16, 16, None, None) == 10001

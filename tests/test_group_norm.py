@@ -71,6 +71,14 @@ def test_segments(channels, groups, lengths, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels,groups", [(8192, 1), (16384, 2), (8191, 1), (3 * 8190, 3)])
+def test_segments_of_the_widest_groups(channels, groups, dtype):
+    x, w, b, gy = make(12, channels, dtype)
+    check(x, groups, w, b, gy, ragged([5, 0, 1, 6]), "silu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("segments", [1, 3, 40])
 def test_long_segments(segments, dtype):
     """Sums joined over many tiles; a mean that is large beside the spread."""
@@ -330,3 +338,22 @@ def test_cpu_tensors_are_refused():
 
     with pytest.raises(ValueError, match="GPU"):
         group_norm(torch.zeros(2, 8), 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offsets", [[0, 300, 100, 400], [400, 0, 400], [399, -5, 700, 2, 400], [400, 300, 200, 0], [0, 9000, 40, 9000]])
+def test_descending_offsets_stay_in_bounds(offsets, dtype):
+    """Such a call ends, and the inputs keep their values (which rows it computes is open)."""
+    from fastmd_amd.ops.group_norm import group_norm_forward, group_norm_vjp
+
+    rows = max(max(offsets) - 300 if 700 in offsets else max(offsets), 400)
+    x, w, b, gy = (t.cuda() for t in make(rows, 32, dtype))
+    kept = [t.clone() for t in (x, w, b, gy)]
+    off = torch.tensor(offsets, device="cuda")
+    for groups in (1, 32):
+        _, saved = group_norm_forward(x, groups, w, b, offsets=off)
+        group_norm_vjp(gy, x, groups, w, b, saved, offsets=off)
+    torch.cuda.synchronize()
+    for a, k in zip((x, w, b, gy), kept):
+        assert torch.equal(a, k)
