@@ -324,17 +324,18 @@ struct Forward {
 };
 
 // Whether the products of a pass go straight from memory to registers (direct_product.h) or through tiles in LDS: by the multiply-adds
-// of the forward pass, where the two forms' times meet. us of the forward pass and of the VJP for x, tiles and straight: float32, 10 000 rows of
-// 64 x 256 36 35, 44 46; 2 000 of 256 x 680 48 47, 58 52; 500 of 512 x 1 376 53 44, 67 52; 64 of 1 024 x 2 736 58 46, 62 75; 16 of
-// 2 048 x 5 504 148 58, 155 79. bf16, 2 000 rows of 128 x 344 14 12, 19 15; 10 000 of 64 x 256 16 22, 21 28; 135 of 512 x 1 376 18 17,
-// 23 26; 16 of 2 048 x 5 504 34 30, 36 56 (its VJP reads weights across their rows, two bytes a lane).
+// of the forward pass, where the two forms' times meet. us of the forward pass and of the VJP for x, tiles and straight, float32: 300 rows of
+// 256 x 680 33 21, 45 31; 2 000 of 256 x 680 48 53, 57 73; 130 of 512 x 1 376 44 31, 48 45; 200 49 41, 49 53; 500 54 59, 67 61; 32 of
+// 1 024 x 2 736 57 31, 61 50; 64 58 46, 62 74; 200 of 768 x 2 048 59 55, 65 75; 400 73 95, 89 132. bf16: 135 rows of 256 x 680 15.7 10.0,
+// 18.2 15.0; 300 16.0 13.3, 20.0 22.3; 500 16.5 13.8, 24.5 18.1; 1 000 17.5 20.7, 25.2 32.1; 16 of 512 x 1 376 16.8 10.0, 18.0 15.5; 64 18.1 11.4, 20.7 22.7; 200 21.4 21.9,
+// 23.9 31.7; 16 of 2 048 x 5 504 34 30, 36 56 (the VJP reads weights across their rows, two bytes a lane).
 bool direct_forward(const Ffn& f) {
   const double work = (double)f.rows * f.hidden * (2 * f.width + f.out);
-  return f.bf16 ? work <= 5.5e8 : work <= 1.1e9 || f.rows <= 64;
+  return f.bf16 ? work <= 2.7e8 || (f.rows <= 32 && work <= 5.5e8) : work <= 9.5e8 || f.rows <= 64;
 }
 bool direct_backward(const Ffn& f) {
   const double weights = (double)f.hidden * (2 * f.width + f.out), work = weights * f.rows;
-  return f.bf16 ? work <= 2.7e8 && weights <= 2.2e6 : work <= 5e8 || f.rows <= 32;
+  return f.bf16 ? work <= 1.2e8 && weights <= 2.2e6 : work <= 3e8 || f.rows <= 32;
 }
 
 // Whether the whole block is one kernel: its hidden layer (in the backward pass the two gradients of it) fits LDS for 16 rows, and the
