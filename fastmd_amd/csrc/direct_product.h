@@ -4,7 +4,8 @@
 // product and join do.
 //
 // A wave has 16 columns n and 16 MT rows m. Its workgroup's other waves have the next columns (WK 1), or the same ones and
-// another part of K each; their sums are then added in order. float32 is split into its three bf16 planes (x3.h) in registers.
+// another part of K each; their sums are then added in order. float32 is split into its three bf16 planes (x3.h) in registers; an m that an
+// earlier product left in planes (float32 three, bf16 two) is read so.
 #pragma once
 
 #include <type_traits>
@@ -32,21 +33,22 @@ struct DpType {  // bf16 and float32: bf16 products
   typedef dp_f32x4 Acc;
   typedef float4 Four;
   static constexpr int PLANES = sizeof(T) == 4 ? 3 : 1, UNIT = 32, EACH = 8;  // K of a product, values of a lane
+  static constexpr int KEPT = sizeof(T) == 4 ? 3 : 2;                         // planes of what is kept between two products
 };
 template <>
 struct DpType<int8_t> {
   typedef int Acc __attribute__((ext_vector_type(4)));
   typedef int4 Four;
-  static constexpr int PLANES = 1, UNIT = 64, EACH = 16;
+  static constexpr int PLANES = 1, UNIT = 64, EACH = 16, KEPT = 1;
 };
 
 // A lane's values of one row (or, across, of one column) as they lie in memory, and as operands. T: float, __bf16, int8_t.
-// SPLIT: float32 that is kept as three planes of bf16.
+// SPLIT: what is kept in planes of bf16.
 template <typename T, bool ACROSS, bool SPLIT>
 struct DpLoad {
   static constexpr int EACH = DpType<T>::EACH;
   typedef typename std::conditional<SPLIT, __bf16, T>::type Stored;
-  static constexpr int VECTORS = SPLIT ? 3 : sizeof(T) == 4 ? 2 : 1;
+  static constexpr int VECTORS = SPLIT ? DpType<T>::KEPT : sizeof(T) == 4 ? 2 : 1, PLANES = SPLIT ? DpType<T>::KEPT : DpType<T>::PLANES;
   tp_i32x4 v[VECTORS];
 
   // values k .. k + EACH - 1 of row `row`; past `most` is zero
@@ -64,7 +66,7 @@ struct DpLoad {
       __builtin_memcpy(v, e, sizeof(e));
     } else if (SPLIT) {  // always whole vectors, zero past K
 #pragma unroll
-      for (int p = 0; p < 3; ++p) v[p] = *reinterpret_cast<const tp_i32x4*>(x + p * o.plane + row * o.ld + k);
+      for (int p = 0; p < VECTORS; ++p) v[p] = *reinterpret_cast<const tp_i32x4*>(x + p * o.plane + row * o.ld + k);
     } else if (o.wide) {
 #pragma unroll
       for (int p = 0; p < VECTORS; ++p) v[p] = reinterpret_cast<const tp_i32x4*>(x + row * o.ld + k)[p];
@@ -78,7 +80,7 @@ struct DpLoad {
     }
   }
 
-  __device__ __forceinline__ void planes(tp_i32x4 (&p)[DpType<T>::PLANES]) const {
+  __device__ __forceinline__ void planes(tp_i32x4 (&p)[PLANES]) const {
     if constexpr (sizeof(T) == 4 && !SPLIT) {
       fmd_bf16x4 lo[3], hi[3];
       x3_split(__builtin_bit_cast(float4, v[0]), lo[0], lo[1], lo[2]);
@@ -87,21 +89,21 @@ struct DpLoad {
       for (int i = 0; i < 3; ++i) p[i] = __builtin_bit_cast(tp_i32x4, __builtin_shufflevector(lo[i], hi[i], 0, 1, 2, 3, 4, 5, 6, 7));
     } else {
 #pragma unroll
-      for (int i = 0; i < DpType<T>::PLANES; ++i) p[i] = v[i];
+      for (int i = 0; i < PLANES; ++i) p[i] = v[i];
     }
   }
 };
 
-template <typename T>
-__device__ __forceinline__ typename DpType<T>::Acc dp_mma(const tp_i32x4 (&a)[DpType<T>::PLANES], const tp_i32x4 (&b)[DpType<T>::PLANES],
-                                                          typename DpType<T>::Acc c) {
+template <typename T, int NP, int MP>
+__device__ __forceinline__ typename DpType<T>::Acc dp_mma(const tp_i32x4 (&a)[NP], const tp_i32x4 (&b)[MP], typename DpType<T>::Acc c) {
   if constexpr (std::is_same<T, int8_t>::value) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a[0], b[0], c, 0, 0, 0);
   } else {
     const auto mma = [](tp_i32x4 x, tp_i32x4 y, dp_f32x4 s) {
       return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fmd_bf16x8, x), __builtin_bit_cast(fmd_bf16x8, y), s, 0, 0, 0);
     };
-    if constexpr (DpType<T>::PLANES == 3) {
+    if constexpr (NP == 1 && MP == 2) c = mma(a[0], b[1], c);
+    if constexpr (NP == 3) {
       c = mma(a[0], b[2], c);
       c = mma(a[1], b[1], c);
       c = mma(a[2], b[0], c);
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(S::THREADS) __attribute__((amdgpu_waves_per_eu
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      tp_i32x4 pn[G][D::PLANES], pm[D::PLANES];
+      tp_i32x4 pn[G][D::PLANES], pm[S::M_SPLIT ? D::KEPT : D::PLANES];
 #pragma unroll
       for (int g = 0; g < G; ++g) ln[g][u].planes(pn[g]);
 #pragma unroll

@@ -9,12 +9,13 @@
 //   gx = dg Wg + du Wu       one product with K of two parts
 //   gWg = dg^T x, gWu = du^T x, gWd = gy^T h   one launch
 // The backward pass takes g and u from the forward in float32: in bf16 their rounding alone would leave dg and du two roundings off,
-// and gx with them. h, dg and du are rounded to bf16 once, as operands of the next product (float32: split into three planes),
-// so that a bf16 result has the error of two roundings, its own and its operand's.
+// and gx with them. h, dg and du are operands of the next product in two planes of bf16 (16 bits; float32: in three), so that a bf16
+// result has the error of one rounding, its own. Of one plane they would cost half as many matrix instructions, with 1.41 times the error.
 //
-// Bound by the matrix cores from some hundred rows on, by reading the weights below. bf16, 8 192 rows of 2 048 x 5 504: projections
-// 430 us (860 TFLOP/s), y 170 (1 090), dg and du 320 (580: their epilogue moves 553 MB besides), gx 323 (1 140), weights 503 (1 100).
-// float32 (six bf16 products a multiply-add), 16 875 rows of 256 x 680, all gradients: 577 us (92 TFLOP/s). bf16, 16 rows of 2 048 x 5 504: 28 us.
+// Bound by the matrix cores from some hundred rows on, by reading the weights below. bf16, 8 192 rows of 2 048 x 5 504 (us, and the
+// rate of its bf16 products, two a multiply-add for h, dg and du): projections 459 (800 TFLOP/s), y 312 (1 180; 170 with h of one plane), dg and
+// du 352 (525: their epilogue moves 733 MB besides), gx 622 (1 190; 323), weights 977 (1 130; 503). float32 (six bf16 products a
+// multiply-add), 16 875 rows of 256 x 680, all gradients: 577 us (92 TFLOP/s). bf16, 16 rows of 2 048 x 5 504: 34 us.
 #include "ffn_block.h"
 
 namespace {
@@ -87,19 +88,11 @@ __global__ void __launch_bounds__(256) ffn_lay_kernel(LayArgs a) {
 
 // ---------------------------------------------------------------------------------------- epilogues
 
-// four values as bf16, or as the three planes of float32
 __device__ __forceinline__ void put_operand(__bf16* p, int64_t plane, int planes, const float (&v)[4]) {
-  if (planes == 3) {
-    fmd_bf16x4 x[3];
-    x3_split(make_float4(v[0], v[1], v[2], v[3]), x[0], x[1], x[2]);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) *reinterpret_cast<fmd_bf16x4*>(p + i * plane) = x[i];
-  } else {
-    fmd_bf16x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = (__bf16)v[e];
-    *reinterpret_cast<fmd_bf16x4*>(p) = x;
-  }
+  if (planes == 3)
+    put_planes<3>(p, plane, v);
+  else
+    put_planes<2>(p, plane, v);
 }
 
 // h [rows, ld] (zero in the columns past hidden), and g, u [rows, ld] for the backward pass
@@ -212,7 +205,7 @@ template <typename Sh, typename Fn>
 int with_shape(TpArgs& a, float heavy, const Fn& fn) {
   int64_t slices = 0;
   for (int i = 0; i < a.count; ++i) {
-    const int64_t s = fmd_cdiv(2 * a.p[i].k, kTpSlice) * a.p[i].parts * (a.p[i].planes == 3 ? 6 : 1);
+    const int64_t s = fmd_cdiv(2 * a.p[i].k, kTpSlice) * a.p[i].parts * a.p[i].pairs.count;
     slices = i == 0 || s < slices ? s : slices;
   }
   int64_t tiles = count_tiles<typename Sh::Large>(a);
@@ -249,7 +242,11 @@ struct Ffn {
   int32_t bf16, act, lay;  // lay: bits of the operands that are laid out in the workspace: x, gate and up, down, gy
   int64_t rows, width, hidden, out;
   int64_t hp() const { return up8(hidden); }
-  int planes() const { return bf16 ? 1 : 3; }
+  int planes() const { return bf16 ? 1 : 3; }  // of x, gy and the weights
+  int kept() const { return bf16 ? 2 : 3; }    // of h, dg and du
+  TpPairs pairs() const { return bf16 ? kTpPlain : kTpThree; }
+  TpPairs kept_m() const { return bf16 ? kTpTwoM : kTpThree; }
+  TpPairs kept_n() const { return bf16 ? kTpTwoN : kTpThree; }
 };
 
 // an operand: the caller's matrix, or its layout in the workspace
@@ -308,9 +305,9 @@ int product(TpArgs& a, Space& s, bool run, const Epi& epi, hipStream_t stream) {
   });
 }
 
-TpArgs one(const TpOperand& n, const TpOperand& m, int64_t rows_n, int64_t rows_m, int64_t k, int parts, int planes) {
+TpArgs one(const TpOperand& n, const TpOperand& m, int64_t rows_n, int64_t rows_m, int64_t k, int parts, const TpPairs& pairs) {
   TpArgs a{};
-  a.p[0] = {n, m, rows_n, rows_m, k, parts, planes, 0, 0, 0};
+  a.p[0] = {n, m, rows_n, rows_m, k, parts, pairs, 0, 0, 0};
   a.count = 1;
   return a;
 }
@@ -344,7 +341,7 @@ bool direct_backward(const Ffn& f) {
 // float32, 135 rows 9.8 12.9, 11.7 23.7, 10 000 rows 38.8 30.0, 52.0 53.0; bf16 8.6 7.6, 11.4 17.2 and 18.9 15.7, 20.2 31.3.
 bool one_kernel(const Ffn& f) {
   const int64_t weights = f.hidden * (2 * f.width + f.out);
-  return weights <= (!f.bf16 && f.rows >= 4096 ? 50000 : 25000) && block_lds((int)f.hidden, f.planes(), 16, true) <= kBlockLds;
+  return weights <= (!f.bf16 && f.rows >= 4096 ? 50000 : 25000) && block_lds((int)f.hidden, f.kept(), 16, true) <= kBlockLds;
 }
 
 template <typename T, bool BACK>
@@ -354,13 +351,13 @@ int block(const Ffn& f, FfnBlock a, hipStream_t stream) {
     for (a.row0 = 0; a.row0 < f.rows; a.row0 += kMostBlocks * 16 * MT) {
       const int64_t left = fmd_cdiv(f.rows - a.row0, 16 * MT);
       ffn_block_kernel<T, MT, BACK><<<(unsigned)(left < kMostBlocks ? left : kMostBlocks), kBlockThreads,
-                                      block_lds((int)f.hidden, f.planes(), 16 * MT, BACK), stream>>>(a);
+                                      block_lds((int)f.hidden, f.kept(), 16 * MT, BACK), stream>>>(a);
       FMD_CHECK_LAUNCH();
     }
     return (int)FMD_OK;
   };
   // 32 rows of a workgroup where those fill the card
-  if (f.rows >= 32 * kTpCus && block_lds((int)f.hidden, f.planes(), 32, BACK) <= kBlockLds) return launch(std::integral_constant<int, 2>{});
+  if (f.rows >= 32 * kTpCus && block_lds((int)f.hidden, f.kept(), 32, BACK) <= kBlockLds) return launch(std::integral_constant<int, 2>{});
   return launch(std::integral_constant<int, 1>{});
 }
 
@@ -375,7 +372,7 @@ DpOperand planes_in_memory(const Ffn& f, const __bf16* a, const __bf16* b, int64
 
 template <bool N_ACROSS, bool GATED, bool OWN, typename Epi>
 int straight(const Ffn& f, const DpArgs& a, const Epi& epi, hipStream_t stream) {  // OWN: m is h, dg or du
-  if (f.bf16) return dp_product<__bf16, N_ACROSS, GATED, false>(a, epi, stream);
+  if (f.bf16) return dp_product<__bf16, N_ACROSS, GATED, OWN>(a, epi, stream);
   return dp_product<float, N_ACROSS, GATED, OWN>(a, epi, stream);
 }
 
@@ -395,10 +392,10 @@ int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t str
     return f.bf16 ? block<__bf16, false>(f, a, stream) : block<float, false>(f, a, stream);
   }
   if (direct_forward(f)) {
-    __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.planes());
+    __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.kept());
     if (size) *size = s.used;
     if (!run) return FMD_OK;
-    const GatedEpi gated{h, io.saved, io.saved ? io.saved + plane : nullptr, f.rows, f.hidden, hp, plane, f.act, f.planes()};
+    const GatedEpi gated{h, io.saved, io.saved ? io.saved + plane : nullptr, f.rows, f.hidden, hp, plane, f.act, f.kept()};
     DpOperand weights = in_memory(f, io.gate, io.up, io.gate_ld, f.width);
     const DpArgs first{weights, in_memory(f, io.x, io.x, io.x_ld, f.width), f.hidden, f.rows, f.width, 1, 0, 0};
     int status = straight<false, true, false>(f, first, gated, stream);
@@ -411,21 +408,21 @@ int forward(const Ffn& f, const Forward& io, Space& s, bool run, hipStream_t str
   const Matrix g = lay.add(f, s, f.lay & 2, io.gate, io.gate_ld, f.hidden, f.width);
   const Matrix u = lay.add(f, s, f.lay & 2, io.up, io.gate_ld, f.hidden, f.width);
   const Matrix d = lay.add(f, s, f.lay & 4, io.down, io.down_ld, f.out, f.hidden);
-  __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.planes());
+  __bf16* h = io.hidden ? io.hidden : s.take<__bf16>(plane * 2 * f.kept());
   if (run) {
     const int status = lay.launch(f, stream);
     if (status) return status;
   }
   int64_t most = s.used;
   const int64_t base = s.used;
-  TpArgs a = one(operand(g, u), operand(x, x), f.hidden, f.rows, f.width, 1, f.planes());
-  const GatedEpi gated{h, io.saved, io.saved ? io.saved + plane : nullptr, f.rows, f.hidden, hp, plane, f.act, f.planes()};
+  TpArgs a = one(operand(g, u), operand(x, x), f.hidden, f.rows, f.width, 1, f.pairs());
+  const GatedEpi gated{h, io.saved, io.saved ? io.saved + plane : nullptr, f.rows, f.hidden, hp, plane, f.act, f.kept()};
   int status = product<Shapes<false, false, true>>(a, s, run, gated, stream);
   if (status) return status;
   most = s.used > most ? s.used : most;
   s.used = base;
   const Matrix hm{h, hp, plane};
-  a = one(operand(d, d), operand(hm, hm), f.out, f.rows, f.hidden, 1, f.planes());
+  a = one(operand(d, d), operand(hm, hm), f.out, f.rows, f.hidden, 1, f.kept_m());
   status = product<Shapes<false, false, false>>(a, s, run, store, stream);
   if (status) return status;
   most = s.used > most ? s.used : most;
@@ -452,7 +449,7 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   if (!straight_on) d = lay.add(f, s, f.lay & 4, io.in.down, io.in.down_ld, f.out, f.hidden);
   if (want_w || !straight_on) gy = lay.add(f, s, f.lay & 8, io.gy, io.gy_ld, f.rows, f.out);
   const int64_t hp = f.hp(), plane = f.rows * hp;
-  __bf16* dgu = together && !want_w ? nullptr : s.take<__bf16>(2 * plane * 2 * f.planes());
+  __bf16* dgu = together && !want_w ? nullptr : s.take<__bf16>(2 * plane * 2 * f.kept());
   if (run) {
     const int status = lay.launch(f, stream);
     if (status) return status;
@@ -461,7 +458,7 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   __bf16* h = io.in.hidden;
   TpArgs a{};
   if (together) {
-    h = want_w ? s.take<__bf16>(plane * 2 * f.planes()) : nullptr;
+    h = want_w ? s.take<__bf16>(plane * 2 * f.kept()) : nullptr;
     most = s.used;
     if (run) {
       FfnBlock b = block_args(f, io.in, io.gy, io.gy_ld, io.gx);
@@ -472,11 +469,11 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
     }
   }
   const int64_t base = s.used;
-  const GatedBackEpi back{dgu, io.in.saved, io.in.saved ? io.in.saved + plane : nullptr, f.rows, f.hidden, hp, 2 * plane, f.act, f.planes()};
+  const GatedBackEpi back{dgu, io.in.saved, io.in.saved ? io.in.saved + plane : nullptr, f.rows, f.hidden, hp, 2 * plane, f.act, f.kept()};
   int status = FMD_OK;
   if (together) {
   } else if (!straight_on) {
-    a = one(operand(d, d), operand(gy, gy), f.hidden, f.rows, f.out, 1, f.planes());
+    a = one(operand(d, d), operand(gy, gy), f.hidden, f.rows, f.out, 1, f.pairs());
     status = product<Shapes<true, false, false>>(a, s, run, back, stream);
     most = s.used > most ? s.used : most;
   } else if (run) {
@@ -489,7 +486,7 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
     s.used = base;
     const StoreEpi store{{io.gx}, {f.rows}, {f.width}, f.bf16};
     if (!straight_on) {
-      a = one(operand(g, u), operand(dg, du), f.width, f.rows, f.hidden, 2, f.planes());
+      a = one(operand(g, u), operand(dg, du), f.width, f.rows, f.hidden, 2, f.kept_m());
       status = product<Shapes<true, false, false>>(a, s, run, store, stream);
       most = s.used > most ? s.used : most;
     } else if (run) {
@@ -501,9 +498,9 @@ int backward(const Ffn& f, const Backward& io, bool want_x, bool want_w, Space& 
   if (want_w) {
     s.used = base;
     const Matrix hm{h, hp, plane};
-    a = one(operand(x, x), operand(dg, dg), f.width, f.hidden, f.rows, 1, f.planes());
-    a.p[1] = {operand(x, x), operand(du, du), f.width, f.hidden, f.rows, 1, f.planes(), 0, 0, 0};
-    a.p[2] = {operand(hm, hm), operand(gy, gy), f.hidden, f.out, f.rows, 1, f.planes(), 0, 0, 0};
+    a = one(operand(x, x), operand(dg, dg), f.width, f.hidden, f.rows, 1, f.kept_m());
+    a.p[1] = {operand(x, x), operand(du, du), f.width, f.hidden, f.rows, 1, f.kept_m(), 0, 0, 0};
+    a.p[2] = {operand(hm, hm), operand(gy, gy), f.hidden, f.out, f.rows, 1, f.kept_n(), 0, 0, 0};
     a.count = 3;
     const StoreEpi store{{io.g_gate, io.g_up, io.g_down}, {f.hidden, f.hidden, f.out}, {f.width, f.width, f.hidden}, f.bf16};
     status = product<Shapes<true, true, false>>(a, s, run, store, stream);

@@ -3,7 +3,8 @@
 // weights, from the caches. The backward pass forms the projections again: at such widths that is less than writing them and
 // reading them back.
 //
-// For the weights' gradients the backward pass also writes what their products multiply: h, dg and du.
+// For the weights' gradients the backward pass also writes what their products multiply: h, dg and du, in the planes that LDS holds of them
+// (float32 three, bf16 two).
 #pragma once
 
 #include "activation.h"
@@ -64,20 +65,18 @@ __device__ __forceinline__ void block_product(typename DpType<T>::Acc (&acc)[G][
   }
 }
 
-// four values of an operand in LDS or in memory: bf16, or the planes of float32
+// Four values of an operand in LDS or in memory: the three planes of float32, or two for a product with bf16. Of an infinite value the
+// second is zero: its products with finite ones stay infinite.
 template <int PLANES>
-__device__ __forceinline__ void block_put(__bf16* p, int64_t plane, const float (&v)[4]) {
-  if constexpr (PLANES == 3) {
-    fmd_bf16x4 x[3];
-    x3_split(make_float4(v[0], v[1], v[2], v[3]), x[0], x[1], x[2]);
+__device__ __forceinline__ void put_planes(__bf16* p, int64_t plane, const float (&v)[4]) {
+  fmd_bf16x4 x[3];
+  x3_split(make_float4(v[0], v[1], v[2], v[3]), x[0], x[1], x[2]);
+  if (PLANES == 2) {
 #pragma unroll
-    for (int i = 0; i < 3; ++i) *reinterpret_cast<fmd_bf16x4*>(p + i * plane) = x[i];
-  } else {
-    fmd_bf16x4 x;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = (__bf16)v[e];
-    *reinterpret_cast<fmd_bf16x4*>(p) = x;
+    for (int e = 0; e < 4; ++e) x[1][e] = fabsf((float)x[0][e]) == INFINITY ? (__bf16)0.f : x[1][e];
   }
+#pragma unroll
+  for (int i = 0; i < PLANES; ++i) *reinterpret_cast<fmd_bf16x4*>(p + i * plane) = x[i];
 }
 
 template <typename T>
@@ -88,7 +87,7 @@ struct RawFour {
 template <typename T, int MT, bool BACK>
 __global__ void __launch_bounds__(kBlockThreads) ffn_block_kernel(FfnBlock a) {
   typedef DpType<T> D;
-  constexpr int ROWS = 16 * MT, P = D::PLANES;
+  constexpr int ROWS = 16 * MT, P = D::KEPT;
   extern __shared__ __attribute__((aligned(16))) char block_lds_space[];
   __bf16* lds = reinterpret_cast<__bf16*>(block_lds_space);  // [BACK ? dg, du : h][planes][ROWS][ld]
   const int ld = block_ld(a.hidden), plane = ROWS * ld;
@@ -125,16 +124,16 @@ __global__ void __launch_bounds__(kBlockThreads) ffn_block_kernel(FfnBlock a) {
       }
       __bf16* to = lds + (16 * t + r) * ld + n0 + 4 * q;
       if (!BACK) {
-        block_put<P>(to, plane, h);
+        put_planes<P>(to, plane, h);
         continue;
       }
-      block_put<P>(to, plane, dg);
-      block_put<P>(to + P * plane, plane, du);
+      put_planes<P>(to, plane, dg);
+      put_planes<P>(to + P * plane, plane, du);
       const int64_t m = m0 + 16 * t + r, n = n0 + 4 * q;
       if (a.d && m < a.rows && n < a.hp) {
-        block_put<P>(a.h + m * a.hp + n, a.rows * a.hp, h);
-        block_put<P>(a.d + m * a.hp + n, 2 * a.rows * a.hp, dg);
-        block_put<P>(a.d + (a.rows + m) * a.hp + n, 2 * a.rows * a.hp, du);
+        put_planes<P>(a.h + m * a.hp + n, a.rows * a.hp, h);
+        put_planes<P>(a.d + m * a.hp + n, 2 * a.rows * a.hp, dg);
+        put_planes<P>(a.d + (a.rows + m) * a.hp + n, 2 * a.rows * a.hp, du);
       }
     }
   }
@@ -159,7 +158,7 @@ __global__ void __launch_bounds__(kBlockThreads) ffn_block_kernel(FfnBlock a) {
         for (int u = 0; u < U; ++u) {
           const int k = first + u * D::UNIT + q * D::EACH;
           if (first + u * D::UNIT >= a.hidden) break;
-          tp_i32x4 pn[P], pm[P];
+          tp_i32x4 pn[D::PLANES], pm[P];
           ln[u].planes(pn);
 #pragma unroll
           for (int t = 0; t < MT; ++t) {

@@ -192,7 +192,7 @@ int with_shape(TpArgs& a, const Fn& fn) {
 
 TpArgs arguments(const int8_t* x, int64_t x_ld, const int8_t* w, int64_t w_ld, int64_t rows, int64_t width, int64_t out) {
   TpArgs a{};
-  a.p[0] = {tp_operand(w, w, w_ld, 0, 1), tp_operand(x, x, x_ld, 0, 1), out, rows, width, 1, 1, 0, 0, 0};
+  a.p[0] = {tp_operand(w, w, w_ld, 0, 1), tp_operand(x, x, x_ld, 0, 1), out, rows, width, 1, kTpPlain, 0, 0, 0};
   a.count = 1;
   return a;
 }

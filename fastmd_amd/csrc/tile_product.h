@@ -8,7 +8,7 @@
 // lane's four consecutive results then lie side by side in a row of the output.
 //
 // float32 operands come as three bf16 planes (x3.h); their six plane products follow each other along K, the small ones
-// first, in one accumulator: K is six times as long, the kernel is the same.
+// first, in one accumulator: K is six times as long, the kernel is the same. Likewise an operand of two planes (16 bits) against one of bf16.
 #pragma once
 
 #include "common.h"
@@ -26,10 +26,19 @@ struct TpOperand {
   int64_t ld, plane;  // bytes from a stored row to the next, and from a plane to the next
 };
 
+// The products of planes, in their order along K: two bits each, the plane of n and that of m
+struct TpPairs {
+  int32_t count;
+  uint32_t n, m;
+};
+constexpr TpPairs kTpPlain{1, 0, 0}, kTpThree{6, 0x124, 0x046};  // of three planes each: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0)
+constexpr TpPairs kTpTwoN{2, 1, 0}, kTpTwoM{2, 0, 1};            // n, or m, of two planes
+
 struct TpProblem {
   TpOperand n, m;
   int64_t rows_n, rows_m, k;  // of one part
-  int32_t parts, planes;      // parts of K; planes 1 or 3
+  int32_t parts;              // of K
+  TpPairs pairs;
   int32_t tiles_n, tiles_m, first;  // tiles, and the number of the first one
 };
 
@@ -237,7 +246,7 @@ tile_product_kernel(TpArgs a, Epi epi) {
 
   // slices of K of all passes (parts, planes), and those of this workgroup
   const int64_t k_bytes = p.k * T::SIZE;
-  const int nk = (int)((k_bytes + kTpSlice - 1) / kTpSlice), passes = p.parts * (p.planes == 3 ? 6 : 1);
+  const int nk = (int)((k_bytes + kTpSlice - 1) / kTpSlice), passes = p.parts * p.pairs.count;
   const int total = nk * passes;  // at least one: K is not empty
   const int begin = (int)((int64_t)total * split / splits), end = (int)((int64_t)total * (split + 1) / splits);
 
@@ -247,10 +256,9 @@ tile_product_kernel(TpArgs a, Epi epi) {
   sm.place(p.m, m0, p.rows_m, wave, lane);
   int pass = begin / nk, ks = begin - pass * nk;  // of the next slice to copy
   auto open = [&]() {
-    const int pair = p.planes == 3 ? pass / p.parts : 5, part = p.planes == 3 ? pass - pair * p.parts : pass;
-    // planes of the six products: (0,2) (1,1) (2,0) (0,1) (1,0) (0,0)
-    sn.begin(p.n, part, (0x124 >> (2 * pair)) & 3, n0, ks);
-    sm.begin(p.m, part, (0x046 >> (2 * pair)) & 3, m0, ks);
+    const int pair = pass / p.parts, part = pass - pair * p.parts;
+    sn.begin(p.n, part, (p.pairs.n >> (2 * pair)) & 3, n0, ks);
+    sm.begin(p.m, part, (p.pairs.m >> (2 * pair)) & 3, m0, ks);
   };
   int next = begin;  // slice to copy; past the end zeros, so that every wait counts the same copies
   constexpr int COPIES = S::StageN::LOADS + S::StageM::LOADS;

@@ -12,8 +12,9 @@ are fixed), of the weights, or of all.
 float32 is computed on the bf16 matrix cores with every operand split into three planes (float32 accuracy; a value that is not
 finite, or rounds to an infinite bfloat16, makes the results that it is a term of NaN), bfloat16 with products of bfloat16
 operands. Sums are float32 in both, and so is the activation. For bfloat16 the hidden layer and, in the VJP, the
-gradients of the two projections are rounded once, as operands of the next product. Gradients take no atomics: the same call
-gives the same bits.
+gradients of the two projections go into the next product as two bfloat16 parts (16 bits), so that each result carries the
+error of one rounding, its own (an infinite value that they are multiplied by gives NaN). Gradients take no atomics: the same
+call gives the same bits.
 """
 from __future__ import annotations
 
@@ -37,7 +38,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 class FeedForwardSaved(NamedTuple):
     """What the VJP needs of the forward besides its inputs, rows of the hidden width rounded up to a multiple of 8:
     ``projections`` float32 [2, rows, .], x w_gate^T and x w_up^T, and ``hidden`` bfloat16 [planes, rows, .], what w_down
-    multiplies (for float32 its three planes). None for blocks of small weights, whose VJP forms both again."""
+    multiplies (for float32 its three planes, for bfloat16 two). None for blocks of small weights, whose VJP forms both again."""
 
     projections: Tensor | None
     hidden: Tensor | None
@@ -130,7 +131,7 @@ def _forward(x, w_gate, w_up, w_down, activation, save):
         if _saves(bf16, rows, width, hidden, out):
             padded = -(-hidden // 8) * 8
             projections = torch.empty((2, rows, padded), dtype=torch.float32, device=device)
-            kept = torch.empty((1 if bf16 else 3, rows, padded), dtype=torch.bfloat16, device=device)
+            kept = torch.empty((2 if bf16 else 3, rows, padded), dtype=torch.bfloat16, device=device)
         saved = FeedForwardSaved(projections, kept)
     if rows == 0:
         return y, saved
@@ -162,7 +163,7 @@ def gated_feed_forward_vjp(gy: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, 
     if rows and _saves(bf16, rows, width, hidden, out):
         padded = -(-hidden // 8) * 8
         for t, shape, dtype in ((projections, (2, rows, padded), torch.float32),
-                                (kept, (1 if bf16 else 3, rows, padded), torch.bfloat16)):
+                                (kept, (2 if bf16 else 3, rows, padded), torch.bfloat16)):
             if t is None or t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.data_ptr() % 16:
                 raise ValueError(f"saved must be the forward's: {dtype} {shape}, got "
                                  f"{None if t is None else (t.dtype, tuple(t.shape))}")

@@ -892,8 +892,9 @@ int fmd_qk_norm_rotary_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q
  * lay: bits of the operands that the call lays out in `work` first: 1 x, 2 gate and up, 4 down, 8 gy. float32: 15. bf16: those
  * whose rows do not start on 16 bytes, whose width is no multiple of 8, whose row stride reaches 2^22 (FMD_EINVAL where such an
  * operand's bit is missing). Few rows and small weights are read where they are.
- * For the VJP (nullable, and unused where fmd_gated_ffn_saves() is 0: it forms them again): saved, float32 [2, rows, hp], the two projections, and hidden, bf16 [planes, rows, hp] (planes 3 for
- * float32, else 1), the product of the two as `down` multiplies it; hp: hidden rounded up to 8; both 16-byte aligned.
+ * For the VJP (nullable, and unused where fmd_gated_ffn_saves() is 0: it forms them again): saved, float32 [2, rows, hp], the
+ * two projections, and hidden, bf16 [planes, rows, hp], what `down` multiplies (in three planes for float32, two for bf16: each what
+ * those before it leave of the value); hp: hidden rounded up to 8; both 16-byte aligned.
  * rows below 2^31, widths below 2^22, and at most 2^21 tiles of 256 x 128 results (FMD_EINVAL). work: fmd_gated_ffn_work_size() bytes on a 256-byte address (keep_hidden: `hidden` is given;
  * null for 0). */
 int32_t fmd_gated_ffn_saves(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out);
