@@ -10,7 +10,7 @@
 
 with the rows of x rounded on the way, or given as ``Int8Rows``. The sums are exact (32-bit integers on the matrix cores), each
 result is rounded once. A row of zeros has the scale 0; one that holds a value that is not finite gives NaN. For evaluation:
-there are no gradients, and inputs that need them are refused.
+there are no gradients, and inputs that need them (x, scales, the bias) are refused.
 """
 from __future__ import annotations
 
@@ -95,6 +95,8 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = No
         raise ValueError("weight must be Int8Rows (quantize_rows)")
     _check_rows("weight", weight)
     rounded = isinstance(x, Int8Rows)
+    if differentiated(x.scales if rounded else x, weight.scales, bias):
+        raise ValueError("linear_int8 has no gradient: detach its inputs")
     if rounded:
         _check_rows("x", x)
         values, kind = x.values, torch.float32 if dtype is None else dtype
@@ -104,8 +106,6 @@ def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = No
         require_cuda(x, weight.values, weight.scales, bias)
         if x.dim() != 2 or x.dtype not in _TYPES:
             raise ValueError(f"x must be a float32 or bfloat16 matrix, or Int8Rows, got {x.dtype} {tuple(x.shape)}")
-        if differentiated(x, bias):
-            raise ValueError("linear_int8 has no gradient: detach its inputs")
     if kind not in _TYPES:
         raise ValueError(f"the result must be float32 or bfloat16, got {kind}")
     (rows, width), out, device = values.shape, weight.values.shape[0], values.device
