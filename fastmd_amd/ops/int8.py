@@ -8,8 +8,8 @@
 
     y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]
 
-with the rows of x rounded on the way, or given as ``Int8Rows``. The sums are exact (32-bit integers on the matrix cores), each
-result is rounded once. A row of zeros has the scale 0; one that holds a value that is not finite gives NaN. For evaluation:
+with the rows of x rounded on the way, or given as ``Int8Rows``. The sums are exact (32-bit integers on the matrix cores),
+scales and bias are applied in float64, and each result is rounded to float32 and, where asked, from there to bfloat16. A row of zeros has the scale 0; one that holds a value that is not finite gives NaN. For evaluation:
 there are no gradients, and inputs that need them (x, scales, the bias) are refused.
 """
 from __future__ import annotations
@@ -24,7 +24,7 @@ from fastmd_amd import _abi
 from fastmd_amd._autograd import differentiated
 from fastmd_amd._device import on_device_of, require_cuda, rows_view, stream
 
-MAX_WIDTH = 131071  # 127^2 times more terms could overflow 32 bits
+MAX_WIDTH = 131071  # 2^17 products of -128 and -128, which given values may hold, would overflow 32 bits
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
