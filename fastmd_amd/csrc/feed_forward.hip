@@ -321,24 +321,33 @@ struct Forward {
 };
 
 // Whether the products of a pass go straight from memory to registers (direct_product.h) or through tiles in LDS: by the multiply-adds
-// of the forward pass, where the two forms' times meet. us of the forward pass and of the VJP for x, tiles and straight, float32: 300 rows of
-// 256 x 680 33 21, 45 31; 2 000 of 256 x 680 48 53, 57 73; 130 of 512 x 1 376 44 31, 48 45; 200 49 41, 49 53; 500 54 59, 67 61; 32 of
-// 1 024 x 2 736 57 31, 61 50; 64 58 46, 62 74; 200 of 768 x 2 048 59 55, 65 75; 400 73 95, 89 132. bf16: 135 rows of 256 x 680 15.7 10.0,
-// 18.2 15.0; 300 16.0 13.3, 20.0 22.3; 500 16.5 13.8, 24.5 18.1; 1 000 17.5 20.7, 25.2 32.1; 16 of 512 x 1 376 16.8 10.0, 18.0 15.5; 64 18.1 11.4, 20.7 22.7; 200 21.4 21.9,
-// 23.9 31.7; 16 of 2 048 x 5 504 34 30, 36 56 (the VJP reads weights across their rows, two bytes a lane).
+// of the forward pass and the rows, where the two forms' times meet. us of tiles, straight:
+// float32, forward: 1 000 rows of 256 x 680 42 39, 2 000 47 53; 200 of 512 x 1 376 47 40, 500 53 58; 200 of 768 x 2 048 59 54, 400 73 93; 4 000 of
+//   128 x 344 37 33; 10 000 of 64 x 256 36 39, of 96 x 192 38 41; 64 of 2 048 x 5 504 157 120; 16 of 4 096 x 11 008 538 153.
+// float32, VJP for x: 500 of 256 x 680 44 26, 1 000 46 57; 64 of 512 x 1 376 44 40, 130 47 45, 200 48 53 (but 500 67 61); 32 of 1 024 x 2 736 60 50, 64
+//   62 75; 2 000 of 128 x 344 39 37, 4 000 44 45; 32 of 2 048 x 5 504 153 105, 64 158 169; 16 of 4 096 x 11 008 530 224.
+// bf16, forward: 500 of 256 x 680 21.8 14.3, 1 000 23.4 25.5; 1 000 of 128 x 344 16.5 13.0, 2 000 17.7 19.4; 130 of 512 x 1 376 20.6 19.7, 200 21.4
+//   24.8; 32 of 1 024 x 2 736 22.8 20.0, 64 25.8 29.3; 64 of 768 x 2 048 22.2 27.7; 16 of 2 048 x 5 504 38.5 34.4, 32 40.2 45.7; 16 of 4 096 x 11 008
+//   92.7 82.1.
+// bf16, VJP for x: 300 of 256 x 680 23.6 23.9, 500 26.3 18.8, 1 000 31.3 39.9; 1 000 of 128 x 344 21.5 19.3, 2 000 27.2 30.1; 32 of 512 x 1 376 26.9
+//   21.7, 64 27.7 28.4, 130 30.3 38.0; 16 of 768 x 2 048 26.3 25.6, of 1 024 x 2 736 33.1 32.5, of 2 048 x 5 504 40.6 61.6 (weights are read across
+//   their rows, two bytes a lane).
 bool direct_forward(const Ffn& f) {
   const double work = (double)f.rows * f.hidden * (2 * f.width + f.out);
-  return f.bf16 ? work <= 2.7e8 || (f.rows <= 32 && work <= 5.5e8) : work <= 9.5e8 || f.rows <= 64;
+  if (f.bf16) return f.rows <= 16 || work <= (f.rows <= 512 ? 2.7e8 : 2e8);
+  return f.rows <= 64 || work <= (f.rows <= 4096 ? 9.5e8 : 2.4e8);
 }
 bool direct_backward(const Ffn& f) {
   const double weights = (double)f.hidden * (2 * f.width + f.out), work = weights * f.rows;
-  return f.bf16 ? work <= 1.2e8 && weights <= 2.2e6 : work <= 3e8 || f.rows <= 32;
+  if (f.bf16) return weights <= 2.2e6 && work <= (weights <= 6e5 && f.rows <= 512 ? 2.7e8 : 1.33e8);
+  return f.rows <= 32 || work <= 3e8;
 }
 
 // Whether the whole block is one kernel: its hidden layer (in the backward pass the two gradients of it) fits LDS for 16 rows, and the
-// weights, which every workgroup walks through, are few. us of the forward pass and of the VJP for x, straight from memory and in one kernel:
-// 64 x 128 float32, 135 rows 10.4 8.6, 10.9 13.5, 10 000 rows 24.7 18.6, 37.1 29.7; bf16 8.4 5.7, 11.1 10.0 and 13.8 10.4, 20.7 18.2. 64 x 256
-// float32, 135 rows 9.8 12.9, 11.7 23.7, 10 000 rows 38.8 30.0, 52.0 53.0; bf16 8.6 7.6, 11.4 17.2 and 18.9 15.7, 20.2 31.3.
+// weights, which every workgroup walks through, are few. us of the forward pass and of the VJP for x, the better of the other forms and in one
+// kernel: 64 x 128 float32, 135 rows 10.6 10.5, 10.9 13.5, 1 000 rows 10.7 8.8, 12.4 13.6, 10 000 rows 24.7 18.5, 36.2 29.5; bf16 8.2 6.7, 11.4 10.2;
+// 10.8 5.9, 12.3 10.3; 14.0 10.9, 20.8 19.7. 64 x 256 float32, 135 rows 9.7 12.7, 11.6 23.3, 10 000 rows 35.8 30.3, 42.8 52.2; bf16 8.8 8.0, 11.7 16.9 and
+// 19.5 16.7, 28.1 34.9.
 bool one_kernel(const Ffn& f) {
   const int64_t weights = f.hidden * (2 * f.width + f.out);
   return weights <= (!f.bf16 && f.rows >= 4096 ? 50000 : 25000) && block_lds((int)f.hidden, f.kept(), 16, true) <= kBlockLds;
