@@ -10,6 +10,7 @@
 
 #include <type_traits>
 
+#include "direct_shape.h"
 #include "tile_product.h"
 
 typedef float dp_f32x4 __attribute__((ext_vector_type(4)));
@@ -206,24 +207,17 @@ inline int dp_launch(DpArgs a, const Epi& epi, hipStream_t stream) {
   return FMD_OK;
 }
 
-// Rows of a wave: those there are, up to 64, where the weights are much to read; otherwise as many as leave the card waves to run (a
-// wave's work is then latency and code that runs once: the four products of 135 rows of 64 x 128, float32, forward and VJP for x, 10.9,
-// 8.7, 10.4 and 6.8 us with 64 rows a wave, 5.7, 5.5, 6.7 and 5.2 with 16). K shared by eight or sixteen waves where the tiles are too few to fill the card with waves of
-// their own.
 template <typename T, bool N_ACROSS, bool GATED, bool M_SPLIT, typename Epi>
 inline int dp_product(const DpArgs& a, const Epi& epi, hipStream_t stream) {
-  const int64_t columns = fmd_cdiv(a.rows_n, 16), units = a.parts * fmd_cdiv(a.k, DpType<T>::UNIT);
+  const DpForm form = dp_form(a.rows_n, a.rows_m, a.k, a.parts, DpType<T>::UNIT);
   const auto with = [&](auto mt) {
     constexpr int MT = decltype(mt)::value;
-    const int64_t waves = columns * fmd_cdiv(a.rows_m, 16 * MT);
     if constexpr (MT == 1)
-      if (waves <= 192 && units >= 64) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 16>>(a, epi, stream);
-    if (waves < 1024 && units >= 8) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 8>>(a, epi, stream);
+      if (form.wk == 16) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 16>>(a, epi, stream);
+    if (form.wk == 8) return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 8>>(a, epi, stream);
     return dp_launch<DpShape<T, N_ACROSS, GATED, M_SPLIT, MT, 1>>(a, epi, stream);
   };
-  const bool much = a.rows_n * a.k * a.parts >= 1 << 20;
-  const auto enough = [&](int64_t mt) { return much || columns * fmd_cdiv(a.rows_m, 16 * mt) >= 1024; };
-  if (a.rows_m > 32 && enough(4)) return with(std::integral_constant<int, 4>{});
-  if (a.rows_m > 16 && enough(2)) return with(std::integral_constant<int, 2>{});
+  if (form.mt == 4) return with(std::integral_constant<int, 4>{});
+  if (form.mt == 2) return with(std::integral_constant<int, 2>{});
   return with(std::integral_constant<int, 1>{});
 }
