@@ -17,16 +17,21 @@ TILES = [
     (F32, 5000, 96, 1100, 40),     # narrow results
     (F32, 9000, 40, 1032, 130),
     (F32, 16384, 136, 520, 256),   # K not shared, in the VJP for x
+    (F32, 16875, 256, 680, 256),
+    (F32, 6000, 520, 1032, 264),
     (F32, 131, 1300, 2100, 1290),  # few rows, large weights
     (BF16, 1500, 301, 1003, 299),
     (BF16, 700, 520, 1376, 264),
     (BF16, 3000, 96, 1100, 40),
     (BF16, 8200, 33, 520, 130),
     (BF16, 40000, 40, 300, 40),    # K not shared
+    (BF16, 9000, 520, 1376, 1032),
+    (BF16, 5000, 1100, 1000, 520),
     (BF16, 131, 1000, 2100, 990),
     (BF16, 600, 344, 872, 344),    # whole vectors: nothing is laid out
 ]
 # 1 024 tiles of 256 rows by 128 columns of the hidden layer and more; narrow inputs keep the oracle quick
+ONE = [(F32, 8200, 64, 120, 64), (F32, 8300, 40, 100, 33), (BF16, 8200, 64, 120, 64), (BF16, 9000, 17, 90, 23)]  # 32 rows of a workgroup
 MANY = [(F32, 8200, 16, 4100, 24), (BF16, 8200, 16, 4100, 24)]
 
 
@@ -51,6 +56,8 @@ def partial(dtype, rows, width, hidden, out):
 def test_the_sizes_take_tiles():
     for dtype, *size in TILES + MANY:
         assert forms(is_bf16(dtype), *size) == ("tiles", "tiles"), size
+    for dtype, *size in ONE:
+        assert forms(is_bf16(dtype), *size) == ("one", "one") and size[0] >= 32 * 256, size
     for _, rows, _, hidden, _ in MANY:
         assert -(-rows // 256) * -(-hidden // 128) >= 1024
     sums = [partial(dtype, *size) for dtype, *size in TILES]
@@ -58,6 +65,12 @@ def test_the_sizes_take_tiles():
     for bf16 in (0, 1):  # K shared and not, in the VJP of either type
         split = [x > 0 for (x, _), (dtype, *_) in zip(sums, TILES) if is_bf16(dtype) == bf16]
         assert any(split) and not all(split)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width,hidden,out", ONE)
+def test_one_kernel_over_many_rows(dtype, rows, width, hidden, out):
+    check(*make(rows, width, hidden, out, dtype))
 
 
 @pytest.mark.gpu
@@ -74,7 +87,7 @@ def test_activations_in_tiles(dtype, activation):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype,rows,width,hidden,out", [TILES[1], TILES[7], TILES[12], TILES[5], TILES[11]])
+@pytest.mark.parametrize("dtype,rows,width,hidden,out", [size for size in TILES if size[1] in (131, 600, 700)])
 def test_strides_in_tiles(dtype, rows, width, hidden, out):
     """Columns of wider buffers, transposed weights, rows off 16 bytes, a packed pair of projections: the same values, whatever lies
     beside them."""
@@ -164,6 +177,19 @@ def test_8_bit_products_straight(rows, width, out, dtype):
     from fastmd_amd.ops.int8 import linear_int8, quantize_rows
     from test_int8 import make as rows_of
 
+    x, w = rows_of(rows, width, dtype), rows_of(out, width, F32, seed=1)
+    y = linear_int8(x.cuda(), quantize_rows(w.cuda()))
+    oracle.near(y, *oracle.linear_int8(*oracle.quantize(x), *oracle.quantize(w), None, dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width,out", [(2000, 1024, 1024), (3000, 600, 2000), (5000, 515, 1030), (700, 3000, 1500), (9000, 300, 300)])
+def test_8_bit_products_in_tiles(rows, width, out, dtype):
+    from fastmd_amd.ops.int8 import linear_int8, quantize_rows
+    from test_int8 import make as rows_of
+
+    assert rows * width * out > 4e8
     x, w = rows_of(rows, width, dtype), rows_of(out, width, F32, seed=1)
     y = linear_int8(x.cuda(), quantize_rows(w.cuda()))
     oracle.near(y, *oracle.linear_int8(*oracle.quantize(x), *oracle.quantize(w), None, dtype))

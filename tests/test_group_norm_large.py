@@ -28,6 +28,11 @@ MERGED = [
     (BF16, 64, 32, [17] * 60 + [30000] + [0, 21] * 40 + [9001] + [1500] * 3, True),
     (BF16, 99, 33, [31] * 90 + [40007, 0, 20001] + [16] * 60, True),
 ]
+# type, channels, groups, rows: tiles of more rows than small calls have, in vectors of each width
+TILES = [(F32, 128, 8, 68001), (F32, 130, 5, 66003), (F32, 130, 26, 131002), (BF16, 132, 3, 66003), (BF16, 132, 12, 132001), (BF16, 130, 13, 66001),
+         (BF16, 128, 4, 70003)]
+# type, channels, rows of one group: vectors of a lane, in vectors of each width
+ROWS = [(dtype, channels, 1) for dtype in TYPES for channels in (63, 99, 255, 66, 130, 258, 300, 400, 1000, 1020, 520, 2040)]
 # type, channels, groups, rows: more workgroups of rows than there are in a launch
 ROUNDS = [
     (F32, 1024, 1, 2101), (BF16, 1024, 1, 2101), (F32, 8192, 1, 601), (BF16, 8190, 1, 601), (F32, 2048, 64, 700), (BF16, 999, 3, 1900),
@@ -95,6 +100,18 @@ def check(dtype, channels, groups, rows, offsets, activation="silu", lead=0, spa
 @pytest.mark.parametrize("dtype,channels,groups,lengths,lead,spare,parts", PARTS)
 def test_several_parts_of_rows_a_tile(dtype, channels, groups, lengths, lead, spare, parts):
     check(dtype, channels, groups, sum(lengths) + lead + spare, ragged(lengths, lead), lead=lead, spare=spare)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,channels,groups,rows", TILES)
+def test_tiles_of_many_rows(dtype, channels, groups, rows):
+    check(dtype, channels, groups, rows, ragged([rows // 2 - 50, 300, rows - rows // 2 - 250]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,channels,groups", ROWS)
+def test_vectors_of_a_lane(dtype, channels, groups):
+    check(dtype, channels, groups, 37, None)
 
 
 @pytest.mark.gpu
