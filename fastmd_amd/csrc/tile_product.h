@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(S::THREADS) tile_join_kernel(TpArgs a, Epi epi
 // Host side: sizes, the split of the tiles that do not fill the card, launches.
 
 constexpr int kTpCus = 256;
-constexpr int64_t kTpMostTiles = 1 << 21;
+constexpr int64_t kTpMostTiles = 1 << 22;  // of 512 threads at most: a launch takes fewer than 2^32
 
 // The operand rows of [base, ld elements of `size` bytes]
 inline TpOperand tp_operand(const void* a, const void* b, int64_t ld, int64_t plane, int size) {

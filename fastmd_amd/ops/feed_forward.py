@@ -31,7 +31,7 @@ from fastmd_amd._device import on_device_of, require_cuda, rows_view, stream
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 MAX_WIDTH = 2 ** 22 - 8
-MAX_ROWS, MAX_VALUES = 2 ** 29, 2 ** 36  # of 2^21 tiles
+MAX_ROWS, MAX_VALUES = 2 ** 29, 2 ** 36  # within the 2^22 tiles of a launch, with every remainder
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 

@@ -895,8 +895,8 @@ int fmd_qk_norm_rotary_bwd(int32_t bf16, const void* q, int64_t q_row, int64_t q
  * For the VJP (nullable, and unused where fmd_gated_ffn_saves() is 0: it forms them again): saved, float32 [2, rows, hp], the
  * two projections, and hidden, bf16 [planes, rows, hp], what `down` multiplies (in three planes for float32, two for bf16: each what
  * those before it leave of the value); hp: hidden rounded up to 8; both 16-byte aligned.
- * rows below 2^31, widths below 2^22, and at most 2^21 tiles of 256 x 128 results (FMD_EINVAL). work: fmd_gated_ffn_work_size() bytes on a 256-byte address (keep_hidden: `hidden` is given;
- * null for 0). */
+ * rows below 2^31, widths below 2^22, and at most 2^22 tiles of 256 x 128 results (FMD_EINVAL). work: fmd_gated_ffn_work_size()
+ * bytes on a 256-byte address (keep_hidden: `hidden` is given; null for 0). */
 int32_t fmd_gated_ffn_saves(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out);
 int64_t fmd_gated_ffn_work_size(int32_t bf16, int64_t rows, int64_t width, int64_t hidden, int64_t out, int32_t lay,
                                 int32_t keep_hidden);

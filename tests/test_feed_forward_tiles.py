@@ -204,3 +204,19 @@ def test_8_bit_products_take_every_straight_form(tmp_path):
         assert rows * width * out <= 4e8 and width * out <= 2.5e7
     assert shapes(tmp_path, [(out, rows, -(-width // 16) * 16, 1, 64) for rows, width, out in sizes]) == [
         "1/16", "2/8", "4/8", "2/1", "4/1", "1/1", "1/8"]
+
+
+def test_no_size_that_the_checks_accept_has_too_many_tiles():
+    """Just below each limit of the argument checks (2^29 rows, 2^36 values of a matrix): sizes are found, which a refused call has none of."""
+    from fastmd_amd import _abi
+    from fastmd_amd.ops import feed_forward as ff
+
+    lib = _abi.load()
+    for hidden, width in ((129, 136), (257, 128), (128, 260), (1025, 100), (700, 2 ** 14 + 1), (2 ** 18 - 1, 2 ** 18 - 1)):
+        widest = max(hidden, width)
+        rows = min(ff.MAX_ROWS - 1, (ff.MAX_VALUES - 1) // widest)
+        assert max(rows, widest) * widest < ff.MAX_VALUES
+        for bf16 in (0, 1):
+            assert forms(bf16, rows, width, hidden, width) == ("tiles", "tiles")
+            assert lib.fmd_gated_ffn_work_size(bf16, rows, width, hidden, width, 15, 0) > 0
+            assert lib.fmd_gated_ffn_bwd_work_size(bf16, rows, width, hidden, width, 15, 1, 1) > 0
