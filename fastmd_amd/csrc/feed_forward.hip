@@ -15,7 +15,7 @@
 // Bound by the matrix cores from some hundred rows on, by reading the weights below. bf16, 8 192 rows of 2 048 x 5 504 (us, and the
 // rate of its bf16 products, two a multiply-add for h, dg and du): projections 459 (800 TFLOP/s), y 312 (1 180; 170 with h of one plane), dg and
 // du 352 (525: their epilogue moves 733 MB besides), gx 622 (1 190; 323), weights 977 (1 130; 503). float32 (six bf16 products a
-// multiply-add), 16 875 rows of 256 x 680, all gradients: 577 us (92 TFLOP/s). bf16, 16 rows of 2 048 x 5 504: 34 us.
+// multiply-add), 16 875 rows of 256 x 680, all gradients: 577 us (92 TFLOP/s). bf16, 16 rows of 2 048 x 5 504: 32 us.
 #include "ffn_block.h"
 
 namespace {
