@@ -9,8 +9,9 @@
     y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]
 
 with the rows of x rounded on the way, or given as ``Int8Rows``. The sums are exact (32-bit integers on the matrix cores),
-scales and bias are applied in float64, and each result is rounded to float32 and, where asked, from there to bfloat16. A row of zeros has the scale 0; one that holds a value that is not finite gives NaN. For evaluation:
-there are no gradients, and inputs that need them (x, scales, the bias) are refused.
+scales and bias are applied in float64, and each result is rounded to float32 and, where asked, from there to bfloat16. A row of
+zeros has the scale 0; one that holds a value that is not finite gives NaN. For evaluation: there are no gradients, and inputs that
+need them (x, scales, the bias) are refused.
 """
 from __future__ import annotations
 
@@ -90,7 +91,8 @@ def _check_rows(name: str, q: Int8Rows) -> None:
 def linear_int8(x: Tensor | Int8Rows, weight: Int8Rows, bias: Tensor | None = None, *, dtype: torch.dtype | None = None) -> Tensor:
     """``x weight^T + bias`` in 8 bits (see the module): ``x`` [rows, width] float32 or bfloat16, or ``Int8Rows``;
     ``weight`` [out, width] (``quantize_rows`` of it, once); ``bias`` float32 [out]; ``dtype`` of the result: x's, float32 for
-    ``Int8Rows``."""
+    ``Int8Rows``. 8-bit values whose rows do not start on 16 bytes, or cannot be read to the width's next multiple of 16, are copied by
+    every call (``quantize_rows`` lays a weight out so that they are not; of ``x``, widths that are multiples of 16 only)."""
     if not isinstance(weight, Int8Rows):
         raise ValueError("weight must be Int8Rows (quantize_rows)")
     _check_rows("weight", weight)
