@@ -2,7 +2,8 @@
 for the rounding errors of a float32 or bfloat16 evaluation a bound of each result, carried along from the absolute values of
 its terms.
 
-Units: u = 2^-24 (half a step of float32), r = 2^-8 for bfloat16 and u for float32 (the rounding of a result or an operand).
+Units: u = 2^-24 (half a step of float32), r = 2^-8 for bfloat16 and u for float32 (the rounding of a result). What is kept between two
+products is off by r^2 = 2^-16 in bfloat16 (two parts, each rounded once) and u in float32.
 A sum of n terms in float32 is off by at most (n u) times the sum of their absolute values, in any order."""
 from __future__ import annotations
 
@@ -40,6 +41,7 @@ def _sum(n, dtype):
 def gated(x, wg, wu, wd, name, gy=None):
     """[(value, bound)] of y, and for gy of the gradients of x, wg, wu, wd."""
     dtype, r = x.dtype, rounding(x.dtype)
+    kept = r * r if dtype == torch.bfloat16 else r
     x, wg, wu, wd = (t.double() for t in (x, wg, wu, wd))
     first, second = SLOPES[name]
     g, u = x @ wg.T, x @ wu.T
@@ -48,7 +50,7 @@ def gated(x, wg, wu, wd, name, gy=None):
     ea = first * eg + 8 * U * (1 + g.abs())
     ed = second * eg + 16 * U * (1 + g.abs())
     h = a * u
-    eh = ea * u.abs() + a.abs() * eu + ea * eu + r * h.abs()
+    eh = ea * u.abs() + a.abs() * eu + ea * eu + kept * h.abs()
     y = h @ wd.T
     out = [(y, eh @ wd.abs().T + _sum(h.shape[1], dtype) * (h.abs() @ wd.abs().T) + r * y.abs())]
     if gy is None:
@@ -57,8 +59,8 @@ def gated(x, wg, wu, wd, name, gy=None):
     gh = gy @ wd
     egh = _sum(gy.shape[1], dtype) * (gy.abs() @ wd.abs())
     dg, du = gh * u * d, gh * a
-    edg = (egh * (u * d).abs() + (gh * d).abs() * eu + (gh * u).abs() * ed) * 1.01 + r * dg.abs()
-    edu = (egh * a.abs() + gh.abs() * ea) * 1.01 + r * du.abs()
+    edg = (egh * (u * d).abs() + (gh * d).abs() * eu + (gh * u).abs() * ed) * 1.01 + kept * dg.abs()
+    edu = (egh * a.abs() + gh.abs() * ea) * 1.01 + kept * du.abs()
     gx = dg @ wg + du @ wu
     terms = dg.abs() @ wg.abs() + du.abs() @ wu.abs()
     out.append((gx, edg @ wg.abs() + edu @ wu.abs() + _sum(2 * h.shape[1], dtype) * terms + r * gx.abs()))
